@@ -1,0 +1,387 @@
+// The paged key/value cache in 8 bits: append (with the norm and the position
+// rotation of the keys on the way) and read.
+//
+// A page holds P tokens; one (page, head) is P x d codes of e4m3 in a row and
+// one scale for keys, one for values: value = code * scale. The scale is a
+// power of two, the smallest (2^-100 at least) that brings the page's largest
+// finite magnitude to 448 or less:
+//   amax = m 2^e, 1 <= m < 2;  448 = 1.75 * 2^8  =>  scale = 2^(e - 8), or 2^(e - 7) where m > 1.75
+// A power of two costs no precision (e4m3 keeps 3 bits below the leading one
+// at any scale) and makes it cheap and nearly exact to raise the scale of a
+// page that is already partly filled: old codes move by whole binades, so only
+// those that become subnormal are rounded again. A page's scale never falls
+// while it fills; a page whose first row is written starts anew. Non-finite
+// inputs do not enter the scale and are stored as NaN.
+//
+// append is bound by memory for long pieces (it reads k and v once and writes
+// one byte a value) and by latency for single tokens.
+#include <c10/cuda/CUDAGuard.h>
+#include <cuda_fp8.h>
+
+#include "kv_common.cuh"
+
+namespace pd {
+namespace kv {
+
+constexpr int kMinExp = -100;
+
+// exponent of the scale of a page whose largest finite magnitude has these bits
+__device__ __forceinline__ int scale_exp(float amax) {
+  if (amax == 0.f) return kMinExp;
+  int e = 0;
+  const float m = frexpf(amax, &e);               // amax = m 2^e, 0.5 <= m < 1
+  return max(kMinExp, m > 0.875f ? e - 8 : e - 9);
+}
+__device__ __forceinline__ float pow2(int e) { return __int_as_float((e + 127) << 23); }   // -126 <= e <= 127
+__device__ __forceinline__ int exp_of(float pow2_scale) { return (__float_as_int(pow2_scale) >> 23) - 127; }
+
+__device__ __forceinline__ uint32_t encode2(float a, float b) {
+  // satfinite would turn an infinity into 448
+  const float na = fabsf(a) == INFINITY ? NAN : a, nb = fabsf(b) == INFINITY ? NAN : b;
+  return __nv_cvt_float2_to_fp8x2(make_float2(na, nb), __NV_SATFINITE, __NV_E4M3);
+}
+__device__ __forceinline__ uint2 encode8(const float* f, float inv) {
+  uint2 u;
+  u.x = encode2(f[0] * inv, f[1] * inv) | (encode2(f[2] * inv, f[3] * inv) << 16);
+  u.y = encode2(f[4] * inv, f[5] * inv) | (encode2(f[6] * inv, f[7] * inv) << 16);
+  return u;
+}
+__device__ __forceinline__ void decode8(uint2 u, float* f) {
+  const uint32_t w[4] = {u.x & 0xffffu, u.x >> 16, u.y & 0xffffu, u.y >> 16};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2(__nv_fp8x2_storage_t(w[i]), __NV_E4M3);
+    const float2 t = __half22float2(*reinterpret_cast<const __half2*>(&h));
+    f[2 * i] = t.x;
+    f[2 * i + 1] = t.y;
+  }
+}
+
+struct AppendArgs {
+  const void* x[2];            // k, v: token strides ts, head strides hs, batch stride bs (uniform form)
+  int64_t bs[2], ts[2], hs[2];
+  uint8_t* code[2];            // [pages, H, P, d]
+  float* scale[2];             // [pages, H]
+  const int* table;            // [B, max_pages]
+  int64_t table_stride;
+  const int* lens;             // tokens before the call
+  const int* cu;               // [B + 1] or null
+  int n, total;                // new tokens of each sequence (uniform) / of all
+  int J, H, P, max_pages, n_pages, n_pos;
+  const float* kw;             // [d] or null
+  const float* rope;           // [n_pos, d] or null
+  bool norm, interleaved, vec;
+  float eps;
+  int* err;
+};
+
+constexpr int kAppendThreads = 128;
+
+// One block: the new tokens of one sequence that fall into one page, for one
+// head, keys (z = 0) or values. The rows stay in registers between the
+// maximum and the encoding.
+template <typename T, int D>
+__global__ void __launch_bounds__(kAppendThreads) append_kernel(const AppendArgs A) {
+  constexpr int L = D / 16;                          // lanes of a row
+  constexpr int R = kAppendThreads / L;              // rows at a time
+  constexpr int PASSES = (64 + R - 1) / R;           // a page has at most 64 rows
+  const int part = blockIdx.z, h = blockIdx.y;
+  const int b = blockIdx.x / A.J, j = blockIdx.x % A.J;
+  const int len = A.lens[b];
+  const int n = A.cu ? A.cu[b + 1] - A.cu[b] : A.n;
+  const int64_t tok0 = A.cu ? A.cu[b] : 0;
+  if (n <= 0) return;
+  if (len < 0 || (A.cu && (tok0 < 0 || tok0 + n > A.total))) {
+    if (threadIdx.x == 0) set_error(A.err, kBadShape);
+    return;
+  }
+  const int64_t pi = len / A.P + j;                  // page of the sequence
+  const int64_t p0 = pi * A.P;                       // position of its first row
+  const int lo = int(max(int64_t(len) - p0, int64_t(0)));
+  const int hi = int(min(int64_t(len) + n - p0, int64_t(A.P)));
+  if (hi <= lo) return;
+  const int page = pi < A.max_pages ? A.table[b * A.table_stride + pi] : -1;
+  if (page < 0 || page >= A.n_pages) {
+    if (threadIdx.x == 0) set_error(A.err, kIdOutOfRange);
+    return;
+  }
+  const T* x = static_cast<const T*>(A.x[part]) + h * A.hs[part] + (A.cu ? 0 : b * A.bs[part]);
+  const int64_t block = int64_t(page) * A.H + h;
+  uint8_t* code = A.code[part] + block * A.P * D;
+  const int lane = threadIdx.x % L, row0 = threadIdx.x / L;
+  int off0, off1;
+  bool turned;
+  pair_offsets<8>(lane, D, A.rope ? D : 0, A.interleaved, off0, off1, turned);
+
+  float a[PASSES][8], c[PASSES][8];
+  float amax = 0.f;
+#pragma unroll
+  for (int ps = 0; ps < PASSES; ++ps) {
+    const int r = ps * R + row0;
+    const bool live = r >= lo && r < hi;
+    const int64_t i = tok0 + p0 + r - len;             // token among the new ones
+#pragma unroll
+    for (int e = 0; e < 8; ++e) a[ps][e] = c[ps][e] = 0.f;
+    if (live) {
+      const T* xr = x + i * A.ts[part];
+      if (A.vec) {
+        load_v<8>(xr + off0, a[ps]);
+        load_v<8>(xr + off1, c[ps]);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          a[ps][e] = to_f(xr[off0 + e]);
+          c[ps][e] = to_f(xr[off1 + e]);
+        }
+      }
+    }
+    if (part == 0 && A.norm) {
+      float ss = 0.f;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) ss += a[ps][e] * a[ps][e] + c[ps][e] * c[ps][e];
+      const float rs = __frsqrt_rn(group_sum<L>(ss) * (1.f / D) + A.eps);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        a[ps][e] = a[ps][e] * rs * (A.kw ? __ldg(A.kw + off0 + e) : 1.f);
+        c[ps][e] = c[ps][e] * rs * (A.kw ? __ldg(A.kw + off1 + e) : 1.f);
+      }
+    }
+    if (part == 0 && A.rope && live) {
+      if (p0 + r < A.n_pos) {
+        float cs[8], sn[8];
+        load_angles<8>(A.rope + (p0 + r) * D, lane, D, A.interleaved, off0, off1, cs, sn);
+        turn<8>(a[ps], c[ps], cs, sn, A.interleaved, 1.f);
+      } else {
+        set_error(A.err, kIdOutOfRange);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) a[ps][e] = c[ps][e] = 0.f;
+      }
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const float u = fabsf(a[ps][e]), v = fabsf(c[ps][e]);
+      if (u < INFINITY) amax = fmaxf(amax, u);          // false for NaN too
+      if (v < INFINITY) amax = fmaxf(amax, v);
+    }
+  }
+  __shared__ float s_max[kAppendThreads / 32];
+  amax = warp_max(amax);
+  if ((threadIdx.x & 31) == 0) s_max[threadIdx.x >> 5] = amax;
+  const float old = lo > 0 ? A.scale[part][block] : 0.f;
+  __syncthreads();                                       // also: everyone has read the old scale
+#pragma unroll
+  for (int w = 0; w < kAppendThreads / 32; ++w) amax = fmaxf(amax, s_max[w]);
+  int e = scale_exp(amax);
+  if (lo > 0) {
+    // a scale from elsewhere that is no power of two counts as the next one
+    e = max(e, max(kMinExp, min(exp_of(old) + ((__float_as_int(old) & 0x7fffff) != 0), 120)));
+    const float ratio = old * pow2(-e);
+    if (ratio != 1.f) {
+      // the page's scale grows: its old rows move to the new one
+#pragma unroll 1
+      for (int r = row0; r < lo; r += R) {
+        uint2* q0 = reinterpret_cast<uint2*>(code + r * D + lane * 16);
+        float f[8];
+        decode8(q0[0], f);
+        q0[0] = encode8(f, ratio);
+        decode8(q0[1], f);
+        q0[1] = encode8(f, ratio);
+      }
+    }
+  }
+  const float inv = pow2(-e);
+#pragma unroll
+  for (int ps = 0; ps < PASSES; ++ps) {
+    const int r = ps * R + row0;
+    if (r >= lo && r < hi) {
+      *reinterpret_cast<uint2*>(code + r * D + off0) = encode8(a[ps], inv);
+      *reinterpret_cast<uint2*>(code + r * D + off1) = encode8(c[ps], inv);
+    }
+  }
+  if (threadIdx.x == 0) A.scale[part][block] = pow2(e);
+}
+
+struct ReadArgs {
+  const uint8_t* code[2];
+  const float* scale[2];
+  const int* table;
+  int64_t table_stride;
+  const int* lens;
+  const int* first;             // [B] or null (0)
+  __nv_bfloat16* out[2];        // [B, n, H, d]
+  int n, H, P, d, max_pages, n_pages;
+  int64_t vecs;                 // 8-element vectors of one output
+  int* err;
+};
+
+__global__ void __launch_bounds__(256) read_kernel(const ReadArgs A) {
+  const int64_t i = int64_t(blockIdx.x) * 256 + threadIdx.x;
+  if (i >= A.vecs) return;
+  const int part = blockIdx.y, dv = A.d / 8;
+  const int c = int(i % dv);
+  const int64_t t = i / dv;
+  const int h = int(t % A.H);
+  const int64_t bt = t / A.H;
+  const int b = int(bt / A.n);
+  const int64_t pos = bt % A.n + (A.first ? A.first[b] : 0);
+  float f[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+  if (pos >= 0 && pos < A.lens[b]) {
+    const int64_t pi = pos / A.P;
+    const int page = pi < A.max_pages ? A.table[b * A.table_stride + pi] : -1;
+    if (page >= 0 && page < A.n_pages) {
+      const int64_t block = int64_t(page) * A.H + h;
+      decode8(*reinterpret_cast<const uint2*>(A.code[part] + (block * A.P + pos % A.P) * A.d + c * 8), f);
+      const float s = A.scale[part][block];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) f[e] *= s;
+    } else {
+      set_error(A.err, kIdOutOfRange);
+    }
+  }
+  store_v<8>(A.out[part] + i * 8, f);
+}
+
+// ---------------------------------------------------------------- entry points
+// The cache's tensors; returns their sizes.
+struct CacheDims { int n_pages, H, P, d; };
+CacheDims check_cache(const at::Tensor& k, const at::Tensor& v, const at::Tensor& ks, const at::Tensor& vs,
+                      const at::Tensor& err) {
+  PD_CHECK(k.is_cuda() && k.dim() == 4 && k.is_contiguous() && k.scalar_type() == at::kFloat8_e4m3fn &&
+           v.is_contiguous() && v.sizes() == k.sizes() && v.scalar_type() == k.scalar_type() && v.device() == k.device(),
+           "the cache's codes must be contiguous float8_e4m3fn [pages, heads, page_size, d] on one CUDA device");
+  PD_CHECK(reinterpret_cast<uintptr_t>(k.data_ptr()) % 16 == 0 && reinterpret_cast<uintptr_t>(v.data_ptr()) % 16 == 0,
+           "the cache's codes must lie on 16-byte boundaries");
+  const int64_t H = k.size(1), P = k.size(2), d = k.size(3);
+  PD_CHECK(P == 16 || P == 32 || P == 64, "page size %d: expected 16, 32 or 64", int(P));
+  PD_CHECK(d == 32 || d == 64 || d == 128, "head dim %d of a cache: expected 32, 64 or 128", int(d));
+  PD_CHECK(k.size(0) > 0 && H > 0 && H < 65536 && k.size(0) * H * P < (int64_t(1) << 31),
+           "a cache has at least one page and head, and fewer than 2^31 rows");
+  for (const at::Tensor* s : {&ks, &vs})
+    PD_CHECK(s->device() == k.device() && s->scalar_type() == at::kFloat && s->is_contiguous() && s->dim() == 2 &&
+             s->size(0) == k.size(0) && s->size(1) == H, "the scales must be contiguous fp32 [pages, heads]");
+  PD_CHECK(err.device() == k.device() && err.scalar_type() == at::kInt && err.numel() == 1, "err must be one int32");
+  return {int(k.size(0)), int(H), int(P), int(d)};
+}
+
+void check_ints(const at::Tensor& t, const at::Tensor& like, int64_t n, const char* what) {
+  PD_CHECK(t.device() == like.device() && t.scalar_type() == at::kInt && t.dim() == 1 && t.is_contiguous() &&
+           t.size(0) == n, "%s must be contiguous int32 [%d] on the cache's device", what, int(n));
+}
+
+void check_table(const at::Tensor& t, const at::Tensor& like) {
+  PD_CHECK(t.device() == like.device() && t.scalar_type() == at::kInt && t.dim() == 2 &&
+           (t.size(1) <= 1 || t.stride(1) == 1), "the page table must be int32 [sequences, pages] on the cache's device");
+}
+
+template <typename T>
+static void append_launch(const AppendArgs& A, dim3 grid, int d) {
+  if (d == 32) append_kernel<T, 32><<<grid, kAppendThreads, 0, stream()>>>(A);
+  else if (d == 64) append_kernel<T, 64><<<grid, kAppendThreads, 0, stream()>>>(A);
+  else append_kernel<T, 128><<<grid, kAppendThreads, 0, stream()>>>(A);
+}
+
+void kv_append(at::Tensor ck, at::Tensor cv, at::Tensor ks, at::Tensor vs, at::Tensor err, at::Tensor k, at::Tensor v,
+               at::Tensor table, at::Tensor lens, c10::optional<at::Tensor> cu, int64_t max_new,
+               c10::optional<at::Tensor> k_weight, c10::optional<double> norm_eps, c10::optional<at::Tensor> rope,
+               bool interleaved) {
+  const CacheDims C = check_cache(ck, cv, ks, vs, err);
+  check_table(table, ck);
+  const int64_t B = table.size(0);
+  check_ints(lens, ck, B, "kv_lens");
+  const int dt = dtype_of(k, "k");
+  const int td = cu.has_value() ? 3 : 4;
+  AppendArgs A{};
+  A.vec = true;
+  for (int i = 0; i < 2; ++i) {
+    const at::Tensor& x = i == 0 ? k : v;
+    PD_CHECK(x.device() == ck.device() && x.scalar_type() == k.scalar_type() && x.dim() == td &&
+             x.size(td - 2) == C.H && x.size(td - 1) == C.d && (x.stride(td - 1) == 1 || x.numel() == 0),
+             "k and v must be %s of one type on the cache's device, with the cache's heads and head dim and unit "
+             "stride on d", cu.has_value() ? "[tokens, heads, d]" : "[sequences, tokens, heads, d]");
+    PD_CHECK(x.size(0) == k.size(0) && x.size(td - 3) == k.size(td - 3), "k and v differ in their tokens");
+    A.x[i] = x.data_ptr();
+    A.bs[i] = td == 4 ? x.stride(0) : 0;
+    A.ts[i] = x.stride(td - 3);
+    A.hs[i] = x.stride(td - 2);
+    const int64_t q = 16 / x.element_size();
+    A.vec = A.vec && reinterpret_cast<uintptr_t>(x.data_ptr()) % 16 == 0 && A.bs[i] % q == 0 && A.ts[i] % q == 0 &&
+            A.hs[i] % q == 0;
+    A.code[i] = static_cast<uint8_t*>((i == 0 ? ck : cv).data_ptr());
+    A.scale[i] = (i == 0 ? ks : vs).data_ptr<float>();
+  }
+  if (cu.has_value()) check_ints(*cu, ck, B + 1, "cu_new");
+  else PD_CHECK(k.size(0) == B, "k has %d sequences and the page table %d", int(k.size(0)), int(B));
+  PD_CHECK(k.size(td - 3) < (int64_t(1) << 31) && max_new >= 0 && max_new < (int64_t(1) << 31), "too many new tokens");
+  A.total = int(cu.has_value() ? k.size(0) : 0);
+  A.n = int(cu.has_value() ? 0 : k.size(1));
+  A.table = table.data_ptr<int>();
+  A.table_stride = table.stride(0);
+  A.max_pages = int(table.size(1));
+  A.lens = lens.data_ptr<int>();
+  A.cu = cu.has_value() ? cu->data_ptr<int>() : nullptr;
+  A.H = C.H; A.P = C.P; A.n_pages = C.n_pages;
+  A.err = err.data_ptr<int>();
+  A.interleaved = interleaved;
+  A.norm = norm_eps.has_value();
+  A.eps = float(norm_eps.value_or(0.));
+  if (k_weight.has_value()) {
+    PD_CHECK(A.norm, "k_weight needs norm_eps");
+    PD_CHECK(k_weight->device() == ck.device() && k_weight->scalar_type() == at::kFloat && k_weight->dim() == 1 &&
+             k_weight->is_contiguous() && k_weight->size(0) == C.d, "k_weight must be contiguous fp32 [d]");
+    A.kw = k_weight->data_ptr<float>();
+  }
+  if (rope.has_value()) {
+    PD_CHECK(rope->device() == ck.device() && rope->scalar_type() == at::kFloat && rope->dim() == 2 &&
+             rope->is_contiguous() && rope->size(1) == C.d && reinterpret_cast<uintptr_t>(rope->data_ptr()) % 16 == 0,
+             "rope must be a contiguous fp32 angle table [positions, d] (the cache rotates whole heads)");
+    A.rope = rope->data_ptr<float>();
+    A.n_pos = int(std::min<int64_t>(rope->size(0), INT32_MAX));
+  }
+  const int64_t most = cu.has_value() ? max_new : k.size(1);
+  if (B == 0 || most == 0 || k.size(td - 3) == 0) return;
+  A.J = int((most + C.P - 2) / C.P + 1);                 // pages that `most` tokens can touch
+  PD_CHECK(B * A.J < (int64_t(1) << 31), "too many sequences and pages for one call");
+  const c10::cuda::CUDAGuard guard(ck.device());
+  const dim3 grid(unsigned(B * A.J), C.H, 2);
+  if (dt == kBf16) append_launch<__nv_bfloat16>(A, grid, C.d);
+  else if (dt == kF16) append_launch<__half>(A, grid, C.d);
+  else append_launch<float>(A, grid, C.d);
+  PD_CHECK_LAUNCH();
+}
+
+std::vector<at::Tensor> kv_read(at::Tensor ck, at::Tensor cv, at::Tensor ks, at::Tensor vs, at::Tensor err,
+                                at::Tensor table, at::Tensor lens, c10::optional<at::Tensor> first, int64_t n) {
+  const CacheDims C = check_cache(ck, cv, ks, vs, err);
+  check_table(table, ck);
+  const int64_t B = table.size(0);
+  check_ints(lens, ck, B, "kv_lens");
+  if (first.has_value()) check_ints(*first, ck, B, "first");
+  PD_CHECK(n >= 0 && n < (int64_t(1) << 31), "n must be from 0 to 2^31 - 1");
+  const c10::cuda::CUDAGuard guard(ck.device());
+  ReadArgs A{};
+  std::vector<at::Tensor> out;
+  for (int i = 0; i < 2; ++i) {
+    A.code[i] = static_cast<const uint8_t*>((i == 0 ? ck : cv).data_ptr());
+    A.scale[i] = (i == 0 ? ks : vs).data_ptr<float>();
+    out.push_back(at::empty({B, n, C.H, C.d}, ck.options().dtype(at::kBFloat16)));
+    A.out[i] = static_cast<__nv_bfloat16*>(out[i].data_ptr());
+  }
+  A.table = table.data_ptr<int>();
+  A.table_stride = table.stride(0);
+  A.max_pages = int(table.size(1));
+  A.lens = lens.data_ptr<int>();
+  A.first = first.has_value() ? first->data_ptr<int>() : nullptr;
+  A.n = int(n); A.H = C.H; A.P = C.P; A.d = C.d; A.n_pages = C.n_pages;
+  A.vecs = B * n * C.H * (C.d / 8);
+  A.err = err.data_ptr<int>();
+  const int64_t blocks = (A.vecs + 255) / 256;
+  PD_CHECK(blocks < (int64_t(1) << 31), "too many values for one call");
+  if (blocks > 0) {
+    read_kernel<<<dim3(unsigned(blocks), 2), 256, 0, stream()>>>(A);
+    PD_CHECK_LAUNCH();
+  }
+  return out;
+}
+
+}  // namespace kv
+}  // namespace pd

@@ -1,7 +1,8 @@
 """Loader for the in-tree sm_100a extensions.
 
 ``core()`` returns the ``_C`` module (embedding, norm, loss, optimizer
-kernels) and ``gemm()`` the ``_gemm`` module (tcgen05 GEMMs, attention).
+kernels), ``gemm()`` the ``_gemm`` module (tcgen05 GEMMs, attention) and
+``kv()`` the ``_kv`` module (rotary and key/value-cache kernels).
 On a machine with a CUDA device a missing or stale extension raises: a GPU
 run never silently falls back to eager PyTorch.  Without a CUDA device the
 eager implementations in ``primus_dlrm_b200.ops`` are the only path (they
@@ -24,7 +25,7 @@ def _load(name: str):
         mod = importlib.import_module(f"primus_dlrm_b200.{name}")
     except ImportError as e:  # pragma: no cover - exercised on GPU boxes only
         src = os.path.join(os.path.dirname(os.path.dirname(os.path.dirname(os.path.abspath(__file__)))),
-                           "csrc", "gemm_bindings.cpp" if name == "_gemm" else "bindings.cpp")
+                           "csrc", {"_gemm": "gemm_bindings.cpp", "_kv": "kv_bindings.cpp"}.get(name, "bindings.cpp"))
         if torch.cuda.is_available() and os.path.exists(src):
             raise RuntimeError(
                 f"primus_dlrm_b200.{name} is not built; run `python setup.py build_ext --inplace` "
@@ -40,6 +41,10 @@ def core():
 
 def gemm():
     return _load("_gemm")
+
+
+def kv():
+    return _load("_kv")
 
 
 def native_enabled(device: torch.device | str | None = None) -> bool:

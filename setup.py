@@ -2,8 +2,9 @@
 
     python setup.py build_ext --inplace
 
-builds ``primus_dlrm_b200/_C*.so`` (core kernels) and
-``primus_dlrm_b200/_gemm*.so`` (tcgen05 GEMM / attention kernels) next to
+builds ``primus_dlrm_b200/_C*.so`` (core kernels),
+``primus_dlrm_b200/_gemm*.so`` (tcgen05 GEMM / attention kernels) and
+``primus_dlrm_b200/_kv*.so`` (rotary and key/value-cache kernels) next to
 the package, so the shared objects travel with the source tree.  Every CUDA
 source is compiled for ``sm_100a`` only.
 """
@@ -29,7 +30,8 @@ CXX = ["-O3", "-std=c++17"]
 
 core_sources = ["csrc/bindings.cpp"] + sorted(
     s for s in glob.glob("csrc/*.cu") if not os.path.basename(s).startswith("gemm")
-    and not os.path.basename(s).startswith("attn"))
+    and not os.path.basename(s).startswith(("attn", "kv_")))
+kv_sources = sorted(glob.glob("csrc/kv_*.cu")) + ["csrc/kv_bindings.cpp"]
 gemm_sources = sorted(glob.glob("csrc/gemm*.cu") + glob.glob("csrc/attn*.cu")) + ["csrc/gemm_bindings.cpp"]
 
 ext_modules = [
@@ -38,6 +40,15 @@ ext_modules = [
         sources=core_sources,
         include_dirs=[os.path.join(ROOT, "csrc")],
         extra_compile_args={"cxx": CXX, "nvcc": NVCC_COMMON},
+    ),
+    CUDAExtension(
+        name="primus_dlrm_b200._kv",
+        sources=kv_sources,
+        include_dirs=[os.path.join(ROOT, "csrc")],
+        extra_compile_args={
+            "cxx": CXX,
+            "nvcc": NVCC_COMMON + (["-Xptxas=-v"] if os.environ.get("PD_PTXAS_V") else []),
+        },
     ),
 ]
 if os.path.exists(os.path.join(ROOT, "csrc", "gemm_bindings.cpp")):
