@@ -6,9 +6,14 @@
 // of len tokens sees the keys j <= len - n + i (all keys without the causal
 // mask). A query without keys gives 0 (and -inf as its log-sum-exp).
 //
-// One warp a (query, head): a lane scores one key of 32, then the lanes own
-// the head's dims for the weighted sum of values; one pass with a running
-// maximum and sum, everything in 32 bits.
+// Arithmetic. Codes of e4m3 are exact in fp16, so both products run on fp16
+// operands with 32-bit sums and no rounding of the cache's values: a query row
+// is scaled by the power of two that brings its largest magnitude to
+// [2^14, 2^15) (elements down to 2^-29 of it keep all bits of bf16) and the
+// softmax scale undoes it; probabilities are held as 2^15 p, which keeps 11
+// bits down to 2^-29 and reaches 2^-39. A page's key scale multiplies its
+// scores in 32 bits; its value scale, relative to the largest of the tile's
+// pages, its probabilities. Running maximum, sum and output stay in 32 bits.
 #include <c10/cuda/CUDAGuard.h>
 #include <cuda_fp8.h>
 
@@ -22,95 +27,838 @@ CacheDims check_cache(const at::Tensor&, const at::Tensor&, const at::Tensor&, c
 void check_ints(const at::Tensor&, const at::Tensor&, int64_t, const char*);
 void check_table(const at::Tensor&, const at::Tensor&);
 
+constexpr uint64_t kWaitLimitNs = 2000000000ull;
+constexpr int kWarps = 4;               // warps of a block: they share a segment's keys
+constexpr int kRows = 16;               // rows (query, head of the group) of a segment
+constexpr int kMaxPages = 4;            // pages of a tile of keys (64 / 16)
+
 struct AttnArgs {
   const void* q;                // token, head (and batch) strides below
   int64_t q_bs, q_ts, q_hs;
-  const uint8_t* kc; const uint8_t* vc;      // [pages, H, P, d]
   const float* ks; const float* vs;          // [pages, H]
   const int* table; int64_t table_stride;
   const int* lens;
   const int* cu;                // [B + 1] or null
   void* o;                      // [tokens, Hq, d]
   float* lse;                   // [tokens, Hq] or null
-  int n, total, Hq, H, G, P, max_pages, n_pages;
-  bool causal;
+  int B, n, total, Hq, H, G, P, logP, max_pages, n_pages;
+  bool causal, split, bf16;
+  int min_units;
   float scale_log2;
+  float* part_o;                // split: [2 grid, 16, d] sums, [2 grid, 16, 2] (max, sum), [2 grid, 4] heads
+  float* part_ml;
+  int* part_head;
   int* err;
 };
 
-__device__ __forceinline__ float fp8_at(const uint8_t* p) {
-  return float(*reinterpret_cast<const __nv_fp8_e4m3*>(p));
+template <int D> struct Cfg;
+// TK keys a tile and warp (8 KB of keys and values for d = 64 and 128), ST tiles in flight
+template <> struct Cfg<32> { static constexpr int TK = 64, ST = 4; };
+template <> struct Cfg<64> { static constexpr int TK = 64, ST = 3; };
+template <> struct Cfg<128> { static constexpr int TK = 32, ST = 3; };
+
+__device__ __forceinline__ uint32_t smem_u32(const void* p) {
+  return static_cast<uint32_t>(__cvta_generic_to_shared(p));
+}
+__device__ __forceinline__ bool mbar_try(uint32_t bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
+      "selp.b32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok) : "r"(bar), "r"(parity), "r"(200000u) : "memory");
+  return ok != 0;
+}
+__device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, int* err) {
+  if (mbar_try(bar, parity)) return true;
+  const uint64_t t0 = globaltimer_ns();
+  while (!mbar_try(bar, parity)) {
+    if (globaltimer_ns() - t0 > kWaitLimitNs) {
+      set_error(err, kWaitTimeout);
+      return false;
+    }
+  }
+  return true;
+}
+__device__ __forceinline__ void tma_rows(uint32_t dst, const CUtensorMap* map, uint32_t bar, int row) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
+      ::"r"(dst), "l"(map), "r"(bar), "r"(0), "r"(row) : "memory");
+}
+__device__ __forceinline__ uint4 lds128(uint32_t a) {
+  uint4 v;
+  asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a));
+  return v;
+}
+__device__ __forceinline__ uint2 lds64(uint32_t a) {
+  uint2 v;
+  asm volatile("ld.shared.v2.b32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(a));
+  return v;
+}
+__device__ __forceinline__ uint32_t lds32(uint32_t a) {
+  uint32_t v;
+  asm volatile("ld.shared.b32 %0, [%1];" : "=r"(v) : "r"(a));
+  return v;
+}
+// two pairs of e4m3 codes -> two f16x2
+__device__ __forceinline__ void cvt4(uint32_t w, uint32_t& lo, uint32_t& hi) {
+  asm("{\n\t.reg .b16 l, h;\n\t"
+      "mov.b32 {l, h}, %2;\n\t"
+      "cvt.rn.f16x2.e4m3x2 %0, l;\n\t"
+      "cvt.rn.f16x2.e4m3x2 %1, h;\n\t}" : "=r"(lo), "=r"(hi) : "r"(w));
+}
+// queries and outputs are bf16 or fp16 by a flag of the call
+__device__ __forceinline__ float to_f_16(uint16_t v, bool bf16) {
+  return bf16 ? __bfloat162float(__ushort_as_bfloat16(v)) : __half2float(__ushort_as_half(v));
+}
+__device__ __forceinline__ void load8_16(const uint16_t* p, bool bf16, float* f) {
+  const uint4 u = *reinterpret_cast<const uint4*>(p);
+  const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    f[2 * i] = to_f_16(uint16_t(w[i] & 0xffffu), bf16);
+    f[2 * i + 1] = to_f_16(uint16_t(w[i] >> 16), bf16);
+  }
+}
+__device__ __forceinline__ uint32_t pack_16(float lo, float hi, bool bf16) {
+  if (bf16) {
+    const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&v);
+  }
+  const __half2 v = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+__device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
+  const __half2 v = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+// D(16x8 f32) += A(16x16 f16, row) * B(16x8 f16, col)
+__device__ __forceinline__ void mma_f16(float* d, const uint32_t* a, uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-template <typename T, int D>
-__global__ void __launch_bounds__(128) paged_attn_simple_kernel(const AttnArgs A) {
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int b = blockIdx.y, hq = blockIdx.z, i = blockIdx.x * 4 + warp;
-  const int n = A.cu ? A.cu[b + 1] - A.cu[b] : A.n;
-  if (i >= n) return;
-  const int64_t tok = A.cu ? int64_t(A.cu[b]) + i : int64_t(b) * A.n + i;
-  if (A.cu && (tok < 0 || tok >= A.total)) return;
-  const int h = hq / A.G;
-  int len = A.lens[b];
-  if (len > A.max_pages * int64_t(A.P)) {
-    set_error(A.err, kBadShape);
-    len = A.max_pages * A.P;
+// The queries and keys of one sequence, with impossible lengths cut (and reported).
+struct Seq {
+  int len, n, tok0, tiles_m;
+  __device__ __forceinline__ void load(const AttnArgs& A, int b) {
+    len = __ldg(A.lens + b);
+    if (A.cu) {
+      tok0 = __ldg(A.cu + b);
+      n = __ldg(A.cu + b + 1) - tok0;
+      if (n < 0 || tok0 < 0 || tok0 > A.total - n) {
+        set_error(A.err, kBadShape);
+        n = 0;
+      }
+    } else {
+      n = A.n;
+      tok0 = b * A.n;
+    }
+    if (int64_t(len) > int64_t(A.max_pages) << A.logP) {
+      set_error(A.err, kBadShape);
+      len = A.max_pages << A.logP;
+    }
+    if (len < 0) {
+      set_error(A.err, kBadShape);
+      len = 0;
+    }
+    tiles_m = int((int64_t(n) * A.G + kRows - 1) / kRows);
   }
-  const int keys = A.causal ? len - n + i + 1 : len;
-  const T* q = static_cast<const T*>(A.q) + (A.cu ? tok * A.q_ts : b * A.q_bs + i * A.q_ts) + hq * A.q_hs;
-  __shared__ float sq[4][D];
-  for (int c = lane; c < D; c += 32) sq[warp][c] = to_f(q[c]);
-  __syncwarp();
-  constexpr int E = D / 32;
-  float m = -INFINITY, l = 0.f, o[E];
-#pragma unroll
-  for (int e = 0; e < E; ++e) o[e] = 0.f;
-  for (int k0 = 0; k0 < keys; k0 += 32) {
-    const int j = k0 + lane;
-    float s = -INFINITY;
-    int64_t row = 0;
-    float vscale = 0.f;
-    if (j < keys) {
-      const int page = A.table[b * A.table_stride + j / A.P];
-      if (page >= 0 && page < A.n_pages) {
-        const int64_t block = int64_t(page) * A.H + h;
-        row = block * A.P + j % A.P;
-        s = 0.f;
-        for (int c = 0; c < D; ++c) s += sq[warp][c] * fp8_at(A.kc + row * D + c);
-        s *= A.ks[block] * A.scale_log2;
-        vscale = A.vs[block];
-      } else {
-        set_error(A.err, kIdOutOfRange);
+  // units of kWarps tiles of keys in each of its segments; a sequence without keys has one (it writes zeros)
+  __device__ __forceinline__ int units(int sup) const { return max(1, (len + sup - 1) / sup); }
+  __device__ __forceinline__ int64_t all(int H, int sup) const { return int64_t(units(sup)) * H * tiles_m; }
+};
+
+// A place in the list of units: sequence b, segment (head, row tile) in it, unit of its keys.
+struct Cursor {
+  int b, h, mt, unit, units;
+  Seq s;
+  int lim;                        // keys that the row tile's last row sees
+  int64_t left;                   // units from here to the end of this block's range
+  __device__ __forceinline__ void limits(const AttnArgs& A) {
+    const int last = min(mt * kRows + kRows, s.n * A.G) - 1;
+    lim = A.causal ? max(0, s.len - s.n + last / A.G + 1) : s.len;
+  }
+  __device__ __forceinline__ void next_seq(const AttnArgs& A, int sup) {
+    do {
+      if (++b >= A.B) { left = 0; return; }
+      s.load(A, b);
+    } while (s.tiles_m == 0);
+    units = s.units(sup);
+  }
+  __device__ __forceinline__ void next(const AttnArgs& A, int sup) {
+    if (--left <= 0) return;
+    if (++unit < units) return;
+    unit = 0;
+    if (++mt == s.tiles_m) {
+      mt = 0;
+      if (++h == A.H) {
+        h = 0;
+        next_seq(A, sup);
+        if (left <= 0) return;
       }
     }
-    const float mx = fmaxf(m, warp_max(s));
-    if (mx == -INFINITY) continue;
-    const float alpha = exp2f(m - mx), p = exp2f(s - mx);
-    m = mx;
-    l = l * alpha + warp_sum(p);
+    limits(A);
+  }
+};
+
+template <int D>
+__global__ void __launch_bounds__(kWarps * 32, D == 128 ? 2 : 3)
+paged_attn_kernel(const AttnArgs A, const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v) {
+  constexpr int TK = Cfg<D>::TK, ST = Cfg<D>::ST;
+  constexpr int SUP = TK * kWarps;
+  constexpr int NT = TK / 8;            // 8-key column tiles of the scores
+  constexpr int KS = D / 16;            // steps of 16 dims
+  constexpr int TS = TK / 16;           // steps of 16 keys
+  constexpr int NO = D / 8;             // 8-column tiles of the output
+  constexpr int kHalf = TK * D;         // bytes of a tile's keys
+  extern __shared__ __align__(1024) uint8_t s_ring[];       // [kWarps][ST] tiles: TK rows of keys, TK rows of values
+  __shared__ float s_merge[2][kRows * D];
+  __shared__ float s_ml[2][kRows][2];
+  __shared__ uint64_t s_bar[kWarps][ST];
+  __shared__ int s_blk[kWarps][ST][kMaxPages];              // page * H + head of each page of a tile, or -1
+  __shared__ int64_t s_scan[kWarps], s_start[2];
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int g = lane >> 2, qd = lane & 3;
+  const uint32_t ring = ((smem_u32(s_ring) + 1023) & ~1023u) + warp * ST * 2 * kHalf;
+  const uint32_t bars = smem_u32(s_bar[warp]);
+  if (lane < ST) {
+    asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(bars + lane * 8));
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (threadIdx.x == 0) {
+    asm volatile("prefetch.tensormap [%0];" ::"l"(&tm_k) : "memory");
+    asm volatile("prefetch.tensormap [%0];" ::"l"(&tm_v) : "memory");
+  }
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+
+  // ---- this block's range of units: each thread counts a run of sequences ----
+  Cursor c;
+  {
+    const int per = (A.B + blockDim.x - 1) / blockDim.x;
+    const int lo = min(int(threadIdx.x) * per, A.B), hi = min(lo + per, A.B);
+    int64_t mine = 0;
+    for (int b = lo; b < hi; ++b) {
+      Seq s;
+      s.load(A, b);
+      mine += A.split ? s.all(A.H, SUP) : int64_t(A.H) * s.tiles_m;
+    }
+    int64_t incl = mine;
 #pragma unroll
-    for (int e = 0; e < E; ++e) o[e] *= alpha;
-    for (int t = 0; t < 32; ++t) {
-      const float pt = __shfl_sync(0xffffffffu, p * vscale, t);
-      const int64_t rt = __shfl_sync(0xffffffffu, (long long)row, t);
-      const bool on = __shfl_sync(0xffffffffu, s, t) != -INFINITY;
-      if (!on) continue;
-#pragma unroll
-      for (int e = 0; e < E; ++e) o[e] += pt * fp8_at(A.vc + rt * D + lane + 32 * e);
+    for (int o = 1; o < 32; o <<= 1) {
+      const int64_t v = __shfl_up_sync(0xffffffffu, incl, o);
+      if (lane >= o) incl += v;
+    }
+    if (lane == 31) s_scan[warp] = incl;
+    __syncthreads();
+    int64_t before = incl - mine, total = 0;
+    for (int w = 0; w < kWarps; ++w) {
+      if (w < warp) before += s_scan[w];
+      total += s_scan[w];
+    }
+    // split: equal shares of the units; else equal shares of the segments
+    const int64_t share = max(int64_t(A.split ? A.min_units : 1), (total + gridDim.x - 1) / gridDim.x);
+    const int64_t u0 = share * blockIdx.x, u1 = min(total, u0 + share);
+    __syncthreads();
+    if (threadIdx.x == 0) s_start[1] = -1;
+    __syncthreads();
+    if (u0 < u1 && before <= u0 && u0 < before + mine) {
+      int64_t at = before;
+      for (int b = lo; b < hi; ++b) {
+        Seq s;
+        s.load(A, b);
+        const int64_t k = A.split ? s.all(A.H, SUP) : int64_t(A.H) * s.tiles_m;
+        if (u0 < at + k) {
+          s_start[0] = u0 - at;
+          s_start[1] = b;
+          break;
+        }
+        at += k;
+      }
+    }
+    __syncthreads();
+    c.b = int(s_start[1]);
+    c.left = 0;
+    if (c.b >= 0) {
+      c.s.load(A, c.b);
+      c.units = c.s.units(SUP);
+      int64_t r = s_start[0];
+      c.unit = A.split ? int(r % c.units) : 0;
+      if (A.split) r /= c.units;
+      c.mt = int(r % c.s.tiles_m);
+      c.h = int(r / c.s.tiles_m);
+      c.left = u1 - u0;
+      if (!A.split) {
+        // whole segments: count their units
+        Cursor t = c;
+        int64_t units = 0, segs = u1 - u0;
+        while (segs > 0) {
+          const int64_t here = min(segs, int64_t(A.H - t.h) * t.s.tiles_m - t.mt);
+          units += here * t.units;
+          segs -= here;
+          t.mt = t.h = 0;
+          t.left = 1;
+          if (segs > 0) t.next_seq(A, SUP);
+        }
+        c.left = units;
+      }
+      c.limits(A);
     }
   }
-  const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
-  T* out = static_cast<T*>(A.o) + (tok * A.Hq + hq) * D;
+  if (A.split && threadIdx.x < 2) A.part_head[(blockIdx.x * 2 + threadIdx.x) * 4] = -1;
+  if (c.left <= 0) return;
+
+  // ---- producer: this warp's tile of each unit ----
+  Cursor p = c;
+  int issued = 0;
+  int page = -1;                            // lane i: id of page i of the tile at p
+  const int box = min(A.P, TK), boxes = TK / box, box_log = min(A.logP, TK == 64 ? 6 : 5);
+  auto fetch_page = [&]() {
+    page = -1;
+    const int key = p.unit * SUP + warp * TK + lane * box;
+    if (p.left > 0 && lane < boxes && key < p.lim) page = __ldg(A.table + p.b * A.table_stride + (key >> A.logP));
+  };
+  auto issue = [&]() {
+    if (p.left <= 0) return;
+    const int st = issued % ST;
+    const uint32_t bar = bars + st * 8, dst = ring + st * 2 * kHalf;
+    const int key = p.unit * SUP + warp * TK + lane * box;
+    const bool want = lane < boxes && key < p.lim;
+    const bool have = want && page >= 0 && page < A.n_pages;
+    if (want && !have) set_error(A.err, kIdOutOfRange);
+    const int block = have ? page * A.H + p.h : -1;
+    if (lane < kMaxPages) s_blk[warp][st][lane] = block;
+    const uint32_t mask = __ballot_sync(0xffffffffu, have);
+    const int row = have ? block * A.P + (key & (A.P - 1)) : 0;
+    int rows_of[kMaxPages];
 #pragma unroll
-  for (int e = 0; e < E; ++e) out[lane + 32 * e] = from_f<T>(o[e] * inv);
-  if (A.lse && lane == 0) A.lse[tok * A.Hq + hq] = l > 0.f ? (m + log2f(l)) * 0.69314718056f : (l == 0.f ? -INFINITY : l);
+    for (int i = 0; i < kMaxPages; ++i) rows_of[i] = __shfl_sync(0xffffffffu, row, i);
+    // one lane issues every copy: a copy's operands are uniform registers
+    if (lane == 0) {
+      asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;"
+                   ::"r"(bar), "r"(uint32_t(__popc(mask) * 2 * box * D)) : "memory");
+#pragma unroll
+      for (int i = 0; i < kMaxPages; ++i)
+        if (mask >> i & 1) {
+          tma_rows(dst + i * box * D, &tm_k, bar, rows_of[i]);
+          tma_rows(dst + kHalf + i * box * D, &tm_v, bar, rows_of[i]);
+        }
+    }
+    __syncwarp();
+    ++issued;
+    p.next(A, SUP);
+    fetch_page();
+  };
+  fetch_page();
+#pragma unroll 1
+  for (int i = 0; i < ST - 1; ++i) issue();
+
+  // ---- consumer ----
+  uint32_t k_off, v_off[2];                 // this lane's bytes in a tile: K row g, V rows 2 qd and 2 qd + 1
+  if (D == 128) {
+    k_off = g * 128 + ((2 * qd) ^ g) * 16;
+    v_off[0] = (2 * qd) * 128 + (g ^ (2 * qd)) * 16;
+    v_off[1] = (2 * qd + 1) * 128 + (g ^ (2 * qd + 1)) * 16;
+  } else if (D == 64) {
+    k_off = g * 64 + (qd ^ (g >> 1)) * 16;
+    v_off[0] = (2 * qd) * 64 + ((g >> 1) ^ qd) * 16 + (g & 1) * 8;
+    v_off[1] = v_off[0] + 64;
+  } else {
+    k_off = g * 32 + ((qd >> 1) ^ (g >> 2)) * 16 + (qd & 1) * 8;
+    v_off[0] = (2 * qd) * 32 + ((g >> 2) ^ (qd >> 1)) * 16 + (g & 3) * 4;
+    v_off[1] = v_off[0] + 32;
+  }
+  float scl = 0.f;                          // lane i < 4: key scale of page i of the next tile, 4 <= i < 8: value scale
+  auto fetch_scales = [&](int t) {
+    scl = 0.f;
+    if (lane < 2 * kMaxPages) {
+      const int bk = s_blk[warp][t % ST][lane & 3];
+      if (bk >= 0) scl = __ldg((lane < kMaxPages ? A.ks : A.vs) + bk);
+    }
+  };
+  __syncwarp();
+  fetch_scales(0);
+  bool alive = true;
+  int taken = 0;
+  bool first = true;                        // of this block's segments
+  while (c.left > 0) {
+    // ---- a segment: this warp's share of its keys ----
+    const int seg_b = c.b, seg_h = c.h, seg_mt = c.mt;
+    const Seq S = c.s;
+    const bool begins = c.unit == 0;
+    const int seg_lim = c.lim;
+    const int r0 = seg_mt * kRows + g, rows = S.n * A.G;
+    int lim0 = 0, lim1 = 0, min_lim = 0;
+    uint32_t qf[KS][4];
+    float rs0, rs1;                         // softmax scale of the two rows, in the log2 domain
+    {
+      float amax[2] = {0.f, 0.f};
+      constexpr int E = D / 4;              // dims of a lane
+      float x[2][E];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int r = r0 + 8 * i;
+        const bool live = r < rows;
+        const int qi = live ? r / A.G : 0;
+        const uint16_t* src = static_cast<const uint16_t*>(A.q) +
+                              (A.cu ? int64_t(S.tok0 + qi) * A.q_ts
+                                    : int64_t(seg_b) * A.q_bs + int64_t(qi) * A.q_ts) +
+                              int64_t(seg_h * A.G + (live ? r - qi * A.G : 0)) * A.q_hs + qd * E;
+#pragma unroll
+        for (int e = 0; e < E; ++e) x[i][e] = 0.f;
+        if (live) {
+          if (reinterpret_cast<uintptr_t>(src) % 16 == 0) {
+#pragma unroll
+            for (int e = 0; e < E; e += 8) load8_16(src + e, A.bf16, &x[i][e]);
+          } else {
+#pragma unroll
+            for (int e = 0; e < E; ++e) x[i][e] = to_f_16(src[e], A.bf16);
+          }
+        }
+#pragma unroll
+        for (int e = 0; e < E; ++e) amax[i] = fmaxf(amax[i], fabsf(x[i][e]));
+        amax[i] = fmaxf(amax[i], __shfl_xor_sync(0xffffffffu, amax[i], 1));
+        amax[i] = fmaxf(amax[i], __shfl_xor_sync(0xffffffffu, amax[i], 2));
+        const int lm = !live ? 0 : A.causal ? max(0, S.len - S.n + qi + 1) : S.len;
+        if (i == 0) lim0 = lm; else lim1 = lm;
+      }
+      // 2^(14 - exponent): an infinity or NaN keeps its row's scale at 1
+      const int e0 = amax[0] < INFINITY ? max(-100, (__float_as_int(amax[0]) >> 23) - 127) : 14;
+      const int e1 = amax[1] < INFINITY ? max(-100, (__float_as_int(amax[1]) >> 23) - 127) : 14;
+      const float up0 = __int_as_float((14 - e0 + 127) << 23), up1 = __int_as_float((14 - e1 + 127) << 23);
+      rs0 = __int_as_float((e0 - 14 + 127) << 23) * A.scale_log2;
+      rs1 = __int_as_float((e1 - 14 + 127) << 23) * A.scale_log2;
+#pragma unroll
+      for (int k = 0; k < KS; ++k) {
+        qf[k][0] = pack_f16(x[0][4 * k] * up0, x[0][4 * k + 1] * up0);
+        qf[k][1] = pack_f16(x[1][4 * k] * up1, x[1][4 * k + 1] * up1);
+        qf[k][2] = pack_f16(x[0][4 * k + 2] * up0, x[0][4 * k + 3] * up0);
+        qf[k][3] = pack_f16(x[1][4 * k + 2] * up1, x[1][4 * k + 3] * up1);
+      }
+      min_lim = A.causal ? S.len - S.n + seg_mt * kRows / A.G + 1 : S.len;
+    }
+    float o[NO][4];
+#pragma unroll
+    for (int u = 0; u < NO; ++u) o[u][0] = o[u][1] = o[u][2] = o[u][3] = 0.f;
+    float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f;
+
+    bool ends = false;
+    do {
+      const int st = taken % ST;
+      const int k0 = c.unit * SUP + warp * TK;
+      issue();                              // refills the slot of the tile before
+      const float my_scl = scl;
+      if (c.left > 1) fetch_scales(taken + 1);
+      if (alive) alive = mbar_wait(bars + st * 8, (taken / ST) & 1, A.err);
+      if (k0 < seg_lim) {
+        const uint32_t kt = ring + st * 2 * kHalf, vt = kt + kHalf;
+        // scores
+        float s[NT][4];
+#pragma unroll
+        for (int j = 0; j < NT; ++j) {
+          uint32_t w[KS];
+          if constexpr (D == 128) {
+            const uint4 a = lds128(kt + k_off + j * 8 * D), b = lds128(kt + (k_off ^ 16) + j * 8 * D);
+            w[0] = a.x; w[1] = a.y; w[2] = a.z; w[3] = a.w;
+            w[4] = b.x; w[5] = b.y; w[6] = b.z; w[7] = b.w;
+          } else if constexpr (D == 64) {
+            const uint4 a = lds128(kt + k_off + j * 8 * D);
+            w[0] = a.x; w[1] = a.y; w[2] = a.z; w[3] = a.w;
+          } else {
+            const uint2 a = lds64(kt + k_off + j * 8 * D);
+            w[0] = a.x; w[1] = a.y;
+          }
+          s[j][0] = s[j][1] = s[j][2] = s[j][3] = 0.f;
+#pragma unroll
+          for (int k = 0; k < KS; ++k) {
+            uint32_t b0, b1;
+            cvt4(w[k], b0, b1);
+            mma_f16(s[j], qf[k], b0, b1);
+          }
+        }
+        // scales of the pages, masks
+        const int end = min(TK, seg_lim - k0);                        // keys of the tile that some row sees
+        bool hole = false;
+        float vrel[TS], vref = 0.f;
+#pragma unroll
+        for (int i = 0; i < TS; ++i) {
+          const int pg = (i * 16) >> box_log;
+          const float ks = __shfl_sync(0xffffffffu, my_scl, pg);
+          const float vs = __shfl_sync(0xffffffffu, my_scl, pg + kMaxPages);
+          vrel[i] = vs;
+          vref = fmaxf(vref, vs);
+          const bool bad = s_blk[warp][st][pg] < 0;              // not loaded: behind the keys, or no such page
+          hole |= bad;
+          const float f0 = ks * rs0, f1 = ks * rs1;
+#pragma unroll
+          for (int j = 2 * i; j < 2 * i + 2; ++j) {
+            s[j][0] = bad ? -INFINITY : s[j][0] * f0;
+            s[j][1] = bad ? -INFINITY : s[j][1] * f0;
+            s[j][2] = bad ? -INFINITY : s[j][2] * f1;
+            s[j][3] = bad ? -INFINITY : s[j][3] * f1;
+          }
+        }
+        if (k0 + TK > min_lim) {
+#pragma unroll
+          for (int j = 0; j < NT; ++j) {
+            const int key = k0 + 8 * j + 2 * qd;
+            if (key >= lim0) s[j][0] = -INFINITY;
+            if (key + 1 >= lim0) s[j][1] = -INFINITY;
+            if (key >= lim1) s[j][2] = -INFINITY;
+            if (key + 1 >= lim1) s[j][3] = -INFINITY;
+          }
+        }
+        // running maximum and sum
+        float x0 = m0, x1 = m1;
+#pragma unroll
+        for (int j = 0; j < NT; ++j) {
+          x0 = fmaxf(x0, fmaxf(s[j][0], s[j][1]));
+          x1 = fmaxf(x1, fmaxf(s[j][2], s[j][3]));
+        }
+        x0 = fmaxf(x0, __shfl_xor_sync(0xffffffffu, x0, 1));
+        x1 = fmaxf(x1, __shfl_xor_sync(0xffffffffu, x1, 1));
+        x0 = fmaxf(x0, __shfl_xor_sync(0xffffffffu, x0, 2));
+        x1 = fmaxf(x1, __shfl_xor_sync(0xffffffffu, x1, 2));
+        const float b0 = x0 == -INFINITY ? 0.f : x0, b1 = x1 == -INFINITY ? 0.f : x1;
+        const float al0 = exp2f_approx(m0 - b0), al1 = exp2f_approx(m1 - b1);
+        m0 = x0;
+        m1 = x1;
+        l0 *= al0;
+        l1 *= al1;
+        const float z0 = 15.f - b0, z1 = 15.f - b1;                   // probabilities times 2^15
+        const float vinv = vref > 0.f ? 1.f / vref : 0.f;
+        uint32_t pf[TS][4];
+#pragma unroll
+        for (int i = 0; i < TS; ++i) {
+          const float f = vrel[i] * vinv;
+#pragma unroll
+          for (int t = 0; t < 2; ++t) {
+            const float* sj = s[2 * i + t];
+            const float p0 = exp2f_approx(sj[0] + z0), p1 = exp2f_approx(sj[1] + z0);
+            const float p2 = exp2f_approx(sj[2] + z1), p3 = exp2f_approx(sj[3] + z1);
+            l0 += p0 + p1;
+            l1 += p2 + p3;
+            pf[i][2 * t] = pack_f16(p0 * f, p1 * f);
+            pf[i][2 * t + 1] = pack_f16(p2 * f, p3 * f);
+          }
+        }
+        // values: what lies behind the keys may be anything, NaN too
+        uint32_t vw[TS][4][D / 32];
+#pragma unroll
+        for (int i = 0; i < TS; ++i)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            const uint32_t a = vt + v_off[r & 1] + (16 * i + 8 * (r >> 1)) * D;
+            if constexpr (D == 128) {
+              const uint4 t = lds128(a);
+              vw[i][r][0] = t.x; vw[i][r][1] = t.y; vw[i][r][2] = t.z; vw[i][r][3] = t.w;
+            } else if constexpr (D == 64) {
+              const uint2 t = lds64(a);
+              vw[i][r][0] = t.x; vw[i][r][1] = t.y;
+            } else {
+              vw[i][r][0] = lds32(a);
+            }
+          }
+        if (hole || end < TK) {
+#pragma unroll
+          for (int i = 0; i < TS; ++i)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+              const bool gone = 16 * i + 2 * qd + (r & 1) + 8 * (r >> 1) >= end ||
+                                s_blk[warp][st][(i * 16) >> box_log] < 0;
+#pragma unroll
+              for (int w = 0; w < D / 32; ++w) vw[i][r][w] = gone ? 0u : vw[i][r][w];
+            }
+        }
+#pragma unroll
+        for (int w = 0; w < D / 32; ++w) {
+          float acc[4][4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) acc[e][0] = acc[e][1] = acc[e][2] = acc[e][3] = 0.f;
+#pragma unroll
+          for (int i = 0; i < TS; ++i) {
+            // pairs of keys for four dims: bytes of two rows side by side
+            uint32_t b0[4], b1[4];
+            cvt4(__byte_perm(vw[i][0][w], vw[i][1][w], 0x5140), b0[0], b0[1]);
+            cvt4(__byte_perm(vw[i][0][w], vw[i][1][w], 0x7362), b0[2], b0[3]);
+            cvt4(__byte_perm(vw[i][2][w], vw[i][3][w], 0x5140), b1[0], b1[1]);
+            cvt4(__byte_perm(vw[i][2][w], vw[i][3][w], 0x7362), b1[2], b1[3]);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) mma_f16(acc[e], pf[i], b0[e], b1[e]);
+          }
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            float* ou = o[4 * w + e];
+            ou[0] = fmaf(acc[e][0], vref, ou[0] * al0);
+            ou[1] = fmaf(acc[e][1], vref, ou[1] * al0);
+            ou[2] = fmaf(acc[e][2], vref, ou[2] * al1);
+            ou[3] = fmaf(acc[e][3], vref, ou[3] * al1);
+          }
+        }
+      }
+      __syncwarp();                         // the slot has been read
+      ++taken;
+      const int was = c.unit;
+      const int64_t left = c.left;
+      c.next(A, SUP);
+      ends = was == S.units(SUP) - 1;
+      if (left == 1) break;
+    } while (!ends);
+
+    // ---- the block's warps become one ----
+    l0 += __shfl_xor_sync(0xffffffffu, l0, 1);
+    l1 += __shfl_xor_sync(0xffffffffu, l1, 1);
+    l0 += __shfl_xor_sync(0xffffffffu, l0, 2);
+    l1 += __shfl_xor_sync(0xffffffffu, l1, 2);
+    const bool alone = S.len <= TK;         // one tile of keys: warp 0 has it all
+    if (!alone) {
+#pragma unroll
+      for (int n = kWarps / 2; n > 0; n /= 2) {             // warps n .. 2 n - 1 go to warps 0 .. n - 1
+        __syncthreads();
+        if (warp >= n && warp < 2 * n) {
+#pragma unroll
+          for (int u = 0; u < NO; ++u)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) s_merge[warp - n][(u * 4 + e) * 32 + lane] = o[u][e];
+          if (qd == 0) {
+            s_ml[warp - n][g][0] = m0;
+            s_ml[warp - n][g][1] = l0;
+            s_ml[warp - n][g + 8][0] = m1;
+            s_ml[warp - n][g + 8][1] = l1;
+          }
+        }
+        __syncthreads();
+        if (warp < n) {
+          const float n0 = s_ml[warp][g][0], n1 = s_ml[warp][g + 8][0];
+          const float x0 = fmaxf(m0, n0), x1 = fmaxf(m1, n1);
+          const float c0 = x0 == -INFINITY ? 0.f : x0, c1 = x1 == -INFINITY ? 0.f : x1;
+          const float a0 = exp2f_approx(m0 - c0), a1 = exp2f_approx(m1 - c1);
+          const float d0 = exp2f_approx(n0 - c0), d1 = exp2f_approx(n1 - c1);
+          l0 = l0 * a0 + s_ml[warp][g][1] * d0;
+          l1 = l1 * a1 + s_ml[warp][g + 8][1] * d1;
+          m0 = x0;
+          m1 = x1;
+#pragma unroll
+          for (int u = 0; u < NO; ++u) {
+            const float* src = &s_merge[warp][u * 128 + lane];
+            o[u][0] = o[u][0] * a0 + src[0] * d0;
+            o[u][1] = o[u][1] * a0 + src[32] * d0;
+            o[u][2] = o[u][2] * a1 + src[64] * d1;
+            o[u][3] = o[u][3] * a1 + src[96] * d1;
+          }
+        }
+      }
+    }
+    if (warp == 0) {
+      if (begins && ends) {
+        // sum of 0: no keys. A NaN stays one
+        const float i0 = l0 == 0.f ? 0.f : 1.f / l0, i1 = l1 == 0.f ? 0.f : 1.f / l1;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const int r = r0 + 8 * i;
+          if (r >= rows) continue;
+          const int qi = r / A.G;
+          const int64_t at = int64_t(S.tok0 + qi) * A.Hq + seg_h * A.G + (r - qi * A.G);
+          uint16_t* dst = static_cast<uint16_t*>(A.o) + at * D + qd * (D / 4);
+          const float inv = i ? i1 : i0;
+#pragma unroll
+          for (int t = 0; t < 2; ++t) {
+            float f[NO];
+#pragma unroll
+            for (int u = 0; u < NO; ++u) f[u] = o[u][2 * i + t] * inv;
+#pragma unroll
+            for (int u = 0; u < NO; u += 4)
+              *reinterpret_cast<uint2*>(dst + t * NO + u) =
+                  make_uint2(pack_16(f[u], f[u + 1], A.bf16), pack_16(f[u + 2], f[u + 3], A.bf16));
+          }
+          const float l = i ? l1 : l0, m = i ? m1 : m0;
+          if (A.lse && qd == 0)
+            A.lse[at] = l == 0.f ? -INFINITY : (m - 15.f + log2f(l)) * 0.6931471805599453f;
+        }
+      } else {
+        const int slot = blockIdx.x * 2 + (first ? 0 : 1);
+        float* dst = A.part_o + int64_t(slot) * kRows * D;
+#pragma unroll
+        for (int u = 0; u < NO; ++u)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) dst[(u * 4 + e) * 32 + lane] = o[u][e];
+        if (qd == 0) {
+          float* ml = A.part_ml + int64_t(slot) * kRows * 2;
+          ml[g * 2] = m0; ml[g * 2 + 1] = l0;
+          ml[(g + 8) * 2] = m1; ml[(g + 8) * 2 + 1] = l1;
+        }
+        if (lane == 0) {
+          int* hd = A.part_head + slot * 4;
+          hd[0] = seg_b;
+          hd[1] = seg_h;
+          hd[2] = seg_mt;
+          hd[3] = (begins ? 1 : 0) | (ends ? 2 : 0);
+        }
+      }
+    }
+    first = false;
+  }
 }
 
-template <typename T>
-static void attn_launch(const AttnArgs& A, dim3 grid, int d) {
-  if (d == 32) paged_attn_simple_kernel<T, 32><<<grid, 128, 0, stream()>>>(A);
-  else if (d == 64) paged_attn_simple_kernel<T, 64><<<grid, 128, 0, stream()>>>(A);
-  else paged_attn_simple_kernel<T, 128><<<grid, 128, 0, stream()>>>(A);
+// Pieces of the segments that blocks share: one block for each piece that
+// begins a segment adds up those that follow in the next blocks, in order.
+template <int D>
+__global__ void __launch_bounds__(256) paged_attn_join_kernel(const AttnArgs A, int blocks) {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  constexpr int PER = kRows * D / 256;
+  __shared__ float s_m[kRows], s_l[kRows], s_f[kRows];
+  // a block's last piece is the only one that can begin a segment without ending it
+  int slot = -1;
+  for (int i = 0; i < 2; ++i) {
+    const int* hd = A.part_head + (blockIdx.x * 2 + i) * 4;
+    if (hd[0] >= 0 && hd[3] == 1) slot = blockIdx.x * 2 + i;
+  }
+  if (slot < 0) return;
+  const int b = A.part_head[slot * 4], h = A.part_head[slot * 4 + 1], mt = A.part_head[slot * 4 + 2];
+  int last = blockIdx.x;                     // block of the piece that ends the segment
+  do { ++last; } while (last < blocks && !(A.part_head[last * 8 + 3] & 2));
+  last = min(last, blocks - 1);
+  const int tid = threadIdx.x;
+  if (tid < kRows) {
+    float m = A.part_ml[(int64_t(slot) * kRows + tid) * 2];
+    for (int k = blockIdx.x + 1; k <= last; ++k) m = fmaxf(m, A.part_ml[(int64_t(k) * 2 * kRows + tid) * 2]);
+    const float base = m == -INFINITY ? 0.f : m;
+    float l = 0.f;
+    for (int k = blockIdx.x; k <= last; ++k) {
+      const float* ml = A.part_ml + (int64_t(k == int(blockIdx.x) ? slot : 2 * k) * kRows + tid) * 2;
+      l += ml[1] * exp2f_approx(ml[0] - base);
+    }
+    s_m[tid] = m;
+    s_l[tid] = l;
+    s_f[tid] = l == 0.f ? 0.f : 1.f / l;
+  }
+  __syncthreads();
+  // element x of a piece: fragment (u, e) of lane x % 32, as the first kernel's registers lie
+  float sum[PER];
+  int row[PER];
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    const int x = i * 256 + tid, ln = x & 31, e = (x >> 5) & 3;
+    row[i] = (ln >> 2) + 8 * (e >> 1);
+    sum[i] = 0.f;
+  }
+  for (int k = blockIdx.x; k <= last; ++k) {
+    const int64_t sl = k == int(blockIdx.x) ? slot : 2 * k;
+    const float* src = A.part_o + sl * kRows * D;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      const float m = s_m[row[i]], base = m == -INFINITY ? 0.f : m;
+      sum[i] += src[i * 256 + tid] * exp2f_approx(A.part_ml[(sl * kRows + row[i]) * 2] - base);
+    }
+  }
+  Seq S;
+  S.load(A, b);
+  const int rows = S.n * A.G;
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    const int x = i * 256 + tid, ln = x & 31, e = (x >> 5) & 3, u = x >> 7;
+    const int r = mt * kRows + row[i];
+    if (r >= rows) continue;
+    const int qi = r / A.G;
+    const int64_t at = int64_t(S.tok0 + qi) * A.Hq + h * A.G + (r - qi * A.G);
+    static_cast<uint16_t*>(A.o)[at * D + (2 * (ln & 3) + (e & 1)) * (D / 8) + u] =
+        uint16_t(pack_16(sum[i] * s_f[row[i]], 0.f, A.bf16));
+  }
+  if (A.lse && tid < kRows && mt * kRows + tid < rows) {
+    const int r = mt * kRows + tid, qi = r / A.G;
+    const int64_t at = int64_t(S.tok0 + qi) * A.Hq + h * A.G + (r - qi * A.G);
+    A.lse[at] = s_l[tid] == 0.f ? -INFINITY : (s_m[tid] - 15.f + log2f(s_l[tid])) * 0.6931471805599453f;
+  }
+}
+
+// cuTensorMapEncodeTiled through the runtime: the extension does not link
+// libcuda, so it imports on machines without a driver.
+static CUresult encode_tiled(CUtensorMap* m, void* base, const cuuint64_t* dims, const cuuint64_t* strides,
+                             const cuuint32_t* box, CUtensorMapSwizzle swizzle) {
+  using Fn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
+                          const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                          CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+  static const Fn fn = [] {
+    void* p = nullptr;
+    cudaDriverEntryPointQueryResult q = cudaDriverEntryPointSymbolNotFound;
+    const cudaError_t e = cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q);
+    PD_CHECK(e == cudaSuccess && q == cudaDriverEntryPointSuccess && p != nullptr,
+             "cuTensorMapEncodeTiled is unavailable (%d, %d)", int(e), int(q));
+    return reinterpret_cast<Fn>(p);
+  }();
+  const cuuint32_t es[2] = {1, 1};
+  return fn(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, base, dims, strides, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle,
+            CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+}
+
+static CUtensorMap code_map(const at::Tensor& x, int box_rows) {
+  CUtensorMap m;
+  const int64_t d = x.size(3), rows = x.numel() / d;
+  const cuuint64_t dims[2] = {cuuint64_t(d), cuuint64_t(rows)}, strides[1] = {cuuint64_t(d)};
+  const cuuint32_t box[2] = {cuuint32_t(d), cuuint32_t(box_rows)};
+  const CUresult r = encode_tiled(&m, x.data_ptr(), dims, strides, box,
+                                  d == 128  ? CU_TENSOR_MAP_SWIZZLE_128B
+                                  : d == 64 ? CU_TENSOR_MAP_SWIZZLE_64B
+                                            : CU_TENSOR_MAP_SWIZZLE_32B);
+  PD_CHECK(r == CUDA_SUCCESS, "cuTensorMapEncodeTiled failed for the cache (%d)", int(r));
+  return m;
+}
+
+template <int D>
+static void attn_launch(AttnArgs& A, const at::Tensor& ck, const at::Tensor& cv, int64_t segments, int64_t max_len) {
+  constexpr int TK = Cfg<D>::TK, ST = Cfg<D>::ST, SUP = TK * kWarps;
+  constexpr int kSmem = 1024 + kWarps * ST * 2 * TK * D;     // the ring, on a 1024-byte boundary
+  auto kern = paged_attn_kernel<D>;
+  static int per_sm[64] = {};                // by device
+  int dev = 0;
+  PD_CHECK_CUDA(cudaGetDevice(&dev));
+  if (dev >= 64 || per_sm[dev] == 0) {
+    PD_CHECK_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem));
+    int n = 0;
+    PD_CHECK_CUDA(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kern, kWarps * 32, kSmem));
+    PD_CHECK(n > 0, "the attention kernel does not fit an SM");
+    if (dev < 64) per_sm[dev] = n;
+  }
+  const int slots = num_sms() * (dev < 64 ? per_sm[dev] : 1);
+  const int64_t units = std::max<int64_t>(1, (max_len + SUP - 1) / SUP);      // of the longest segment
+  A.min_units = 2;
+  A.split = segments < int64_t(slots) * 8 && units > A.min_units;
+  const int64_t most = A.split ? (segments * units + A.min_units - 1) / A.min_units : segments;
+  const int grid = int(std::min<int64_t>(slots, most));
+  at::Tensor part;
+  if (A.split) {
+    const int64_t n = 2 * int64_t(grid);
+    part = at::empty({n * (kRows * D + kRows * 2 + 4)}, ck.options().dtype(at::kFloat));
+    A.part_o = part.data_ptr<float>();
+    A.part_ml = A.part_o + n * kRows * D;
+    A.part_head = reinterpret_cast<int*>(A.part_ml + n * kRows * 2);
+  }
+  const int box = std::min(A.P, TK);
+  kern<<<grid, kWarps * 32, kSmem, stream()>>>(A, code_map(ck, box), code_map(cv, box));
+  PD_CHECK_LAUNCH();
+  if (A.split) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = 256;
+    cfg.stream = stream();
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = 1;
+    PD_CHECK_CUDA(cudaLaunchKernelEx(&cfg, paged_attn_join_kernel<D>, (const AttnArgs)A, grid));
+    PD_CHECK_LAUNCH();
+  }
+}
+
+static void attn_dispatch(AttnArgs& A, const at::Tensor& ck, const at::Tensor& cv, int d, int64_t segments,
+                          int64_t max_len) {
+  if (d == 32) attn_launch<32>(A, ck, cv, segments, max_len);
+  else if (d == 64) attn_launch<64>(A, ck, cv, segments, max_len);
+  else attn_launch<128>(A, ck, cv, segments, max_len);
 }
 
 // (o, lse): lse is an undefined tensor unless asked for.
@@ -138,8 +886,6 @@ std::vector<at::Tensor> paged_attention(at::Tensor q, at::Tensor ck, at::Tensor 
   A.q_bs = qd == 4 ? q.stride(0) : 0;
   A.q_ts = q.stride(qd - 3);
   A.q_hs = q.stride(qd - 2);
-  A.kc = static_cast<const uint8_t*>(ck.data_ptr());
-  A.vc = static_cast<const uint8_t*>(cv.data_ptr());
   A.ks = ks.data_ptr<float>();
   A.vs = vs.data_ptr<float>();
   A.table = table.data_ptr<int>();
@@ -148,9 +894,11 @@ std::vector<at::Tensor> paged_attention(at::Tensor q, at::Tensor ck, at::Tensor 
   A.cu = cu.has_value() ? cu->data_ptr<int>() : nullptr;
   A.n = int(qd == 4 ? q.size(1) : 0);
   A.total = int(qd == 3 ? q.size(0) : 0);
-  A.Hq = int(Hq); A.H = C.H; A.G = int(Hq / C.H); A.P = C.P; A.n_pages = C.n_pages;
+  A.B = int(B); A.Hq = int(Hq); A.H = C.H; A.G = int(Hq / C.H); A.P = C.P; A.n_pages = C.n_pages;
+  A.logP = C.P == 16 ? 4 : C.P == 32 ? 5 : 6;
   A.max_pages = int(table.size(1));
   A.causal = causal;
+  A.bf16 = q.scalar_type() == at::kBFloat16;
   A.scale_log2 = float(scale * 1.4426950408889634);
   A.err = err.data_ptr<int>();
   at::Tensor o = at::empty(q.sizes(), q.options());
@@ -160,12 +908,15 @@ std::vector<at::Tensor> paged_attention(at::Tensor q, at::Tensor ck, at::Tensor 
     lse = at::empty(q.sizes().slice(0, qd - 1), q.options().dtype(at::kFloat));
     A.lse = lse.data_ptr<float>();
   }
-  const int64_t most = qd == 4 ? q.size(1) : std::min<int64_t>(max_q, q.size(0));
+  const int64_t most = qd == 4 ? q.size(1) : std::min<int64_t>(std::max<int64_t>(max_q, 0), q.size(0));
+  PD_CHECK((qd == 3 ? q.size(0) : B * q.size(1)) * A.G < (int64_t(1) << 31) - kRows && B < (int64_t(1) << 31),
+           "too many queries");
   if (B > 0 && most > 0 && q.numel() > 0) {
-    const dim3 grid(unsigned((most + 3) / 4), unsigned(B), unsigned(Hq));
-    if (q.scalar_type() == at::kBFloat16) attn_launch<__nv_bfloat16>(A, grid, C.d);
-    else attn_launch<__half>(A, grid, C.d);
-    PD_CHECK_LAUNCH();
+    // upper bounds of what the lengths on the device can ask for; they only decide how the work is split
+    const int64_t segments = B * C.H * ((most * A.G + kRows - 1) / kRows);
+    const int64_t room = table.size(1) * C.P;
+    const int64_t longest = std::min<int64_t>(room, std::max<int64_t>(max_len, 0));
+    attn_dispatch(A, ck, cv, C.d, segments, longest);
   }
   return want_lse ? std::vector<at::Tensor>{o, lse} : std::vector<at::Tensor>{o};
 }

@@ -220,6 +220,9 @@ class TransformerConfig:
     attention_impl: str = "turbo"
     # --- additive ---
     norm: str = "rmsnorm"
+    # queries and keys normed per head and rotated by their positions
+    rotary: bool = False
+    rope_theta: float = 10000.0
 
 
 @dataclass

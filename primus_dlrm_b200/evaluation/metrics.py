@@ -65,17 +65,21 @@ def _aggregate(per_user: list[dict[str, float]], ks: list[int]) -> dict[str, flo
 
 @torch.no_grad()
 def score_candidates(model, user_batch: dict[str, torch.Tensor], candidate_batch: dict[str, torch.Tensor],
-                     task: str, batch_size: int = 1024) -> torch.Tensor:
+                     task: str, batch_size: int = 1024, kv_cache: str | None = None) -> torch.Tensor:
     """Scores [C] of one user's history against C candidates (device tensor).
 
     ``user_batch`` holds the user-side tensors with a leading dim of 1;
     ``candidate_batch`` holds per-candidate tensors with leading dim C.
+    ``kv_cache="fp8"`` keeps a OneTrans model's keys and values of the history
+    in 8-bit pages.
     """
     inner = getattr(model, "module", model)
     if hasattr(inner, "score_candidates"):
         from primus_dlrm_b200.parallel.fsdp import full_params
         with full_params(inner):          # FSDP units: the scorer reads block weights directly
-            return inner.score_candidates(user_batch, candidate_batch, task, batch_size)
+            return inner.score_candidates(user_batch, candidate_batch, task, batch_size, kv_cache)
+    if kv_cache is not None:
+        raise ValueError("kv_cache: this model keeps no keys and values")
     C = next(iter(candidate_batch.values())).shape[0]
     out = []
     for s in range(0, C, batch_size):
@@ -90,7 +94,7 @@ def score_candidates(model, user_batch: dict[str, torch.Tensor], candidate_batch
 
 
 def evaluate_ranking(model, eval_dataset, device, candidate_item_ids=None, ks=None, task: str = "listen_plus",
-                     batch_size: int = 1024, log_interval: int = 0) -> dict[str, float]:
+                     batch_size: int = 1024, log_interval: int = 0, kv_cache: str | None = None) -> dict[str, float]:
     """Global candidate list (default: top popular items) per test user."""
     ks = ks or [10, 100]
     model.eval()
@@ -105,7 +109,7 @@ def evaluate_ranking(model, eval_dataset, device, candidate_item_ids=None, ks=No
             continue
         ub = eval_dataset.user_batch(sample, device)
         s = score_candidates(model, ub, eval_dataset.with_user_features(cand, sample, candidate_item_ids, device),
-                             task, batch_size)
+                             task, batch_size, kv_cache)
         order = torch.argsort(s, descending=True)[: max(ks)].cpu().numpy()
         per_user.append(metrics_from_ranking(np.asarray(candidate_item_ids)[order], gt, ks))
         if log_interval and (idx + 1) % log_interval == 0:
@@ -114,7 +118,8 @@ def evaluate_ranking(model, eval_dataset, device, candidate_item_ids=None, ks=No
 
 
 def evaluate_ranking_peruser(model, eval_dataset, device, ks=None, task: str = "listen_plus", top_n: int = 100,
-                             batch_size: int = 1024, log_interval: int = 0) -> dict[str, float]:
+                             batch_size: int = 1024, log_interval: int = 0,
+                             kv_cache: str | None = None) -> dict[str, float]:
     """Per-user candidates = the user's unique train items; metrics on the top-N."""
     ks = ks or [10, 50, 100]
     model.eval()
@@ -130,7 +135,7 @@ def evaluate_ranking_peruser(model, eval_dataset, device, ks=None, task: str = "
         cand = eval_dataset.candidate_batch(items, device)
         ub = eval_dataset.user_batch(sample, device)
         s = score_candidates(model, ub, eval_dataset.with_user_features(cand, sample, items, device), task,
-                             batch_size)
+                             batch_size, kv_cache)
         order = torch.argsort(s, descending=True)[:top_n].cpu().numpy()
         per_user.append(metrics_from_ranking(np.asarray(items)[order], gt, ks))
         if log_interval and (idx + 1) % log_interval == 0:

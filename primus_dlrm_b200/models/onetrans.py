@@ -36,7 +36,9 @@ from primus_dlrm_b200.ops.attention import (
     _native_ok as _fmha_native_ok, causal_attention_all_rows, pyramid_attention, pyramid_attention_qkv,
 )
 from primus_dlrm_b200.ops.embedding import SparseOptimizer
-from primus_dlrm_b200.ops.norm import add_norm, make_norm, norm_with_tail
+from primus_dlrm_b200.ops.kv_cache import PagedKVCache, paged_attention
+from primus_dlrm_b200.ops.norm import RMSNorm, add_norm, make_norm, norm_with_tail
+from primus_dlrm_b200.ops.rotary import qk_norm_rope, rope_table
 
 
 def pyramid_schedule(l_s: int, l_ns: int, n_layers: int) -> list[int]:
@@ -55,7 +57,7 @@ def _xavier_per_token(w: torch.Tensor) -> None:
 
 class MixedAttention(nn.Module):
     def __init__(self, d_model: int, n_heads: int, n_ns_tokens: int, dropout: float = 0.0,
-                 attention_impl: str = "sdpa"):
+                 attention_impl: str = "sdpa", rotary: bool = False, rope_theta: float = 10000.0):
         super().__init__()
         if d_model % n_heads:
             raise ValueError("d_model must be divisible by n_heads")
@@ -74,6 +76,22 @@ class MixedAttention(nn.Module):
         nn.init.xavier_uniform_(self.s_qkv.weight)
         nn.init.xavier_uniform_(self.out_proj.weight)
         _xavier_per_token(self.ns_qkv_weight)
+        self.rotary, self.rope_theta = rotary, rope_theta
+        if rotary:
+            self.q_norm, self.k_norm = RMSNorm(self.d_head), RMSNorm(self.d_head)
+            self._rope: torch.Tensor | None = None
+
+    def rope(self, tokens: int, device) -> torch.Tensor:
+        """Angle table of at least ``tokens`` positions."""
+        if self._rope is None or self._rope.shape[0] < tokens or self._rope.device != torch.device(device):
+            self._rope = rope_table(max(256, 1 << (tokens - 1).bit_length()), self.d_head, self.rope_theta, device)
+        return self._rope
+
+    def norm_rope(self, q: torch.Tensor, k: torch.Tensor | None, tokens: int) -> tuple[torch.Tensor, torch.Tensor | None]:
+        """q (the last rows) and k of a ``tokens`` long sequence, normed per head and rotated."""
+        table = self.rope(tokens, q.device)
+        pos = None if k is not None else torch.arange(tokens - q.shape[1], tokens, device=q.device)
+        return qk_norm_rope(q, k, self.q_norm.weight, self.k_norm.weight, table, pos, eps=self.q_norm.eps)
 
     def forward(self, x: torch.Tensor, n_s: int, q_len: int) -> torch.Tensor:
         """x [B, T, D] (normed) -> out-projected attention of the last q_len
@@ -82,6 +100,12 @@ class MixedAttention(nn.Module):
         B, T, D = x.shape
         qkv = dense.mixed_linear(x, n_s, self.s_qkv.weight, self.ns_qkv_weight)  # [B, T, 3D]
         qkv = qkv.view(B, T, 3, self.n_heads, self.d_head)
+        if self.rotary:
+            q, k = self.norm_rope(qkv[:, T - q_len:, 0], qkv[:, :, 1], T)
+            impl = "mask" if not x.is_cuda or self.attention_impl in ("sdpa", "mask") else "auto"
+            drop = self.attn_drop if (self.training and self.attention_impl in ("sdpa", "fav2", "turbo")) else 0.0
+            out = pyramid_attention(q, k, qkv[:, :, 2].contiguous(), impl=impl, dropout_p=drop)
+            return dense.linear(self.out_proj, out.reshape(B, q_len, D))
         no_drop = not (self.training and self.attn_drop > 0 and self.attention_impl != "fav4")
         if x.is_cuda and self.attention_impl in ("fav4", "fav2", "turbo", "native") and no_drop \
                 and _fmha_native_ok(qkv):
@@ -127,10 +151,11 @@ class OneTransBlock(nn.Module):
     """Pre-norm block: z = x_tail + Attn(N1(x)); out = z + FFN(N2(z))."""
 
     def __init__(self, d_model: int, n_heads: int, n_ns_tokens: int, ffn_mult: int = 4,
-                 dropout: float = 0.0, attention_impl: str = "sdpa", norm: str = "rmsnorm"):
+                 dropout: float = 0.0, attention_impl: str = "sdpa", norm: str = "rmsnorm", rotary: bool = False,
+                 rope_theta: float = 10000.0):
         super().__init__()
         self.norm1 = make_norm(norm, d_model)
-        self.attn = MixedAttention(d_model, n_heads, n_ns_tokens, dropout, attention_impl)
+        self.attn = MixedAttention(d_model, n_heads, n_ns_tokens, dropout, attention_impl, rotary, rope_theta)
         self.norm2 = make_norm(norm, d_model)
         self.ffn = MixedFFN(d_model, d_model * ffn_mult, n_ns_tokens, dropout)
 
@@ -172,6 +197,52 @@ class AutoSplitTokenizer(nn.Module):
         return dense.mlp2(ns, self.proj[0], self.proj[2]).view(-1, self.n_ns_tokens, self.d_model)
 
 
+class _UserPages:
+    """One layer's 8-bit pages for scoring: a user's history, then the tokens of
+    up to ``slots`` candidates behind it at a time."""
+
+    def __init__(self, attn: MixedAttention, n_s: int, n_ns: int, slots: int, device):
+        self.attn, self.n_s, self.n_ns = attn, n_s, n_ns
+        P = 64
+        full, tail = divmod(n_s, P)                          # the history's full pages, tokens in the one behind
+        own = -(-(tail + n_ns) // P)                         # pages of a candidate
+        shared = full + (tail > 0)
+        self.cache = PagedKVCache(shared + slots * own, attn.n_heads, attn.d_head, P, device=device)
+        first = torch.arange(shared, dtype=torch.int32, device=device)
+        mine = shared + torch.arange(slots * own, dtype=torch.int32, device=device).view(slots, own)
+        self.history_table = first[None]
+        self.table = torch.cat([first[:full].expand(slots, -1), mine], dim=1)
+        self.tail = (first[full:].long().expand(slots), mine[:, 0].long()) if tail else None
+        self.norm = {}
+        if attn.rotary:
+            self.norm = dict(k_weight=attn.k_norm.weight, norm_eps=attn.k_norm.eps, rope=attn.rope(n_s + n_ns, device))
+
+    def _attend(self, q, table, tokens: int):
+        """The last rows' attention over ``tokens`` tokens of each sequence."""
+        lens = torch.full((q.shape[0],), tokens, dtype=torch.int32, device=q.device)
+        if self.attn.rotary:
+            q, _ = self.attn.norm_rope(q, None, tokens)
+        half = q.dtype if q.dtype in (torch.bfloat16, torch.float16) or not q.is_cuda else torch.bfloat16
+        return paged_attention(q.to(half), self.cache, table, lens, max_len=tokens).to(q.dtype)
+
+    def _append(self, k, v, table, held: int):
+        lens = torch.full((k.shape[0],), held, dtype=torch.int32, device=k.device)
+        self.cache.append(k, v, table, lens, **self.norm)
+
+    def history(self, q, k, v):
+        """Attention of the history's last queries; its keys and values stay in the cache."""
+        self._append(k, v, self.history_table, 0)
+        return self._attend(q, self.history_table, self.n_s)
+
+    def candidates(self, q, k, v):
+        """Attention of each candidate's tokens over the history and themselves."""
+        table = self.table[:q.shape[0]]
+        if self.tail is not None:                            # a copy of the partly filled page for each candidate
+            self.cache.copy_pages(self.tail[0][:q.shape[0]], self.tail[1][:q.shape[0]])
+        self._append(k, v, table, self.n_s)
+        return self._attend(q, table, self.n_s + self.n_ns)
+
+
 class OneTransModel(BaseModel):
     def __init__(self, config: Config, device: torch.device | None = None, meta_device: bool = False):
         super().__init__()
@@ -205,7 +276,7 @@ class OneTransModel(BaseModel):
         self.ns_tokenizer = AutoSplitTokenizer(ns_raw, ot.d_model, ot.n_ns_tokens).to(device)
         self.blocks = nn.ModuleList([
             OneTransBlock(ot.d_model, ot.n_heads, ot.n_ns_tokens, ot.ffn_mult, ot.dropout,
-                          attention_impl=ot.attention_impl, norm=ot.norm)
+                          attention_impl=ot.attention_impl, norm=ot.norm, rotary=ot.rotary, rope_theta=ot.rope_theta)
             for _ in range(ot.n_layers)
         ]).to(device)
         self.final_norm = make_norm(ot.norm, ot.d_model).to(device)
@@ -314,7 +385,7 @@ class OneTransModel(BaseModel):
     # ------------------------------------------------------------------
     @torch.no_grad()
     def score_candidates(self, user_batch: dict[str, torch.Tensor], candidate_batch: dict[str, torch.Tensor],
-                         task: str, batch_size: int = 1024) -> torch.Tensor:
+                         task: str, batch_size: int = 1024, kv_cache: str | None = None) -> torch.Tensor:
         """Scores [C] of one user against C candidates with an S-side K/V cache.
 
         S tokens sit before the NS tokens and attention is causal, so the S
@@ -325,7 +396,15 @@ class OneTransModel(BaseModel):
         same function as ``forward`` on (user history, candidate), at the cost
         of n_ns tokens per candidate instead of L_S + n_ns
         (``primus_dlrm/evaluation/metrics.py:200-279`` recomputes everything).
+
+        ``kv_cache="fp8"`` keeps the keys and values in pages of 8 bits
+        (``ops.kv_cache``): every candidate's page table names the user's full
+        pages, and only the last, partly filled one is copied, instead of
+        expanding the cache to each candidate.  The head dim is then 32, 64 or
+        128, and scores carry the rounding of 8-bit keys and values.
         """
+        if kv_cache not in (None, "fp8"):
+            raise ValueError(f"kv_cache {kv_cache!r}: expected None or 'fp8'")
         ot = self.config.model.transformer
         n_ns, H = ot.n_ns_tokens, ot.n_heads
         D = ot.d_model
@@ -347,10 +426,16 @@ class OneTransModel(BaseModel):
             qkv = (h @ at.s_qkv.weight.t().to(h.dtype)).view(1, -1, 3, H, dh)
             q_s = sched[l]                                   # S queries kept by this layer
             k_s, v_s = qkv[:, :, 1], qkv[:, :, 2]            # [1, n_s, H, dh]
-            cache.append((k_s, v_s))
             n_s = xs.shape[1]
             q = qkv[:, n_s - q_s:, 0]
-            o = pyramid_attention(q, k_s, v_s, impl="mask").reshape(1, q_s, D)
+            if kv_cache:
+                cache.append(_UserPages(at, n_s, n_ns, min(C, batch_size), xs.device))
+                o = cache[-1].history(q, k_s, v_s).reshape(1, q_s, D)
+            else:
+                if at.rotary:
+                    q, k_s = at.norm_rope(q, k_s, n_s)
+                cache.append((k_s, v_s))
+                o = pyramid_attention(q, k_s, v_s, impl="mask").reshape(1, q_s, D)
             z = at.out_proj(o) + xs[:, n_s - q_s:]
             y = blk.norm2(z)
             xs = z + blk.ffn.s_w2(F.gelu(blk.ffn.s_w1(y)))
@@ -367,14 +452,21 @@ class OneTransModel(BaseModel):
             x = self.ns_tokenizer(ns_raw)                    # [nb, n_ns, D]
             for l, blk in enumerate(self.blocks):
                 at = blk.attn
-                k_s, v_s = cache[l]
-                n_s = k_s.shape[1]
                 h = blk.norm1(x)
                 qkv = torch.einsum("btk,tnk->btn", h, at.ns_qkv_weight.to(h.dtype)).view(nb, n_ns, 3, H, dh)
                 q, k_n, v_n = qkv[:, :, 0], qkv[:, :, 1], qkv[:, :, 2]
-                k = torch.cat([k_s.expand(nb, -1, -1, -1).to(k_n.dtype), k_n], dim=1)
-                v = torch.cat([v_s.expand(nb, -1, -1, -1).to(v_n.dtype), v_n], dim=1)
-                o = pyramid_attention(q, k, v, impl="mask").reshape(nb, n_ns, D)
+                if kv_cache:
+                    o = cache[l].candidates(q, k_n, v_n).reshape(nb, n_ns, D)
+                else:
+                    k_s, v_s = cache[l]
+                    if at.rotary:                            # the last n_ns of n_s + n_ns tokens
+                        q, _ = at.norm_rope(q, None, k_s.shape[1] + n_ns)
+                        k_n, _ = qk_norm_rope(k_n, None, at.k_norm.weight, None, at.rope(k_s.shape[1] + n_ns, x.device),
+                                              torch.arange(k_s.shape[1], k_s.shape[1] + n_ns, device=x.device),
+                                              eps=at.k_norm.eps)
+                    k = torch.cat([k_s.expand(nb, -1, -1, -1).to(k_n.dtype), k_n], dim=1)
+                    v = torch.cat([v_s.expand(nb, -1, -1, -1).to(v_n.dtype), v_n], dim=1)
+                    o = pyramid_attention(q, k, v, impl="mask").reshape(nb, n_ns, D)
                 z = at.out_proj(o) + x
                 y = blk.norm2(z)
                 f = torch.einsum("btk,tnk->btn", y, blk.ffn.ns_w1.to(y.dtype))
@@ -383,6 +475,8 @@ class OneTransModel(BaseModel):
             x = self.final_norm(x)
             hh = self.head_proj(x.reshape(nb, -1))
             scores.append(self.heads[task](hh).squeeze(-1).float())
+        for pages in cache if kv_cache else ():
+            pages.cache.check_errors()
         return torch.cat(scores)
 
     def _ns_raw(self, batch: dict[str, torch.Tensor]) -> torch.Tensor:

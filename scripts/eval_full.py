@@ -34,6 +34,8 @@ def main(argv=None) -> dict:
     p.add_argument("--eval-top-k", type=int, default=0, help="global mode: 0 = full catalog, K = top-K popular")
     p.add_argument("--top-n", type=int, default=100)
     p.add_argument("--score-batch-size", type=int, default=8192)
+    p.add_argument("--kv-cache", choices=["fp8"], default=None,
+                   help="OneTrans: keep the history's keys and values in 8-bit pages (head dim 32, 64 or 128)")
     a = p.parse_args(argv)
     from primus_dlrm_b200.config import Config
     from primus_dlrm_b200.data.dataset import DataPaths, YambdaEvalDataset
@@ -60,10 +62,10 @@ def main(argv=None) -> dict:
                 cand = (np.arange(ds.num_items) if a.eval_top_k <= 0
                         else np.argsort(-ds.item_popularity)[: a.eval_top_k])
                 res = evaluate_ranking(model, ds, dev, candidate_item_ids=cand, ks=ks, task=a.task,
-                                       batch_size=a.score_batch_size)
+                                       batch_size=a.score_batch_size, kv_cache=a.kv_cache)
             else:
                 res = evaluate_ranking_peruser(model, ds, dev, ks=ks, task=a.task, top_n=a.top_n,
-                                               batch_size=a.score_batch_size)
+                                               batch_size=a.score_batch_size, kv_cache=a.kv_cache)
     logger.info("[%s %s] %s", a.mode, a.task, " | ".join(f"{k}={v:.4f}" if isinstance(v, float) else f"{k}={v}"
                                                          for k, v in sorted(res.items())))
     return res

@@ -45,10 +45,7 @@ ext_modules = [
         name="primus_dlrm_b200._kv",
         sources=kv_sources,
         include_dirs=[os.path.join(ROOT, "csrc")],
-        extra_compile_args={
-            "cxx": CXX,
-            "nvcc": NVCC_COMMON + (["-Xptxas=-v"] if os.environ.get("PD_PTXAS_V") else []),
-        },
+        extra_compile_args={"cxx": CXX, "nvcc": NVCC_COMMON},
     ),
 ]
 if os.path.exists(os.path.join(ROOT, "csrc", "gemm_bindings.cpp")):
