@@ -28,9 +28,7 @@ void check_ints(const at::Tensor&, const at::Tensor&, int64_t, const char*);
 void check_table(const at::Tensor&, const at::Tensor&);
 
 constexpr uint64_t kWaitLimitNs = 2000000000ull;
-constexpr int kWarps = 4;               // warps of a block: they share a segment's keys
-constexpr int kRows = 16;               // rows (query, head of the group) of a segment
-constexpr int kMaxPages = 4;            // pages of a tile of keys (64 / 16)
+constexpr int kWarps = 4;               // warps of a block
 
 struct AttnArgs {
   const void* q;                // token, head (and batch) strides below
@@ -45,17 +43,18 @@ struct AttnArgs {
   bool causal, split, bf16;
   int min_units;
   float scale_log2;
-  float* part_o;                // split: [2 grid, 16, d] sums, [2 grid, 16, 2] (max, sum), [2 grid, 4] heads
+  float* part_o;                // split: [2 grid, R, d] sums, [2 grid, R, 2] (max, sum), [2 grid, 4] heads
   float* part_ml;
   int* part_head;
   int* err;
 };
 
 template <int D> struct Cfg;
-// TK keys a tile and warp (8 KB of keys and values for d = 64 and 128), ST tiles in flight
-template <> struct Cfg<32> { static constexpr int TK = 64, ST = 4; };
-template <> struct Cfg<64> { static constexpr int TK = 64, ST = 3; };
-template <> struct Cfg<128> { static constexpr int TK = 32, ST = 3; };
+// TK keys a tile and warp (8 KB of keys and values), ST tiles in flight: three
+// blocks of four warps an SM
+template <> struct Cfg<32> { static constexpr int TK = 128, ST = 2; };
+template <> struct Cfg<64> { static constexpr int TK = 64, ST = 2; };
+template <> struct Cfg<128> { static constexpr int TK = 32, ST = 2; };
 
 __device__ __forceinline__ uint32_t smem_u32(const void* p) {
   return static_cast<uint32_t>(__cvta_generic_to_shared(p));
@@ -132,17 +131,24 @@ __device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
   const __half2 v = __floats2half2_rn(lo, hi);
   return *reinterpret_cast<const uint32_t*>(&v);
 }
+// the transpose of an 8 x 8 tile of 16-bit values (lane: row lane / 4, columns 2 (lane % 4) and the next)
+__device__ __forceinline__ uint32_t transpose8(uint32_t x) {
+  uint32_t y;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
 // D(16x8 f32) += A(16x16 f16, row) * B(16x8 f16, col)
 __device__ __forceinline__ void mma_f16(float* d, const uint32_t* a, uint32_t b0, uint32_t b1) {
-  asm volatile(
+  asm(
       "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
 // The queries and keys of one sequence, with impossible lengths cut (and reported).
+template <int R>
 struct Seq {
-  int len, n, tok0, tiles_m;
+  int len, n, tok0, tiles_m;                // tiles_m: segments of R rows (query, head of the group) for a key head
   __device__ __forceinline__ void load(const AttnArgs& A, int b) {
     len = __ldg(A.lens + b);
     if (A.cu) {
@@ -164,21 +170,22 @@ struct Seq {
       set_error(A.err, kBadShape);
       len = 0;
     }
-    tiles_m = int((int64_t(n) * A.G + kRows - 1) / kRows);
+    tiles_m = int((int64_t(n) * A.G + R - 1) / R);
   }
-  // units of kWarps tiles of keys in each of its segments; a sequence without keys has one (it writes zeros)
+  // units of `sup` keys in each of its segments; a sequence without keys has one (it writes zeros)
   __device__ __forceinline__ int units(int sup) const { return max(1, (len + sup - 1) / sup); }
   __device__ __forceinline__ int64_t all(int H, int sup) const { return int64_t(units(sup)) * H * tiles_m; }
 };
 
 // A place in the list of units: sequence b, segment (head, row tile) in it, unit of its keys.
+template <int R>
 struct Cursor {
   int b, h, mt, unit, units;
-  Seq s;
+  Seq<R> s;
   int lim;                        // keys that the row tile's last row sees
-  int64_t left;                   // units from here to the end of this block's range
+  int left;                       // units from here to the end of this worker's range
   __device__ __forceinline__ void limits(const AttnArgs& A) {
-    const int last = min(mt * kRows + kRows, s.n * A.G) - 1;
+    const int last = min(mt * R + R, s.n * A.G) - 1;
     lim = A.causal ? max(0, s.len - s.n + last / A.G + 1) : s.len;
   }
   __device__ __forceinline__ void next_seq(const AttnArgs& A, int sup) {
@@ -204,26 +211,43 @@ struct Cursor {
   }
 };
 
-template <int D>
-__global__ void __launch_bounds__(kWarps * 32, D == 128 ? 2 : 3)
+// Few rows to a segment (one or some query tokens of one sequence, the heads
+// that share a key head): bound by reading the cache.
+//
+// W warps take a segment's keys in turn, a tile of TK keys each, from rings of
+// their own that TMA fills (one copy a page, 32 to 128 bytes a row, swizzled by
+// the hardware so that fragments load without bank conflicts); W = 1 where
+// there are segments enough for every warp. Blocks (W = 4) take equal shares
+// of all tiles of all segments where segments are few, their pieces are joined
+// by a second launch.
+//
+// R = 16: a warp's rows are the A operand of S = Q K^T, R = 8 (up to 8 rows):
+// keys and values are, S^T = K Q^T and O^T = V^T P^T, with half the products
+// and registers; P^T turns from accumulator into operand by movmatrix. Dims
+// are dealt to lanes so that a lane's four codes of a step of 16 dims are
+// neighbours: lane % 4 owns a quarter of a key's dims, lane / 4 an eighth of a
+// value's, and keys go to registers in the order of memory.
+template <int D, int R, int W>
+__global__ void __launch_bounds__(kWarps * 32, D == 128 && R == 16 ? 2 : 3)
 paged_attn_kernel(const AttnArgs A, const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v) {
   constexpr int TK = Cfg<D>::TK, ST = Cfg<D>::ST;
-  constexpr int SUP = TK * kWarps;
-  constexpr int NT = TK / 8;            // 8-key column tiles of the scores
+  constexpr int SUP = TK * W;           // keys of a unit
   constexpr int KS = D / 16;            // steps of 16 dims
   constexpr int TS = TK / 16;           // steps of 16 keys
-  constexpr int NO = D / 8;             // 8-column tiles of the output
+  constexpr int SF = R == 16 ? 2 * TS : TS;   // score fragments of a tile
+  constexpr int NO = R * D / 128;       // output fragments
+  constexpr int NP = TK / 16;           // most pages of a tile
   constexpr int kHalf = TK * D;         // bytes of a tile's keys
   extern __shared__ __align__(1024) uint8_t s_ring[];       // [kWarps][ST] tiles: TK rows of keys, TK rows of values
-  __shared__ float s_merge[2][kRows * D];
-  __shared__ float s_ml[2][kRows][2];
+  __shared__ float s_merge[W > 1 ? 2 : 1][W > 1 ? R * D : 1];
+  __shared__ float s_ml[2][R][2];
   __shared__ uint64_t s_bar[kWarps][ST];
-  __shared__ int s_blk[kWarps][ST][kMaxPages];              // page * H + head of each page of a tile, or -1
-  __shared__ int64_t s_scan[kWarps], s_start[2];
+  __shared__ int64_t s_scan[kWarps], s_start[kWarps / W][2];
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int part = W == 1 ? 0 : warp;                       // of the segment's warps
   const int g = lane >> 2, qd = lane & 3;
-  const uint32_t ring = ((smem_u32(s_ring) + 1023) & ~1023u) + warp * ST * 2 * kHalf;
+  const uint32_t ring = smem_u32(s_ring) + warp * ST * 2 * kHalf;
   const uint32_t bars = smem_u32(s_bar[warp]);
   if (lane < ST) {
     asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(bars + lane * 8));
@@ -233,16 +257,19 @@ paged_attn_kernel(const AttnArgs A, const __grid_constant__ CUtensorMap tm_k, co
     asm volatile("prefetch.tensormap [%0];" ::"l"(&tm_k) : "memory");
     asm volatile("prefetch.tensormap [%0];" ::"l"(&tm_v) : "memory");
   }
+  if (threadIdx.x < kWarps / W) s_start[threadIdx.x][1] = -1;
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
-  // ---- this block's range of units: each thread counts a run of sequences ----
-  Cursor c;
+  // ---- this worker's range of units: each thread counts a run of sequences ----
+  Cursor<R> c;
+  c.left = 0;
   {
-    const int per = (A.B + blockDim.x - 1) / blockDim.x;
+    constexpr int kWorkers = kWarps / W;                    // of a block
+    const int per = (A.B + kWarps * 32 - 1) / (kWarps * 32);
     const int lo = min(int(threadIdx.x) * per, A.B), hi = min(lo + per, A.B);
     int64_t mine = 0;
     for (int b = lo; b < hi; ++b) {
-      Seq s;
+      Seq<R> s;
       s.load(A, b);
       mine += A.split ? s.all(A.H, SUP) : int64_t(A.H) * s.tiles_m;
     }
@@ -255,45 +282,48 @@ paged_attn_kernel(const AttnArgs A, const __grid_constant__ CUtensorMap tm_k, co
     if (lane == 31) s_scan[warp] = incl;
     __syncthreads();
     int64_t before = incl - mine, total = 0;
+#pragma unroll
     for (int w = 0; w < kWarps; ++w) {
       if (w < warp) before += s_scan[w];
       total += s_scan[w];
     }
     // split: equal shares of the units; else equal shares of the segments
-    const int64_t share = max(int64_t(A.split ? A.min_units : 1), (total + gridDim.x - 1) / gridDim.x);
-    const int64_t u0 = share * blockIdx.x, u1 = min(total, u0 + share);
-    __syncthreads();
-    if (threadIdx.x == 0) s_start[1] = -1;
-    __syncthreads();
-    if (u0 < u1 && before <= u0 && u0 < before + mine) {
-      int64_t at = before;
-      for (int b = lo; b < hi; ++b) {
-        Seq s;
-        s.load(A, b);
-        const int64_t k = A.split ? s.all(A.H, SUP) : int64_t(A.H) * s.tiles_m;
-        if (u0 < at + k) {
-          s_start[0] = u0 - at;
-          s_start[1] = b;
-          break;
+    const int64_t workers = int64_t(gridDim.x) * kWorkers;
+    const int64_t share = max(int64_t(A.split ? A.min_units : 1), (total + workers - 1) / workers);
+#pragma unroll 1
+    for (int w = 0; w < kWorkers; ++w) {
+      const int64_t u0 = share * (int64_t(blockIdx.x) * kWorkers + w);
+      if (u0 < total && before <= u0 && u0 < before + mine) {
+        int64_t at = before;
+        for (int b = lo; b < hi; ++b) {
+          Seq<R> s;
+          s.load(A, b);
+          const int64_t k = A.split ? s.all(A.H, SUP) : int64_t(A.H) * s.tiles_m;
+          if (u0 < at + k) {
+            s_start[w][0] = u0 - at;
+            s_start[w][1] = b;
+            break;
+          }
+          at += k;
         }
-        at += k;
       }
     }
     __syncthreads();
-    c.b = int(s_start[1]);
-    c.left = 0;
+    const int me = W == 1 ? warp : 0;
+    const int64_t u0 = share * (int64_t(blockIdx.x) * kWorkers + me), u1 = min(total, u0 + share);
+    c.b = int(s_start[me][1]);
     if (c.b >= 0) {
       c.s.load(A, c.b);
       c.units = c.s.units(SUP);
-      int64_t r = s_start[0];
+      int64_t r = s_start[me][0];
       c.unit = A.split ? int(r % c.units) : 0;
       if (A.split) r /= c.units;
       c.mt = int(r % c.s.tiles_m);
       c.h = int(r / c.s.tiles_m);
-      c.left = u1 - u0;
+      c.left = int(u1 - u0);
       if (!A.split) {
         // whole segments: count their units
-        Cursor t = c;
+        Cursor<R> t = c;
         int64_t units = 0, segs = u1 - u0;
         while (segs > 0) {
           const int64_t here = min(segs, int64_t(A.H - t.h) * t.s.tiles_m - t.mt);
@@ -303,61 +333,64 @@ paged_attn_kernel(const AttnArgs A, const __grid_constant__ CUtensorMap tm_k, co
           t.left = 1;
           if (segs > 0) t.next_seq(A, SUP);
         }
-        c.left = units;
+        c.left = int(units);
       }
       c.limits(A);
     }
   }
   if (A.split && threadIdx.x < 2) A.part_head[(blockIdx.x * 2 + threadIdx.x) * 4] = -1;
-  if (c.left <= 0) return;
+  if (c.left <= 0) return;                  // a whole block for W > 1, a warp for W = 1
 
   // ---- producer: this warp's tile of each unit ----
-  Cursor p = c;
-  int issued = 0;
+  // Lane i < NP loads key scales, lane NP + i value scales, of page i of a tile, into a register for each tile in
+  // flight; `gone` has a bit for each of its pages that is not loaded (behind the keys, or no such page).
+  Cursor<R> p = c;
   int page = -1;                            // lane i: id of page i of the tile at p
-  const int box = min(A.P, TK), boxes = TK / box, box_log = min(A.logP, TK == 64 ? 6 : 5);
+  const int box = min(A.P, TK), boxes = TK / box;
+  const int box_log = TK <= 64 ? min(A.logP, TK == 64 ? 6 : 5) : A.logP;
+  float scl[ST];
+  uint32_t gone[ST];
+#pragma unroll
+  for (int i = 0; i < ST; ++i) scl[i] = 0.f, gone[i] = 0;
   auto fetch_page = [&]() {
     page = -1;
-    const int key = p.unit * SUP + warp * TK + lane * box;
+    const int key = p.unit * SUP + part * TK + lane * box;
     if (p.left > 0 && lane < boxes && key < p.lim) page = __ldg(A.table + p.b * A.table_stride + (key >> A.logP));
   };
-  auto issue = [&]() {
+  auto issue = [&](int st, float& sc, uint32_t& gn) {
     if (p.left <= 0) return;
-    const int st = issued % ST;
     const uint32_t bar = bars + st * 8, dst = ring + st * 2 * kHalf;
-    const int key = p.unit * SUP + warp * TK + lane * box;
+    const int key = p.unit * SUP + part * TK + lane * box;
     const bool want = lane < boxes && key < p.lim;
     const bool have = want && page >= 0 && page < A.n_pages;
     if (want && !have) set_error(A.err, kIdOutOfRange);
     const int block = have ? page * A.H + p.h : -1;
-    if (lane < kMaxPages) s_blk[warp][st][lane] = block;
     const uint32_t mask = __ballot_sync(0xffffffffu, have);
+    gn = ~mask;
+    const int bk = __shfl_sync(0xffffffffu, block, lane % NP);
     const int row = have ? block * A.P + (key & (A.P - 1)) : 0;
-    int rows_of[kMaxPages];
-#pragma unroll
-    for (int i = 0; i < kMaxPages; ++i) rows_of[i] = __shfl_sync(0xffffffffu, row, i);
-    // one lane issues every copy: a copy's operands are uniform registers
-    if (lane == 0) {
+    if (lane == 0)
       asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;"
                    ::"r"(bar), "r"(uint32_t(__popc(mask) * 2 * box * D)) : "memory");
-#pragma unroll
-      for (int i = 0; i < kMaxPages; ++i)
-        if (mask >> i & 1) {
-          tma_rows(dst + i * box * D, &tm_k, bar, rows_of[i]);
-          tma_rows(dst + kHalf + i * box * D, &tm_v, bar, rows_of[i]);
-        }
+#pragma unroll 1
+    for (int i = 0; i < boxes; ++i) {
+      const int row_i = __shfl_sync(0xffffffffu, row, i);
+      if (lane == 0 && (mask >> i & 1)) {
+        tma_rows(dst + i * box * D, &tm_k, bar, row_i);
+        tma_rows(dst + kHalf + i * box * D, &tm_v, bar, row_i);
+      }
     }
+    sc = lane < 2 * NP && bk >= 0 ? __ldg((lane < NP ? A.ks : A.vs) + bk) : 0.f;
     __syncwarp();
-    ++issued;
     p.next(A, SUP);
     fetch_page();
   };
   fetch_page();
-#pragma unroll 1
-  for (int i = 0; i < ST - 1; ++i) issue();
+#pragma unroll
+  for (int i = 0; i < ST - 1; ++i) issue(i, scl[i], gone[i]);
 
   // ---- consumer ----
-  uint32_t k_off, v_off[2];                 // this lane's bytes in a tile: K row g, V rows 2 qd and 2 qd + 1
+  uint32_t k_off, v_off[2];                 // this lane's bytes in a tile: key row g, value rows 2 qd and 2 qd + 1
   if (D == 128) {
     k_off = g * 128 + ((2 * qd) ^ g) * 16;
     v_off[0] = (2 * qd) * 128 + (g ^ (2 * qd)) * 16;
@@ -371,36 +404,26 @@ paged_attn_kernel(const AttnArgs A, const __grid_constant__ CUtensorMap tm_k, co
     v_off[0] = (2 * qd) * 32 + ((g >> 2) ^ (qd >> 1)) * 16 + (g & 3) * 4;
     v_off[1] = v_off[0] + 32;
   }
-  float scl = 0.f;                          // lane i < 4: key scale of page i of the next tile, 4 <= i < 8: value scale
-  auto fetch_scales = [&](int t) {
-    scl = 0.f;
-    if (lane < 2 * kMaxPages) {
-      const int bk = s_blk[warp][t % ST][lane & 3];
-      if (bk >= 0) scl = __ldg((lane < kMaxPages ? A.ks : A.vs) + bk);
-    }
-  };
-  __syncwarp();
-  fetch_scales(0);
+  // the two rows of this lane's accumulators
+  const int row_a = R == 16 ? g : 2 * qd, row_b = R == 16 ? g + 8 : 2 * qd + 1;
   bool alive = true;
-  int taken = 0;
-  bool first = true;                        // of this block's segments
+  uint32_t st = 0, phase = 0;               // slot of the ring and its turn
+  bool first = true;                        // of this worker's segments
   while (c.left > 0) {
     // ---- a segment: this warp's share of its keys ----
-    const int seg_b = c.b, seg_h = c.h, seg_mt = c.mt;
-    const Seq S = c.s;
+    const int seg_b = c.b, seg_h = c.h, r0 = c.mt * R;
+    const Seq<R> S = c.s;
     const bool begins = c.unit == 0;
-    const int seg_lim = c.lim;
-    const int r0 = seg_mt * kRows + g, rows = S.n * A.G;
-    int lim0 = 0, lim1 = 0, min_lim = 0;
-    uint32_t qf[KS][4];
+    const int seg_lim = c.lim, rows = S.n * A.G;
+    const int seg_mt = c.mt;
+    uint32_t qf[KS][R / 4];
     float rs0, rs1;                         // softmax scale of the two rows, in the log2 domain
     {
-      float amax[2] = {0.f, 0.f};
       constexpr int E = D / 4;              // dims of a lane
-      float x[2][E];
+      float x[R / 8][E], back[R / 8];
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const int r = r0 + 8 * i;
+      for (int i = 0; i < R / 8; ++i) {
+        const int r = r0 + g + 8 * i;
         const bool live = r < rows;
         const int qi = live ? r / A.G : 0;
         const uint16_t* src = static_cast<const uint16_t*>(A.q) +
@@ -418,28 +441,42 @@ paged_attn_kernel(const AttnArgs A, const __grid_constant__ CUtensorMap tm_k, co
             for (int e = 0; e < E; ++e) x[i][e] = to_f_16(src[e], A.bf16);
           }
         }
+        float amax = 0.f;
 #pragma unroll
-        for (int e = 0; e < E; ++e) amax[i] = fmaxf(amax[i], fabsf(x[i][e]));
-        amax[i] = fmaxf(amax[i], __shfl_xor_sync(0xffffffffu, amax[i], 1));
-        amax[i] = fmaxf(amax[i], __shfl_xor_sync(0xffffffffu, amax[i], 2));
-        const int lm = !live ? 0 : A.causal ? max(0, S.len - S.n + qi + 1) : S.len;
-        if (i == 0) lim0 = lm; else lim1 = lm;
-      }
-      // 2^(14 - exponent): an infinity or NaN keeps its row's scale at 1
-      const int e0 = amax[0] < INFINITY ? max(-100, (__float_as_int(amax[0]) >> 23) - 127) : 14;
-      const int e1 = amax[1] < INFINITY ? max(-100, (__float_as_int(amax[1]) >> 23) - 127) : 14;
-      const float up0 = __int_as_float((14 - e0 + 127) << 23), up1 = __int_as_float((14 - e1 + 127) << 23);
-      rs0 = __int_as_float((e0 - 14 + 127) << 23) * A.scale_log2;
-      rs1 = __int_as_float((e1 - 14 + 127) << 23) * A.scale_log2;
+        for (int e = 0; e < E; ++e) amax = fmaxf(amax, fabsf(x[i][e]));
+        amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+        amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
+        // 2^(14 - exponent), negative for a negative softmax scale; a row of zeros, an infinity or NaN stays as it is
+        const int ex = amax > 0.f && amax < INFINITY ? max(-100, (__float_as_int(amax) >> 23) - 127) : 14;
+        const float up = copysignf(__int_as_float((14 - ex + 127) << 23), A.scale_log2);
+        back[i] = __int_as_float((ex - 14 + 127) << 23) * fabsf(A.scale_log2);
 #pragma unroll
-      for (int k = 0; k < KS; ++k) {
-        qf[k][0] = pack_f16(x[0][4 * k] * up0, x[0][4 * k + 1] * up0);
-        qf[k][1] = pack_f16(x[1][4 * k] * up1, x[1][4 * k + 1] * up1);
-        qf[k][2] = pack_f16(x[0][4 * k + 2] * up0, x[0][4 * k + 3] * up0);
-        qf[k][3] = pack_f16(x[1][4 * k + 2] * up1, x[1][4 * k + 3] * up1);
+        for (int e = 0; e < E; ++e) x[i][e] *= up;
       }
-      min_lim = A.causal ? S.len - S.n + seg_mt * kRows / A.G + 1 : S.len;
+      if constexpr (R == 16) {
+        rs0 = back[0];
+        rs1 = back[R / 8 - 1];
+#pragma unroll
+        for (int k = 0; k < KS; ++k) {
+          qf[k][0] = pack_f16(x[0][4 * k], x[0][4 * k + 1]);
+          qf[k][1] = pack_f16(x[R / 8 - 1][4 * k], x[R / 8 - 1][4 * k + 1]);
+          qf[k][R / 4 - 2] = pack_f16(x[0][4 * k + 2], x[0][4 * k + 3]);
+          qf[k][R / 4 - 1] = pack_f16(x[R / 8 - 1][4 * k + 2], x[R / 8 - 1][4 * k + 3]);
+        }
+      } else {
+        rs0 = __shfl_sync(0xffffffffu, back[0], row_a * 4);
+        rs1 = __shfl_sync(0xffffffffu, back[0], row_b * 4);
+#pragma unroll
+        for (int k = 0; k < KS; ++k) {
+          qf[k][0] = pack_f16(x[0][4 * k], x[0][4 * k + 1]);
+          qf[k][1] = pack_f16(x[0][4 * k + 2], x[0][4 * k + 3]);
+        }
+      }
     }
+    // keys that each of the two rows sees, and the fewest of any row
+    auto limit = [&](int r) { return r >= rows ? 0 : A.causal ? max(0, S.len - S.n + r / A.G + 1) : S.len; };
+    const int lim0 = limit(r0 + row_a), lim1 = limit(r0 + row_b);
+    const int min_lim = A.causal ? S.len - S.n + r0 / A.G + 1 : S.len;
     float o[NO][4];
 #pragma unroll
     for (int u = 0; u < NO; ++u) o[u][0] = o[u][1] = o[u][2] = o[u][3] = 0.f;
@@ -447,137 +484,197 @@ paged_attn_kernel(const AttnArgs A, const __grid_constant__ CUtensorMap tm_k, co
 
     bool ends = false;
     do {
-      const int st = taken % ST;
-      const int k0 = c.unit * SUP + warp * TK;
-      issue();                              // refills the slot of the tile before
-      const float my_scl = scl;
-      if (c.left > 1) fetch_scales(taken + 1);
-      if (alive) alive = mbar_wait(bars + st * 8, (taken / ST) & 1, A.err);
+      const int k0 = c.unit * SUP + part * TK;
+      issue(st == 0 ? ST - 1 : st - 1, scl[ST - 1], gone[ST - 1]);    // refills the slot of the tile before
+      const float my_scl = scl[0];
+      const uint32_t my_gone = gone[0];
+      if (alive) alive = mbar_wait(bars + st * 8, phase, A.err);
+      __syncwarp();
       if (k0 < seg_lim) {
         const uint32_t kt = ring + st * 2 * kHalf, vt = kt + kHalf;
-        // scores
-        float s[NT][4];
-#pragma unroll
-        for (int j = 0; j < NT; ++j) {
-          uint32_t w[KS];
+        // ---- scores: fragment j holds keys 8 j.. (R = 16) or 16 j.. (R = 8) ----
+        float s[SF][4];
+        auto load_keys = [&](int row, uint32_t* w) {          // words of this lane's dims of key `row` + g
           if constexpr (D == 128) {
-            const uint4 a = lds128(kt + k_off + j * 8 * D), b = lds128(kt + (k_off ^ 16) + j * 8 * D);
+            const uint4 a = lds128(kt + k_off + row * D), b = lds128(kt + (k_off ^ 16) + row * D);
             w[0] = a.x; w[1] = a.y; w[2] = a.z; w[3] = a.w;
             w[4] = b.x; w[5] = b.y; w[6] = b.z; w[7] = b.w;
           } else if constexpr (D == 64) {
-            const uint4 a = lds128(kt + k_off + j * 8 * D);
+            const uint4 a = lds128(kt + k_off + row * D);
             w[0] = a.x; w[1] = a.y; w[2] = a.z; w[3] = a.w;
           } else {
-            const uint2 a = lds64(kt + k_off + j * 8 * D);
+            const uint2 a = lds64(kt + k_off + row * D);
             w[0] = a.x; w[1] = a.y;
           }
-          s[j][0] = s[j][1] = s[j][2] = s[j][3] = 0.f;
+        };
 #pragma unroll
-          for (int k = 0; k < KS; ++k) {
-            uint32_t b0, b1;
-            cvt4(w[k], b0, b1);
-            mma_f16(s[j], qf[k], b0, b1);
+        for (int j = 0; j < SF; ++j) {
+          s[j][0] = s[j][1] = s[j][2] = s[j][3] = 0.f;
+          if constexpr (R == 16) {
+            uint32_t w[KS];
+            load_keys(8 * j, w);
+#pragma unroll
+            for (int k = 0; k < KS; ++k) {
+              uint32_t b0, b1;
+              cvt4(w[k], b0, b1);
+              mma_f16(s[j], qf[k], b0, b1);
+            }
+          } else {
+            uint32_t w[KS], x[KS];
+            load_keys(16 * j, w);
+            load_keys(16 * j + 8, x);
+#pragma unroll
+            for (int k = 0; k < KS; ++k) {
+              uint32_t a[4];
+              cvt4(w[k], a[0], a[2]);
+              cvt4(x[k], a[1], a[3]);
+              mma_f16(s[j], a, qf[k][0], qf[k][1]);
+            }
           }
         }
-        // scales of the pages, masks
+        uint32_t vw[TS][4][D / 32];
+        auto load_values = [&]() {
+#pragma unroll
+          for (int i = 0; i < TS; ++i)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+              const uint32_t a = vt + v_off[r & 1] + (16 * i + 8 * (r >> 1)) * D;
+              if constexpr (D == 128) {
+                const uint4 t = lds128(a);
+                vw[i][r][0] = t.x; vw[i][r][1] = t.y; vw[i][r][2] = t.z; vw[i][r][3] = t.w;
+              } else if constexpr (D == 64) {
+                const uint2 t = lds64(a);
+                vw[i][r][0] = t.x; vw[i][r][1] = t.y;
+              } else {
+                vw[i][r][0] = lds32(a);
+              }
+            }
+        };
+        if constexpr (R == 8) load_values();  // on their way while the softmax runs; R = 16 has no registers for that
+        // ---- masks: behind a row's keys, and pages that were not loaded ----
         const int end = min(TK, seg_lim - k0);                        // keys of the tile that some row sees
-        bool hole = false;
-        float vrel[TS], vref = 0.f;
+        // a page in front of `end` is missing
+        const bool hole = my_gone & ((1u << ((end + box - 1) >> box_log)) - 1);
+        if (k0 + TK > min_lim || hole) {
+#pragma unroll
+          for (int j = 0; j < SF; ++j)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const int at = R == 16 ? 8 * j + 2 * qd + (e & 1) : 16 * j + g + 8 * (e >> 1);
+              const bool second = R == 16 ? e >> 1 : e & 1;
+              if (k0 + at >= (second ? lim1 : lim0)) s[j][e] = -INFINITY;
+              if (my_gone >> (at >> box_log) & 1) s[j][e] = -INFINITY;
+            }
+        }
+        // ---- running maximum ----
+        float vref, f0[TS], f1[TS], rel[TS];                          // by step of 16 keys
+        float x0 = -INFINITY, x1 = -INFINITY;
+        if (boxes == 1) {
+          const float ks = __shfl_sync(0xffffffffu, my_scl, 0);
+          vref = __shfl_sync(0xffffffffu, my_scl, NP);
+#pragma unroll
+          for (int i = 0; i < TS; ++i) {
+            f0[i] = fmaxf(ks * rs0, 1.17549435e-38f);                 // 0 would turn -inf into NaN
+            f1[i] = fmaxf(ks * rs1, 1.17549435e-38f);
+            rel[i] = 1.f;
+          }
+        } else {
+          vref = 0.f;
+#pragma unroll
+          for (int i = 0; i < TS; ++i) {
+            const int pg = (i * 16) >> box_log;
+            const float ks = __shfl_sync(0xffffffffu, my_scl, pg);
+            f0[i] = fmaxf(ks * rs0, 1.17549435e-38f);
+            f1[i] = fmaxf(ks * rs1, 1.17549435e-38f);
+            rel[i] = __shfl_sync(0xffffffffu, my_scl, pg + NP);
+            vref = fmaxf(vref, rel[i]);
+          }
+          const float vinv = vref > 0.f ? 1.f / vref : 0.f;
+#pragma unroll
+          for (int i = 0; i < TS; ++i) rel[i] *= vinv;
+        }
+        constexpr int PS = SF / TS;                                   // fragments of a step of 16 keys
 #pragma unroll
         for (int i = 0; i < TS; ++i) {
-          const int pg = (i * 16) >> box_log;
-          const float ks = __shfl_sync(0xffffffffu, my_scl, pg);
-          const float vs = __shfl_sync(0xffffffffu, my_scl, pg + kMaxPages);
-          vrel[i] = vs;
-          vref = fmaxf(vref, vs);
-          const bool bad = s_blk[warp][st][pg] < 0;              // not loaded: behind the keys, or no such page
-          hole |= bad;
-          const float f0 = ks * rs0, f1 = ks * rs1;
+          float y0 = -INFINITY, y1 = -INFINITY;
 #pragma unroll
-          for (int j = 2 * i; j < 2 * i + 2; ++j) {
-            s[j][0] = bad ? -INFINITY : s[j][0] * f0;
-            s[j][1] = bad ? -INFINITY : s[j][1] * f0;
-            s[j][2] = bad ? -INFINITY : s[j][2] * f1;
-            s[j][3] = bad ? -INFINITY : s[j][3] * f1;
+          for (int j = PS * i; j < PS * i + PS; ++j) {
+            y0 = fmaxf(y0, fmaxf(s[j][0], s[j][R == 16 ? 1 : 2]));
+            y1 = fmaxf(y1, fmaxf(s[j][R == 16 ? 2 : 1], s[j][3]));
           }
+          x0 = fmaxf(x0, y0 * f0[i]);
+          x1 = fmaxf(x1, y1 * f1[i]);
         }
-        if (k0 + TK > min_lim) {
 #pragma unroll
-          for (int j = 0; j < NT; ++j) {
-            const int key = k0 + 8 * j + 2 * qd;
-            if (key >= lim0) s[j][0] = -INFINITY;
-            if (key + 1 >= lim0) s[j][1] = -INFINITY;
-            if (key >= lim1) s[j][2] = -INFINITY;
-            if (key + 1 >= lim1) s[j][3] = -INFINITY;
-          }
+        for (int t = R == 16 ? 1 : 4; t < (R == 16 ? 4 : 32); t *= 2) {
+          x0 = fmaxf(x0, __shfl_xor_sync(0xffffffffu, x0, t));
+          x1 = fmaxf(x1, __shfl_xor_sync(0xffffffffu, x1, t));
         }
-        // running maximum and sum
-        float x0 = m0, x1 = m1;
-#pragma unroll
-        for (int j = 0; j < NT; ++j) {
-          x0 = fmaxf(x0, fmaxf(s[j][0], s[j][1]));
-          x1 = fmaxf(x1, fmaxf(s[j][2], s[j][3]));
-        }
-        x0 = fmaxf(x0, __shfl_xor_sync(0xffffffffu, x0, 1));
-        x1 = fmaxf(x1, __shfl_xor_sync(0xffffffffu, x1, 1));
-        x0 = fmaxf(x0, __shfl_xor_sync(0xffffffffu, x0, 2));
-        x1 = fmaxf(x1, __shfl_xor_sync(0xffffffffu, x1, 2));
+        x0 = fmaxf(x0, m0);
+        x1 = fmaxf(x1, m1);
         const float b0 = x0 == -INFINITY ? 0.f : x0, b1 = x1 == -INFINITY ? 0.f : x1;
         const float al0 = exp2f_approx(m0 - b0), al1 = exp2f_approx(m1 - b1);
         m0 = x0;
         m1 = x1;
-        l0 *= al0;
-        l1 *= al1;
-        const float z0 = 15.f - b0, z1 = 15.f - b1;                   // probabilities times 2^15
-        const float vinv = vref > 0.f ? 1.f / vref : 0.f;
+        // ---- probabilities (times 2^15) and their sum ----
+        const float z0 = 15.f - b0, z1 = 15.f - b1;
+        uint64_t sum = pk2(0.f, 0.f), sum2 = pk2(0.f, 0.f);          // R = 16: row a and row b apart; R = 8: (a, b)
         uint32_t pf[TS][4];
 #pragma unroll
         for (int i = 0; i < TS; ++i) {
-          const float f = vrel[i] * vinv;
 #pragma unroll
-          for (int t = 0; t < 2; ++t) {
-            const float* sj = s[2 * i + t];
-            const float p0 = exp2f_approx(sj[0] + z0), p1 = exp2f_approx(sj[1] + z0);
-            const float p2 = exp2f_approx(sj[2] + z1), p3 = exp2f_approx(sj[3] + z1);
-            l0 += p0 + p1;
-            l1 += p2 + p3;
-            pf[i][2 * t] = pack_f16(p0 * f, p1 * f);
-            pf[i][2 * t + 1] = pack_f16(p2 * f, p3 * f);
+          for (int t = 0; t < PS; ++t) {
+            const float* sj = s[PS * i + t];
+            const uint64_t fa = R == 16 ? pk2s(f0[i]) : pk2(f0[i], f1[i]), za = R == 16 ? pk2s(z0) : pk2(z0, z1);
+            const uint64_t fb = R == 16 ? pk2s(f1[i]) : fa, zb = R == 16 ? pk2s(z1) : za;
+            float p0, p1, p2, p3;
+            pk2_split(pk2_fma(pk2(sj[0], sj[1]), fa, za), p0, p1);
+            pk2_split(pk2_fma(pk2(sj[2], sj[3]), fb, zb), p2, p3);
+            p0 = exp2f_approx(p0);
+            p1 = exp2f_approx(p1);
+            p2 = exp2f_approx(p2);
+            p3 = exp2f_approx(p3);
+            sum = pk2_add(sum, pk2(p0, p1));
+            sum2 = pk2_add(sum2, pk2(p2, p3));
+            if (boxes > 1) {
+              p0 *= rel[i];
+              p1 *= rel[i];
+              p2 *= rel[i];
+              p3 *= rel[i];
+            }
+            pf[i][2 * t] = pack_f16(p0, p1);
+            pf[i][2 * t + 1] = pack_f16(p2, p3);
+          }
+          if constexpr (R == 8) {
+            pf[i][0] = transpose8(pf[i][0]);
+            pf[i][1] = transpose8(pf[i][1]);
           }
         }
-        // values: what lies behind the keys may be anything, NaN too
-        uint32_t vw[TS][4][D / 32];
-#pragma unroll
-        for (int i = 0; i < TS; ++i)
-#pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            const uint32_t a = vt + v_off[r & 1] + (16 * i + 8 * (r >> 1)) * D;
-            if constexpr (D == 128) {
-              const uint4 t = lds128(a);
-              vw[i][r][0] = t.x; vw[i][r][1] = t.y; vw[i][r][2] = t.z; vw[i][r][3] = t.w;
-            } else if constexpr (D == 64) {
-              const uint2 t = lds64(a);
-              vw[i][r][0] = t.x; vw[i][r][1] = t.y;
-            } else {
-              vw[i][r][0] = lds32(a);
-            }
-          }
+        float t0, t1, t2, t3;
+        pk2_split(sum, t0, t1);
+        pk2_split(sum2, t2, t3);
+        l0 = l0 * al0 + (R == 16 ? t0 + t1 : t0 + t2);
+        l1 = l1 * al1 + (R == 16 ? t2 + t3 : t1 + t3);
+        // ---- values: what lies behind the keys may be anything, NaN too ----
+        if constexpr (R == 16) load_values();
         if (hole || end < TK) {
 #pragma unroll
           for (int i = 0; i < TS; ++i)
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-              const bool gone = 16 * i + 2 * qd + (r & 1) + 8 * (r >> 1) >= end ||
-                                s_blk[warp][st][(i * 16) >> box_log] < 0;
+              const int at = 16 * i + 2 * qd + (r & 1) + 8 * (r >> 1);
+              const bool drop = at >= end || (my_gone >> (at >> box_log) & 1);
 #pragma unroll
-              for (int w = 0; w < D / 32; ++w) vw[i][r][w] = gone ? 0u : vw[i][r][w];
+              for (int w = 0; w < D / 32; ++w) vw[i][r][w] = drop ? 0u : vw[i][r][w];
             }
         }
+        const uint64_t alx = R == 16 ? pk2s(al0) : pk2(al0, al1), aly = R == 16 ? pk2s(al1) : alx, vr = pk2s(vref);
 #pragma unroll
         for (int w = 0; w < D / 32; ++w) {
-          float acc[4][4];
+          constexpr int F = R / 4;                                    // output fragments of four of the lane's dims
+          float acc[F][4];
 #pragma unroll
-          for (int e = 0; e < 4; ++e) acc[e][0] = acc[e][1] = acc[e][2] = acc[e][3] = 0.f;
+          for (int e = 0; e < F; ++e) acc[e][0] = acc[e][1] = acc[e][2] = acc[e][3] = 0.f;
 #pragma unroll
           for (int i = 0; i < TS; ++i) {
             // pairs of keys for four dims: bytes of two rows side by side
@@ -586,109 +683,126 @@ paged_attn_kernel(const AttnArgs A, const __grid_constant__ CUtensorMap tm_k, co
             cvt4(__byte_perm(vw[i][0][w], vw[i][1][w], 0x7362), b0[2], b0[3]);
             cvt4(__byte_perm(vw[i][2][w], vw[i][3][w], 0x5140), b1[0], b1[1]);
             cvt4(__byte_perm(vw[i][2][w], vw[i][3][w], 0x7362), b1[2], b1[3]);
+            if constexpr (R == 16) {
 #pragma unroll
-            for (int e = 0; e < 4; ++e) mma_f16(acc[e], pf[i], b0[e], b1[e]);
+              for (int e = 0; e < 4; ++e) mma_f16(acc[e % F], pf[i], b0[e], b1[e]);
+            } else {
+#pragma unroll
+              for (int e = 0; e < 2; ++e) {
+                const uint32_t a[4] = {b0[2 * e], b0[2 * e + 1], b1[2 * e], b1[2 * e + 1]};
+                mma_f16(acc[e], a, pf[i][0], pf[i][1]);
+              }
+            }
           }
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            float* ou = o[4 * w + e];
-            ou[0] = fmaf(acc[e][0], vref, ou[0] * al0);
-            ou[1] = fmaf(acc[e][1], vref, ou[1] * al0);
-            ou[2] = fmaf(acc[e][2], vref, ou[2] * al1);
-            ou[3] = fmaf(acc[e][3], vref, ou[3] * al1);
+          for (int e = 0; e < F; ++e) {
+            float* ou = o[F * w + e];
+            pk2_split(pk2_fma(pk2(acc[e][0], acc[e][1]), vr, pk2_mul(pk2(ou[0], ou[1]), alx)), ou[0], ou[1]);
+            pk2_split(pk2_fma(pk2(acc[e][2], acc[e][3]), vr, pk2_mul(pk2(ou[2], ou[3]), aly)), ou[2], ou[3]);
           }
         }
       }
       __syncwarp();                         // the slot has been read
-      ++taken;
-      const int was = c.unit;
-      const int64_t left = c.left;
+#pragma unroll
+      for (int i = 0; i + 1 < ST; ++i) scl[i] = scl[i + 1], gone[i] = gone[i + 1];
+      if (++st == ST) {
+        st = 0;
+        phase ^= 1;
+      }
+      const int was = c.unit, left = c.left;
       c.next(A, SUP);
       ends = was == S.units(SUP) - 1;
       if (left == 1) break;
     } while (!ends);
 
-    // ---- the block's warps become one ----
-    l0 += __shfl_xor_sync(0xffffffffu, l0, 1);
-    l1 += __shfl_xor_sync(0xffffffffu, l1, 1);
-    l0 += __shfl_xor_sync(0xffffffffu, l0, 2);
-    l1 += __shfl_xor_sync(0xffffffffu, l1, 2);
-    const bool alone = S.len <= TK;         // one tile of keys: warp 0 has it all
-    if (!alone) {
+    // ---- the segment's warps become one ----
 #pragma unroll
-      for (int n = kWarps / 2; n > 0; n /= 2) {             // warps n .. 2 n - 1 go to warps 0 .. n - 1
-        __syncthreads();
-        if (warp >= n && warp < 2 * n) {
+    for (int t = R == 16 ? 1 : 4; t < (R == 16 ? 4 : 32); t *= 2) {
+      l0 += __shfl_xor_sync(0xffffffffu, l0, t);
+      l1 += __shfl_xor_sync(0xffffffffu, l1, t);
+    }
+    const bool writes_ml = R == 16 ? qd == 0 : g == 0;      // one lane for each pair of rows
+    if constexpr (W > 1) {
+      if (S.len > TK) {                     // else warp 0 has it all
 #pragma unroll
-          for (int u = 0; u < NO; ++u)
+        for (int n = W / 2; n > 0; n /= 2) {                // warps n .. 2 n - 1 go to warps 0 .. n - 1
+          __syncthreads();
+          if (warp >= n && warp < 2 * n) {
 #pragma unroll
-            for (int e = 0; e < 4; ++e) s_merge[warp - n][(u * 4 + e) * 32 + lane] = o[u][e];
-          if (qd == 0) {
-            s_ml[warp - n][g][0] = m0;
-            s_ml[warp - n][g][1] = l0;
-            s_ml[warp - n][g + 8][0] = m1;
-            s_ml[warp - n][g + 8][1] = l1;
+            for (int u = 0; u < NO; ++u)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) s_merge[warp - n][(u * 4 + e) * 32 + lane] = o[u][e];
+            if (writes_ml) {
+              s_ml[warp - n][row_a][0] = m0;
+              s_ml[warp - n][row_a][1] = l0;
+              s_ml[warp - n][row_b][0] = m1;
+              s_ml[warp - n][row_b][1] = l1;
+            }
           }
-        }
-        __syncthreads();
-        if (warp < n) {
-          const float n0 = s_ml[warp][g][0], n1 = s_ml[warp][g + 8][0];
-          const float x0 = fmaxf(m0, n0), x1 = fmaxf(m1, n1);
-          const float c0 = x0 == -INFINITY ? 0.f : x0, c1 = x1 == -INFINITY ? 0.f : x1;
-          const float a0 = exp2f_approx(m0 - c0), a1 = exp2f_approx(m1 - c1);
-          const float d0 = exp2f_approx(n0 - c0), d1 = exp2f_approx(n1 - c1);
-          l0 = l0 * a0 + s_ml[warp][g][1] * d0;
-          l1 = l1 * a1 + s_ml[warp][g + 8][1] * d1;
-          m0 = x0;
-          m1 = x1;
+          __syncthreads();
+          if (warp < n) {
+            const float n0 = s_ml[warp][row_a][0], n1 = s_ml[warp][row_b][0];
+            const float x0 = fmaxf(m0, n0), x1 = fmaxf(m1, n1);
+            const float c0 = x0 == -INFINITY ? 0.f : x0, c1 = x1 == -INFINITY ? 0.f : x1;
+            const float a0 = exp2f_approx(m0 - c0), a1 = exp2f_approx(m1 - c1);
+            const float d0 = exp2f_approx(n0 - c0), d1 = exp2f_approx(n1 - c1);
+            l0 = l0 * a0 + s_ml[warp][row_a][1] * d0;
+            l1 = l1 * a1 + s_ml[warp][row_b][1] * d1;
+            m0 = x0;
+            m1 = x1;
 #pragma unroll
-          for (int u = 0; u < NO; ++u) {
-            const float* src = &s_merge[warp][u * 128 + lane];
-            o[u][0] = o[u][0] * a0 + src[0] * d0;
-            o[u][1] = o[u][1] * a0 + src[32] * d0;
-            o[u][2] = o[u][2] * a1 + src[64] * d1;
-            o[u][3] = o[u][3] * a1 + src[96] * d1;
+            for (int u = 0; u < NO; ++u)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                const bool second = R == 16 ? e >> 1 : e & 1;
+                o[u][e] = o[u][e] * (second ? a1 : a0) + s_merge[warp][(u * 4 + e) * 32 + lane] * (second ? d1 : d0);
+              }
           }
         }
       }
     }
-    if (warp == 0) {
+    if (part == 0) {
       if (begins && ends) {
-        // sum of 0: no keys. A NaN stays one
+        // a sum of 0: no keys. A NaN stays one
         const float i0 = l0 == 0.f ? 0.f : 1.f / l0, i1 = l1 == 0.f ? 0.f : 1.f / l1;
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-          const int r = r0 + 8 * i;
+          const int r = r0 + (i ? row_b : row_a);
           if (r >= rows) continue;
           const int qi = r / A.G;
           const int64_t at = int64_t(S.tok0 + qi) * A.Hq + seg_h * A.G + (r - qi * A.G);
-          uint16_t* dst = static_cast<uint16_t*>(A.o) + at * D + qd * (D / 4);
           const float inv = i ? i1 : i0;
+          if constexpr (R == 16) {
+            uint16_t* dst = static_cast<uint16_t*>(A.o) + at * D + qd * (D / 4);
 #pragma unroll
-          for (int t = 0; t < 2; ++t) {
-            float f[NO];
+            for (int t = 0; t < 2; ++t)
 #pragma unroll
-            for (int u = 0; u < NO; ++u) f[u] = o[u][2 * i + t] * inv;
+              for (int u = 0; u < NO; u += 4)
+                *reinterpret_cast<uint2*>(dst + t * NO + u) =
+                    make_uint2(pack_16(o[u][2 * i + t] * inv, o[u + 1][2 * i + t] * inv, A.bf16),
+                               pack_16(o[u + 2][2 * i + t] * inv, o[u + 3][2 * i + t] * inv, A.bf16));
+          } else {
+            uint16_t* dst = static_cast<uint16_t*>(A.o) + at * D + g * (D / 8);
 #pragma unroll
-            for (int u = 0; u < NO; u += 4)
-              *reinterpret_cast<uint2*>(dst + t * NO + u) =
-                  make_uint2(pack_16(f[u], f[u + 1], A.bf16), pack_16(f[u + 2], f[u + 3], A.bf16));
+            for (int u = 0; u < NO; ++u)
+              *reinterpret_cast<uint32_t*>(dst + 2 * u) = pack_16(o[u][i] * inv, o[u][i + 2] * inv, A.bf16);
           }
           const float l = i ? l1 : l0, m = i ? m1 : m0;
-          if (A.lse && qd == 0)
-            A.lse[at] = l == 0.f ? -INFINITY : (m - 15.f + log2f(l)) * 0.6931471805599453f;
+          if (A.lse && writes_ml) A.lse[at] = l == 0.f ? -INFINITY : (m - 15.f + log2f(l)) * 0.6931471805599453f;
         }
       } else {
         const int slot = blockIdx.x * 2 + (first ? 0 : 1);
-        float* dst = A.part_o + int64_t(slot) * kRows * D;
+        float* dst = A.part_o + int64_t(slot) * R * D;
 #pragma unroll
         for (int u = 0; u < NO; ++u)
 #pragma unroll
           for (int e = 0; e < 4; ++e) dst[(u * 4 + e) * 32 + lane] = o[u][e];
-        if (qd == 0) {
-          float* ml = A.part_ml + int64_t(slot) * kRows * 2;
-          ml[g * 2] = m0; ml[g * 2 + 1] = l0;
-          ml[(g + 8) * 2] = m1; ml[(g + 8) * 2 + 1] = l1;
+        if (writes_ml) {
+          float* ml = A.part_ml + int64_t(slot) * R * 2;
+          ml[row_a * 2] = m0;
+          ml[row_a * 2 + 1] = l0;
+          ml[row_b * 2] = m1;
+          ml[row_b * 2 + 1] = l1;
         }
         if (lane == 0) {
           int* hd = A.part_head + slot * 4;
@@ -705,11 +819,11 @@ paged_attn_kernel(const AttnArgs A, const __grid_constant__ CUtensorMap tm_k, co
 
 // Pieces of the segments that blocks share: one block for each piece that
 // begins a segment adds up those that follow in the next blocks, in order.
-template <int D>
+template <int D, int R>
 __global__ void __launch_bounds__(256) paged_attn_join_kernel(const AttnArgs A, int blocks) {
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  constexpr int PER = kRows * D / 256;
-  __shared__ float s_m[kRows], s_l[kRows], s_f[kRows];
+  constexpr int PER = (R * D + 255) / 256;
+  __shared__ float s_m[R], s_l[R], s_f[R];
   // a block's last piece is the only one that can begin a segment without ending it
   int slot = -1;
   for (int i = 0; i < 2; ++i) {
@@ -722,13 +836,13 @@ __global__ void __launch_bounds__(256) paged_attn_join_kernel(const AttnArgs A, 
   do { ++last; } while (last < blocks && !(A.part_head[last * 8 + 3] & 2));
   last = min(last, blocks - 1);
   const int tid = threadIdx.x;
-  if (tid < kRows) {
-    float m = A.part_ml[(int64_t(slot) * kRows + tid) * 2];
-    for (int k = blockIdx.x + 1; k <= last; ++k) m = fmaxf(m, A.part_ml[(int64_t(k) * 2 * kRows + tid) * 2]);
+  if (tid < R) {
+    float m = A.part_ml[(int64_t(slot) * R + tid) * 2];
+    for (int k = blockIdx.x + 1; k <= last; ++k) m = fmaxf(m, A.part_ml[(int64_t(k) * 2 * R + tid) * 2]);
     const float base = m == -INFINITY ? 0.f : m;
     float l = 0.f;
     for (int k = blockIdx.x; k <= last; ++k) {
-      const float* ml = A.part_ml + (int64_t(k == int(blockIdx.x) ? slot : 2 * k) * kRows + tid) * 2;
+      const float* ml = A.part_ml + (int64_t(k == int(blockIdx.x) ? slot : 2 * k) * R + tid) * 2;
       l += ml[1] * exp2f_approx(ml[0] - base);
     }
     s_m[tid] = m;
@@ -738,37 +852,36 @@ __global__ void __launch_bounds__(256) paged_attn_join_kernel(const AttnArgs A, 
   __syncthreads();
   // element x of a piece: fragment (u, e) of lane x % 32, as the first kernel's registers lie
   float sum[PER];
-  int row[PER];
+  int row[PER], dim[PER];
 #pragma unroll
   for (int i = 0; i < PER; ++i) {
-    const int x = i * 256 + tid, ln = x & 31, e = (x >> 5) & 3;
-    row[i] = (ln >> 2) + 8 * (e >> 1);
+    const int x = i * 256 + tid, ln = x & 31, e = (x >> 5) & 3, u = x >> 7;
+    row[i] = R == 16 ? (ln >> 2) + 8 * (e >> 1) : 2 * (ln & 3) + (e & 1);
+    dim[i] = R == 16 ? (2 * (ln & 3) + (e & 1)) * (D / 8) + u : (ln >> 2) * (D / 8) + 2 * u + (e >> 1);
     sum[i] = 0.f;
   }
   for (int k = blockIdx.x; k <= last; ++k) {
     const int64_t sl = k == int(blockIdx.x) ? slot : 2 * k;
-    const float* src = A.part_o + sl * kRows * D;
+    const float* src = A.part_o + sl * R * D;
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
       const float m = s_m[row[i]], base = m == -INFINITY ? 0.f : m;
-      sum[i] += src[i * 256 + tid] * exp2f_approx(A.part_ml[(sl * kRows + row[i]) * 2] - base);
+      sum[i] += src[i * 256 + tid] * exp2f_approx(A.part_ml[(sl * R + row[i]) * 2] - base);
     }
   }
-  Seq S;
+  Seq<R> S;
   S.load(A, b);
   const int rows = S.n * A.G;
 #pragma unroll
   for (int i = 0; i < PER; ++i) {
-    const int x = i * 256 + tid, ln = x & 31, e = (x >> 5) & 3, u = x >> 7;
-    const int r = mt * kRows + row[i];
+    const int r = mt * R + row[i];
     if (r >= rows) continue;
     const int qi = r / A.G;
     const int64_t at = int64_t(S.tok0 + qi) * A.Hq + h * A.G + (r - qi * A.G);
-    static_cast<uint16_t*>(A.o)[at * D + (2 * (ln & 3) + (e & 1)) * (D / 8) + u] =
-        uint16_t(pack_16(sum[i] * s_f[row[i]], 0.f, A.bf16));
+    static_cast<uint16_t*>(A.o)[at * D + dim[i]] = uint16_t(pack_16(sum[i] * s_f[row[i]], 0.f, A.bf16));
   }
-  if (A.lse && tid < kRows && mt * kRows + tid < rows) {
-    const int r = mt * kRows + tid, qi = r / A.G;
+  if (A.lse && tid < R && mt * R + tid < rows) {
+    const int r = mt * R + tid, qi = r / A.G;
     const int64_t at = int64_t(S.tok0 + qi) * A.Hq + h * A.G + (r - qi * A.G);
     A.lse[at] = s_l[tid] == 0.f ? -INFINITY : (s_m[tid] - 15.f + log2f(s_l[tid])) * 0.6931471805599453f;
   }
@@ -807,34 +920,44 @@ static CUtensorMap code_map(const at::Tensor& x, int box_rows) {
   return m;
 }
 
-template <int D>
-static void attn_launch(AttnArgs& A, const at::Tensor& ck, const at::Tensor& cv, int64_t segments, int64_t max_len) {
-  constexpr int TK = Cfg<D>::TK, ST = Cfg<D>::ST, SUP = TK * kWarps;
-  constexpr int kSmem = 1024 + kWarps * ST * 2 * TK * D;     // the ring, on a 1024-byte boundary
-  auto kern = paged_attn_kernel<D>;
-  static int per_sm[64] = {};                // by device
+// Blocks of a kernel that an SM of this device holds.
+template <typename K>
+static int blocks_per_sm(K kern, int threads, int smem, int (&known)[64]) {
   int dev = 0;
   PD_CHECK_CUDA(cudaGetDevice(&dev));
-  if (dev >= 64 || per_sm[dev] == 0) {
-    PD_CHECK_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem));
-    int n = 0;
-    PD_CHECK_CUDA(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kern, kWarps * 32, kSmem));
-    PD_CHECK(n > 0, "the attention kernel does not fit an SM");
-    if (dev < 64) per_sm[dev] = n;
-  }
-  const int slots = num_sms() * (dev < 64 ? per_sm[dev] : 1);
-  const int64_t units = std::max<int64_t>(1, (max_len + SUP - 1) / SUP);      // of the longest segment
+  if (dev < 64 && known[dev] > 0) return known[dev];
+  PD_CHECK_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+  int n = 0;
+  PD_CHECK_CUDA(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kern, threads, smem));
+  PD_CHECK(n > 0, "an attention kernel does not fit an SM");
+  if (dev < 64) known[dev] = n;
+  return n;
+}
+
+struct Bounds {                 // of what the lengths on the device can ask for; they only decide how the work is split
+  int64_t B, rows, len;         // rows: most (query, head of the group) of a sequence and key head
+};
+
+template <int D, int R, int W>
+static void few_launch(AttnArgs& A, const at::Tensor& ck, const at::Tensor& cv, const Bounds& U) {
+  constexpr int TK = Cfg<D>::TK, ST = Cfg<D>::ST, SUP = TK * W;
+  constexpr int kSmem = kWarps * ST * 2 * TK * D;
+  static int known[64] = {};
+  auto kern = paged_attn_kernel<D, R, W>;
+  const int64_t slots = int64_t(num_sms()) * blocks_per_sm(kern, kWarps * 32, kSmem, known);
+  const int64_t segments = U.B * A.H * ((U.rows + R - 1) / R);
+  const int64_t units = std::max<int64_t>(1, (U.len + SUP - 1) / SUP);        // of the longest segment
   A.min_units = 2;
-  A.split = segments < int64_t(slots) * 8 && units > A.min_units;
-  const int64_t most = A.split ? (segments * units + A.min_units - 1) / A.min_units : segments;
+  A.split = W > 1 && segments < slots * 8 && units > A.min_units;
+  const int64_t most = A.split ? (segments * units + A.min_units - 1) / A.min_units : (segments * W + kWarps - 1) / kWarps;
   const int grid = int(std::min<int64_t>(slots, most));
   at::Tensor part;
   if (A.split) {
     const int64_t n = 2 * int64_t(grid);
-    part = at::empty({n * (kRows * D + kRows * 2 + 4)}, ck.options().dtype(at::kFloat));
+    part = at::empty({n * (R * D + R * 2 + 4)}, ck.options().dtype(at::kFloat));
     A.part_o = part.data_ptr<float>();
-    A.part_ml = A.part_o + n * kRows * D;
-    A.part_head = reinterpret_cast<int*>(A.part_ml + n * kRows * 2);
+    A.part_ml = A.part_o + n * R * D;
+    A.part_head = reinterpret_cast<int*>(A.part_ml + n * R * 2);
   }
   const int box = std::min(A.P, TK);
   kern<<<grid, kWarps * 32, kSmem, stream()>>>(A, code_map(ck, box), code_map(cv, box));
@@ -849,16 +972,17 @@ static void attn_launch(AttnArgs& A, const at::Tensor& ck, const at::Tensor& cv,
     at[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = at;
     cfg.numAttrs = 1;
-    PD_CHECK_CUDA(cudaLaunchKernelEx(&cfg, paged_attn_join_kernel<D>, (const AttnArgs)A, grid));
+    PD_CHECK_CUDA(cudaLaunchKernelEx(&cfg, paged_attn_join_kernel<D, R>, (const AttnArgs)A, grid));
     PD_CHECK_LAUNCH();
   }
 }
 
-static void attn_dispatch(AttnArgs& A, const at::Tensor& ck, const at::Tensor& cv, int d, int64_t segments,
-                          int64_t max_len) {
-  if (d == 32) attn_launch<32>(A, ck, cv, segments, max_len);
-  else if (d == 64) attn_launch<64>(A, ck, cv, segments, max_len);
-  else attn_launch<128>(A, ck, cv, segments, max_len);
+template <int D>
+static void attn_dispatch(AttnArgs& A, const at::Tensor& ck, const at::Tensor& cv, const Bounds& U) {
+  // a warp a segment where there are eight segments and more for every warp of the device (12 warps an SM)
+  const bool many = U.B * A.H * ((U.rows + 15) / 16) >= int64_t(num_sms()) * 12 * 4;
+  if (U.rows <= 8) return many ? few_launch<D, 8, 1>(A, ck, cv, U) : few_launch<D, 8, 4>(A, ck, cv, U);
+  return many ? few_launch<D, 16, 1>(A, ck, cv, U) : few_launch<D, 16, 4>(A, ck, cv, U);
 }
 
 // (o, lse): lse is an undefined tensor unless asked for.
@@ -909,14 +1033,13 @@ std::vector<at::Tensor> paged_attention(at::Tensor q, at::Tensor ck, at::Tensor 
     A.lse = lse.data_ptr<float>();
   }
   const int64_t most = qd == 4 ? q.size(1) : std::min<int64_t>(std::max<int64_t>(max_q, 0), q.size(0));
-  PD_CHECK((qd == 3 ? q.size(0) : B * q.size(1)) * A.G < (int64_t(1) << 31) - kRows && B < (int64_t(1) << 31),
+  PD_CHECK((qd == 3 ? q.size(0) : B * q.size(1)) * A.G < (int64_t(1) << 31) - 128 && B < (int64_t(1) << 31),
            "too many queries");
   if (B > 0 && most > 0 && q.numel() > 0) {
-    // upper bounds of what the lengths on the device can ask for; they only decide how the work is split
-    const int64_t segments = B * C.H * ((most * A.G + kRows - 1) / kRows);
-    const int64_t room = table.size(1) * C.P;
-    const int64_t longest = std::min<int64_t>(room, std::max<int64_t>(max_len, 0));
-    attn_dispatch(A, ck, cv, C.d, segments, longest);
+    const Bounds U{B, most * A.G, std::min<int64_t>(table.size(1) * C.P, std::max<int64_t>(max_len, 0))};
+    if (C.d == 32) attn_dispatch<32>(A, ck, cv, U);
+    else if (C.d == 64) attn_dispatch<64>(A, ck, cv, U);
+    else attn_dispatch<128>(A, ck, cv, U);
   }
   return want_lse ? std::vector<at::Tensor>{o, lse} : std::vector<at::Tensor>{o};
 }

@@ -122,6 +122,12 @@ __device__ __forceinline__ void turn(float* a, float* b, const float* c, const f
   }
 }
 
+__device__ __forceinline__ uint64_t pk2_add(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+
 template <int L>
 __device__ __forceinline__ float group_sum(float v) {
 #pragma unroll
