@@ -52,7 +52,7 @@ struct AttnArgs {
 template <int D> struct Cfg;
 // TK keys a tile and warp (8 KB of keys and values), ST tiles in flight: three
 // blocks of four warps an SM
-template <> struct Cfg<32> { static constexpr int TK = 128, ST = 2; };
+template <> struct Cfg<32> { static constexpr int TK = 64, ST = 3; };
 template <> struct Cfg<64> { static constexpr int TK = 64, ST = 2; };
 template <> struct Cfg<128> { static constexpr int TK = 32, ST = 2; };
 
@@ -228,7 +228,7 @@ struct Cursor {
 // neighbours: lane % 4 owns a quarter of a key's dims, lane / 4 an eighth of a
 // value's, and keys go to registers in the order of memory.
 template <int D, int R, int W>
-__global__ void __launch_bounds__(kWarps * 32, D == 128 && R == 16 ? 2 : 3)
+__global__ void __launch_bounds__(kWarps * 32, D == 128 && R == 16 ? 2 : D == 32 ? 4 : 3)
 paged_attn_kernel(const AttnArgs A, const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v) {
   constexpr int TK = Cfg<D>::TK, ST = Cfg<D>::ST;
   constexpr int SUP = TK * W;           // keys of a unit
@@ -263,6 +263,7 @@ paged_attn_kernel(const AttnArgs A, const __grid_constant__ CUtensorMap tm_k, co
   // ---- this worker's range of units: each thread counts a run of sequences ----
   Cursor<R> c;
   c.left = 0;
+  int64_t share;
   {
     constexpr int kWorkers = kWarps / W;                    // of a block
     const int per = (A.B + kWarps * 32 - 1) / (kWarps * 32);
@@ -289,7 +290,7 @@ paged_attn_kernel(const AttnArgs A, const __grid_constant__ CUtensorMap tm_k, co
     }
     // split: equal shares of the units; else equal shares of the segments
     const int64_t workers = int64_t(gridDim.x) * kWorkers;
-    const int64_t share = max(int64_t(A.split ? A.min_units : 1), (total + workers - 1) / workers);
+    share = max(int64_t(A.split ? A.min_units : 1), (total + workers - 1) / workers);
 #pragma unroll 1
     for (int w = 0; w < kWorkers; ++w) {
       const int64_t u0 = share * (int64_t(blockIdx.x) * kWorkers + w);
@@ -483,6 +484,7 @@ paged_attn_kernel(const AttnArgs A, const __grid_constant__ CUtensorMap tm_k, co
     float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f;
 
     bool ends = false;
+    int used = 0;                           // units of the segment so far, for a segment that begins here
     do {
       const int k0 = c.unit * SUP + part * TK;
       issue(st == 0 ? ST - 1 : st - 1, scl[ST - 1], gone[ST - 1]);    // refills the slot of the tile before
@@ -568,6 +570,7 @@ paged_attn_kernel(const AttnArgs A, const __grid_constant__ CUtensorMap tm_k, co
         }
         // ---- running maximum ----
         float vref, f0[TS], f1[TS], rel[TS];                          // by step of 16 keys
+        bool flat = true;                                             // one value scale for the whole tile
         float x0 = -INFINITY, x1 = -INFINITY;
         if (boxes == 1) {
           const float ks = __shfl_sync(0xffffffffu, my_scl, 0);
@@ -589,6 +592,9 @@ paged_attn_kernel(const AttnArgs A, const __grid_constant__ CUtensorMap tm_k, co
             rel[i] = __shfl_sync(0xffffffffu, my_scl, pg + NP);
             vref = fmaxf(vref, rel[i]);
           }
+          // (a page that was not loaded has scale 0, and its probabilities are 0)
+#pragma unroll
+          for (int i = 0; i < TS; ++i) flat = flat && (rel[i] == vref || rel[i] == 0.f);
           const float vinv = vref > 0.f ? 1.f / vref : 0.f;
 #pragma unroll
           for (int i = 0; i < TS; ++i) rel[i] *= vinv;
@@ -636,7 +642,7 @@ paged_attn_kernel(const AttnArgs A, const __grid_constant__ CUtensorMap tm_k, co
             p3 = exp2f_approx(p3);
             sum = pk2_add(sum, pk2(p0, p1));
             sum2 = pk2_add(sum2, pk2(p2, p3));
-            if (boxes > 1) {
+            if (!flat) {
               p0 *= rel[i];
               p1 *= rel[i];
               p2 *= rel[i];
@@ -710,6 +716,7 @@ paged_attn_kernel(const AttnArgs A, const __grid_constant__ CUtensorMap tm_k, co
         phase ^= 1;
       }
       const int was = c.unit, left = c.left;
+      used = was + 1;
       c.next(A, SUP);
       ends = was == S.units(SUP) - 1;
       if (left == 1) break;
@@ -796,7 +803,9 @@ paged_attn_kernel(const AttnArgs A, const __grid_constant__ CUtensorMap tm_k, co
 #pragma unroll
         for (int u = 0; u < NO; ++u)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) dst[(u * 4 + e) * 32 + lane] = o[u][e];
+          for (int e = 0; e < 4; ++e)
+            if constexpr (R == 16) dst[(e >> 1 ? row_b : row_a) * D + (2 * qd + (e & 1)) * (D / 8) + u] = o[u][e];
+            else dst[(e & 1 ? row_b : row_a) * D + g * (D / 8) + 2 * u + (e >> 1)] = o[u][e];
         if (writes_ml) {
           float* ml = A.part_ml + int64_t(slot) * R * 2;
           ml[row_a * 2] = m0;
@@ -809,7 +818,8 @@ paged_attn_kernel(const AttnArgs A, const __grid_constant__ CUtensorMap tm_k, co
           hd[0] = seg_b;
           hd[1] = seg_h;
           hd[2] = seg_mt;
-          hd[3] = (begins ? 1 : 0) | (ends ? 2 : 0);
+          // a piece that begins a segment: how many blocks hold the rest of it
+          hd[3] = begins ? int((S.units(SUP) - used + share - 1) / share) : 0;
         }
       }
     }
@@ -817,74 +827,58 @@ paged_attn_kernel(const AttnArgs A, const __grid_constant__ CUtensorMap tm_k, co
   }
 }
 
-// Pieces of the segments that blocks share: one block for each piece that
-// begins a segment adds up those that follow in the next blocks, in order.
+// Pieces of the segments that blocks share: one block for each row of each
+// piece that begins a segment takes those that follow in the next blocks, a
+// group of D / 4 threads a piece at a time, and adds the groups in order.
 template <int D, int R>
-__global__ void __launch_bounds__(256) paged_attn_join_kernel(const AttnArgs A, int blocks) {
+__global__ void __launch_bounds__(256) paged_attn_join_kernel(const AttnArgs A) {
+  constexpr int L = D / 4, GR = 256 / L;
+  __shared__ float4 s_o[GR][L];
+  __shared__ float s_m[GR], s_l[GR];
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  constexpr int PER = (R * D + 255) / 256;
-  __shared__ float s_m[R], s_l[R], s_f[R];
+  const int here = blockIdx.x, row = blockIdx.y, tid = threadIdx.x, gr = tid / L, ln = tid % L;
   // a block's last piece is the only one that can begin a segment without ending it
-  int slot = -1;
-  for (int i = 0; i < 2; ++i) {
-    const int* hd = A.part_head + (blockIdx.x * 2 + i) * 4;
-    if (hd[0] >= 0 && hd[3] == 1) slot = blockIdx.x * 2 + i;
+  const int4 h0 = reinterpret_cast<const int4*>(A.part_head)[here * 2];
+  const int4 h1 = reinterpret_cast<const int4*>(A.part_head)[here * 2 + 1];
+  const bool second = h1.x >= 0 && h1.w > 0;
+  const int4 hd = second ? h1 : h0;
+  if (hd.x < 0 || hd.w <= 0) return;
+  Seq<R> S;
+  S.load(A, hd.x);
+  const int r = hd.z * R + row;
+  if (r >= S.n * A.G) return;
+  float m = -INFINITY, l = 0.f;
+  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+  auto take = [&](float n, float k, float4 x) {
+    const float top = fmaxf(m, n), base = top == -INFINITY ? 0.f : top;
+    const float a = exp2f_approx(m - base), c = exp2f_approx(n - base);
+    m = top;
+    l = l * a + k * c;
+    o.x = o.x * a + x.x * c;
+    o.y = o.y * a + x.y * c;
+    o.z = o.z * a + x.z * c;
+    o.w = o.w * a + x.w * c;
+  };
+#pragma unroll 4
+  for (int i = gr; i <= hd.w; i += GR) {
+    const int64_t at = (i == 0 ? here * 2 + int(second) : 2 * (here + i)) * int64_t(R) + row;
+    const float2 ml = *reinterpret_cast<const float2*>(A.part_ml + at * 2);
+    take(ml.x, ml.y, *reinterpret_cast<const float4*>(A.part_o + at * D + ln * 4));
   }
-  if (slot < 0) return;
-  const int b = A.part_head[slot * 4], h = A.part_head[slot * 4 + 1], mt = A.part_head[slot * 4 + 2];
-  int last = blockIdx.x;                     // block of the piece that ends the segment
-  do { ++last; } while (last < blocks && !(A.part_head[last * 8 + 3] & 2));
-  last = min(last, blocks - 1);
-  const int tid = threadIdx.x;
-  if (tid < R) {
-    float m = A.part_ml[(int64_t(slot) * R + tid) * 2];
-    for (int k = blockIdx.x + 1; k <= last; ++k) m = fmaxf(m, A.part_ml[(int64_t(k) * 2 * R + tid) * 2]);
-    const float base = m == -INFINITY ? 0.f : m;
-    float l = 0.f;
-    for (int k = blockIdx.x; k <= last; ++k) {
-      const float* ml = A.part_ml + (int64_t(k == int(blockIdx.x) ? slot : 2 * k) * R + tid) * 2;
-      l += ml[1] * exp2f_approx(ml[0] - base);
-    }
-    s_m[tid] = m;
-    s_l[tid] = l;
-    s_f[tid] = l == 0.f ? 0.f : 1.f / l;
+  s_o[gr][ln] = o;
+  if (ln == 0) {
+    s_m[gr] = m;
+    s_l[gr] = l;
   }
   __syncthreads();
-  // element x of a piece: fragment (u, e) of lane x % 32, as the first kernel's registers lie
-  float sum[PER];
-  int row[PER], dim[PER];
-#pragma unroll
-  for (int i = 0; i < PER; ++i) {
-    const int x = i * 256 + tid, ln = x & 31, e = (x >> 5) & 3, u = x >> 7;
-    row[i] = R == 16 ? (ln >> 2) + 8 * (e >> 1) : 2 * (ln & 3) + (e & 1);
-    dim[i] = R == 16 ? (2 * (ln & 3) + (e & 1)) * (D / 8) + u : (ln >> 2) * (D / 8) + 2 * u + (e >> 1);
-    sum[i] = 0.f;
-  }
-  for (int k = blockIdx.x; k <= last; ++k) {
-    const int64_t sl = k == int(blockIdx.x) ? slot : 2 * k;
-    const float* src = A.part_o + sl * R * D;
-#pragma unroll
-    for (int i = 0; i < PER; ++i) {
-      const float m = s_m[row[i]], base = m == -INFINITY ? 0.f : m;
-      sum[i] += src[i * 256 + tid] * exp2f_approx(A.part_ml[(sl * R + row[i]) * 2] - base);
-    }
-  }
-  Seq<R> S;
-  S.load(A, b);
-  const int rows = S.n * A.G;
-#pragma unroll
-  for (int i = 0; i < PER; ++i) {
-    const int r = mt * R + row[i];
-    if (r >= rows) continue;
-    const int qi = r / A.G;
-    const int64_t at = int64_t(S.tok0 + qi) * A.Hq + h * A.G + (r - qi * A.G);
-    static_cast<uint16_t*>(A.o)[at * D + dim[i]] = uint16_t(pack_16(sum[i] * s_f[row[i]], 0.f, A.bf16));
-  }
-  if (A.lse && tid < R && mt * R + tid < rows) {
-    const int r = mt * R + tid, qi = r / A.G;
-    const int64_t at = int64_t(S.tok0 + qi) * A.Hq + h * A.G + (r - qi * A.G);
-    A.lse[at] = s_l[tid] == 0.f ? -INFINITY : (s_m[tid] - 15.f + log2f(s_l[tid])) * 0.6931471805599453f;
-  }
+  if (gr > 0) return;
+  for (int i = 1; i < min(GR, hd.w + 1); ++i) take(s_m[i], s_l[i], s_o[i][ln]);
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+  const int qi = r / A.G;
+  const int64_t at = int64_t(S.tok0 + qi) * A.Hq + hd.y * A.G + (r - qi * A.G);
+  *reinterpret_cast<uint2*>(static_cast<uint16_t*>(A.o) + at * D + ln * 4) =
+      make_uint2(pack_16(o.x * inv, o.y * inv, A.bf16), pack_16(o.z * inv, o.w * inv, A.bf16));
+  if (A.lse && ln == 0) A.lse[at] = l == 0.f ? -INFINITY : (m - 15.f + log2f(l)) * 0.6931471805599453f;
 }
 
 // cuTensorMapEncodeTiled through the runtime: the extension does not link
@@ -947,8 +941,9 @@ static void few_launch(AttnArgs& A, const at::Tensor& ck, const at::Tensor& cv, 
   const int64_t slots = int64_t(num_sms()) * blocks_per_sm(kern, kWarps * 32, kSmem, known);
   const int64_t segments = U.B * A.H * ((U.rows + R - 1) / R);
   const int64_t units = std::max<int64_t>(1, (U.len + SUP - 1) / SUP);        // of the longest segment
-  A.min_units = 2;
-  A.split = W > 1 && segments < slots * 8 && units > A.min_units;
+  // A unit takes a block about 1 us and the second launch about 4: pieces of 4 units at least, of segments of 9 at least
+  A.min_units = 4;
+  A.split = W > 1 && segments < slots * 8 && units > 2 * A.min_units;
   const int64_t most = A.split ? (segments * units + A.min_units - 1) / A.min_units : (segments * W + kWarps - 1) / kWarps;
   const int grid = int(std::min<int64_t>(slots, most));
   at::Tensor part;
@@ -964,7 +959,7 @@ static void few_launch(AttnArgs& A, const at::Tensor& ck, const at::Tensor& cv, 
   PD_CHECK_LAUNCH();
   if (A.split) {
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = grid;
+    cfg.gridDim = dim3(grid, R);
     cfg.blockDim = 256;
     cfg.stream = stream();
     cudaLaunchAttribute at[1];
@@ -972,7 +967,7 @@ static void few_launch(AttnArgs& A, const at::Tensor& ck, const at::Tensor& cv, 
     at[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = at;
     cfg.numAttrs = 1;
-    PD_CHECK_CUDA(cudaLaunchKernelEx(&cfg, paged_attn_join_kernel<D, R>, (const AttnArgs)A, grid));
+    PD_CHECK_CUDA(cudaLaunchKernelEx(&cfg, paged_attn_join_kernel<D, R>, (const AttnArgs)A));
     PD_CHECK_LAUNCH();
   }
 }
