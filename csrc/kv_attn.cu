@@ -50,11 +50,10 @@ struct AttnArgs {
 };
 
 template <int D> struct Cfg;
-// TK keys a tile and warp (8 KB of keys and values), ST tiles in flight: three
-// blocks of four warps an SM
-template <> struct Cfg<32> { static constexpr int TK = 64, ST = 3; };
-template <> struct Cfg<64> { static constexpr int TK = 64, ST = 2; };
-template <> struct Cfg<128> { static constexpr int TK = 32, ST = 2; };
+// TK keys of products and softmax at a time, SUB such tiles (8 KB of keys and values) to a copy, ST copies in flight
+template <> struct Cfg<32> { static constexpr int TK = 64, SUB = 2, ST = 2; };
+template <> struct Cfg<64> { static constexpr int TK = 64, SUB = 1, ST = 2; };
+template <> struct Cfg<128> { static constexpr int TK = 32, SUB = 1, ST = 2; };
 
 __device__ __forceinline__ uint32_t smem_u32(const void* p) {
   return static_cast<uint32_t>(__cvta_generic_to_shared(p));
@@ -105,6 +104,13 @@ __device__ __forceinline__ void cvt4(uint32_t w, uint32_t& lo, uint32_t& hi) {
       "mov.b32 {l, h}, %2;\n\t"
       "cvt.rn.f16x2.e4m3x2 %0, l;\n\t"
       "cvt.rn.f16x2.e4m3x2 %1, h;\n\t}" : "=r"(lo), "=r"(hi) : "r"(w));
+}
+// D = A * B
+__device__ __forceinline__ void mma_f16_0(float* d, const uint32_t* a, uint32_t b0, uint32_t b1) {
+  asm(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};\n"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
 }
 // queries and outputs are bf16 or fp16 by a flag of the call
 __device__ __forceinline__ float to_f_16(uint16_t v, bool bf16) {
@@ -228,17 +234,18 @@ struct Cursor {
 // neighbours: lane % 4 owns a quarter of a key's dims, lane / 4 an eighth of a
 // value's, and keys go to registers in the order of memory.
 template <int D, int R, int W>
-__global__ void __launch_bounds__(kWarps * 32, D == 128 && R == 16 ? 2 : D == 32 ? 4 : 3)
+__global__ void __launch_bounds__(kWarps * 32, D == 128 && R == 16 ? 2 : 3)
 paged_attn_kernel(const AttnArgs A, const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v) {
-  constexpr int TK = Cfg<D>::TK, ST = Cfg<D>::ST;
-  constexpr int SUP = TK * W;           // keys of a unit
+  constexpr int TK = Cfg<D>::TK, SUB = Cfg<D>::SUB, ST = Cfg<D>::ST;
+  constexpr int WK = TK * SUB;          // keys of a warp's copy
+  constexpr int SUP = WK * W;           // keys of a unit
   constexpr int KS = D / 16;            // steps of 16 dims
   constexpr int TS = TK / 16;           // steps of 16 keys
   constexpr int SF = R == 16 ? 2 * TS : TS;   // score fragments of a tile
   constexpr int NO = R * D / 128;       // output fragments
-  constexpr int NP = TK / 16;           // most pages of a tile
-  constexpr int kHalf = TK * D;         // bytes of a tile's keys
-  extern __shared__ __align__(1024) uint8_t s_ring[];       // [kWarps][ST] tiles: TK rows of keys, TK rows of values
+  constexpr int NP = WK / 16;           // most pages of a copy
+  constexpr int kHalf = WK * D;         // bytes of its keys
+  extern __shared__ __align__(1024) uint8_t s_ring[];       // [kWarps][ST] copies: WK rows of keys, WK rows of values
   __shared__ float s_merge[W > 1 ? 2 : 1][W > 1 ? R * D : 1];
   __shared__ float s_ml[2][R][2];
   __shared__ uint64_t s_bar[kWarps][ST];
@@ -347,21 +354,20 @@ paged_attn_kernel(const AttnArgs A, const __grid_constant__ CUtensorMap tm_k, co
   // flight; `gone` has a bit for each of its pages that is not loaded (behind the keys, or no such page).
   Cursor<R> p = c;
   int page = -1;                            // lane i: id of page i of the tile at p
-  const int box = min(A.P, TK), boxes = TK / box;
-  const int box_log = TK <= 64 ? min(A.logP, TK == 64 ? 6 : 5) : A.logP;
+  const int box = min(A.P, TK), boxes = WK / box, box_log = min(A.logP, TK == 64 ? 6 : 5);
   float scl[ST];
   uint32_t gone[ST];
 #pragma unroll
   for (int i = 0; i < ST; ++i) scl[i] = 0.f, gone[i] = 0;
   auto fetch_page = [&]() {
     page = -1;
-    const int key = p.unit * SUP + part * TK + lane * box;
+    const int key = p.unit * SUP + part * WK + lane * box;
     if (p.left > 0 && lane < boxes && key < p.lim) page = __ldg(A.table + p.b * A.table_stride + (key >> A.logP));
   };
   auto issue = [&](int st, float& sc, uint32_t& gn) {
     if (p.left <= 0) return;
     const uint32_t bar = bars + st * 8, dst = ring + st * 2 * kHalf;
-    const int key = p.unit * SUP + part * TK + lane * box;
+    const int key = p.unit * SUP + part * WK + lane * box;
     const bool want = lane < boxes && key < p.lim;
     const bool have = want && page >= 0 && page < A.n_pages;
     if (want && !have) set_error(A.err, kIdOutOfRange);
@@ -486,14 +492,18 @@ paged_attn_kernel(const AttnArgs A, const __grid_constant__ CUtensorMap tm_k, co
     bool ends = false;
     int used = 0;                           // units of the segment so far, for a segment that begins here
     do {
-      const int k0 = c.unit * SUP + part * TK;
       issue(st == 0 ? ST - 1 : st - 1, scl[ST - 1], gone[ST - 1]);    // refills the slot of the tile before
       const float my_scl = scl[0];
       const uint32_t my_gone = gone[0];
       if (alive) alive = mbar_wait(bars + st * 8, phase, A.err);
       __syncwarp();
-      if (k0 < seg_lim) {
-        const uint32_t kt = ring + st * 2 * kHalf, vt = kt + kHalf;
+#pragma unroll 1
+      for (int sub = 0; sub < SUB; ++sub) {
+        const int k0 = c.unit * SUP + part * WK + sub * TK;
+        if (k0 >= seg_lim) break;
+        const uint32_t kt = ring + st * 2 * kHalf + sub * TK * D, vt = kt + kHalf;
+        const int pg0 = (sub * TK) >> box_log;                        // the tile's first page in the copy
+        const uint32_t missing = my_gone >> pg0;                      // its pages that were not loaded
         // ---- scores: fragment j holds keys 8 j.. (R = 16) or 16 j.. (R = 8) ----
         float s[SF][4];
         auto load_keys = [&](int row, uint32_t* w) {          // words of this lane's dims of key `row` + g
@@ -511,7 +521,6 @@ paged_attn_kernel(const AttnArgs A, const __grid_constant__ CUtensorMap tm_k, co
         };
 #pragma unroll
         for (int j = 0; j < SF; ++j) {
-          s[j][0] = s[j][1] = s[j][2] = s[j][3] = 0.f;
           if constexpr (R == 16) {
             uint32_t w[KS];
             load_keys(8 * j, w);
@@ -519,7 +528,8 @@ paged_attn_kernel(const AttnArgs A, const __grid_constant__ CUtensorMap tm_k, co
             for (int k = 0; k < KS; ++k) {
               uint32_t b0, b1;
               cvt4(w[k], b0, b1);
-              mma_f16(s[j], qf[k], b0, b1);
+              if (k == 0) mma_f16_0(s[j], qf[k], b0, b1);
+              else mma_f16(s[j], qf[k], b0, b1);
             }
           } else {
             uint32_t w[KS], x[KS];
@@ -530,7 +540,8 @@ paged_attn_kernel(const AttnArgs A, const __grid_constant__ CUtensorMap tm_k, co
               uint32_t a[4];
               cvt4(w[k], a[0], a[2]);
               cvt4(x[k], a[1], a[3]);
-              mma_f16(s[j], a, qf[k][0], qf[k][1]);
+              if (k == 0) mma_f16_0(s[j], a, qf[k][0], qf[k][1]);
+              else mma_f16(s[j], a, qf[k][0], qf[k][1]);
             }
           }
         }
@@ -556,7 +567,7 @@ paged_attn_kernel(const AttnArgs A, const __grid_constant__ CUtensorMap tm_k, co
         // ---- masks: behind a row's keys, and pages that were not loaded ----
         const int end = min(TK, seg_lim - k0);                        // keys of the tile that some row sees
         // a page in front of `end` is missing
-        const bool hole = my_gone & ((1u << ((end + box - 1) >> box_log)) - 1);
+        const bool hole = missing & ((1u << ((end + box - 1) >> box_log)) - 1);
         if (k0 + TK > min_lim || hole) {
 #pragma unroll
           for (int j = 0; j < SF; ++j)
@@ -565,39 +576,41 @@ paged_attn_kernel(const AttnArgs A, const __grid_constant__ CUtensorMap tm_k, co
               const int at = R == 16 ? 8 * j + 2 * qd + (e & 1) : 16 * j + g + 8 * (e >> 1);
               const bool second = R == 16 ? e >> 1 : e & 1;
               if (k0 + at >= (second ? lim1 : lim0)) s[j][e] = -INFINITY;
-              if (my_gone >> (at >> box_log) & 1) s[j][e] = -INFINITY;
+              if (missing >> (at >> box_log) & 1) s[j][e] = -INFINITY;
             }
         }
         // ---- running maximum ----
-        float vref, f0[TS], f1[TS], rel[TS];                          // by step of 16 keys
-        bool flat = true;                                             // one value scale for the whole tile
+        float vref, f0[TS], f1[TS], lrel[TS], irel[TS];               // by step of 16 keys
         float x0 = -INFINITY, x1 = -INFINITY;
-        if (boxes == 1) {
-          const float ks = __shfl_sync(0xffffffffu, my_scl, 0);
-          vref = __shfl_sync(0xffffffffu, my_scl, NP);
+        if (box == TK) {
+          const float ks = __shfl_sync(0xffffffffu, my_scl, pg0);
+          vref = __shfl_sync(0xffffffffu, my_scl, pg0 + NP);
 #pragma unroll
           for (int i = 0; i < TS; ++i) {
             f0[i] = fmaxf(ks * rs0, 1.17549435e-38f);                 // 0 would turn -inf into NaN
             f1[i] = fmaxf(ks * rs1, 1.17549435e-38f);
-            rel[i] = 1.f;
+            lrel[i] = 0.f;
+            irel[i] = 1.f;
           }
         } else {
           vref = 0.f;
 #pragma unroll
           for (int i = 0; i < TS; ++i) {
-            const int pg = (i * 16) >> box_log;
+            const int pg = pg0 + ((i * 16) >> box_log);
             const float ks = __shfl_sync(0xffffffffu, my_scl, pg);
             f0[i] = fmaxf(ks * rs0, 1.17549435e-38f);
             f1[i] = fmaxf(ks * rs1, 1.17549435e-38f);
-            rel[i] = __shfl_sync(0xffffffffu, my_scl, pg + NP);
-            vref = fmaxf(vref, rel[i]);
+            irel[i] = __shfl_sync(0xffffffffu, my_scl, pg + NP);
+            vref = fmaxf(vref, irel[i]);
           }
-          // (a page that was not loaded has scale 0, and its probabilities are 0)
+          // A page's value scale relative to vref goes into the exponent, and out of the sum again. Below 2^-60 its
+          // probabilities are zeros in fp16 whatever they are; one that was not loaded (scale 0) has none.
+          const float lref = __log2f(vref);
 #pragma unroll
-          for (int i = 0; i < TS; ++i) flat = flat && (rel[i] == vref || rel[i] == 0.f);
-          const float vinv = vref > 0.f ? 1.f / vref : 0.f;
-#pragma unroll
-          for (int i = 0; i < TS; ++i) rel[i] *= vinv;
+          for (int i = 0; i < TS; ++i) {
+            lrel[i] = irel[i] > 0.f ? fmaxf(__log2f(irel[i]) - lref, -60.f) : 0.f;
+            irel[i] = exp2f_approx(-lrel[i]);
+          }
         }
         constexpr int PS = SF / TS;                                   // fragments of a step of 16 keys
 #pragma unroll
@@ -628,11 +641,13 @@ paged_attn_kernel(const AttnArgs A, const __grid_constant__ CUtensorMap tm_k, co
         uint32_t pf[TS][4];
 #pragma unroll
         for (int i = 0; i < TS; ++i) {
+          const float y0 = z0 + lrel[i], y1 = z1 + lrel[i];
+          const uint64_t fa = R == 16 ? pk2s(f0[i]) : pk2(f0[i], f1[i]), za = R == 16 ? pk2s(y0) : pk2(y0, y1);
+          const uint64_t fb = R == 16 ? pk2s(f1[i]) : fa, zb = R == 16 ? pk2s(y1) : za;
+          uint64_t part_a, part_b;
 #pragma unroll
           for (int t = 0; t < PS; ++t) {
             const float* sj = s[PS * i + t];
-            const uint64_t fa = R == 16 ? pk2s(f0[i]) : pk2(f0[i], f1[i]), za = R == 16 ? pk2s(z0) : pk2(z0, z1);
-            const uint64_t fb = R == 16 ? pk2s(f1[i]) : fa, zb = R == 16 ? pk2s(z1) : za;
             float p0, p1, p2, p3;
             pk2_split(pk2_fma(pk2(sj[0], sj[1]), fa, za), p0, p1);
             pk2_split(pk2_fma(pk2(sj[2], sj[3]), fb, zb), p2, p3);
@@ -640,17 +655,13 @@ paged_attn_kernel(const AttnArgs A, const __grid_constant__ CUtensorMap tm_k, co
             p1 = exp2f_approx(p1);
             p2 = exp2f_approx(p2);
             p3 = exp2f_approx(p3);
-            sum = pk2_add(sum, pk2(p0, p1));
-            sum2 = pk2_add(sum2, pk2(p2, p3));
-            if (!flat) {
-              p0 *= rel[i];
-              p1 *= rel[i];
-              p2 *= rel[i];
-              p3 *= rel[i];
-            }
+            part_a = t == 0 ? pk2(p0, p1) : pk2_add(part_a, pk2(p0, p1));
+            part_b = t == 0 ? pk2(p2, p3) : pk2_add(part_b, pk2(p2, p3));
             pf[i][2 * t] = pack_f16(p0, p1);
             pf[i][2 * t + 1] = pack_f16(p2, p3);
           }
+          sum = pk2_fma(part_a, pk2s(irel[i]), sum);
+          sum2 = pk2_fma(part_b, pk2s(irel[i]), sum2);
           if constexpr (R == 8) {
             pf[i][0] = transpose8(pf[i][0]);
             pf[i][1] = transpose8(pf[i][1]);
@@ -669,7 +680,7 @@ paged_attn_kernel(const AttnArgs A, const __grid_constant__ CUtensorMap tm_k, co
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
               const int at = 16 * i + 2 * qd + (r & 1) + 8 * (r >> 1);
-              const bool drop = at >= end || (my_gone >> (at >> box_log) & 1);
+              const bool drop = at >= end || (missing >> (at >> box_log) & 1);
 #pragma unroll
               for (int w = 0; w < D / 32; ++w) vw[i][r][w] = drop ? 0u : vw[i][r][w];
             }
@@ -680,8 +691,6 @@ paged_attn_kernel(const AttnArgs A, const __grid_constant__ CUtensorMap tm_k, co
           constexpr int F = R / 4;                                    // output fragments of four of the lane's dims
           float acc[F][4];
 #pragma unroll
-          for (int e = 0; e < F; ++e) acc[e][0] = acc[e][1] = acc[e][2] = acc[e][3] = 0.f;
-#pragma unroll
           for (int i = 0; i < TS; ++i) {
             // pairs of keys for four dims: bytes of two rows side by side
             uint32_t b0[4], b1[4];
@@ -691,12 +700,15 @@ paged_attn_kernel(const AttnArgs A, const __grid_constant__ CUtensorMap tm_k, co
             cvt4(__byte_perm(vw[i][2][w], vw[i][3][w], 0x7362), b1[2], b1[3]);
             if constexpr (R == 16) {
 #pragma unroll
-              for (int e = 0; e < 4; ++e) mma_f16(acc[e % F], pf[i], b0[e], b1[e]);
+              for (int e = 0; e < 4; ++e)
+                if (i == 0) mma_f16_0(acc[e % F], pf[i], b0[e], b1[e]);
+                else mma_f16(acc[e % F], pf[i], b0[e], b1[e]);
             } else {
 #pragma unroll
               for (int e = 0; e < 2; ++e) {
                 const uint32_t a[4] = {b0[2 * e], b0[2 * e + 1], b1[2 * e], b1[2 * e + 1]};
-                mma_f16(acc[e], a, pf[i][0], pf[i][1]);
+                if (i == 0) mma_f16_0(acc[e], a, pf[i][0], pf[i][1]);
+                else mma_f16(acc[e], a, pf[i][0], pf[i][1]);
               }
             }
           }
@@ -730,7 +742,7 @@ paged_attn_kernel(const AttnArgs A, const __grid_constant__ CUtensorMap tm_k, co
     }
     const bool writes_ml = R == 16 ? qd == 0 : g == 0;      // one lane for each pair of rows
     if constexpr (W > 1) {
-      if (S.len > TK) {                     // else warp 0 has it all
+      if (S.len > WK) {                     // else warp 0 has it all
 #pragma unroll
         for (int n = W / 2; n > 0; n /= 2) {                // warps n .. 2 n - 1 go to warps 0 .. n - 1
           __syncthreads();
@@ -881,6 +893,396 @@ __global__ void __launch_bounds__(256) paged_attn_join_kernel(const AttnArgs A) 
   if (A.lse && ln == 0) A.lse[at] = l == 0.f ? -INFINITY : (m - 15.f + log2f(l)) * 0.6931471805599453f;
 }
 
+// Many rows to a key head (prompts, pieces of prompts): bound by the products.
+//
+// A block takes 16 MT CW rows of one sequence and key head; CW warps of 16 MT
+// rows each share the copies of 64 keys that one more warp has TMA load. The
+// fragments of a tile are converted once for the MT row tiles of a warp. Value
+// scales are taken relative to the largest of all pages that the block reads,
+// so that products go straight into the output; the output is scaled only when
+// some row's maximum has grown by more than 2^8 (probabilities are held as
+// 2^7 p and reach 2^15). Blocks with many keys come first.
+template <int D> struct Many;
+template <> struct Many<32> { static constexpr int MT = 2, TK = 32, ST = 4, PER_SM = 3; };
+template <> struct Many<64> { static constexpr int MT = 2, TK = 32, ST = 4, PER_SM = 2; };
+template <> struct Many<128> { static constexpr int MT = 1, TK = 32, ST = 3, PER_SM = 2; };
+constexpr int kCW = 4;                  // warps that compute
+constexpr int kUnit = 64;               // keys of a copy
+
+template <int D>
+__global__ void __launch_bounds__((kCW + 1) * 32, Many<D>::PER_SM)
+paged_attn_many_kernel(const AttnArgs A, const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v) {
+  constexpr int MT = Many<D>::MT, TK = Many<D>::TK, ST = Many<D>::ST;
+  constexpr int R = 16 * MT * kCW;
+  constexpr int KS = D / 16, NT = TK / 8, TS = TK / 16, NO = D / 8;
+  constexpr int kHalf = kUnit * D;
+  extern __shared__ __align__(1024) uint8_t s_ring[];       // [ST] copies: 64 rows of keys, 64 rows of values
+  __shared__ uint64_t s_full[ST], s_empty[ST];
+  __shared__ float s_ks[ST][4], s_lv[ST][4];                // scales of a copy's pages: keys, log2 of values' (relative)
+  __shared__ uint32_t s_gone[ST];
+  __shared__ float s_top[kCW + 1];
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int b = blockIdx.x / A.H, h = blockIdx.x % A.H, mt = gridDim.y - 1 - blockIdx.y;
+  Seq<R> S;
+  S.load(A, b);
+  if (mt >= S.tiles_m) return;
+  const int rows = S.n * A.G, r0 = mt * R;
+  const int last = min(r0 + R, rows) - 1;
+  const int lim = A.causal ? max(0, S.len - S.n + last / A.G + 1) : S.len;    // keys that the last row sees
+  const int units = (lim + kUnit - 1) / kUnit;
+  const int* table = A.table + b * A.table_stride;
+  if (threadIdx.x < ST) {
+    asm volatile("mbarrier.init.shared::cta.b64 [%0], 2;" ::"r"(smem_u32(&s_full[threadIdx.x])));
+    asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(smem_u32(&s_empty[threadIdx.x])), "r"(kCW));
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  // the largest value scale of the block's pages
+  float top = 0.f;
+  for (int i = threadIdx.x; i * A.P < lim; i += (kCW + 1) * 32) {
+    const int page = __ldg(table + i);
+    if (page >= 0 && page < A.n_pages) top = fmaxf(top, __ldg(A.vs + page * A.H + h));
+  }
+  top = warp_max(top);
+  if (lane == 0) s_top[warp] = top;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w <= kCW; ++w) top = fmaxf(top, s_top[w]);
+
+  const uint32_t ring = smem_u32(s_ring);
+  if (warp == kCW) {
+    // ---- copies ----
+    const int boxes = kUnit >> A.logP;
+    const float ltop = __log2f(top);
+    bool alive = true;
+    int page = -1;
+    auto fetch = [&](int u) {
+      const int key = u * kUnit + lane * A.P;
+      page = lane < boxes && key < lim ? __ldg(table + (key >> A.logP)) : -1;
+    };
+    fetch(0);
+    for (int u = 0; u < units; ++u) {
+      const int st = u % ST, turn = u / ST;
+      const uint32_t full = smem_u32(&s_full[st]), dst = ring + st * 2 * kHalf;
+      const bool want = lane < boxes && u * kUnit + lane * A.P < lim;
+      const bool have = want && page >= 0 && page < A.n_pages;
+      if (want && !have) set_error(A.err, kIdOutOfRange);
+      const int block = have ? page * A.H + h : 0;
+      const uint32_t mask = __ballot_sync(0xffffffffu, have);
+      fetch(u + 1);
+      if (alive && turn > 0) alive = mbar_wait(smem_u32(&s_empty[st]), (turn - 1) & 1, A.err);
+      alive = __all_sync(0xffffffffu, alive);
+      if (lane == 0)
+        asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;"
+                     ::"r"(full), "r"(uint32_t(__popc(mask) * 2 * A.P * D)) : "memory");
+#pragma unroll 1
+      for (int i = 0; i < boxes; ++i) {
+        const int row = __shfl_sync(0xffffffffu, block, i) * A.P;
+        if (lane == 0 && (mask >> i & 1)) {
+          tma_rows(dst + i * A.P * D, &tm_k, full, row);
+          tma_rows(dst + kHalf + i * A.P * D, &tm_v, full, row);
+        }
+      }
+      if (lane < boxes) {
+        s_ks[st][lane] = have ? __ldg(A.ks + block) : 0.f;
+        // below 2^-60 of the largest its probabilities are zeros in fp16 whatever they are
+        const float v = have ? __ldg(A.vs + block) : 0.f;
+        s_lv[st][lane] = v > 0.f ? fmaxf(__log2f(v) - ltop, -60.f) : -60.f;
+      }
+      if (lane == 0) s_gone[st] = ~mask;
+      __syncwarp();
+      if (lane == 0)
+        asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(full) : "memory");
+    }
+    return;
+  }
+
+  // ---- rows ----
+  const int g = lane >> 2, qd = lane & 3;
+  const int w0 = r0 + warp * 16 * MT;                       // this warp's first row
+  uint32_t qf[MT][KS][4];
+  float rs[MT][2];
+  int lims[MT][2];
+  int min_lim, max_lim;
+  {
+    constexpr int E = D / 4;
+#pragma unroll
+    for (int t = 0; t < MT; ++t) {
+      float x[2][E];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int r = w0 + 16 * t + 8 * i + g;
+        const bool live = r < rows;
+        const int qi = live ? r / A.G : 0;
+        const uint16_t* src = static_cast<const uint16_t*>(A.q) +
+                              (A.cu ? int64_t(S.tok0 + qi) * A.q_ts : int64_t(b) * A.q_bs + int64_t(qi) * A.q_ts) +
+                              int64_t(h * A.G + (live ? r - qi * A.G : 0)) * A.q_hs + qd * E;
+#pragma unroll
+        for (int e = 0; e < E; ++e) x[i][e] = 0.f;
+        if (live) {
+          if (reinterpret_cast<uintptr_t>(src) % 16 == 0) {
+#pragma unroll
+            for (int e = 0; e < E; e += 8) load8_16(src + e, A.bf16, &x[i][e]);
+          } else {
+#pragma unroll
+            for (int e = 0; e < E; ++e) x[i][e] = to_f_16(src[e], A.bf16);
+          }
+        }
+        float amax = 0.f;
+#pragma unroll
+        for (int e = 0; e < E; ++e) amax = fmaxf(amax, fabsf(x[i][e]));
+        amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+        amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
+        const int ex = amax > 0.f && amax < INFINITY ? max(-100, (__float_as_int(amax) >> 23) - 127) : 14;
+        const float up = copysignf(__int_as_float((14 - ex + 127) << 23), A.scale_log2);
+        rs[t][i] = __int_as_float((ex - 14 + 127) << 23) * fabsf(A.scale_log2);
+        lims[t][i] = !live ? 0 : A.causal ? max(0, S.len - S.n + qi + 1) : S.len;
+#pragma unroll
+        for (int e = 0; e < E; ++e) x[i][e] *= up;
+      }
+#pragma unroll
+      for (int k = 0; k < KS; ++k) {
+        qf[t][k][0] = pack_f16(x[0][4 * k], x[0][4 * k + 1]);
+        qf[t][k][1] = pack_f16(x[1][4 * k], x[1][4 * k + 1]);
+        qf[t][k][2] = pack_f16(x[0][4 * k + 2], x[0][4 * k + 3]);
+        qf[t][k][3] = pack_f16(x[1][4 * k + 2], x[1][4 * k + 3]);
+      }
+    }
+    min_lim = A.causal ? S.len - S.n + w0 / A.G + 1 : S.len;
+    const int wl = min(w0 + 16 * MT, rows) - 1;             // this warp's last row
+    max_lim = wl < w0 ? 0 : A.causal ? max(0, S.len - S.n + wl / A.G + 1) : S.len;
+  }
+  uint32_t k_off, v_off[2];
+  if (D == 128) {
+    k_off = g * 128 + ((2 * qd) ^ g) * 16;
+    v_off[0] = (2 * qd) * 128 + (g ^ (2 * qd)) * 16;
+    v_off[1] = (2 * qd + 1) * 128 + (g ^ (2 * qd + 1)) * 16;
+  } else if (D == 64) {
+    k_off = g * 64 + (qd ^ (g >> 1)) * 16;
+    v_off[0] = (2 * qd) * 64 + ((g >> 1) ^ qd) * 16 + (g & 1) * 8;
+    v_off[1] = v_off[0] + 64;
+  } else {
+    k_off = g * 32 + ((qd >> 1) ^ (g >> 2)) * 16 + (qd & 1) * 8;
+    v_off[0] = (2 * qd) * 32 + ((g >> 2) ^ (qd >> 1)) * 16 + (g & 3) * 4;
+    v_off[1] = v_off[0] + 32;
+  }
+  float o[MT][NO][4], m[MT][2], l[MT][2];
+#pragma unroll
+  for (int t = 0; t < MT; ++t) {
+    m[t][0] = m[t][1] = -INFINITY;
+    l[t][0] = l[t][1] = 0.f;
+#pragma unroll
+    for (int u = 0; u < NO; ++u) o[t][u][0] = o[t][u][1] = o[t][u][2] = o[t][u][3] = 0.f;
+  }
+  bool alive = true;
+  uint32_t st = 0, phase = 0;
+#pragma unroll 1
+  for (int u = 0; u < units; ++u) {
+    if (alive) alive = mbar_wait(smem_u32(&s_full[st]), phase, A.err);
+    __syncwarp();
+    const uint32_t all_gone = s_gone[st];
+#pragma unroll 1
+    for (int sub = 0; sub < kUnit / TK; ++sub) {
+      const int k0 = u * kUnit + sub * TK;
+      if (k0 >= max_lim) break;
+      const uint32_t kt = ring + st * 2 * kHalf + sub * TK * D, vt = kt + kHalf;
+      // ---- scores ----
+      float s[MT][NT][4];
+#pragma unroll
+      for (int j = 0; j < NT; ++j) {
+        uint32_t w[KS];
+        if constexpr (D == 128) {
+          const uint4 a = lds128(kt + k_off + 8 * j * D), c = lds128(kt + (k_off ^ 16) + 8 * j * D);
+          w[0] = a.x; w[1] = a.y; w[2] = a.z; w[3] = a.w;
+          w[4] = c.x; w[5] = c.y; w[6] = c.z; w[7] = c.w;
+        } else if constexpr (D == 64) {
+          const uint4 a = lds128(kt + k_off + 8 * j * D);
+          w[0] = a.x; w[1] = a.y; w[2] = a.z; w[3] = a.w;
+        } else {
+          const uint2 a = lds64(kt + k_off + 8 * j * D);
+          w[0] = a.x; w[1] = a.y;
+        }
+#pragma unroll
+        for (int k = 0; k < KS; ++k) {
+          uint32_t b0, b1;
+          cvt4(w[k], b0, b1);
+#pragma unroll
+          for (int t = 0; t < MT; ++t)
+            if (k == 0) mma_f16_0(s[t][j], qf[t][k], b0, b1);
+            else mma_f16(s[t][j], qf[t][k], b0, b1);
+        }
+      }
+      // ---- masks ----
+      const int end = min(TK, max_lim - k0);                // keys of the tile that some row of the warp sees
+      const uint32_t seen = (2u << ((sub * TK + end - 1) >> A.logP)) - 1;     // pages of the copy up to there
+      const bool hole = all_gone & seen;
+      if (k0 + TK > min_lim || hole) {
+#pragma unroll
+        for (int j = 0; j < NT; ++j)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const int at = sub * TK + 8 * j + 2 * qd + e, key = u * kUnit + at;
+            const bool drop = all_gone >> (at >> A.logP) & 1;
+#pragma unroll
+            for (int t = 0; t < MT; ++t) {
+              if (drop || key >= lims[t][0]) s[t][j][e] = -INFINITY;
+              if (drop || key >= lims[t][1]) s[t][j][2 + e] = -INFINITY;
+            }
+          }
+      }
+      // ---- scores of the pages: maxima in the log2 domain ----
+      float ks[TS], lv[TS], iv[TS];
+#pragma unroll
+      for (int i = 0; i < TS; ++i) {
+        const int pg = (sub * TK + 16 * i) >> A.logP;
+        ks[i] = s_ks[st][pg];
+        lv[i] = s_lv[st][pg];
+        iv[i] = exp2f_approx(-lv[i]);
+      }
+      bool grows = false;
+      float x[MT][2];
+#pragma unroll
+      for (int t = 0; t < MT; ++t)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          float y = -INFINITY;
+#pragma unroll
+          for (int k = 0; k < TS; ++k)
+            y = fmaxf(y, fmaxf(fmaxf(s[t][2 * k][2 * i], s[t][2 * k][2 * i + 1]),
+                               fmaxf(s[t][2 * k + 1][2 * i], s[t][2 * k + 1][2 * i + 1])) *
+                             fmaxf(ks[k] * rs[t][i], 1.17549435e-38f));
+          y = fmaxf(y, __shfl_xor_sync(0xffffffffu, y, 1));
+          y = fmaxf(y, __shfl_xor_sync(0xffffffffu, y, 2));
+          x[t][i] = y;
+          grows |= y > m[t][i] + 8.f;
+        }
+      if (__any_sync(0xffffffffu, grows)) {
+#pragma unroll
+        for (int t = 0; t < MT; ++t) {
+          float al[2];
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const float n = x[t][i] > m[t][i] + 8.f ? x[t][i] : m[t][i];
+            al[i] = m[t][i] == n ? 1.f : exp2f_approx(m[t][i] - n);
+            m[t][i] = n;
+            l[t][i] *= al[i];
+          }
+#pragma unroll
+          for (int v = 0; v < NO; ++v) {
+            o[t][v][0] *= al[0];
+            o[t][v][1] *= al[0];
+            o[t][v][2] *= al[1];
+            o[t][v][3] *= al[1];
+          }
+        }
+      }
+      // ---- probabilities (times 2^7 and the page's relative value scale) and their sum ----
+      uint32_t pf[MT][TS][4];
+#pragma unroll
+      for (int t = 0; t < MT; ++t) {
+        const float z0 = 7.f - (m[t][0] == -INFINITY ? 0.f : m[t][0]), z1 = 7.f - (m[t][1] == -INFINITY ? 0.f : m[t][1]);
+        uint64_t sum0 = pk2(0.f, 0.f), sum1 = pk2(0.f, 0.f);
+#pragma unroll
+        for (int i = 0; i < TS; ++i) {
+          const uint64_t fa = pk2s(fmaxf(ks[i] * rs[t][0], 1.17549435e-38f)), za = pk2s(z0 + lv[i]);
+          const uint64_t fb = pk2s(fmaxf(ks[i] * rs[t][1], 1.17549435e-38f)), zb = pk2s(z1 + lv[i]);
+          uint64_t pa, pb;
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            const float* sj = s[t][2 * i + c];
+            float p0, p1, p2, p3;
+            pk2_split(pk2_fma(pk2(sj[0], sj[1]), fa, za), p0, p1);
+            pk2_split(pk2_fma(pk2(sj[2], sj[3]), fb, zb), p2, p3);
+            p0 = exp2f_approx(p0);
+            p1 = exp2f_approx(p1);
+            p2 = exp2f_approx(p2);
+            p3 = exp2f_approx(p3);
+            pa = c == 0 ? pk2(p0, p1) : pk2_add(pa, pk2(p0, p1));
+            pb = c == 0 ? pk2(p2, p3) : pk2_add(pb, pk2(p2, p3));
+            pf[t][i][2 * c] = pack_f16(p0, p1);
+            pf[t][i][2 * c + 1] = pack_f16(p2, p3);
+          }
+          sum0 = pk2_fma(pa, pk2s(iv[i]), sum0);
+          sum1 = pk2_fma(pb, pk2s(iv[i]), sum1);
+        }
+        float a0, a1;
+        pk2_split(sum0, a0, a1);
+        l[t][0] += a0 + a1;
+        pk2_split(sum1, a0, a1);
+        l[t][1] += a0 + a1;
+      }
+      // ---- values: what lies behind the keys may be anything, NaN too ----
+#pragma unroll
+      for (int i = 0; i < TS; ++i) {
+        uint32_t vw[4][D / 32];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const uint32_t a = vt + v_off[r & 1] + (16 * i + 8 * (r >> 1)) * D;
+          if constexpr (D == 128) {
+            const uint4 c = lds128(a);
+            vw[r][0] = c.x; vw[r][1] = c.y; vw[r][2] = c.z; vw[r][3] = c.w;
+          } else if constexpr (D == 64) {
+            const uint2 c = lds64(a);
+            vw[r][0] = c.x; vw[r][1] = c.y;
+          } else {
+            vw[r][0] = lds32(a);
+          }
+        }
+        if (hole || end < TK) {
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            const int at = 16 * i + 2 * qd + (r & 1) + 8 * (r >> 1);
+            const bool drop = at >= end || (all_gone >> ((sub * TK + at) >> A.logP) & 1);
+#pragma unroll
+            for (int w = 0; w < D / 32; ++w) vw[r][w] = drop ? 0u : vw[r][w];
+          }
+        }
+#pragma unroll
+        for (int w = 0; w < D / 32; ++w) {
+          uint32_t b0[4], b1[4];
+          cvt4(__byte_perm(vw[0][w], vw[1][w], 0x5140), b0[0], b0[1]);
+          cvt4(__byte_perm(vw[0][w], vw[1][w], 0x7362), b0[2], b0[3]);
+          cvt4(__byte_perm(vw[2][w], vw[3][w], 0x5140), b1[0], b1[1]);
+          cvt4(__byte_perm(vw[2][w], vw[3][w], 0x7362), b1[2], b1[3]);
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+#pragma unroll
+            for (int t = 0; t < MT; ++t) mma_f16(o[t][4 * w + e], pf[t][i], b0[e], b1[e]);
+        }
+      }
+    }
+    __syncwarp();                           // the copy has been read
+    if (lane == 0)
+      asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(&s_empty[st])) : "memory");
+    if (++st == ST) {
+      st = 0;
+      phase ^= 1;
+    }
+  }
+#pragma unroll
+  for (int t = 0; t < MT; ++t)
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      float sum = l[t][i];
+      sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+      sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+      const int r = w0 + 16 * t + 8 * i + g;
+      if (r >= rows) continue;
+      const int qi = r / A.G;
+      const int64_t at = int64_t(S.tok0 + qi) * A.Hq + h * A.G + (r - qi * A.G);
+      const float inv = sum == 0.f ? 0.f : top / sum;       // a sum of 0: no keys. A NaN stays one
+      uint16_t* dst = static_cast<uint16_t*>(A.o) + at * D + qd * (D / 4);
+#pragma unroll
+      for (int c = 0; c < 2; ++c)
+#pragma unroll
+        for (int u = 0; u < NO; u += 4)
+          *reinterpret_cast<uint2*>(dst + c * NO + u) =
+              make_uint2(pack_16(o[t][u][2 * i + c] * inv, o[t][u + 1][2 * i + c] * inv, A.bf16),
+                         pack_16(o[t][u + 2][2 * i + c] * inv, o[t][u + 3][2 * i + c] * inv, A.bf16));
+      if (A.lse && qd == 0) A.lse[at] = sum == 0.f ? -INFINITY : (m[t][i] - 7.f + log2f(sum)) * 0.6931471805599453f;
+    }
+}
+
 // cuTensorMapEncodeTiled through the runtime: the extension does not link
 // libcuda, so it imports on machines without a driver.
 static CUresult encode_tiled(CUtensorMap* m, void* base, const cuuint64_t* dims, const cuuint64_t* strides,
@@ -934,8 +1336,8 @@ struct Bounds {                 // of what the lengths on the device can ask for
 
 template <int D, int R, int W>
 static void few_launch(AttnArgs& A, const at::Tensor& ck, const at::Tensor& cv, const Bounds& U) {
-  constexpr int TK = Cfg<D>::TK, ST = Cfg<D>::ST, SUP = TK * W;
-  constexpr int kSmem = kWarps * ST * 2 * TK * D;
+  constexpr int TK = Cfg<D>::TK, WK = TK * Cfg<D>::SUB, SUP = WK * W;
+  constexpr int kSmem = kWarps * Cfg<D>::ST * 2 * WK * D;
   static int known[64] = {};
   auto kern = paged_attn_kernel<D, R, W>;
   const int64_t slots = int64_t(num_sms()) * blocks_per_sm(kern, kWarps * 32, kSmem, known);
@@ -973,9 +1375,24 @@ static void few_launch(AttnArgs& A, const at::Tensor& ck, const at::Tensor& cv, 
 }
 
 template <int D>
+static void many_launch(AttnArgs& A, const at::Tensor& ck, const at::Tensor& cv, const Bounds& U) {
+  constexpr int kSmem = Many<D>::ST * 2 * kUnit * D;
+  constexpr int R = 16 * Many<D>::MT * kCW;
+  static int known[64] = {};
+  auto kern = paged_attn_many_kernel<D>;
+  blocks_per_sm(kern, (kCW + 1) * 32, kSmem, known);
+  const dim3 grid(unsigned(U.B * A.H), unsigned((U.rows + R - 1) / R));
+  kern<<<grid, (kCW + 1) * 32, kSmem, stream()>>>(A, code_map(ck, A.P), code_map(cv, A.P));
+  PD_CHECK_LAUNCH();
+}
+
+template <int D>
 static void attn_dispatch(AttnArgs& A, const at::Tensor& ck, const at::Tensor& cv, const Bounds& U) {
   // a warp a segment where there are eight segments and more for every warp of the device (12 warps an SM)
   const bool many = U.B * A.H * ((U.rows + 15) / 16) >= int64_t(num_sms()) * 12 * 4;
+  const int64_t tiles = (U.rows + 16 * Many<D>::MT * kCW - 1) / (16 * Many<D>::MT * kCW);
+  if (U.rows > 32 && U.B * A.H * tiles >= num_sms() && tiles < 65536 && U.B * A.H < (int64_t(1) << 31))
+    return many_launch<D>(A, ck, cv, U);
   if (U.rows <= 8) return many ? few_launch<D, 8, 1>(A, ck, cv, U) : few_launch<D, 8, 4>(A, ck, cv, U);
   return many ? few_launch<D, 16, 1>(A, ck, cv, U) : few_launch<D, 16, 4>(A, ck, cv, U);
 }
