@@ -895,32 +895,34 @@ __global__ void __launch_bounds__(256) paged_attn_join_kernel(const AttnArgs A) 
 
 // Many rows to a key head (prompts, pieces of prompts): bound by the products.
 //
-// A block takes 16 MT CW rows of one sequence and key head; CW warps of 16 MT
-// rows each share the copies of 64 keys that one more warp has TMA load. The
-// fragments of a tile are converted once for the MT row tiles of a warp. Value
-// scales are taken relative to the largest of all pages that the block reads,
-// so that products go straight into the output; the output is scaled only when
-// some row's maximum has grown by more than 2^8 (probabilities are held as
-// 2^7 p and reach 2^15). Blocks with many keys come first.
+// A block takes 16 MT rows a warp of one sequence and key head; its warps
+// share copies of 64 keys that warp 0 has TMA load two copies ahead. The
+// fragments of a tile are converted once for the MT row tiles of a warp;
+// queries wait in shared memory in the order of their fragments, which leaves
+// registers for three (d = 32: four) blocks an SM. Value scales are taken
+// relative to the largest of all pages that the block reads, so that products
+// go straight into the output; the output is scaled only when some row's
+// maximum has grown by more than 2^8 (probabilities are held as 2^7 p and
+// reach 2^15). Blocks with many keys come first.
 template <int D> struct Many;
-template <> struct Many<32> { static constexpr int MT = 2, TK = 32, ST = 4, PER_SM = 3; };
-template <> struct Many<64> { static constexpr int MT = 2, TK = 32, ST = 4, PER_SM = 2; };
-template <> struct Many<128> { static constexpr int MT = 1, TK = 32, ST = 3, PER_SM = 2; };
-constexpr int kCW = 4;                  // warps that compute
+template <> struct Many<32> { static constexpr int MT = 2, TK = 32, ST = 4, PER_SM = 4; };
+template <> struct Many<64> { static constexpr int MT = 2, TK = 32, ST = 4, PER_SM = 3; };
+template <> struct Many<128> { static constexpr int MT = 1, TK = 32, ST = 3, PER_SM = 3; };
 constexpr int kUnit = 64;               // keys of a copy
 
 template <int D>
-__global__ void __launch_bounds__((kCW + 1) * 32, Many<D>::PER_SM)
+__global__ void __launch_bounds__(kWarps * 32, Many<D>::PER_SM)
 paged_attn_many_kernel(const AttnArgs A, const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v) {
   constexpr int MT = Many<D>::MT, TK = Many<D>::TK, ST = Many<D>::ST;
-  constexpr int R = 16 * MT * kCW;
+  constexpr int R = 16 * MT * kWarps;
   constexpr int KS = D / 16, NT = TK / 8, TS = TK / 16, NO = D / 8;
   constexpr int kHalf = kUnit * D;
   extern __shared__ __align__(1024) uint8_t s_ring[];       // [ST] copies: 64 rows of keys, 64 rows of values
+  __shared__ uint4 s_q[kWarps][MT][KS][32];
   __shared__ uint64_t s_full[ST], s_empty[ST];
   __shared__ float s_ks[ST][4], s_lv[ST][4];                // scales of a copy's pages: keys, log2 of values' (relative)
   __shared__ uint32_t s_gone[ST];
-  __shared__ float s_top[kCW + 1];
+  __shared__ float s_top[kWarps];
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int b = blockIdx.x / A.H, h = blockIdx.x % A.H, mt = gridDim.y - 1 - blockIdx.y;
@@ -934,12 +936,12 @@ paged_attn_many_kernel(const AttnArgs A, const __grid_constant__ CUtensorMap tm_
   const int* table = A.table + b * A.table_stride;
   if (threadIdx.x < ST) {
     asm volatile("mbarrier.init.shared::cta.b64 [%0], 2;" ::"r"(smem_u32(&s_full[threadIdx.x])));
-    asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(smem_u32(&s_empty[threadIdx.x])), "r"(kCW));
+    asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(smem_u32(&s_empty[threadIdx.x])), "r"(kWarps));
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   // the largest value scale of the block's pages
   float top = 0.f;
-  for (int i = threadIdx.x; i * A.P < lim; i += (kCW + 1) * 32) {
+  for (int i = threadIdx.x; i * A.P < lim; i += kWarps * 32) {
     const int page = __ldg(table + i);
     if (page >= 0 && page < A.n_pages) top = fmaxf(top, __ldg(A.vs + page * A.H + h));
   }
@@ -947,60 +949,72 @@ paged_attn_many_kernel(const AttnArgs A, const __grid_constant__ CUtensorMap tm_
   if (lane == 0) s_top[warp] = top;
   __syncthreads();
 #pragma unroll
-  for (int w = 0; w <= kCW; ++w) top = fmaxf(top, s_top[w]);
+  for (int w = 0; w < kWarps; ++w) top = fmaxf(top, s_top[w]);
 
+  // ---- copies (warp 0): those of unit v, then, a step later, its pages' scales ----
   const uint32_t ring = smem_u32(s_ring);
-  if (warp == kCW) {
-    // ---- copies ----
-    const int boxes = kUnit >> A.logP;
-    const float ltop = __log2f(top);
-    bool alive = true;
-    int page = -1;
-    auto fetch = [&](int u) {
-      const int key = u * kUnit + lane * A.P;
-      page = lane < boxes && key < lim ? __ldg(table + (key >> A.logP)) : -1;
-    };
-    fetch(0);
-    for (int u = 0; u < units; ++u) {
-      const int st = u % ST, turn = u / ST;
-      const uint32_t full = smem_u32(&s_full[st]), dst = ring + st * 2 * kHalf;
-      const bool want = lane < boxes && u * kUnit + lane * A.P < lim;
-      const bool have = want && page >= 0 && page < A.n_pages;
-      if (want && !have) set_error(A.err, kIdOutOfRange);
-      const int block = have ? page * A.H + h : 0;
-      const uint32_t mask = __ballot_sync(0xffffffffu, have);
-      fetch(u + 1);
-      if (alive && turn > 0) alive = mbar_wait(smem_u32(&s_empty[st]), (turn - 1) & 1, A.err);
-      alive = __all_sync(0xffffffffu, alive);
-      if (lane == 0)
-        asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;"
-                     ::"r"(full), "r"(uint32_t(__popc(mask) * 2 * A.P * D)) : "memory");
-#pragma unroll 1
-      for (int i = 0; i < boxes; ++i) {
-        const int row = __shfl_sync(0xffffffffu, block, i) * A.P;
-        if (lane == 0 && (mask >> i & 1)) {
-          tma_rows(dst + i * A.P * D, &tm_k, full, row);
-          tma_rows(dst + kHalf + i * A.P * D, &tm_v, full, row);
-        }
-      }
-      if (lane < boxes) {
-        s_ks[st][lane] = have ? __ldg(A.ks + block) : 0.f;
-        // below 2^-60 of the largest its probabilities are zeros in fp16 whatever they are
-        const float v = have ? __ldg(A.vs + block) : 0.f;
-        s_lv[st][lane] = v > 0.f ? fmaxf(__log2f(v) - ltop, -60.f) : -60.f;
-      }
-      if (lane == 0) s_gone[st] = ~mask;
-      __syncwarp();
-      if (lane == 0)
-        asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(full) : "memory");
+  bool alive = true;
+  int page = -1, pending = -1;              // lane i: page i of the next unit; slot whose scales are on their way
+  float new_ks = 0.f, new_vs = 0.f;
+  uint32_t new_gone = 0;
+  const int boxes = kUnit >> A.logP;
+  auto fetch = [&](int v) {
+    const int key = v * kUnit + lane * A.P;
+    page = lane < boxes && key < lim ? __ldg(table + (key >> A.logP)) : -1;
+  };
+  auto settle = [&]() {
+    if (pending < 0) return;
+    if (lane < boxes) {
+      s_ks[pending][lane] = new_ks;
+      // below 2^-60 of the largest its probabilities are zeros in fp16 whatever they are
+      s_lv[pending][lane] = new_vs > 0.f ? fmaxf(__log2f(new_vs) - __log2f(top), -60.f) : -60.f;
     }
-    return;
+    if (lane == 0) s_gone[pending] = new_gone;
+    __syncwarp();
+    if (lane == 0)
+      asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(&s_full[pending])) : "memory");
+    pending = -1;
+  };
+  auto copy = [&](int v) {
+    if (v >= units) return;
+    const int sl = v % ST, turn = v / ST;
+    const uint32_t full = smem_u32(&s_full[sl]), dst = ring + sl * 2 * kHalf;
+    const bool want = lane < boxes && v * kUnit + lane * A.P < lim;
+    const bool have = want && page >= 0 && page < A.n_pages;
+    if (want && !have) set_error(A.err, kIdOutOfRange);
+    const int block = have ? page * A.H + h : 0;
+    const uint32_t mask = __ballot_sync(0xffffffffu, have);
+    if (alive && turn > 0) alive = mbar_wait(smem_u32(&s_empty[sl]), (turn - 1) & 1, A.err);
+    __syncwarp();
+    if (lane == 0)
+      asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;"
+                   ::"r"(full), "r"(uint32_t(__popc(mask) * 2 * A.P * D)) : "memory");
+#pragma unroll 1
+    for (int i = 0; i < boxes; ++i) {
+      const int row = __shfl_sync(0xffffffffu, block, i) * A.P;
+      if (lane == 0 && (mask >> i & 1)) {
+        tma_rows(dst + i * A.P * D, &tm_k, full, row);
+        tma_rows(dst + kHalf + i * A.P * D, &tm_v, full, row);
+      }
+    }
+    new_ks = have ? __ldg(A.ks + block) : 0.f;
+    new_vs = have ? __ldg(A.vs + block) : 0.f;
+    new_gone = ~mask;
+    pending = sl;
+    fetch(v + 1);
+  };
+  if (warp == 0) {
+    fetch(0);
+#pragma unroll 1
+    for (int v = 0; v < ST - 2; ++v) {
+      settle();
+      copy(v);
+    }
   }
 
   // ---- rows ----
   const int g = lane >> 2, qd = lane & 3;
   const int w0 = r0 + warp * 16 * MT;                       // this warp's first row
-  uint32_t qf[MT][KS][4];
   float rs[MT][2];
   int lims[MT][2];
   int min_lim, max_lim;
@@ -1041,12 +1055,10 @@ paged_attn_many_kernel(const AttnArgs A, const __grid_constant__ CUtensorMap tm_
         for (int e = 0; e < E; ++e) x[i][e] *= up;
       }
 #pragma unroll
-      for (int k = 0; k < KS; ++k) {
-        qf[t][k][0] = pack_f16(x[0][4 * k], x[0][4 * k + 1]);
-        qf[t][k][1] = pack_f16(x[1][4 * k], x[1][4 * k + 1]);
-        qf[t][k][2] = pack_f16(x[0][4 * k + 2], x[0][4 * k + 3]);
-        qf[t][k][3] = pack_f16(x[1][4 * k + 2], x[1][4 * k + 3]);
-      }
+      for (int k = 0; k < KS; ++k)
+        s_q[warp][t][k][lane] = make_uint4(pack_f16(x[0][4 * k], x[0][4 * k + 1]), pack_f16(x[1][4 * k], x[1][4 * k + 1]),
+                                           pack_f16(x[0][4 * k + 2], x[0][4 * k + 3]),
+                                           pack_f16(x[1][4 * k + 2], x[1][4 * k + 3]));
     }
     min_lim = A.causal ? S.len - S.n + w0 / A.G + 1 : S.len;
     const int wl = min(w0 + 16 * MT, rows) - 1;             // this warp's last row
@@ -1074,10 +1086,13 @@ paged_attn_many_kernel(const AttnArgs A, const __grid_constant__ CUtensorMap tm_
 #pragma unroll
     for (int u = 0; u < NO; ++u) o[t][u][0] = o[t][u][1] = o[t][u][2] = o[t][u][3] = 0.f;
   }
-  bool alive = true;
   uint32_t st = 0, phase = 0;
 #pragma unroll 1
   for (int u = 0; u < units; ++u) {
+    if (warp == 0) {
+      settle();
+      copy(u + ST - 2);
+    }
     if (alive) alive = mbar_wait(smem_u32(&s_full[st]), phase, A.err);
     __syncwarp();
     const uint32_t all_gone = s_gone[st];
@@ -1088,6 +1103,15 @@ paged_attn_many_kernel(const AttnArgs A, const __grid_constant__ CUtensorMap tm_
       const uint32_t kt = ring + st * 2 * kHalf + sub * TK * D, vt = kt + kHalf;
       // ---- scores ----
       float s[MT][NT][4];
+      {
+      uint32_t qf[MT][KS][4];
+#pragma unroll
+      for (int t = 0; t < MT; ++t)
+#pragma unroll
+        for (int k = 0; k < KS; ++k) {
+          const uint4 v = lds128(smem_u32(&s_q[warp][t][k][lane]));
+          qf[t][k][0] = v.x; qf[t][k][1] = v.y; qf[t][k][2] = v.z; qf[t][k][3] = v.w;
+        }
 #pragma unroll
       for (int j = 0; j < NT; ++j) {
         uint32_t w[KS];
@@ -1111,6 +1135,7 @@ paged_attn_many_kernel(const AttnArgs A, const __grid_constant__ CUtensorMap tm_
             if (k == 0) mma_f16_0(s[t][j], qf[t][k], b0, b1);
             else mma_f16(s[t][j], qf[t][k], b0, b1);
         }
+      }
       }
       // ---- masks ----
       const int end = min(TK, max_lim - k0);                // keys of the tile that some row of the warp sees
@@ -1377,12 +1402,12 @@ static void few_launch(AttnArgs& A, const at::Tensor& ck, const at::Tensor& cv, 
 template <int D>
 static void many_launch(AttnArgs& A, const at::Tensor& ck, const at::Tensor& cv, const Bounds& U) {
   constexpr int kSmem = Many<D>::ST * 2 * kUnit * D;
-  constexpr int R = 16 * Many<D>::MT * kCW;
+  constexpr int R = 16 * Many<D>::MT * kWarps;
   static int known[64] = {};
   auto kern = paged_attn_many_kernel<D>;
-  blocks_per_sm(kern, (kCW + 1) * 32, kSmem, known);
+  blocks_per_sm(kern, kWarps * 32, kSmem, known);
   const dim3 grid(unsigned(U.B * A.H), unsigned((U.rows + R - 1) / R));
-  kern<<<grid, (kCW + 1) * 32, kSmem, stream()>>>(A, code_map(ck, A.P), code_map(cv, A.P));
+  kern<<<grid, kWarps * 32, kSmem, stream()>>>(A, code_map(ck, A.P), code_map(cv, A.P));
   PD_CHECK_LAUNCH();
 }
 
@@ -1390,7 +1415,7 @@ template <int D>
 static void attn_dispatch(AttnArgs& A, const at::Tensor& ck, const at::Tensor& cv, const Bounds& U) {
   // a warp a segment where there are eight segments and more for every warp of the device (12 warps an SM)
   const bool many = U.B * A.H * ((U.rows + 15) / 16) >= int64_t(num_sms()) * 12 * 4;
-  const int64_t tiles = (U.rows + 16 * Many<D>::MT * kCW - 1) / (16 * Many<D>::MT * kCW);
+  const int64_t tiles = (U.rows + 16 * Many<D>::MT * kWarps - 1) / (16 * Many<D>::MT * kWarps);
   if (U.rows > 32 && U.B * A.H * tiles >= num_sms() && tiles < 65536 && U.B * A.H < (int64_t(1) << 31))
     return many_launch<D>(A, ck, cv, U);
   if (U.rows <= 8) return many ? few_launch<D, 8, 1>(A, ck, cv, U) : few_launch<D, 8, 4>(A, ck, cv, U);
