@@ -18,12 +18,63 @@ std::vector<at::Tensor> paged_attention(at::Tensor, at::Tensor, at::Tensor, at::
 long long launches();
 }  // namespace pd
 
+// Gradient through qk_norm_rope. In C++ so that a small call is not bound by
+// the interpreter: a backward in Python takes the interpreter's lock on the
+// autograd thread.
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+namespace {
+using OptTensor = c10::optional<at::Tensor>;
+
+OptTensor fp32(const OptTensor& w) { return w.has_value() ? OptTensor(w->to(at::kFloat).contiguous()) : w; }
+
+struct QkNormRope : public torch::autograd::Function<QkNormRope> {
+  static variable_list forward(AutogradContext* ctx, at::Tensor q, OptTensor k, OptTensor wq, OptTensor wk,
+                               at::Tensor table, OptTensor pos, double eps, bool interleaved, at::Tensor err) {
+    const OptTensor fq = fp32(wq), fk = fp32(wk);
+    auto y = pd::kv::qk_norm_rope(q, k, fq, fk, table, pos, eps, interleaved, err, c10::nullopt, c10::nullopt);
+    auto or_none = [](const OptTensor& t) { return t.has_value() ? *t : at::Tensor(); };
+    ctx->save_for_backward({q, or_none(k), or_none(fq), or_none(fk), table, or_none(pos), err});
+    ctx->saved_data["eps"] = eps;
+    ctx->saved_data["interleaved"] = interleaved;
+    ctx->saved_data["wq"] = wq.has_value() ? int64_t(wq->scalar_type()) : int64_t(-1);
+    ctx->saved_data["wk"] = wk.has_value() ? int64_t(wk->scalar_type()) : int64_t(-1);
+    return y;
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list dy) {
+    const auto v = ctx->get_saved_variables();
+    auto opt = [&](int i) { return v[i].defined() ? OptTensor(v[i]) : OptTensor(); };
+    const OptTensor k = opt(1);
+    auto grad = [&](size_t i, const at::Tensor& x) {
+      return i < dy.size() && dy[i].defined() ? dy[i].to(x.scalar_type()).contiguous()
+                                              : at::zeros(x.sizes(), x.options());
+    };
+    auto g = pd::kv::qk_norm_rope(v[0], k, opt(2), opt(3), v[4], opt(5), ctx->saved_data["eps"].toDouble(),
+                                  ctx->saved_data["interleaved"].toBool(), v[6], grad(0, v[0]),
+                                  k.has_value() ? OptTensor(grad(1, *k)) : OptTensor());
+    auto weight = [&](const char* name, size_t i) {
+      const int64_t t = ctx->saved_data[name].toInt();
+      return t < 0 || i >= g.size() ? at::Tensor() : g[i].to(at::ScalarType(t));
+    };
+    const bool two = k.has_value();
+    return {g[0], two ? g[1] : at::Tensor(), weight("wq", two ? 2 : 1), two ? weight("wk", 3) : at::Tensor(),
+            at::Tensor(), at::Tensor(), at::Tensor(), at::Tensor(), at::Tensor()};
+  }
+};
+
+std::vector<at::Tensor> qk_norm_rope_grad(at::Tensor q, OptTensor k, OptTensor wq, OptTensor wk, at::Tensor table,
+                                          OptTensor pos, double eps, bool interleaved, at::Tensor err) {
+  return QkNormRope::apply(q, k, wq, wk, table, pos, eps, interleaved, err);
+}
+}  // namespace
+
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.doc() = "primus_dlrm_b200 sm_100a kernels: query/key norm with rotation, paged 8-bit key/value cache, attention";
   m.def("qk_norm_rope", &pd::kv::qk_norm_rope, py::arg("q"), py::arg("k"), py::arg("w_q"), py::arg("w_k"),
         py::arg("table"), py::arg("positions"), py::arg("eps"), py::arg("interleaved"), py::arg("err"),
         py::arg("dy_q") = py::none(), py::arg("dy_k") = py::none(),
         "[y_q, y_k]; with the outputs' gradients [dq, dk, dw_q, dw_k] (without k: its entries are left out)");
+  m.def("qk_norm_rope_grad", &qk_norm_rope_grad, "[y_q, y_k] with their gradients in q, k and the weights");
   m.def("append", &pd::kv::kv_append, "new tokens' keys and values into the pages of a cache");
   m.def("read", &pd::kv::kv_read, "tokens [first, first + n) of each sequence as bf16 [B, n, H, d]");
   m.def("paged_attention", &pd::kv::paged_attention, "attention of the last tokens over a cache -> [o(, lse)]");

@@ -35,10 +35,9 @@ __device__ __forceinline__ int scale_exp(float amax) {
 __device__ __forceinline__ float pow2(int e) { return __int_as_float((e + 127) << 23); }   // -126 <= e <= 127
 __device__ __forceinline__ int exp_of(float pow2_scale) { return (__float_as_int(pow2_scale) >> 23) - 127; }
 
+// finite values or NaN (an infinity would come out as 448)
 __device__ __forceinline__ uint32_t encode2(float a, float b) {
-  // satfinite would turn an infinity into 448
-  const float na = fabsf(a) == INFINITY ? NAN : a, nb = fabsf(b) == INFINITY ? NAN : b;
-  return __nv_cvt_float2_to_fp8x2(make_float2(na, nb), __NV_SATFINITE, __NV_E4M3);
+  return __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3);
 }
 __device__ __forceinline__ uint2 encode8(const float* f, float inv) {
   uint2 u;
@@ -55,6 +54,11 @@ __device__ __forceinline__ void decode8(uint2 u, float* f) {
     f[2 * i] = t.x;
     f[2 * i + 1] = t.y;
   }
+}
+
+__device__ __forceinline__ void load_w(const float* p, float* f) {
+  const float4 a = __ldg(reinterpret_cast<const float4*>(p)), b = __ldg(reinterpret_cast<const float4*>(p) + 1);
+  f[0] = a.x; f[1] = a.y; f[2] = a.z; f[3] = a.w; f[4] = b.x; f[5] = b.y; f[6] = b.z; f[7] = b.w;
 }
 
 struct AppendArgs {
@@ -114,9 +118,10 @@ __global__ void __launch_bounds__(kAppendThreads) append_kernel(const AppendArgs
   pair_offsets<8>(lane, D, A.rope ? D : 0, A.interleaved, off0, off1, turned);
 
   float a[PASSES][8], c[PASSES][8];
-  float amax = 0.f;
+  float amax = 0.f;                                      // infinities count, NaN does not
 #pragma unroll
   for (int ps = 0; ps < PASSES; ++ps) {
+    if (ps * R >= A.P) break;
     const int r = ps * R + row0;
     const bool live = r >= lo && r < hi;
     const int64_t i = tok0 + p0 + r - len;             // token among the new ones
@@ -135,6 +140,11 @@ __global__ void __launch_bounds__(kAppendThreads) append_kernel(const AppendArgs
         }
       }
     }
+  }
+#pragma unroll
+  for (int ps = 0; ps < PASSES; ++ps) {
+    if (ps * R >= A.P) break;
+    const int r = ps * R + row0;
     if (part == 0 && A.norm) {
       float ss = 0.f;
 #pragma unroll
@@ -142,11 +152,21 @@ __global__ void __launch_bounds__(kAppendThreads) append_kernel(const AppendArgs
       const float rs = __frsqrt_rn(group_sum<L>(ss) * (1.f / D) + A.eps);
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        a[ps][e] = a[ps][e] * rs * (A.kw ? __ldg(A.kw + off0 + e) : 1.f);
-        c[ps][e] = c[ps][e] * rs * (A.kw ? __ldg(A.kw + off1 + e) : 1.f);
+        a[ps][e] *= rs;
+        c[ps][e] *= rs;
+      }
+      if (A.kw) {
+        float w0[8], w1[8];
+        load_w(A.kw + off0, w0);
+        load_w(A.kw + off1, w1);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          a[ps][e] *= w0[e];
+          c[ps][e] *= w1[e];
+        }
       }
     }
-    if (part == 0 && A.rope && live) {
+    if (part == 0 && A.rope && r >= lo && r < hi) {
       if (p0 + r < A.n_pos) {
         float cs[8], sn[8];
         load_angles<8>(A.rope + (p0 + r) * D, lane, D, A.interleaved, off0, off1, cs, sn);
@@ -158,11 +178,7 @@ __global__ void __launch_bounds__(kAppendThreads) append_kernel(const AppendArgs
       }
     }
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const float u = fabsf(a[ps][e]), v = fabsf(c[ps][e]);
-      if (u < INFINITY) amax = fmaxf(amax, u);          // false for NaN too
-      if (v < INFINITY) amax = fmaxf(amax, v);
-    }
+    for (int e = 0; e < 8; ++e) amax = fmaxf(amax, fmaxf(fabsf(a[ps][e]), fabsf(c[ps][e])));
   }
   __shared__ float s_max[kAppendThreads / 32];
   amax = warp_max(amax);
@@ -171,6 +187,26 @@ __global__ void __launch_bounds__(kAppendThreads) append_kernel(const AppendArgs
   __syncthreads();                                       // also: everyone has read the old scale
 #pragma unroll
   for (int w = 0; w < kAppendThreads / 32; ++w) amax = fmaxf(amax, s_max[w]);
+  if (amax == INFINITY) {
+    // seldom: infinities become NaN and leave the maximum
+    amax = 0.f;
+#pragma unroll
+    for (int ps = 0; ps < PASSES; ++ps) {
+      if (ps * R >= A.P) break;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        if (fabsf(a[ps][e]) == INFINITY) a[ps][e] = NAN;
+        if (fabsf(c[ps][e]) == INFINITY) c[ps][e] = NAN;
+        amax = fmaxf(amax, fmaxf(fabsf(a[ps][e]), fabsf(c[ps][e])));
+      }
+    }
+    __syncthreads();
+    amax = warp_max(amax);
+    if ((threadIdx.x & 31) == 0) s_max[threadIdx.x >> 5] = amax;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < kAppendThreads / 32; ++w) amax = fmaxf(amax, s_max[w]);
+  }
   int e = scale_exp(amax);
   if (lo > 0) {
     // a scale from elsewhere that is no power of two counts as the next one
@@ -192,6 +228,7 @@ __global__ void __launch_bounds__(kAppendThreads) append_kernel(const AppendArgs
   const float inv = pow2(-e);
 #pragma unroll
   for (int ps = 0; ps < PASSES; ++ps) {
+    if (ps * R >= A.P) break;
     const int r = ps * R + row0;
     if (r >= lo && r < hi) {
       *reinterpret_cast<uint2*>(code + r * D + off0) = encode8(a[ps], inv);
@@ -209,36 +246,59 @@ struct ReadArgs {
   const int* lens;
   const int* first;             // [B] or null (0)
   __nv_bfloat16* out[2];        // [B, n, H, d]
-  int n, H, P, d, max_pages, n_pages;
-  int64_t vecs;                 // 8-element vectors of one output
+  int n, H, P, logP, max_pages, n_pages;
+  int chunks;                   // blocks of a sequence
   int* err;
 };
 
+// One block: up to 32 tokens of one sequence, all heads. A thread takes 16
+// codes of one head's row at a time; the pages of the block's tokens are looked
+// up once. Bound by the writes (2 bytes a value, 1 read).
+template <int D>
 __global__ void __launch_bounds__(256) read_kernel(const ReadArgs A) {
-  const int64_t i = int64_t(blockIdx.x) * 256 + threadIdx.x;
-  if (i >= A.vecs) return;
-  const int part = blockIdx.y, dv = A.d / 8;
-  const int c = int(i % dv);
-  const int64_t t = i / dv;
-  const int h = int(t % A.H);
-  const int64_t bt = t / A.H;
-  const int b = int(bt / A.n);
-  const int64_t pos = bt % A.n + (A.first ? A.first[b] : 0);
-  float f[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-  if (pos >= 0 && pos < A.lens[b]) {
-    const int64_t pi = pos / A.P;
-    const int page = pi < A.max_pages ? A.table[b * A.table_stride + pi] : -1;
-    if (page >= 0 && page < A.n_pages) {
-      const int64_t block = int64_t(page) * A.H + h;
-      decode8(*reinterpret_cast<const uint2*>(A.code[part] + (block * A.P + pos % A.P) * A.d + c * 8), f);
-      const float s = A.scale[part][block];
-#pragma unroll
-      for (int e = 0; e < 8; ++e) f[e] *= s;
-    } else {
-      set_error(A.err, kIdOutOfRange);
+  constexpr int TOK = 32, L = D / 16;                // threads of a row
+  __shared__ int s_row[TOK];                          // page * H * P + row in the page, or -1
+  __shared__ int s_page[TOK];
+  const int part = blockIdx.y, b = blockIdx.x / A.chunks, t0 = (blockIdx.x - b * A.chunks) * TOK;
+  const int tokens = min(TOK, A.n - t0);
+  if (threadIdx.x < tokens) {
+    const int64_t pos = int64_t(A.first ? A.first[b] : 0) + t0 + threadIdx.x;
+    int page = -1;
+    if (pos >= 0 && pos < A.lens[b]) {
+      const int64_t pi = pos >> A.logP;
+      page = pi < A.max_pages ? A.table[b * A.table_stride + pi] : -1;
+      if (page < 0 || page >= A.n_pages) {
+        page = -1;
+        set_error(A.err, kIdOutOfRange);
+      }
     }
+    s_page[threadIdx.x] = page;
+    s_row[threadIdx.x] = int(pos & (A.P - 1));
   }
-  store_v<8>(A.out[part] + i * 8, f);
+  __syncthreads();
+  const uint8_t* code = part ? A.code[1] : A.code[0];
+  const float* scale = part ? A.scale[1] : A.scale[0];
+  __nv_bfloat16* out = (part ? A.out[1] : A.out[0]) + (int64_t(b) * A.n + t0) * A.H * D;
+  const int per_token = A.H * L, all = tokens * per_token;
+#pragma unroll 2
+  for (int i = threadIdx.x; i < all; i += 256) {
+    const int t = i / per_token, j = i - t * per_token, h = j / L, c = j % L;
+    const int page = s_page[t];
+    float f[16];
+#pragma unroll
+    for (int e = 0; e < 16; ++e) f[e] = 0.f;
+    if (page >= 0) {
+      const int block = page * A.H + h;
+      const uint4 u = *reinterpret_cast<const uint4*>(code + (int64_t(block) * A.P + s_row[t]) * D + c * 16);
+      const float s = scale[block];
+      decode8(make_uint2(u.x, u.y), f);
+      decode8(make_uint2(u.z, u.w), f + 8);
+#pragma unroll
+      for (int e = 0; e < 16; ++e) f[e] *= s;
+    }
+    store_v<8>(out + int64_t(i) * 16, f);
+    store_v<8>(out + int64_t(i) * 16 + 8, f + 8);
+  }
 }
 
 // ---------------------------------------------------------------- entry points
@@ -327,7 +387,8 @@ void kv_append(at::Tensor ck, at::Tensor cv, at::Tensor ks, at::Tensor vs, at::T
   if (k_weight.has_value()) {
     PD_CHECK(A.norm, "k_weight needs norm_eps");
     PD_CHECK(k_weight->device() == ck.device() && k_weight->scalar_type() == at::kFloat && k_weight->dim() == 1 &&
-             k_weight->is_contiguous() && k_weight->size(0) == C.d, "k_weight must be contiguous fp32 [d]");
+             k_weight->is_contiguous() && k_weight->size(0) == C.d && reinterpret_cast<uintptr_t>(k_weight->data_ptr()) % 16 == 0,
+             "k_weight must be contiguous fp32 [d] on a 16-byte boundary");
     A.kw = k_weight->data_ptr<float>();
   }
   if (rope.has_value()) {
@@ -371,13 +432,16 @@ std::vector<at::Tensor> kv_read(at::Tensor ck, at::Tensor cv, at::Tensor ks, at:
   A.max_pages = int(table.size(1));
   A.lens = lens.data_ptr<int>();
   A.first = first.has_value() ? first->data_ptr<int>() : nullptr;
-  A.n = int(n); A.H = C.H; A.P = C.P; A.d = C.d; A.n_pages = C.n_pages;
-  A.vecs = B * n * C.H * (C.d / 8);
+  A.n = int(n); A.H = C.H; A.P = C.P; A.n_pages = C.n_pages;
+  A.logP = C.P == 16 ? 4 : C.P == 32 ? 5 : 6;
   A.err = err.data_ptr<int>();
-  const int64_t blocks = (A.vecs + 255) / 256;
-  PD_CHECK(blocks < (int64_t(1) << 31), "too many values for one call");
-  if (blocks > 0) {
-    read_kernel<<<dim3(unsigned(blocks), 2), 256, 0, stream()>>>(A);
+  A.chunks = int((n + 31) / 32);
+  PD_CHECK(B * A.chunks < (int64_t(1) << 31), "too many tokens for one call");
+  if (B > 0 && n > 0) {
+    const dim3 grid(unsigned(B * A.chunks), 2);
+    if (C.d == 32) read_kernel<32><<<grid, 256, 0, stream()>>>(A);
+    else if (C.d == 64) read_kernel<64><<<grid, 256, 0, stream()>>>(A);
+    else read_kernel<128><<<grid, 256, 0, stream()>>>(A);
     PD_CHECK_LAUNCH();
   }
   return out;

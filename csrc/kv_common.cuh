@@ -26,21 +26,41 @@ template <> __device__ __forceinline__ float from_f(float v) { return v; }
 template <> __device__ __forceinline__ __half from_f(float v) { return __float2half_rn(v); }
 template <> __device__ __forceinline__ __nv_bfloat16 from_f(float v) { return __float2bfloat16_rn(v); }
 
-// V consecutive elements; V = 8 moves 16 bytes an access and needs 16-byte
-// aligned addresses, V = 1 takes any element.
+// V consecutive elements as they lie in memory; V = 8 moves 16 bytes an access
+// and needs 16-byte aligned addresses, V = 1 takes any element.
+template <int V, typename T>
+struct Raw {
+  static constexpr int N = V == 1 ? 1 : int(sizeof(T)) / 2;      // uint4s of 8 elements
+  T one;
+  uint4 v[N];
+  __device__ __forceinline__ void load(const T* p) {
+    if constexpr (V == 1) {
+      one = *p;
+    } else {
+#pragma unroll
+      for (int i = 0; i < N; ++i) v[i] = *(reinterpret_cast<const uint4*>(p) + i);
+    }
+  }
+  __device__ __forceinline__ void zero() {
+    one = T(0.f);
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = make_uint4(0, 0, 0, 0);
+  }
+  __device__ __forceinline__ void floats(float* f) const {
+    if constexpr (V == 1) {
+      f[0] = to_f(one);
+    } else {
+      const T* e = reinterpret_cast<const T*>(v);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) f[i] = to_f(e[i]);
+    }
+  }
+};
 template <int V, typename T>
 __device__ __forceinline__ void load_v(const T* p, float* f) {
-  if constexpr (V == 1) {
-    f[0] = to_f(*p);
-  } else if constexpr (sizeof(T) == 4) {
-    const float4 a = *reinterpret_cast<const float4*>(p), b = *(reinterpret_cast<const float4*>(p) + 1);
-    f[0] = a.x; f[1] = a.y; f[2] = a.z; f[3] = a.w; f[4] = b.x; f[5] = b.y; f[6] = b.z; f[7] = b.w;
-  } else {
-    const uint4 u = *reinterpret_cast<const uint4*>(p);
-    const T* e = reinterpret_cast<const T*>(&u);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) f[i] = to_f(e[i]);
-  }
+  Raw<V, T> r;
+  r.load(p);
+  r.floats(f);
 }
 template <int V, typename T>
 __device__ __forceinline__ void store_v(T* p, const float* f) {

@@ -15,11 +15,15 @@
 // of a token are neighbouring groups: they share the angles in L1, and the
 // loads of a warp are contiguous where the heads are. Rows that no 16-byte
 // access fits (odd strides, dims that are no multiple of 16) go through the
-// same code with single elements and a warp a row.
+// same code with single elements and a warp a row. A block walks over rows
+// (weights stay in registers) and loads its next row before it works on the
+// one it has.
 //
 // dw: each lane keeps its 16 columns' sums over all rows of its block, blocks
 // write theirs to a workspace and a second launch adds them in a fixed order,
 // so that the same inputs give the same bits.
+#include <c10/cuda/CUDAGuard.h>
+
 #include "kv_common.cuh"
 
 namespace pd {
@@ -63,7 +67,7 @@ __device__ __forceinline__ uint32_t fast_div(uint32_t n, uint32_t mul, uint32_t 
 }
 
 template <typename T, int V, int L, int NP, bool BWD>
-__global__ void __launch_bounds__(kThreads) qk_norm_rope_kernel(const Args A) {
+__global__ void __launch_bounds__(kThreads, BWD ? 2 : 3) qk_norm_rope_kernel(const __grid_constant__ Args A) {
   constexpr int G = kThreads / L;                       // rows of a block at a time
   const bool second = int(blockIdx.x) >= A.blocks0;
   const Part& P = A.p[second ? 1 : 0];
@@ -92,48 +96,77 @@ __global__ void __launch_bounds__(kThreads) qk_norm_rope_kernel(const Args A) {
       acc0[i][e] = acc1[i][e] = 0.f;
     }
   }
+  // a row on its way: its elements, its place in the output (or -1) and its angles' (or -1: a position outside)
+  Raw<V, T> xa[NP], xb[NP], ya[NP], yb[NP];
+  int row_of = -1, at_of = -1;
+  auto fetch = [&](int it) {
+    const uint32_t row = uint32_t(it * blocks + block) * G + threadIdx.x / L;
+    row_of = row < uint32_t(P.rows) ? int(row) : -1;
+    at_of = -1;
+    if (row_of < 0) {
+#pragma unroll
+      for (int i = 0; i < NP; ++i) {
+        xa[i].zero();
+        xb[i].zero();
+        if (BWD) {
+          ya[i].zero();
+          yb[i].zero();
+        }
+      }
+      return;
+    }
+    const uint32_t tok = fast_div(row, P.mul_h, P.sh_h), h = row - tok * P.H;
+    const uint32_t bb = fast_div(tok, P.mul_t, P.sh_t), t = tok - bb * P.T;
+    const T* xr = x + int64_t(bb) * P.bs + int64_t(t) * P.ts + int64_t(h) * P.hs;
+    const T* dr = dy + int64_t(row) * d;
+#pragma unroll
+    for (int i = 0; i < NP; ++i) {
+      if (on[i]) {
+        xa[i].load(xr + off0[i]);
+        xb[i].load(xr + off1[i]);
+        if (BWD) {
+          ya[i].load(dr + off0[i]);
+          yb[i].load(dr + off1[i]);
+        }
+      } else {
+        xa[i].zero();
+        xb[i].zero();
+        if (BWD) {
+          ya[i].zero();
+          yb[i].zero();
+        }
+      }
+    }
+    const int64_t pi = int64_t(bb) * A.pos_bs + t + P.t_off;
+    const int64_t pos = A.pos == nullptr ? int64_t(t) + P.t_off
+                        : A.pos64        ? __ldg(static_cast<const long long*>(A.pos) + pi)
+                                         : int64_t(__ldg(static_cast<const int*>(A.pos) + pi));
+    if (pos >= 0 && pos < A.n_pos) at_of = int(pos);
+    else set_error(A.err, kIdOutOfRange);
+  };
   // every lane of a warp takes part in the group sums of each turn
   const int turns = (P.rows + blocks * G - 1) / (blocks * G);
+  fetch(0);
   for (int it = 0; it < turns; ++it) {
-    const uint32_t row = uint32_t(it * blocks + block) * G + threadIdx.x / L;
-    const bool live = row < uint32_t(P.rows);
+    const int row = row_of;
+    const bool live = row >= 0, good = at_of >= 0;
+    const float* at = A.table + int64_t(good ? at_of : 0) * A.rot;
     float a[NP][V], b[NP][V], ga[NP][V], gb[NP][V];
     float ss = 0.f;
-    bool good = live;
-    int64_t out = 0;
-    const float* at = A.table;
 #pragma unroll
-    for (int i = 0; i < NP; ++i)
+    for (int i = 0; i < NP; ++i) {
+      xa[i].floats(a[i]);
+      xb[i].floats(b[i]);
+      if (BWD) {
+        ya[i].floats(ga[i]);
+        yb[i].floats(gb[i]);
+      }
 #pragma unroll
-      for (int e = 0; e < V; ++e) a[i][e] = b[i][e] = ga[i][e] = gb[i][e] = 0.f;
-    if (live) {
-      const uint32_t tok = fast_div(row, P.mul_h, P.sh_h), h = row - tok * P.H;
-      const uint32_t bb = fast_div(tok, P.mul_t, P.sh_t), t = tok - bb * P.T;
-      const T* xr = x + int64_t(bb) * P.bs + int64_t(t) * P.ts + int64_t(h) * P.hs;
-      out = int64_t(row) * d;
-#pragma unroll
-      for (int i = 0; i < NP; ++i)
-        if (on[i]) {
-          load_v<V>(xr + off0[i], a[i]);
-          load_v<V>(xr + off1[i], b[i]);
-          if (BWD) {
-            load_v<V>(dy + out + off0[i], ga[i]);
-            load_v<V>(dy + out + off1[i], gb[i]);
-          }
-        }
-      const int64_t pi = int64_t(bb) * A.pos_bs + t + P.t_off;
-      const int64_t pos = A.pos == nullptr ? int64_t(t) + P.t_off
-                          : A.pos64        ? __ldg(static_cast<const long long*>(A.pos) + pi)
-                                           : int64_t(__ldg(static_cast<const int*>(A.pos) + pi));
-      good = pos >= 0 && pos < A.n_pos;
-      if (good) at += pos * A.rot;
-      else set_error(A.err, kIdOutOfRange);
-#pragma unroll
-      for (int i = 0; i < NP; ++i)
-#pragma unroll
-        for (int e = 0; e < V; ++e) ss += a[i][e] * a[i][e] + b[i][e] * b[i][e];
+      for (int e = 0; e < V; ++e) ss += a[i][e] * a[i][e] + b[i][e] * b[i][e];
     }
+    if (it + 1 < turns) fetch(it + 1);
     const float r = __frsqrt_rn(group_sum<L>(ss) * inv_d + A.eps);
+    const int64_t out = int64_t(row) * d;
     if (!BWD) {
       if (live) {
 #pragma unroll
@@ -144,7 +177,7 @@ __global__ void __launch_bounds__(kThreads) qk_norm_rope_kernel(const Args A) {
               a[i][e] = good ? a[i][e] * r * w0[i][e] : 0.f;
               b[i][e] = good ? b[i][e] * r * w1[i][e] : 0.f;
             }
-            if (turned[i]) {
+            if (turned[i] && good) {
               float c[V], s[V];
               load_angles<V>(at, lane + i * L, A.rot, A.interleaved, off0[i], off1[i], c, s);
               turn<V>(a[i], b[i], c, s, A.interleaved, 1.f);
@@ -228,8 +261,10 @@ __global__ void __launch_bounds__(1024) dw_sum_kernel(const float* part, int blo
   const int c = blockIdx.x * 32 + threadIdx.x;
   const int lo = blockIdx.y == 0 ? 0 : blocks0, hi = blockIdx.y == 0 ? blocks0 : blocks;
   float s = 0.f;
-  if (c < d)
+  if (c < d) {
+#pragma unroll 8
     for (int r = lo + threadIdx.y; r < hi; r += 32) s += part[int64_t(r) * d + c];
+  }
   t[threadIdx.y][threadIdx.x] = s;
   __syncthreads();
   s = warp_sum(t[threadIdx.x][threadIdx.y]);
@@ -326,6 +361,7 @@ std::vector<at::Tensor> qk_norm_rope(at::Tensor q, c10::optional<at::Tensor> k, 
     A.pos64 = st == at::kLong;
     A.pos_bs = pos->dim() == 2 ? t_all : 0;
   }
+  const c10::cuda::CUDAGuard guard(q.device());
   fill(A.p[0], q, wq, t_all, "q");
   if (n_parts == 2) fill(A.p[1], *k, wk, t_all, "k");
 
@@ -349,17 +385,14 @@ std::vector<at::Tensor> qk_norm_rope(at::Tensor q, c10::optional<at::Tensor> k, 
   int lanes = 32;
   if (vec) for (lanes = 1; lanes * 16 < A.d; lanes *= 2) {}
   const int64_t G = kThreads / lanes;
-  // forward: a block a batch of rows. backward: a few rows a lane at least, so that the
-  // workspace of column sums stays small beside the rows (8 blocks an SM at most)
+  // blocks that the device holds at once, shared out by rows
   int64_t nb[2] = {0, 0};
   const int64_t rows_all = int64_t(A.p[0].rows) + (n_parts == 2 ? A.p[1].rows : 0);
-  for (int i = 0; i < n_parts; ++i) {
-    nb[i] = (A.p[i].rows + G - 1) / G;
-    if (bwd && nb[i] > 0) {
-      const int64_t most = std::max<int64_t>(1, int64_t(num_sms()) * 8 * A.p[i].rows / std::max<int64_t>(1, rows_all));
-      nb[i] = std::min<int64_t>(nb[i], most);
-    }
-  }
+  const int64_t slots = int64_t(num_sms()) * (bwd ? 2 : 3);
+  for (int i = 0; i < n_parts; ++i)
+    if (A.p[i].rows > 0)
+      nb[i] = std::min<int64_t>((A.p[i].rows + G - 1) / G,
+                                std::max<int64_t>(1, (slots * A.p[i].rows + rows_all / 2) / rows_all));
   const int64_t grid = nb[0] + nb[1];
   A.blocks0 = int(nb[0]);
   at::Tensor part;

@@ -6,8 +6,8 @@ one launch, forward and backward.  Rotated queries and keys depend on their
 positions only through differences, so a model that uses it attends over
 histories that grow, and over a key/value cache, without learned positions.
 
-Native path: ``_kv.qk_norm_rope`` (bf16, fp16 or fp32 in and out, 32-bit
-arithmetic).  Eager path: the same formulas in PyTorch.
+Native path: ``_kv.qk_norm_rope`` / ``_kv.qk_norm_rope_grad`` (bf16, fp16 or
+fp32 in and out, 32-bit arithmetic).  Eager path: the same formulas in PyTorch.
 """
 from __future__ import annotations
 
@@ -82,31 +82,6 @@ def _w32(w):
     return w if w is None or (w.dtype == torch.float32 and w.is_contiguous()) else w.float().contiguous()
 
 
-class _QKNormRope(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, q, k, wq, wk, table, positions, eps, interleaved):
-        ctx.wdt = [None if w is None else w.dtype for w in (wq, wk)]
-        wq, wk = _w32(wq), _w32(wk)
-        out = _ext.kv().qk_norm_rope(q, k, wq, wk, table, positions, eps, interleaved, _err_word(q.device))
-        ctx.save_for_backward(q, k, wq, wk, table, positions)
-        ctx.eps, ctx.interleaved = eps, interleaved
-        return out[0], out[1] if k is not None else None
-
-    @staticmethod
-    def backward(ctx, dyq, dyk):
-        q, k, wq, wk, table, positions = ctx.saved_tensors
-
-        def grad(dy, x):
-            return torch.zeros(x.shape, dtype=x.dtype, device=x.device) if dy is None else dy.to(x.dtype).contiguous()
-
-        got = _ext.kv().qk_norm_rope(q, k, wq, wk, table, positions, ctx.eps, ctx.interleaved, _err_word(q.device),
-                                     grad(dyq, q), grad(dyk, k) if k is not None else None)
-        dq, dk = got[0], got[1] if k is not None else None
-        dw = [got[2 if k is not None else 1], got[3] if k is not None else None]
-        dw = [None if t is None or w is None else w.to(t) for t, w in zip(ctx.wdt, dw)]
-        return dq, dk, dw[0], dw[1], None, None, None, None
-
-
 def qk_norm_rope(q: torch.Tensor, k: torch.Tensor | None, q_weight: torch.Tensor | None,
                  k_weight: torch.Tensor | None, table: torch.Tensor, positions: torch.Tensor | None = None, *,
                  eps: float = 1e-6, interleaved: bool = False) -> tuple[torch.Tensor, torch.Tensor | None]:
@@ -136,7 +111,9 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor | None, q_weight: torch.Tensor
     if positions is not None and not positions.is_contiguous():
         positions = positions.contiguous()
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, q_weight, k_weight)):
-        return _QKNormRope.apply(q, k, q_weight, k_weight, table, positions, eps, interleaved)
-    out = _ext.kv().qk_norm_rope(q, k, _w32(q_weight), _w32(k_weight), table, positions, eps, interleaved,
-                                 _err_word(q.device))
+        out = _ext.kv().qk_norm_rope_grad(q, k, q_weight, k_weight, table, positions, eps, interleaved,
+                                          _err_word(q.device))
+    else:
+        out = _ext.kv().qk_norm_rope(q, k, _w32(q_weight), _w32(k_weight), table, positions, eps, interleaved,
+                                     _err_word(q.device))
     return out[0], out[1] if k is not None else None
