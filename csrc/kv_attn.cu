@@ -17,6 +17,8 @@
 #include <c10/cuda/CUDAGuard.h>
 #include <cuda_fp8.h>
 
+#include <cmath>
+
 #include "kv_common.cuh"
 
 namespace pd {
@@ -1425,13 +1427,15 @@ static void attn_dispatch(AttnArgs& A, const at::Tensor& ck, const at::Tensor& c
 // (o, lse): lse is an undefined tensor unless asked for.
 std::vector<at::Tensor> paged_attention(at::Tensor q, at::Tensor ck, at::Tensor cv, at::Tensor ks, at::Tensor vs,
                                         at::Tensor err, at::Tensor table, at::Tensor lens,
-                                        c10::optional<at::Tensor> cu, int64_t max_q, int64_t max_len, double scale,
-                                        bool causal, bool want_lse) {
+                                        c10::optional<at::Tensor> cu, c10::optional<int64_t> max_q,
+                                        c10::optional<int64_t> max_len, c10::optional<double> scale, bool causal,
+                                        bool want_lse) {
   const CacheDims C = check_cache(ck, cv, ks, vs, err);
   check_table(table, ck);
   const int64_t B = table.size(0);
   check_ints(lens, ck, B, "kv_lens");
   const int qd = cu.has_value() ? 3 : 4;
+  if (q.dim() > 0 && q.stride(-1) != 1) q = q.contiguous();
   PD_CHECK(q.device() == ck.device() && (q.scalar_type() == at::kBFloat16 || q.scalar_type() == at::kHalf),
            "q must be bf16 or fp16 on the cache's device");
   PD_CHECK(q.dim() == qd && q.size(qd - 1) == C.d && (q.stride(qd - 1) == 1 || q.numel() == 0),
@@ -1460,7 +1464,7 @@ std::vector<at::Tensor> paged_attention(at::Tensor q, at::Tensor ck, at::Tensor 
   A.max_pages = int(table.size(1));
   A.causal = causal;
   A.bf16 = q.scalar_type() == at::kBFloat16;
-  A.scale_log2 = float(scale * 1.4426950408889634);
+  A.scale_log2 = float(scale.value_or(1. / std::sqrt(double(C.d))) * 1.4426950408889634);
   A.err = err.data_ptr<int>();
   at::Tensor o = at::empty(q.sizes(), q.options());
   at::Tensor lse;
@@ -1469,11 +1473,11 @@ std::vector<at::Tensor> paged_attention(at::Tensor q, at::Tensor ck, at::Tensor 
     lse = at::empty(q.sizes().slice(0, qd - 1), q.options().dtype(at::kFloat));
     A.lse = lse.data_ptr<float>();
   }
-  const int64_t most = qd == 4 ? q.size(1) : std::min<int64_t>(std::max<int64_t>(max_q, 0), q.size(0));
+  const int64_t most = qd == 4 ? q.size(1) : std::min<int64_t>(std::max<int64_t>(max_q.value_or(q.size(0)), 0), q.size(0));
   PD_CHECK((qd == 3 ? q.size(0) : B * q.size(1)) * A.G < (int64_t(1) << 31) - 128 && B < (int64_t(1) << 31),
            "too many queries");
   if (B > 0 && most > 0 && q.numel() > 0) {
-    const Bounds U{B, most * A.G, std::min<int64_t>(table.size(1) * C.P, std::max<int64_t>(max_len, 0))};
+    const Bounds U{B, most * A.G, std::min<int64_t>(table.size(1) * C.P, std::max<int64_t>(max_len.value_or(INT64_MAX), 0))};
     if (C.d == 32) attn_dispatch<32>(A, ck, cv, U);
     else if (C.d == 64) attn_dispatch<64>(A, ck, cv, U);
     else attn_dispatch<128>(A, ck, cv, U);

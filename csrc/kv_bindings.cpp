@@ -1,19 +1,22 @@
 // Python bindings of the rotary and key/value-cache kernels (module `_kv`).
 #include <torch/extension.h>
 
+#include <tuple>
+#include <vector>
+
 namespace pd {
 namespace kv {
 std::vector<at::Tensor> qk_norm_rope(at::Tensor, c10::optional<at::Tensor>, c10::optional<at::Tensor>,
                                      c10::optional<at::Tensor>, at::Tensor, c10::optional<at::Tensor>, double, bool,
                                      at::Tensor, c10::optional<at::Tensor>, c10::optional<at::Tensor>);
 void kv_append(at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor,
-               at::Tensor, c10::optional<at::Tensor>, int64_t, c10::optional<at::Tensor>, c10::optional<double>,
+               at::Tensor, c10::optional<at::Tensor>, c10::optional<int64_t>, c10::optional<at::Tensor>, c10::optional<double>,
                c10::optional<at::Tensor>, bool);
 std::vector<at::Tensor> kv_read(at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor,
-                                c10::optional<at::Tensor>, int64_t);
+                                c10::optional<at::Tensor>, c10::optional<int64_t>);
 std::vector<at::Tensor> paged_attention(at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor,
-                                        at::Tensor, at::Tensor, c10::optional<at::Tensor>, int64_t, int64_t, double,
-                                        bool, bool);
+                                        at::Tensor, at::Tensor, c10::optional<at::Tensor>, c10::optional<int64_t>,
+                                        c10::optional<int64_t>, c10::optional<double>, bool, bool);
 }  // namespace kv
 long long launches();
 }  // namespace pd
@@ -26,7 +29,10 @@ using torch::autograd::variable_list;
 namespace {
 using OptTensor = c10::optional<at::Tensor>;
 
-OptTensor fp32(const OptTensor& w) { return w.has_value() ? OptTensor(w->to(at::kFloat).contiguous()) : w; }
+OptTensor fp32(const OptTensor& w) {
+  return !w.has_value() || (w->scalar_type() == at::kFloat && w->is_contiguous()) ? w
+                                                                                  : OptTensor(w->to(at::kFloat).contiguous());
+}
 
 struct QkNormRope : public torch::autograd::Function<QkNormRope> {
   static variable_list forward(AutogradContext* ctx, at::Tensor q, OptTensor k, OptTensor wq, OptTensor wk,
@@ -62,19 +68,39 @@ struct QkNormRope : public torch::autograd::Function<QkNormRope> {
   }
 };
 
-std::vector<at::Tensor> qk_norm_rope_grad(at::Tensor q, OptTensor k, OptTensor wq, OptTensor wk, at::Tensor table,
-                                          OptTensor pos, double eps, bool interleaved, at::Tensor err) {
-  return QkNormRope::apply(q, k, wq, wk, table, pos, eps, interleaved, err);
+OptTensor unit_stride(const OptTensor& x) {
+  return !x.has_value() || x->dim() == 0 || x->stride(-1) == 1 ? x : OptTensor(x->contiguous());
+}
+
+// One error word a device for the calls that have no object to keep one in.
+at::Tensor rotary_err(int64_t device) {
+  static auto* words = new std::vector<at::Tensor>(64);      // never freed: the driver may be gone at exit
+  TORCH_CHECK(device >= 0 && device < 64, "no such device");
+  at::Tensor& w = (*words)[size_t(device)];
+  if (!w.defined()) w = at::zeros({1}, at::TensorOptions().dtype(at::kInt).device(at::kCUDA, c10::DeviceIndex(device)));
+  return w;
+}
+
+std::tuple<at::Tensor, OptTensor> rotary(at::Tensor q, OptTensor k, OptTensor wq, OptTensor wk, at::Tensor table,
+                                         OptTensor pos, double eps, bool interleaved) {
+  TORCH_CHECK(q.is_cuda() && q.dim() == 4, "q must be a CUDA tensor [B, T, H, d]");
+  const at::Tensor err = rotary_err(q.get_device());
+  q = *unit_stride(q);
+  k = unit_stride(k);
+  if (pos.has_value() && !pos->is_contiguous()) pos = pos->contiguous();
+  auto needs = [](const OptTensor& t) { return t.has_value() && t->requires_grad(); };
+  const bool grad = at::GradMode::is_enabled() && (q.requires_grad() || needs(k) || needs(wq) || needs(wk));
+  std::vector<at::Tensor> y =
+      grad ? QkNormRope::apply(q, k, wq, wk, table, pos, eps, interleaved, err)
+           : pd::kv::qk_norm_rope(q, k, fp32(wq), fp32(wk), table, pos, eps, interleaved, err, c10::nullopt, c10::nullopt);
+  return {y[0], k.has_value() ? OptTensor(y[1]) : OptTensor()};
 }
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.doc() = "primus_dlrm_b200 sm_100a kernels: query/key norm with rotation, paged 8-bit key/value cache, attention";
-  m.def("qk_norm_rope", &pd::kv::qk_norm_rope, py::arg("q"), py::arg("k"), py::arg("w_q"), py::arg("w_k"),
-        py::arg("table"), py::arg("positions"), py::arg("eps"), py::arg("interleaved"), py::arg("err"),
-        py::arg("dy_q") = py::none(), py::arg("dy_k") = py::none(),
-        "[y_q, y_k]; with the outputs' gradients [dq, dk, dw_q, dw_k] (without k: its entries are left out)");
-  m.def("qk_norm_rope_grad", &qk_norm_rope_grad, "[y_q, y_k] with their gradients in q, k and the weights");
+  m.def("rotary", &rotary, "(q', k') of qk_norm_rope, with gradients where asked for");
+  m.def("rotary_err", &rotary_err, "the device's int32 error word of `rotary`");
   m.def("append", &pd::kv::kv_append, "new tokens' keys and values into the pages of a cache");
   m.def("read", &pd::kv::kv_read, "tokens [first, first + n) of each sequence as bf16 [B, n, H, d]");
   m.def("paged_attention", &pd::kv::paged_attention, "attention of the last tokens over a cache -> [o(, lse)]");

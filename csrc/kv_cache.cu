@@ -341,7 +341,7 @@ static void append_launch(const AppendArgs& A, dim3 grid, int d) {
 }
 
 void kv_append(at::Tensor ck, at::Tensor cv, at::Tensor ks, at::Tensor vs, at::Tensor err, at::Tensor k, at::Tensor v,
-               at::Tensor table, at::Tensor lens, c10::optional<at::Tensor> cu, int64_t max_new,
+               at::Tensor table, at::Tensor lens, c10::optional<at::Tensor> cu, c10::optional<int64_t> max,
                c10::optional<at::Tensor> k_weight, c10::optional<double> norm_eps, c10::optional<at::Tensor> rope,
                bool interleaved) {
   const CacheDims C = check_cache(ck, cv, ks, vs, err);
@@ -349,6 +349,8 @@ void kv_append(at::Tensor ck, at::Tensor cv, at::Tensor ks, at::Tensor vs, at::T
   const int64_t B = table.size(0);
   check_ints(lens, ck, B, "kv_lens");
   const int dt = dtype_of(k, "k");
+  if (k.dim() > 0 && k.stride(-1) != 1) k = k.contiguous();
+  if (v.dim() > 0 && v.stride(-1) != 1) v = v.contiguous();
   const int td = cu.has_value() ? 3 : 4;
   AppendArgs A{};
   A.vec = true;
@@ -371,6 +373,7 @@ void kv_append(at::Tensor ck, at::Tensor cv, at::Tensor ks, at::Tensor vs, at::T
   }
   if (cu.has_value()) check_ints(*cu, ck, B + 1, "cu_new");
   else PD_CHECK(k.size(0) == B, "k has %d sequences and the page table %d", int(k.size(0)), int(B));
+  const int64_t max_new = max.value_or(k.size(td - 3));
   PD_CHECK(k.size(td - 3) < (int64_t(1) << 31) && max_new >= 0 && max_new < (int64_t(1) << 31), "too many new tokens");
   A.total = int(cu.has_value() ? k.size(0) : 0);
   A.n = int(cu.has_value() ? 0 : k.size(1));
@@ -384,6 +387,8 @@ void kv_append(at::Tensor ck, at::Tensor cv, at::Tensor ks, at::Tensor vs, at::T
   A.interleaved = interleaved;
   A.norm = norm_eps.has_value();
   A.eps = float(norm_eps.value_or(0.));
+  if (k_weight.has_value() && !(k_weight->scalar_type() == at::kFloat && k_weight->is_contiguous()))
+    k_weight = k_weight->to(at::kFloat).contiguous();
   if (k_weight.has_value()) {
     PD_CHECK(A.norm, "k_weight needs norm_eps");
     PD_CHECK(k_weight->device() == ck.device() && k_weight->scalar_type() == at::kFloat && k_weight->dim() == 1 &&
@@ -398,7 +403,7 @@ void kv_append(at::Tensor ck, at::Tensor cv, at::Tensor ks, at::Tensor vs, at::T
     A.rope = rope->data_ptr<float>();
     A.n_pos = int(std::min<int64_t>(rope->size(0), INT32_MAX));
   }
-  const int64_t most = cu.has_value() ? max_new : k.size(1);
+  const int64_t most = cu.has_value() ? std::min(max_new, k.size(0)) : k.size(1);
   if (B == 0 || most == 0 || k.size(td - 3) == 0) return;
   A.J = int((most + C.P - 2) / C.P + 1);                 // pages that `most` tokens can touch
   PD_CHECK(B * A.J < (int64_t(1) << 31), "too many sequences and pages for one call");
@@ -411,12 +416,14 @@ void kv_append(at::Tensor ck, at::Tensor cv, at::Tensor ks, at::Tensor vs, at::T
 }
 
 std::vector<at::Tensor> kv_read(at::Tensor ck, at::Tensor cv, at::Tensor ks, at::Tensor vs, at::Tensor err,
-                                at::Tensor table, at::Tensor lens, c10::optional<at::Tensor> first, int64_t n) {
+                                at::Tensor table, at::Tensor lens, c10::optional<at::Tensor> first,
+                                c10::optional<int64_t> most) {
   const CacheDims C = check_cache(ck, cv, ks, vs, err);
   check_table(table, ck);
   const int64_t B = table.size(0);
   check_ints(lens, ck, B, "kv_lens");
   if (first.has_value()) check_ints(*first, ck, B, "first");
+  const int64_t n = most.value_or(table.size(1) * C.P);
   PD_CHECK(n >= 0 && n < (int64_t(1) << 31), "n must be from 0 to 2^31 - 1");
   const c10::cuda::CUDAGuard guard(ck.device());
   ReadArgs A{};

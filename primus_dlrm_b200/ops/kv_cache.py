@@ -19,11 +19,12 @@ Native path: ``_kv`` kernels.  Eager path (CPU tensors, or
 from __future__ import annotations
 
 import math
+import os
 
 import torch
 
 from primus_dlrm_b200.ops import _ext
-from primus_dlrm_b200.ops.rotary import _w32, rotate_ref
+from primus_dlrm_b200.ops.rotary import rotate_ref
 
 _E4M3 = torch.float8_e4m3fn
 _MIN_EXP = -100              # the smallest scale is 2^-100
@@ -80,6 +81,7 @@ class PagedKVCache:
         self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
         self.err = torch.zeros(1, dtype=torch.int32, device=k.device)
         self._parts = (k, v, k_scale, v_scale, self.err)
+        self._cuda = k.is_cuda
 
     # ------------------------------------------------------------------
     @property
@@ -118,10 +120,9 @@ class PagedKVCache:
                                     e, "paged cache: a sequence's length does not fit its tokens or its page table"))
 
     def _native(self) -> bool:
-        return self.k.is_cuda and _ext.native_enabled(self.k.device)
+        return self._cuda and os.environ.get("PD_KERNELS") != "eager"
 
     # ------------------------------------------------------------------
-    @torch.no_grad()
     def append(self, k: torch.Tensor, v: torch.Tensor, page_table: torch.Tensor, kv_lens: torch.Tensor,
                cu_new: torch.Tensor | None = None, max_new: int | None = None, *,
                k_weight: torch.Tensor | None = None, norm_eps: float | None = None,
@@ -145,18 +146,12 @@ class PagedKVCache:
         and where it grows the page's earlier tokens are rounded again.
         Non-finite values are stored as NaN and do not enter the scale.
         """
-        if k_weight is not None and norm_eps is None:
-            raise ValueError("k_weight needs norm_eps")
         if self._native():
-            if max_new is None:
-                max_new = k.shape[0] if cu_new is not None else 0
-            if k.stride(-1) != 1:
-                k = k.contiguous()
-            if v.stride(-1) != 1:
-                v = v.contiguous()
-            _ext.kv().append(*self._parts, k, v, page_table, kv_lens, cu_new, max_new, _w32(k_weight), norm_eps, rope,
+            _ext.kv().append(*self._parts, k, v, page_table, kv_lens, cu_new, max_new, k_weight, norm_eps, rope,
                              interleaved)
             return
+        if k_weight is not None and norm_eps is None:
+            raise ValueError("k_weight needs norm_eps")
         B = page_table.shape[0]
         if cu_new is None:
             if k.dim() != 4 or k.shape[0] != B:
@@ -172,10 +167,10 @@ class PagedKVCache:
                 continue
             if start < 0 or start + n > page_table.shape[1] * P:
                 raise ValueError(f"sequence {b}: {start} + {n} tokens do not fit its page table")
-            kb, vb = kb.float(), vb.float()
+            kb, vb = kb.detach().float(), vb.detach().float()
             if norm_eps is not None:
                 kb = kb * torch.rsqrt(kb.pow(2).mean(-1, keepdim=True) + norm_eps)
-                kb = kb if k_weight is None else kb * k_weight.float()
+                kb = kb if k_weight is None else kb * k_weight.detach().float()
             if rope is not None:
                 if start + n > rope.shape[0]:
                     raise IndexError(f"a position lies outside the angle table of {rope.shape[0]} rows")
@@ -200,16 +195,15 @@ class PagedKVCache:
             raise IndexError(f"sequence {b}: page id {p} is out of range")
         return p
 
-    @torch.no_grad()
     def read(self, page_table: torch.Tensor, kv_lens: torch.Tensor, first: torch.Tensor | None = None,
              n: int | None = None) -> tuple[torch.Tensor, torch.Tensor]:
         """Tokens ``first[b] .. first[b] + n - 1`` of each sequence as the values
         that their codes stand for: two bf16 ``[B, n, H, d]``, zeros behind
         ``kv_lens[b]``.  By default every token that the page table has room for."""
-        if n is None:
-            n = page_table.shape[1] * self.page_size
         if self._native():
             return tuple(_ext.kv().read(*self._parts, page_table, kv_lens, first, n))
+        if n is None:
+            n = page_table.shape[1] * self.page_size
         B, P = page_table.shape[0], self.page_size
         out = [torch.zeros(B, n, self.n_kv_heads, self.head_dim, dtype=torch.bfloat16, device=self.device)
                for _ in range(2)]
@@ -261,7 +255,6 @@ def paged_attention_ref(q, cache: PagedKVCache, page_table, kv_lens, cu_q=None, 
     return o.reshape(q.shape), lse.reshape(q.shape[:-1])
 
 
-@torch.no_grad()
 def paged_attention(q: torch.Tensor, cache: PagedKVCache, page_table: torch.Tensor, kv_lens: torch.Tensor,
                     cu_q: torch.Tensor | None = None, max_q: int | None = None, *, max_len: int | None = None,
                     scale: float | None = None, causal: bool = True, return_lse: bool = False):
@@ -283,12 +276,8 @@ def paged_attention(q: torch.Tensor, cache: PagedKVCache, page_table: torch.Tens
     zeros and ``-inf``.
     """
     if cache._native():
-        if q.stride(-1) != 1:
-            q = q.contiguous()
-        out = _ext.kv().paged_attention(q, *cache._parts, page_table, kv_lens, cu_q,
-                                        q.shape[0] if max_q is None else max_q,
-                                        page_table.shape[1] * cache.page_size if max_len is None else max_len,
-                                        cache.head_dim ** -0.5 if scale is None else scale, causal, return_lse)
+        out = _ext.kv().paged_attention(q, *cache._parts, page_table, kv_lens, cu_q, max_q, max_len, scale, causal,
+                                        return_lse)
         return (out[0], out[1]) if return_lse else out[0]
-    o, lse = paged_attention_ref(q, cache, page_table, kv_lens, cu_q, scale, causal)
+    o, lse = paged_attention_ref(q.detach(), cache, page_table, kv_lens, cu_q, scale, causal)
     return (o.to(q.dtype), lse) if return_lse else o.to(q.dtype)

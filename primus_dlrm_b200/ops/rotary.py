@@ -6,31 +6,26 @@ one launch, forward and backward.  Rotated queries and keys depend on their
 positions only through differences, so a model that uses it attends over
 histories that grow, and over a key/value cache, without learned positions.
 
-Native path: ``_kv.qk_norm_rope`` / ``_kv.qk_norm_rope_grad`` (bf16, fp16 or
-fp32 in and out, 32-bit arithmetic).  Eager path: the same formulas in PyTorch.
+Native path: ``_kv.rotary`` (bf16, fp16 or fp32 in and out, 32-bit arithmetic,
+its gradient node in C++).  Eager path: the same formulas in PyTorch.
 """
 from __future__ import annotations
+
+import os
 
 import torch
 
 from primus_dlrm_b200.ops import _ext
 
-_ERR: dict = {}
-
-
 def _err_word(device) -> torch.Tensor:
-    w = _ERR.get(device)
-    if w is None:
-        w = torch.zeros(1, dtype=torch.int32, device=device)
-        _ERR[device] = w
-    return w
+    device = torch.device(device)
+    return _ext.kv().rotary_err(torch.cuda.current_device() if device.index is None else device.index)
 
 
 def rotary_error_code(device) -> int:
     """Error word of the rotary kernels (0 = ok, 1 = a position outside the
     angle table: its rows came out as zeros)."""
-    w = _ERR.get(torch.device(device))
-    return int(w.item()) if w is not None else 0
+    return int(_err_word(device).item())
 
 
 def rope_table(n_pos: int, rotary_dim: int, theta: float = 10000.0, device=None) -> torch.Tensor:
@@ -74,14 +69,6 @@ def qk_norm_rope_ref(q, k, q_weight, k_weight, table, positions=None, eps: float
     return yq, None if k is None else _norm_rope_ref(k, k_weight, ang, eps, interleaved)
 
 
-def _unit(x):
-    return x if x is None or x.stride(-1) == 1 else x.contiguous()
-
-
-def _w32(w):
-    return w if w is None or (w.dtype == torch.float32 and w.is_contiguous()) else w.float().contiguous()
-
-
 def qk_norm_rope(q: torch.Tensor, k: torch.Tensor | None, q_weight: torch.Tensor | None,
                  k_weight: torch.Tensor | None, table: torch.Tensor, positions: torch.Tensor | None = None, *,
                  eps: float = 1e-6, interleaved: bool = False) -> tuple[torch.Tensor, torch.Tensor | None]:
@@ -101,19 +88,10 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor | None, q_weight: torch.Tensor
     table comes out as zeros and sets :func:`rotary_error_code` (IndexError on
     the eager path).
     """
+    if q.is_cuda and os.environ.get("PD_KERNELS") != "eager":
+        return _ext.kv().rotary(q, k, q_weight, k_weight, table, positions, eps, interleaved)
     if q.dim() != 4 or (k is not None and k.dim() != 4):
         raise ValueError("q and k must be [B, T, H, d]")
     if k is not None and q.shape[1] > k.shape[1]:
         raise ValueError(f"more query tokens ({q.shape[1]}) than key tokens ({k.shape[1]})")
-    if not (q.is_cuda and _ext.native_enabled(q.device)):
-        return qk_norm_rope_ref(q, k, q_weight, k_weight, table, positions, eps, interleaved)
-    q, k = _unit(q), _unit(k)
-    if positions is not None and not positions.is_contiguous():
-        positions = positions.contiguous()
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, q_weight, k_weight)):
-        out = _ext.kv().qk_norm_rope_grad(q, k, q_weight, k_weight, table, positions, eps, interleaved,
-                                          _err_word(q.device))
-    else:
-        out = _ext.kv().qk_norm_rope(q, k, _w32(q_weight), _w32(k_weight), table, positions, eps, interleaved,
-                                     _err_word(q.device))
-    return out[0], out[1] if k is not None else None
+    return qk_norm_rope_ref(q, k, q_weight, k_weight, table, positions, eps, interleaved)
