@@ -71,7 +71,7 @@ struct AppendArgs {
   const int* lens;             // tokens before the call
   const int* cu;               // [B + 1] or null
   int n, total;                // new tokens of each sequence (uniform) / of all
-  int J, H, P, max_pages, n_pages, n_pos;
+  int J, H, P, logP, max_pages, n_pages, n_pos;
   const float* kw;             // [d] or null
   const float* rope;           // [n_pos, d] or null
   bool norm, interleaved, vec;
@@ -81,26 +81,27 @@ struct AppendArgs {
 
 constexpr int kAppendThreads = 128;
 
-// One block: the new tokens of one sequence that fall into one page, for one
-// head, keys (z = 0) or values. The rows stay in registers between the
-// maximum and the encoding.
-template <typename T, int D>
-__global__ void __launch_bounds__(kAppendThreads) append_kernel(const AppendArgs A) {
+// One block: the new tokens of one sequence that fall into one page, for the
+// units (keys, then values, of one head) blockIdx.y, blockIdx.y + gridDim.y,
+// ... A unit's rows stay in registers between the maximum and the encoding;
+// the next unit's are on their way meanwhile. A row belongs to D / 16 lanes of
+// 8 + 8 elements that turn against each other; PASSES times 128 / (D / 16) rows
+// make a page.
+template <typename T, int D, int PASSES>
+__global__ void __launch_bounds__(kAppendThreads) append_kernel(const __grid_constant__ AppendArgs A) {
   constexpr int L = D / 16;                          // lanes of a row
   constexpr int R = kAppendThreads / L;              // rows at a time
-  constexpr int PASSES = (64 + R - 1) / R;           // a page has at most 64 rows
-  const int part = blockIdx.z, h = blockIdx.y;
-  const int b = blockIdx.x / A.J, j = blockIdx.x % A.J;
+  const int b = blockIdx.x / A.J, j = blockIdx.x - b * A.J;
   const int len = A.lens[b];
-  const int n = A.cu ? A.cu[b + 1] - A.cu[b] : A.n;
-  const int64_t tok0 = A.cu ? A.cu[b] : 0;
+  const int tok0 = A.cu ? A.cu[b] : 0;
+  const int n = A.cu ? A.cu[b + 1] - tok0 : A.n;
   if (n <= 0) return;
-  if (len < 0 || (A.cu && (tok0 < 0 || tok0 + n > A.total))) {
+  if (len < 0 || len > INT32_MAX - 64 - n || (A.cu && (tok0 < 0 || tok0 > A.total - n))) {
     if (threadIdx.x == 0) set_error(A.err, kBadShape);
     return;
   }
-  const int64_t pi = len / A.P + j;                  // page of the sequence
-  const int64_t p0 = pi * A.P;                       // position of its first row
+  const int pi = (len >> A.logP) + j;                // page of the sequence
+  const int64_t p0 = int64_t(pi) << A.logP;          // position of its first row
   const int lo = int(max(int64_t(len) - p0, int64_t(0)));
   const int hi = int(min(int64_t(len) + n - p0, int64_t(A.P)));
   if (hi <= lo) return;
@@ -109,133 +110,141 @@ __global__ void __launch_bounds__(kAppendThreads) append_kernel(const AppendArgs
     if (threadIdx.x == 0) set_error(A.err, kIdOutOfRange);
     return;
   }
-  const T* x = static_cast<const T*>(A.x[part]) + h * A.hs[part] + (A.cu ? 0 : b * A.bs[part]);
-  const int64_t block = int64_t(page) * A.H + h;
-  uint8_t* code = A.code[part] + block * A.P * D;
+  const int first = tok0 + int(p0 - len);            // token of the page's row 0 among the new ones (may be < tok0)
   const int lane = threadIdx.x % L, row0 = threadIdx.x / L;
   int off0, off1;
   bool turned;
   pair_offsets<8>(lane, D, A.rope ? D : 0, A.interleaved, off0, off1, turned);
+  __shared__ float s_max[2][kAppendThreads / 32];
 
-  float a[PASSES][8], c[PASSES][8];
-  float amax = 0.f;                                      // infinities count, NaN does not
-#pragma unroll
-  for (int ps = 0; ps < PASSES; ++ps) {
-    if (ps * R >= A.P) break;
-    const int r = ps * R + row0;
-    const bool live = r >= lo && r < hi;
-    const int64_t i = tok0 + p0 + r - len;             // token among the new ones
-#pragma unroll
-    for (int e = 0; e < 8; ++e) a[ps][e] = c[ps][e] = 0.f;
-    if (live) {
-      const T* xr = x + i * A.ts[part];
-      if (A.vec) {
-        load_v<8>(xr + off0, a[ps]);
-        load_v<8>(xr + off1, c[ps]);
-      } else {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          a[ps][e] = to_f(xr[off0 + e]);
-          c[ps][e] = to_f(xr[off1 + e]);
-        }
-      }
-    }
-  }
-#pragma unroll
-  for (int ps = 0; ps < PASSES; ++ps) {
-    if (ps * R >= A.P) break;
-    const int r = ps * R + row0;
-    if (part == 0 && A.norm) {
-      float ss = 0.f;
-#pragma unroll
-      for (int e = 0; e < 8; ++e) ss += a[ps][e] * a[ps][e] + c[ps][e] * c[ps][e];
-      const float rs = __frsqrt_rn(group_sum<L>(ss) * (1.f / D) + A.eps);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        a[ps][e] *= rs;
-        c[ps][e] *= rs;
-      }
-      if (A.kw) {
-        float w0[8], w1[8];
-        load_w(A.kw + off0, w0);
-        load_w(A.kw + off1, w1);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          a[ps][e] *= w0[e];
-          c[ps][e] *= w1[e];
-        }
-      }
-    }
-    if (part == 0 && A.rope && r >= lo && r < hi) {
-      if (p0 + r < A.n_pos) {
-        float cs[8], sn[8];
-        load_angles<8>(A.rope + (p0 + r) * D, lane, D, A.interleaved, off0, off1, cs, sn);
-        turn<8>(a[ps], c[ps], cs, sn, A.interleaved, 1.f);
-      } else {
-        set_error(A.err, kIdOutOfRange);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) a[ps][e] = c[ps][e] = 0.f;
-      }
-    }
-#pragma unroll
-    for (int e = 0; e < 8; ++e) amax = fmaxf(amax, fmaxf(fabsf(a[ps][e]), fabsf(c[ps][e])));
-  }
-  __shared__ float s_max[kAppendThreads / 32];
-  amax = warp_max(amax);
-  if ((threadIdx.x & 31) == 0) s_max[threadIdx.x >> 5] = amax;
-  const float old = lo > 0 ? A.scale[part][block] : 0.f;
-  __syncthreads();                                       // also: everyone has read the old scale
-#pragma unroll
-  for (int w = 0; w < kAppendThreads / 32; ++w) amax = fmaxf(amax, s_max[w]);
-  if (amax == INFINITY) {
-    // seldom: infinities become NaN and leave the maximum
-    amax = 0.f;
+  Raw<8, T> xa[PASSES], xc[PASSES];
+  auto fetch = [&](int u) {
+    const int part = u >= A.H, h = part ? u - A.H : u;
+    const T* x = static_cast<const T*>(part ? A.x[1] : A.x[0]) + h * (part ? A.hs[1] : A.hs[0]) +
+                 (A.cu ? 0 : b * (part ? A.bs[1] : A.bs[0]));
+    const int64_t ts = part ? A.ts[1] : A.ts[0];
 #pragma unroll
     for (int ps = 0; ps < PASSES; ++ps) {
-      if (ps * R >= A.P) break;
+      const int r = ps * R + row0;
+      if (r >= lo && r < hi) {
+        const T* xr = x + (first + r) * ts;
+        if (A.vec) {
+          xa[ps].load(xr + off0);
+          xc[ps].load(xr + off1);
+        } else {
+          T* ea = reinterpret_cast<T*>(xa[ps].v);
+          T* ec = reinterpret_cast<T*>(xc[ps].v);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        if (fabsf(a[ps][e]) == INFINITY) a[ps][e] = NAN;
-        if (fabsf(c[ps][e]) == INFINITY) c[ps][e] = NAN;
-        amax = fmaxf(amax, fmaxf(fabsf(a[ps][e]), fabsf(c[ps][e])));
+          for (int e = 0; e < 8; ++e) {
+            ea[e] = xr[off0 + e];
+            ec[e] = xr[off1 + e];
+          }
+        }
+      } else {
+        xa[ps].zero();
+        xc[ps].zero();
       }
     }
-    __syncthreads();
-    amax = warp_max(amax);
-    if ((threadIdx.x & 31) == 0) s_max[threadIdx.x >> 5] = amax;
-    __syncthreads();
-#pragma unroll
-    for (int w = 0; w < kAppendThreads / 32; ++w) amax = fmaxf(amax, s_max[w]);
-  }
-  int e = scale_exp(amax);
-  if (lo > 0) {
-    // a scale from elsewhere that is no power of two counts as the next one
-    e = max(e, max(kMinExp, min(exp_of(old) + ((__float_as_int(old) & 0x7fffff) != 0), 120)));
-    const float ratio = old * pow2(-e);
-    if (ratio != 1.f) {
-      // the page's scale grows: its old rows move to the new one
+  };
+  fetch(blockIdx.y);
+  int buf = 0;
 #pragma unroll 1
-      for (int r = row0; r < lo; r += R) {
-        uint2* q0 = reinterpret_cast<uint2*>(code + r * D + lane * 16);
-        float f[8];
-        decode8(q0[0], f);
-        q0[0] = encode8(f, ratio);
-        decode8(q0[1], f);
-        q0[1] = encode8(f, ratio);
+  for (int u = blockIdx.y; u < 2 * A.H; u += gridDim.y, buf ^= 1) {
+    const bool keys = u < A.H;
+    const int64_t block = int64_t(page) * A.H + (keys ? u : u - A.H);
+    uint8_t* code = (keys ? A.code[0] : A.code[1]) + (block << A.logP) * D;
+    float* scale = (keys ? A.scale[0] : A.scale[1]) + block;
+    const float old = lo > 0 ? *scale : 0.f;
+    float a[PASSES][8], c[PASSES][8];
+#pragma unroll
+    for (int ps = 0; ps < PASSES; ++ps) {
+      xa[ps].floats(a[ps]);
+      xc[ps].floats(c[ps]);
+    }
+    if (u + int(gridDim.y) < 2 * A.H) fetch(u + gridDim.y);
+    float amax = 0.f;                                    // infinities count, NaN does not
+#pragma unroll
+    for (int ps = 0; ps < PASSES; ++ps) {
+      const int r = ps * R + row0;
+      if (keys && A.norm) {
+        const float rs = __frsqrt_rn(group_sum<L>(dot_v<8>(a[ps], a[ps], c[ps], c[ps])) * (1.f / D) + A.eps);
+        scale_v<8>(a[ps], rs);
+        scale_v<8>(c[ps], rs);
+        if (A.kw) {
+          float w0[8], w1[8];
+          load_w(A.kw + off0, w0);
+          load_w(A.kw + off1, w1);
+          mul_v<8>(a[ps], w0);
+          mul_v<8>(c[ps], w1);
+        }
+      }
+      if (keys && A.rope && r >= lo && r < hi) {
+        if (p0 + r < A.n_pos) {
+          float cs[8], sn[8];
+          load_angles<8>(A.rope + (p0 + r) * D, lane, D, A.interleaved, off0, off1, cs, sn);
+          turn<8>(a[ps], c[ps], cs, sn, A.interleaved, 1.f);
+        } else {
+          set_error(A.err, kIdOutOfRange);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) a[ps][e] = c[ps][e] = 0.f;
+        }
+      }
+#pragma unroll
+      for (int e = 0; e < 8; ++e) amax = fmaxf(amax, fmaxf(fabsf(a[ps][e]), fabsf(c[ps][e])));
+    }
+    amax = warp_max(amax);
+    if ((threadIdx.x & 31) == 0) s_max[buf][threadIdx.x >> 5] = amax;
+    __syncthreads();                                     // also: everyone has read the old scale
+#pragma unroll
+    for (int w = 0; w < kAppendThreads / 32; ++w) amax = fmaxf(amax, s_max[buf][w]);
+    if (amax == INFINITY) {
+      // seldom: infinities become NaN and leave the maximum
+      amax = 0.f;
+#pragma unroll
+      for (int ps = 0; ps < PASSES; ++ps) {
+  #pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          if (fabsf(a[ps][e]) == INFINITY) a[ps][e] = NAN;
+          if (fabsf(c[ps][e]) == INFINITY) c[ps][e] = NAN;
+          amax = fmaxf(amax, fmaxf(fabsf(a[ps][e]), fabsf(c[ps][e])));
+        }
+      }
+      __syncthreads();
+      amax = warp_max(amax);
+      if ((threadIdx.x & 31) == 0) s_max[buf][threadIdx.x >> 5] = amax;
+      __syncthreads();
+#pragma unroll
+      for (int w = 0; w < kAppendThreads / 32; ++w) amax = fmaxf(amax, s_max[buf][w]);
+    }
+    int e = scale_exp(amax);
+    if (lo > 0) {
+      // a scale from elsewhere that is no power of two counts as the next one
+      e = max(e, max(kMinExp, min(exp_of(old) + ((__float_as_int(old) & 0x7fffff) != 0), 120)));
+      const float ratio = old * pow2(-e);
+      if (ratio != 1.f) {
+        // the page's scale grows: its old rows move to the new one
+#pragma unroll 1
+        for (int r = row0; r < lo; r += R) {
+          uint2* q0 = reinterpret_cast<uint2*>(code + r * D + lane * 16);
+          float f[8];
+          decode8(q0[0], f);
+          q0[0] = encode8(f, ratio);
+          decode8(q0[1], f);
+          q0[1] = encode8(f, ratio);
+        }
       }
     }
-  }
-  const float inv = pow2(-e);
+    const float inv = pow2(-e);
 #pragma unroll
-  for (int ps = 0; ps < PASSES; ++ps) {
-    if (ps * R >= A.P) break;
-    const int r = ps * R + row0;
-    if (r >= lo && r < hi) {
-      *reinterpret_cast<uint2*>(code + r * D + off0) = encode8(a[ps], inv);
-      *reinterpret_cast<uint2*>(code + r * D + off1) = encode8(c[ps], inv);
+    for (int ps = 0; ps < PASSES; ++ps) {
+      const int r = ps * R + row0;
+      if (r >= lo && r < hi) {
+        *reinterpret_cast<uint2*>(code + r * D + off0) = encode8(a[ps], inv);
+        *reinterpret_cast<uint2*>(code + r * D + off1) = encode8(c[ps], inv);
+      }
     }
+    if (threadIdx.x == 0) *scale = pow2(e);
   }
-  if (threadIdx.x == 0) A.scale[part][block] = pow2(e);
 }
 
 struct ReadArgs {
@@ -251,14 +260,15 @@ struct ReadArgs {
   int* err;
 };
 
-// One block: up to 32 tokens of one sequence, all heads. A thread takes 16
+// One block: up to 128 tokens of one sequence, all heads. A thread takes 16
 // codes of one head's row at a time; the pages of the block's tokens are looked
 // up once. Bound by the writes (2 bytes a value, 1 read).
+constexpr int kReadTokens = 128;
+
 template <int D>
 __global__ void __launch_bounds__(256) read_kernel(const ReadArgs A) {
-  constexpr int TOK = 32, L = D / 16;                // threads of a row
-  __shared__ int s_row[TOK];                          // page * H * P + row in the page, or -1
-  __shared__ int s_page[TOK];
+  constexpr int TOK = kReadTokens, L = D / 16;       // threads of a row
+  __shared__ int s_row[TOK], s_page[TOK];             // row in its page, its page (or -1)
   const int part = blockIdx.y, b = blockIdx.x / A.chunks, t0 = (blockIdx.x - b * A.chunks) * TOK;
   const int tokens = min(TOK, A.n - t0);
   if (threadIdx.x < tokens) {
@@ -280,7 +290,7 @@ __global__ void __launch_bounds__(256) read_kernel(const ReadArgs A) {
   const float* scale = part ? A.scale[1] : A.scale[0];
   __nv_bfloat16* out = (part ? A.out[1] : A.out[0]) + (int64_t(b) * A.n + t0) * A.H * D;
   const int per_token = A.H * L, all = tokens * per_token;
-#pragma unroll 2
+#pragma unroll 4
   for (int i = threadIdx.x; i < all; i += 256) {
     const int t = i / per_token, j = i - t * per_token, h = j / L, c = j % L;
     const int page = s_page[t];
@@ -314,7 +324,7 @@ CacheDims check_cache(const at::Tensor& k, const at::Tensor& v, const at::Tensor
   const int64_t H = k.size(1), P = k.size(2), d = k.size(3);
   PD_CHECK(P == 16 || P == 32 || P == 64, "page size %d: expected 16, 32 or 64", int(P));
   PD_CHECK(d == 32 || d == 64 || d == 128, "head dim %d of a cache: expected 32, 64 or 128", int(d));
-  PD_CHECK(k.size(0) > 0 && H > 0 && H < 65536 && k.size(0) * H * P < (int64_t(1) << 31),
+  PD_CHECK(k.size(0) > 0 && H > 0 && H < 32768 && k.size(0) * H * P < (int64_t(1) << 31),
            "a cache has at least one page and head, and fewer than 2^31 rows");
   for (const at::Tensor* s : {&ks, &vs})
     PD_CHECK(s->device() == k.device() && s->scalar_type() == at::kFloat && s->is_contiguous() && s->dim() == 2 &&
@@ -335,9 +345,14 @@ void check_table(const at::Tensor& t, const at::Tensor& like) {
 
 template <typename T>
 static void append_launch(const AppendArgs& A, dim3 grid, int d) {
-  if (d == 32) append_kernel<T, 32><<<grid, kAppendThreads, 0, stream()>>>(A);
-  else if (d == 64) append_kernel<T, 64><<<grid, kAppendThreads, 0, stream()>>>(A);
-  else append_kernel<T, 128><<<grid, kAppendThreads, 0, stream()>>>(A);
+#define PD_GO(D, PASSES) append_kernel<T, D, PASSES><<<grid, kAppendThreads, 0, stream()>>>(A)
+  if (d == 32) PD_GO(32, 1);
+  else if (d == 64 && A.P <= 32) PD_GO(64, 1);
+  else if (d == 64) PD_GO(64, 2);
+  else if (A.P == 16) PD_GO(128, 1);
+  else if (A.P == 32) PD_GO(128, 2);
+  else PD_GO(128, 4);
+#undef PD_GO
 }
 
 void kv_append(at::Tensor ck, at::Tensor cv, at::Tensor ks, at::Tensor vs, at::Tensor err, at::Tensor k, at::Tensor v,
@@ -383,6 +398,7 @@ void kv_append(at::Tensor ck, at::Tensor cv, at::Tensor ks, at::Tensor vs, at::T
   A.lens = lens.data_ptr<int>();
   A.cu = cu.has_value() ? cu->data_ptr<int>() : nullptr;
   A.H = C.H; A.P = C.P; A.n_pages = C.n_pages;
+  A.logP = C.P == 16 ? 4 : C.P == 32 ? 5 : 6;
   A.err = err.data_ptr<int>();
   A.interleaved = interleaved;
   A.norm = norm_eps.has_value();
@@ -408,7 +424,9 @@ void kv_append(at::Tensor ck, at::Tensor cv, at::Tensor ks, at::Tensor vs, at::T
   A.J = int((most + C.P - 2) / C.P + 1);                 // pages that `most` tokens can touch
   PD_CHECK(B * A.J < (int64_t(1) << 31), "too many sequences and pages for one call");
   const c10::cuda::CUDAGuard guard(ck.device());
-  const dim3 grid(unsigned(B * A.J), C.H, 2);
+  // units that a block takes in turn: fewer blocks where there are many pages (16 blocks an SM are enough)
+  const int64_t want = (int64_t(num_sms()) * 16 + B * A.J - 1) / (B * A.J);
+  const dim3 grid(unsigned(B * A.J), unsigned(std::min<int64_t>(std::max<int64_t>(want, 1), 2 * C.H)));
   if (dt == kBf16) append_launch<__nv_bfloat16>(A, grid, C.d);
   else if (dt == kF16) append_launch<__half>(A, grid, C.d);
   else append_launch<float>(A, grid, C.d);
@@ -442,7 +460,7 @@ std::vector<at::Tensor> kv_read(at::Tensor ck, at::Tensor cv, at::Tensor ks, at:
   A.n = int(n); A.H = C.H; A.P = C.P; A.n_pages = C.n_pages;
   A.logP = C.P == 16 ? 4 : C.P == 32 ? 5 : 6;
   A.err = err.data_ptr<int>();
-  A.chunks = int((n + 31) / 32);
+  A.chunks = int((n + kReadTokens - 1) / kReadTokens);
   PD_CHECK(B * A.chunks < (int64_t(1) << 31), "too many tokens for one call");
   if (B > 0 && n > 0) {
     const dim3 grid(unsigned(B * A.chunks), 2);

@@ -119,6 +119,59 @@ __device__ __forceinline__ void load_angles(const float* at, int j, int rot, boo
   }
 }
 
+__device__ __forceinline__ uint64_t pk2_add(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+
+// Vectors of V values as packed pairs (one instruction for two values).
+template <int V>
+__device__ __forceinline__ void scale_v(float* a, float r) {               // a *= r
+  if constexpr (V == 1) {
+    a[0] *= r;
+  } else {
+#pragma unroll
+    for (int i = 0; i < V; i += 2) pk2_split(pk2_mul(pk2(a[i], a[i + 1]), pk2s(r)), a[i], a[i + 1]);
+  }
+}
+template <int V>
+__device__ __forceinline__ void mul_v(float* a, const float* w) {          // a *= w
+  if constexpr (V == 1) {
+    a[0] *= w[0];
+  } else {
+#pragma unroll
+    for (int i = 0; i < V; i += 2) pk2_split(pk2_mul(pk2(a[i], a[i + 1]), pk2(w[i], w[i + 1])), a[i], a[i + 1]);
+  }
+}
+template <int V>
+__device__ __forceinline__ void add_mul_v(float* s, const float* a, const float* b) {     // s += a b
+  if constexpr (V == 1) {
+    s[0] = fmaf(a[0], b[0], s[0]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < V; i += 2)
+      pk2_split(pk2_fma(pk2(a[i], a[i + 1]), pk2(b[i], b[i + 1]), pk2(s[i], s[i + 1])), s[i], s[i + 1]);
+  }
+}
+// sum of a0 b0 + a1 b1 over the vectors
+template <int V>
+__device__ __forceinline__ float dot_v(const float* a0, const float* b0, const float* a1, const float* b1) {
+  if constexpr (V == 1) {
+    return a0[0] * b0[0] + a1[0] * b1[0];
+  } else {
+    uint64_t s = pk2_mul(pk2(a0[0], a0[1]), pk2(b0[0], b0[1])), t = pk2_mul(pk2(a1[0], a1[1]), pk2(b1[0], b1[1]));
+#pragma unroll
+    for (int i = 2; i < V; i += 2) {
+      s = pk2_fma(pk2(a0[i], a0[i + 1]), pk2(b0[i], b0[i + 1]), s);
+      t = pk2_fma(pk2(a1[i], a1[i + 1]), pk2(b1[i], b1[i + 1]), t);
+    }
+    float x, y;
+    pk2_split(pk2_add(s, t), x, y);
+    return x + y;
+  }
+}
+
 // Turns a pair in place by the angles of load_angles (sgn = 1) or back (sgn = -1).
 template <int V>
 __device__ __forceinline__ void turn(float* a, float* b, const float* c, const float* s, bool interleaved, float sgn) {
@@ -132,20 +185,19 @@ __device__ __forceinline__ void turn(float* a, float* b, const float* c, const f
       b[2 * i] = z * c[V / 2 + i] - w * s1;
       b[2 * i + 1] = z * s1 + w * c[V / 2 + i];
     }
+  } else if constexpr (V == 1) {
+    const float x = a[0], y = b[0], si = s[0] * sgn;
+    a[0] = x * c[0] - y * si;
+    b[0] = x * si + y * c[0];
   } else {
 #pragma unroll
-    for (int i = 0; i < V; ++i) {
-      const float x = a[i], y = b[i], si = s[i] * sgn;
-      a[i] = x * c[i] - y * si;
-      b[i] = x * si + y * c[i];
+    for (int i = 0; i < V; i += 2) {
+      const uint64_t x = pk2(a[i], a[i + 1]), y = pk2(b[i], b[i + 1]), cc = pk2(c[i], c[i + 1]);
+      const uint64_t ps = pk2(s[i], s[i + 1]), ns = pk2(-s[i], -s[i + 1]);
+      pk2_split(pk2_fma(y, sgn > 0.f ? ns : ps, pk2_mul(x, cc)), a[i], a[i + 1]);
+      pk2_split(pk2_fma(x, sgn > 0.f ? ps : ns, pk2_mul(y, cc)), b[i], b[i + 1]);
     }
   }
-}
-
-__device__ __forceinline__ uint64_t pk2_add(uint64_t a, uint64_t b) {
-  uint64_t d;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
-  return d;
 }
 
 template <int L>

@@ -103,18 +103,7 @@ __global__ void __launch_bounds__(kThreads, BWD ? 2 : 3) qk_norm_rope_kernel(con
     const uint32_t row = uint32_t(it * blocks + block) * G + threadIdx.x / L;
     row_of = row < uint32_t(P.rows) ? int(row) : -1;
     at_of = -1;
-    if (row_of < 0) {
-#pragma unroll
-      for (int i = 0; i < NP; ++i) {
-        xa[i].zero();
-        xb[i].zero();
-        if (BWD) {
-          ya[i].zero();
-          yb[i].zero();
-        }
-      }
-      return;
-    }
+    if (row_of < 0) return;
     const uint32_t tok = fast_div(row, P.mul_h, P.sh_h), h = row - tok * P.H;
     const uint32_t bb = fast_div(tok, P.mul_t, P.sh_t), t = tok - bb * P.T;
     const T* xr = x + int64_t(bb) * P.bs + int64_t(t) * P.ts + int64_t(h) * P.hs;
@@ -149,8 +138,19 @@ __global__ void __launch_bounds__(kThreads, BWD ? 2 : 3) qk_norm_rope_kernel(con
   fetch(0);
   for (int it = 0; it < turns; ++it) {
     const int row = row_of;
-    const bool live = row >= 0, good = at_of >= 0;
-    const float* at = A.table + int64_t(good ? at_of : 0) * A.rot;
+    const bool live = row >= 0;
+    const float* at = A.table + int64_t(max(at_of, 0)) * A.rot;
+    if (at_of < 0) {                                    // behind the rows, or a position outside: zeros
+#pragma unroll
+      for (int i = 0; i < NP; ++i) {
+        xa[i].zero();
+        xb[i].zero();
+        if (BWD) {
+          ya[i].zero();
+          yb[i].zero();
+        }
+      }
+    }
     float a[NP][V], b[NP][V], ga[NP][V], gb[NP][V];
     float ss = 0.f;
 #pragma unroll
@@ -161,68 +161,52 @@ __global__ void __launch_bounds__(kThreads, BWD ? 2 : 3) qk_norm_rope_kernel(con
         ya[i].floats(ga[i]);
         yb[i].floats(gb[i]);
       }
-#pragma unroll
-      for (int e = 0; e < V; ++e) ss += a[i][e] * a[i][e] + b[i][e] * b[i][e];
+      ss += dot_v<V>(a[i], a[i], b[i], b[i]);
     }
     if (it + 1 < turns) fetch(it + 1);
     const float r = __frsqrt_rn(group_sum<L>(ss) * inv_d + A.eps);
-    const int64_t out = int64_t(row) * d;
-    if (!BWD) {
-      if (live) {
+    T* out = y + int64_t(row) * d;
+    float dot = 0.f;
 #pragma unroll
-        for (int i = 0; i < NP; ++i)
-          if (on[i]) {
-#pragma unroll
-            for (int e = 0; e < V; ++e) {
-              a[i][e] = good ? a[i][e] * r * w0[i][e] : 0.f;
-              b[i][e] = good ? b[i][e] * r * w1[i][e] : 0.f;
-            }
-            if (turned[i] && good) {
-              float c[V], s[V];
-              load_angles<V>(at, lane + i * L, A.rot, A.interleaved, off0[i], off1[i], c, s);
-              turn<V>(a[i], b[i], c, s, A.interleaved, 1.f);
-            }
-            store_v<V>(y + out + off0[i], a[i]);
-            store_v<V>(y + out + off1[i], b[i]);
-          }
+    for (int i = 0; i < NP; ++i) {
+      scale_v<V>(a[i], r);                              // xh
+      scale_v<V>(b[i], r);
+      if (!BWD) {
+        mul_v<V>(a[i], w0[i]);
+        mul_v<V>(b[i], w1[i]);
       }
-    } else {
-      float dot = 0.f;
-      if (good) {
-#pragma unroll
-        for (int i = 0; i < NP; ++i)
-          if (on[i]) {
-            if (turned[i]) {
-              float c[V], s[V];
-              load_angles<V>(at, lane + i * L, A.rot, A.interleaved, off0[i], off1[i], c, s);
-              turn<V>(ga[i], gb[i], c, s, A.interleaved, -1.f);
-            }
-#pragma unroll
-            for (int e = 0; e < V; ++e) {
-              a[i][e] *= r;                                   // xh
-              b[i][e] *= r;
-              acc0[i][e] += ga[i][e] * a[i][e];
-              acc1[i][e] += gb[i][e] * b[i][e];
-              ga[i][e] *= w0[i][e];
-              gb[i][e] *= w1[i][e];
-              dot += ga[i][e] * a[i][e] + gb[i][e] * b[i][e];
-            }
-          }
+      if (turned[i]) {
+        float c[V], s[V];
+        load_angles<V>(at, lane + i * L, A.rot, A.interleaved, off0[i], off1[i], c, s);
+        if (BWD) turn<V>(ga[i], gb[i], c, s, A.interleaved, -1.f);
+        else turn<V>(a[i], b[i], c, s, A.interleaved, 1.f);
       }
-      dot = group_sum<L>(dot) * inv_d;
-      if (live) {
-#pragma unroll
-        for (int i = 0; i < NP; ++i)
-          if (on[i]) {
-#pragma unroll
-            for (int e = 0; e < V; ++e) {
-              a[i][e] = good ? r * (ga[i][e] - a[i][e] * dot) : 0.f;
-              b[i][e] = good ? r * (gb[i][e] - b[i][e] * dot) : 0.f;
-            }
-            store_v<V>(y + out + off0[i], a[i]);
-            store_v<V>(y + out + off1[i], b[i]);
-          }
+      if (BWD) {
+        add_mul_v<V>(acc0[i], ga[i], a[i]);
+        add_mul_v<V>(acc1[i], gb[i], b[i]);
+        mul_v<V>(ga[i], w0[i]);
+        mul_v<V>(gb[i], w1[i]);
+        dot += dot_v<V>(ga[i], a[i], gb[i], b[i]);
       }
+    }
+    if (BWD) {
+      dot = -group_sum<L>(dot) * inv_d;
+#pragma unroll
+      for (int i = 0; i < NP; ++i) {
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+          a[i][e] = r * fmaf(a[i][e], dot, ga[i][e]);
+          b[i][e] = r * fmaf(b[i][e], dot, gb[i][e]);
+        }
+      }
+    }
+    if (live) {
+#pragma unroll
+      for (int i = 0; i < NP; ++i)
+        if (on[i]) {
+          store_v<V>(out + off0[i], a[i]);
+          store_v<V>(out + off1[i], b[i]);
+        }
     }
   }
   if (BWD) {
