@@ -81,9 +81,8 @@ struct AppendArgs {
 
 constexpr int kAppendThreads = 128;
 
-// One block: the new tokens of one sequence that fall into one page, for the
-// units (keys, then values, of one head) blockIdx.y, blockIdx.y + gridDim.y,
-// ... A unit's rows stay in registers between the maximum and the encoding;
+// One block: the new tokens of one sequence that fall into one page, for a run
+// of units (keys, then values, of one head each). A unit's rows stay in registers between the maximum and the encoding;
 // the next unit's are on their way meanwhile. A row belongs to D / 16 lanes of
 // 8 + 8 elements that turn against each other; PASSES times 128 / (D / 16) rows
 // make a page.
@@ -146,10 +145,12 @@ __global__ void __launch_bounds__(kAppendThreads) append_kernel(const __grid_con
       }
     }
   };
-  fetch(blockIdx.y);
+  const int per = (2 * A.H + gridDim.y - 1) / gridDim.y, u0 = blockIdx.y * per, u1 = min(2 * A.H, u0 + per);
+  if (u0 >= u1) return;
+  fetch(u0);
   int buf = 0;
 #pragma unroll 1
-  for (int u = blockIdx.y; u < 2 * A.H; u += gridDim.y, buf ^= 1) {
+  for (int u = u0; u < u1; ++u, buf ^= 1) {
     const bool keys = u < A.H;
     const int64_t block = int64_t(page) * A.H + (keys ? u : u - A.H);
     uint8_t* code = (keys ? A.code[0] : A.code[1]) + (block << A.logP) * D;
@@ -161,7 +162,7 @@ __global__ void __launch_bounds__(kAppendThreads) append_kernel(const __grid_con
       xa[ps].floats(a[ps]);
       xc[ps].floats(c[ps]);
     }
-    if (u + int(gridDim.y) < 2 * A.H) fetch(u + gridDim.y);
+    if (u + 1 < u1) fetch(u + 1);
     float amax = 0.f;                                    // infinities count, NaN does not
 #pragma unroll
     for (int ps = 0; ps < PASSES; ++ps) {
@@ -260,14 +261,14 @@ struct ReadArgs {
   int* err;
 };
 
-// One block: up to 128 tokens of one sequence, all heads. A thread takes 16
-// codes of one head's row at a time; the pages of the block's tokens are looked
+// One block: up to 64 tokens of one sequence, all heads. A thread takes 8
+// codes of one head's row at a time (16 bytes out, side by side); the pages of the block's tokens are looked
 // up once. Bound by the writes (2 bytes a value, 1 read).
-constexpr int kReadTokens = 128;
+constexpr int kReadTokens = 64;
 
 template <int D>
 __global__ void __launch_bounds__(256) read_kernel(const ReadArgs A) {
-  constexpr int TOK = kReadTokens, L = D / 16;       // threads of a row
+  constexpr int TOK = kReadTokens, L = D / 8;        // threads of a row
   __shared__ int s_row[TOK], s_page[TOK];             // row in its page, its page (or -1)
   const int part = blockIdx.y, b = blockIdx.x / A.chunks, t0 = (blockIdx.x - b * A.chunks) * TOK;
   const int tokens = min(TOK, A.n - t0);
@@ -294,20 +295,15 @@ __global__ void __launch_bounds__(256) read_kernel(const ReadArgs A) {
   for (int i = threadIdx.x; i < all; i += 256) {
     const int t = i / per_token, j = i - t * per_token, h = j / L, c = j % L;
     const int page = s_page[t];
-    float f[16];
+    float f[8];
 #pragma unroll
-    for (int e = 0; e < 16; ++e) f[e] = 0.f;
+    for (int e = 0; e < 8; ++e) f[e] = 0.f;
     if (page >= 0) {
       const int block = page * A.H + h;
-      const uint4 u = *reinterpret_cast<const uint4*>(code + (int64_t(block) * A.P + s_row[t]) * D + c * 16);
-      const float s = scale[block];
-      decode8(make_uint2(u.x, u.y), f);
-      decode8(make_uint2(u.z, u.w), f + 8);
-#pragma unroll
-      for (int e = 0; e < 16; ++e) f[e] *= s;
+      decode8(*reinterpret_cast<const uint2*>(code + (int64_t(block) * A.P + s_row[t]) * D + c * 8), f);
+      scale_v<8>(f, scale[block]);
     }
-    store_v<8>(out + int64_t(i) * 16, f);
-    store_v<8>(out + int64_t(i) * 16 + 8, f + 8);
+    store_v<8>(out + int64_t(i) * 8, f);
   }
 }
 

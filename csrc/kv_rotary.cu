@@ -15,9 +15,9 @@
 // of a token are neighbouring groups: they share the angles in L1, and the
 // loads of a warp are contiguous where the heads are. Rows that no 16-byte
 // access fits (odd strides, dims that are no multiple of 16) go through the
-// same code with single elements and a warp a row. A block walks over rows
-// (weights stay in registers) and loads its next row before it works on the
-// one it has.
+// same code with single elements and a warp a row. A block walks over rows and
+// has the next two (in 32 bits: one) on their way while it works on one: at two
+// to three blocks of 256 threads an SM that is 48 to 64 KB in flight.
 //
 // dw: each lane keeps its 16 columns' sums over all rows of its block, blocks
 // write theirs to a workspace and a second launch adds them in a fixed order,
@@ -79,9 +79,12 @@ __global__ void __launch_bounds__(kThreads, BWD ? 2 : 3) qk_norm_rope_kernel(con
   T* y = static_cast<T*>(P.y);
   const float inv_d = 1.f / float(d);
 
+  __shared__ __align__(16) float s_w[256];
+  for (int c = threadIdx.x; c < d; c += kThreads) s_w[c] = P.w ? P.w[c] : 1.f;
+  __syncthreads();
   int off0[NP], off1[NP];
   bool on[NP], turned[NP];
-  float w0[NP][V], w1[NP][V], acc0[NP][V], acc1[NP][V];
+  float acc0[NP][V], acc1[NP][V];
 #pragma unroll
   for (int i = 0; i < NP; ++i) {
     const int j = lane + i * L;
@@ -90,16 +93,26 @@ __global__ void __launch_bounds__(kThreads, BWD ? 2 : 3) qk_norm_rope_kernel(con
     turned[i] = false;
     if (on[i]) pair_offsets<V>(j, d, A.rot, A.interleaved, off0[i], off1[i], turned[i]);
 #pragma unroll
-    for (int e = 0; e < V; ++e) {
-      w0[i][e] = on[i] && P.w ? __ldg(P.w + off0[i] + e) : 1.f;
-      w1[i][e] = on[i] && P.w ? __ldg(P.w + off1[i] + e) : 1.f;
-      acc0[i][e] = acc1[i][e] = 0.f;
-    }
+    for (int e = 0; e < V; ++e) acc0[i][e] = acc1[i][e] = 0.f;
   }
-  // a row on its way: its elements, its place in the output (or -1) and its angles' (or -1: a position outside)
-  Raw<V, T> xa[NP], xb[NP], ya[NP], yb[NP];
-  int row_of = -1, at_of = -1;
-  auto fetch = [&](int it) {
+  auto weights = [&](int off, float* w) {
+    if constexpr (V == 1) {
+      w[0] = s_w[off];
+    } else {
+      const float4 a = *reinterpret_cast<const float4*>(s_w + off), c = *reinterpret_cast<const float4*>(s_w + off + 4);
+      w[0] = a.x; w[1] = a.y; w[2] = a.z; w[3] = a.w; w[4] = c.x; w[5] = c.y; w[6] = c.z; w[7] = c.w;
+    }
+  };
+  // rows on their way: elements, place in the output (or -1) and the angles' (or -1: a position outside)
+  struct Row {
+    Raw<V, T> xa[NP], xb[NP], ya[NP], yb[NP];
+    int row_of = -1, at_of = -1;
+  };
+  constexpr int PF = 1;
+  Row next[PF];
+  auto fetch = [&](int it, Row& F) {
+    Raw<V, T>*xa = F.xa, *xb = F.xb, *ya = F.ya, *yb = F.yb;
+    int &row_of = F.row_of, &at_of = F.at_of;
     const uint32_t row = uint32_t(it * blocks + block) * G + threadIdx.x / L;
     row_of = row < uint32_t(P.rows) ? int(row) : -1;
     at_of = -1;
@@ -135,9 +148,16 @@ __global__ void __launch_bounds__(kThreads, BWD ? 2 : 3) qk_norm_rope_kernel(con
   };
   // every lane of a warp takes part in the group sums of each turn
   const int turns = (P.rows + blocks * G - 1) / (blocks * G);
-  fetch(0);
-  for (int it = 0; it < turns; ++it) {
-    const int row = row_of;
+#pragma unroll
+  for (int k = 0; k < PF; ++k)
+    if (k < turns) fetch(k, next[k]);
+  for (int it0 = 0; it0 < turns; it0 += PF) {
+#pragma unroll
+   for (int k = 0; k < PF; ++k) {
+    const int it = it0 + k;
+    if (it >= turns) break;
+    Raw<V, T>*xa = next[k].xa, *xb = next[k].xb, *ya = next[k].ya, *yb = next[k].yb;
+    const int row = next[k].row_of, at_of = next[k].at_of;
     const bool live = row >= 0;
     const float* at = A.table + int64_t(max(at_of, 0)) * A.rot;
     if (at_of < 0) {                                    // behind the rows, or a position outside: zeros
@@ -151,6 +171,10 @@ __global__ void __launch_bounds__(kThreads, BWD ? 2 : 3) qk_norm_rope_kernel(con
         }
       }
     }
+    float c[NP][V], s[NP][V];
+#pragma unroll
+    for (int i = 0; i < NP; ++i)
+      if (turned[i]) load_angles<V>(at, lane + i * L, A.rot, A.interleaved, off0[i], off1[i], c[i], s[i]);
     float a[NP][V], b[NP][V], ga[NP][V], gb[NP][V];
     float ss = 0.f;
 #pragma unroll
@@ -163,7 +187,7 @@ __global__ void __launch_bounds__(kThreads, BWD ? 2 : 3) qk_norm_rope_kernel(con
       }
       ss += dot_v<V>(a[i], a[i], b[i], b[i]);
     }
-    if (it + 1 < turns) fetch(it + 1);
+    if (it + PF < turns) fetch(it + PF, next[k]);
     const float r = __frsqrt_rn(group_sum<L>(ss) * inv_d + A.eps);
     T* out = y + int64_t(row) * d;
     float dot = 0.f;
@@ -171,21 +195,22 @@ __global__ void __launch_bounds__(kThreads, BWD ? 2 : 3) qk_norm_rope_kernel(con
     for (int i = 0; i < NP; ++i) {
       scale_v<V>(a[i], r);                              // xh
       scale_v<V>(b[i], r);
+      float w0[V], w1[V];
+      weights(off0[i], w0);
+      weights(off1[i], w1);
       if (!BWD) {
-        mul_v<V>(a[i], w0[i]);
-        mul_v<V>(b[i], w1[i]);
+        mul_v<V>(a[i], w0);
+        mul_v<V>(b[i], w1);
       }
       if (turned[i]) {
-        float c[V], s[V];
-        load_angles<V>(at, lane + i * L, A.rot, A.interleaved, off0[i], off1[i], c, s);
-        if (BWD) turn<V>(ga[i], gb[i], c, s, A.interleaved, -1.f);
-        else turn<V>(a[i], b[i], c, s, A.interleaved, 1.f);
+        if (BWD) turn<V>(ga[i], gb[i], c[i], s[i], A.interleaved, -1.f);
+        else turn<V>(a[i], b[i], c[i], s[i], A.interleaved, 1.f);
       }
       if (BWD) {
         add_mul_v<V>(acc0[i], ga[i], a[i]);
         add_mul_v<V>(acc1[i], gb[i], b[i]);
-        mul_v<V>(ga[i], w0[i]);
-        mul_v<V>(gb[i], w1[i]);
+        mul_v<V>(ga[i], w0);
+        mul_v<V>(gb[i], w1);
         dot += dot_v<V>(ga[i], a[i], gb[i], b[i]);
       }
     }
@@ -208,6 +233,7 @@ __global__ void __launch_bounds__(kThreads, BWD ? 2 : 3) qk_norm_rope_kernel(con
           store_v<V>(out + off1[i], b[i]);
         }
     }
+   }
   }
   if (BWD) {
     // groups of a warp by shuffles, warps through shared memory, both in a fixed order
