@@ -14,210 +14,16 @@
 // bits down to 2^-29 and reaches 2^-39. A page's key scale multiplies its
 // scores in 32 bits; its value scale, relative to the largest of the tile's
 // pages, its probabilities. Running maximum, sum and output stay in 32 bits.
-#include <c10/cuda/CUDAGuard.h>
-#include <cuda_fp8.h>
-
-#include <cmath>
-
-#include "kv_common.cuh"
+#include "kv_attn.cuh"
 
 namespace pd {
 namespace kv {
-
-struct CacheDims { int n_pages, H, P, d; };
-CacheDims check_cache(const at::Tensor&, const at::Tensor&, const at::Tensor&, const at::Tensor&, const at::Tensor&);
-void check_ints(const at::Tensor&, const at::Tensor&, int64_t, const char*);
-void check_table(const at::Tensor&, const at::Tensor&);
-
-constexpr uint64_t kWaitLimitNs = 2000000000ull;
-constexpr int kWarps = 4;               // warps of a block
-
-struct AttnArgs {
-  const void* q;                // token, head (and batch) strides below
-  int64_t q_bs, q_ts, q_hs;
-  const float* ks; const float* vs;          // [pages, H]
-  const int* table; int64_t table_stride;
-  const int* lens;
-  const int* cu;                // [B + 1] or null
-  void* o;                      // [tokens, Hq, d]
-  float* lse;                   // [tokens, Hq] or null
-  int B, n, total, Hq, H, G, P, logP, max_pages, n_pages;
-  bool causal, split, bf16;
-  int min_units;
-  float scale_log2;
-  float* part_o;                // split: [2 grid, R, d] sums, [2 grid, R, 2] (max, sum), [2 grid, 4] heads
-  float* part_ml;
-  int* part_head;
-  int* err;
-};
 
 template <int D> struct Cfg;
 // TK keys of products and softmax at a time, SUB such tiles (8 KB of keys and values) to a copy, ST copies in flight
 template <> struct Cfg<32> { static constexpr int TK = 64, SUB = 2, ST = 2; };
 template <> struct Cfg<64> { static constexpr int TK = 64, SUB = 1, ST = 2; };
 template <> struct Cfg<128> { static constexpr int TK = 32, SUB = 1, ST = 2; };
-
-__device__ __forceinline__ uint32_t smem_u32(const void* p) {
-  return static_cast<uint32_t>(__cvta_generic_to_shared(p));
-}
-__device__ __forceinline__ bool mbar_try(uint32_t bar, uint32_t parity) {
-  uint32_t ok;
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
-      "selp.b32 %0, 1, 0, p;\n\t}"
-      : "=r"(ok) : "r"(bar), "r"(parity), "r"(200000u) : "memory");
-  return ok != 0;
-}
-__device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, int* err) {
-  if (mbar_try(bar, parity)) return true;
-  const uint64_t t0 = globaltimer_ns();
-  while (!mbar_try(bar, parity)) {
-    if (globaltimer_ns() - t0 > kWaitLimitNs) {
-      set_error(err, kWaitTimeout);
-      return false;
-    }
-  }
-  return true;
-}
-__device__ __forceinline__ void tma_rows(uint32_t dst, const CUtensorMap* map, uint32_t bar, int row) {
-  asm volatile(
-      "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
-      ::"r"(dst), "l"(map), "r"(bar), "r"(0), "r"(row) : "memory");
-}
-__device__ __forceinline__ uint4 lds128(uint32_t a) {
-  uint4 v;
-  asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a));
-  return v;
-}
-__device__ __forceinline__ uint2 lds64(uint32_t a) {
-  uint2 v;
-  asm volatile("ld.shared.v2.b32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(a));
-  return v;
-}
-__device__ __forceinline__ uint32_t lds32(uint32_t a) {
-  uint32_t v;
-  asm volatile("ld.shared.b32 %0, [%1];" : "=r"(v) : "r"(a));
-  return v;
-}
-// two pairs of e4m3 codes -> two f16x2
-__device__ __forceinline__ void cvt4(uint32_t w, uint32_t& lo, uint32_t& hi) {
-  asm("{\n\t.reg .b16 l, h;\n\t"
-      "mov.b32 {l, h}, %2;\n\t"
-      "cvt.rn.f16x2.e4m3x2 %0, l;\n\t"
-      "cvt.rn.f16x2.e4m3x2 %1, h;\n\t}" : "=r"(lo), "=r"(hi) : "r"(w));
-}
-// D = A * B
-__device__ __forceinline__ void mma_f16_0(float* d, const uint32_t* a, uint32_t b0, uint32_t b1) {
-  asm(
-      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};\n"
-      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
-      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
-}
-// queries and outputs are bf16 or fp16 by a flag of the call
-__device__ __forceinline__ float to_f_16(uint16_t v, bool bf16) {
-  return bf16 ? __bfloat162float(__ushort_as_bfloat16(v)) : __half2float(__ushort_as_half(v));
-}
-__device__ __forceinline__ void load8_16(const uint16_t* p, bool bf16, float* f) {
-  const uint4 u = *reinterpret_cast<const uint4*>(p);
-  const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    f[2 * i] = to_f_16(uint16_t(w[i] & 0xffffu), bf16);
-    f[2 * i + 1] = to_f_16(uint16_t(w[i] >> 16), bf16);
-  }
-}
-__device__ __forceinline__ uint32_t pack_16(float lo, float hi, bool bf16) {
-  if (bf16) {
-    const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
-    return *reinterpret_cast<const uint32_t*>(&v);
-  }
-  const __half2 v = __floats2half2_rn(lo, hi);
-  return *reinterpret_cast<const uint32_t*>(&v);
-}
-__device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
-  const __half2 v = __floats2half2_rn(lo, hi);
-  return *reinterpret_cast<const uint32_t*>(&v);
-}
-// the transpose of an 8 x 8 tile of 16-bit values (lane: row lane / 4, columns 2 (lane % 4) and the next)
-__device__ __forceinline__ uint32_t transpose8(uint32_t x) {
-  uint32_t y;
-  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
-  return y;
-}
-// D(16x8 f32) += A(16x16 f16, row) * B(16x8 f16, col)
-__device__ __forceinline__ void mma_f16(float* d, const uint32_t* a, uint32_t b0, uint32_t b1) {
-  asm(
-      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
-      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
-
-// The queries and keys of one sequence, with impossible lengths cut (and reported).
-template <int R>
-struct Seq {
-  int len, n, tok0, tiles_m;                // tiles_m: segments of R rows (query, head of the group) for a key head
-  __device__ __forceinline__ void load(const AttnArgs& A, int b) {
-    len = __ldg(A.lens + b);
-    if (A.cu) {
-      tok0 = __ldg(A.cu + b);
-      n = __ldg(A.cu + b + 1) - tok0;
-      if (n < 0 || tok0 < 0 || tok0 > A.total - n) {
-        set_error(A.err, kBadShape);
-        n = 0;
-      }
-    } else {
-      n = A.n;
-      tok0 = b * A.n;
-    }
-    if (int64_t(len) > int64_t(A.max_pages) << A.logP) {
-      set_error(A.err, kBadShape);
-      len = A.max_pages << A.logP;
-    }
-    if (len < 0) {
-      set_error(A.err, kBadShape);
-      len = 0;
-    }
-    tiles_m = int((int64_t(n) * A.G + R - 1) / R);
-  }
-  // units of `sup` keys in each of its segments; a sequence without keys has one (it writes zeros)
-  __device__ __forceinline__ int units(int sup) const { return max(1, (len + sup - 1) / sup); }
-  __device__ __forceinline__ int64_t all(int H, int sup) const { return int64_t(units(sup)) * H * tiles_m; }
-};
-
-// A place in the list of units: sequence b, segment (head, row tile) in it, unit of its keys.
-template <int R>
-struct Cursor {
-  int b, h, mt, unit, units;
-  Seq<R> s;
-  int lim;                        // keys that the row tile's last row sees
-  int left;                       // units from here to the end of this worker's range
-  __device__ __forceinline__ void limits(const AttnArgs& A) {
-    const int last = min(mt * R + R, s.n * A.G) - 1;
-    lim = A.causal ? max(0, s.len - s.n + last / A.G + 1) : s.len;
-  }
-  __device__ __forceinline__ void next_seq(const AttnArgs& A, int sup) {
-    do {
-      if (++b >= A.B) { left = 0; return; }
-      s.load(A, b);
-    } while (s.tiles_m == 0);
-    units = s.units(sup);
-  }
-  __device__ __forceinline__ void next(const AttnArgs& A, int sup) {
-    if (--left <= 0) return;
-    if (++unit < units) return;
-    unit = 0;
-    if (++mt == s.tiles_m) {
-      mt = 0;
-      if (++h == A.H) {
-        h = 0;
-        next_seq(A, sup);
-        if (left <= 0) return;
-      }
-    }
-    limits(A);
-  }
-};
 
 // Few rows to a segment (one or some query tokens of one sequence, the heads
 // that share a key head): bound by reading the cache.
@@ -910,7 +716,6 @@ template <int D> struct Many;
 template <> struct Many<32> { static constexpr int MT = 2, TK = 32, ST = 4, PER_SM = 4; };
 template <> struct Many<64> { static constexpr int MT = 2, TK = 32, ST = 4, PER_SM = 3; };
 template <> struct Many<128> { static constexpr int MT = 1, TK = 32, ST = 3, PER_SM = 3; };
-constexpr int kUnit = 64;               // keys of a copy
 
 template <int D>
 __global__ void __launch_bounds__(kWarps * 32, Many<D>::PER_SM)
@@ -1310,57 +1115,6 @@ paged_attn_many_kernel(const AttnArgs A, const __grid_constant__ CUtensorMap tm_
     }
 }
 
-// cuTensorMapEncodeTiled through the runtime: the extension does not link
-// libcuda, so it imports on machines without a driver.
-static CUresult encode_tiled(CUtensorMap* m, void* base, const cuuint64_t* dims, const cuuint64_t* strides,
-                             const cuuint32_t* box, CUtensorMapSwizzle swizzle) {
-  using Fn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
-                          const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
-                          CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-  static const Fn fn = [] {
-    void* p = nullptr;
-    cudaDriverEntryPointQueryResult q = cudaDriverEntryPointSymbolNotFound;
-    const cudaError_t e = cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q);
-    PD_CHECK(e == cudaSuccess && q == cudaDriverEntryPointSuccess && p != nullptr,
-             "cuTensorMapEncodeTiled is unavailable (%d, %d)", int(e), int(q));
-    return reinterpret_cast<Fn>(p);
-  }();
-  const cuuint32_t es[2] = {1, 1};
-  return fn(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, base, dims, strides, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle,
-            CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-}
-
-static CUtensorMap code_map(const at::Tensor& x, int box_rows) {
-  CUtensorMap m;
-  const int64_t d = x.size(3), rows = x.numel() / d;
-  const cuuint64_t dims[2] = {cuuint64_t(d), cuuint64_t(rows)}, strides[1] = {cuuint64_t(d)};
-  const cuuint32_t box[2] = {cuuint32_t(d), cuuint32_t(box_rows)};
-  const CUresult r = encode_tiled(&m, x.data_ptr(), dims, strides, box,
-                                  d == 128  ? CU_TENSOR_MAP_SWIZZLE_128B
-                                  : d == 64 ? CU_TENSOR_MAP_SWIZZLE_64B
-                                            : CU_TENSOR_MAP_SWIZZLE_32B);
-  PD_CHECK(r == CUDA_SUCCESS, "cuTensorMapEncodeTiled failed for the cache (%d)", int(r));
-  return m;
-}
-
-// Blocks of a kernel that an SM of this device holds.
-template <typename K>
-static int blocks_per_sm(K kern, int threads, int smem, int (&known)[64]) {
-  int dev = 0;
-  PD_CHECK_CUDA(cudaGetDevice(&dev));
-  if (dev < 64 && known[dev] > 0) return known[dev];
-  PD_CHECK_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
-  int n = 0;
-  PD_CHECK_CUDA(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kern, threads, smem));
-  PD_CHECK(n > 0, "an attention kernel does not fit an SM");
-  if (dev < 64) known[dev] = n;
-  return n;
-}
-
-struct Bounds {                 // of what the lengths on the device can ask for; they only decide how the work is split
-  int64_t B, rows, len;         // rows: most (query, head of the group) of a sequence and key head
-};
-
 template <int D, int R, int W>
 static void few_launch(AttnArgs& A, const at::Tensor& ck, const at::Tensor& cv, const Bounds& U) {
   constexpr int TK = Cfg<D>::TK, WK = TK * Cfg<D>::SUB, SUP = WK * W;
@@ -1418,8 +1172,11 @@ static void attn_dispatch(AttnArgs& A, const at::Tensor& ck, const at::Tensor& c
   // a warp a segment where there are eight segments and more for every warp of the device (12 warps an SM)
   const bool many = U.B * A.H * ((U.rows + 15) / 16) >= int64_t(num_sms()) * 12 * 4;
   const int64_t tiles = (U.rows + 16 * Many<D>::MT * kWarps - 1) / (16 * Many<D>::MT * kWarps);
-  if (U.rows > 32 && U.B * A.H * tiles >= num_sms() && tiles < 65536 && U.B * A.H < (int64_t(1) << 31))
+  if (U.rows > 32 && U.B * A.H * tiles >= num_sms() && tiles < 65536 && U.B * A.H < (int64_t(1) << 31)) {
+    if constexpr (D <= 64)
+      if (U.rows > 64) return attn_tc_launch(A, ck, cv, D, U);
     return many_launch<D>(A, ck, cv, U);
+  }
   if (U.rows <= 8) return many ? few_launch<D, 8, 1>(A, ck, cv, U) : few_launch<D, 8, 4>(A, ck, cv, U);
   return many ? few_launch<D, 16, 1>(A, ck, cv, U) : few_launch<D, 16, 4>(A, ck, cv, U);
 }

@@ -259,6 +259,50 @@ def test_attention_ragged(P, d, H, G, lens, new):
     _attn_check(q, c, table, _i32(lens), cu, causal=False, scale=0.05)
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("P,d,H,G,most", [(64, 64, 4, 1, 300), (16, 64, 2, 3, 90), (32, 32, 4, 2, 130), (64, 32, 2, 1, 200),
+                                          (16, 32, 8, 1, 65), (64, 128, 4, 1, 150), (32, 128, 2, 2, 70), (16, 128, 8, 1, 40),
+                                          (32, 64, 8, 1, 40), (64, 32, 8, 1, 33)])
+def test_many_rows(P, d, H, G, most, causal, dtype):
+    """Enough rows and sequences for the forms that share copies among rows (more than 32 and more than 64 rows to a
+    key head, at least a block an SM), ragged, with rows without keys and empty sequences among them."""
+    g = torch.Generator(device=DEV).manual_seed(d + most)
+    B = 160 // H + 3
+    new = [max(1, most - (i * 37) % most) for i in range(B)]
+    lens = [max(0, n + (i * 53) % 211 - 40) for i, n in enumerate(new)]
+    new[1], lens[1], lens[2], new[3] = 0, 40, 0, most
+    c = _cache(sum(-(-t // P) for t in lens) + 1, H, d, P, seed=most)
+    table = _table(lens, P, c.n_pages, room=1)
+    q = (1.5 * torch.randn(sum(new), H * G, d, generator=g, device=DEV)).to(dtype)
+    cu = _i32([0] + list(torch.tensor(new).cumsum(0)))
+    o, _ = _attn_check(q, c, table, _i32(lens), cu, max(new), causal=causal)
+    # the same, a sequence at a time (other forms): within both forms' tolerances
+    for b in (0, 3, B - 1):
+        a, e = int(cu[b]), int(cu[b + 1])
+        _attn_check(q[None, a:e], c, table[b:b + 1], _i32(lens[b:b + 1]), causal=causal)
+
+
+def test_many_rows_that_need_rescaling():
+    """Scores that keep growing along the keys, so that running maxima are raised again and again; very different
+    pages; and stale NaN codes behind every sequence's keys."""
+    g = torch.Generator(device=DEV).manual_seed(2)
+    for d, P in ((64, 64), (32, 16), (128, 32)):
+        B, H, n, T = 40, 4, 100, 300
+        c = _cache(B * -(-T // P), H, d, P, spread=2.0)
+        table = _table([T] * B, P, c.n_pages)
+        for j in range(table.shape[1]):
+            c.k_scale[table[:, j].long()] *= 2.0 ** (j * P // 64)
+        q = torch.randn(B, n, H, d, generator=g, device=DEV).bfloat16()
+        lens = [T - 7 - i for i in range(B)]
+        for x in (c.k, c.v):
+            codes = x.view(torch.uint8)
+            for b, t in enumerate(lens):
+                codes[table[b, t // P].long(), :, t % P:] = 0x7F
+                codes[table[b, t // P + 1:].long()] = 0x7F
+        _attn_check(q, c, table, _i32(lens))
+
+
 @pytest.mark.parametrize("n,lens", [(4, [2, 0, 4, 70]), (1, [0, 1, 0]), (70, [3, 65, 0])])
 def test_rows_without_keys(n, lens):
     """More queries than tokens: the first rows see nothing and give zeros."""
