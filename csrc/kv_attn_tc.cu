@@ -4,7 +4,7 @@
 // Same sums as kv_attn.cu. A block takes 128 rows (query, head of the group)
 // of one sequence and key head and walks over the keys they see, 64 at a time:
 //
-//   warp 0      copies: TMA loads of codes (two tiles ahead), and the scales of their pages
+//   warp 0      copies: TMA loads of codes (four tiles), and the scales of their pages
 //   warps 2, 3  conversion: e4m3 codes -> fp16 operand tiles in the swizzled layout that the products read
 //   warp 1      products, issued by one lane: S = Q K^T two tiles ahead of the softmax, O += P V (P from TMEM)
 //   warps 4-7   softmax, a thread a row: 64 scores from TMEM to registers, P (fp16) back over them
@@ -32,9 +32,9 @@ namespace kv {
 
 constexpr int kTcRows = 128;
 constexpr int kTcThreads = 256;
-constexpr int kRaw = 2;                 // tiles of codes in flight
+constexpr int kRaw = 4;                 // tiles of codes in flight
 constexpr int kOps = 3;                 // operand tiles, and S / P buffers
-constexpr int kSc = 8;                  // tiles whose scales are kept (more than kRaw + kOps apart from writer to reader)
+constexpr int kSc = 8;                  // tiles whose scales are kept (writer and reader are at most kRaw + kOps apart)
 
 __device__ __forceinline__ void mbar_init(uint64_t* b, int n) {
   asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(smem_u32(b)), "r"(n));
@@ -174,6 +174,9 @@ paged_attn_tc_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__
   auto aborted = [&]() { return __any_sync(0xffffffffu, s_abort != 0); };    // one answer for a whole warp
   auto wait = [&](uint64_t* bar, int turn) { return mbar_wait(smem_u32(bar), uint32_t(turn) & 1u, A.err); };
 
+  // the softmax warps take the registers that the others do not need: (64 + 192) x 128 = 128 x 256
+  if (warp < 4) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
   if (warp == 0) {
     // ---------------- copies ----------------
     const int boxes = kUnit >> A.logP;
@@ -267,7 +270,7 @@ paged_attn_tc_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__
       tc_commit(&mma_done);
       (void)wait(&mma_done, 0);
     }
-  } else if (warp < 4) {
+  } else {
     // ---------------- conversion ----------------
     const int ct = threadIdx.x - 64;
     constexpr int C = D / 16;               // chunks of 16 codes of a row
@@ -303,7 +306,9 @@ paged_attn_tc_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__
       mbar_arrive(&raw_empty[sl]);
     }
     if (!ok) s_abort = 1;
+  }
   } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 192;");
     // ---------------- softmax, a thread a row ----------------
     const int quarter = warp & 3, r = quarter * 32 + lane, row = r0 + r;
     const uint32_t lane_base = tmem + (uint32_t(quarter * 32) << 16);
@@ -357,11 +362,15 @@ paged_attn_tc_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__
       tm_ld_wait(sr + 32);
       const uint32_t gone = s_gone[e];
       const int see = my_lim - k0;                          // columns c < see are visible
+      if (__any_sync(0xffffffffu, see < kUnit)) {
+#pragma unroll
+        for (int c = 0; c < 64; ++c) sr[c] = c < see ? sr[c] : __float_as_uint(-INFINITY);
+      }
       const uint32_t seen = (2u << ((min(kUnit, lim - k0) - 1) >> A.logP)) - 1;
-      if (__any_sync(0xffffffffu, see < kUnit) || (gone & seen)) {
+      if (gone & seen) {                                    // seldom: a page in front of the end is missing
 #pragma unroll
         for (int c = 0; c < 64; ++c)
-          if (c >= see || (gone >> (c >> A.logP) & 1)) sr[c] = __float_as_uint(-INFINITY);
+          if (gone >> (c >> A.logP) & 1) sr[c] = __float_as_uint(-INFINITY);
       }
       float f[4], lv[4];
       float mx = -INFINITY;
