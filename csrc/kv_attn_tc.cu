@@ -274,6 +274,8 @@ paged_attn_tc_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__
     // ---------------- conversion ----------------
     const int ct = threadIdx.x - 64;
     constexpr int C = D / 16;               // chunks of 16 codes of a row
+    const int row0 = ct / C;                // this thread converts chunk ct % C of rows row0, row0 + 64 / C, ...
+    const uint32_t to0 = Op<D>::chunk(row0, 2 * (ct % C)), to1 = Op<D>::chunk(row0, 2 * (ct % C) + 1);
     bool ok = true;
     for (int v = 0; v < units && ok && !s_abort; ++v) {
       const int sl = v % kRaw, op = v % kOps, e = v % kSc;
@@ -282,24 +284,35 @@ paged_attn_tc_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__
       if (!ok) break;
       const uint32_t gone = s_gone[e];
       const int keys = min(kUnit, lim - v * kUnit);         // of the tile that some row sees
-      const uint32_t src = sRaw + sl * 2 * kRawBytes;
+      const bool whole = keys == kUnit && !(gone & ((2u << ((kUnit - 1) >> A.logP)) - 1));
+      const uint32_t src = sRaw + sl * 2 * kRawBytes + ct * 16;
 #pragma unroll
-      for (int i = 0; i < 2 * C; ++i) {
-        const bool val = i >= C;
-        const int x = (val ? i - C : i) * 64 + ct, row = x / C, c = x % C;
-        uint4 u = lds128(src + (val ? kRawBytes : 0) + row * D + c * 16);
-        // values behind the keys may be anything, NaN too; scores of such keys are masked
-        if (val && (row >= keys || (gone >> (row >> A.logP) & 1))) u = make_uint4(0, 0, 0, 0);
-        uint32_t w[8];
-        cvt4(u.x, w[0], w[1]);
-        cvt4(u.y, w[2], w[3]);
-        cvt4(u.z, w[4], w[5]);
-        cvt4(u.w, w[6], w[7]);
-        const uint32_t dst = (val ? sV : sK) + op * kOpBytes;
-        asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(dst + Op<D>::chunk(row, 2 * c)), "r"(w[0]), "r"(w[1]),
-                     "r"(w[2]), "r"(w[3]) : "memory");
-        asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(dst + Op<D>::chunk(row, 2 * c + 1)), "r"(w[4]),
-                     "r"(w[5]), "r"(w[6]), "r"(w[7]) : "memory");
+      for (int half = 0; half < 2; ++half) {                // keys, values
+        uint4 u[C];
+#pragma unroll
+        for (int i = 0; i < C; ++i) u[i] = lds128(src + half * kRawBytes + i * 1024);
+        if (half == 1 && !whole) {
+          // values behind the keys may be anything, NaN too; scores of such keys are masked
+#pragma unroll
+          for (int i = 0; i < C; ++i) {
+            const int row = row0 + i * (64 / C);
+            if (row >= keys || (gone >> (row >> A.logP) & 1)) u[i] = make_uint4(0, 0, 0, 0);
+          }
+        }
+        const uint32_t dst = (half ? sV : sK) + op * kOpBytes;
+#pragma unroll
+        for (int i = 0; i < C; ++i) {
+          uint32_t w[8];
+          cvt4(u[i].x, w[0], w[1]);
+          cvt4(u[i].y, w[2], w[3]);
+          cvt4(u[i].z, w[4], w[5]);
+          cvt4(u[i].w, w[6], w[7]);
+          const uint32_t at = dst + i * (64 / C) * Op<D>::kRow;       // the exchange of chunks repeats every 8 rows
+          asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(at + to0), "r"(w[0]), "r"(w[1]), "r"(w[2]),
+                       "r"(w[3]) : "memory");
+          asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(at + to1), "r"(w[4]), "r"(w[5]), "r"(w[6]),
+                       "r"(w[7]) : "memory");
+        }
       }
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       mbar_arrive(&kv_full[op]);
