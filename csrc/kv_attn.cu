@@ -205,20 +205,8 @@ paged_attn_kernel(const AttnArgs A, const __grid_constant__ CUtensorMap tm_k, co
   for (int i = 0; i < ST - 1; ++i) issue(i, scl[i], gone[i]);
 
   // ---- consumer ----
-  uint32_t k_off, v_off[2];                 // this lane's bytes in a tile: key row g, value rows 2 qd and 2 qd + 1
-  if (D == 128) {
-    k_off = g * 128 + ((2 * qd) ^ g) * 16;
-    v_off[0] = (2 * qd) * 128 + (g ^ (2 * qd)) * 16;
-    v_off[1] = (2 * qd + 1) * 128 + (g ^ (2 * qd + 1)) * 16;
-  } else if (D == 64) {
-    k_off = g * 64 + (qd ^ (g >> 1)) * 16;
-    v_off[0] = (2 * qd) * 64 + ((g >> 1) ^ qd) * 16 + (g & 1) * 8;
-    v_off[1] = v_off[0] + 64;
-  } else {
-    k_off = g * 32 + ((qd >> 1) ^ (g >> 2)) * 16 + (qd & 1) * 8;
-    v_off[0] = (2 * qd) * 32 + ((g >> 2) ^ (qd >> 1)) * 16 + (g & 3) * 4;
-    v_off[1] = v_off[0] + 32;
-  }
+  uint32_t k_off, v_off[2];
+  lane_offsets<D>(g, qd, k_off, v_off);
   // the two rows of this lane's accumulators
   const int row_a = R == 16 ? g : 2 * qd, row_b = R == 16 ? g + 8 : 2 * qd + 1;
   bool alive = true;
@@ -247,24 +235,13 @@ paged_attn_kernel(const AttnArgs A, const __grid_constant__ CUtensorMap tm_k, co
                               int64_t(seg_h * A.G + (live ? r - qi * A.G : 0)) * A.q_hs + qd * E;
 #pragma unroll
         for (int e = 0; e < E; ++e) x[i][e] = 0.f;
-        if (live) {
-          if (reinterpret_cast<uintptr_t>(src) % 16 == 0) {
-#pragma unroll
-            for (int e = 0; e < E; e += 8) load8_16(src + e, A.bf16, &x[i][e]);
-          } else {
-#pragma unroll
-            for (int e = 0; e < E; ++e) x[i][e] = to_f_16(src[e], A.bf16);
-          }
-        }
+        if (live) load_row<E>(src, A.bf16, x[i]);
         float amax = 0.f;
 #pragma unroll
         for (int e = 0; e < E; ++e) amax = fmaxf(amax, fabsf(x[i][e]));
         amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
         amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
-        // 2^(14 - exponent), negative for a negative softmax scale; a row of zeros, an infinity or NaN stays as it is
-        const int ex = amax > 0.f && amax < INFINITY ? max(-100, (__float_as_int(amax) >> 23) - 127) : 14;
-        const float up = copysignf(__int_as_float((14 - ex + 127) << 23), A.scale_log2);
-        back[i] = __int_as_float((ex - 14 + 127) << 23) * fabsf(A.scale_log2);
+        const float up = row_scale(amax, A.scale_log2, back[i]);
 #pragma unroll
         for (int e = 0; e < E; ++e) x[i][e] *= up;
       }
@@ -314,24 +291,11 @@ paged_attn_kernel(const AttnArgs A, const __grid_constant__ CUtensorMap tm_k, co
         const uint32_t missing = my_gone >> pg0;                      // its pages that were not loaded
         // ---- scores: fragment j holds keys 8 j.. (R = 16) or 16 j.. (R = 8) ----
         float s[SF][4];
-        auto load_keys = [&](int row, uint32_t* w) {          // words of this lane's dims of key `row` + g
-          if constexpr (D == 128) {
-            const uint4 a = lds128(kt + k_off + row * D), b = lds128(kt + (k_off ^ 16) + row * D);
-            w[0] = a.x; w[1] = a.y; w[2] = a.z; w[3] = a.w;
-            w[4] = b.x; w[5] = b.y; w[6] = b.z; w[7] = b.w;
-          } else if constexpr (D == 64) {
-            const uint4 a = lds128(kt + k_off + row * D);
-            w[0] = a.x; w[1] = a.y; w[2] = a.z; w[3] = a.w;
-          } else {
-            const uint2 a = lds64(kt + k_off + row * D);
-            w[0] = a.x; w[1] = a.y;
-          }
-        };
 #pragma unroll
         for (int j = 0; j < SF; ++j) {
           if constexpr (R == 16) {
             uint32_t w[KS];
-            load_keys(8 * j, w);
+            load_key<D>(kt + k_off + 8 * j * D, w);
 #pragma unroll
             for (int k = 0; k < KS; ++k) {
               uint32_t b0, b1;
@@ -341,8 +305,8 @@ paged_attn_kernel(const AttnArgs A, const __grid_constant__ CUtensorMap tm_k, co
             }
           } else {
             uint32_t w[KS], x[KS];
-            load_keys(16 * j, w);
-            load_keys(16 * j + 8, x);
+            load_key<D>(kt + k_off + 16 * j * D, w);
+            load_key<D>(kt + k_off + (16 * j + 8) * D, x);
 #pragma unroll
             for (int k = 0; k < KS; ++k) {
               uint32_t a[4];
@@ -358,18 +322,7 @@ paged_attn_kernel(const AttnArgs A, const __grid_constant__ CUtensorMap tm_k, co
 #pragma unroll
           for (int i = 0; i < TS; ++i)
 #pragma unroll
-            for (int r = 0; r < 4; ++r) {
-              const uint32_t a = vt + v_off[r & 1] + (16 * i + 8 * (r >> 1)) * D;
-              if constexpr (D == 128) {
-                const uint4 t = lds128(a);
-                vw[i][r][0] = t.x; vw[i][r][1] = t.y; vw[i][r][2] = t.z; vw[i][r][3] = t.w;
-              } else if constexpr (D == 64) {
-                const uint2 t = lds64(a);
-                vw[i][r][0] = t.x; vw[i][r][1] = t.y;
-              } else {
-                vw[i][r][0] = lds32(a);
-              }
-            }
+            for (int r = 0; r < 4; ++r) load_value<D>(vt + v_off[r & 1] + (16 * i + 8 * (r >> 1)) * D, vw[i][r]);
         };
         if constexpr (R == 8) load_values();  // on their way while the softmax runs; R = 16 has no registers for that
         // ---- masks: behind a row's keys, and pages that were not loaded ----
@@ -395,8 +348,8 @@ paged_attn_kernel(const AttnArgs A, const __grid_constant__ CUtensorMap tm_k, co
           vref = __shfl_sync(0xffffffffu, my_scl, pg0 + NP);
 #pragma unroll
           for (int i = 0; i < TS; ++i) {
-            f0[i] = fmaxf(ks * rs0, 1.17549435e-38f);                 // 0 would turn -inf into NaN
-            f1[i] = fmaxf(ks * rs1, 1.17549435e-38f);
+            f0[i] = fmaxf(ks * rs0, kTiny);
+            f1[i] = fmaxf(ks * rs1, kTiny);
             lrel[i] = 0.f;
             irel[i] = 1.f;
           }
@@ -406,8 +359,8 @@ paged_attn_kernel(const AttnArgs A, const __grid_constant__ CUtensorMap tm_k, co
           for (int i = 0; i < TS; ++i) {
             const int pg = pg0 + ((i * 16) >> box_log);
             const float ks = __shfl_sync(0xffffffffu, my_scl, pg);
-            f0[i] = fmaxf(ks * rs0, 1.17549435e-38f);
-            f1[i] = fmaxf(ks * rs1, 1.17549435e-38f);
+            f0[i] = fmaxf(ks * rs0, kTiny);
+            f1[i] = fmaxf(ks * rs1, kTiny);
             irel[i] = __shfl_sync(0xffffffffu, my_scl, pg + NP);
             vref = fmaxf(vref, irel[i]);
           }
@@ -703,29 +656,23 @@ __global__ void __launch_bounds__(256) paged_attn_join_kernel(const AttnArgs A) 
 
 // Many rows to a key head (prompts, pieces of prompts): bound by the products.
 //
-// A block takes 16 MT rows a warp of one sequence and key head; its warps
-// share copies of 64 keys that warp 0 has TMA load two copies ahead. The
-// fragments of a tile are converted once for the MT row tiles of a warp;
-// queries wait in shared memory in the order of their fragments, which leaves
-// registers for three (d = 32: four) blocks an SM. Value scales are taken
-// relative to the largest of all pages that the block reads, so that products
-// go straight into the output; the output is scaled only when some row's
-// maximum has grown by more than 2^8 (probabilities are held as 2^7 p and
-// reach 2^15). Blocks with many keys come first.
-template <int D> struct Many;
-template <> struct Many<32> { static constexpr int MT = 2, TK = 32, ST = 4, PER_SM = 4; };
-template <> struct Many<64> { static constexpr int MT = 2, TK = 32, ST = 4, PER_SM = 3; };
-template <> struct Many<128> { static constexpr int MT = 1, TK = 32, ST = 3, PER_SM = 3; };
+// A block takes 64 rows, 16 a warp, of one sequence and key head; its warps
+// share copies of 64 keys that warp 0 has TMA load a copy ahead. Queries wait
+// in shared memory in the order of their fragments, which leaves registers for
+// three blocks an SM. Value scales are taken relative to the largest of all
+// pages that the block reads, so that products go straight into the output;
+// the output is scaled only when some row's maximum has grown by more than 2^8
+// (probabilities are held as 2^7 p and reach 2^15). Blocks with many keys come
+// first.
+constexpr int kManyRows = 16 * kWarps, kManyCopies = 3;
 
-template <int D>
-__global__ void __launch_bounds__(kWarps * 32, Many<D>::PER_SM)
+__global__ void __launch_bounds__(kWarps * 32, 3)
 paged_attn_many_kernel(const AttnArgs A, const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v) {
-  constexpr int MT = Many<D>::MT, TK = Many<D>::TK, ST = Many<D>::ST;
-  constexpr int R = 16 * MT * kWarps;
+  constexpr int D = 128, TK = 32, ST = kManyCopies, R = kManyRows;
   constexpr int KS = D / 16, NT = TK / 8, TS = TK / 16, NO = D / 8;
   constexpr int kHalf = kUnit * D;
   extern __shared__ __align__(1024) uint8_t s_ring[];       // [ST] copies: 64 rows of keys, 64 rows of values
-  __shared__ uint4 s_q[kWarps][MT][KS][32];
+  __shared__ uint4 s_q[kWarps][KS][32];
   __shared__ uint64_t s_full[ST], s_empty[ST];
   __shared__ float s_ks[ST][4], s_lv[ST][4];                // scales of a copy's pages: keys, log2 of values' (relative)
   __shared__ uint32_t s_gone[ST];
@@ -821,78 +768,48 @@ paged_attn_many_kernel(const AttnArgs A, const __grid_constant__ CUtensorMap tm_
 
   // ---- rows ----
   const int g = lane >> 2, qd = lane & 3;
-  const int w0 = r0 + warp * 16 * MT;                       // this warp's first row
-  float rs[MT][2];
-  int lims[MT][2];
+  const int w0 = r0 + warp * 16;            // this warp's first row
+  float rs[2];                              // softmax scale of rows g and g + 8, in the log2 domain
+  int lims[2];
   int min_lim, max_lim;
   {
     constexpr int E = D / 4;
+    float x[2][E];
 #pragma unroll
-    for (int t = 0; t < MT; ++t) {
-      float x[2][E];
+    for (int i = 0; i < 2; ++i) {
+      const int r = w0 + 8 * i + g;
+      const bool live = r < rows;
+      const int qi = live ? r / A.G : 0;
+      const uint16_t* src = static_cast<const uint16_t*>(A.q) +
+                            (A.cu ? int64_t(S.tok0 + qi) * A.q_ts : int64_t(b) * A.q_bs + int64_t(qi) * A.q_ts) +
+                            int64_t(h * A.G + (live ? r - qi * A.G : 0)) * A.q_hs + qd * E;
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const int r = w0 + 16 * t + 8 * i + g;
-        const bool live = r < rows;
-        const int qi = live ? r / A.G : 0;
-        const uint16_t* src = static_cast<const uint16_t*>(A.q) +
-                              (A.cu ? int64_t(S.tok0 + qi) * A.q_ts : int64_t(b) * A.q_bs + int64_t(qi) * A.q_ts) +
-                              int64_t(h * A.G + (live ? r - qi * A.G : 0)) * A.q_hs + qd * E;
+      for (int e = 0; e < E; ++e) x[i][e] = 0.f;
+      if (live) load_row<E>(src, A.bf16, x[i]);
+      float amax = 0.f;
 #pragma unroll
-        for (int e = 0; e < E; ++e) x[i][e] = 0.f;
-        if (live) {
-          if (reinterpret_cast<uintptr_t>(src) % 16 == 0) {
+      for (int e = 0; e < E; ++e) amax = fmaxf(amax, fabsf(x[i][e]));
+      amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+      amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
+      const float up = row_scale(amax, A.scale_log2, rs[i]);
+      lims[i] = !live ? 0 : A.causal ? max(0, S.len - S.n + qi + 1) : S.len;
 #pragma unroll
-            for (int e = 0; e < E; e += 8) load8_16(src + e, A.bf16, &x[i][e]);
-          } else {
-#pragma unroll
-            for (int e = 0; e < E; ++e) x[i][e] = to_f_16(src[e], A.bf16);
-          }
-        }
-        float amax = 0.f;
-#pragma unroll
-        for (int e = 0; e < E; ++e) amax = fmaxf(amax, fabsf(x[i][e]));
-        amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
-        amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
-        const int ex = amax > 0.f && amax < INFINITY ? max(-100, (__float_as_int(amax) >> 23) - 127) : 14;
-        const float up = copysignf(__int_as_float((14 - ex + 127) << 23), A.scale_log2);
-        rs[t][i] = __int_as_float((ex - 14 + 127) << 23) * fabsf(A.scale_log2);
-        lims[t][i] = !live ? 0 : A.causal ? max(0, S.len - S.n + qi + 1) : S.len;
-#pragma unroll
-        for (int e = 0; e < E; ++e) x[i][e] *= up;
-      }
-#pragma unroll
-      for (int k = 0; k < KS; ++k)
-        s_q[warp][t][k][lane] = make_uint4(pack_f16(x[0][4 * k], x[0][4 * k + 1]), pack_f16(x[1][4 * k], x[1][4 * k + 1]),
-                                           pack_f16(x[0][4 * k + 2], x[0][4 * k + 3]),
-                                           pack_f16(x[1][4 * k + 2], x[1][4 * k + 3]));
+      for (int e = 0; e < E; ++e) x[i][e] *= up;
     }
+#pragma unroll
+    for (int k = 0; k < KS; ++k)
+      s_q[warp][k][lane] = make_uint4(pack_f16(x[0][4 * k], x[0][4 * k + 1]), pack_f16(x[1][4 * k], x[1][4 * k + 1]),
+                                      pack_f16(x[0][4 * k + 2], x[0][4 * k + 3]),
+                                      pack_f16(x[1][4 * k + 2], x[1][4 * k + 3]));
     min_lim = A.causal ? S.len - S.n + w0 / A.G + 1 : S.len;
-    const int wl = min(w0 + 16 * MT, rows) - 1;             // this warp's last row
+    const int wl = min(w0 + 16, rows) - 1;                  // this warp's last row
     max_lim = wl < w0 ? 0 : A.causal ? max(0, S.len - S.n + wl / A.G + 1) : S.len;
   }
   uint32_t k_off, v_off[2];
-  if (D == 128) {
-    k_off = g * 128 + ((2 * qd) ^ g) * 16;
-    v_off[0] = (2 * qd) * 128 + (g ^ (2 * qd)) * 16;
-    v_off[1] = (2 * qd + 1) * 128 + (g ^ (2 * qd + 1)) * 16;
-  } else if (D == 64) {
-    k_off = g * 64 + (qd ^ (g >> 1)) * 16;
-    v_off[0] = (2 * qd) * 64 + ((g >> 1) ^ qd) * 16 + (g & 1) * 8;
-    v_off[1] = v_off[0] + 64;
-  } else {
-    k_off = g * 32 + ((qd >> 1) ^ (g >> 2)) * 16 + (qd & 1) * 8;
-    v_off[0] = (2 * qd) * 32 + ((g >> 2) ^ (qd >> 1)) * 16 + (g & 3) * 4;
-    v_off[1] = v_off[0] + 32;
-  }
-  float o[MT][NO][4], m[MT][2], l[MT][2];
+  lane_offsets<D>(g, qd, k_off, v_off);
+  float o[NO][4], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
 #pragma unroll
-  for (int t = 0; t < MT; ++t) {
-    m[t][0] = m[t][1] = -INFINITY;
-    l[t][0] = l[t][1] = 0.f;
-#pragma unroll
-    for (int u = 0; u < NO; ++u) o[t][u][0] = o[t][u][1] = o[t][u][2] = o[t][u][3] = 0.f;
-  }
+  for (int u = 0; u < NO; ++u) o[u][0] = o[u][1] = o[u][2] = o[u][3] = 0.f;
   uint32_t st = 0, phase = 0;
 #pragma unroll 1
   for (int u = 0; u < units; ++u) {
@@ -909,40 +826,26 @@ paged_attn_many_kernel(const AttnArgs A, const __grid_constant__ CUtensorMap tm_
       if (k0 >= max_lim) break;
       const uint32_t kt = ring + st * 2 * kHalf + sub * TK * D, vt = kt + kHalf;
       // ---- scores ----
-      float s[MT][NT][4];
+      float s[NT][4];
       {
-      uint32_t qf[MT][KS][4];
-#pragma unroll
-      for (int t = 0; t < MT; ++t)
+        uint32_t qf[KS][4];
 #pragma unroll
         for (int k = 0; k < KS; ++k) {
-          const uint4 v = lds128(smem_u32(&s_q[warp][t][k][lane]));
-          qf[t][k][0] = v.x; qf[t][k][1] = v.y; qf[t][k][2] = v.z; qf[t][k][3] = v.w;
+          const uint4 v = lds128(smem_u32(&s_q[warp][k][lane]));
+          qf[k][0] = v.x; qf[k][1] = v.y; qf[k][2] = v.z; qf[k][3] = v.w;
         }
 #pragma unroll
-      for (int j = 0; j < NT; ++j) {
-        uint32_t w[KS];
-        if constexpr (D == 128) {
-          const uint4 a = lds128(kt + k_off + 8 * j * D), c = lds128(kt + (k_off ^ 16) + 8 * j * D);
-          w[0] = a.x; w[1] = a.y; w[2] = a.z; w[3] = a.w;
-          w[4] = c.x; w[5] = c.y; w[6] = c.z; w[7] = c.w;
-        } else if constexpr (D == 64) {
-          const uint4 a = lds128(kt + k_off + 8 * j * D);
-          w[0] = a.x; w[1] = a.y; w[2] = a.z; w[3] = a.w;
-        } else {
-          const uint2 a = lds64(kt + k_off + 8 * j * D);
-          w[0] = a.x; w[1] = a.y;
-        }
+        for (int j = 0; j < NT; ++j) {
+          uint32_t w[KS];
+          load_key<D>(kt + k_off + 8 * j * D, w);
 #pragma unroll
-        for (int k = 0; k < KS; ++k) {
-          uint32_t b0, b1;
-          cvt4(w[k], b0, b1);
-#pragma unroll
-          for (int t = 0; t < MT; ++t)
-            if (k == 0) mma_f16_0(s[t][j], qf[t][k], b0, b1);
-            else mma_f16(s[t][j], qf[t][k], b0, b1);
+          for (int k = 0; k < KS; ++k) {
+            uint32_t b0, b1;
+            cvt4(w[k], b0, b1);
+            if (k == 0) mma_f16_0(s[j], qf[k], b0, b1);
+            else mma_f16(s[j], qf[k], b0, b1);
+          }
         }
-      }
       }
       // ---- masks ----
       const int end = min(TK, max_lim - k0);                // keys of the tile that some row of the warp sees
@@ -955,11 +858,8 @@ paged_attn_many_kernel(const AttnArgs A, const __grid_constant__ CUtensorMap tm_
           for (int e = 0; e < 2; ++e) {
             const int at = sub * TK + 8 * j + 2 * qd + e, key = u * kUnit + at;
             const bool drop = all_gone >> (at >> A.logP) & 1;
-#pragma unroll
-            for (int t = 0; t < MT; ++t) {
-              if (drop || key >= lims[t][0]) s[t][j][e] = -INFINITY;
-              if (drop || key >= lims[t][1]) s[t][j][2 + e] = -INFINITY;
-            }
+            if (drop || key >= lims[0]) s[j][e] = -INFINITY;
+            if (drop || key >= lims[1]) s[j][2 + e] = -INFINITY;
           }
       }
       // ---- scores of the pages: maxima in the log2 domain ----
@@ -972,56 +872,49 @@ paged_attn_many_kernel(const AttnArgs A, const __grid_constant__ CUtensorMap tm_
         iv[i] = exp2f_approx(-lv[i]);
       }
       bool grows = false;
-      float x[MT][2];
+      float x[2];
 #pragma unroll
-      for (int t = 0; t < MT; ++t)
+      for (int i = 0; i < 2; ++i) {
+        float y = -INFINITY;
+#pragma unroll
+        for (int k = 0; k < TS; ++k)
+          y = fmaxf(y, fmaxf(fmaxf(s[2 * k][2 * i], s[2 * k][2 * i + 1]), fmaxf(s[2 * k + 1][2 * i], s[2 * k + 1][2 * i + 1])) *
+                           fmaxf(ks[k] * rs[i], kTiny));
+        y = fmaxf(y, __shfl_xor_sync(0xffffffffu, y, 1));
+        y = fmaxf(y, __shfl_xor_sync(0xffffffffu, y, 2));
+        x[i] = y;
+        grows |= y > m[i] + 8.f;
+      }
+      if (__any_sync(0xffffffffu, grows)) {
+        float al[2];
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-          float y = -INFINITY;
-#pragma unroll
-          for (int k = 0; k < TS; ++k)
-            y = fmaxf(y, fmaxf(fmaxf(s[t][2 * k][2 * i], s[t][2 * k][2 * i + 1]),
-                               fmaxf(s[t][2 * k + 1][2 * i], s[t][2 * k + 1][2 * i + 1])) *
-                             fmaxf(ks[k] * rs[t][i], 1.17549435e-38f));
-          y = fmaxf(y, __shfl_xor_sync(0xffffffffu, y, 1));
-          y = fmaxf(y, __shfl_xor_sync(0xffffffffu, y, 2));
-          x[t][i] = y;
-          grows |= y > m[t][i] + 8.f;
+          const float n = x[i] > m[i] + 8.f ? x[i] : m[i];
+          al[i] = m[i] == n ? 1.f : exp2f_approx(m[i] - n);
+          m[i] = n;
+          l[i] *= al[i];
         }
-      if (__any_sync(0xffffffffu, grows)) {
 #pragma unroll
-        for (int t = 0; t < MT; ++t) {
-          float al[2];
-#pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            const float n = x[t][i] > m[t][i] + 8.f ? x[t][i] : m[t][i];
-            al[i] = m[t][i] == n ? 1.f : exp2f_approx(m[t][i] - n);
-            m[t][i] = n;
-            l[t][i] *= al[i];
-          }
-#pragma unroll
-          for (int v = 0; v < NO; ++v) {
-            o[t][v][0] *= al[0];
-            o[t][v][1] *= al[0];
-            o[t][v][2] *= al[1];
-            o[t][v][3] *= al[1];
-          }
+        for (int v = 0; v < NO; ++v) {
+          o[v][0] *= al[0];
+          o[v][1] *= al[0];
+          o[v][2] *= al[1];
+          o[v][3] *= al[1];
         }
       }
       // ---- probabilities (times 2^7 and the page's relative value scale) and their sum ----
-      uint32_t pf[MT][TS][4];
-#pragma unroll
-      for (int t = 0; t < MT; ++t) {
-        const float z0 = 7.f - (m[t][0] == -INFINITY ? 0.f : m[t][0]), z1 = 7.f - (m[t][1] == -INFINITY ? 0.f : m[t][1]);
+      uint32_t pf[TS][4];
+      {
+        const float z0 = 7.f - (m[0] == -INFINITY ? 0.f : m[0]), z1 = 7.f - (m[1] == -INFINITY ? 0.f : m[1]);
         uint64_t sum0 = pk2(0.f, 0.f), sum1 = pk2(0.f, 0.f);
 #pragma unroll
         for (int i = 0; i < TS; ++i) {
-          const uint64_t fa = pk2s(fmaxf(ks[i] * rs[t][0], 1.17549435e-38f)), za = pk2s(z0 + lv[i]);
-          const uint64_t fb = pk2s(fmaxf(ks[i] * rs[t][1], 1.17549435e-38f)), zb = pk2s(z1 + lv[i]);
+          const uint64_t fa = pk2s(fmaxf(ks[i] * rs[0], kTiny)), za = pk2s(z0 + lv[i]);
+          const uint64_t fb = pk2s(fmaxf(ks[i] * rs[1], kTiny)), zb = pk2s(z1 + lv[i]);
           uint64_t pa, pb;
 #pragma unroll
           for (int c = 0; c < 2; ++c) {
-            const float* sj = s[t][2 * i + c];
+            const float* sj = s[2 * i + c];
             float p0, p1, p2, p3;
             pk2_split(pk2_fma(pk2(sj[0], sj[1]), fa, za), p0, p1);
             pk2_split(pk2_fma(pk2(sj[2], sj[3]), fb, zb), p2, p3);
@@ -1031,35 +924,24 @@ paged_attn_many_kernel(const AttnArgs A, const __grid_constant__ CUtensorMap tm_
             p3 = exp2f_approx(p3);
             pa = c == 0 ? pk2(p0, p1) : pk2_add(pa, pk2(p0, p1));
             pb = c == 0 ? pk2(p2, p3) : pk2_add(pb, pk2(p2, p3));
-            pf[t][i][2 * c] = pack_f16(p0, p1);
-            pf[t][i][2 * c + 1] = pack_f16(p2, p3);
+            pf[i][2 * c] = pack_f16(p0, p1);
+            pf[i][2 * c + 1] = pack_f16(p2, p3);
           }
           sum0 = pk2_fma(pa, pk2s(iv[i]), sum0);
           sum1 = pk2_fma(pb, pk2s(iv[i]), sum1);
         }
         float a0, a1;
         pk2_split(sum0, a0, a1);
-        l[t][0] += a0 + a1;
+        l[0] += a0 + a1;
         pk2_split(sum1, a0, a1);
-        l[t][1] += a0 + a1;
+        l[1] += a0 + a1;
       }
       // ---- values: what lies behind the keys may be anything, NaN too ----
 #pragma unroll
       for (int i = 0; i < TS; ++i) {
         uint32_t vw[4][D / 32];
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const uint32_t a = vt + v_off[r & 1] + (16 * i + 8 * (r >> 1)) * D;
-          if constexpr (D == 128) {
-            const uint4 c = lds128(a);
-            vw[r][0] = c.x; vw[r][1] = c.y; vw[r][2] = c.z; vw[r][3] = c.w;
-          } else if constexpr (D == 64) {
-            const uint2 c = lds64(a);
-            vw[r][0] = c.x; vw[r][1] = c.y;
-          } else {
-            vw[r][0] = lds32(a);
-          }
-        }
+        for (int r = 0; r < 4; ++r) load_value<D>(vt + v_off[r & 1] + (16 * i + 8 * (r >> 1)) * D, vw[r]);
         if (hole || end < TK) {
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
@@ -1077,9 +959,7 @@ paged_attn_many_kernel(const AttnArgs A, const __grid_constant__ CUtensorMap tm_
           cvt4(__byte_perm(vw[2][w], vw[3][w], 0x5140), b1[0], b1[1]);
           cvt4(__byte_perm(vw[2][w], vw[3][w], 0x7362), b1[2], b1[3]);
 #pragma unroll
-          for (int e = 0; e < 4; ++e)
-#pragma unroll
-            for (int t = 0; t < MT; ++t) mma_f16(o[t][4 * w + e], pf[t][i], b0[e], b1[e]);
+          for (int e = 0; e < 4; ++e) mma_f16(o[4 * w + e], pf[i], b0[e], b1[e]);
         }
       }
     }
@@ -1092,27 +972,25 @@ paged_attn_many_kernel(const AttnArgs A, const __grid_constant__ CUtensorMap tm_
     }
   }
 #pragma unroll
-  for (int t = 0; t < MT; ++t)
+  for (int i = 0; i < 2; ++i) {
+    float sum = l[i];
+    sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+    sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+    const int r = w0 + 8 * i + g;
+    if (r >= rows) continue;
+    const int qi = r / A.G;
+    const int64_t at = int64_t(S.tok0 + qi) * A.Hq + h * A.G + (r - qi * A.G);
+    const float inv = sum == 0.f ? 0.f : top / sum;         // a sum of 0: no keys. A NaN stays one
+    uint16_t* dst = static_cast<uint16_t*>(A.o) + at * D + qd * (D / 4);
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      float sum = l[t][i];
-      sum += __shfl_xor_sync(0xffffffffu, sum, 1);
-      sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-      const int r = w0 + 16 * t + 8 * i + g;
-      if (r >= rows) continue;
-      const int qi = r / A.G;
-      const int64_t at = int64_t(S.tok0 + qi) * A.Hq + h * A.G + (r - qi * A.G);
-      const float inv = sum == 0.f ? 0.f : top / sum;       // a sum of 0: no keys. A NaN stays one
-      uint16_t* dst = static_cast<uint16_t*>(A.o) + at * D + qd * (D / 4);
+    for (int c = 0; c < 2; ++c)
 #pragma unroll
-      for (int c = 0; c < 2; ++c)
-#pragma unroll
-        for (int u = 0; u < NO; u += 4)
-          *reinterpret_cast<uint2*>(dst + c * NO + u) =
-              make_uint2(pack_16(o[t][u][2 * i + c] * inv, o[t][u + 1][2 * i + c] * inv, A.bf16),
-                         pack_16(o[t][u + 2][2 * i + c] * inv, o[t][u + 3][2 * i + c] * inv, A.bf16));
-      if (A.lse && qd == 0) A.lse[at] = sum == 0.f ? -INFINITY : (m[t][i] - 7.f + log2f(sum)) * 0.6931471805599453f;
-    }
+      for (int u = 0; u < NO; u += 4)
+        *reinterpret_cast<uint2*>(dst + c * NO + u) =
+            make_uint2(pack_16(o[u][2 * i + c] * inv, o[u + 1][2 * i + c] * inv, A.bf16),
+                       pack_16(o[u + 2][2 * i + c] * inv, o[u + 3][2 * i + c] * inv, A.bf16));
+    if (A.lse && qd == 0) A.lse[at] = sum == 0.f ? -INFINITY : (m[i] - 7.f + log2f(sum)) * 0.6931471805599453f;
+  }
 }
 
 template <int D, int R, int W>
@@ -1124,9 +1002,11 @@ static void few_launch(AttnArgs& A, const at::Tensor& ck, const at::Tensor& cv, 
   const int64_t slots = int64_t(num_sms()) * blocks_per_sm(kern, kWarps * 32, kSmem, known);
   const int64_t segments = U.B * A.H * ((U.rows + R - 1) / R);
   const int64_t units = std::max<int64_t>(1, (U.len + SUP - 1) / SUP);        // of the longest segment
-  // A unit takes a block about 1 us and the second launch about 4: pieces of 4 units at least, of segments of 9 at least
-  A.min_units = 4;
-  A.split = W > 1 && segments < slots * 8 && units > 2 * A.min_units;
+  // Shares of units instead of whole segments: the second launch and the pieces cost about 4 us, a unit about 1.2 us
+  // of its block. d = 64, 8 key heads, us without / with: one sequence of 500 keys 10.5 / 11.4, of 1000 12.4 / 12.4, of
+  // 2000 18.0 / 12.3; 64 of 2000 41.1 / 35.0; 512 ragged up to 2000 160 / 145. Pieces of 2 units (4: 2 us more).
+  A.min_units = 2;
+  A.split = W > 1 && units > 4;
   const int64_t most = A.split ? (segments * units + A.min_units - 1) / A.min_units : (segments * W + kWarps - 1) / kWarps;
   const int grid = int(std::min<int64_t>(slots, most));
   at::Tensor part;
@@ -1155,30 +1035,59 @@ static void few_launch(AttnArgs& A, const at::Tensor& ck, const at::Tensor& cv, 
   }
 }
 
-template <int D>
+template <int D, int R>
+static void few_dispatch(AttnArgs& A, const at::Tensor& ck, const at::Tensor& cv, const Bounds& U) {
+  // A warp a segment needs no merge, but pays where warps stay without one or sequences differ. R = 8, us with 4 warps
+  // a segment / with one: 1000 keys, d = 64: 2368 segments 74 / 82, 4736 130 / 121, 18944 489 / 429; d = 32: 101 / 91 and
+  // 375 / 313 (4736, 18944); d = 128 level. Keys of one unit, d = 32 (200): 592 14.4 / 12.4, 2368 33 / 25, 9472 113 / 66.
+  constexpr int SUP = Cfg<D>::TK * Cfg<D>::SUB * kWarps;
+  const int64_t segments = U.B * A.H * ((U.rows + R - 1) / R), warps = int64_t(num_sms()) * 12;
+  const int64_t rounds = (segments + warps - 1) / warps;
+  const bool one = U.len <= SUP ? segments >= int64_t(num_sms()) * 8 : rounds >= 3 && segments * 20 >= rounds * warps * 17;
+  if (one) few_launch<D, R, 1>(A, ck, cv, U);
+  else few_launch<D, R, 4>(A, ck, cv, U);
+}
+
 static void many_launch(AttnArgs& A, const at::Tensor& ck, const at::Tensor& cv, const Bounds& U) {
-  constexpr int kSmem = Many<D>::ST * 2 * kUnit * D;
-  constexpr int R = 16 * Many<D>::MT * kWarps;
+  constexpr int kSmem = kManyCopies * 2 * kUnit * 128;
   static int known[64] = {};
-  auto kern = paged_attn_many_kernel<D>;
-  blocks_per_sm(kern, kWarps * 32, kSmem, known);
-  const dim3 grid(unsigned(U.B * A.H), unsigned((U.rows + R - 1) / R));
-  kern<<<grid, kWarps * 32, kSmem, stream()>>>(A, code_map(ck, A.P), code_map(cv, A.P));
+  blocks_per_sm(paged_attn_many_kernel, kWarps * 32, kSmem, known);
+  const dim3 grid(unsigned(U.B * A.H), unsigned((U.rows + kManyRows - 1) / kManyRows));
+  paged_attn_many_kernel<<<grid, kWarps * 32, kSmem, stream()>>>(A, code_map(ck, A.P), code_map(cv, A.P));
   PD_CHECK_LAUNCH();
+}
+
+// The forms for many rows (tcgen05 for d = 32 and 64, shared copies for d = 128) do not split the keys, the form for
+// few rows reads them again for every 16 rows. Which is faster is estimated in us from what they measured:
+//   few   15 + (16-row tiles x keys) / 63e3, 40e3, 21e3 (d = 32, 64, 128)
+//   many  waves of blocks x (5 + 64-key units x time of one), a unit 0.85 (tcgen05) or 2.4 with an SM to itself, 1.5 or
+//         3.7 where two or three blocks share one
+// d = 64, us few / tcgen05: 40 sequences x 8 heads over 1000 keys: 64 rows 43 / 47, 96 rows 70 / 47, 256 rows 122 / 64;
+// one of 1824 x 16 heads 95 / 38; four of 128 rows over 4000 45 / 62; one of 512 over 16000 63 / 215.
+// d = 128, few / many: 40 x 8 x 64 rows over 1000 92 / 64, 2 x 8 x 512 over 8000 204 / 287.
+template <int D>
+static bool use_many(const AttnArgs& A, const Bounds& U) {
+  if (U.rows <= 16) return false;
+  constexpr int rows = D <= 64 ? 128 : kManyRows, per_sm = D <= 64 ? 2 : 3;
+  const int64_t tiles = (U.rows + rows - 1) / rows;
+  if (tiles > 65535 || U.B * A.H >= (int64_t(1) << 31)) return false;
+  const double blocks = double(U.B * A.H) * double(tiles), units = double((U.len + kUnit - 1) / kUnit);
+  const double few = 15. + double(U.B * A.H) * double((U.rows + 15) / 16) * double(U.len) /
+                               (D == 32 ? 63e3 : D == 64 ? 40e3 : 21e3);
+  const double unit = D <= 64 ? (blocks <= num_sms() ? 0.85 : 1.5) : (blocks <= num_sms() ? 2.4 : 3.7);
+  return std::ceil(blocks / (num_sms() * per_sm)) * (5. + units * unit) < few;
 }
 
 template <int D>
 static void attn_dispatch(AttnArgs& A, const at::Tensor& ck, const at::Tensor& cv, const Bounds& U) {
-  // a warp a segment where there are eight segments and more for every warp of the device (12 warps an SM)
-  const bool many = U.B * A.H * ((U.rows + 15) / 16) >= int64_t(num_sms()) * 12 * 4;
-  const int64_t tiles = (U.rows + 16 * Many<D>::MT * kWarps - 1) / (16 * Many<D>::MT * kWarps);
-  if (U.rows > 32 && U.B * A.H * tiles >= num_sms() && tiles < 65536 && U.B * A.H < (int64_t(1) << 31)) {
-    if constexpr (D <= 64)
-      if (U.rows > 64) return attn_tc_launch(A, ck, cv, D, U);
-    return many_launch<D>(A, ck, cv, U);
+  if (use_many<D>(A, U)) {
+    if constexpr (D <= 64) attn_tc_launch(A, ck, cv, D, U);
+    else many_launch(A, ck, cv, U);
+  } else if (U.rows <= 8) {
+    few_dispatch<D, 8>(A, ck, cv, U);
+  } else {
+    few_dispatch<D, 16>(A, ck, cv, U);
   }
-  if (U.rows <= 8) return many ? few_launch<D, 8, 1>(A, ck, cv, U) : few_launch<D, 8, 4>(A, ck, cv, U);
-  return many ? few_launch<D, 16, 1>(A, ck, cv, U) : few_launch<D, 16, 4>(A, ck, cv, U);
 }
 
 // (o, lse): lse is an undefined tensor unless asked for.

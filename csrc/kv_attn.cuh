@@ -111,6 +111,73 @@ __device__ __forceinline__ void load8_16(const uint16_t* p, bool bf16, float* f)
     f[2 * i + 1] = to_f_16(uint16_t(w[i] >> 16), bf16);
   }
 }
+// n elements of a query row, at any alignment
+template <int N>
+__device__ __forceinline__ void load_row(const uint16_t* p, bool bf16, float* f) {
+  if (reinterpret_cast<uintptr_t>(p) % 16 == 0) {
+#pragma unroll
+    for (int e = 0; e < N; e += 8) load8_16(p + e, bf16, f + e);
+  } else {
+#pragma unroll
+    for (int e = 0; e < N; ++e) f[e] = to_f_16(p[e], bf16);
+  }
+}
+// The power of two that brings a row's largest magnitude to [2^14, 2^15), negative for a negative softmax scale, and in
+// `back` what undoes it times the softmax scale. A row of zeros, an infinity or NaN stays as it is.
+__device__ __forceinline__ float row_scale(float amax, float scale_log2, float& back) {
+  const int ex = amax > 0.f && amax < INFINITY ? max(-100, (__float_as_int(amax) >> 23) - 127) : 14;
+  back = __int_as_float((ex - 14 + 127) << 23) * fabsf(scale_log2);
+  return copysignf(__int_as_float((14 - ex + 127) << 23), scale_log2);
+}
+// the least factor of scores: 0 would turn a masked score's -inf into NaN
+constexpr float kTiny = 1.17549435e-38f;
+
+// Where a lane (g = lane / 4, qd = lane % 4) finds its codes in a tile of rows of D bytes that TMA has swizzled: its
+// quarter of key row g, and its eighth of value rows 2 qd and 2 qd + 1.
+template <int D>
+__device__ __forceinline__ void lane_offsets(int g, int qd, uint32_t& k_off, uint32_t* v_off) {
+  if constexpr (D == 128) {
+    k_off = g * 128 + ((2 * qd) ^ g) * 16;
+    v_off[0] = (2 * qd) * 128 + (g ^ (2 * qd)) * 16;
+    v_off[1] = (2 * qd + 1) * 128 + (g ^ (2 * qd + 1)) * 16;
+  } else if constexpr (D == 64) {
+    k_off = g * 64 + (qd ^ (g >> 1)) * 16;
+    v_off[0] = (2 * qd) * 64 + ((g >> 1) ^ qd) * 16 + (g & 1) * 8;
+    v_off[1] = v_off[0] + 64;
+  } else {
+    k_off = g * 32 + ((qd >> 1) ^ (g >> 2)) * 16 + (qd & 1) * 8;
+    v_off[0] = (2 * qd) * 32 + ((g >> 2) ^ (qd >> 1)) * 16 + (g & 3) * 4;
+    v_off[1] = v_off[0] + 32;
+  }
+}
+// the lane's D / 4 codes of a key, a word for each step of 16 dims
+template <int D>
+__device__ __forceinline__ void load_key(uint32_t a, uint32_t* w) {
+  if constexpr (D == 128) {
+    const uint4 x = lds128(a), y = lds128(a ^ 16);
+    w[0] = x.x; w[1] = x.y; w[2] = x.z; w[3] = x.w;
+    w[4] = y.x; w[5] = y.y; w[6] = y.z; w[7] = y.w;
+  } else if constexpr (D == 64) {
+    const uint4 x = lds128(a);
+    w[0] = x.x; w[1] = x.y; w[2] = x.z; w[3] = x.w;
+  } else {
+    const uint2 x = lds64(a);
+    w[0] = x.x; w[1] = x.y;
+  }
+}
+// the lane's D / 8 codes of a value
+template <int D>
+__device__ __forceinline__ void load_value(uint32_t a, uint32_t* w) {
+  if constexpr (D == 128) {
+    const uint4 x = lds128(a);
+    w[0] = x.x; w[1] = x.y; w[2] = x.z; w[3] = x.w;
+  } else if constexpr (D == 64) {
+    const uint2 x = lds64(a);
+    w[0] = x.x; w[1] = x.y;
+  } else {
+    w[0] = lds32(a);
+  }
+}
 __device__ __forceinline__ uint32_t pack_16(float lo, float hi, bool bf16) {
   if (bf16) {
     const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);

@@ -336,21 +336,11 @@ paged_attn_tc_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__
       float x[D];
 #pragma unroll
       for (int e = 0; e < D; ++e) x[e] = 0.f;
-      if (live) {
-        if (reinterpret_cast<uintptr_t>(src) % 16 == 0) {
-#pragma unroll
-          for (int e = 0; e < D; e += 8) load8_16(src + e, A.bf16, &x[e]);
-        } else {
-#pragma unroll
-          for (int e = 0; e < D; ++e) x[e] = to_f_16(src[e], A.bf16);
-        }
-      }
+      if (live) load_row<D>(src, A.bf16, x);
       float amax = 0.f;
 #pragma unroll
       for (int e = 0; e < D; ++e) amax = fmaxf(amax, fabsf(x[e]));
-      const int ex = amax > 0.f && amax < INFINITY ? max(-100, (__float_as_int(amax) >> 23) - 127) : 14;
-      const float up = copysignf(__int_as_float((14 - ex + 127) << 23), A.scale_log2);
-      rs = __int_as_float((ex - 14 + 127) << 23) * fabsf(A.scale_log2);
+      const float up = row_scale(amax, A.scale_log2, rs);
 #pragma unroll
       for (int c = 0; c < D / 8; ++c)
         asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(sQ + Op<D>::chunk(r, c)),
@@ -390,7 +380,7 @@ paged_attn_tc_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const int pg = (16 * i) >> A.logP;
-        f[i] = fmaxf(s_ks[e][pg] * rs, 1.17549435e-38f);    // 0 would turn -inf into NaN
+        f[i] = fmaxf(s_ks[e][pg] * rs, kTiny);
         lv[i] = s_lv[e][pg];
         float y0 = -INFINITY, y1 = -INFINITY;
 #pragma unroll

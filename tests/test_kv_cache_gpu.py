@@ -263,10 +263,10 @@ def test_attention_ragged(P, d, H, G, lens, new):
 @pytest.mark.parametrize("causal", [True, False])
 @pytest.mark.parametrize("P,d,H,G,most", [(64, 64, 4, 1, 300), (16, 64, 2, 3, 90), (32, 32, 4, 2, 130), (64, 32, 2, 1, 200),
                                           (16, 32, 8, 1, 65), (64, 128, 4, 1, 150), (32, 128, 2, 2, 70), (16, 128, 8, 1, 40),
-                                          (32, 64, 8, 1, 40), (64, 32, 8, 1, 33)])
+                                          (32, 64, 8, 1, 40), (64, 32, 8, 1, 33), (64, 32, 4, 1, 300), (64, 128, 4, 1, 400)])
 def test_many_rows(P, d, H, G, most, causal, dtype):
-    """Enough rows and sequences for the forms that share copies among rows (more than 32 and more than 64 rows to a
-    key head, at least a block an SM), ragged, with rows without keys and empty sequences among them."""
+    """Enough rows and sequences for the forms that share copies among rows (and some just below), ragged, with rows
+    without keys and empty sequences among them."""
     g = torch.Generator(device=DEV).manual_seed(d + most)
     B = 160 // H + 3
     new = [max(1, most - (i * 37) % most) for i in range(B)]
