@@ -41,6 +41,15 @@ template <> struct Cfg<128> { static constexpr int TK = 32, SUB = 1, ST = 2; };
 // are dealt to lanes so that a lane's four codes of a step of 16 dims are
 // neighbours: lane % 4 owns a quarter of a key's dims, lane / 4 an eighth of a
 // value's, and keys go to registers in the order of memory.
+//
+// B200: 64 single tokens over 300 to 8191 keys, 32 heads over 8 x 128 (R = 8):
+// 114 us, 4.9 TB/s of the cache (floor 85 us); three over 65537 to 131071 keys, 16
+// heads over 4 x 64, pages of 16: 43 us, 3.5 TB/s (floor 23 us). Neither pipe is full (issue
+// slots 37%, DRAM 75%): 12 warps an SM, bound by registers, wait on their own
+// chains. 1024 x 16 candidate tokens behind 896 shared keys, 8 x 32 (R = 16, W =
+// 1): 140 us; the keys come from L2 and the instructions around 16-row products
+// bound it (issue 55% of active cycles; a copy's bookkeeping is 30% of them: 64
+// keys a copy instead of 128 cost 179 us).
 template <int D, int R, int W>
 __global__ void __launch_bounds__(kWarps * 32, D == 128 && R == 16 ? 2 : 3)
 paged_attn_kernel(const AttnArgs A, const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v) {
@@ -663,7 +672,9 @@ __global__ void __launch_bounds__(256) paged_attn_join_kernel(const AttnArgs A) 
 // pages that the block reads, so that products go straight into the output;
 // the output is scaled only when some row's maximum has grown by more than 2^8
 // (probabilities are held as 2^7 p and reach 2^15). Blocks with many keys come
-// first.
+// first. With 16 rows a warp every code is converted for 16 rows' products; 32
+// rows a warp need more registers than two blocks an SM leave at d = 128.
+// B200: 40 sequences x 8 heads x 256 rows over 1000 keys: 166 us (16-row form: 274).
 constexpr int kManyRows = 16 * kWarps, kManyCopies = 3;
 
 __global__ void __launch_bounds__(kWarps * 32, 3)

