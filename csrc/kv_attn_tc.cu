@@ -105,9 +105,11 @@ struct Op {
     return uint64_t((at >> 4) & 0x3FFF) | (uint64_t((lead >> 4) & 0x3FFF) << 16) |
            (uint64_t((kAtom >> 4) & 0x3FFF) << 32) | (uint64_t(1) << 46) | (kSwizzle << 61);
   }
-  // step k of 16 dims of rows (rows = M or N), and of 16 rows (rows = K, dims = N)
-  __device__ static __forceinline__ uint64_t dims(uint32_t tile, int k) { return desc(tile + k * 32, 16); }
-  __device__ static __forceinline__ uint64_t rows(uint32_t tile, int k) { return desc(tile + k * 2 * kAtom, kUnit * kRow); }
+  // Descriptors of step 0 of 16 dims (rows = M or N) and of 16 rows (rows = K, dims = N) of a tile; those of another
+  // step or tile differ by the distance in 16-byte units, whose sum stays within the 14 bits of an address.
+  __device__ static __forceinline__ uint64_t dims(uint32_t tile) { return desc(tile, 16); }
+  __device__ static __forceinline__ uint64_t rows(uint32_t tile) { return desc(tile, kUnit * kRow); }
+  static constexpr uint32_t kDims = 32 / 16, kRows = 2 * kAtom / 16, kTile = kUnit * kRow / 16;
 };
 // fp16 operands, 32-bit sums; b_mn: B's rows are its K
 constexpr uint32_t tc_id(int m, int n, int b_mn) {
@@ -246,6 +248,7 @@ paged_attn_tc_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__
       // ---------------- products ----------------
       if (lane == 0 && units > 0) {
         constexpr uint32_t id_s = tc_id(kTcRows, kUnit, 0), id_pv = tc_id(kTcRows, D, 1);
+        const uint64_t dq = Op<D>::dims(sQ), dk = Op<D>::dims(sK), dv = Op<D>::rows(sV);
         bool ok = wait(&q_full, 0);
         auto scores = [&](int t) {
           const int sl = t % kOps;
@@ -254,7 +257,7 @@ paged_attn_tc_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__
           tc_after();
 #pragma unroll
           for (int k = 0; k < D / 16; ++k)
-            mma_ss(tmem + kUnit * sl, Op<D>::dims(sQ, k), Op<D>::dims(sK + sl * kOpBytes, k), id_s, k > 0);
+            mma_ss(tmem + kUnit * sl, dq + k * Op<D>::kDims, dk + sl * Op<D>::kTile + k * Op<D>::kDims, id_s, k > 0);
           tc_commit(&s_full[sl]);
           return true;
         };
@@ -266,7 +269,7 @@ paged_attn_tc_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__
           tc_after();
 #pragma unroll
           for (int k = 0; k < kUnit / 16; ++k)
-            mma_ts(tmem + cO, tmem + kUnit * sl + 8 * k, Op<D>::rows(sV + sl * kOpBytes, k), id_pv, t > 0 || k > 0);
+            mma_ts(tmem + cO, tmem + kUnit * sl + 8 * k, dv + sl * Op<D>::kTile + k * Op<D>::kRows, id_pv, t > 0 || k > 0);
           tc_commit(&kv_empty[sl]);
           tc_commit(&pv_done[sl]);
           if (t + 1 == units) tc_commit(&o_full);
