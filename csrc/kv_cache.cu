@@ -154,6 +154,11 @@ __global__ void __launch_bounds__(kAppendThreads) append_kernel(const __grid_con
   const int per = (2 * A.H + gridDim.y - 1) / gridDim.y, u0 = blockIdx.y * per, u1 = min(2 * A.H, u0 + per);
   if (u0 >= u1) return;
   fetch(u0);
+  // where a thread has one row, its angles serve every head
+  constexpr bool kHold = PASSES == 1;
+  float held_c[8], held_s[8];
+  if (kHold && A.rope && u0 < A.H && row0 >= lo && row0 < hi && p0 + row0 < A.n_pos)
+    load_angles<8>(A.rope + (p0 + row0) * D, lane, D, A.interleaved, off0, off1, held_c, held_s);
   int buf = 0;
 #pragma unroll 1
   for (int u = u0; u < u1; ++u, buf ^= 1) {
@@ -187,9 +192,13 @@ __global__ void __launch_bounds__(kAppendThreads) append_kernel(const __grid_con
       }
       if (keys && A.rope && r >= lo && r < hi) {
         if (p0 + r < A.n_pos) {
-          float cs[8], sn[8];
-          load_angles<8>(A.rope + (p0 + r) * D, lane, D, A.interleaved, off0, off1, cs, sn);
-          turn<8>(a[ps], c[ps], cs, sn, A.interleaved, 1.f);
+          if constexpr (kHold) {
+            turn<8>(a[ps], c[ps], held_c, held_s, A.interleaved, 1.f);
+          } else {
+            float cs[8], sn[8];
+            load_angles<8>(A.rope + (p0 + r) * D, lane, D, A.interleaved, off0, off1, cs, sn);
+            turn<8>(a[ps], c[ps], cs, sn, A.interleaved, 1.f);
+          }
         } else {
           set_error(A.err, kIdOutOfRange);
 #pragma unroll
