@@ -1134,7 +1134,6 @@ std::vector<at::Tensor> paged_attention(at::Tensor q, at::Tensor ck, at::Tensor 
   A.table_stride = table.stride(0);
   A.lens = lens.data_ptr<int>();
   A.cu = cu.has_value() ? cu->data_ptr<int>() : nullptr;
-  A.n = int(qd == 4 ? q.size(1) : 0);
   A.total = int(qd == 3 ? q.size(0) : 0);
   A.B = int(B); A.Hq = int(Hq); A.H = C.H; A.G = int(Hq / C.H); A.P = C.P; A.n_pages = C.n_pages;
   A.logP = C.P == 16 ? 4 : C.P == 32 ? 5 : 6;
@@ -1153,11 +1152,15 @@ std::vector<at::Tensor> paged_attention(at::Tensor q, at::Tensor ck, at::Tensor 
   const int64_t most = qd == 4 ? q.size(1) : std::min<int64_t>(std::max<int64_t>(max_q.value_or(q.size(0)), 0), q.size(0));
   PD_CHECK((qd == 3 ? q.size(0) : B * q.size(1)) * A.G < (int64_t(1) << 31) - 128 && B < (int64_t(1) << 31),
            "too many queries");
+  A.n = int(most);
   if (B > 0 && most > 0 && q.numel() > 0) {
     const Bounds U{B, most * A.G, std::min<int64_t>(table.size(1) * C.P, std::max<int64_t>(max_len.value_or(INT64_MAX), 0))};
     if (C.d == 32) attn_dispatch<32>(A, ck, cv, U);
     else if (C.d == 64) attn_dispatch<64>(A, ck, cv, U);
     else attn_dispatch<128>(A, ck, cv, U);
+  } else {
+    o.zero_();
+    if (want_lse) lse.fill_(-INFINITY);
   }
   return want_lse ? std::vector<at::Tensor>{o, lse} : std::vector<at::Tensor>{o};
 }

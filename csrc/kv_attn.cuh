@@ -31,7 +31,8 @@ struct AttnArgs {
   const int* cu;                // [B + 1] or null
   void* o;                      // [tokens, Hq, d]
   float* lse;                   // [tokens, Hq] or null
-  int B, n, total, Hq, H, G, P, logP, max_pages, n_pages;
+  int B, n, total;              // n: queries of each sequence, with `cu` the most of one; total: rows of q
+  int Hq, H, G, P, logP, max_pages, n_pages;
   bool causal, split, bf16;
   int min_units;
   float scale_log2;
@@ -213,7 +214,7 @@ struct Seq {
     if (A.cu) {
       tok0 = __ldg(A.cu + b);
       n = __ldg(A.cu + b + 1) - tok0;
-      if (n < 0 || tok0 < 0 || tok0 > A.total - n) {
+      if (n < 0 || n > A.n || tok0 < 0 || tok0 > A.total - n) {
         set_error(A.err, kBadShape);
         n = 0;
       }

@@ -48,6 +48,8 @@ struct QkNormRope : public torch::autograd::Function<QkNormRope> {
     return y;
   }
   static variable_list backward(AutogradContext* ctx, variable_list dy) {
+    // the kernel's outputs carry no graph: a gradient of this gradient would be wrong without a word
+    TORCH_CHECK(!at::GradMode::is_enabled(), "qk_norm_rope is differentiable once (no create_graph)");
     const auto v = ctx->get_saved_variables();
     auto opt = [&](int i) { return v[i].defined() ? OptTensor(v[i]) : OptTensor(); };
     const OptTensor k = opt(1);

@@ -76,7 +76,7 @@ struct AppendArgs {
   int64_t table_stride;
   const int* lens;             // tokens before the call
   const int* cu;               // [B + 1] or null
-  int n, total;                // new tokens of each sequence (uniform) / of all
+  int n, total;                // new tokens of each sequence, with `cu` the most of one; of all
   int J, H, P, logP, max_pages, n_pages, n_pos;
   const float* kw;             // [d] or null
   const float* rope;           // [n_pos, d] or null
@@ -101,7 +101,7 @@ __global__ void __launch_bounds__(kAppendThreads) append_kernel(const __grid_con
   const int tok0 = A.cu ? A.cu[b] : 0;
   const int n = A.cu ? A.cu[b + 1] - tok0 : A.n;
   if (n <= 0) return;
-  if (len < 0 || len > INT32_MAX - 64 - n || (A.cu && (tok0 < 0 || tok0 > A.total - n))) {
+  if (len < 0 || len > INT32_MAX - 64 - n || n > A.n || (A.cu && (tok0 < 0 || tok0 > A.total - n))) {
     if (threadIdx.x == 0) set_error(A.err, kBadShape);
     return;
   }
@@ -402,7 +402,7 @@ void kv_append(at::Tensor ck, at::Tensor cv, at::Tensor ks, at::Tensor vs, at::T
   const int64_t max_new = max.value_or(k.size(td - 3));
   PD_CHECK(k.size(td - 3) < (int64_t(1) << 31) && max_new >= 0 && max_new < (int64_t(1) << 31), "too many new tokens");
   A.total = int(cu.has_value() ? k.size(0) : 0);
-  A.n = int(cu.has_value() ? 0 : k.size(1));
+  A.n = int(cu.has_value() ? max_new : k.size(1));
   A.table = table.data_ptr<int>();
   A.table_stride = table.stride(0);
   A.max_pages = int(table.size(1));

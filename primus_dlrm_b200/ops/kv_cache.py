@@ -132,7 +132,8 @@ class PagedKVCache:
         ``k`` / ``v`` (bf16, fp16 or fp32, any strides over tokens and heads):
         ``[B, n, H, d]``, or ``[tokens, H, d]`` with ``cu_new`` int32 ``[B + 1]``,
         the offsets of each sequence's tokens; ``max_new`` is then the most of
-        one sequence (by default all of them).  ``page_table`` int32
+        one sequence (by default all of them; a longer sequence is skipped and
+        reported by :meth:`check_errors`).  ``page_table`` int32
         ``[B, pages]``, ``kv_lens`` int32 ``[B]`` (not changed).  No two
         sequences may write into one page.
 
@@ -262,7 +263,9 @@ def paged_attention(q: torch.Tensor, cache: PagedKVCache, page_table: torch.Tens
 
     ``q`` (bf16 or fp16, any strides over tokens and heads): ``[B, n, Hq, d]``,
     or ``[tokens, Hq, d]`` with ``cu_q`` int32 ``[B + 1]``; ``max_q`` is then the
-    most queries of one sequence (by default all of them).  ``Hq`` is a
+    most queries of one sequence (by default all of them; a longer sequence is
+    skipped and reported by ``cache.check_errors``; rows of ``q`` that no
+    sequence covers are not computed).  ``Hq`` is a
     multiple of the cache's heads: neighbours share one.  ``kv_lens`` int32
     ``[B]`` counts the tokens in the cache, the queries' own among them, so a
     sequence's ``n`` queries are its last ``n`` tokens: query ``i`` sees the

@@ -419,6 +419,31 @@ def test_shared_pages():
             (paged_attention(q[i:i + 1], c, table[i:i + 1], lens[i:i + 1])[0].float() - o[i].float()).abs().max() < 2e-2
 
 
+def test_longer_than_the_stated_most():
+    """A sequence of more tokens than ``max_new`` / ``max_q`` is skipped and reported; the others are served."""
+    from primus_dlrm_b200.ops.kv_cache import paged_attention
+    c = _cache(8, 1, 32, 16)
+    x = torch.ones(33, 1, 32, device=DEV)
+    before = _clone(c, DEV)
+    c.append(x, x, _i32([[0, 1, 2], [3, 4, 5]]), _i32([0, 0]), _i32([0, 1, 33]), 16)
+    assert c.k_scale[0, 0].item() == 2.0 ** -8
+    assert torch.equal(c.k_scale[1:], before.k_scale[1:])
+    with pytest.raises(RuntimeError, match="length"):
+        c.check_errors()
+    for n in (2, 140):                                                # few rows, many rows
+        q = torch.randn(3 * n, 1, 32, device=DEV).bfloat16()
+        table, lens, cu = _i32([[0, 1]] * 2), _i32([32, 32]), _i32([0, n, 3 * n])
+        o = paged_attention(q, c, table, lens, cu, n)
+        with pytest.raises(RuntimeError, match="length"):
+            c.check_errors()
+        # values lie in [0, 1]; either side is within 2^-9 (bf16) + 2^-10 (probabilities) of the exact sum
+        alone = paged_attention(q[:n], c, table[:1], lens[:1], cu[:2], n)
+        assert (o[:n].float() - alone.float()).abs().max() <= 2.0 ** -7
+        c.check_errors()
+    o, lse = paged_attention(q, c, table, lens, cu, 0, return_lse=True)
+    assert (o == 0).all() and (lse == -torch.inf).all()
+
+
 def test_attention_errors_mask():
     """A page id outside the pool counts as masked tokens; a length behind the page table is cut; both are reported."""
     from primus_dlrm_b200.ops.kv_cache import paged_attention

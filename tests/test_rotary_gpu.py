@@ -234,3 +234,11 @@ def test_refusals():
     ):
         with pytest.raises((RuntimeError, ValueError)):
             bad()
+
+
+def test_second_derivatives_are_refused():
+    from primus_dlrm_b200.ops.rotary import qk_norm_rope, rope_table
+    x = torch.randn(1, 4, 2, 32, device=DEV, requires_grad=True)
+    y, _ = qk_norm_rope(x, None, None, None, rope_table(4, 32, device=DEV))
+    with pytest.raises(RuntimeError, match="once"):
+        torch.autograd.grad(y.pow(2).sum(), x, create_graph=True)
