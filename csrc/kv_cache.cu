@@ -280,6 +280,7 @@ struct ReadArgs {
 // codes of one head's row at a time (16 bytes out, side by side); the pages of the block's tokens are looked
 // up once. Bound by the writes (2 bytes a value, 1 read).
 constexpr int kReadTokens = 64;
+constexpr int U = 4;                                 // vectors of a thread on their way
 
 template <int D>
 __global__ void __launch_bounds__(256) read_kernel(const ReadArgs A) {
@@ -306,19 +307,38 @@ __global__ void __launch_bounds__(256) read_kernel(const ReadArgs A) {
   const float* scale = part ? A.scale[1] : A.scale[0];
   __nv_bfloat16* out = (part ? A.out[1] : A.out[0]) + (int64_t(b) * A.n + t0) * A.H * D;
   const int per_token = A.H * L, all = tokens * per_token;
-#pragma unroll 4
-  for (int i = threadIdx.x; i < all; i += 256) {
-    const int t = i / per_token, j = i - t * per_token, h = j / L, c = j % L;
-    const int page = s_page[t];
-    float f[8];
+  const int dt = 256 / per_token, dj = 256 - dt * per_token;              // from a thread's vector to its next
+  int t = threadIdx.x / per_token, j = threadIdx.x - t * per_token;
+#pragma unroll 1
+  for (int i0 = threadIdx.x; i0 < all; i0 += 256 * U) {
+    uint2 u[U];
+    float sc[U];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) f[e] = 0.f;
-    if (page >= 0) {
-      const int block = page * A.H + h;
-      decode8(*reinterpret_cast<const uint2*>(code + (int64_t(block) * A.P + s_row[t]) * D + c * 8), f);
-      scale_v<8>(f, scale[block]);
+    for (int k = 0; k < U; ++k) {
+      const int page = i0 + 256 * k < all ? s_page[t] : -1;
+      u[k] = make_uint2(0, 0);
+      sc[k] = 0.f;
+      if (page >= 0) {
+        const int block = page * A.H + j / L;
+        u[k] = __ldg(reinterpret_cast<const uint2*>(code + (int64_t(block) * A.P + s_row[t]) * D + j % L * 8));
+        sc[k] = __ldg(scale + block);
+      }
+      t += dt;
+      j += dj;
+      if (j >= per_token) {
+        j -= per_token;
+        ++t;
+      }
     }
-    store_v<8>(out + int64_t(i) * 8, f);
+#pragma unroll
+    for (int k = 0; k < U; ++k) {
+      const int i = i0 + 256 * k;
+      if (i >= all) break;
+      float f[8];
+      decode8(u[k], f);
+      scale_v<8>(f, sc[k]);
+      store_v<8>(out + int64_t(i) * 8, f);
+    }
   }
 }
 
