@@ -26,6 +26,10 @@ template <> __device__ __forceinline__ float from_f(float v) { return v; }
 template <> __device__ __forceinline__ __half from_f(float v) { return __float2half_rn(v); }
 template <> __device__ __forceinline__ __nv_bfloat16 from_f(float v) { return __float2bfloat16_rn(v); }
 
+__device__ __forceinline__ uint32_t smem_u32(const void* p) {
+  return static_cast<uint32_t>(__cvta_generic_to_shared(p));
+}
+
 // V consecutive elements as they lie in memory; V = 8 moves 16 bytes an access
 // and needs 16-byte aligned addresses, V = 1 takes any element.
 template <int V, typename T>

@@ -15,16 +15,20 @@
 // of a token are neighbouring groups: they share the angles in L1, and the
 // loads of a warp are contiguous where the heads are. Rows that no 16-byte
 // access fits (odd strides, dims that are no multiple of 16) go through the
-// same code with single elements and a warp a row. A block walks over rows and
-// has the next one on its way while it works on one (two on their way, at the
-// same registers, measured slower: 301 against 276 us), and loads the row's
-// angles before its sum of squares.
+// same code with single elements and a warp a row. A block walks over rows. Of
+// 16-bit types each lane has three (backward two) rows to come on their way into
+// slots of shared memory that it alone writes and reads, so that they cost no
+// registers and no barrier; of 32-bit ones, whose vectors are two accesses, the
+// next row comes straight to registers (46 us below; 66 with slots). The row's
+// angles are loaded before its sum of squares.
 //
 // B200, 912 x 8 x 32 queries and keys (786 x 8 x 32) of a projection, batch 256,
-// bf16, forward and backward: 258 us, 4.3 TB/s over the 1.11 GB that both cannot
-// do without (floor 170 us at the copy rate of 6.5 TB/s); the forward runs 24
-// and the backward 16 warps an SM, and what bounds them now is the loads that
-// these have in flight. 2049 x 40 x 128 in 32 bits, half turned: 46 us, 5.5 TB/s.
+// bf16, forward and backward: 250 us, 4.4 TB/s over the 1.11 GB that both cannot
+// do without (floor 170 us at the copy rate of 6.5 TB/s; 260 us with the next row
+// in registers). The forward runs 24 and the backward 16 warps an SM; issue slots
+// are 52 to 63% full and the ALU pipe 50%, mostly conversions and addresses, and
+// neither more rows on their way nor a fourth forward block changes the time.
+// 2049 x 40 x 128 in 32 bits, half turned: 46 us, 5.5 TB/s.
 //
 // dw: each lane keeps its 16 columns' sums over all rows of its block, blocks
 // write theirs to a workspace and a second launch adds them in a fixed order,
@@ -73,6 +77,19 @@ __device__ __forceinline__ uint32_t fast_div(uint32_t n, uint32_t mul, uint32_t 
   return uint32_t((uint64_t(n) * mul) >> (31 + sh));
 }
 
+// 16-byte copies to shared memory that a thread issues and reads itself, in groups a row
+__device__ __forceinline__ void copy16(uint32_t to, const void* from) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory");
+}
+__device__ __forceinline__ void copy_group() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N> __device__ __forceinline__ void copy_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
+// rows that a lane holds in shared memory at once (1: none, the next one is in registers)
+template <typename T, int V> constexpr bool kRinged = V == 8 && sizeof(T) == 2;
+template <typename T, int V, bool BWD> constexpr int kStages = !kRinged<T, V> ? 1 : BWD ? 3 : 4;
+template <typename T, int V, bool BWD>
+constexpr int kRingBytes = !kRinged<T, V> ? 0 : kStages<T, V, BWD> * (BWD ? 4 : 2) * Raw<V, T>::N * 16 * kThreads;
+
 template <typename T, int V, int L, int NP, bool BWD>
 __global__ void __launch_bounds__(kThreads, BWD ? 2 : 3) qk_norm_rope_kernel(const __grid_constant__ Args A) {
   constexpr int G = kThreads / L;                       // rows of a block at a time
@@ -110,59 +127,89 @@ __global__ void __launch_bounds__(kThreads, BWD ? 2 : 3) qk_norm_rope_kernel(con
       w[0] = a.x; w[1] = a.y; w[2] = a.z; w[3] = a.w; w[4] = c.x; w[5] = c.y; w[6] = c.z; w[7] = c.w;
     }
   };
-  // a row on its way: elements, place in the output (or -1) and the angles' (or -1: a position outside)
+  // a row on its way: its place in the output (or -1), its position, its elements where no 16-byte copy takes them
+  constexpr bool RING = kRinged<T, V>;
+  constexpr int S = kStages<T, V, BWD>, N = Raw<V, T>::N;
+  extern __shared__ uint4 s_ring[];                     // [S][x, then dy: 2 N vectors each][thread]
+  const auto slot = [&](int st, int k) { return s_ring + (st * (BWD ? 4 : 2) * N + k) * kThreads + threadIdx.x; };
   struct Row {
-    Raw<V, T> xa[NP], xb[NP], ya[NP], yb[NP];
-    int row_of = -1, at_of = -1;
+    Raw<V, T> xa[RING ? 1 : NP], xb[RING ? 1 : NP], ya[RING ? 1 : NP], yb[RING ? 1 : NP];
+    int row_of = -1;
+    int64_t pos = -1;
   };
-  Row next;
-  auto fetch = [&](int it, Row& F) {
-    Raw<V, T>*xa = F.xa, *xb = F.xb, *ya = F.ya, *yb = F.yb;
-    int &row_of = F.row_of, &at_of = F.at_of;
+  Row next[S];
+  auto fetch = [&](int it, int st, Row& F) {
     const uint32_t row = uint32_t(it * blocks + block) * G + threadIdx.x / L;
-    row_of = row < uint32_t(P.rows) ? int(row) : -1;
-    at_of = -1;
-    if (row_of < 0) return;
-    const uint32_t tok = fast_div(row, P.mul_h, P.sh_h), h = row - tok * P.H;
-    const uint32_t bb = fast_div(tok, P.mul_t, P.sh_t), t = tok - bb * P.T;
-    const T* xr = x + int64_t(bb) * P.bs + int64_t(t) * P.ts + int64_t(h) * P.hs;
-    const T* dr = dy + int64_t(row) * d;
+    F.row_of = row < uint32_t(P.rows) ? int(row) : -1;
+    if (F.row_of >= 0) {
+      const uint32_t tok = fast_div(row, P.mul_h, P.sh_h), h = row - tok * P.H;
+      const uint32_t bb = fast_div(tok, P.mul_t, P.sh_t), t = tok - bb * P.T;
+      const T* xr = x + int64_t(bb) * P.bs + int64_t(t) * P.ts + int64_t(h) * P.hs;
+      const T* dr = dy + int64_t(row) * d;
 #pragma unroll
-    for (int i = 0; i < NP; ++i) {
-      if (on[i]) {
-        xa[i].load(xr + off0[i]);
-        xb[i].load(xr + off1[i]);
-        if (BWD) {
-          ya[i].load(dr + off0[i]);
-          yb[i].load(dr + off1[i]);
-        }
-      } else {
-        xa[i].zero();
-        xb[i].zero();
-        if (BWD) {
-          ya[i].zero();
-          yb[i].zero();
+      for (int i = 0; i < NP; ++i) {
+        if (!on[i]) continue;
+        if constexpr (RING) {
+#pragma unroll
+          for (int k = 0; k < N; ++k) {
+            copy16(smem_u32(slot(st, k)), reinterpret_cast<const uint4*>(xr + off0[i]) + k);
+            copy16(smem_u32(slot(st, N + k)), reinterpret_cast<const uint4*>(xr + off1[i]) + k);
+            if (BWD) {
+              copy16(smem_u32(slot(st, 2 * N + k)), reinterpret_cast<const uint4*>(dr + off0[i]) + k);
+              copy16(smem_u32(slot(st, 3 * N + k)), reinterpret_cast<const uint4*>(dr + off1[i]) + k);
+            }
+          }
+        } else {
+          F.xa[i].load(xr + off0[i]);
+          F.xb[i].load(xr + off1[i]);
+          if (BWD) {
+            F.ya[i].load(dr + off0[i]);
+            F.yb[i].load(dr + off1[i]);
+          }
         }
       }
+      const int64_t pi = int64_t(bb) * A.pos_bs + t + P.t_off;
+      F.pos = A.pos == nullptr ? int64_t(t) + P.t_off
+              : A.pos64        ? __ldg(static_cast<const long long*>(A.pos) + pi)
+                               : int64_t(__ldg(static_cast<const int*>(A.pos) + pi));
     }
-    const int64_t pi = int64_t(bb) * A.pos_bs + t + P.t_off;
-    const int64_t pos = A.pos == nullptr ? int64_t(t) + P.t_off
-                        : A.pos64        ? __ldg(static_cast<const long long*>(A.pos) + pi)
-                                         : int64_t(__ldg(static_cast<const int*>(A.pos) + pi));
-    if (pos >= 0 && pos < A.n_pos) at_of = int(pos);
-    else set_error(A.err, kIdOutOfRange);
+    if (RING) copy_group();
   };
   // every lane of a warp takes part in the group sums of each turn
   const int turns = int((int64_t(P.rows) + blocks * G - 1) / (blocks * G));
-  if (turns > 0) fetch(0, next);
-  for (int it = 0; it < turns; ++it) {
-    Raw<V, T>*xa = next.xa, *xb = next.xb, *ya = next.ya, *yb = next.yb;
-    const int row = next.row_of, at_of = next.at_of;
-    const bool live = row >= 0;
-    const float* at = A.table + int64_t(max(at_of, 0)) * A.rot;
-    if (at_of < 0) {                                    // behind the rows, or a position outside: zeros
+  constexpr int AHEAD = RING ? S - 1 : 1;
 #pragma unroll
-      for (int i = 0; i < NP; ++i) {
+  for (int i = 0; i < AHEAD; ++i) fetch(i, i, next[i]);
+  int st = 0;
+  for (int it = 0; it < turns; ++it) {
+    Raw<V, T> xa[NP], xb[NP], ya[NP], yb[NP];
+    const int row = next[0].row_of;
+    const bool live = row >= 0, known = live && next[0].pos >= 0 && next[0].pos < A.n_pos;
+    if (live && !known) set_error(A.err, kIdOutOfRange);
+    const float* at = A.table + (known ? next[0].pos : 0) * A.rot;
+    if (RING) copy_wait<AHEAD - 1>();
+#pragma unroll
+    for (int i = 0; i < NP; ++i) {
+      if (known && on[i]) {
+        if constexpr (RING) {
+#pragma unroll
+          for (int k = 0; k < N; ++k) {
+            xa[i].v[k] = *slot(st, k);
+            xb[i].v[k] = *slot(st, N + k);
+            if (BWD) {
+              ya[i].v[k] = *slot(st, 2 * N + k);
+              yb[i].v[k] = *slot(st, 3 * N + k);
+            }
+          }
+        } else {
+          xa[i] = next[0].xa[i];
+          xb[i] = next[0].xb[i];
+          if (BWD) {
+            ya[i] = next[0].ya[i];
+            yb[i] = next[0].yb[i];
+          }
+        }
+      } else {                                          // behind the rows, or a position outside: zeros
         xa[i].zero();
         xb[i].zero();
         if (BWD) {
@@ -171,6 +218,8 @@ __global__ void __launch_bounds__(kThreads, BWD ? 2 : 3) qk_norm_rope_kernel(con
         }
       }
     }
+#pragma unroll
+    for (int i = 0; i + 1 < AHEAD; ++i) next[i] = next[i + 1];
     float c[NP][V], s[NP][V];
 #pragma unroll
     for (int i = 0; i < NP; ++i)
@@ -187,8 +236,10 @@ __global__ void __launch_bounds__(kThreads, BWD ? 2 : 3) qk_norm_rope_kernel(con
       }
       ss += dot_v<V>(a[i], a[i], b[i], b[i]);
     }
-    if (it + 1 < turns) fetch(it + 1, next);
     const float r = __frsqrt_rn(group_sum<L>(ss) * inv_d + A.eps);
+    // the stage read in the last turn is free
+    fetch(it + AHEAD, st == 0 ? S - 1 : st - 1, next[AHEAD - 1]);
+    st = st + 1 == S ? 0 : st + 1;
     T* out = y + int64_t(row) * d;
     float dot = 0.f;
 #pragma unroll
@@ -282,11 +333,24 @@ __global__ void __launch_bounds__(1024) dw_sum_kernel(const float* part, int blo
   if (threadIdx.x == 0 && col < d && dw != nullptr) dw[col] = s;
 }
 
+template <typename T, int V, int L, int NP, bool BWD>
+static void launch(const Args& A, int grid) {
+  constexpr int kRing = kRingBytes<T, V, BWD>;
+  const auto kern = qk_norm_rope_kernel<T, V, L, NP, BWD>;
+  static bool known[64] = {};
+  int dev = 0;
+  PD_CHECK_CUDA(cudaGetDevice(&dev));
+  if (kRing > 32 * 1024 && (dev >= 64 || !known[dev])) {
+    PD_CHECK_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kRing));
+    if (dev < 64) known[dev] = true;
+  }
+  kern<<<grid, kThreads, kRing, stream()>>>(A);
+  PD_CHECK_LAUNCH();
+}
 template <typename T, int V, int L, int NP>
 static void launch(const Args& A, int grid, bool bwd) {
-  if (bwd) qk_norm_rope_kernel<T, V, L, NP, true><<<grid, kThreads, 0, stream()>>>(A);
-  else qk_norm_rope_kernel<T, V, L, NP, false><<<grid, kThreads, 0, stream()>>>(A);
-  PD_CHECK_LAUNCH();
+  if (bwd) launch<T, V, L, NP, true>(A, grid);
+  else launch<T, V, L, NP, false>(A, grid);
 }
 
 template <typename T>
