@@ -16,11 +16,11 @@
 // append is bound by memory for long pieces (it reads k and v once and writes
 // one byte a value) and by latency for single tokens, read by its writes.
 // B200, append and read together: 128 histories of 896 x 8 x 32 (bf16, keys
-// normed and rotated, pages of 64) 104 us for 361 MB (floor 55 us), of which the
-// append takes about 60: its rows are 64 bytes, 16 an access, and the maximum of
-// a page stands between its loads and its stores. 48 ragged pieces of 8 x 128
-// (pages of 16) 85 us for 280 MB (floor 43 us). One token each of 64 sequences:
-// 13 us, the two launches' host time.
+// normed and rotated, pages of 64) 86 us for 361 MB (floor 55 us), of which the
+// append takes about 52: its rows are 64 bytes, 16 an access, and the maximum of
+// a page stands between its loads and its stores (24 warps an SM, issue slots 56%
+// full). 48 ragged pieces of 8 x 128 (pages of 16) 72 us for 280 MB (floor 43 us).
+// One token each of 64 sequences: 13 us, the two launches' host time.
 #include <c10/cuda/CUDAGuard.h>
 #include <cuda_fp8.h>
 
@@ -88,10 +88,11 @@ struct AppendArgs {
 constexpr int kAppendThreads = 128;
 
 // One block: the new tokens of one sequence that fall into one page, for a run
-// of units (keys, then values, of one head each). A unit's rows stay in registers between the maximum and the encoding;
-// the next unit's are on their way meanwhile. A row belongs to D / 16 lanes of
-// 8 + 8 elements that turn against each other; PASSES times 128 / (D / 16) rows
-// make a page.
+// of units (keys, then values, of one head each). Blocks for 16 an SM: with 8 the
+// histories above take 90, with 48 88 us instead of 86. A unit's rows stay in
+// registers between the maximum and the encoding; the next unit's are on their
+// way meanwhile. A row belongs to D / 16 lanes of 8 + 8 elements that turn against
+// each other; PASSES times 128 / (D / 16) rows make a page.
 template <typename T, int D, int PASSES>
 __global__ void __launch_bounds__(kAppendThreads) append_kernel(const __grid_constant__ AppendArgs A) {
   constexpr int L = D / 16;                          // lanes of a row
@@ -277,8 +278,9 @@ struct ReadArgs {
 };
 
 // One block: up to 64 tokens of one sequence, all heads. A thread takes 8
-// codes of one head's row at a time (16 bytes out, side by side); the pages of the block's tokens are looked
-// up once. Bound by the writes (2 bytes a value, 1 read).
+// codes of one head's row at a time (16 bytes out, side by side), four times on their way; the pages of the
+// block's tokens are looked up once. Bound by the writes (2 bytes a value, 1 read): 34 us for 128 histories, 41 with
+// one vector on its way and a division each; eight cost registers and gain nothing.
 constexpr int kReadTokens = 64;
 constexpr int U = 4;                                 // vectors of a thread on their way
 

@@ -82,7 +82,9 @@ __device__ __forceinline__ void copy16(uint32_t to, const void* from) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory");
 }
 __device__ __forceinline__ void copy_group() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N> __device__ __forceinline__ void copy_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+template <int N> __device__ __forceinline__ void copy_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
 
 // rows that a lane holds in shared memory at once (1: none, the next one is in registers)
 template <typename T, int V> constexpr bool kRinged = V == 8 && sizeof(T) == 2;
