@@ -25,6 +25,17 @@ template <> struct Cfg<32> { static constexpr int TK = 64, SUB = 2, ST = 2; };
 template <> struct Cfg<64> { static constexpr int TK = 64, SUB = 1, ST = 2; };
 template <> struct Cfg<128> { static constexpr int TK = 32, SUB = 1, ST = 2; };
 
+// A wait has run out: the n copies on their way, from slot st on, land before the block may end.
+__device__ __noinline__ void drain(uint32_t bars, uint32_t slots, uint32_t st, uint32_t phase, int n, int* err) {
+  for (int i = 0; i < n; ++i) {
+    (void)mbar_wait(bars + st * 8, phase, err);
+    if (++st == slots) {
+      st = 0;
+      phase ^= 1;
+    }
+  }
+}
+
 // Few rows to a segment (one or some query tokens of one sequence, the heads
 // that share a key head): bound by reading the cache.
 //
@@ -218,7 +229,7 @@ paged_attn_kernel(const AttnArgs A, const __grid_constant__ CUtensorMap tm_k, co
   lane_offsets<D>(g, qd, k_off, v_off);
   // the two rows of this lane's accumulators
   const int row_a = R == 16 ? g : 2 * qd, row_b = R == 16 ? g + 8 : 2 * qd + 1;
-  bool alive = true;
+  bool alive = true;                        // no wait of this warp has run out
   uint32_t st = 0, phase = 0;               // slot of the ring and its turn
   bool first = true;                        // of this worker's segments
   while (c.left > 0) {
@@ -289,7 +300,14 @@ paged_attn_kernel(const AttnArgs A, const __grid_constant__ CUtensorMap tm_k, co
       issue(st == 0 ? ST - 1 : st - 1, scl[ST - 1], gone[ST - 1]);    // refills the slot of the tile before
       const float my_scl = scl[0];
       const uint32_t my_gone = gone[0];
-      if (alive) alive = mbar_wait(bars + st * 8, phase, A.err);
+      if (alive) {
+        alive = __all_sync(0xffffffffu, mbar_wait(bars + st * 8, phase, A.err));
+        if (!alive) {
+          // nothing more is copied; what the ring holds is computed on, for the block's barriers (the error word says so)
+          drain(bars, ST, st, phase, c.left - max(p.left, 0), A.err);
+          p.left = 0;
+        }
+      }
       __syncwarp();
 #pragma unroll 1
       for (int sub = 0; sub < SUB; ++sub) {
@@ -688,6 +706,7 @@ paged_attn_many_kernel(const AttnArgs A, const __grid_constant__ CUtensorMap tm_
   __shared__ float s_ks[ST][4], s_lv[ST][4];                // scales of a copy's pages: keys, log2 of values' (relative)
   __shared__ uint32_t s_gone[ST];
   __shared__ float s_top[kWarps];
+  __shared__ volatile int s_abort;          // a wait has run out: every warp leaves its loop
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int b = blockIdx.x / A.H, h = blockIdx.x % A.H, mt = gridDim.y - 1 - blockIdx.y;
@@ -699,6 +718,7 @@ paged_attn_many_kernel(const AttnArgs A, const __grid_constant__ CUtensorMap tm_
   const int lim = A.causal ? max(0, S.len - S.n + last / A.G + 1) : S.len;    // keys that the last row sees
   const int units = (lim + kUnit - 1) / kUnit;
   const int* table = A.table + b * A.table_stride;
+  if (threadIdx.x == 0) s_abort = 0;
   if (threadIdx.x < ST) {
     asm volatile("mbarrier.init.shared::cta.b64 [%0], 2;" ::"r"(smem_u32(&s_full[threadIdx.x])));
     asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(smem_u32(&s_empty[threadIdx.x])), "r"(kWarps));
@@ -718,7 +738,7 @@ paged_attn_many_kernel(const AttnArgs A, const __grid_constant__ CUtensorMap tm_
 
   // ---- copies (warp 0): those of unit v, then, a step later, its pages' scales ----
   const uint32_t ring = smem_u32(s_ring);
-  bool alive = true;
+  int issued = 0;                           // units
   int page = -1, pending = -1;              // lane i: page i of the next unit; slot whose scales are on their way
   float new_ks = 0.f, new_vs = 0.f;
   uint32_t new_gone = 0;
@@ -749,8 +769,10 @@ paged_attn_many_kernel(const AttnArgs A, const __grid_constant__ CUtensorMap tm_
     if (want && !have) set_error(A.err, kIdOutOfRange);
     const int block = have ? page * A.H + h : 0;
     const uint32_t mask = __ballot_sync(0xffffffffu, have);
-    if (alive && turn > 0) alive = mbar_wait(smem_u32(&s_empty[sl]), (turn - 1) & 1, A.err);
-    __syncwarp();
+    if (turn > 0 && !__all_sync(0xffffffffu, mbar_wait(smem_u32(&s_empty[sl]), (turn - 1) & 1, A.err))) {
+      s_abort = 1;
+      return;
+    }
     if (lane == 0)
       asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;"
                    ::"r"(full), "r"(uint32_t(__popc(mask) * 2 * A.P * D)) : "memory");
@@ -766,6 +788,7 @@ paged_attn_many_kernel(const AttnArgs A, const __grid_constant__ CUtensorMap tm_
     new_vs = have ? __ldg(A.vs + block) : 0.f;
     new_gone = ~mask;
     pending = sl;
+    issued = v + 1;
     fetch(v + 1);
   };
   if (warp == 0) {
@@ -823,13 +846,15 @@ paged_attn_many_kernel(const AttnArgs A, const __grid_constant__ CUtensorMap tm_
   for (int u = 0; u < NO; ++u) o[u][0] = o[u][1] = o[u][2] = o[u][3] = 0.f;
   uint32_t st = 0, phase = 0;
 #pragma unroll 1
-  for (int u = 0; u < units; ++u) {
+  for (int u = 0; u < units && !__any_sync(0xffffffffu, s_abort); ++u) {
     if (warp == 0) {
       settle();
       copy(u + ST - 2);
     }
-    if (alive) alive = mbar_wait(smem_u32(&s_full[st]), phase, A.err);
-    __syncwarp();
+    if (!__all_sync(0xffffffffu, mbar_wait(smem_u32(&s_full[st]), phase, A.err))) {
+      s_abort = 1;
+      break;
+    }
     const uint32_t all_gone = s_gone[st];
 #pragma unroll 1
     for (int sub = 0; sub < kUnit / TK; ++sub) {
@@ -981,6 +1006,11 @@ paged_attn_many_kernel(const AttnArgs A, const __grid_constant__ CUtensorMap tm_
       st = 0;
       phase ^= 1;
     }
+  }
+  if (warp == 0 && __any_sync(0xffffffffu, s_abort)) {
+    // every copy lands before the block may end
+    settle();
+    for (int v = max(0, issued - ST); v < issued; ++v) (void)mbar_wait(smem_u32(&s_full[v % ST]), v / ST & 1, A.err);
   }
 #pragma unroll
   for (int i = 0; i < 2; ++i) {

@@ -245,8 +245,9 @@ paged_attn_tc_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__
       }
       settle();
       if (!ok) s_abort = 1;
-      if (s_abort)                            // every copy lands before the block may end
-        for (int v = max(0, issued - kRaw); v < issued; ++v) (void)wait(&raw_full[v % kRaw], v / kRaw);
+      // Every copy lands before the block may end, whichever role gives up, and when; else the last ones are all that
+      // this waits for.
+      for (int v = max(0, issued - kRaw); v < issued; ++v) (void)wait(&raw_full[v % kRaw], v / kRaw);
     } else if (warp == 1) {
       // ---------------- products ----------------
       if (lane == 0 && units > 0) {
