@@ -439,6 +439,9 @@ std::vector<at::Tensor> qk_norm_rope(at::Tensor q, c10::optional<at::Tensor> k, 
   const c10::cuda::CUDAGuard guard(q.device());
   fill(A.p[0], q, wq, t_all, "q");
   if (n_parts == 2) fill(A.p[1], *k, wk, t_all, "k");
+  // rows outside the table take the angles of its first row, times zeros: there has to be one
+  TORCH_CHECK_INDEX(A.n_pos > 0 || A.rot == 0 || (A.p[0].rows == 0 && A.p[1].rows == 0),
+                    "every position lies outside an angle table of 0 rows");
 
   std::vector<at::Tensor> out;
   bool vec = A.d % 16 == 0 && A.rot % 16 == 0;
