@@ -385,7 +385,7 @@ static void fill(Part& P, const at::Tensor& x, const c10::optional<at::Tensor>& 
   P.t_off = t_all - P.T;
   P.w = nullptr;
   if (w.has_value()) {
-    PD_CHECK(w->is_cuda() && w->scalar_type() == at::kFloat && w->is_contiguous() && w->dim() == 1 &&
+    PD_CHECK(w->device() == x.device() && w->scalar_type() == at::kFloat && w->is_contiguous() && w->dim() == 1 &&
              w->size(0) == x.size(3), "the weight of %s must be a contiguous fp32 [d] on its device", what);
     P.w = w->data_ptr<float>();
   }

@@ -18,3 +18,13 @@ def test_an_empty_angle_table_is_refused():
             qk_norm_rope(x[:, :0], x, None, None, none, positions)
     y, _ = qk_norm_rope(x[:, :0], None, None, None, none)              # no rows, no angles
     assert y.shape == (1, 0, 2, 32)
+
+
+def test_weights_lie_on_the_device_of_the_rows():
+    from primus_dlrm_b200.ops.rotary import qk_norm_rope, rope_table
+    x, t = torch.ones(1, 4, 2, 32, device=DEV), rope_table(4, 32, device=DEV)
+    for other in ["cpu"] + [f"cuda:{i}" for i in range(1, torch.cuda.device_count())]:
+        w = torch.ones(32, device=other)
+        for a, b in ((w, None), (None, w)):
+            with pytest.raises(RuntimeError, match="on its device"):
+                qk_norm_rope(x, x, a, b, t)
