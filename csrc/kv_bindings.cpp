@@ -12,6 +12,7 @@ std::vector<at::Tensor> qk_norm_rope(at::Tensor, c10::optional<at::Tensor>, c10:
 void kv_append(at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor,
                at::Tensor, c10::optional<at::Tensor>, c10::optional<int64_t>, c10::optional<at::Tensor>, c10::optional<double>,
                c10::optional<at::Tensor>, bool);
+void kv_copy_pages(at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor);
 std::vector<at::Tensor> kv_read(at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor,
                                 c10::optional<at::Tensor>, c10::optional<int64_t>);
 std::vector<at::Tensor> paged_attention(at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor,
@@ -104,6 +105,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("rotary", &rotary, "(q', k') of qk_norm_rope, with gradients where asked for");
   m.def("rotary_err", &rotary_err, "the device's int32 error word of `rotary`");
   m.def("append", &pd::kv::kv_append, "new tokens' keys and values into the pages of a cache");
+  m.def("copy_pages", &pd::kv::kv_copy_pages, "pages dst become copies of pages src");
   m.def("read", &pd::kv::kv_read, "tokens [first, first + n) of each sequence as bf16 [B, n, H, d]");
   m.def("paged_attention", &pd::kv::paged_attention, "attention of the last tokens over a cache -> [o(, lse)]");
   m.def("launch_count", &pd::launches);

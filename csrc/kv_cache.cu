@@ -344,6 +344,32 @@ __global__ void __launch_bounds__(256) read_kernel(const ReadArgs A) {
   }
 }
 
+// Pages to or from a copy of them, keys or values: block x takes pair x, blocks y share its 16-byte vectors. A pair with
+// an id outside the pool is reported and left alone. All sources are read before the first page is written, so a page
+// may be another pair's source and destination. Moves each byte four times; not a path whose time matters.
+template <bool OUT>
+__global__ void __launch_bounds__(256) copy_pages_kernel(const long long* src, const long long* dst, uint4* code,
+                                                         float* scale, uint4* tmp, float* tmp_scale, int vecs, int H,
+                                                         int n_pages, int* err) {
+  const int i = blockIdx.x;
+  const long long from = src[i], to = dst[i];
+  if (from < 0 || from >= n_pages || to < 0 || to >= n_pages) {
+    if (threadIdx.x == 0) set_error(err, kIdOutOfRange);
+    return;
+  }
+  uint4* page = code + (OUT ? from : to) * vecs;
+  uint4* copy = tmp + int64_t(i) * vecs;
+  for (int v = blockIdx.y * 256 + threadIdx.x; v < vecs; v += gridDim.y * 256) {
+    if (OUT) copy[v] = page[v];
+    else page[v] = copy[v];
+  }
+  if (blockIdx.y > 0) return;
+  for (int h = threadIdx.x; h < H; h += 256) {
+    if (OUT) tmp_scale[int64_t(i) * H + h] = scale[from * H + h];
+    else scale[to * H + h] = tmp_scale[int64_t(i) * H + h];
+  }
+}
+
 // ---------------------------------------------------------------- entry points
 // The cache's tensors; returns their sizes.
 struct CacheDims { int n_pages, H, P, d; };
@@ -464,6 +490,34 @@ void kv_append(at::Tensor ck, at::Tensor cv, at::Tensor ks, at::Tensor vs, at::T
   else if (dt == kF16) append_launch<__half>(A, grid, C.d);
   else append_launch<float>(A, grid, C.d);
   PD_CHECK_LAUNCH();
+}
+
+void kv_copy_pages(at::Tensor ck, at::Tensor cv, at::Tensor ks, at::Tensor vs, at::Tensor err, at::Tensor src,
+                   at::Tensor dst) {
+  const CacheDims C = check_cache(ck, cv, ks, vs, err);
+  for (const at::Tensor* t : {&src, &dst})
+    PD_CHECK(t->device() == ck.device() && t->scalar_type() == at::kLong && t->dim() == 1 && t->is_contiguous() &&
+             t->size(0) == src.size(0), "src and dst must be contiguous int64 [n] on the cache's device");
+  const int64_t n = src.size(0), vecs = int64_t(C.H) * C.P * C.d / 16;
+  PD_CHECK(n < (int64_t(1) << 31) && vecs < (int64_t(1) << 31) - (1 << 24), "too many pages, or too large ones");
+  if (n == 0) return;
+  const c10::cuda::CUDAGuard guard(ck.device());
+  const at::Tensor tmp = at::empty({n, vecs * 16}, ck.options().dtype(at::kByte));
+  const at::Tensor tmp_scale = at::empty({n, C.H}, ks.options());
+  const dim3 grid(unsigned(n), unsigned(std::min<int64_t>((vecs + 1023) / 1024, 64)));
+  for (int i = 0; i < 2; ++i) {
+    uint4* code = static_cast<uint4*>((i == 0 ? ck : cv).data_ptr());
+    float* scale = (i == 0 ? ks : vs).data_ptr<float>();
+    const auto go = [&](auto kern) {
+      kern<<<grid, 256, 0, stream()>>>(reinterpret_cast<const long long*>(src.data_ptr<int64_t>()),
+                                       reinterpret_cast<const long long*>(dst.data_ptr<int64_t>()), code, scale,
+                                       static_cast<uint4*>(tmp.data_ptr()), tmp_scale.data_ptr<float>(), int(vecs), C.H,
+                                       C.n_pages, err.data_ptr<int>());
+      PD_CHECK_LAUNCH();
+    };
+    go(copy_pages_kernel<true>);
+    go(copy_pages_kernel<false>);
+  }
 }
 
 std::vector<at::Tensor> kv_read(at::Tensor ck, at::Tensor cv, at::Tensor ks, at::Tensor vs, at::Tensor err,

@@ -218,8 +218,18 @@ class PagedKVCache:
 
     @torch.no_grad()
     def copy_pages(self, src: torch.Tensor, dst: torch.Tensor) -> None:
-        """Pages ``dst`` become copies of pages ``src`` (int64 ``[n]`` each): how a
-        sequence gets a page of its own before it appends behind a shared one."""
+        """Pages ``dst`` become copies of pages ``src`` (integers ``[n]`` each, ``dst``
+        all different): how a sequence gets a page of its own before it appends
+        behind a shared one.  Every source is read before the first page is
+        written.  A pair with an id outside the pool is skipped and reported by
+        :meth:`check_errors` (IndexError on the eager path)."""
+        src, dst = (t.to(self.device, torch.int64) for t in torch.broadcast_tensors(src, dst))
+        if self._native():
+            _ext.kv().copy_pages(*self._parts, src.contiguous(), dst.contiguous())
+            return
+        for t in (src, dst):
+            if t.numel() and not 0 <= int(t.min()) <= int(t.max()) < self.n_pages:
+                raise IndexError(f"a page id lies outside the pool of {self.n_pages}")
         for t in (self.k.view(torch.uint8), self.v.view(torch.uint8), self.k_scale, self.v_scale):
             t[dst] = t[src]
 

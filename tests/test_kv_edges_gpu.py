@@ -2,7 +2,7 @@
 that nobody computes, refusals."""
 import pytest
 import torch
-from test_kv_cache_gpu import DEV
+from test_kv_cache_gpu import DEV, _cache, _clone, _same
 
 pytestmark = pytest.mark.gpu
 
@@ -28,3 +28,33 @@ def test_weights_lie_on_the_device_of_the_rows():
         for a, b in ((w, None), (None, w)):
             with pytest.raises(RuntimeError, match="on its device"):
                 qk_norm_rope(x, x, a, b, t)
+
+
+@pytest.mark.parametrize("P,d,H", [(16, 32, 1), (64, 128, 3), (32, 64, 16)])
+@pytest.mark.parametrize("src,dst", [([0], [5]), ([3, 3, 1], [0, 2, 4]), ([0, 1, 2], [1, 2, 0]), ([4], [4]), ([], []),
+                                     ([6], [0, 1, 2, 3])])
+def test_copy_pages(P, d, H, src, dst):
+    """As an assignment by index: every source is read first, one source serves many."""
+    c = _cache(7, H, d, P, spread=2.0)
+    want = _clone(c, "cpu")
+    for t in (want.k.view(torch.uint8), want.v.view(torch.uint8), want.k_scale, want.v_scale):
+        t[dst] = t[src]
+    for kind in (torch.int64, torch.int32):
+        got = _clone(c, DEV)
+        got.copy_pages(torch.tensor(src, dtype=kind, device=DEV), torch.tensor(dst, dtype=kind, device=DEV))
+        _same(got, want)
+        got.check_errors()
+
+
+def test_copy_pages_outside_the_pool_are_skipped_and_reported():
+    """An id that a page table holds for no page (-1) must not become the last page."""
+    c = _cache(4, 2, 64, 16)
+    for src, dst in (([-1, 0], [1, 2]), ([1, 0], [4, 2]), ([0, 1 << 40], [2, 3]), ([0, 1], [2, -(1 << 40)])):
+        before = _clone(c, "cpu")
+        c.copy_pages(torch.tensor(src, device=DEV), torch.tensor(dst, device=DEV))
+        with pytest.raises(RuntimeError, match="out of range"):
+            c.check_errors()
+        before.copy_pages(torch.tensor([0]), torch.tensor([2]))
+        _same(c, before)
+        c.v_scale *= 2
+    c.check_errors()
