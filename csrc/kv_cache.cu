@@ -400,6 +400,8 @@ void check_ints(const at::Tensor& t, const at::Tensor& like, int64_t n, const ch
 void check_table(const at::Tensor& t, const at::Tensor& like) {
   PD_CHECK(t.device() == like.device() && t.scalar_type() == at::kInt && t.dim() == 2 &&
            (t.size(1) <= 1 || t.stride(1) == 1), "the page table must be int32 [sequences, pages] on the cache's device");
+  // kernels count a sequence's keys in 32 bits, rounded up to their tiles
+  PD_CHECK(t.size(1) * like.size(2) <= INT32_MAX - 4096, "a page table has room for 2^31 - 4096 tokens of a sequence at most");
 }
 
 template <typename T>

@@ -2,7 +2,7 @@
 that nobody computes, refusals."""
 import pytest
 import torch
-from test_kv_cache_gpu import DEV, _cache, _clone, _same
+from test_kv_cache_gpu import DEV, _cache, _clone, _i32, _same
 
 pytestmark = pytest.mark.gpu
 
@@ -57,4 +57,21 @@ def test_copy_pages_outside_the_pool_are_skipped_and_reported():
         before.copy_pages(torch.tensor([0]), torch.tensor([2]))
         _same(c, before)
         c.v_scale *= 2
+    c.check_errors()
+
+
+def test_a_page_table_beyond_32_bits_of_tokens_is_refused():
+    """Before anything is launched: a length near 2^31 would overflow the kernels' counts of keys."""
+    from primus_dlrm_b200.ops.kv_cache import paged_attention
+    c = _cache(2, 1, 32, 64)
+    table = torch.zeros(1, (1 << 25) - 64, dtype=torch.int32, device=DEV)
+    one, x = _i32([1]), torch.ones(1, 1, 1, 32, device=DEV, dtype=torch.bfloat16)
+    for bad in (lambda: paged_attention(x, c, table, one), lambda: c.append(x, x, table, one),
+                lambda: c.read(table, one, n=4)):
+        with pytest.raises(RuntimeError, match="room"):
+            bad()
+    ok = table[:, :-1]
+    c.append(x, x, ok, one)
+    paged_attention(x, c, ok, one, max_len=64)
+    c.read(ok, one, n=4)
     c.check_errors()
