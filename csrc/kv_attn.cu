@@ -79,6 +79,9 @@ paged_attn_kernel(const AttnArgs A, const __grid_constant__ CUtensorMap tm_k, co
   __shared__ uint64_t s_bar[kWarps][ST];
   __shared__ int64_t s_scan[kWarps], s_start[kWarps / W][2];
 
+  // no pieces yet; the threads that set these are lanes of the warp that writes pieces
+  if (A.split && threadIdx.x < 2) A.part_head[(blockIdx.x * 2 + threadIdx.x) * 4] = -1;
+  if (!tiles_aligned(s_ring, A.err)) return;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int part = W == 1 ? 0 : warp;                       // of the segment's warps
   const int g = lane >> 2, qd = lane & 3;
@@ -174,7 +177,6 @@ paged_attn_kernel(const AttnArgs A, const __grid_constant__ CUtensorMap tm_k, co
       c.limits(A);
     }
   }
-  if (A.split && threadIdx.x < 2) A.part_head[(blockIdx.x * 2 + threadIdx.x) * 4] = -1;
   if (c.left <= 0) return;                  // a whole block for W > 1, a warp for W = 1
 
   // ---- producer: this warp's tile of each unit ----
@@ -708,6 +710,7 @@ paged_attn_many_kernel(const AttnArgs A, const __grid_constant__ CUtensorMap tm_
   __shared__ float s_top[kWarps];
   __shared__ volatile int s_abort;          // a wait has run out: every warp leaves its loop
 
+  if (!tiles_aligned(s_ring, A.err)) return;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int b = blockIdx.x / A.H, h = blockIdx.x % A.H, mt = gridDim.y - 1 - blockIdx.y;
   Seq<R> S;

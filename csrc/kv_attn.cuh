@@ -18,6 +18,8 @@ CacheDims check_cache(const at::Tensor&, const at::Tensor&, const at::Tensor&, c
 void check_ints(const at::Tensor&, const at::Tensor&, int64_t, const char*);
 void check_table(const at::Tensor&, const at::Tensor&);
 
+constexpr int kMisaligned = 4;           // error word: behind the codes of all kernels
+
 constexpr uint64_t kWaitLimitNs = 2000000000ull;
 constexpr int kWarps = 4;               // warps of a block
 constexpr int kUnit = 64;               // keys of a copy that a block shares
@@ -42,6 +44,16 @@ struct AttnArgs {
   int* err;
 };
 
+// The hardware's exchange of 16-byte chunks goes by address bits up to 2^10, and so does the code that reads the tiles:
+// tiles off that boundary would be read wrongly without a word. The address goes through asm so that the check is not
+// taken for granted.
+__device__ __forceinline__ bool tiles_aligned(const void* tiles, int* err) {
+  uint32_t at;
+  asm volatile("mov.u32 %0, %1;" : "=r"(at) : "r"(smem_u32(tiles)));
+  if (!(at & 1023)) return true;
+  set_error(err, kMisaligned);
+  return false;
+}
 __device__ __forceinline__ bool mbar_try(uint32_t bar, uint32_t parity) {
   uint32_t ok;
   asm volatile(

@@ -134,6 +134,7 @@ paged_attn_tc_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__
   __shared__ uint32_t s_tmem;
   __shared__ volatile int s_abort;
 
+  if (!tiles_aligned(s_tiles, A.err)) return;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int b = blockIdx.x / A.H, h = blockIdx.x % A.H, mt = gridDim.y - 1 - blockIdx.y;
   Seq<kTcRows> S;

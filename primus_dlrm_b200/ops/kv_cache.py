@@ -116,7 +116,8 @@ class PagedKVCache:
         if e:
             self.err.zero_()
             raise RuntimeError({1: "paged cache: a page id, or a position, is out of range",
-                                2: "paged cache: a bounded wait in a kernel ran out"}.get(
+                                2: "paged cache: a bounded wait in a kernel ran out",
+                                4: "paged cache: a kernel's shared memory is not aligned"}.get(
                                     e, "paged cache: a sequence's length does not fit its tokens or its page table"))
 
     def _native(self) -> bool:
