@@ -238,7 +238,8 @@ __global__ void __launch_bounds__(kThreads, BWD ? 2 : 3) qk_norm_rope_kernel(con
       }
       ss += dot_v<V>(a[i], a[i], b[i], b[i]);
     }
-    const float r = __frsqrt_rn(group_sum<L>(ss) * inv_d + A.eps);
+    // groups without a row hold zeros: with eps = 0 their root would be infinite, and NaN in the sums of dw
+    const float rt = __frsqrt_rn(group_sum<L>(ss) * inv_d + A.eps), r = known ? rt : 0.f;
     // the stage read in the last turn is free
     fetch(it + AHEAD, st == 0 ? S - 1 : st - 1, next[AHEAD - 1]);
     st = st + 1 == S ? 0 : st + 1;

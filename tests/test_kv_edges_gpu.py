@@ -75,3 +75,41 @@ def test_a_page_table_beyond_32_bits_of_tokens_is_refused():
     paged_attention(x, c, ok, one, max_len=64)
     c.read(ok, one, n=4)
     c.check_errors()
+
+
+def _norm_ref(x, w, ang, dy):
+    x, w = x.detach().double().requires_grad_(), w.detach().double().requires_grad_()
+    y = x / torch.sqrt((x * x).mean(-1, keepdim=True)) * w
+    h = ang.shape[-1] // 2
+    c, s = ang[:, None, :h].double(), ang[:, None, h:].double()
+    y = torch.cat([y[..., :h] * c - y[..., h:] * s, y[..., :h] * s + y[..., h:] * c], -1)
+    return (y.detach(), *torch.autograd.grad(y, (x, w), dy.double()))
+
+
+@pytest.mark.parametrize("B,T,H", [(1, 1, 1), (1, 5, 3), (3, 37, 2), (70, 101, 5)])
+@pytest.mark.parametrize("d", [32, 96, 128])
+def test_rotary_without_eps(B, T, H, d):
+    """eps = 0 with rows that are not zero, of any count: nothing of the rows that fill up a block reaches the sums. A
+    position outside the table gives zeros, in the gradients too. 24 roundings of 2^-24 bound the chain of a row, whose
+    gradient is a difference of terms of up to |dy| |w| sqrt(d) r each; sums of n products of some 16 each."""
+    from primus_dlrm_b200.ops import rotary
+    g = torch.Generator(device=DEV).manual_seed(T)
+    x, dy = (torch.randn(B, T, H, d, generator=g, device=DEV) for _ in range(2))
+    w = 1 + 0.3 * torch.randn(d, generator=g, device=DEV)
+    table, pos = rotary.rope_table(T + 3, d, device=DEV), torch.arange(T, device=DEV)
+    want = _norm_ref(x, w, table[pos], dy)
+    leaf = [x.detach().requires_grad_(), w.detach().requires_grad_()]
+    y, _ = rotary.qk_norm_rope(leaf[0], None, leaf[1], None, table, pos, eps=0.0)
+    got = (y.detach(), *torch.autograd.grad(y, leaf, dy))
+    for a, b, size in zip(got, want, (16.0, 64.0, 16.0 * (B * T * H + 30))):
+        assert torch.isfinite(a).all() and (a.double() - b).abs().max().item() <= 24 * 2.0 ** -24 * size
+    out = pos.clone()
+    out[T // 2] = T + 3
+    y, _ = rotary.qk_norm_rope(leaf[0], None, leaf[1], None, table, out, eps=0.0)
+    dx, dw = torch.autograd.grad(y, leaf, dy)
+    keep = torch.arange(T, device=DEV) != T // 2
+    assert (y[:, T // 2] == 0).all() and (dx[:, T // 2] == 0).all()
+    assert torch.equal(y[:, keep], got[0][:, keep]) and torch.equal(dx[:, keep], got[1][:, keep])
+    assert torch.isfinite(dw).all()
+    assert rotary.rotary_error_code(DEV) == 1
+    rotary._err_word(DEV).zero_()
