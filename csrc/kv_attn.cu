@@ -393,12 +393,12 @@ paged_attn_kernel(const AttnArgs A, const __grid_constant__ CUtensorMap tm_k, co
             irel[i] = __shfl_sync(0xffffffffu, my_scl, pg + NP);
             vref = fmaxf(vref, irel[i]);
           }
-          // A page's value scale relative to vref goes into the exponent, and out of the sum again. Below 2^-60 its
-          // probabilities are zeros in fp16 whatever they are; one that was not loaded (scale 0) has none.
+          // A page's value scale relative to vref goes into the exponent, and out of the sum again. Below 2^-60, a scale
+          // of 0 among them, its probabilities are zeros in fp16 whatever they are; a page not loaded has none.
           const float lref = __log2f(vref);
 #pragma unroll
           for (int i = 0; i < TS; ++i) {
-            lrel[i] = irel[i] > 0.f ? fmaxf(__log2f(irel[i]) - lref, -60.f) : 0.f;
+            lrel[i] = irel[i] > 0.f ? fmaxf(__log2f(irel[i]) - lref, -60.f) : -60.f;
             irel[i] = exp2f_approx(-lrel[i]);
           }
         }

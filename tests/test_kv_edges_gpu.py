@@ -1,10 +1,77 @@
 """Edges of the rotary norm, the paged 8-bit cache and its attention on the GPU: values of very different sizes, rows
 that nobody computes, refusals."""
+import math
+
 import pytest
 import torch
-from test_kv_cache_gpu import DEV, _cache, _clone, _i32, _same
+from test_kv_cache_gpu import DEV, E4M3, _cache, _clone, _i32, _same, _table
 
 pytestmark = pytest.mark.gpu
+
+# forms of the attention: (d, page, heads, group, sequences, queries of each, keys) -> few rows of 8 and of 16 (shares of
+# the keys, and a warp a segment), many rows on tcgen05, many rows at d = 128
+FORMS = {
+    "8 rows, d 32": (32, 16, 2, 1, 2, 7, 150), "8 rows, d 64": (64, 32, 2, 4, 2, 2, 900),
+    "8 rows, d 128": (128, 16, 1, 2, 3, 4, 130), "8 rows, whole pages": (64, 64, 2, 1, 2, 6, 300),
+    "16 rows, d 32": (32, 32, 2, 2, 2, 8, 140), "16 rows, d 64": (64, 16, 1, 1, 2, 12, 64),
+    "16 rows, d 128": (128, 16, 2, 1, 1, 13, 200), "16 rows, long": (64, 16, 2, 1, 1, 40, 2500), "a warp a segment": (32, 16, 8, 1, 160, 16, 100),
+    "tcgen05, d 32": (32, 16, 4, 1, 40, 128, 300), "tcgen05, d 64": (64, 32, 4, 1, 40, 100, 300),
+    "many, d 128": (128, 32, 4, 1, 40, 100, 300), "many, d 128, pages of 16": (128, 16, 4, 2, 40, 50, 257),
+}
+
+
+def _plain(q, c, table, lens, causal=True, scale=None):
+    """In 64 bits: o, sum_j p |v|, the largest p_j 448 vs_j of each row (keys that it sees only), and lse."""
+    B, n, Hq, d = q.shape
+    P, G, scale = c.page_size, Hq // c.n_kv_heads, d ** -0.5 if scale is None else scale
+    o, a, top = (torch.zeros(q.shape, dtype=torch.float64, device=q.device) for _ in range(3))
+    lse = torch.full(q.shape[:3], -math.inf, dtype=torch.float64, device=q.device)
+    for b in range(B):
+        T = int(lens[b])
+        if T == 0:
+            continue
+        ids = table[b, :-(-T // P)].long()
+        k, v = ((x.view(torch.uint8)[ids].view(E4M3).double() * s[ids].double()[..., None, None]).transpose(0, 1)
+                .flatten(1, 2)[:, :T].repeat_interleave(G, 0) for x, s in ((c.k, c.k_scale), (c.v, c.v_scale)))
+        vs = c.v_scale[ids].double().T.repeat_interleave(P, 1)[:, :T].repeat_interleave(G, 0)
+        w = q[b].double().transpose(0, 1) @ k.transpose(1, 2) * scale
+        if causal:
+            w = w.masked_fill(torch.arange(T, device=q.device) > (T - n + torch.arange(n, device=q.device))[:, None], -math.inf)
+        z = torch.logsumexp(w, -1)
+        p = torch.where(z[..., None] == -math.inf, 0.0, torch.exp(w - z[..., None]))
+        o[b], a[b] = (p @ v).transpose(0, 1), (p @ v.abs()).transpose(0, 1)
+        top[b] = (p * 448 * vs[:, None]).amax(-1).transpose(0, 1)[..., None]
+        lse[b] = z.transpose(0, 1)
+    return o, a, top, lse
+
+
+def _check_rows(q, c, table, lens, **kw):
+    """Every row against its own size: a rounding to the output's type (8 or 11 significant bits); probabilities in 11
+    bits, 2^-11 of sum p |v|, and what falls below them, 2^-30 of the largest product for each key; exponents off by the
+    32-bit error of the scores, d + 8 roundings of 2^-24 of |q| |k| each, twice, and 2^-20 from the exponentials."""
+    from primus_dlrm_b200.ops.kv_cache import paged_attention
+    ref, size, top, lref = _plain(q, c, table, lens, kw.get("causal", True), kw.get("scale"))
+    o, lse = paged_attention(q, c, table, lens, return_lse=True, **kw)
+    c.check_errors()
+    d = q.shape[-1]
+    unit = 2.0 ** -8 if q.dtype == torch.bfloat16 else 2.0 ** -11
+    kmax = (c.k.float().nan_to_num().norm(dim=-1).amax(-1) * c.k_scale).max().item()
+    score = abs(kw.get("scale") or d ** -0.5) * q.float().norm(dim=-1).max().item() * kmax
+    soft = 2.0 ** -11 + 2 * (d + 8) * 2.0 ** -24 * score + 2.0 ** -20
+    tol = unit * ref.abs() * 1.01 + soft * size + int(lens.max()) * 2.0 ** -30 * top + 2.0 ** -120
+    assert torch.isfinite(o).all()
+    worst = ((o.double() - ref).abs() / tol).max().item()
+    assert worst <= 1.0, worst
+    assert torch.equal(lref == -math.inf, lse == -math.inf)
+    return o
+
+
+def _queries(form, seed):
+    d, P, H, G, B, n, T = FORMS[form]
+    g = torch.Generator(device=DEV).manual_seed(seed)
+    c = _cache(B * -(-T // P), H, d, P, seed=seed)
+    table = _table([T] * B, P, c.n_pages)
+    return c, table, torch.randn(B, n, H * G, d, generator=g, device=DEV).bfloat16(), _i32([T - i % 9 for i in range(B)])
 
 
 def test_an_empty_angle_table_is_refused():
@@ -113,3 +180,13 @@ def test_rotary_without_eps(B, T, H, d):
     assert torch.isfinite(dw).all()
     assert rotary.rotary_error_code(DEV) == 1
     rotary._err_word(DEV).zero_()
+
+
+@pytest.mark.parametrize("form", [f for f in FORMS if "rows" in f or "warp" in f])
+def test_value_scale_of_zero(form):
+    """A page whose value scale is 0 holds zeros: it takes part in the softmax and adds nothing."""
+    c, table, q, lens = _queries(form, 1)
+    c.v_scale[table[:, 1].long()] = 0
+    _check_rows(q, c, table, lens)
+    c.v_scale.zero_()
+    assert (_check_rows(q, c, table, lens, causal=False) == 0).all()
