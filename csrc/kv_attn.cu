@@ -79,9 +79,7 @@ paged_attn_kernel(const AttnArgs A, const __grid_constant__ CUtensorMap tm_k, co
   __shared__ uint64_t s_bar[kWarps][ST];
   __shared__ int64_t s_scan[kWarps], s_start[kWarps / W][2];
 
-  // no pieces yet; the threads that set these are lanes of the warp that writes pieces
-  if (A.split && threadIdx.x < 2) A.part_head[(blockIdx.x * 2 + threadIdx.x) * 4] = -1;
-  if (!tiles_aligned(s_ring, A.err)) return;
+  tiles_aligned(s_ring, A.err);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int part = W == 1 ? 0 : warp;                       // of the segment's warps
   const int g = lane >> 2, qd = lane & 3;
@@ -177,6 +175,7 @@ paged_attn_kernel(const AttnArgs A, const __grid_constant__ CUtensorMap tm_k, co
       c.limits(A);
     }
   }
+  if (A.split && threadIdx.x < 2) A.part_head[(blockIdx.x * 2 + threadIdx.x) * 4] = -1;
   if (c.left <= 0) return;                  // a whole block for W > 1, a warp for W = 1
 
   // ---- producer: this warp's tile of each unit ----
@@ -402,6 +401,10 @@ paged_attn_kernel(const AttnArgs A, const __grid_constant__ CUtensorMap tm_k, co
             irel[i] = exp2f_approx(-lrel[i]);
           }
         }
+        float f_top = 0.f;
+#pragma unroll
+        for (int i = 0; i < TS; ++i) f_top = fmaxf(f_top, fmaxf(f0[i], f1[i]));
+        const bool large = __any_sync(0xffffffffu, f_top >= kLargeFactor);
         constexpr int PS = SF / TS;                                   // fragments of a step of 16 keys
 #pragma unroll
         for (int i = 0; i < TS; ++i) {
@@ -426,7 +429,21 @@ paged_attn_kernel(const AttnArgs A, const __grid_constant__ CUtensorMap tm_k, co
         m0 = x0;
         m1 = x1;
         // ---- probabilities (times 2^15) and their sum ----
-        const float z0 = 15.f - b0, z1 = 15.f - b1;
+        float z0 = 15.f - b0, z1 = 15.f - b1;
+        if (large) {
+#pragma unroll
+          for (int i = 0; i < TS; ++i) {
+#pragma unroll
+            for (int j = PS * i; j < PS * i + PS; ++j)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                const bool second = R == 16 ? e >> 1 : e & 1;
+                s[j][e] = score_diff(s[j][e], second ? f1[i] : f0[i], second ? b1 : b0);
+              }
+            f0[i] = f1[i] = 1.f;
+          }
+          z0 = z1 = 15.f;
+        }
         uint64_t sum = pk2(0.f, 0.f), sum2 = pk2(0.f, 0.f);          // R = 16: row a and row b apart; R = 8: (a, b)
         uint32_t pf[TS][4];
 #pragma unroll
@@ -910,6 +927,7 @@ paged_attn_many_kernel(const AttnArgs A, const __grid_constant__ CUtensorMap tm_
         lv[i] = s_lv[st][pg];
         iv[i] = exp2f_approx(-lv[i]);
       }
+      const bool large = __any_sync(0xffffffffu, fmaxf(ks[0], ks[1]) * fmaxf(rs[0], rs[1]) >= kLargeFactor);
       bool grows = false;
       float x[2];
 #pragma unroll
@@ -944,12 +962,21 @@ paged_attn_many_kernel(const AttnArgs A, const __grid_constant__ CUtensorMap tm_
       // ---- probabilities (times 2^7 and the page's relative value scale) and their sum ----
       uint32_t pf[TS][4];
       {
-        const float z0 = 7.f - (m[0] == -INFINITY ? 0.f : m[0]), z1 = 7.f - (m[1] == -INFINITY ? 0.f : m[1]);
+        const float b0 = m[0] == -INFINITY ? 0.f : m[0], b1 = m[1] == -INFINITY ? 0.f : m[1];
+        float z0 = 7.f - b0, z1 = 7.f - b1;
+        if (large) {
+#pragma unroll
+          for (int j = 0; j < NT; ++j)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              s[j][e] = score_diff(s[j][e], fmaxf(ks[j / 2] * rs[e >> 1], kTiny), e >> 1 ? b1 : b0);
+          z0 = z1 = 7.f;
+        }
         uint64_t sum0 = pk2(0.f, 0.f), sum1 = pk2(0.f, 0.f);
 #pragma unroll
         for (int i = 0; i < TS; ++i) {
-          const uint64_t fa = pk2s(fmaxf(ks[i] * rs[0], kTiny)), za = pk2s(z0 + lv[i]);
-          const uint64_t fb = pk2s(fmaxf(ks[i] * rs[1], kTiny)), zb = pk2s(z1 + lv[i]);
+          const uint64_t fa = pk2s(large ? 1.f : fmaxf(ks[i] * rs[0], kTiny)), za = pk2s(z0 + lv[i]);
+          const uint64_t fb = pk2s(large ? 1.f : fmaxf(ks[i] * rs[1], kTiny)), zb = pk2s(z1 + lv[i]);
           uint64_t pa, pb;
 #pragma unroll
           for (int c = 0; c < 2; ++c) {

@@ -139,6 +139,13 @@ __device__ __forceinline__ float row_scale(float amax, float scale_log2, float& 
   back = __int_as_float((ex - 14 + 127) << 23) * fabsf(scale_log2);
   return copysignf(__int_as_float((14 - ex + 127) << 23), scale_log2);
 }
+// Scores (log2 domain) beyond some 2^18 are multiplied by their factor before the maximum is subtracted, in a rounding of
+// its own: the one fused operation that serves below leaves what the maximum's own rounding cut off, 2^-24 of it, which
+// passes the range of fp16 at 2^24. A product of a scaled query and codes is below 2^15 * 448 * d <= 2^31, so a factor
+// below this cannot get there; the check so stands off the chain from products to exponentials. Usual factors are some
+// 2^-20.
+constexpr float kLargeFactor = 1.220703125e-4f;             // 2^-13
+__device__ __forceinline__ float score_diff(float s, float f, float base) { return __fsub_rn(__fmul_rn(s, f), base); }
 // the least factor of scores: 0 would turn a masked score's -inf into NaN
 constexpr float kTiny = 1.17549435e-38f;
 

@@ -364,7 +364,7 @@ paged_attn_tc_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       mbar_arrive(&q_full);
     }
-    float m = -1e30f;
+    float m = -INFINITY;
     uint64_t l2 = pk2(0.f, 0.f);
     bool ok = true;
     for (int t = 0; t < units && ok && !aborted(); ++t) {
@@ -372,12 +372,27 @@ paged_attn_tc_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__
       ok = wait(&sc_full[e], t / kSc) && wait(&s_full[sl], t / kOps);
       if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
       tc_after();
+      float f[4], lv[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int pg = (16 * i) >> A.logP;
+        f[i] = fmaxf(s_ks[e][pg] * rs, kTiny);
+        lv[i] = s_lv[e][pg];
+      }
+      const bool large = __any_sync(0xffffffffu, fmaxf(fmaxf(f[0], f[1]), fmaxf(f[2], f[3])) >= kLargeFactor);
       uint32_t sr[64];
       tm_ld32(lane_base + kUnit * sl, sr);
       tm_ld32(lane_base + kUnit * sl + 32, sr + 32);
       tm_ld_wait(sr);
       tm_ld_wait(sr + 32);
       const uint32_t gone = s_gone[e];
+      if (large) {
+        // the products of scores and factors are rounded by themselves, as those of the maximum are; 7 - m is then at most
+        // 8 - m in 32 bits, and no score passes m
+#pragma unroll
+        for (int c = 0; c < 64; ++c) sr[c] = __float_as_uint(__fmul_rn(__uint_as_float(sr[c]), f[c / 16]));
+        f[0] = f[1] = f[2] = f[3] = 1.f;
+      }
       const int see = my_lim - k0;                          // columns c < see are visible
       if (__any_sync(0xffffffffu, see < kUnit)) {
 #pragma unroll
@@ -389,13 +404,9 @@ paged_attn_tc_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__
         for (int c = 0; c < 64; ++c)
           if (gone >> (c >> A.logP) & 1) sr[c] = __float_as_uint(-INFINITY);
       }
-      float f[4], lv[4];
       float mx = -INFINITY;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const int pg = (16 * i) >> A.logP;
-        f[i] = fmaxf(s_ks[e][pg] * rs, kTiny);
-        lv[i] = s_lv[e][pg];
         float y0 = -INFINITY, y1 = -INFINITY;
 #pragma unroll
         for (int c = 16 * i; c < 16 * i + 16; c += 4) {
@@ -404,7 +415,7 @@ paged_attn_tc_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__
         }
         mx = fmaxf(mx, fmaxf(y0, y1) * f[i]);
       }
-      const bool need = mx > m + 8.f;
+      const bool need = mx > m + (large ? 0.f : 8.f);
       const float top_m = need ? mx : m;
       if (__any_sync(0xffffffffu, need)) {
         const float al = need ? exp2f_approx(m - top_m) : 1.f;
@@ -427,10 +438,11 @@ paged_attn_tc_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__
         l2 = pk2_mul(l2, pk2s(al));
         m = top_m;
       }
+      const float z = m == -INFINITY ? 7.f : 7.f - m;
       uint32_t pk[32];
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const uint64_t ff = pk2s(f[i]), zz = pk2s(7.f - m + lv[i]);
+        const uint64_t ff = pk2s(f[i]), zz = pk2s(z + lv[i]);
         uint64_t s0 = pk2(0.f, 0.f), s1 = s0;
 #pragma unroll
         for (int c = 16 * i; c < 16 * i + 16; c += 2) {

@@ -190,3 +190,22 @@ def test_value_scale_of_zero(form):
     _check_rows(q, c, table, lens)
     c.v_scale.zero_()
     assert (_check_rows(q, c, table, lens, causal=False) == 0).all()
+
+
+@pytest.mark.parametrize("form", FORMS)
+def test_scores_of_large_magnitude(form):
+    """Scores far below -1e30: the largest of them still takes the whole probability."""
+    c, table, q, lens = _queries(form, 2)
+    c.k.view(torch.uint8).fill_(0x38)                                # keys of 1.0 times their scale
+    c.k_scale.fill_(2.0 ** 60)
+    first = table[:, 0].long()
+    c.k.view(torch.uint8)[first, :, 3] = 0x30                        # the fourth key of each sequence: 0.5
+    q.fill_(-2.0 ** 60)
+    q.view(torch.int16)[..., 0] ^= 1                                 # queries that are not all alike
+    from primus_dlrm_b200.ops.kv_cache import paged_attention
+    o, lse = paged_attention(q, c, table, lens, return_lse=True, causal=False)
+    G = q.shape[2] // c.n_kv_heads
+    v = (c.v.view(torch.uint8)[first, :, 3].view(E4M3).float() * c.v_scale[first][..., None]).repeat_interleave(G, 1)
+    assert torch.equal(o, v[:, None].expand(o.shape).to(o.dtype))    # an e4m3 code times 2^e is a bf16 number
+    assert torch.isfinite(lse).all() and (lse < -1e30).all()
+    c.check_errors()
