@@ -36,6 +36,10 @@ __device__ __noinline__ void drain(uint32_t bars, uint32_t slots, uint32_t st, u
   }
 }
 
+// Sums of 2^15 p v are held in this unit (few rows): 65536 of the largest 32-bit numbers fit, and the smallest page scale
+// times it still has 18 bits.
+constexpr float kSumUnit = 0x1p-31f;
+
 // Few rows to a segment (one or some query tokens of one sequence, the heads
 // that share a key head): bound by reading the cache.
 //
@@ -492,7 +496,8 @@ paged_attn_kernel(const AttnArgs A, const __grid_constant__ CUtensorMap tm_k, co
               for (int w = 0; w < D / 32; ++w) vw[i][r][w] = drop ? 0u : vw[i][r][w];
             }
         }
-        const uint64_t alx = R == 16 ? pk2s(al0) : pk2(al0, al1), aly = R == 16 ? pk2s(al1) : alx, vr = pk2s(vref);
+        const uint64_t alx = R == 16 ? pk2s(al0) : pk2(al0, al1), aly = R == 16 ? pk2s(al1) : alx;
+        const uint64_t vr = pk2s(vref * kSumUnit);
 #pragma unroll
         for (int w = 0; w < D / 32; ++w) {
           constexpr int F = R / 4;                                    // output fragments of four of the lane's dims
@@ -590,7 +595,7 @@ paged_attn_kernel(const AttnArgs A, const __grid_constant__ CUtensorMap tm_k, co
     if (part == 0) {
       if (begins && ends) {
         // a sum of 0: no keys. A NaN stays one
-        const float i0 = l0 == 0.f ? 0.f : 1.f / l0, i1 = l1 == 0.f ? 0.f : 1.f / l1;
+        const float i0 = l0 == 0.f ? 0.f : 1.f / kSumUnit / l0, i1 = l1 == 0.f ? 0.f : 1.f / kSumUnit / l1;
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
           const int r = r0 + (i ? row_b : row_a);
@@ -692,7 +697,7 @@ __global__ void __launch_bounds__(256) paged_attn_join_kernel(const AttnArgs A) 
   __syncthreads();
   if (gr > 0) return;
   for (int i = 1; i < min(GR, hd.w + 1); ++i) take(s_m[i], s_l[i], s_o[i][ln]);
-  const float inv = l == 0.f ? 0.f : 1.f / l;
+  const float inv = l == 0.f ? 0.f : 1.f / kSumUnit / l;
   const int qi = r / A.G;
   const int64_t at = int64_t(S.tok0 + qi) * A.Hq + hd.y * A.G + (r - qi * A.G);
   *reinterpret_cast<uint2*>(static_cast<uint16_t*>(A.o) + at * D + ln * 4) =

@@ -209,3 +209,15 @@ def test_scores_of_large_magnitude(form):
     assert torch.equal(o, v[:, None].expand(o.shape).to(o.dtype))    # an e4m3 code times 2^e is a bf16 number
     assert torch.isfinite(lse).all() and (lse < -1e30).all()
     c.check_errors()
+
+
+@pytest.mark.parametrize("form", FORMS)
+def test_values_near_the_largest(form):
+    """Values whose sums over the keys would pass the largest 32-bit number."""
+    c, table, q, lens = _queries(form, 3)
+    c.v.view(torch.uint8)[:] &= 0x7F                                 # all of one sign, so that sums do not cancel
+    c.v.copy_(c.v.float().clamp(min=240).to(E4M3))
+    c.v_scale.fill_(2.0 ** 119)                                      # up to 448 * 2^119 = 2^127.8
+    _check_rows(q, c, table, lens)
+    c.v_scale.fill_(2.0 ** -100)                                     # and the smallest scale
+    _check_rows(q, c, table, lens)
