@@ -10,10 +10,11 @@
 // operands with 32-bit sums and no rounding of the cache's values: a query row
 // is scaled by the power of two that brings its largest magnitude to
 // [2^14, 2^15) (elements down to 2^-29 of it keep all bits of bf16) and the
-// softmax scale undoes it; probabilities are held as 2^15 p, which keeps 11
-// bits down to 2^-29 and reaches 2^-39. A page's key scale multiplies its
-// scores in 32 bits; its value scale, relative to the largest of the tile's
-// pages, its probabilities. Running maximum, sum and output stay in 32 bits.
+// softmax scale undoes it. A page's key scale multiplies its scores in 32 bits,
+// its value scale t = log2 its probabilities, in the exponent: a row's operand
+// of the second product is 2^15 2^(s + t - w) with w the largest s + t of the
+// tile's keys that it sees, 11 bits down to 2^-29 of the largest product and
+// some down to 2^-39. Running maximum, sum (without t) and output stay in 32 bits.
 #include "kv_attn.cuh"
 
 namespace pd {
@@ -38,7 +39,7 @@ __device__ __noinline__ void drain(uint32_t bars, uint32_t slots, uint32_t st, u
 
 // Sums of 2^15 p v are held in this unit (few rows): 65536 of the largest 32-bit numbers fit, and the smallest page scale
 // times it still has 18 bits.
-constexpr float kSumUnit = 0x1p-31f;
+constexpr float kSumUnit = 0x1p-31f, kSumLog2 = -31.f;
 
 // Few rows to a segment (one or some query tokens of one sequence, the heads
 // that share a key head): bound by reading the cache.
@@ -57,15 +58,18 @@ constexpr float kSumUnit = 0x1p-31f;
 // neighbours: lane % 4 owns a quarter of a key's dims, lane / 4 an eighth of a
 // value's, and keys go to registers in the order of memory.
 //
+// ONE: pages hold whole tiles, which then have one pair of scales each (the
+// single tokens below 113 us, the candidates 134; the general form 126 and 152).
+//
 // B200: 64 single tokens over 300 to 8191 keys, 32 heads over 8 x 128 (R = 8):
-// 114 us, 4.9 TB/s of the cache (floor 85 us); three over 65537 to 131071 keys, 16
-// heads over 4 x 64, pages of 16: 43 us, 3.5 TB/s (floor 23 us). Neither pipe is full (issue
+// 113 us, 4.9 TB/s of the cache (floor 85 us); three over 65537 to 131071 keys, 16
+// heads over 4 x 64, pages of 16: 44 us, 3.5 TB/s (floor 23 us). Neither pipe is full (issue
 // slots 37%, DRAM 75%): 12 warps an SM, bound by registers, wait on their own
 // chains. 1024 x 16 candidate tokens behind 896 shared keys, 8 x 32 (R = 16, W =
-// 1): 140 us; the keys come from L2 and the instructions around 16-row products
+// 1): 134 us; the keys come from L2 and the instructions around 16-row products
 // bound it (issue 55% of active cycles; a copy's bookkeeping is 30% of them: 64
 // keys a copy instead of 128 cost 179 us).
-template <int D, int R, int W>
+template <int D, int R, int W, bool ONE>
 __global__ void __launch_bounds__(kWarps * 32, D == 128 && R == 16 ? 2 : 3)
 paged_attn_kernel(const AttnArgs A, const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v) {
   constexpr int TK = Cfg<D>::TK, SUB = Cfg<D>::SUB, ST = Cfg<D>::ST;
@@ -187,7 +191,7 @@ paged_attn_kernel(const AttnArgs A, const __grid_constant__ CUtensorMap tm_k, co
   // flight; `gone` has a bit for each of its pages that is not loaded (behind the keys, or no such page).
   Cursor<R> p = c;
   int page = -1;                            // lane i: id of page i of the tile at p
-  const int box = min(A.P, TK), boxes = WK / box, box_log = min(A.logP, TK == 64 ? 6 : 5);
+  const int box = ONE ? TK : A.P, boxes = WK / box, box_log = ONE ? (TK == 64 ? 6 : 5) : A.logP;
   float scl[ST];
   uint32_t gone[ST];
 #pragma unroll
@@ -303,7 +307,7 @@ paged_attn_kernel(const AttnArgs A, const __grid_constant__ CUtensorMap tm_k, co
     int used = 0;                           // units of the segment so far, for a segment that begins here
     do {
       issue(st == 0 ? ST - 1 : st - 1, scl[ST - 1], gone[ST - 1]);    // refills the slot of the tile before
-      const float my_scl = scl[0];
+      const float my_scl = scl[0], my_lv = scale_log2_of(my_scl);
       const uint32_t my_gone = gone[0];
       if (alive) {
         alive = __all_sync(0xffffffffu, mbar_wait(bars + st * 8, phase, A.err));
@@ -372,68 +376,60 @@ paged_attn_kernel(const AttnArgs A, const __grid_constant__ CUtensorMap tm_k, co
               if (missing >> (at >> box_log) & 1) s[j][e] = -INFINITY;
             }
         }
-        // ---- running maximum ----
-        float vref, f0[TS], f1[TS], lrel[TS], irel[TS];               // by step of 16 keys
-        float x0 = -INFINITY, x1 = -INFINITY;
-        if (box == TK) {
-          const float ks = __shfl_sync(0xffffffffu, my_scl, pg0);
-          vref = __shfl_sync(0xffffffffu, my_scl, pg0 + NP);
+        // ---- running maximum, and the largest product of probability and value scale of the tile ----
+        float f0[TS], f1[TS], lv[TS];                                 // by step of 16 keys (ONE: all alike)
 #pragma unroll
-          for (int i = 0; i < TS; ++i) {
-            f0[i] = fmaxf(ks * rs0, kTiny);
-            f1[i] = fmaxf(ks * rs1, kTiny);
-            lrel[i] = 0.f;
-            irel[i] = 1.f;
+        for (int i = 0; i < TS; ++i) {
+          if (ONE && i > 0) {
+            f0[i] = f0[0], f1[i] = f1[0], lv[i] = lv[0];
+            continue;
           }
-        } else {
-          vref = 0.f;
-#pragma unroll
-          for (int i = 0; i < TS; ++i) {
-            const int pg = pg0 + ((i * 16) >> box_log);
-            const float ks = __shfl_sync(0xffffffffu, my_scl, pg);
-            f0[i] = fmaxf(ks * rs0, kTiny);
-            f1[i] = fmaxf(ks * rs1, kTiny);
-            irel[i] = __shfl_sync(0xffffffffu, my_scl, pg + NP);
-            vref = fmaxf(vref, irel[i]);
-          }
-          // A page's value scale relative to vref goes into the exponent, and out of the sum again. Below 2^-60, a scale
-          // of 0 among them, its probabilities are zeros in fp16 whatever they are; a page not loaded has none.
-          const float lref = __log2f(vref);
-#pragma unroll
-          for (int i = 0; i < TS; ++i) {
-            lrel[i] = irel[i] > 0.f ? fmaxf(__log2f(irel[i]) - lref, -60.f) : -60.f;
-            irel[i] = exp2f_approx(-lrel[i]);
-          }
+          const int pg = pg0 + (ONE ? 0 : (i * 16) >> box_log);
+          const float ks = __shfl_sync(0xffffffffu, my_scl, pg);
+          f0[i] = fmaxf(ks * rs0, kTiny);
+          f1[i] = fmaxf(ks * rs1, kTiny);
+          lv[i] = __shfl_sync(0xffffffffu, my_lv, pg + NP);
         }
         float f_top = 0.f;
 #pragma unroll
         for (int i = 0; i < TS; ++i) f_top = fmaxf(f_top, fmaxf(f0[i], f1[i]));
         const bool large = __any_sync(0xffffffffu, f_top >= kLargeFactor);
         constexpr int PS = SF / TS;                                   // fragments of a step of 16 keys
+        float x0 = -INFINITY, x1 = -INFINITY, v0 = -INFINITY, v1 = -INFINITY;
+        auto reduce = [&](float& a, float& b) {                       // over the lanes of a row
 #pragma unroll
-        for (int i = 0; i < TS; ++i) {
-          float y0 = -INFINITY, y1 = -INFINITY;
-#pragma unroll
-          for (int j = PS * i; j < PS * i + PS; ++j) {
-            y0 = fmaxf(y0, fmaxf(s[j][0], s[j][R == 16 ? 1 : 2]));
-            y1 = fmaxf(y1, fmaxf(s[j][R == 16 ? 2 : 1], s[j][3]));
+          for (int t = R == 16 ? 1 : 4; t < (R == 16 ? 4 : 32); t *= 2) {
+            a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, t));
+            b = fmaxf(b, __shfl_xor_sync(0xffffffffu, b, t));
           }
-          x0 = fmaxf(x0, y0 * f0[i]);
-          x1 = fmaxf(x1, y1 * f1[i]);
-        }
+        };
+        auto maxima = [&]() {
 #pragma unroll
-        for (int t = R == 16 ? 1 : 4; t < (R == 16 ? 4 : 32); t *= 2) {
-          x0 = fmaxf(x0, __shfl_xor_sync(0xffffffffu, x0, t));
-          x1 = fmaxf(x1, __shfl_xor_sync(0xffffffffu, x1, t));
-        }
-        x0 = fmaxf(x0, m0);
-        x1 = fmaxf(x1, m1);
-        const float b0 = x0 == -INFINITY ? 0.f : x0, b1 = x1 == -INFINITY ? 0.f : x1;
+          for (int i = 0; i < TS; ++i) {
+            float y0 = -INFINITY, y1 = -INFINITY;
+#pragma unroll
+            for (int j = PS * i; j < PS * i + PS; ++j) {
+              y0 = fmaxf(y0, fmaxf(s[j][0], s[j][R == 16 ? 1 : 2]));
+              y1 = fmaxf(y1, fmaxf(s[j][R == 16 ? 2 : 1], s[j][3]));
+            }
+            x0 = fmaxf(x0, y0 * f0[i]);
+            x1 = fmaxf(x1, y1 * f1[i]);
+            if (!ONE) {
+              v0 = fmaxf(v0, fmaf(y0, f0[i], lv[i]));
+              v1 = fmaxf(v1, fmaf(y1, f1[i], lv[i]));
+            }
+          }
+          reduce(x0, x1);
+          if (!ONE) reduce(v0, v1);
+        };
+        maxima();
+        const float n0 = fmaxf(x0, m0), n1 = fmaxf(x1, m1);
+        const float b0 = n0 == -INFINITY ? 0.f : n0, b1 = n1 == -INFINITY ? 0.f : n1;
         const float al0 = exp2f_approx(m0 - b0), al1 = exp2f_approx(m1 - b1);
-        m0 = x0;
-        m1 = x1;
-        // ---- probabilities (times 2^15) and their sum ----
+        m0 = n0;
+        m1 = n1;
         float z0 = 15.f - b0, z1 = 15.f - b1;
+        float w0 = ONE ? (x0 - b0) + lv[0] : v0 - b0, w1 = ONE ? (x1 - b1) + lv[0] : v1 - b1;
         if (large) {
 #pragma unroll
           for (int i = 0; i < TS; ++i) {
@@ -447,14 +443,32 @@ paged_attn_kernel(const AttnArgs A, const __grid_constant__ CUtensorMap tm_k, co
             f0[i] = f1[i] = 1.f;
           }
           z0 = z1 = 15.f;
+          if (!ONE) {
+            v0 = v1 = -INFINITY;
+            maxima();
+            w0 = v0;
+            w1 = v1;
+          }
         }
+        // log2 of the row's reference for this tile, relative to its running maximum; no key in sight: any
+        w0 = fmaxf(w0, kLeastScale - 100.f);
+        w1 = fmaxf(w1, kLeastScale - 100.f);
+        // ---- probabilities (times 2^15 and the page's relative value scale) and their sum ----
         uint64_t sum = pk2(0.f, 0.f), sum2 = pk2(0.f, 0.f);          // R = 16: row a and row b apart; R = 8: (a, b)
         uint32_t pf[TS][4];
+        float c0, c1, i0, i1;                                         // log2 of the page's factor, and what takes it out
 #pragma unroll
         for (int i = 0; i < TS; ++i) {
-          const float y0 = z0 + lrel[i], y1 = z1 + lrel[i];
-          const uint64_t fa = R == 16 ? pk2s(f0[i]) : pk2(f0[i], f1[i]), za = R == 16 ? pk2s(y0) : pk2(y0, y1);
-          const uint64_t fb = R == 16 ? pk2s(f1[i]) : fa, zb = R == 16 ? pk2s(y1) : za;
+          if (!ONE || i == 0) {
+            c0 = fmaxf(lv[i] - w0, kLeastRel);
+            c1 = fmaxf(lv[i] - w1, kLeastRel);
+            i0 = exp2f_approx(-c0);
+            i1 = exp2f_approx(-c1);
+            c0 += z0;
+            c1 += z1;
+          }
+          const uint64_t fa = R == 16 ? pk2s(f0[i]) : pk2(f0[i], f1[i]), za = R == 16 ? pk2s(c0) : pk2(c0, c1);
+          const uint64_t fb = R == 16 ? pk2s(f1[i]) : fa, zb = R == 16 ? pk2s(c1) : za;
           uint64_t part_a, part_b;
 #pragma unroll
           for (int t = 0; t < PS; ++t) {
@@ -471,8 +485,9 @@ paged_attn_kernel(const AttnArgs A, const __grid_constant__ CUtensorMap tm_k, co
             pf[i][2 * t] = pack_f16(p0, p1);
             pf[i][2 * t + 1] = pack_f16(p2, p3);
           }
-          sum = pk2_fma(part_a, pk2s(irel[i]), sum);
-          sum2 = pk2_fma(part_b, pk2s(irel[i]), sum2);
+          const uint64_t ia = R == 16 ? pk2s(i0) : pk2(i0, i1), ib = R == 16 ? pk2s(i1) : ia;
+          sum = pk2_fma(part_a, ia, sum);
+          sum2 = pk2_fma(part_b, ib, sum2);
           if constexpr (R == 8) {
             pf[i][0] = transpose8(pf[i][0]);
             pf[i][1] = transpose8(pf[i][1]);
@@ -497,7 +512,8 @@ paged_attn_kernel(const AttnArgs A, const __grid_constant__ CUtensorMap tm_k, co
             }
         }
         const uint64_t alx = R == 16 ? pk2s(al0) : pk2(al0, al1), aly = R == 16 ? pk2s(al1) : alx;
-        const uint64_t vr = pk2s(vref * kSumUnit);
+        const float ref0 = exp2f_small(w0 + kSumLog2), ref1 = exp2f_small(w1 + kSumLog2);
+        const uint64_t vrx = R == 16 ? pk2s(ref0) : pk2(ref0, ref1), vry = R == 16 ? pk2s(ref1) : vrx;
 #pragma unroll
         for (int w = 0; w < D / 32; ++w) {
           constexpr int F = R / 4;                                    // output fragments of four of the lane's dims
@@ -527,8 +543,8 @@ paged_attn_kernel(const AttnArgs A, const __grid_constant__ CUtensorMap tm_k, co
 #pragma unroll
           for (int e = 0; e < F; ++e) {
             float* ou = o[F * w + e];
-            pk2_split(pk2_fma(pk2(acc[e][0], acc[e][1]), vr, pk2_mul(pk2(ou[0], ou[1]), alx)), ou[0], ou[1]);
-            pk2_split(pk2_fma(pk2(acc[e][2], acc[e][3]), vr, pk2_mul(pk2(ou[2], ou[3]), aly)), ou[2], ou[3]);
+            pk2_split(pk2_fma(pk2(acc[e][0], acc[e][1]), vrx, pk2_mul(pk2(ou[0], ou[1]), alx)), ou[0], ou[1]);
+            pk2_split(pk2_fma(pk2(acc[e][2], acc[e][3]), vry, pk2_mul(pk2(ou[2], ou[3]), aly)), ou[2], ou[3]);
           }
         }
       }
@@ -710,15 +726,17 @@ __global__ void __launch_bounds__(256) paged_attn_join_kernel(const AttnArgs A) 
 // A block takes 64 rows, 16 a warp, of one sequence and key head; its warps
 // share copies of 64 keys that warp 0 has TMA load a copy ahead. Queries wait
 // in shared memory in the order of their fragments, which leaves registers for
-// three blocks an SM. Value scales are taken relative to the largest of all
-// pages that the block reads, so that products go straight into the output;
-// the output is scaled only when some row's maximum has grown by more than 2^8
-// (probabilities are held as 2^7 p and reach 2^15). Blocks with many keys come
-// first. With 16 rows a warp every code is converted for 16 rows' products; 32
+// three blocks an SM. Value scales are taken relative to a reference of each
+// row, so that products go straight into the output; the output is scaled only
+// when some row's maximum, or its reference (the largest product of probability
+// and scale that it has seen), has grown by more than 2^8 (products are held
+// times 2^7 and reach 2^15). Blocks with many keys come first. With 16 rows a warp every code is converted for 16 rows' products; 32
 // rows a warp need more registers than two blocks an SM leave at d = 128.
-// B200: 40 sequences x 8 heads x 256 rows over 1000 keys: 166 us (16-row form: 274).
+// B200: 40 sequences x 8 heads x 256 rows over 1000 keys, pages of 64: 176 us
+// (16-row form: 274); of 16, whose tiles have two pairs of scales: 202 us.
 constexpr int kManyRows = 16 * kWarps, kManyCopies = 3;
 
+template <bool ONE>                       // a page holds a whole tile of 32 keys
 __global__ void __launch_bounds__(kWarps * 32, 3)
 paged_attn_many_kernel(const AttnArgs A, const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v) {
   constexpr int D = 128, TK = 32, ST = kManyCopies, R = kManyRows;
@@ -727,9 +745,8 @@ paged_attn_many_kernel(const AttnArgs A, const __grid_constant__ CUtensorMap tm_
   extern __shared__ __align__(1024) uint8_t s_ring[];       // [ST] copies: 64 rows of keys, 64 rows of values
   __shared__ uint4 s_q[kWarps][KS][32];
   __shared__ uint64_t s_full[ST], s_empty[ST];
-  __shared__ float s_ks[ST][4], s_lv[ST][4];                // scales of a copy's pages: keys, log2 of values' (relative)
+  __shared__ float s_ks[ST][4], s_lv[ST][4];                // scales of a copy's pages: keys, log2 of values'
   __shared__ uint32_t s_gone[ST];
-  __shared__ float s_top[kWarps];
   __shared__ volatile int s_abort;          // a wait has run out: every warp leaves its loop
 
   if (!tiles_aligned(s_ring, A.err)) return;
@@ -749,17 +766,7 @@ paged_attn_many_kernel(const AttnArgs A, const __grid_constant__ CUtensorMap tm_
     asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(smem_u32(&s_empty[threadIdx.x])), "r"(kWarps));
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
-  // the largest value scale of the block's pages
-  float top = 0.f;
-  for (int i = threadIdx.x; i * A.P < lim; i += kWarps * 32) {
-    const int page = __ldg(table + i);
-    if (page >= 0 && page < A.n_pages) top = fmaxf(top, __ldg(A.vs + page * A.H + h));
-  }
-  top = warp_max(top);
-  if (lane == 0) s_top[warp] = top;
   __syncthreads();
-#pragma unroll
-  for (int w = 0; w < kWarps; ++w) top = fmaxf(top, s_top[w]);
 
   // ---- copies (warp 0): those of unit v, then, a step later, its pages' scales ----
   const uint32_t ring = smem_u32(s_ring);
@@ -776,8 +783,7 @@ paged_attn_many_kernel(const AttnArgs A, const __grid_constant__ CUtensorMap tm_
     if (pending < 0) return;
     if (lane < boxes) {
       s_ks[pending][lane] = new_ks;
-      // below 2^-60 of the largest its probabilities are zeros in fp16 whatever they are
-      s_lv[pending][lane] = new_vs > 0.f ? fmaxf(__log2f(new_vs) - __log2f(top), -60.f) : -60.f;
+      s_lv[pending][lane] = scale_log2_of(new_vs);
     }
     if (lane == 0) s_gone[pending] = new_gone;
     __syncwarp();
@@ -866,7 +872,8 @@ paged_attn_many_kernel(const AttnArgs A, const __grid_constant__ CUtensorMap tm_
   }
   uint32_t k_off, v_off[2];
   lane_offsets<D>(g, qd, k_off, v_off);
-  float o[NO][4], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+  // running maxima and sums; log2 of the rows' value references, relative to the maxima
+  float o[NO][4], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f}, w[2] = {0.f, 0.f};
 #pragma unroll
   for (int u = 0; u < NO; ++u) o[u][0] = o[u][1] = o[u][2] = o[u][3] = 0.f;
   uint32_t st = 0, phase = 0;
@@ -923,38 +930,53 @@ paged_attn_many_kernel(const AttnArgs A, const __grid_constant__ CUtensorMap tm_
             if (drop || key >= lims[1]) s[j][2 + e] = -INFINITY;
           }
       }
-      // ---- scores of the pages: maxima in the log2 domain ----
-      float ks[TS], lv[TS], iv[TS];
+      // ---- maxima in the log2 domain: scores, and scores times value scales ----
+      float ks[TS], lv[TS];
 #pragma unroll
       for (int i = 0; i < TS; ++i) {
-        const int pg = (sub * TK + 16 * i) >> A.logP;
-        ks[i] = s_ks[st][pg];
-        lv[i] = s_lv[st][pg];
-        iv[i] = exp2f_approx(-lv[i]);
+        const int pg = (sub * TK + (ONE ? 0 : 16 * i)) >> A.logP;
+        ks[i] = ONE && i > 0 ? ks[0] : s_ks[st][pg];
+        lv[i] = ONE && i > 0 ? lv[0] : s_lv[st][pg];
       }
       const bool large = __any_sync(0xffffffffu, fmaxf(ks[0], ks[1]) * fmaxf(rs[0], rs[1]) >= kLargeFactor);
       bool grows = false;
-      float x[2];
+      float n[2], x[2], seen_w[2];          // running maximum to come; log2 of the reference, and what it would have to be
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        float y = -INFINITY;
+        float y[TS], top = -INFINITY, v = -INFINITY;
 #pragma unroll
-        for (int k = 0; k < TS; ++k)
-          y = fmaxf(y, fmaxf(fmaxf(s[2 * k][2 * i], s[2 * k][2 * i + 1]), fmaxf(s[2 * k + 1][2 * i], s[2 * k + 1][2 * i + 1])) *
-                           fmaxf(ks[k] * rs[i], kTiny));
-        y = fmaxf(y, __shfl_xor_sync(0xffffffffu, y, 1));
-        y = fmaxf(y, __shfl_xor_sync(0xffffffffu, y, 2));
-        x[i] = y;
-        grows |= y > m[i] + 8.f;
+        for (int k = 0; k < TS; ++k) {
+          y[k] = fmaxf(fmaxf(s[2 * k][2 * i], s[2 * k][2 * i + 1]), fmaxf(s[2 * k + 1][2 * i], s[2 * k + 1][2 * i + 1])) *
+                 fmaxf(ks[k] * rs[i], kTiny);
+          top = fmaxf(top, y[k]);
+          v = fmaxf(v, y[k] + lv[k]);
+        }
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        if (!ONE) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 1));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        if (!ONE) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 2));
+        n[i] = top > m[i] + 8.f ? top : m[i];
+        const float base = n[i] == -INFINITY ? 0.f : n[i];
+        v = ONE ? (top - base) + lv[0] : v - base;
+        if (!ONE && large) {                        // differences first: the sum above has lost the scales
+          v = -INFINITY;
+#pragma unroll
+          for (int k = 0; k < TS; ++k) v = fmaxf(v, (y[k] - base) + lv[k]);
+          v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 1));
+          v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 2));
+        }
+        x[i] = n[i] == m[i] ? w[i] : w[i] + (m[i] - n[i]);
+        seen_w[i] = v;
+        grows |= top > m[i] + 8.f || v > x[i] + 8.f;
       }
       if (__any_sync(0xffffffffu, grows)) {
         float al[2];
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-          const float n = x[i] > m[i] + 8.f ? x[i] : m[i];
-          al[i] = m[i] == n ? 1.f : exp2f_approx(m[i] - n);
-          m[i] = n;
-          l[i] *= al[i];
+          if (m[i] != n[i]) l[i] *= exp2f_approx(m[i] - n[i]);
+          m[i] = n[i];
+          w[i] = seen_w[i] > x[i] + 8.f ? seen_w[i] : x[i];
+          al[i] = exp2f_approx(x[i] - w[i]);
         }
 #pragma unroll
         for (int v = 0; v < NO; ++v) {
@@ -978,10 +1000,17 @@ paged_attn_many_kernel(const AttnArgs A, const __grid_constant__ CUtensorMap tm_
           z0 = z1 = 7.f;
         }
         uint64_t sum0 = pk2(0.f, 0.f), sum1 = pk2(0.f, 0.f);
+        float c0, c1, i0, i1;               // log2 of the page's factor, and what takes it out
 #pragma unroll
         for (int i = 0; i < TS; ++i) {
-          const uint64_t fa = pk2s(large ? 1.f : fmaxf(ks[i] * rs[0], kTiny)), za = pk2s(z0 + lv[i]);
-          const uint64_t fb = pk2s(large ? 1.f : fmaxf(ks[i] * rs[1], kTiny)), zb = pk2s(z1 + lv[i]);
+          if (!ONE || i == 0) {
+            c0 = fmaxf(lv[i] - w[0], kLeastRel);
+            c1 = fmaxf(lv[i] - w[1], kLeastRel);
+            i0 = exp2f_approx(-c0);
+            i1 = exp2f_approx(-c1);
+          }
+          const uint64_t fa = pk2s(large ? 1.f : fmaxf(ks[i] * rs[0], kTiny)), za = pk2s(z0 + c0);
+          const uint64_t fb = pk2s(large ? 1.f : fmaxf(ks[i] * rs[1], kTiny)), zb = pk2s(z1 + c1);
           uint64_t pa, pb;
 #pragma unroll
           for (int c = 0; c < 2; ++c) {
@@ -998,8 +1027,8 @@ paged_attn_many_kernel(const AttnArgs A, const __grid_constant__ CUtensorMap tm_
             pf[i][2 * c] = pack_f16(p0, p1);
             pf[i][2 * c + 1] = pack_f16(p2, p3);
           }
-          sum0 = pk2_fma(pa, pk2s(iv[i]), sum0);
-          sum1 = pk2_fma(pb, pk2s(iv[i]), sum1);
+          sum0 = pk2_fma(pa, pk2s(i0), sum0);
+          sum1 = pk2_fma(pb, pk2s(i1), sum1);
         }
         float a0, a1;
         pk2_split(sum0, a0, a1);
@@ -1056,25 +1085,26 @@ paged_attn_many_kernel(const AttnArgs A, const __grid_constant__ CUtensorMap tm_
     if (r >= rows) continue;
     const int qi = r / A.G;
     const int64_t at = int64_t(S.tok0 + qi) * A.Hq + h * A.G + (r - qi * A.G);
-    const float inv = sum == 0.f ? 0.f : top / sum;         // a sum of 0: no keys. A NaN stays one
+    // a sum of 0: no keys. A NaN stays one. The reference may be near the largest number: half of it at a time
+    const float half = exp2f_approx(0.5f * w[i]), inv = sum == 0.f ? 0.f : half / sum;
     uint16_t* dst = static_cast<uint16_t*>(A.o) + at * D + qd * (D / 4);
 #pragma unroll
     for (int c = 0; c < 2; ++c)
 #pragma unroll
       for (int u = 0; u < NO; u += 4)
         *reinterpret_cast<uint2*>(dst + c * NO + u) =
-            make_uint2(pack_16(o[u][2 * i + c] * inv, o[u + 1][2 * i + c] * inv, A.bf16),
-                       pack_16(o[u + 2][2 * i + c] * inv, o[u + 3][2 * i + c] * inv, A.bf16));
+            make_uint2(pack_16(o[u][2 * i + c] * inv * half, o[u + 1][2 * i + c] * inv * half, A.bf16),
+                       pack_16(o[u + 2][2 * i + c] * inv * half, o[u + 3][2 * i + c] * inv * half, A.bf16));
     if (A.lse && qd == 0) A.lse[at] = sum == 0.f ? -INFINITY : (m[i] - 7.f + log2f(sum)) * 0.6931471805599453f;
   }
 }
 
-template <int D, int R, int W>
+template <int D, int R, int W, bool ONE>
 static void few_launch(AttnArgs& A, const at::Tensor& ck, const at::Tensor& cv, const Bounds& U) {
   constexpr int TK = Cfg<D>::TK, WK = TK * Cfg<D>::SUB, SUP = WK * W;
   constexpr int kSmem = kWarps * Cfg<D>::ST * 2 * WK * D;
   static int known[64] = {};
-  auto kern = paged_attn_kernel<D, R, W>;
+  auto kern = paged_attn_kernel<D, R, W, ONE>;
   const int64_t slots = int64_t(num_sms()) * blocks_per_sm(kern, kWarps * 32, kSmem, known);
   const int64_t segments = U.B * A.H * ((U.rows + R - 1) / R);
   const int64_t units = std::max<int64_t>(1, (U.len + SUP - 1) / SUP);        // of the longest segment
@@ -1120,16 +1150,19 @@ static void few_dispatch(AttnArgs& A, const at::Tensor& ck, const at::Tensor& cv
   const int64_t segments = U.B * A.H * ((U.rows + R - 1) / R), warps = int64_t(num_sms()) * 12;
   const int64_t rounds = (segments + warps - 1) / warps;
   const bool one = U.len <= SUP ? segments >= int64_t(num_sms()) * 8 : rounds >= 3 && segments * 20 >= rounds * warps * 17;
-  if (one) few_launch<D, R, 1>(A, ck, cv, U);
-  else few_launch<D, R, 4>(A, ck, cv, U);
+  // pages that hold whole tiles of keys have one pair of scales a tile
+  if (A.P >= Cfg<D>::TK) one ? few_launch<D, R, 1, true>(A, ck, cv, U) : few_launch<D, R, 4, true>(A, ck, cv, U);
+  else one ? few_launch<D, R, 1, false>(A, ck, cv, U) : few_launch<D, R, 4, false>(A, ck, cv, U);
 }
 
+template <bool ONE>
 static void many_launch(AttnArgs& A, const at::Tensor& ck, const at::Tensor& cv, const Bounds& U) {
   constexpr int kSmem = kManyCopies * 2 * kUnit * 128;
   static int known[64] = {};
-  blocks_per_sm(paged_attn_many_kernel, kWarps * 32, kSmem, known);
+  auto kern = paged_attn_many_kernel<ONE>;
+  blocks_per_sm(kern, kWarps * 32, kSmem, known);
   const dim3 grid(unsigned(U.B * A.H), unsigned((U.rows + kManyRows - 1) / kManyRows));
-  paged_attn_many_kernel<<<grid, kWarps * 32, kSmem, stream()>>>(A, code_map(ck, A.P), code_map(cv, A.P));
+  kern<<<grid, kWarps * 32, kSmem, stream()>>>(A, code_map(ck, A.P), code_map(cv, A.P));
   PD_CHECK_LAUNCH();
 }
 
@@ -1158,7 +1191,7 @@ template <int D>
 static void attn_dispatch(AttnArgs& A, const at::Tensor& ck, const at::Tensor& cv, const Bounds& U) {
   if (use_many<D>(A, U)) {
     if constexpr (D <= 64) attn_tc_launch(A, ck, cv, D, U);
-    else many_launch(A, ck, cv, U);
+    else A.P >= 32 ? many_launch<true>(A, ck, cv, U) : many_launch<false>(A, ck, cv, U);
   } else if (U.rows <= 8) {
     few_dispatch<D, 8>(A, ck, cv, U);
   } else {

@@ -146,6 +146,18 @@ __device__ __forceinline__ float row_scale(float amax, float scale_log2, float& 
 // 2^-20.
 constexpr float kLargeFactor = 1.220703125e-4f;             // 2^-13
 __device__ __forceinline__ float score_diff(float s, float f, float base) { return __fsub_rn(__fmul_rn(s, f), base); }
+// Value scales act in the exponent of the probabilities, relative to a reference of each row, and out of the sum again: a
+// page's factor 2^z, z = log2 of its scale - reference, is cut at 2^-60, where probabilities are zeros in fp16 whatever
+// they are. The reference comes from products of probability and scale that the row has seen, so that neither pages that
+// it does not see nor those that hardly count cost its values bits. A scale of 0, or below 2^-200, counts as 2^-200.
+constexpr float kLeastScale = -200.f, kLeastRel = -60.f;
+__device__ __forceinline__ float scale_log2_of(float vs) { return fmaxf(__log2f(vs), kLeastScale); }
+// 2^x, with results below 2^-126 too
+__device__ __forceinline__ float exp2f_small(float x) {
+  float y;
+  asm("ex2.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
 // the least factor of scores: 0 would turn a masked score's -inf into NaN
 constexpr float kTiny = 1.17549435e-38f;
 

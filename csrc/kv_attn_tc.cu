@@ -16,12 +16,14 @@
 // softmax, and two blocks an SM fill each other's gaps.
 //
 // A page's key scale multiplies its 16 to 64 columns of scores; its value
-// scale, relative to the largest of the block's pages, goes into the exponent
-// and out of the sum again. Probabilities are held as 2^7 p against a maximum
-// that is raised only when it grows by more than 2^8, so the output in TMEM is
-// seldom scaled. TMEM (256 columns): S / P of tile t at 64 (t % 3), O at 192.
+// scale goes into the exponent, relative to a reference of the row, and out of
+// the sum again. Products of probability and relative scale are held as 2^7
+// times themselves. A row's maximum, and its reference (the largest product that
+// it has seen), are raised only when they grow by more than 2^8, so the output
+// in TMEM is seldom scaled. Pages of 64 (one pair of scales a tile) have a
+// variant of their own: 152 us below, 164 with the general one. TMEM (256 columns): S / P of tile t at 64 (t % 3), O at 192.
 //
-// B200: 12 prompts of 911 to 1824 tokens, 16 x 64: 154 us, 296 TFLOP/s of the
+// B200: 12 prompts of 911 to 1824 tokens, 16 x 64: 152 us, 300 TFLOP/s of the
 // products that the mask leaves (floor 27 us by the products, 45 by the
 // exponentials); the same on mma.sync took 254 us. Of the 2890 cycles a block
 // spends on a tile, the softmax warps work 2400 (two warps a sub-partition, each
@@ -119,7 +121,7 @@ constexpr uint32_t tc_id(int m, int n, int b_mn) {
   return (1u << 4) | (uint32_t(b_mn) << 16) | (uint32_t(n >> 3) << 17) | (uint32_t(m >> 4) << 24);
 }
 
-template <int D>
+template <int D, bool ONE>               // ONE: a page holds a whole tile of keys, so a tile has one pair of scales
 __global__ void __launch_bounds__(kTcThreads, 2)
 paged_attn_tc_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ CUtensorMap tm_k,
                      const __grid_constant__ CUtensorMap tm_v) {
@@ -128,9 +130,8 @@ paged_attn_tc_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__
   extern __shared__ __align__(1024) uint8_t s_tiles[];      // Q, kOps x K, kOps x V (fp16), kRaw x (codes of K, of V)
   __shared__ uint64_t raw_full[kRaw], raw_empty[kRaw], sc_full[kSc], kv_full[kOps], kv_empty[kOps];
   __shared__ uint64_t s_full[kOps], p_full[kOps], pv_done[kOps], q_full, o_full, mma_done;
-  __shared__ float s_ks[kSc][4], s_lv[kSc][4];              // scales of a tile's pages: keys, log2 of values' (relative)
+  __shared__ float s_ks[kSc][4], s_lv[kSc][4];              // scales of a tile's pages: keys, log2 of values'
   __shared__ uint32_t s_gone[kSc];
-  __shared__ float s_top[kTcThreads / 32];
   __shared__ uint32_t s_tmem;
   __shared__ volatile int s_abort;
 
@@ -169,19 +170,9 @@ paged_attn_tc_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__
                  ::"r"(smem_u32(&s_tmem)), "r"(kCols) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
-  // the largest value scale of the block's pages
-  float top = 0.f;
-  for (int i = threadIdx.x; i * A.P < lim; i += kTcThreads) {
-    const int page = __ldg(table + i);
-    if (page >= 0 && page < A.n_pages) top = fmaxf(top, __ldg(A.vs + page * A.H + h));
-  }
-  top = warp_max(top);
-  if (lane == 0) s_top[warp] = top;
   tc_before();
   __syncthreads();
   tc_after();
-#pragma unroll
-  for (int w = 0; w < kTcThreads / 32; ++w) top = fmaxf(top, s_top[w]);
   const uint32_t tmem = s_tmem;
   auto aborted = [&]() { return __any_sync(0xffffffffu, s_abort != 0); };    // one answer for a whole warp
   auto wait = [&](uint64_t* bar, int turn) { return mbar_wait(smem_u32(bar), uint32_t(turn) & 1u, A.err); };
@@ -192,7 +183,6 @@ paged_attn_tc_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__
     if (warp == 0) {
       // ---------------- copies ----------------
       const int boxes = kUnit >> A.logP;
-      const float ltop = __log2f(top);
       int page = -1, pending = -1, issued = 0;
       float new_ks = 0.f, new_vs = 0.f;
       uint32_t new_gone = 0;
@@ -205,8 +195,7 @@ paged_attn_tc_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__
         const int e = pending % kSc;
         if (lane < boxes) {
           s_ks[e][lane] = new_ks;
-          // below 2^-60 of the largest its probabilities are zeros in fp16 whatever they are
-          s_lv[e][lane] = new_vs > 0.f ? fmaxf(__log2f(new_vs) - ltop, -60.f) : -60.f;
+          s_lv[e][lane] = scale_log2_of(new_vs);
         }
         if (lane == 0) s_gone[e] = new_gone;
         __syncwarp();
@@ -364,7 +353,7 @@ paged_attn_tc_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       mbar_arrive(&q_full);
     }
-    float m = -INFINITY;
+    float m = -INFINITY, w = 0.f;           // running maximum; log2 of the value reference, relative to it
     uint64_t l2 = pk2(0.f, 0.f);
     bool ok = true;
     for (int t = 0; t < units && ok && !aborted(); ++t) {
@@ -375,9 +364,9 @@ paged_attn_tc_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__
       float f[4], lv[4];
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const int pg = (16 * i) >> A.logP;
-        f[i] = fmaxf(s_ks[e][pg] * rs, kTiny);
-        lv[i] = s_lv[e][pg];
+        const int pg = ONE ? 0 : (16 * i) >> A.logP;
+        f[i] = ONE && i > 0 ? f[0] : fmaxf(s_ks[e][pg] * rs, kTiny);
+        lv[i] = ONE && i > 0 ? lv[0] : s_lv[e][pg];
       }
       const bool large = __any_sync(0xffffffffu, fmaxf(fmaxf(f[0], f[1]), fmaxf(f[2], f[3])) >= kLargeFactor);
       uint32_t sr[64];
@@ -404,7 +393,7 @@ paged_attn_tc_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__
         for (int c = 0; c < 64; ++c)
           if (gone >> (c >> A.logP) & 1) sr[c] = __float_as_uint(-INFINITY);
       }
-      float mx = -INFINITY;
+      float y[4], mx = -INFINITY;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         float y0 = -INFINITY, y1 = -INFINITY;
@@ -413,12 +402,19 @@ paged_attn_tc_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__
           y0 = fmaxf(y0, fmaxf(__uint_as_float(sr[c]), __uint_as_float(sr[c + 1])));
           y1 = fmaxf(y1, fmaxf(__uint_as_float(sr[c + 2]), __uint_as_float(sr[c + 3])));
         }
-        mx = fmaxf(mx, fmaxf(y0, y1) * f[i]);
+        y[i] = fmaxf(y0, y1) * f[i];
+        mx = fmaxf(mx, y[i]);
       }
-      const bool need = mx > m + (large ? 0.f : 8.f);
-      const float top_m = need ? mx : m;
-      if (__any_sync(0xffffffffu, need)) {
-        const float al = need ? exp2f_approx(m - top_m) : 1.f;
+      if (ONE) y[0] = mx;
+      // the running maximum and the value reference (relative to it) lag by up to 2^8
+      const float lag = large ? 0.f : 8.f;
+      const float top_m = mx > m + lag ? mx : m, base = top_m == -INFINITY ? 0.f : top_m;
+      float v = -INFINITY;
+#pragma unroll
+      for (int i = 0; i < (ONE ? 1 : 4); ++i) v = fmaxf(v, (y[i] - base) + lv[i]);
+      const float x = top_m == m ? w : w + (m - top_m);     // the reference as it is, relative to the new maximum
+      if (__any_sync(0xffffffffu, mx > m + lag || v > x + lag)) {
+        const float top_w = v > x + lag ? v : x, al = exp2f_approx(x - top_w);
         if (t > 0) {
           // the output is scaled once the products of the tile before, its last writers, are done
           ok = wait(&pv_done[(t - 1) % kOps], (t - 1) / kOps);
@@ -435,15 +431,19 @@ paged_attn_tc_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__
           }
           tm_st_wait();
         }
-        l2 = pk2_mul(l2, pk2s(al));
+        if (top_m != m) l2 = pk2_mul(l2, pk2s(exp2f_approx(m - top_m)));
         m = top_m;
+        w = top_w;
       }
-      const float z = m == -INFINITY ? 7.f : 7.f - m;
+      const float z = 7.f - base;
+      float rel;                              // log2 of the page's factor
       uint32_t pk[32];
+      uint64_t s0 = pk2(0.f, 0.f), s1 = s0;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const uint64_t ff = pk2s(f[i]), zz = pk2s(z + lv[i]);
-        uint64_t s0 = pk2(0.f, 0.f), s1 = s0;
+        if (!ONE || i == 0) rel = fmaxf(lv[i] - w, kLeastRel);
+        const uint64_t ff = pk2s(f[i]), zz = pk2s(z + rel);
+        if (!ONE) s0 = s1 = pk2(0.f, 0.f);
 #pragma unroll
         for (int c = 16 * i; c < 16 * i + 16; c += 2) {
           float p0, p1;
@@ -454,7 +454,7 @@ paged_attn_tc_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__
           else s0 = pk2_add(s0, pk2(p0, p1));
           pk[c / 2] = pack_f16(p0, p1);
         }
-        l2 = pk2_fma(pk2_add(s0, s1), pk2s(exp2f_approx(-lv[i])), l2);
+        if (!ONE || i == 3) l2 = pk2_fma(pk2_add(s0, s1), pk2s(exp2f_approx(-rel)), l2);
       }
       tm_st32(lane_base + kUnit * sl, pk);
       tm_st_wait();
@@ -467,9 +467,11 @@ paged_attn_tc_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__
     float l, l1;
     pk2_split(l2, l, l1);
     l += l1;
-    const float inv = l == 0.f ? 0.f : top / l;             // a sum of 0: no keys. A NaN stays one
+    // a sum of 0: no keys. A NaN stays one. The reference may be near the largest number: half of it at a time
+    const float half = exp2f_approx(0.5f * w), inv = l == 0.f ? 0.f : half / l;
     const int64_t at = int64_t(S.tok0 + qi) * A.Hq + h * A.G + (live ? row - qi * A.G : 0);
     uint16_t* dst = static_cast<uint16_t*>(A.o) + at * D;
+    const auto out = [&](uint32_t v) { return __uint_as_float(v) * inv * half; };
 #pragma unroll
     for (int c0 = 0; c0 < D; c0 += 32) {
       uint32_t o[32];
@@ -484,10 +486,8 @@ paged_attn_tc_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__
 #pragma unroll
         for (int c = 0; c < 32; c += 8)
           *reinterpret_cast<uint4*>(dst + c0 + c) =
-              make_uint4(pack_16(__uint_as_float(o[c]) * inv, __uint_as_float(o[c + 1]) * inv, A.bf16),
-                         pack_16(__uint_as_float(o[c + 2]) * inv, __uint_as_float(o[c + 3]) * inv, A.bf16),
-                         pack_16(__uint_as_float(o[c + 4]) * inv, __uint_as_float(o[c + 5]) * inv, A.bf16),
-                         pack_16(__uint_as_float(o[c + 6]) * inv, __uint_as_float(o[c + 7]) * inv, A.bf16));
+              make_uint4(pack_16(out(o[c]), out(o[c + 1]), A.bf16), pack_16(out(o[c + 2]), out(o[c + 3]), A.bf16),
+                         pack_16(out(o[c + 4]), out(o[c + 5]), A.bf16), pack_16(out(o[c + 6]), out(o[c + 7]), A.bf16));
       }
     }
     if (live && A.lse) A.lse[at] = l == 0.f ? -INFINITY : (m - 7.f + log2f(l)) * 0.6931471805599453f;
@@ -501,11 +501,11 @@ paged_attn_tc_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__
   }
 }
 
-template <int D>
+template <int D, bool ONE>
 static void tc_launch(AttnArgs& A, const at::Tensor& ck, const at::Tensor& cv, const Bounds& U) {
   constexpr int kSmem = kTcRows * Op<D>::kRow + 2 * kOps * kUnit * Op<D>::kRow + kRaw * 2 * kUnit * D;
   static int known[64] = {};
-  auto kern = paged_attn_tc_kernel<D>;
+  auto kern = paged_attn_tc_kernel<D, ONE>;
   blocks_per_sm(kern, kTcThreads, kSmem, known);
   const dim3 grid(unsigned(U.B * A.H), unsigned((U.rows + kTcRows - 1) / kTcRows));
   kern<<<grid, kTcThreads, kSmem, stream()>>>(A, code_map(ck, A.P, false), code_map(cv, A.P, false));
@@ -513,8 +513,8 @@ static void tc_launch(AttnArgs& A, const at::Tensor& ck, const at::Tensor& cv, c
 }
 
 void attn_tc_launch(AttnArgs& A, const at::Tensor& ck, const at::Tensor& cv, int d, const Bounds& U) {
-  if (d == 32) tc_launch<32>(A, ck, cv, U);
-  else tc_launch<64>(A, ck, cv, U);
+  if (A.P == kUnit) d == 32 ? tc_launch<32, true>(A, ck, cv, U) : tc_launch<64, true>(A, ck, cv, U);
+  else d == 32 ? tc_launch<32, false>(A, ck, cv, U) : tc_launch<64, false>(A, ck, cv, U);
 }
 
 }  // namespace kv

@@ -182,7 +182,7 @@ def test_rotary_without_eps(B, T, H, d):
     rotary._err_word(DEV).zero_()
 
 
-@pytest.mark.parametrize("form", [f for f in FORMS if "rows" in f or "warp" in f])
+@pytest.mark.parametrize("form", FORMS)
 def test_value_scale_of_zero(form):
     """A page whose value scale is 0 holds zeros: it takes part in the softmax and adds nothing."""
     c, table, q, lens = _queries(form, 1)
@@ -220,4 +220,33 @@ def test_values_near_the_largest(form):
     c.v_scale.fill_(2.0 ** 119)                                      # up to 448 * 2^119 = 2^127.8
     _check_rows(q, c, table, lens)
     c.v_scale.fill_(2.0 ** -100)                                     # and the smallest scale
+    _check_rows(q, c, table, lens)
+
+
+@pytest.mark.parametrize("step", [12, 26, 40, -26, 61])
+@pytest.mark.parametrize("form", FORMS)
+def test_pages_of_very_different_values(form, step):
+    """Each page's values 2^step times those before: a row is as exact as the values that it sees allow, whatever the
+    pages behind it hold."""
+    c, table, q, lens = _queries(form, 4)
+    for j in range(table.shape[1]):
+        c.v_scale[table[:, j].long()] *= 2.0 ** (step * (j % 4) - (100 if step == 61 else 0))
+    _check_rows(q, c, table, lens)
+    _check_rows(q, c, table, lens, causal=False, scale=0.02)
+
+
+@pytest.mark.parametrize("reach,step", [(40, 20), (60, 40), (70, 90), (50, 45)])
+@pytest.mark.parametrize("form", FORMS)
+def test_unlikely_keys_with_large_values(form, reach, step):
+    """Keys of probability 2^-reach whose values are 2^step times the others', in the middle of a page's run: they count
+    for what they are, be it nothing or nearly all."""
+    c, table, q, lens = _queries(form, 5)
+    d = q.shape[-1]
+    c.k.view(torch.uint8)[:] = 0x38
+    c.k_scale.fill_(1.0)
+    page = table[:, 1].long()
+    c.k.view(torch.uint8)[page] = 0xB8                               # -1
+    c.v_scale[page] *= 2.0 ** step
+    # q . k = +- reach / 2 in the log2 domain: each element reach ln 2 / (2 d scale)
+    q = torch.full_like(q, reach * math.log(2) / (2 * d * d ** -0.5))
     _check_rows(q, c, table, lens)
