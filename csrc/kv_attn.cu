@@ -71,7 +71,7 @@ constexpr float kSumUnit = 0x1p-31f, kSumLog2 = -31.f;
 // keys a copy instead of 128 cost 179 us).
 template <int D, int R, int W, bool ONE>
 __global__ void __launch_bounds__(kWarps * 32, D == 128 && R == 16 ? 2 : 3)
-paged_attn_kernel(const AttnArgs A, const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v) {
+paged_attn_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v) {
   constexpr int TK = Cfg<D>::TK, SUB = Cfg<D>::SUB, ST = Cfg<D>::ST;
   constexpr int WK = TK * SUB;          // keys of a warp's copy
   constexpr int SUP = WK * W;           // keys of a unit
@@ -113,9 +113,11 @@ paged_attn_kernel(const AttnArgs A, const __grid_constant__ CUtensorMap tm_k, co
     const int per = (A.B + kWarps * 32 - 1) / (kWarps * 32);
     const int lo = min(int(threadIdx.x) * per, A.B), hi = min(lo + per, A.B);
     int64_t mine = 0;
+    bool gaps = false;                                      // rows of q that no sequence computes
     for (int b = lo; b < hi; ++b) {
       Seq<R> s;
       s.load(A, b);
+      gaps |= s.gaps(A, b);
       mine += A.split ? s.all(A.H, SUP) : int64_t(A.H) * s.tiles_m;
     }
     int64_t incl = mine;
@@ -125,7 +127,8 @@ paged_attn_kernel(const AttnArgs A, const __grid_constant__ CUtensorMap tm_k, co
       if (lane >= o) incl += v;
     }
     if (lane == 31) s_scan[warp] = incl;
-    __syncthreads();
+    if (__syncthreads_or(gaps))
+      clear_gaps<D>(A, 0, A.B, 0, A.Hq, int64_t(blockIdx.x) * kWarps * 32 + threadIdx.x, int64_t(gridDim.x) * kWarps * 32);
     int64_t before = incl - mine, total = 0;
 #pragma unroll
     for (int w = 0; w < kWarps; ++w) {
@@ -738,7 +741,7 @@ constexpr int kManyRows = 16 * kWarps, kManyCopies = 3;
 
 template <bool ONE>                       // a page holds a whole tile of 32 keys
 __global__ void __launch_bounds__(kWarps * 32, 3)
-paged_attn_many_kernel(const AttnArgs A, const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v) {
+paged_attn_many_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v) {
   constexpr int D = 128, TK = 32, ST = kManyCopies, R = kManyRows;
   constexpr int KS = D / 16, NT = TK / 8, TS = TK / 16, NO = D / 8;
   constexpr int kHalf = kUnit * D;
@@ -754,6 +757,8 @@ paged_attn_many_kernel(const AttnArgs A, const __grid_constant__ CUtensorMap tm_
   const int b = blockIdx.x / A.H, h = blockIdx.x % A.H, mt = gridDim.y - 1 - blockIdx.y;
   Seq<R> S;
   S.load(A, b);
+  if (S.gaps(A, b))
+    clear_gaps<D>(A, b, b + 1, h * A.G, A.G, mt * kWarps * 32 + threadIdx.x, gridDim.y * kWarps * 32);
   if (mt >= S.tiles_m) return;
   const int rows = S.n * A.G, r0 = mt * R;
   const int last = min(r0 + R, rows) - 1;

@@ -233,20 +233,51 @@ __device__ __forceinline__ void mma_f16(float* d, const uint32_t* a, uint32_t b0
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
+// Offsets of queries that are not served: they do not ascend or lie outside q, or are more than the call states.
+__device__ __forceinline__ bool impossible(const AttnArgs& A, int tok0, int n) {
+  return n < 0 || n > A.n || tok0 < 0 || tok0 > A.total - n;
+}
+// Zeros, and -inf for the sums, in rows [lo, hi) of packed outputs, query heads [h0, h0 + nh): thread `first` of `step`.
+template <int D>
+__device__ __forceinline__ void clear_rows(const AttnArgs& A, int lo, int hi, int h0, int nh, int64_t first, int64_t step) {
+  lo = min(max(lo, 0), A.total);
+  hi = min(max(hi, 0), A.total);
+  constexpr int V = D / 8;                  // vectors of a row
+  for (int64_t i = first; i < int64_t(hi - lo) * nh * V; i += step) {
+    const int64_t r = i / V, at = (lo + r / nh) * A.Hq + h0 + r % nh;
+    *(reinterpret_cast<uint4*>(static_cast<uint16_t*>(A.o) + at * D) + i % V) = make_uint4(0, 0, 0, 0);
+    if (A.lse && i % V == 0) A.lse[at] = -INFINITY;
+  }
+}
+// The same for what no sequence computes: rows in front of the first and behind the last one, and those of sequences
+// that are not served, among sequences [b0, b1).
+template <int D>
+__device__ __noinline__ void clear_gaps(const AttnArgs& A, int b0, int b1, int h0, int nh, int64_t first, int64_t step) {
+  if (b0 == 0) clear_rows<D>(A, 0, A.cu[0], h0, nh, first, step);
+  if (b1 == A.B) clear_rows<D>(A, A.cu[A.B], A.total, h0, nh, first, step);
+  for (int b = b0; b < b1; ++b) {
+    const int lo = A.cu[b], hi = A.cu[b + 1];
+    if (impossible(A, lo, hi - lo)) clear_rows<D>(A, lo, hi, h0, nh, first, step);
+  }
+}
+
 // The queries and keys of one sequence, with impossible lengths cut (and reported).
 template <int R>
 struct Seq {
   int len, n, tok0, tiles_m;                // tiles_m: segments of R rows (query, head of the group) for a key head
+  bool refused;                             // its offsets are impossible, or it is longer than stated
   __device__ __forceinline__ void load(const AttnArgs& A, int b) {
     len = __ldg(A.lens + b);
     if (A.cu) {
       tok0 = __ldg(A.cu + b);
       n = __ldg(A.cu + b + 1) - tok0;
-      if (n < 0 || n > A.n || tok0 < 0 || tok0 > A.total - n) {
+      refused = impossible(A, tok0, n);
+      if (refused) {
         set_error(A.err, kBadShape);
         n = 0;
       }
     } else {
+      refused = false;
       n = A.n;
       tok0 = b * A.n;
     }
@@ -259,6 +290,10 @@ struct Seq {
       len = 0;
     }
     tiles_m = int((int64_t(n) * A.G + R - 1) / R);
+  }
+  // rows of q in front of the first sequence, behind the last one, or this one's that nobody computes
+  __device__ __forceinline__ bool gaps(const AttnArgs& A, int b) const {
+    return A.cu && (refused || (b == 0 && tok0 != 0) || (b == A.B - 1 && tok0 + n != A.total));
   }
   // units of `sup` keys in each of its segments; a sequence without keys has one (it writes zeros)
   __device__ __forceinline__ int units(int sup) const { return max(1, (len + sup - 1) / sup); }

@@ -21,9 +21,9 @@
 // times themselves. A row's maximum, and its reference (the largest product that
 // it has seen), are raised only when they grow by more than 2^8, so the output
 // in TMEM is seldom scaled. Pages of 64 (one pair of scales a tile) have a
-// variant of their own: 152 us below, 164 with the general one. TMEM (256 columns): S / P of tile t at 64 (t % 3), O at 192.
+// variant of their own: 153 us below, 164 with the general one. TMEM (256 columns): S / P of tile t at 64 (t % 3), O at 192.
 //
-// B200: 12 prompts of 911 to 1824 tokens, 16 x 64: 152 us, 300 TFLOP/s of the
+// B200: 12 prompts of 911 to 1824 tokens, 16 x 64: 153 us, 298 TFLOP/s of the
 // products that the mask leaves (floor 27 us by the products, 45 by the
 // exponentials); the same on mma.sync took 254 us. Of the 2890 cycles a block
 // spends on a tile, the softmax warps work 2400 (two warps a sub-partition, each
@@ -140,6 +140,8 @@ paged_attn_tc_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__
   const int b = blockIdx.x / A.H, h = blockIdx.x % A.H, mt = gridDim.y - 1 - blockIdx.y;
   Seq<kTcRows> S;
   S.load(A, b);
+  if (S.gaps(A, b))
+    clear_gaps<D>(A, b, b + 1, h * A.G, A.G, mt * kTcThreads + threadIdx.x, gridDim.y * kTcThreads);
   if (mt >= S.tiles_m) return;
   const int rows = S.n * A.G, r0 = mt * kTcRows;
   const int last = min(r0 + kTcRows, rows) - 1;

@@ -275,8 +275,8 @@ def paged_attention(q: torch.Tensor, cache: PagedKVCache, page_table: torch.Tens
     ``q`` (bf16 or fp16, any strides over tokens and heads): ``[B, n, Hq, d]``,
     or ``[tokens, Hq, d]`` with ``cu_q`` int32 ``[B + 1]``; ``max_q`` is then the
     most queries of one sequence (by default all of them; a longer sequence is
-    skipped and reported by ``cache.check_errors``; rows of ``q`` that no
-    sequence covers are not computed).  ``Hq`` is a
+    skipped and reported by ``cache.check_errors``; its rows, and those of ``q``
+    that no sequence covers, give zeros and ``-inf``).  ``Hq`` is a
     multiple of the cache's heads: neighbours share one.  ``kv_lens`` int32
     ``[B]`` counts the tokens in the cache, the queries' own among them, so a
     sequence's ``n`` queries are its last ``n`` tokens: query ``i`` sees the

@@ -250,3 +250,42 @@ def test_unlikely_keys_with_large_values(form, reach, step):
     # q . k = +- reach / 2 in the log2 domain: each element reach ln 2 / (2 d scale)
     q = torch.full_like(q, reach * math.log(2) / (2 * d * d ** -0.5))
     _check_rows(q, c, table, lens)
+
+
+@pytest.mark.parametrize("n,d,H", [(2, 32, 1), (2, 128, 2), (140, 32, 8), (140, 64, 8), (140, 128, 8)])
+def test_rows_of_no_sequence_are_zeros(n, d, H):
+    """Rows in front of the first and behind the last sequence, and those of a sequence longer than stated: zeros and
+    -inf whatever the memory held, next to the results of the others."""
+    from primus_dlrm_b200.ops.kv_cache import paged_attention
+    B = 40
+    c = _cache(4, H, d, 16)
+    table, lens = _i32([[0, 1, 2]] * B), _i32([40] * B)
+    off = [3]
+    for b in range(B):
+        off.append(off[-1] + (n + 1 + b % 3 if b % 7 == 2 else n - b % 2))
+    total = off[-1] + 5
+    q = torch.randn(total, 2 * H, d, device=DEV).bfloat16()
+    for lse_too in (True, False):
+        junk = [torch.full_like(q, float("nan")), torch.full(q.shape[:2], float("nan"), device=DEV)]
+        torch.cuda.synchronize()
+        del junk                                                     # the next allocations find NaN
+        out = paged_attention(q, c, table, lens, _i32(off), n, return_lse=lse_too)
+        o = out[0] if lse_too else out
+        with pytest.raises(RuntimeError, match="length"):
+            c.check_errors()
+        live = torch.zeros(total, dtype=torch.bool, device=DEV)
+        for b in range(B):
+            if b % 7 != 2:
+                live[off[b]:off[b + 1]] = True
+        assert (o[~live] == 0).all() and torch.isfinite(o).all()
+        if lse_too:
+            seen = torch.ones(total, dtype=torch.bool, device=DEV)       # rows that have keys
+            for b in range(B):
+                seen[off[b]:max(off[b], off[b + 1] - 40)] = False
+            assert torch.equal((out[1] > -math.inf).all(1), live & seen) and torch.equal((out[1] > -math.inf).any(1), live & seen)
+        # the others: within two roundings of bf16 and of the probabilities of a call without the long ones
+        good = [b for b in range(B) if b % 7 != 2]
+        cut = [0] + list(torch.tensor([off[b + 1] - off[b] for b in good]).cumsum(0))
+        alone = paged_attention(q[live], c, table[good], lens[good], _i32(cut), n)
+        c.check_errors()
+        assert (o[live].float() - alone.float()).abs().max() <= 2.0 ** -6 * (c.v.float().abs().amax((1, 2, 3)) * c.v_scale.amax(1)).max()
