@@ -1256,8 +1256,9 @@ std::vector<at::Tensor> paged_attention(at::Tensor q, at::Tensor ck, at::Tensor 
   PD_CHECK((qd == 3 ? q.size(0) : B * q.size(1)) * A.G < (int64_t(1) << 31) - 128 && B < (int64_t(1) << 31),
            "too many queries");
   A.n = int(most);
-  if (B > 0 && most > 0 && q.numel() > 0) {
-    const Bounds U{B, most * A.G, std::min<int64_t>(table.size(1) * C.P, std::max<int64_t>(max_len.value_or(INT64_MAX), 0))};
+  if (B > 0 && q.numel() > 0) {
+    // a stated most of 0 launches too: queries that there are all the same are reported
+    const Bounds U{B, std::max<int64_t>(most, 1) * A.G, std::min<int64_t>(table.size(1) * C.P, std::max<int64_t>(max_len.value_or(INT64_MAX), 0))};
     if (C.d == 32) attn_dispatch<32>(A, ck, cv, U);
     else if (C.d == 64) attn_dispatch<64>(A, ck, cv, U);
     else attn_dispatch<128>(A, ck, cv, U);

@@ -480,8 +480,9 @@ void kv_append(at::Tensor ck, at::Tensor cv, at::Tensor ks, at::Tensor vs, at::T
     A.rope = rope->data_ptr<float>();
     A.n_pos = int(std::min<int64_t>(rope->size(0), INT32_MAX));
   }
-  const int64_t most = cu.has_value() ? std::min(max_new, k.size(0)) : k.size(1);
-  if (B == 0 || most == 0 || k.size(td - 3) == 0) return;
+  if (B == 0 || k.size(td - 3) == 0) return;
+  // a stated most of 0 launches too: tokens that there are all the same are reported
+  const int64_t most = cu.has_value() ? std::max<int64_t>(std::min(max_new, k.size(0)), 1) : k.size(1);
   A.J = int((most + C.P - 2) / C.P + 1);                 // pages that `most` tokens can touch
   PD_CHECK(B * A.J < (int64_t(1) << 31), "too many sequences and pages for one call");
   const c10::cuda::CUDAGuard guard(ck.device());

@@ -289,3 +289,21 @@ def test_rows_of_no_sequence_are_zeros(n, d, H):
         alone = paged_attention(q[live], c, table[good], lens[good], _i32(cut), n)
         c.check_errors()
         assert (o[live].float() - alone.float()).abs().max() <= 2.0 ** -6 * (c.v.float().abs().amax((1, 2, 3)) * c.v_scale.amax(1)).max()
+
+
+def test_a_stated_most_of_zero_is_reported():
+    from primus_dlrm_b200.ops.kv_cache import paged_attention
+    c = _cache(4, 1, 32, 16)
+    before = _clone(c, DEV)
+    x = torch.ones(3, 1, 32, device=DEV)
+    c.append(x, x, _i32([[0]]), _i32([0]), _i32([0, 3]), 0)
+    _same(c, before)
+    with pytest.raises(RuntimeError, match="length"):
+        c.check_errors()
+    o = paged_attention(x.bfloat16(), c, _i32([[0]]), _i32([3]), _i32([0, 3]), 0)
+    assert (o == 0).all()
+    with pytest.raises(RuntimeError, match="length"):
+        c.check_errors()
+    c.append(x, x, _i32([[0]]), _i32([0]), _i32([0, 0]), 0)            # no tokens: nothing to report
+    paged_attention(x.bfloat16(), c, _i32([[0]]), _i32([3]), _i32([0, 0]), 0)
+    c.check_errors()
