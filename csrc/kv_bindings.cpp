@@ -71,6 +71,11 @@ struct QkNormRope : public torch::autograd::Function<QkNormRope> {
   }
 };
 
+// Forward-mode derivatives do not pass through the kernels: refused, not dropped.
+void no_tangent(const OptTensor& t, const char* who) {
+  TORCH_CHECK(!t.has_value() || !t->_fw_grad(0).defined(), who, " has no forward-mode derivative");
+}
+
 OptTensor unit_stride(const OptTensor& x) {
   return !x.has_value() || x->dim() == 0 || x->stride(-1) == 1 ? x : OptTensor(x->contiguous());
 }
@@ -87,6 +92,9 @@ at::Tensor rotary_err(int64_t device) {
 std::tuple<at::Tensor, OptTensor> rotary(at::Tensor q, OptTensor k, OptTensor wq, OptTensor wk, at::Tensor table,
                                          OptTensor pos, double eps, bool interleaved) {
   TORCH_CHECK(q.is_cuda() && q.dim() == 4, "q must be a CUDA tensor [B, T, H, d]");
+  for (const OptTensor& t : {OptTensor(q), k, wq, wk, OptTensor(table)}) no_tangent(t, "qk_norm_rope");
+  TORCH_CHECK(!(at::GradMode::is_enabled() && table.requires_grad()),
+              "qk_norm_rope gives the angle table no gradient: detach it");
   const at::Tensor err = rotary_err(q.get_device());
   q = *unit_stride(q);
   k = unit_stride(k);

@@ -83,8 +83,9 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor | None, q_weight: torch.Tensor
     or int64), by default ``0..T-1``.  ``interleaved`` pairs neighbours
     ``(2i, 2i + 1)`` instead of halves ``(i, i + rotary_dim / 2)``.
 
-    Returns contiguous ``(q', k')`` of the inputs' type; differentiable once in
-    ``q``, ``k`` and both weights.  A row whose position lies outside the
+    Returns contiguous ``(q', k')`` of the inputs' type; differentiable once,
+    backward, in ``q``, ``k`` and both weights (the native path refuses a table
+    that requires a gradient, and forward-mode tangents).  A row whose position lies outside the
     table comes out as zeros and sets :func:`rotary_error_code` (IndexError on
     the eager path).
     """

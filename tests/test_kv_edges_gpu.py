@@ -307,3 +307,30 @@ def test_a_stated_most_of_zero_is_reported():
     c.append(x, x, _i32([[0]]), _i32([0]), _i32([0, 0]), 0)            # no tokens: nothing to report
     paged_attention(x.bfloat16(), c, _i32([[0]]), _i32([3]), _i32([0, 0]), 0)
     c.check_errors()
+
+
+def test_tangents_are_refused():
+    """Forward-mode derivatives do not go through the kernels: refused, not dropped."""
+    import torch.autograd.forward_ad as fw
+    from primus_dlrm_b200.ops.kv_cache import paged_attention
+    from primus_dlrm_b200.ops.rotary import qk_norm_rope, rope_table
+    t, x = rope_table(4, 32, device=DEV), torch.randn(1, 4, 2, 32, device=DEV)
+    w = torch.ones(32, device=DEV)
+    c = _cache(4, 2, 32, 16)
+    with fw.dual_level():
+        dual, dw, dt = (fw.make_dual(a, torch.ones_like(a)) for a in (x, w, t))
+        for bad in (lambda: qk_norm_rope(dual, x, w, w, t), lambda: qk_norm_rope(x, dual, w, w, t),
+                    lambda: qk_norm_rope(x, x, dw, w, t), lambda: qk_norm_rope(x, x, w, dw, t),
+                    lambda: qk_norm_rope(x, x, w, w, dt)):
+            with pytest.raises(RuntimeError, match="forward"):
+                bad()
+        qk_norm_rope(x, x, w, w, t)
+
+
+def test_gradients_of_the_angles_are_refused():
+    from primus_dlrm_b200.ops.rotary import qk_norm_rope, rope_table
+    t, x = rope_table(4, 32, device=DEV).requires_grad_(), torch.randn(1, 4, 2, 32, device=DEV)
+    with pytest.raises(RuntimeError, match="angle"):
+        qk_norm_rope(x, x, None, None, t)
+    with torch.no_grad():
+        qk_norm_rope(x, x, None, None, t)
