@@ -76,6 +76,28 @@ void no_tangent(const OptTensor& t, const char* who) {
   TORCH_CHECK(!t.has_value() || !t->_fw_grad(0).defined(), who, " has no forward-mode derivative");
 }
 
+// Attention over a cache has no gradient: its output of a query that requires one says so where it is asked for.
+using Attended = std::vector<at::Tensor>;
+struct PagedAttention : public torch::autograd::Function<PagedAttention> {
+  static variable_list forward(AutogradContext*, at::Tensor q, at::Tensor k, at::Tensor v, at::Tensor ks, at::Tensor vs,
+                               at::Tensor err, at::Tensor table, at::Tensor lens, OptTensor cu,
+                               c10::optional<int64_t> max_q, c10::optional<int64_t> max_len, c10::optional<double> scale,
+                               bool causal, bool want_lse) {
+    return pd::kv::paged_attention(q, k, v, ks, vs, err, table, lens, cu, max_q, max_len, scale, causal, want_lse);
+  }
+  static variable_list backward(AutogradContext*, variable_list) {
+    TORCH_CHECK(false, "paged_attention has no gradient: call it under no_grad, or with a detached query");
+  }
+};
+Attended attend(at::Tensor q, at::Tensor k, at::Tensor v, at::Tensor ks, at::Tensor vs, at::Tensor err, at::Tensor table,
+                at::Tensor lens, OptTensor cu, c10::optional<int64_t> max_q, c10::optional<int64_t> max_len,
+                c10::optional<double> scale, bool causal, bool want_lse) {
+  no_tangent(q, "paged_attention");
+  if (at::GradMode::is_enabled() && q.requires_grad())
+    return PagedAttention::apply(q, k, v, ks, vs, err, table, lens, cu, max_q, max_len, scale, causal, want_lse);
+  return pd::kv::paged_attention(q, k, v, ks, vs, err, table, lens, cu, max_q, max_len, scale, causal, want_lse);
+}
+
 OptTensor unit_stride(const OptTensor& x) {
   return !x.has_value() || x->dim() == 0 || x->stride(-1) == 1 ? x : OptTensor(x->contiguous());
 }
@@ -115,6 +137,6 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("append", &pd::kv::kv_append, "new tokens' keys and values into the pages of a cache");
   m.def("copy_pages", &pd::kv::kv_copy_pages, "pages dst become copies of pages src");
   m.def("read", &pd::kv::kv_read, "tokens [first, first + n) of each sequence as bf16 [B, n, H, d]");
-  m.def("paged_attention", &pd::kv::paged_attention, "attention of the last tokens over a cache -> [o(, lse)]");
+  m.def("paged_attention", &attend, "attention of the last tokens over a cache -> [o(, lse)]");
   m.def("launch_count", &pd::launches);
 }

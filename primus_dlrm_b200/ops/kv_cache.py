@@ -146,7 +146,8 @@ class PagedKVCache:
         A page's scale is the smallest power of two that brings its largest
         finite magnitude to 448 or less; it never falls while the page fills,
         and where it grows the page's earlier tokens are rounded again.
-        Non-finite values are stored as NaN and do not enter the scale.
+        Non-finite values are stored as NaN and do not enter the scale.  No
+        gradient passes through the cache: what it holds has none.
         """
         if self._native():
             _ext.kv().append(*self._parts, k, v, page_table, kv_lens, cu_new, max_new, k_weight, norm_eps, rope,
@@ -267,10 +268,23 @@ def paged_attention_ref(q, cache: PagedKVCache, page_table, kv_lens, cu_q=None, 
     return o.reshape(q.shape), lse.reshape(q.shape[:-1])
 
 
+class _NoGradient(torch.autograd.Function):
+    """Results of a query that requires a gradient: the backward pass says that there is none."""
+
+    @staticmethod
+    def forward(ctx, q, *out):
+        return tuple(x.view_as(x) for x in out)
+
+    @staticmethod
+    def backward(ctx, *_):
+        raise RuntimeError("paged_attention has no gradient: call it under no_grad, or with a detached query")
+
+
 def paged_attention(q: torch.Tensor, cache: PagedKVCache, page_table: torch.Tensor, kv_lens: torch.Tensor,
                     cu_q: torch.Tensor | None = None, max_q: int | None = None, *, max_len: int | None = None,
                     scale: float | None = None, causal: bool = True, return_lse: bool = False):
-    """Attention of each sequence's last tokens over the cache (no gradient).
+    """Attention of each sequence's last tokens over the cache (no gradient: a
+    backward pass through it raises, as do forward-mode tangents).
 
     ``q`` (bf16 or fp16, any strides over tokens and heads): ``[B, n, Hq, d]``,
     or ``[tokens, Hq, d]`` with ``cu_q`` int32 ``[B + 1]``; ``max_q`` is then the
@@ -293,5 +307,10 @@ def paged_attention(q: torch.Tensor, cache: PagedKVCache, page_table: torch.Tens
         out = _ext.kv().paged_attention(q, *cache._parts, page_table, kv_lens, cu_q, max_q, max_len, scale, causal,
                                         return_lse)
         return (out[0], out[1]) if return_lse else out[0]
+    if torch.autograd.forward_ad.unpack_dual(q).tangent is not None:
+        raise RuntimeError("paged_attention has no forward-mode derivative")
     o, lse = paged_attention_ref(q.detach(), cache, page_table, kv_lens, cu_q, scale, causal)
-    return (o.to(q.dtype), lse) if return_lse else o.to(q.dtype)
+    o = o.to(q.dtype)
+    if torch.is_grad_enabled() and q.requires_grad:
+        o, lse = _NoGradient.apply(q, o, lse)
+    return (o, lse) if return_lse else o

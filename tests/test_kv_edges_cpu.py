@@ -2,7 +2,7 @@
 import pytest
 import torch
 
-from primus_dlrm_b200.ops.kv_cache import PagedKVCache
+from primus_dlrm_b200.ops.kv_cache import PagedKVCache, paged_attention
 
 
 def test_copy_pages_outside_the_pool():
@@ -14,3 +14,17 @@ def test_copy_pages_outside_the_pool():
     assert c.k_scale.flatten().tolist() == [1, 2, 3, 4]
     c.copy_pages(torch.tensor([0, 1], dtype=torch.int32), torch.tensor([1, 0], dtype=torch.int32))
     assert c.k_scale.flatten().tolist() == [2, 1, 3, 4]
+
+
+def test_attention_has_no_gradient():
+    c, table, lens = PagedKVCache(2, 1, 32, 16), torch.tensor([[0, 1]], dtype=torch.int32), torch.tensor([20], dtype=torch.int32)
+    q = torch.randn(1, 2, 1, 32, requires_grad=True)
+    o, lse = paged_attention(q, c, table, lens, return_lse=True)
+    for y in (o, lse, paged_attention(q, c, table, lens)):
+        with pytest.raises(RuntimeError, match="no gradient"):
+            y.sum().backward(retain_graph=True)
+    with torch.no_grad():
+        assert not paged_attention(q, c, table, lens).requires_grad
+    with torch.autograd.forward_ad.dual_level():
+        with pytest.raises(RuntimeError, match="forward"):
+            paged_attention(torch.autograd.forward_ad.make_dual(q.detach(), torch.ones(1, 2, 1, 32)), c, table, lens)

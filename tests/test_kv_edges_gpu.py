@@ -334,3 +334,26 @@ def test_gradients_of_the_angles_are_refused():
         qk_norm_rope(x, x, None, None, t)
     with torch.no_grad():
         qk_norm_rope(x, x, None, None, t)
+
+
+@pytest.mark.parametrize("n", [1, 40])
+def test_attention_has_no_gradient(n):
+    """The output of a query that requires a gradient says so where the gradient is asked for."""
+    import torch.autograd.forward_ad as fw
+    from primus_dlrm_b200.ops.kv_cache import paged_attention
+    c = _cache(4, 2, 32, 16)
+    table, lens = _i32([[0, 1, 2]]), _i32([45])
+    q = torch.randn(1, n, 4, 32, device=DEV).bfloat16()
+    want = paged_attention(q, c, table, lens)
+    assert not want.requires_grad
+    leaf = q.clone().requires_grad_()
+    o, lse = paged_attention(leaf, c, table, lens, return_lse=True)
+    assert torch.equal(o.detach(), want)
+    for y in (o, lse):
+        with pytest.raises(RuntimeError, match="no gradient"):
+            y.sum().backward(retain_graph=True)
+    with torch.no_grad():
+        assert not paged_attention(leaf, c, table, lens).requires_grad
+    with fw.dual_level():
+        with pytest.raises(RuntimeError, match="forward"):
+            paged_attention(fw.make_dual(q, torch.ones_like(q)), c, table, lens)
