@@ -84,7 +84,8 @@ class MixedAttention(nn.Module):
     def rope(self, tokens: int, device) -> torch.Tensor:
         """Angle table of at least ``tokens`` positions."""
         if self._rope is None or self._rope.shape[0] < tokens or self._rope.device != torch.device(device):
-            self._rope = rope_table(max(256, 1 << (tokens - 1).bit_length()), self.d_head, self.rope_theta, device)
+            with torch.inference_mode(False):                # a later training step saves it for its backward
+                self._rope = rope_table(max(256, 1 << (tokens - 1).bit_length()), self.d_head, self.rope_theta, device)
         return self._rope
 
     def norm_rope(self, q: torch.Tensor, k: torch.Tensor | None, tokens: int) -> tuple[torch.Tensor, torch.Tensor | None]:

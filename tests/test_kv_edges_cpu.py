@@ -28,3 +28,16 @@ def test_attention_has_no_gradient():
     with torch.autograd.forward_ad.dual_level():
         with pytest.raises(RuntimeError, match="forward"):
             paged_attention(torch.autograd.forward_ad.make_dual(q.detach(), torch.ones(1, 2, 1, 32)), c, table, lens)
+
+
+def test_training_after_inference_mode():
+    """The angle table that a first call under inference mode built serves a training step too."""
+    from test_models_cpu import _batch
+    from test_onetrans_rotary import _model
+    model, batch = _model(rotary=True), _batch(B=4, windows=2)
+    with torch.inference_mode():
+        model(batch)
+    model.train()
+    total, _, _ = model.forward_loss(batch, {"listen_plus": 1.0}, [])
+    total.backward()
+    assert all(b.attn.q_norm.weight.grad is not None for b in model.blocks)
