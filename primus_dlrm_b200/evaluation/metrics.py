@@ -77,7 +77,8 @@ def score_candidates(model, user_batch: dict[str, torch.Tensor], candidate_batch
     if hasattr(inner, "score_candidates"):
         from primus_dlrm_b200.parallel.fsdp import full_params
         with full_params(inner):          # FSDP units: the scorer reads block weights directly
-            return inner.score_candidates(user_batch, candidate_batch, task, batch_size, kv_cache)
+            extra = {} if kv_cache is None else {"kv_cache": kv_cache}      # not every scorer knows one
+            return inner.score_candidates(user_batch, candidate_batch, task, batch_size, **extra)
     if kv_cache is not None:
         raise ValueError("kv_cache: this model keeps no keys and values")
     C = next(iter(candidate_batch.values())).shape[0]

@@ -41,3 +41,17 @@ def test_training_after_inference_mode():
     total, _, _ = model.forward_loss(batch, {"listen_plus": 1.0}, [])
     total.backward()
     assert all(b.attn.q_norm.weight.grad is not None for b in model.blocks)
+
+
+def test_models_that_score_without_a_cache():
+    """A model whose ``score_candidates`` knows no cache is called as it always was, and refuses one."""
+    from primus_dlrm_b200.evaluation.metrics import score_candidates
+
+    class Model(torch.nn.Module):
+        def score_candidates(self, user, cand, task, batch_size=1024):
+            return cand["x"] * batch_size
+
+    cand = {"x": torch.arange(3.0)}
+    assert score_candidates(Model(), {}, cand, "t", 2).tolist() == [0, 2, 4]
+    with pytest.raises(TypeError):
+        score_candidates(Model(), {}, cand, "t", 2, kv_cache="fp8")
