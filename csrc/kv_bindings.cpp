@@ -107,7 +107,10 @@ at::Tensor rotary_err(int64_t device) {
   static auto* words = new std::vector<at::Tensor>(64);      // never freed: the driver may be gone at exit
   TORCH_CHECK(device >= 0 && device < 64, "no such device");
   at::Tensor& w = (*words)[size_t(device)];
-  if (!w.defined()) w = at::zeros({1}, at::TensorOptions().dtype(at::kInt).device(at::kCUDA, c10::DeviceIndex(device)));
+  if (!w.defined()) {
+    const c10::InferenceMode normal(false);                  // a later training step saves it for its backward
+    w = at::zeros({1}, at::TensorOptions().dtype(at::kInt).device(at::kCUDA, c10::DeviceIndex(device)));
+  }
   return w;
 }
 

@@ -30,19 +30,6 @@ def test_attention_has_no_gradient():
             paged_attention(torch.autograd.forward_ad.make_dual(q.detach(), torch.ones(1, 2, 1, 32)), c, table, lens)
 
 
-def test_training_after_inference_mode():
-    """The angle table that a first call under inference mode built serves a training step too."""
-    from test_models_cpu import _batch
-    from test_onetrans_rotary import _model
-    model, batch = _model(rotary=True), _batch(B=4, windows=2)
-    with torch.inference_mode():
-        model(batch)
-    model.train()
-    total, _, _ = model.forward_loss(batch, {"listen_plus": 1.0}, [])
-    total.backward()
-    assert all(b.attn.q_norm.weight.grad is not None for b in model.blocks)
-
-
 def test_models_that_score_without_a_cache():
     """A model whose ``score_candidates`` knows no cache is called as it always was, and refuses one."""
     from primus_dlrm_b200.evaluation.metrics import score_candidates

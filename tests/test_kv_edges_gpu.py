@@ -357,3 +357,14 @@ def test_attention_has_no_gradient(n):
     with fw.dual_level():
         with pytest.raises(RuntimeError, match="forward"):
             paged_attention(fw.make_dual(q, torch.ones_like(q)), c, table, lens)
+
+
+def test_training_after_inference_mode():
+    """The angle table that a first call under inference mode built serves a training step too."""
+    from test_onetrans_rotary import _model
+    attn, x = _model("cuda", rotary=True, attention_impl="sdpa").blocks[0].attn, torch.randn(2, 30, 64, device=DEV)
+    n_s = 30 - attn.n_ns
+    with torch.inference_mode():
+        attn(x, n_s, 20)
+    attn(x, n_s, 20).sum().backward()
+    assert attn.q_norm.weight.grad.abs().max() > 0
