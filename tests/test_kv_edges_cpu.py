@@ -42,3 +42,18 @@ def test_models_that_score_without_a_cache():
     assert score_candidates(Model(), {}, cand, "t", 2).tolist() == [0, 2, 4]
     with pytest.raises(TypeError):
         score_candidates(Model(), {}, cand, "t", 2, kv_cache="fp8")
+
+
+@pytest.mark.parametrize("rotary", [True, False])
+def test_scores_over_8_bit_pages_are_near_the_exact_ones(rotary):
+    """Keys and values carry 2^-4 relative error each, of random sign, averaged over some 30 tokens and added to a
+    residual stream twice: a quarter of the scores' size bounds what reaches them by a wide margin, and any fault of
+    pages or positions exceeds it."""
+    from test_models_cpu import _batch
+    from test_onetrans_rotary import _model, _split
+    model = _model(rotary=rotary)
+    user, cand, _ = _split(_batch(B=7, L=30, windows=2, seed=5), 7)
+    with torch.no_grad():
+        exact = model.score_candidates(user, cand, "listen_plus")
+        got = model.score_candidates(user, cand, "listen_plus", kv_cache="fp8")
+    assert (got - exact).abs().max() <= 0.25 * exact.abs().max()

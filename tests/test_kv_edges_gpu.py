@@ -368,3 +368,27 @@ def test_training_after_inference_mode():
         attn(x, n_s, 20)
     attn(x, n_s, 20).sum().backward()
     assert attn.q_norm.weight.grad.abs().max() > 0
+
+
+@pytest.mark.parametrize("q_len", [200, 77])
+@pytest.mark.parametrize("impl,dtype,most", [("sdpa", torch.float32, 1e-4), ("fav4", torch.bfloat16, 0.06)])
+def test_gradients_of_a_rotary_layer(impl, dtype, most, q_len):
+    """Every parameter's gradient, the projection's among them, and the input's, against the CPU in 32 bits. 32 bits: sums
+    of some 1600 products, 2^-24 each in random order, and differences that cancel by 10 or so; bf16: some eight roundings
+    of 2^-8 on the way down and up again, that do not all point the same way."""
+    from test_onetrans_rotary import _model
+    gpu, cpu = (_model(d, rotary=True, attention_impl=impl).blocks[0].attn.train() for d in ("cuda", "cpu"))
+    cpu.load_state_dict({k: v.cpu() for k, v in gpu.state_dict().items()})
+    g = torch.Generator().manual_seed(q_len)
+    x, dy = torch.randn(8, 200, 64, generator=g), torch.randn(8, q_len, 64, generator=g)
+    grads = []
+    for m, dev in ((gpu, "cuda"), (cpu, "cpu")):
+        leaf = x.to(dev).requires_grad_()
+        with torch.autocast("cuda", dtype=torch.bfloat16, enabled=dtype != torch.float32 and dev == "cuda"):
+            y = m(leaf.to(dtype if dev == "cuda" else torch.float32), 200 - m.n_ns, q_len)
+        y.backward(dy.to(dev, y.dtype))
+        grads.append({"x": leaf.grad, **{k: p.grad for k, p in m.named_parameters()}})
+    assert {"s_qkv.weight", "ns_qkv_weight", "q_norm.weight", "k_norm.weight"} <= set(grads[0])
+    for k, want in grads[1].items():
+        got = grads[0][k].float().cpu()
+        assert (got - want).norm() <= most * want.norm(), (k, ((got - want).norm() / want.norm()).item())
