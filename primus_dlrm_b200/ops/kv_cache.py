@@ -114,7 +114,8 @@ class PagedKVCache:
         are skipped on append, zeros on read and masked in attention)."""
         e = int(self.err.item())
         if e:
-            self.err.zero_()
+            with torch.inference_mode():                # open to caches made in either mode
+                self.err.zero_()
             raise RuntimeError({1: "paged cache: a page id, or a position, is out of range",
                                 2: "paged cache: a bounded wait in a kernel ran out",
                                 4: "paged cache: a kernel's shared memory is not aligned"}.get(

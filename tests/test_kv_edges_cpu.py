@@ -57,3 +57,12 @@ def test_scores_over_8_bit_pages_are_near_the_exact_ones(rotary):
         exact = model.score_candidates(user, cand, "listen_plus")
         got = model.score_candidates(user, cand, "listen_plus", kv_cache="fp8")
     assert (got - exact).abs().max() <= 0.25 * exact.abs().max()
+
+
+def test_errors_of_a_cache_made_in_inference_mode():
+    with torch.inference_mode():
+        c = PagedKVCache(2, 1, 32, 16)
+        c.err.fill_(1)
+    with pytest.raises(RuntimeError, match="out of range"):
+        c.check_errors()
+    c.check_errors()
