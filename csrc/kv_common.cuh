@@ -61,12 +61,6 @@ struct Raw {
   }
 };
 template <int V, typename T>
-__device__ __forceinline__ void load_v(const T* p, float* f) {
-  Raw<V, T> r;
-  r.load(p);
-  r.floats(f);
-}
-template <int V, typename T>
 __device__ __forceinline__ void store_v(T* p, const float* f) {
   if constexpr (V == 1) {
     *p = from_f<T>(f[0]);
