@@ -25,10 +25,10 @@
 //
 // B200: 12 prompts of 911 to 1824 tokens, 16 x 64: 153 us, 298 TFLOP/s of the
 // products that the mask leaves (floor 27 us by the products, 45 by the
-// exponentials); the same on mma.sync took 254 us. Of the 2890 cycles a block
-// spends on a tile, the softmax warps work 2400 (two warps a sub-partition, each
+// exponentials); the same on mma.sync took 254 us. Of the 2890 cycles that a block
+// spent on a tile (at 154 us, before rows had references), the softmax warps worked 2400 (two warps a sub-partition, each
 // waiting on its own chain) and the issuing lane 1800 (100 to 200 a product).
-// The exponential unit is 39% and issue slots 42% busy. Four more softmax warps, each
+// The exponential unit is 37% and issue slots 41% busy. Four more softmax warps, each
 // pair of warps sharing a quarter of the rows, took 160 us, and 164 to 186 with the
 // two products issued by different warps.
 //

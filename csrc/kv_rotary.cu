@@ -23,10 +23,10 @@
 // angles are loaded before its sum of squares.
 //
 // B200, 912 x 8 x 32 queries and keys (786 x 8 x 32) of a projection, batch 256,
-// bf16, forward and backward: 250 us, 4.4 TB/s over the 1.11 GB that both cannot
+// bf16, forward and backward: 252 us, 4.4 TB/s over the 1.11 GB that both cannot
 // do without (floor 170 us at the copy rate of 6.5 TB/s; 260 us with the next row
-// in registers). The forward runs 24 and the backward 16 warps an SM; issue slots
-// are 52 to 63% full and the ALU pipe 50%, mostly conversions and addresses, and
+// in registers). The forward runs 22 and the backward 15 warps an SM; issue slots
+// are 52 to 60% full and the ALU pipe 50%, mostly conversions and addresses, and
 // neither more rows on their way nor a fourth forward block changes the time.
 // 2049 x 40 x 128 in 32 bits, half turned: 46 us, 5.5 TB/s.
 //

@@ -402,7 +402,8 @@ class OneTransModel(BaseModel):
         (``ops.kv_cache``): every candidate's page table names the user's full
         pages, and only the last, partly filled one is copied, instead of
         expanding the cache to each candidate.  The head dim is then 32, 64 or
-        128, and scores carry the rounding of 8-bit keys and values.
+        128, and scores carry the rounding of 8-bit keys and values; on a GPU the
+        queries and outputs of a 32-bit model are rounded to bf16 there.
         """
         if kv_cache not in (None, "fp8"):
             raise ValueError(f"kv_cache {kv_cache!r}: expected None or 'fp8'")

@@ -50,7 +50,7 @@ class PagedKVCache:
     ``k`` / ``v``: float8_e4m3fn ``[n_pages, n_kv_heads, page_size, head_dim]``;
     ``k_scale`` / ``v_scale``: fp32 ``[n_pages, n_kv_heads]``.  Which pages are
     in use is the caller's business.  ``page_size`` 16, 32 or 64, ``head_dim``
-    32, 64 or 128.
+    32, 64 or 128.  Scales are finite and not negative.
     """
 
     def __init__(self, n_pages: int, n_kv_heads: int, head_dim: int, page_size: int = 64, device=None):
@@ -111,7 +111,8 @@ class PagedKVCache:
     def check_errors(self) -> None:
         """Raises if a kernel met a page id outside the pool, a position outside
         the page table or the angle table, or an impossible length (such tokens
-        are skipped on append, zeros on read and masked in attention)."""
+        are skipped on append, zeros on read and masked in attention; a token
+        outside the angle table alone is kept with a key of zeros)."""
         e = int(self.err.item())
         if e:
             with torch.inference_mode():                # open to caches made in either mode
@@ -297,7 +298,8 @@ def paged_attention(q: torch.Tensor, cache: PagedKVCache, page_table: torch.Tens
     sequence's ``n`` queries are its last ``n`` tokens: query ``i`` sees the
     keys ``j <= kv_lens[b] - n + i``, or with ``causal=False`` all of them.
     ``max_len`` is an upper bound of ``kv_lens`` (by default the page table's
-    room); it only decides how the work is split.  ``scale`` is ``d ** -0.5``
+    room); it only decides how the work is split.  State it, and ``max_q``, where
+    they are known: from the defaults a slower form may be chosen.  ``scale`` is ``d ** -0.5``
     unless given.
 
     Returns ``o`` like ``q`` (contiguous), or ``(o, lse)`` with the natural
