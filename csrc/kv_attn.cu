@@ -59,14 +59,14 @@ constexpr float kSumUnit = 0x1p-31f, kSumLog2 = -31.f;
 // value's, and keys go to registers in the order of memory.
 //
 // ONE: pages hold whole tiles, which then have one pair of scales each (the
-// single tokens below 113 us, the candidates 134; the general form 126 and 152).
+// single tokens below 111 us, the candidates 133; the general form 126 and 152).
 //
 // B200: 64 single tokens over 300 to 8191 keys, 32 heads over 8 x 128 (R = 8):
-// 113 us, 4.9 TB/s of the cache (floor 85 us); three over 65537 to 131071 keys, 16
+// 111 us, 5.0 TB/s of the cache (floor 85 us); three over 65537 to 131071 keys, 16
 // heads over 4 x 64, pages of 16: 44 us, 3.5 TB/s (floor 23 us). Neither pipe is full (issue
 // slots 38%, DRAM 75%): 12 warps an SM, bound by registers and the ring (by the ring
 // alone at d = 64), wait on their own chains. 1024 x 16 candidate tokens behind 896 shared keys, 8 x 32 (R = 16, W =
-// 1): 134 us; the keys come from L2 and the instructions around 16-row products
+// 1): 133 us; the keys come from L2 and the instructions around 16-row products
 // bound it (issue 50% of active cycles; a copy's bookkeeping is 30% of them: 64
 // keys a copy instead of 128 cost 179 us).
 template <int D, int R, int W, bool ONE>
@@ -87,7 +87,10 @@ paged_attn_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ CU
   __shared__ uint64_t s_bar[kWarps][ST];
   __shared__ int64_t s_scan[kWarps], s_start[kWarps / W][2];
 
-  tiles_aligned(s_ring, A.err);
+  if (!tiles_aligned(s_ring, A.err)) {
+    if (A.split && threadIdx.x < 2) A.part_head[(blockIdx.x * 2 + threadIdx.x) * 4] = -1;      // no pieces
+    return;
+  }
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int part = W == 1 ? 0 : warp;                       // of the segment's warps
   const int g = lane >> 2, qd = lane & 3;
