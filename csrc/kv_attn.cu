@@ -63,7 +63,7 @@ constexpr float kSumUnit = 0x1p-31f, kSumLog2 = -31.f;
 //
 // B200: 64 single tokens over 300 to 8191 keys, 32 heads over 8 x 128 (R = 8):
 // 111 us, 5.0 TB/s of the cache (floor 85 us); three over 65537 to 131071 keys, 16
-// heads over 4 x 64, pages of 16: 44 us, 3.5 TB/s (floor 23 us). Neither pipe is full (issue
+// heads over 4 x 64, pages of 16: 45 us, 3.4 TB/s (floor 23 us). Neither pipe is full (issue
 // slots 38%, DRAM 75%): 12 warps an SM, bound by registers and the ring (by the ring
 // alone at d = 64), wait on their own chains. 1024 x 16 candidate tokens behind 896 shared keys, 8 x 32 (R = 16, W =
 // 1): 133 us; the keys come from L2 and the instructions around 16-row products

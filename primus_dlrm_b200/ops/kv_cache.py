@@ -227,7 +227,10 @@ class PagedKVCache:
         behind a shared one.  Every source is read before the first page is
         written.  A pair with an id outside the pool is skipped and reported by
         :meth:`check_errors` (IndexError on the eager path)."""
-        src, dst = (t.to(self.device, torch.int64) for t in torch.broadcast_tensors(src, dst))
+        src, dst = torch.broadcast_tensors(torch.as_tensor(src), torch.as_tensor(dst))
+        if src.numel() and any(t.dtype == torch.bool or t.is_floating_point() for t in (src, dst)):
+            raise TypeError("page ids must be integers")
+        src, dst = (t.to(self.device, torch.int64).reshape(-1) for t in (src, dst))
         if self._native():
             _ext.kv().copy_pages(*self._parts, src.contiguous(), dst.contiguous())
             return

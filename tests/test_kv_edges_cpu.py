@@ -66,3 +66,16 @@ def test_errors_of_a_cache_made_in_inference_mode():
     with pytest.raises(RuntimeError, match="out of range"):
         c.check_errors()
     c.check_errors()
+
+
+def test_copy_pages_of_other_kinds():
+    """Lists, scalars for many, and shapes of ids as an assignment by index takes them; masks are no ids."""
+    for src, dst, want in (([0], [1, 2], [1, 1, 1, 4]), (0, [3], [1, 2, 3, 1]), ([[0, 1]], [[2, 3]], [1, 2, 1, 2]), ([], [], [1, 2, 3, 4])):
+        c = PagedKVCache(4, 1, 32, 16)
+        c.k_scale.copy_(torch.arange(4.0)[:, None] + 1)
+        c.copy_pages(src, torch.tensor(dst))
+        assert c.k_scale.flatten().tolist() == want
+    with pytest.raises(TypeError):
+        c.copy_pages(torch.tensor([True, False, False, False]), torch.tensor([1]))
+    with pytest.raises(TypeError):
+        c.copy_pages(torch.tensor([0.0]), torch.tensor([1]))
