@@ -166,7 +166,7 @@ def _gelu_grad(x):
 def _linear_plain(s):
     x, w, t = s["x"].float(), s["codes"].float(), s["scale"]
     sx = (x.abs().amax(-1, keepdim=True) / 127).clamp(min=2.0 ** -126)
-    a = torch.round(x / sx)
+    a = torch.round(x * (1 / sx))
     if w.dim() == 3:
         y = (a.transpose(0, 1) @ w.transpose(1, 2)).transpose(0, 1)
     else:
@@ -287,9 +287,9 @@ def run(state):
 def _exact_linear(s):
     case = s["case"]
     x, w, t = s["x"].double(), s["codes"].double(), s["scale"].double()
-    # the scale is a 32-bit number and a code the integer nearest to the 32-bit quotient: both are of the definition
+    # a token's scale, its reciprocal and the product that a code is nearest to are 32-bit numbers by definition
     sx = torch.clamp(s["x"].float().abs().max(-1, keepdim=True).values / 127, min=2.0 ** -126)
-    a = torch.round(s["x"].float() / sx).double()
+    a = torch.round(s["x"].float() * torch.reciprocal(sx)).double()
     y = torch.einsum("mk,nk->mn", a, w) if w.dim() == 2 else torch.einsum("mgk,gnk->mgn", a, w)
     y = y * sx.double() * t
     if s["bias"] is not None:
