@@ -34,7 +34,15 @@ inline CUresult tensor_map_encode_tiled(CUtensorMap* map, CUtensorMapDataType dt
                           const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
                           CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
   static Fn fn = driver_entry<Fn>("cuTensorMapEncodeTiled");
-  return fn(map, dtype, rank, base, dims, strides, box, estrides, interleave, swizzle, l2, oob);
+  CUresult r = fn(map, dtype, rank, base, dims, strides, box, estrides, interleave, swizzle, l2, oob);
+  if (r == CUDA_ERROR_INVALID_CONTEXT) {
+    // the thread's first call (a backward pass that begins with a GEMM runs on autograd's own thread): the runtime
+    // binds the device's context to a thread when the thread sets its device
+    int dev = 0;
+    if (cudaGetDevice(&dev) == cudaSuccess && cudaSetDevice(dev) == cudaSuccess)
+      r = fn(map, dtype, rank, base, dims, strides, box, estrides, interleave, swizzle, l2, oob);
+  }
+  return r;
 }
 
 inline CUresult mem_get_address_range(CUdeviceptr* base, size_t* size, CUdeviceptr ptr) {
