@@ -32,8 +32,13 @@
 // in-flight operations (bounded) and the CTA frees its TMEM and exits.
 #include "common.cuh"
 #include "driver_api.h"
+#include "int8_common.cuh"
+#include "tc_common.cuh"
 
 #include <cuda.h>
+
+#include <c10/cuda/CUDAGuard.h>
+#include <type_traits>
 
 namespace pd {
 namespace tc {
@@ -42,7 +47,6 @@ constexpr int BM = 128;
 constexpr int BK = 64;
 constexpr int kEpiWarps = 12;  // three warps per TMEM lane quarter, splitting the columns
 constexpr int kThreads = 64 + 32 * kEpiWarps;
-constexpr uint64_t kWaitLimitNs = 2000000000ull;
 
 // kGeluD: C = GELU(x), AUX = GELU'(x) for x = acc + R in fp32 -- the derivative
 // stored in the forward makes the backward's epilogue a plain product (kMul:
@@ -70,156 +74,15 @@ struct Params {
   int b_shared;         // B has one batch shared by every l
   int b_kn;             // B stored [L, K, N] (N contiguous: a weight used transposed), loaded MN-major
   int* err;
+  // pre-activations in 8 bits (int8_common.cuh): codes [L, M, N] and scale bytes [L, M, N / 32]
+  int8_t* X8; int64_t x8_ls, x8_ms;
+  uint8_t* E; int64_t e_ls, e_ms, e_bs;
 };
 
-__device__ __forceinline__ uint32_t smem_u32(const void* p) {
-  return static_cast<uint32_t>(__cvta_generic_to_shared(p));
-}
-
-// ---- mbarrier --------------------------------------------------------------
-__device__ __forceinline__ void mbar_init(uint64_t* b, uint32_t count) {
-  asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(smem_u32(b)), "r"(count));
-}
-__device__ __forceinline__ void mbar_expect_tx(uint64_t* b, uint32_t bytes) {
-  asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(smem_u32(b)), "r"(bytes) : "memory");
-}
-__device__ __forceinline__ void mbar_arrive(uint64_t* b) {
-  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(b)) : "memory");
-}
-// try_wait with a suspend-time hint: a waiting warp sleeps until the phase
-// completes or ~0.2 ms pass instead of spinning on issue slots.
-__device__ __forceinline__ bool mbar_try(uint64_t* b, uint32_t parity) {
-  uint32_t ok;
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
-      "selp.b32 %0, 1, 0, p;\n\t}"
-      : "=r"(ok) : "r"(smem_u32(b)), "r"(parity), "r"(200000u) : "memory");
-  return ok != 0;
-}
-// Bounded wait: false (and the error word set) after kWaitLimitNs.
-__device__ __forceinline__ bool mbar_wait(uint64_t* b, uint32_t parity, int* err) {
-  if (mbar_try(b, parity)) return true;
-  const uint64_t t0 = globaltimer_ns();
-  while (!mbar_try(b, parity)) {
-    if (globaltimer_ns() - t0 > kWaitLimitNs) {
-      set_error(err, kWaitTimeout);
-      return false;
-    }
-  }
-  return true;
-}
-
-// ---- TMA -------------------------------------------------------------------
-__device__ __forceinline__ void tma_load_3d(void* dst, const CUtensorMap* map, uint64_t* bar, int c0, int c1, int c2);
-// Load rows [row, row + box) of batch l; mode 1 maps have dims {K, L, rows}.
-__device__ __forceinline__ void tma_load_rows(void* dst, const CUtensorMap* map, uint64_t* bar, int mode, int k, int row,
-                                              int l) {
-  if (mode == 0) tma_load_3d(dst, map, bar, k, row, l);
-  else tma_load_3d(dst, map, bar, k, l, row);
-}
-__device__ __forceinline__ void tma_load_3d(void* dst, const CUtensorMap* map, uint64_t* bar, int c0, int c1, int c2) {
-  asm volatile(
-      "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];"
-      ::"r"(smem_u32(dst)), "l"(map), "r"(smem_u32(bar)), "r"(c0), "r"(c1), "r"(c2) : "memory");
-}
-
-// TMA store of one 32 x 32 bf16 block staged in shared memory (64-byte
-// swizzle); mode 1 maps have dims {N, L, rows}.  Rows past the tensor's end
-// are clipped by the copy engine.
-__device__ __forceinline__ void tma_store_3d(const CUtensorMap* map, const void* src, int c0, int c1, int c2) {
-  asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.bulk_group [%0, {%2, %3, %4}], [%1];"
-               ::"l"(map), "r"(smem_u32(src)), "r"(c0), "r"(c1), "r"(c2) : "memory");
-}
-__device__ __forceinline__ void tma_store_rows(const CUtensorMap* map, const void* src, int mode, int n, int row,
-                                               int l) {
-  if (mode == 0) tma_store_3d(map, src, n, row, l);
-  else tma_store_3d(map, src, n, l, row);
-}
-__device__ __forceinline__ void bulk_commit() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); }
-// the staged source of every committed store has been read (the buffer may be rewritten)
-__device__ __forceinline__ void bulk_wait_read_all() { asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory"); }
-__device__ __forceinline__ void bulk_wait_all() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
-// generic-proxy shared-memory writes -> visible to the async proxy (TMA)
-__device__ __forceinline__ void fence_async_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
-
-// ---- tcgen05 ---------------------------------------------------------------
-__device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
-__device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
-
-// K-major, 128-byte-swizzled operand tile: rows of 64 bf16 (128 B), 8-row
-// atoms of 1024 B.  start advances by 32 B per 16-element k-step.
-__device__ __forceinline__ uint64_t smem_desc(uint32_t addr) {
-  uint64_t d = 0;
-  d |= uint64_t((addr >> 4) & 0x3FFF);        // start address
-  d |= uint64_t(1) << 16;                       // leading byte offset (unused for swizzled K-major)
-  d |= uint64_t(1024 >> 4) << 32;               // stride byte offset: 8 rows x 128 B
-  d |= uint64_t(1) << 46;                       // descriptor version (sm_100)
-  d |= uint64_t(2) << 61;                       // SWIZZLE_128B
-  return d;
-}
-// MN-major, 128-byte-swizzled B tile: BN / 64 groups of [64 k-rows][64 n]
-// (8 KB each, 128 B per k-row); a 16-row k-step starts 2048 B further, the
-// groups are 8192 B apart (leading byte offset), 8-row atoms 1024 B apart.
-__device__ __forceinline__ uint64_t smem_desc_mn(uint32_t addr) {
-  uint64_t d = 0;
-  d |= uint64_t((addr >> 4) & 0x3FFF);
-  d |= uint64_t(8192 >> 4) << 16;
-  d |= uint64_t(1024 >> 4) << 32;
-  d |= uint64_t(1) << 46;
-  d |= uint64_t(2) << 61;
-  return d;
-}
-// kind::f16 instruction descriptor: f32 accumulate, bf16 A/B, both K-major.
-__host__ __device__ constexpr uint32_t instr_desc(int m, int n) {
-  return (1u << 4) | (1u << 7) | (1u << 10) | (uint32_t(n >> 3) << 17) | (uint32_t(m >> 4) << 24);
-}
-__device__ __forceinline__ void tc_mma(uint32_t tmem_d, uint64_t da, uint64_t db, uint32_t idesc, uint32_t acc) {
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
-      ::"r"(tmem_d), "l"(da), "l"(db), "r"(idesc), "r"(acc) : "memory");
-}
-__device__ __forceinline__ void tc_commit(uint64_t* bar) {
-  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];"
-               ::"r"(smem_u32(bar)) : "memory");
-}
-// tcgen05.ld of 32 columns without the wait (registers undefined until
-// tc_ld_wait on the same array, which ties them to the wait instruction).
-__device__ __forceinline__ void tc_ld32_issue(uint32_t taddr, uint32_t (&r)[32]) {
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
-      "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
-      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
-        "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
-        "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
-        "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
-      : "r"(taddr) : "memory");
-}
-__device__ __forceinline__ void tc_ld_wait(uint32_t (&r)[32]) {
-  asm volatile("tcgen05.wait::ld.sync.aligned;"
-               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
-                 "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]),
-                 "+r"(r[15]), "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]),
-                 "+r"(r[22]), "+r"(r[23]), "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]),
-                 "+r"(r[29]), "+r"(r[30]), "+r"(r[31])
-               :: "memory");
-}
-__device__ __forceinline__ void tc_ld32(uint32_t taddr, float* v) {
-  uint32_t r[32];
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
-      "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
-      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
-        "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
-        "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
-        "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
-      : "r"(taddr));
-  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-#pragma unroll
-  for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
-}
+// What the epilogue does with pre-activations in 8 bits. kSave: C = GELU(acc) and the pre-activation acc leaves as
+// codes: a thread holds 32 columns of its row, which is one block of codes, so the block's maximum and scale take no
+// exchange. kUse: p = the values of such codes, C = acc * GELU'(p) and AUX = GELU(p).
+enum Saved8 : int { kNotSaved = 0, kSave = 1, kUse = 2 };
 
 __device__ __forceinline__ void tile_coords(const Params& p, int t, int& l, int& mb, int& nb) {
   nb = t % p.n_blocks;
@@ -228,7 +91,7 @@ __device__ __forceinline__ void tile_coords(const Params& p, int t, int& l, int&
   l = r / p.m_blocks;
 }
 
-template <int BN, int STAGES>
+template <int BN, int STAGES, int SAVED8 = kNotSaved>
 __global__ void __launch_bounds__(kThreads, 1) gemm_kernel(const __grid_constant__ CUtensorMap tmA,
                                                            const __grid_constant__ CUtensorMap tmB,
                                                            const __grid_constant__ CUtensorMap tmC,
@@ -373,7 +236,7 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_kernel(const __grid_constant
     int r_pending = 0;   // R blocks issued and not yet waited for
     const int cr = lane >> 2, cc = lane & 3;
     auto sw = [](int r, int c) { return r * 64 + ((c ^ ((r >> 1) & 3)) << 4); };
-    const bool has_r = (p.R != nullptr);   // addend (bias / residual), or GELU's pre-activation for kDGelu
+    const bool has_r = SAVED8 == kNotSaved && p.R != nullptr;   // addend (bias / residual), or GELU's pre-activation for kDGelu
     // work items: (tile, chunk) in this warp's order
     auto first_chunk = [&]() { return part * 32; };
     auto next_work = [&](int& t, int& c) {
@@ -399,6 +262,23 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_kernel(const __grid_constant
       mbar_expect_tx(&rbar[buf], 32 * 32 * 2);
       tma_load_rows(stR0 + (buf << 11), &tmR, &rbar[buf], p.r_mode, nb * BN + c, mb * BM + q * 32, l);
     };
+    // the codes and scale byte of this thread's next row and chunk, on their way (kUse)
+    uint4 code0 = make_uint4(0, 0, 0, 0), code1 = code0;
+    uint32_t code_scale = 1;
+    auto load_codes = [&](int t, int c) {
+      int l, mb, nb;
+      tile_coords(p, t, l, mb, nb);
+      const int m = mb * BM + q * 32 + lane, n = nb * BN + c;
+      if (m < p.M) {
+        const uint4* src = reinterpret_cast<const uint4*>(p.X8 + l * p.x8_ls + int64_t(m) * p.x8_ms + n);
+        code0 = __ldcs(src);
+        code1 = __ldcs(src + 1);
+        code_scale = p.E[l * p.e_ls + m * p.e_ms + (n >> 5) * p.e_bs];
+      }
+    };
+    if constexpr (SAVED8 == kUse) {
+      if (first_chunk() < BN && blockIdx.x < p.tiles) load_codes(blockIdx.x, first_chunk());
+    }
     uint4 pref[4];
     if (has_r && first_chunk() < BN && blockIdx.x < p.tiles) {
       if (r_tma) {
@@ -455,7 +335,55 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_kernel(const __grid_constant
         float v[32];
 #pragma unroll
         for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
-        if (has_r && p.epi != kDGelu && p.epi != kMul && p.epi != kMaskPos && p.epi != kMulAdd) {
+        if constexpr (SAVED8 == kSave) {
+          uint32_t most = 0;
+#pragma unroll
+          for (int i = 0; i < 32; ++i) most = max(most, i8::abs_bits(v[i]));
+          const uint32_t byte = i8::scale_byte(most);
+          const float inv = i8::inv_scale(byte), lim = i8::most_code(byte, i8::kTopWide);
+          uint32_t w[8];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) w[i] = i8::codes4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3], inv, lim);
+          if (m0 + lane < p.M) {
+            uint4* dst = reinterpret_cast<uint4*>(p.X8 + l * p.x8_ls + int64_t(m0 + lane) * p.x8_ms + n0 + c);
+            dst[0] = make_uint4(w[0], w[1], w[2], w[3]);
+            dst[1] = make_uint4(w[4], w[5], w[6], w[7]);
+            p.E[l * p.e_ls + (m0 + lane) * p.e_ms + ((n0 + c) >> 5) * p.e_bs] = uint8_t(byte);
+          }
+#pragma unroll
+          for (int j = 0; j < 32; j += 2) gelu2(v[j], v[j + 1]);
+        } else if constexpr (SAVED8 == kUse) {
+          const uint32_t w[8] = {code0.x, code0.y, code0.z, code0.w, code1.x, code1.y, code1.z, code1.w};
+          const float scale = i8::scale_of(code_scale);
+          {
+            int tn = t, cn = c;
+            next_work(tn, cn);
+            if (tn < p.tiles) load_codes(tn, cn);          // in flight during this chunk
+          }
+          wait_staging();
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            float g[8];
+            i8::ints4(w[2 * j], g);
+            i8::ints4(w[2 * j + 1], g + 4);
+#pragma unroll
+            for (int e = 0; e < 8; e += 2) {
+              float d0, d1;
+              pk2_split(pk2_mul(pk2(g[e], g[e + 1]), pk2s(scale)), g[e], g[e + 1]);
+              gelu_grad2<true>(g[e], g[e + 1], d0, d1);
+              v[8 * j + e] *= d0;
+              v[8 * j + e + 1] *= d1;
+            }
+            uint4 pk;
+            __nv_bfloat162 h0 = __floats2bfloat162_rn(g[0], g[1]);
+            __nv_bfloat162 h1 = __floats2bfloat162_rn(g[2], g[3]);
+            __nv_bfloat162 h2 = __floats2bfloat162_rn(g[4], g[5]);
+            __nv_bfloat162 h3 = __floats2bfloat162_rn(g[6], g[7]);
+            pk.x = *reinterpret_cast<uint32_t*>(&h0); pk.y = *reinterpret_cast<uint32_t*>(&h1);
+            pk.z = *reinterpret_cast<uint32_t*>(&h2); pk.w = *reinterpret_cast<uint32_t*>(&h3);
+            *reinterpret_cast<uint4*>(stX + sw(lane, j)) = pk;
+          }
+        } else if (has_r && p.epi != kDGelu && p.epi != kMul && p.epi != kMaskPos && p.epi != kMulAdd) {
           // addend before the activation: residual, or a bias broadcast through a zero row stride
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
@@ -469,7 +397,8 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_kernel(const __grid_constant
             }
           }
         }
-        if (p.epi == kGelu && p.AUX) {
+        if (SAVED8 != kNotSaved) {
+        } else if (p.epi == kGelu && p.AUX) {
           wait_staging();
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
@@ -483,7 +412,8 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_kernel(const __grid_constant
             *reinterpret_cast<uint4*>(stX + sw(lane, j)) = pk;
           }
         }
-        if (p.epi == kGelu) {
+        if (SAVED8 != kNotSaved) {
+        } else if (p.epi == kGelu) {
           // GELU of the bf16-rounded pre-activation (the value AUX stores)
 #pragma unroll
           for (int j = 0; j < 32; j += 2) {
@@ -607,7 +537,7 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_kernel(const __grid_constant
         __syncwarp();
         if (lane == 0) {
           tma_store_rows(&tmC, stC, p.c_mode, n0 + c, m0, l);
-          if ((p.epi == kGelu || p.epi == kGeluD || p.epi == kMulAdd) && p.AUX)
+          if (SAVED8 == kUse || (SAVED8 == kNotSaved && (p.epi == kGelu || p.epi == kGeluD || p.epi == kMulAdd) && p.AUX))
             tma_store_rows(&tmX, stX, p.x_mode, n0 + c, m0, l);
           bulk_commit();
         }
@@ -936,19 +866,19 @@ void check_operand(const at::Tensor& t, const char* name) {
   check_extent(t, name);
 }
 
-template <int BN, int STAGES>
+template <int BN, int STAGES, int SAVED8 = tc::kNotSaved>
 void launch(const CUtensorMap& ta, const CUtensorMap& tb, const CUtensorMap& tcm, const CUtensorMap& txm,
             const CUtensorMap& trm, const tc::Params& p) {
   constexpr size_t smem = STAGES * (tc::BM * tc::BK * 2 + BN * tc::BK * 2) + 1024 + 1024 + tc::kEpiWarps * 3 * 2048;
   static_assert(smem <= 232448, "GEMM shared memory over the 227 KB per-block limit");
   static bool attr = false;
   if (!attr) {
-    PD_CHECK_CUDA(cudaFuncSetAttribute(tc::gemm_kernel<BN, STAGES>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                       int(smem)));
+    PD_CHECK_CUDA(cudaFuncSetAttribute(tc::gemm_kernel<BN, STAGES, SAVED8>,
+                                       cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem)));
     attr = true;
   }
   int grid = p.tiles < num_sms() ? p.tiles : num_sms();
-  tc::gemm_kernel<BN, STAGES><<<grid, tc::kThreads, smem, stream()>>>(ta, tb, tcm, txm, trm, p);
+  tc::gemm_kernel<BN, STAGES, SAVED8><<<grid, tc::kThreads, smem, stream()>>>(ta, tb, tcm, txm, trm, p);
   PD_CHECK_LAUNCH();
 }
 
@@ -1030,6 +960,68 @@ void tc_gemm(at::Tensor A, at::Tensor B, at::Tensor C, int64_t epi, c10::optiona
   else launch<64, 6>(ta, tb, tcm, txm, trm, p);
 }
 
+// The two GEMMs around pre-activations kept in 8 bits: codes [L, M, N] int8 views with rows on 16 bytes, exps [L, M, N / 32]
+// uint8 views of any strides. With AUX undefined (the up projection): C = GELU(A @ B^T), codes and exps are written. With
+// AUX (the down projection's data gradient): p = the values of codes, C = (A @ B^T) * GELU'(p), AUX = GELU(p).
+void tc_gemm_saved8(at::Tensor A, at::Tensor B, at::Tensor C, at::Tensor codes, at::Tensor exps,
+                    c10::optional<at::Tensor> AUX, at::Tensor err, bool b_kn) {
+  check_operand(A, "A");
+  check_operand(B, "B");
+  const int64_t L = A.size(0), M = A.size(1), K = A.size(2), N = b_kn ? B.size(2) : B.size(1);
+  PD_CHECK((b_kn ? B.size(1) : B.size(2)) == K && (B.size(0) == L || B.size(0) == 1), "B must fit A");
+  PD_CHECK(N % 64 == 0, "N must be a multiple of 64");
+  auto matrix = [&](const at::Tensor& t, at::ScalarType type, int64_t n, const char* what) {
+    PD_CHECK(t.is_cuda() && t.device() == A.device() && t.scalar_type() == type && t.dim() == 3 && t.size(0) == L &&
+                 t.size(1) == M && t.size(2) == n, "%s does not fit the product", what);
+    check_extent(t, what);
+  };
+  auto rows16 = [&](const at::Tensor& t, const char* what) {
+    const int64_t e = t.element_size();
+    PD_CHECK(t.stride(2) == 1 && t.stride(1) * e % 16 == 0 && (L == 1 || t.stride(0) * e % 16 == 0) &&
+                 reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0, "%s: rows must lie on 16 bytes", what);
+  };
+  matrix(C, at::kBFloat16, N, "C");
+  rows16(C, "C");
+  matrix(codes, at::kChar, N, "codes");
+  rows16(codes, "codes");
+  matrix(exps, at::kByte, N / 32, "exps");
+  PD_CHECK(B.device() == A.device() && err.device() == A.device(), "operands lie on two devices");
+  if (M == 0 || L == 0) return;
+  const c10::cuda::CUDAGuard guard(A.device());
+  tc::Params p{};
+  p.M = int(M); p.N = int(N); p.K = int(K); p.L = int(L);
+  p.m_blocks = int((M + tc::BM - 1) / tc::BM);
+  p.k_blocks = int((K + tc::BK - 1) / tc::BK);
+  p.C = reinterpret_cast<__nv_bfloat16*>(C.data_ptr()); p.c_ls = C.stride(0); p.c_ms = C.stride(1);
+  p.err = err.data_ptr<int>();
+  p.X8 = codes.data_ptr<int8_t>(); p.x8_ls = codes.stride(0); p.x8_ms = codes.stride(1);
+  p.E = exps.data_ptr<uint8_t>(); p.e_ls = exps.stride(0); p.e_ms = exps.stride(1); p.e_bs = exps.stride(2);
+  const int BN = (N % 256 == 0) ? 256 : (N % 128 == 0 ? 128 : 64);
+  p.n_blocks = int(N / BN);
+  p.tiles = int(L) * p.m_blocks * p.n_blocks;
+  const CUtensorMap ta = make_map(A.data_ptr(), K, M, L, A.stride(1), A.stride(0), tc::BM, p.a_mode);
+  p.b_kn = b_kn ? 1 : 0;
+  const CUtensorMap tb = b_kn ? make_map(B.data_ptr(), N, K, B.size(0), B.stride(1), B.stride(0), tc::BK, p.b_mode)
+                              : make_map(B.data_ptr(), K, N, B.size(0), B.stride(1), B.stride(0), BN, p.b_mode);
+  p.b_shared = (B.size(0) == 1) ? 1 : 0;
+  const CUtensorMap tcm = make_store_map(C.data_ptr(), N, M, L, C.stride(1), C.stride(0), p.c_mode);
+  auto go = [&](auto mode, const CUtensorMap& tx) {
+    constexpr int kMode = decltype(mode)::value;
+    if (BN == 256) launch<256, 3, kMode>(ta, tb, tcm, tx, tcm, p);
+    else if (BN == 128) launch<128, 4, kMode>(ta, tb, tcm, tx, tcm, p);
+    else launch<64, 6, kMode>(ta, tb, tcm, tx, tcm, p);
+  };
+  if (AUX && AUX->defined()) {
+    matrix(*AUX, at::kBFloat16, N, "AUX");
+    rows16(*AUX, "AUX");
+    p.AUX = reinterpret_cast<__nv_bfloat16*>(AUX->data_ptr());
+    const CUtensorMap tx = make_store_map(AUX->data_ptr(), N, M, L, AUX->stride(1), AUX->stride(0), p.x_mode);
+    go(std::integral_constant<int, tc::kUse>(), tx);
+  } else {
+    p.x_mode = p.c_mode;
+    go(std::integral_constant<int, tc::kSave>(), tcm);
+  }
+}
 
 // C[l] (fp32 [M, N], zeroed by the caller) += A[l]^T B[l] over the rows:
 // A [L, K, M], B [L, K, N] bf16 views with unit stride on the last dim.

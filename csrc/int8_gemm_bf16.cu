@@ -1,0 +1,8 @@
+// The 8-bit integer products with results of this type.
+#include "int8_gemm.cuh"
+
+namespace pd {
+namespace i8 {
+template void product<__nv_bfloat16>(const CUtensorMap&, const void*, int64_t, int64_t, const CUtensorMap&, Params&);
+}  // namespace i8
+}  // namespace pd

@@ -1,0 +1,320 @@
+// Activations to 8-bit integers and back: blocks of 32 values with a
+// power-of-two scale (save8 / load8, for training), and whole rows with a
+// 32-bit scale (quantize_rows, for integer products).
+#include "int8_common.cuh"
+#include "kv_common.cuh"
+
+#include <c10/cuda/CUDAGuard.h>
+
+#include <algorithm>
+#include <type_traits>
+
+namespace pd {
+namespace i8 {
+
+using kv::Raw;
+
+// Eight consecutive values of a row from element k on, zeros behind its end.
+template <bool VEC, typename T>
+struct Eight {
+  Raw<VEC ? 8 : 1, T> r[VEC ? 1 : 8];
+  __device__ __forceinline__ void load(const T* row, int64_t k, int64_t K) {
+    if constexpr (VEC) {
+      if (k < K) r[0].load(row + k); else r[0].zero();
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        if (k + i < K) r[i].load(row + k + i); else r[i].zero();
+      }
+    }
+  }
+  __device__ __forceinline__ void floats(float* f) const {
+    if constexpr (VEC) {
+      r[0].floats(f);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) r[i].floats(f + i);
+    }
+  }
+};
+template <bool VEC>
+__device__ __forceinline__ void store_codes(int8_t* row, int64_t k, int64_t K, uint2 c) {
+  if constexpr (VEC) {
+    if (k < K) *reinterpret_cast<uint2*>(row + k) = c;
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (k + i < K) row[k + i] = int8_t(__byte_perm(c.x, c.y, i));
+  }
+}
+__device__ __forceinline__ uint32_t most_bits(const float* f) {
+  uint32_t m = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) m = max(m, abs_bits(f[i]));
+  return m;
+}
+
+// save8. A warp takes 8 rows x 4 blocks at a time: four lanes hold a block, so
+// its maximum takes two shuffles, a row's 64 to 128 bytes of each load are
+// whole sectors and four loads of a lane are on their way. Scale bytes lie
+// block-major ([blocks, rows]): that is how the GEMM epilogues, whose threads
+// own rows, write and read them in whole sectors.
+constexpr int kRows = 8, kBlocks = 4;
+template <bool VEC, typename T>
+__global__ void __launch_bounds__(256) save_kernel(const T* __restrict__ x, int64_t x_stride, int8_t* __restrict__ codes,
+                                                   uint8_t* __restrict__ exps, int64_t rows, int64_t K, int64_t blocks,
+                                                   uint32_t top) {
+  const int lane = threadIdx.x & 31, q = lane & 3;
+  const int64_t across = (blocks + kBlocks - 1) / kBlocks;
+  const int64_t tiles = (rows + kRows - 1) / kRows * across;
+  for (int64_t t = int64_t(blockIdx.x) * 8 + (threadIdx.x >> 5); t < tiles; t += int64_t(gridDim.x) * 8) {
+    const int64_t row = t / across * kRows + (lane >> 2), b0 = t % across * kBlocks;
+    const bool there = row < rows;
+    const T* src = x + (there ? row : 0) * x_stride;
+    Eight<VEC, T> raw[kBlocks];
+#pragma unroll
+    for (int j = 0; j < kBlocks; ++j) raw[j].load(src, (b0 + j) * kBlock + q * 8, there ? K : 0);
+    uint32_t mine = 0;
+#pragma unroll
+    for (int j = 0; j < kBlocks; ++j) {
+      float f[8];
+      raw[j].floats(f);
+      uint32_t m = most_bits(f);
+      m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
+      m = max(m, __shfl_xor_sync(0xffffffffu, m, 2));
+      const uint32_t b = scale_byte(m);
+      if (q == j) mine = b;
+      const float inv = inv_scale(b), most = most_code(b, top);
+      const uint2 c = make_uint2(codes4(f[0], f[1], f[2], f[3], inv, most), codes4(f[4], f[5], f[6], f[7], inv, most));
+      if (there) store_codes<VEC>(codes + row * K, (b0 + j) * kBlock + q * 8, K, c);
+    }
+    if (there && b0 + q < blocks) exps[(b0 + q) * rows + row] = uint8_t(mine);
+  }
+}
+
+template <bool VEC, typename T>
+__global__ void __launch_bounds__(256) load_kernel(const int8_t* __restrict__ codes, const uint8_t* __restrict__ exps,
+                                                   T* __restrict__ y, int64_t rows, int64_t K, int64_t blocks) {
+  const int lane = threadIdx.x & 31, q = lane & 3;
+  const int64_t across = (blocks + kBlocks - 1) / kBlocks;
+  const int64_t tiles = (rows + kRows - 1) / kRows * across;
+  for (int64_t t = int64_t(blockIdx.x) * 8 + (threadIdx.x >> 5); t < tiles; t += int64_t(gridDim.x) * 8) {
+    const int64_t row = t / across * kRows + (lane >> 2), b0 = t % across * kBlocks;
+    if (row >= rows) continue;
+    uint2 c[kBlocks];
+    uint32_t e[kBlocks];
+#pragma unroll
+    for (int j = 0; j < kBlocks; ++j) {
+      const int64_t k = (b0 + j) * kBlock + q * 8;
+      c[j] = make_uint2(0, 0);
+      e[j] = b0 + j < blocks ? exps[(b0 + j) * rows + row] : 1;
+      if constexpr (VEC) {
+        if (k < K) c[j] = *reinterpret_cast<const uint2*>(codes + row * K + k);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          if (k + i < K) (i < 4 ? c[j].x : c[j].y) |= uint32_t(uint8_t(codes[row * K + k + i])) << (8 * (i & 3));
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < kBlocks; ++j) {
+      const int64_t k = (b0 + j) * kBlock + q * 8;
+      float f[8];
+      ints4(c[j].x, f);
+      ints4(c[j].y, f + 4);
+      const float s = scale_of(e[j]);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) f[i] *= s;
+      if constexpr (VEC) {
+        if (k < K) kv::store_v<8, T>(y + row * K + k, f);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          if (k + i < K) y[row * K + k + i] = kv::from_f<T>(f[i]);
+      }
+    }
+  }
+}
+
+// quantize_rows: TPR threads share a row and keep it in registers between the
+// maximum and the codes (NV vectors of 8 a thread); longer rows are read again.
+// Codes lie in rows of `pitch` bytes, zeros behind a row's end.
+template <bool VEC, int TPR, int NV, typename T>
+__global__ void __launch_bounds__(256) rows_kernel(const T* __restrict__ x, int64_t x_outer, int64_t x_inner, int64_t inner,
+                                                   int8_t* __restrict__ codes, int64_t pitch, float* __restrict__ scale,
+                                                   int64_t rows, int64_t K) {
+  constexpr int kPer = 256 / TPR;
+  __shared__ uint32_t s_most[8];
+  const int part = threadIdx.x % TPR;
+  for (int64_t r0 = int64_t(blockIdx.x) * kPer; r0 < rows; r0 += int64_t(gridDim.x) * kPer) {
+    const int64_t row = r0 + threadIdx.x / TPR;
+    const bool there = row < rows;
+    const T* src = x + (there ? row / inner * x_outer + row % inner * x_inner : 0);
+    Eight<VEC, T> raw[NV];
+    uint32_t m = 0;
+    const int64_t len = there ? K : 0;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) raw[i].load(src, (int64_t(i) * TPR + part) * 8, len);
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      float f[8];
+      raw[i].floats(f);
+      m = max(m, most_bits(f));
+    }
+    for (int64_t k = int64_t(NV) * TPR * 8 + part * 8; k < len; k += TPR * 8) {
+      Eight<VEC, T> e;
+      float f[8];
+      e.load(src, k, len);
+      e.floats(f);
+      m = max(m, most_bits(f));
+    }
+    m = __reduce_max_sync(0xffffffffu, m);
+    if constexpr (TPR > 32) {
+      __syncthreads();                                     // the row before has been read out of s_most
+      if ((threadIdx.x & 31) == 0) s_most[threadIdx.x >> 5] = m;
+      __syncthreads();
+#pragma unroll
+      for (int w = 0; w < TPR / 32; ++w) m = max(m, s_most[threadIdx.x / TPR * (TPR / 32) + w]);
+    }
+    const bool fine = m < 0x7f800000u;
+    const float s = fine ? fmaxf(__fmul_rn(__uint_as_float(m), 1.0f / 127.0f), 1.17549435e-38f) : __uint_as_float(0x7fc00000u);
+    const float inv = fine ? __frcp_rn(s) : 0.0f, most = fine ? 127.0f : 0.0f;
+    if (!there) continue;
+    if (part == 0) scale[row] = s;
+    int8_t* dst = codes + row * pitch;
+    auto put = [&](const float* f, int64_t k) {
+      store_codes<VEC>(dst, k, pitch, make_uint2(codes4(f[0], f[1], f[2], f[3], inv, most),
+                                                 codes4(f[4], f[5], f[6], f[7], inv, most)));
+    };
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      float f[8];
+      raw[i].floats(f);
+      put(f, (int64_t(i) * TPR + part) * 8);
+    }
+    for (int64_t k = int64_t(NV) * TPR * 8 + part * 8; k < pitch; k += TPR * 8) {
+      Eight<VEC, T> e;
+      float f[8];
+      e.load(src, k, len);
+      e.floats(f);
+      put(f, k);
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------
+namespace {
+
+bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
+
+int grid_for(int64_t work, int per_sm) {
+  return int(std::max<int64_t>(1, std::min<int64_t>(work, int64_t(num_sms()) * per_sm)));
+}
+
+template <typename F>
+void by_type(int dtype, F&& f) {
+  if (dtype == kv::kBf16) f(static_cast<__nv_bfloat16*>(nullptr));
+  else if (dtype == kv::kF16) f(static_cast<__half*>(nullptr));
+  else f(static_cast<float*>(nullptr));
+}
+
+}  // namespace
+
+// x [rows, K] (unit stride over K, any stride over rows) -> codes [rows, K], scale bytes [blocks, rows]
+std::vector<at::Tensor> save8(at::Tensor x) {
+  PD_CHECK(x.is_cuda() && x.dim() == 2, "save8: a CUDA matrix is expected");
+  const int dtype = kv::dtype_of(x, "save8");
+  const c10::cuda::CUDAGuard guard(x.device());
+  const int64_t rows = x.size(0), K = x.size(1), blocks = (K + kBlock - 1) / kBlock;
+  at::Tensor codes = at::empty({rows, K}, x.options().dtype(at::kChar));
+  at::Tensor exps = at::empty({blocks, rows}, x.options().dtype(at::kByte));
+  if (rows == 0 || K == 0) return {codes, exps};
+  PD_CHECK(K == 1 || x.stride(1) == 1, "save8: unit stride over the last dim is expected");
+  const int64_t tiles = (rows + kRows - 1) / kRows * ((blocks + kBlocks - 1) / kBlocks);
+  const int grid = grid_for((tiles + 7) / 8, 8);
+  by_type(dtype, [&](auto* tag) {
+    using T = std::remove_pointer_t<decltype(tag)>;
+    const T* p = static_cast<const T*>(x.data_ptr());
+    const int64_t stride = rows == 1 ? K : x.stride(0);
+    const bool vec = K % 8 == 0 && aligned16(p) && stride * int64_t(sizeof(T)) % 16 == 0;
+    auto* kern = vec ? save_kernel<true, T> : save_kernel<false, T>;
+    kern<<<grid, 256, 0, stream()>>>(p, stride, codes.data_ptr<int8_t>(), exps.data_ptr<uint8_t>(), rows, K, blocks,
+                                     dtype == kv::kF16 ? kTopHalf : kTopWide);
+  });
+  PD_CHECK_LAUNCH();
+  return {codes, exps};
+}
+
+at::Tensor load8(at::Tensor codes, at::Tensor exps, int64_t dtype) {
+  PD_CHECK(codes.is_cuda() && codes.dim() == 2 && codes.scalar_type() == at::kChar && codes.is_contiguous(),
+           "load8: contiguous int8 codes [rows, K] are expected");
+  const int64_t rows = codes.size(0), K = codes.size(1), blocks = (K + kBlock - 1) / kBlock;
+  PD_CHECK(exps.is_cuda() && exps.device() == codes.device() && exps.scalar_type() == at::kByte && exps.is_contiguous() &&
+               exps.dim() == 2 && exps.size(0) == blocks && exps.size(1) == rows,
+           "load8: contiguous uint8 scale bytes [blocks, rows] are expected");
+  const c10::cuda::CUDAGuard guard(codes.device());
+  at::Tensor y = at::empty({rows, K}, codes.options().dtype(at::ScalarType(dtype)));
+  const int t = kv::dtype_of(y, "load8");
+  if (rows == 0 || K == 0) return y;
+  const int64_t tiles = (rows + kRows - 1) / kRows * ((blocks + kBlocks - 1) / kBlocks);
+  const int grid = grid_for((tiles + 7) / 8, 8);
+  by_type(t, [&](auto* tag) {
+    using T = std::remove_pointer_t<decltype(tag)>;
+    auto* kern = K % 8 == 0 ? load_kernel<true, T> : load_kernel<false, T>;
+    kern<<<grid, 256, 0, stream()>>>(codes.data_ptr<int8_t>(), exps.data_ptr<uint8_t>(), static_cast<T*>(y.data_ptr()),
+                                     rows, K, blocks);
+  });
+  PD_CHECK_LAUNCH();
+  return y;
+}
+
+// Rows of x [outer, inner, K] into codes (rows of `pitch` bytes) and scale [outer * inner].
+void quantize_into(const at::Tensor& x, int8_t* codes, int64_t pitch, float* scale) {
+  const int64_t outer = x.size(0), inner = x.size(1), K = x.size(2), rows = outer * inner;
+  if (rows == 0) return;
+  by_type(kv::dtype_of(x, "quantize_rows"), [&](auto* tag) {
+    using T = std::remove_pointer_t<decltype(tag)>;
+    const T* p = static_cast<const T*>(x.data_ptr());
+    const int64_t so = outer == 1 ? 0 : x.stride(0), si = inner == 1 ? 0 : x.stride(1);
+    const bool vec = K % 8 == 0 && pitch % 8 == 0 && aligned16(p) && so * int64_t(sizeof(T)) % 16 == 0 &&
+                     si * int64_t(sizeof(T)) % 16 == 0;
+    auto go = [&](auto* kern, int per_block) {
+      kern<<<grid_for((rows + per_block - 1) / per_block, 8), 256, 0, stream()>>>(p, so, si, inner, codes, pitch, scale,
+                                                                                rows, K);
+      PD_CHECK_LAUNCH();
+    };
+    // few rows: a block for each, so that a row's reads are spread over threads
+    if (!vec) {
+      if (rows >= 1184) go(rows_kernel<false, 32, 1, T>, 8);
+      else go(rows_kernel<false, 256, 1, T>, 1);
+    } else if (rows < 1184 && K > 256) {
+      if (K <= 2048) go(rows_kernel<true, 256, 1, T>, 1);
+      else go(rows_kernel<true, 256, 2, T>, 1);
+    } else if (K <= 256) {
+      go(rows_kernel<true, 32, 1, T>, 8);
+    } else if (K <= 512) {
+      go(rows_kernel<true, 32, 2, T>, 8);
+    } else if (K <= 1024) {
+      go(rows_kernel<true, 32, 4, T>, 8);
+    } else {
+      go(rows_kernel<true, 256, 2, T>, 1);
+    }
+  });
+}
+
+std::vector<at::Tensor> quantize_rows(at::Tensor x) {
+  PD_CHECK(x.is_cuda() && x.dim() == 3, "quantize_rows: a CUDA tensor [outer, inner, K] is expected");
+  kv::dtype_of(x, "quantize_rows");
+  PD_CHECK(x.size(2) <= 1 || x.stride(2) == 1, "quantize_rows: unit stride over the last dim is expected");
+  const c10::cuda::CUDAGuard guard(x.device());
+  at::Tensor codes = at::empty(x.sizes(), x.options().dtype(at::kChar));
+  at::Tensor scale = at::empty({x.size(0), x.size(1)}, x.options().dtype(at::kFloat));
+  quantize_into(x, codes.data_ptr<int8_t>(), x.size(2), scale.data_ptr<float>());
+  return {codes, scale};
+}
+
+}  // namespace i8
+
+long long launches() { return launch_counter().load(); }
+
+}  // namespace pd

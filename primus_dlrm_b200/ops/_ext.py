@@ -2,7 +2,8 @@
 
 ``core()`` returns the ``_C`` module (embedding, norm, loss, optimizer
 kernels), ``gemm()`` the ``_gemm`` module (tcgen05 GEMMs, attention) and
-``kv()`` the ``_kv`` module (rotary and key/value-cache kernels).
+``kv()`` the ``_kv`` module (rotary and key/value-cache kernels), ``int8()``
+the ``_int8`` module (8-bit integer kernels).
 On a machine with a CUDA device a missing or stale extension raises: a GPU
 run never silently falls back to eager PyTorch.  Without a CUDA device the
 eager implementations in ``primus_dlrm_b200.ops`` are the only path (they
@@ -25,7 +26,8 @@ def _load(name: str):
         mod = importlib.import_module(f"primus_dlrm_b200.{name}")
     except ImportError as e:  # pragma: no cover - exercised on GPU boxes only
         src = os.path.join(os.path.dirname(os.path.dirname(os.path.dirname(os.path.abspath(__file__)))),
-                           "csrc", {"_gemm": "gemm_bindings.cpp", "_kv": "kv_bindings.cpp"}.get(name, "bindings.cpp"))
+                           "csrc", {"_gemm": "gemm_bindings.cpp", "_kv": "kv_bindings.cpp",
+                                    "_int8": "int8_bindings.cpp"}.get(name, "bindings.cpp"))
         if torch.cuda.is_available() and os.path.exists(src):
             raise RuntimeError(
                 f"primus_dlrm_b200.{name} is not built; run `python setup.py build_ext --inplace` "
@@ -45,6 +47,10 @@ def gemm():
 
 def kv():
     return _load("_kv")
+
+
+def int8():
+    return _load("_int8")
 
 
 def native_enabled(device: torch.device | str | None = None) -> bool:

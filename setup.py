@@ -3,9 +3,9 @@
     python setup.py build_ext --inplace
 
 builds ``primus_dlrm_b200/_C*.so`` (core kernels),
-``primus_dlrm_b200/_gemm*.so`` (tcgen05 GEMM / attention kernels) and
-``primus_dlrm_b200/_kv*.so`` (rotary and key/value-cache kernels) next to
-the package, so the shared objects travel with the source tree.  Every CUDA
+``primus_dlrm_b200/_gemm*.so`` (tcgen05 GEMM / attention kernels),
+``primus_dlrm_b200/_kv*.so`` (rotary and key/value-cache kernels) and
+``primus_dlrm_b200/_int8*.so`` (8-bit integer kernels) next to the package, so the shared objects travel with the source tree.  Every CUDA
 source is compiled for ``sm_100a`` only.
 """
 from __future__ import annotations
@@ -30,7 +30,8 @@ CXX = ["-O3", "-std=c++17"]
 
 core_sources = ["csrc/bindings.cpp"] + sorted(
     s for s in glob.glob("csrc/*.cu") if not os.path.basename(s).startswith("gemm")
-    and not os.path.basename(s).startswith(("attn", "kv_")))
+    and not os.path.basename(s).startswith(("attn", "kv_", "int8_")))
+int8_sources = sorted(glob.glob("csrc/int8_*.cu")) + ["csrc/int8_bindings.cpp"]
 kv_sources = sorted(glob.glob("csrc/kv_*.cu")) + ["csrc/kv_bindings.cpp"]
 gemm_sources = sorted(glob.glob("csrc/gemm*.cu") + glob.glob("csrc/attn*.cu")) + ["csrc/gemm_bindings.cpp"]
 
@@ -46,6 +47,12 @@ ext_modules = [
         sources=kv_sources,
         include_dirs=[os.path.join(ROOT, "csrc")],
         extra_compile_args={"cxx": CXX, "nvcc": NVCC_COMMON},
+    ),
+    CUDAExtension(
+        name="primus_dlrm_b200._int8",
+        sources=int8_sources,
+        include_dirs=[os.path.join(ROOT, "csrc")],
+        extra_compile_args={"cxx": CXX, "nvcc": NVCC_COMMON + (["-Xptxas=-v"] if os.environ.get("PD_PTXAS_V") else [])},
     ),
 ]
 if os.path.exists(os.path.join(ROOT, "csrc", "gemm_bindings.cpp")):
