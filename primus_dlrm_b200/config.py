@@ -223,6 +223,9 @@ class TransformerConfig:
     # queries and keys normed per head and rotated by their positions
     rotary: bool = False
     rope_theta: float = 10000.0
+    # 8: a block's QKV and FFN inputs and its FFN pre-activations wait for the
+    # backward pass in 8 bits (less than half the block's saved activations)
+    activation_bits: int = 16
 
 
 @dataclass

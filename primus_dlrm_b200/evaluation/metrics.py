@@ -63,24 +63,41 @@ def _aggregate(per_user: list[dict[str, float]], ks: list[int]) -> dict[str, flo
     return res
 
 
+def serving_weights(model, weights: str | None):
+    """What :func:`score_candidates` takes for ``weights`` None or ``"int8"``: a OneTrans model's projection weights laid
+    out once as 8-bit integers."""
+    if weights is None:
+        return None
+    inner = getattr(model, "module", model)
+    if weights != "int8" or not hasattr(inner, "int8_weights"):
+        raise ValueError(f"weights {weights!r}: expected None, or 'int8' for a OneTrans model")
+    from primus_dlrm_b200.parallel.fsdp import full_params
+    with full_params(inner):
+        return inner.int8_weights()
+
+
 @torch.no_grad()
 def score_candidates(model, user_batch: dict[str, torch.Tensor], candidate_batch: dict[str, torch.Tensor],
-                     task: str, batch_size: int = 1024, kv_cache: str | None = None) -> torch.Tensor:
+                     task: str, batch_size: int = 1024, kv_cache: str | None = None, weights=None) -> torch.Tensor:
     """Scores [C] of one user's history against C candidates (device tensor).
 
     ``user_batch`` holds the user-side tensors with a leading dim of 1;
     ``candidate_batch`` holds per-candidate tensors with leading dim C.
     ``kv_cache="fp8"`` keeps a OneTrans model's keys and values of the history
-    in 8-bit pages.
+    in 8-bit pages; ``weights`` is what :func:`serving_weights` gives.
     """
     inner = getattr(model, "module", model)
     if hasattr(inner, "score_candidates"):
         from primus_dlrm_b200.parallel.fsdp import full_params
         with full_params(inner):          # FSDP units: the scorer reads block weights directly
-            extra = {} if kv_cache is None else {"kv_cache": kv_cache}      # not every scorer knows one
+            extra = {} if kv_cache is None else {"kv_cache": kv_cache}      # not every scorer knows them
+            if weights is not None:
+                extra["weights"] = weights
             return inner.score_candidates(user_batch, candidate_batch, task, batch_size, **extra)
     if kv_cache is not None:
         raise ValueError("kv_cache: this model keeps no keys and values")
+    if weights is not None:
+        raise ValueError("weights: this model scores with its own")
     C = next(iter(candidate_batch.values())).shape[0]
     out = []
     for s in range(0, C, batch_size):
@@ -95,10 +112,12 @@ def score_candidates(model, user_batch: dict[str, torch.Tensor], candidate_batch
 
 
 def evaluate_ranking(model, eval_dataset, device, candidate_item_ids=None, ks=None, task: str = "listen_plus",
-                     batch_size: int = 1024, log_interval: int = 0, kv_cache: str | None = None) -> dict[str, float]:
+                     batch_size: int = 1024, log_interval: int = 0, kv_cache: str | None = None,
+                     weights: str | None = None) -> dict[str, float]:
     """Global candidate list (default: top popular items) per test user."""
     ks = ks or [10, 100]
     model.eval()
+    extra = {} if weights is None else {"weights": serving_weights(model, weights)}
     if candidate_item_ids is None:
         candidate_item_ids = np.argsort(-eval_dataset.item_popularity)[:10000]
     cand = eval_dataset.candidate_batch(candidate_item_ids, device)
@@ -110,7 +129,7 @@ def evaluate_ranking(model, eval_dataset, device, candidate_item_ids=None, ks=No
             continue
         ub = eval_dataset.user_batch(sample, device)
         s = score_candidates(model, ub, eval_dataset.with_user_features(cand, sample, candidate_item_ids, device),
-                             task, batch_size, kv_cache)
+                             task, batch_size, kv_cache, **extra)
         order = torch.argsort(s, descending=True)[: max(ks)].cpu().numpy()
         per_user.append(metrics_from_ranking(np.asarray(candidate_item_ids)[order], gt, ks))
         if log_interval and (idx + 1) % log_interval == 0:
@@ -120,10 +139,11 @@ def evaluate_ranking(model, eval_dataset, device, candidate_item_ids=None, ks=No
 
 def evaluate_ranking_peruser(model, eval_dataset, device, ks=None, task: str = "listen_plus", top_n: int = 100,
                              batch_size: int = 1024, log_interval: int = 0,
-                             kv_cache: str | None = None) -> dict[str, float]:
+                             kv_cache: str | None = None, weights: str | None = None) -> dict[str, float]:
     """Per-user candidates = the user's unique train items; metrics on the top-N."""
     ks = ks or [10, 50, 100]
     model.eval()
+    extra = {} if weights is None else {"weights": serving_weights(model, weights)}
     per_user = []
     for idx in range(len(eval_dataset)):
         sample = eval_dataset[idx]
@@ -136,7 +156,7 @@ def evaluate_ranking_peruser(model, eval_dataset, device, ks=None, task: str = "
         cand = eval_dataset.candidate_batch(items, device)
         ub = eval_dataset.user_batch(sample, device)
         s = score_candidates(model, ub, eval_dataset.with_user_features(cand, sample, items, device), task,
-                             batch_size, kv_cache)
+                             batch_size, kv_cache, **extra)
         order = torch.argsort(s, descending=True)[:top_n].cpu().numpy()
         per_user.append(metrics_from_ranking(np.asarray(items)[order], gt, ks))
         if log_interval and (idx + 1) % log_interval == 0:

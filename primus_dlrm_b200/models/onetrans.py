@@ -36,6 +36,7 @@ from primus_dlrm_b200.ops.attention import (
     _native_ok as _fmha_native_ok, causal_attention_all_rows, pyramid_attention, pyramid_attention_qkv,
 )
 from primus_dlrm_b200.ops.embedding import SparseOptimizer
+from primus_dlrm_b200.ops.int8 import Int8Weight, int8_linear
 from primus_dlrm_b200.ops.kv_cache import PagedKVCache, paged_attention
 from primus_dlrm_b200.ops.norm import RMSNorm, add_norm, make_norm, norm_with_tail
 from primus_dlrm_b200.ops.rotary import qk_norm_rope, rope_table
@@ -57,7 +58,8 @@ def _xavier_per_token(w: torch.Tensor) -> None:
 
 class MixedAttention(nn.Module):
     def __init__(self, d_model: int, n_heads: int, n_ns_tokens: int, dropout: float = 0.0,
-                 attention_impl: str = "sdpa", rotary: bool = False, rope_theta: float = 10000.0):
+                 attention_impl: str = "sdpa", rotary: bool = False, rope_theta: float = 10000.0,
+                 save8: bool = False):
         super().__init__()
         if d_model % n_heads:
             raise ValueError("d_model must be divisible by n_heads")
@@ -76,7 +78,7 @@ class MixedAttention(nn.Module):
         nn.init.xavier_uniform_(self.s_qkv.weight)
         nn.init.xavier_uniform_(self.out_proj.weight)
         _xavier_per_token(self.ns_qkv_weight)
-        self.rotary, self.rope_theta = rotary, rope_theta
+        self.rotary, self.rope_theta, self.save8 = rotary, rope_theta, save8
         if rotary:
             self.q_norm, self.k_norm = RMSNorm(self.d_head), RMSNorm(self.d_head)
             self._rope: torch.Tensor | None = None
@@ -99,7 +101,7 @@ class MixedAttention(nn.Module):
         queries, [B, q_len, D].  On CUDA (no dropout, native impls) all T rows
         are computed and the result is a [B, q_len, D] view of [B, T, D]."""
         B, T, D = x.shape
-        qkv = dense.mixed_linear(x, n_s, self.s_qkv.weight, self.ns_qkv_weight)  # [B, T, 3D]
+        qkv = dense.mixed_linear(x, n_s, self.s_qkv.weight, self.ns_qkv_weight, save8=self.save8)  # [B, T, 3D]
         qkv = qkv.view(B, T, 3, self.n_heads, self.d_head)
         if self.rotary:
             q, k = self.norm_rope(qkv[:, T - q_len:, 0], qkv[:, :, 1], T)
@@ -128,9 +130,9 @@ class MixedAttention(nn.Module):
 
 
 class MixedFFN(nn.Module):
-    def __init__(self, d_model: int, ffn_dim: int, n_ns_tokens: int, dropout: float = 0.0):
+    def __init__(self, d_model: int, ffn_dim: int, n_ns_tokens: int, dropout: float = 0.0, save8: bool = False):
         super().__init__()
-        self.n_ns = n_ns_tokens
+        self.n_ns, self.save8 = n_ns_tokens, save8
         self.d_model = d_model
         self.s_w1 = nn.Linear(d_model, ffn_dim, bias=False)
         self.s_w2 = nn.Linear(ffn_dim, d_model, bias=False)
@@ -143,9 +145,9 @@ class MixedFFN(nn.Module):
         _xavier_per_token(self.ns_w2)
 
     def forward(self, x: torch.Tensor, n_s: int) -> torch.Tensor:
-        h = dense.mixed_linear(x, n_s, self.s_w1.weight, self.ns_w1, act="gelu")
+        h = dense.mixed_linear(x, n_s, self.s_w1.weight, self.ns_w1, act="gelu", save8=self.save8)
         h = self.dropout(h)
-        return dense.mixed_linear(h, n_s, self.s_w2.weight, self.ns_w2)
+        return dense.mixed_linear(h, n_s, self.s_w2.weight, self.ns_w2, save8=self.save8)
 
 
 class OneTransBlock(nn.Module):
@@ -153,12 +155,15 @@ class OneTransBlock(nn.Module):
 
     def __init__(self, d_model: int, n_heads: int, n_ns_tokens: int, ffn_mult: int = 4,
                  dropout: float = 0.0, attention_impl: str = "sdpa", norm: str = "rmsnorm", rotary: bool = False,
-                 rope_theta: float = 10000.0):
+                 rope_theta: float = 10000.0, activation_bits: int = 16):
         super().__init__()
+        if activation_bits not in (8, 16):
+            raise ValueError(f"activation_bits {activation_bits}: expected 16 or 8")
+        save8 = activation_bits == 8
         self.norm1 = make_norm(norm, d_model)
-        self.attn = MixedAttention(d_model, n_heads, n_ns_tokens, dropout, attention_impl, rotary, rope_theta)
+        self.attn = MixedAttention(d_model, n_heads, n_ns_tokens, dropout, attention_impl, rotary, rope_theta, save8)
         self.norm2 = make_norm(norm, d_model)
-        self.ffn = MixedFFN(d_model, d_model * ffn_mult, n_ns_tokens, dropout)
+        self.ffn = MixedFFN(d_model, d_model * ffn_mult, n_ns_tokens, dropout, save8)
 
     def forward(self, x: torch.Tensor, q_len: int, n_s_tokens: int) -> torch.Tensor:
         kv_len = x.shape[1]
@@ -168,7 +173,7 @@ class OneTransBlock(nn.Module):
         y, z = add_norm(a, x_tail, self.norm2.weight,
                         getattr(self.norm2, "bias", None), self.norm2.eps, self.norm2.kind)
         fused = dense.mixed_ffn(y, z, q_len - n_ns, self.ffn.s_w1.weight, self.ffn.s_w2.weight,
-                                self.ffn.ns_w1, self.ffn.ns_w2) if (self.ffn.dropout.p == 0 or not self.training) else None
+                                self.ffn.ns_w1, self.ffn.ns_w2, save8=self.ffn.save8) if (self.ffn.dropout.p == 0 or not self.training) else None
         if fused is not None:
             return fused
         f = self.ffn(y, n_s=q_len - n_ns)
@@ -277,7 +282,8 @@ class OneTransModel(BaseModel):
         self.ns_tokenizer = AutoSplitTokenizer(ns_raw, ot.d_model, ot.n_ns_tokens).to(device)
         self.blocks = nn.ModuleList([
             OneTransBlock(ot.d_model, ot.n_heads, ot.n_ns_tokens, ot.ffn_mult, ot.dropout,
-                          attention_impl=ot.attention_impl, norm=ot.norm, rotary=ot.rotary, rope_theta=ot.rope_theta)
+                          attention_impl=ot.attention_impl, norm=ot.norm, rotary=ot.rotary, rope_theta=ot.rope_theta,
+                          activation_bits=ot.activation_bits)
             for _ in range(ot.n_layers)
         ]).to(device)
         self.final_norm = make_norm(ot.norm, ot.d_model).to(device)
@@ -385,8 +391,18 @@ class OneTransModel(BaseModel):
 
     # ------------------------------------------------------------------
     @torch.no_grad()
+    def int8_weights(self) -> list[dict[str, Int8Weight]]:
+        """The blocks' projection weights as 8-bit integers, for :meth:`score_candidates`; later training steps do not
+        reach them."""
+        return [{"s_qkv": Int8Weight.from_float(b.attn.s_qkv.weight), "ns_qkv": Int8Weight.from_float(b.attn.ns_qkv_weight),
+                 "out": Int8Weight.from_float(b.attn.out_proj.weight), "s_w1": Int8Weight.from_float(b.ffn.s_w1.weight),
+                 "s_w2": Int8Weight.from_float(b.ffn.s_w2.weight), "ns_w1": Int8Weight.from_float(b.ffn.ns_w1),
+                 "ns_w2": Int8Weight.from_float(b.ffn.ns_w2)} for b in self.blocks]
+
+    @torch.no_grad()
     def score_candidates(self, user_batch: dict[str, torch.Tensor], candidate_batch: dict[str, torch.Tensor],
-                         task: str, batch_size: int = 1024, kv_cache: str | None = None) -> torch.Tensor:
+                         task: str, batch_size: int = 1024, kv_cache: str | None = None,
+                         weights: list[dict[str, Int8Weight]] | None = None) -> torch.Tensor:
         """Scores [C] of one user against C candidates with an S-side K/V cache.
 
         S tokens sit before the NS tokens and attention is causal, so the S
@@ -404,9 +420,15 @@ class OneTransModel(BaseModel):
         expanding the cache to each candidate.  The head dim is then 32, 64 or
         128, and scores carry the rounding of 8-bit keys and values; on a GPU the
         queries and outputs of a 32-bit model are rounded to bf16 there.
+
+        ``weights`` (:meth:`int8_weights`, laid out once for many users) runs the
+        blocks' projections as products of 8-bit integers (``ops.int8``); scores
+        carry the rounding of 8-bit weights and activations.
         """
         if kv_cache not in (None, "fp8"):
             raise ValueError(f"kv_cache {kv_cache!r}: expected None or 'fp8'")
+        if weights is not None and len(weights) != len(self.blocks):
+            raise ValueError(f"weights of {len(weights)} blocks for a model of {len(self.blocks)}")
         ot = self.config.model.transformer
         n_ns, H = ot.n_ns_tokens, ot.n_heads
         D = ot.d_model
@@ -425,7 +447,9 @@ class OneTransModel(BaseModel):
         for l, blk in enumerate(self.blocks):
             at = blk.attn
             h = blk.norm1(xs)
-            qkv = (h @ at.s_qkv.weight.t().to(h.dtype)).view(1, -1, 3, H, dh)
+            w8 = weights[l] if weights else None
+            qkv = int8_linear(h, w8["s_qkv"]) if w8 else h @ at.s_qkv.weight.t().to(h.dtype)
+            qkv = qkv.view(1, -1, 3, H, dh)
             q_s = sched[l]                                   # S queries kept by this layer
             k_s, v_s = qkv[:, :, 1], qkv[:, :, 2]            # [1, n_s, H, dh]
             n_s = xs.shape[1]
@@ -438,7 +462,13 @@ class OneTransModel(BaseModel):
                     q, k_s = at.norm_rope(q, k_s, n_s)
                 cache.append((k_s, v_s))
                 o = pyramid_attention(q, k_s, v_s, impl="mask").reshape(1, q_s, D)
-            z = at.out_proj(o) + xs[:, n_s - q_s:]
+            tail = xs[:, n_s - q_s:]
+            if w8:
+                z = int8_linear(o, w8["out"], residual=tail.to(o.dtype))
+                f = int8_linear(blk.norm2(z), w8["s_w1"], act="gelu")
+                xs = int8_linear(f, w8["s_w2"], residual=z.to(f.dtype))
+                continue
+            z = at.out_proj(o) + tail
             y = blk.norm2(z)
             xs = z + blk.ffn.s_w2(F.gelu(blk.ffn.s_w1(y)))
         # ---- candidate side: NS tokens only ----
@@ -455,7 +485,10 @@ class OneTransModel(BaseModel):
             for l, blk in enumerate(self.blocks):
                 at = blk.attn
                 h = blk.norm1(x)
-                qkv = torch.einsum("btk,tnk->btn", h, at.ns_qkv_weight.to(h.dtype)).view(nb, n_ns, 3, H, dh)
+                w8 = weights[l] if weights else None
+                qkv = (int8_linear(h, w8["ns_qkv"]) if w8
+                       else torch.einsum("btk,tnk->btn", h, at.ns_qkv_weight.to(h.dtype)))
+                qkv = qkv.view(nb, n_ns, 3, H, dh)
                 q, k_n, v_n = qkv[:, :, 0], qkv[:, :, 1], qkv[:, :, 2]
                 if kv_cache:
                     o = cache[l].candidates(q, k_n, v_n).reshape(nb, n_ns, D)
@@ -469,6 +502,11 @@ class OneTransModel(BaseModel):
                     k = torch.cat([k_s.expand(nb, -1, -1, -1).to(k_n.dtype), k_n], dim=1)
                     v = torch.cat([v_s.expand(nb, -1, -1, -1).to(v_n.dtype), v_n], dim=1)
                     o = pyramid_attention(q, k, v, impl="mask").reshape(nb, n_ns, D)
+                if w8:
+                    z = int8_linear(o, w8["out"], residual=x.to(o.dtype))
+                    f = int8_linear(blk.norm2(z), w8["ns_w1"], act="gelu")
+                    x = int8_linear(f, w8["ns_w2"], residual=z.to(f.dtype))
+                    continue
                 z = at.out_proj(o) + x
                 y = blk.norm2(z)
                 f = torch.einsum("btk,tnk->btn", y, blk.ffn.ns_w1.to(y.dtype))
