@@ -15,6 +15,7 @@ void tc_gemm(at::Tensor, at::Tensor, at::Tensor, int64_t, c10::optional<at::Tens
              at::Tensor, bool, c10::optional<at::Tensor>);
 void tc_gemm_saved8(at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor, c10::optional<at::Tensor>, at::Tensor, bool);
 void tc_wgrad(at::Tensor, at::Tensor, at::Tensor, at::Tensor, bool);
+at::Tensor tc_wgrad_as(at::Tensor, at::Tensor, at::Tensor, bool, int64_t);
 at::Tensor tc_mma_rate(int64_t, int64_t, int64_t, int64_t, int64_t, int64_t, at::Tensor);
 at::Tensor tc_mma_burst(int64_t, int64_t, int64_t, int64_t, int64_t, int64_t, int64_t, int64_t, at::Tensor);
 }  // namespace pd
@@ -41,6 +42,9 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("tc_wgrad", &pd::tc_wgrad, py::arg("A"), py::arg("B"), py::arg("C"), py::arg("err"), py::arg("l_sum") = false,
         "C[l] (fp32, zeroed) += A[l]^T B[l] over rows on tcgen05, split over rows (A [L,K,M], B [L,K,N] bf16 views); "
         "l_sum: one C summed over the batches too");
+  m.def("tc_wgrad_as", [](at::Tensor A, at::Tensor B, at::Tensor err, bool l_sum, at::ScalarType t) {
+          return pd::tc_wgrad_as(A, B, err, l_sum, int64_t(t)); },
+        "the weight gradient of tc_wgrad as a new tensor of a type (l_sum: [M, N])");
   m.def("tc_mma_rate", &pd::tc_mma_rate, py::arg("mode"), py::arg("n"), py::arg("iters"), py::arg("nacc"),
         py::arg("swz"), py::arg("issue"), py::arg("err"),
         "tcgen05.mma probe: int64 [SMs, 2] (issue cycles, issue + execution cycles) for `iters` M=128 x n x 16 "

@@ -591,7 +591,7 @@ struct WgParams {
   int m_blocks, n_blocks, k_blocks, tiles, splits, kb_per_split, items;
   int l_sum;        // 1: the L batches are part of the reduction (one output); k-blocks run over (l, k)
   int kb_per_l;     // k-blocks of one batch when l_sum
-  float* C; int64_t c_ls, c_ms;
+  void* C; int64_t c_ls, c_ms;
   int a_mode, b_mode;
   int* err;
 };
@@ -612,7 +612,15 @@ __device__ __forceinline__ void red_add_v4(float* addr, float a, float b, float 
                : "memory");
 }
 
-template <int BN, int STAGES>
+// 32 bytes of one row in one store (a whole sector).
+__device__ __forceinline__ void store_sector(void* dst, const uint32_t* w) {
+  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};"
+               ::"l"(dst), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7]) : "memory");
+}
+
+// Out = void: partial tiles are added into fp32 C. Out = float or __nv_bfloat16 (one split): a tile is the whole sum, so
+// it is stored in the gradient's type at once, with no zeroing, no reductions in memory and no conversion afterwards.
+template <int BN, int STAGES, typename Out = void>
 __global__ void __launch_bounds__(kThreads, 1) wgrad_kernel(const __grid_constant__ CUtensorMap tmA,
                                                             const __grid_constant__ CUtensorMap tmB,
                                                             const WgParams p) {
@@ -738,8 +746,27 @@ __global__ void __launch_bounds__(kThreads, 1) wgrad_kernel(const __grid_constan
         uint32_t r[32];
         tc_ld32_issue(tbase + c, r);
         tc_ld_wait(r);
-        if (row < p.M && kb1 > kb0) {
-          float* dst = p.C + l * p.c_ls + int64_t(row) * p.c_ms + nb * BN + c;
+        if constexpr (!std::is_void_v<Out>) {
+          if (row < p.M) {
+            Out* dst = static_cast<Out*>(p.C) + l * p.c_ls + int64_t(row) * p.c_ms + nb * BN + c;
+            if constexpr (sizeof(Out) == 4) {
+#pragma unroll
+              for (int j = 0; j < 32; j += 8) store_sector(dst + j, r + j);
+            } else {
+#pragma unroll
+              for (int j = 0; j < 32; j += 16) {
+                uint32_t w[8];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                  const __nv_bfloat162 h = __floats2bfloat162_rn(__uint_as_float(r[j + 2 * e]), __uint_as_float(r[j + 2 * e + 1]));
+                  w[e] = *reinterpret_cast<const uint32_t*>(&h);
+                }
+                store_sector(dst + j, w);
+              }
+            }
+          }
+        } else if (row < p.M && kb1 > kb0) {
+          float* dst = static_cast<float*>(p.C) + l * p.c_ls + int64_t(row) * p.c_ms + nb * BN + c;
 #pragma unroll
           for (int j = 0; j < 32; j += 4)
             red_add_v4(dst + j, __uint_as_float(r[j]), __uint_as_float(r[j + 1]), __uint_as_float(r[j + 2]),
@@ -1023,6 +1050,55 @@ void tc_gemm_saved8(at::Tensor A, at::Tensor B, at::Tensor C, at::Tensor codes, 
   }
 }
 
+namespace {
+
+// Blocks, tiles and splits of a weight gradient [M, N] over L batches of K rows.
+tc::WgParams wgrad_plan(int64_t L, int64_t K, int64_t M, int64_t N, bool l_sum) {
+  tc::WgParams p{};
+  p.M = int(M); p.N = int(N); p.K = int(K); p.L = int(L);
+  p.m_blocks = int((M + tc::BM - 1) / tc::BM);
+  const int BN = (N % 256 == 0) ? 256 : (N % 128 == 0 ? 128 : 64);
+  p.n_blocks = int(N / BN);
+  p.l_sum = l_sum ? 1 : 0;
+  p.kb_per_l = int((K + tc::BK - 1) / tc::BK);
+  p.k_blocks = l_sum ? int(L) * p.kb_per_l : p.kb_per_l;
+  p.tiles = int(l_sum ? 1 : L) * p.m_blocks * p.n_blocks;
+  // about two items per SM without a ragged last wave, each at least 8 k-blocks long
+  int splits = std::max(1, (2 * num_sms()) / p.tiles);
+  splits = std::min(splits, std::max(1, p.k_blocks / 8));
+  p.kb_per_split = (p.k_blocks + splits - 1) / splits;
+  p.splits = (p.k_blocks + p.kb_per_split - 1) / p.kb_per_split;
+  p.items = p.tiles * p.splits;
+  return p;
+}
+
+// direct: C in its own type, stored by the one split.
+void run_wgrad(const at::Tensor& A, const at::Tensor& B, const at::Tensor& C, tc::WgParams p, const at::Tensor& err, bool direct) {
+  p.C = C.data_ptr(); p.c_ls = C.stride(0); p.c_ms = C.stride(1);
+  p.err = err.data_ptr<int>();
+  // MN-major operands: [64 k-rows][64 cols] boxes over dims {cols, rows, L}
+  const CUtensorMap ta = make_map(A.data_ptr(), p.M, p.K, p.L, A.stride(1), A.stride(0), tc::BK, p.a_mode);
+  const CUtensorMap tb = make_map(B.data_ptr(), p.N, p.K, p.L, B.stride(1), B.stride(0), tc::BK, p.b_mode);
+  auto go = [&](auto kern, int bn, int stages) {
+    const size_t smem = size_t(stages) * (tc::BM * tc::BK * 2 + bn * tc::BK * 2) + 1024 + 1024;
+    PD_CHECK_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem)));
+    const int grid = p.items < num_sms() ? p.items : num_sms();
+    kern<<<grid, tc::kThreads, smem, stream()>>>(ta, tb, p);
+  };
+  auto by_width = [&](auto* tag) {
+    using Out = std::remove_pointer_t<decltype(tag)>;
+    if (p.N % 256 == 0) go(tc::wgrad_kernel<256, 4, Out>, 256, 4);
+    else if (p.N % 128 == 0) go(tc::wgrad_kernel<128, 6, Out>, 128, 6);
+    else go(tc::wgrad_kernel<64, 8, Out>, 64, 8);
+  };
+  if (!direct) by_width(static_cast<void*>(nullptr));
+  else if (C.scalar_type() == at::kFloat) by_width(static_cast<float*>(nullptr));
+  else by_width(static_cast<__nv_bfloat16*>(nullptr));
+  PD_CHECK_LAUNCH();
+}
+
+}  // namespace
+
 // C[l] (fp32 [M, N], zeroed by the caller) += A[l]^T B[l] over the rows:
 // A [L, K, M], B [L, K, N] bf16 views with unit stride on the last dim.
 // With l_sum, C is [1, M, N] and the sum runs over the batches as well.
@@ -1038,36 +1114,33 @@ void tc_wgrad(at::Tensor A, at::Tensor B, at::Tensor C, at::Tensor err, bool l_s
                   reinterpret_cast<uintptr_t>(C.data_ptr()) % 16 == 0,
               "wgrad: C must be an fp32 [L, M, N] view with 16-byte aligned rows");
   if (K == 0 || L == 0) return;
-  tc::WgParams p{};
-  p.M = int(M); p.N = int(N); p.K = int(K); p.L = int(L);
-  p.m_blocks = int((M + tc::BM - 1) / tc::BM);
-  const int BN = (N % 256 == 0) ? 256 : (N % 128 == 0 ? 128 : 64);
-  p.n_blocks = int(N / BN);
-  p.l_sum = l_sum ? 1 : 0;
-  p.kb_per_l = int((K + tc::BK - 1) / tc::BK);
-  p.k_blocks = l_sum ? int(L) * p.kb_per_l : p.kb_per_l;
-  p.tiles = int(LC) * p.m_blocks * p.n_blocks;
-  // about two items per SM without a ragged last wave, each at least 8 k-blocks long
-  int splits = std::max(1, (2 * num_sms()) / p.tiles);
-  splits = std::min(splits, std::max(1, p.k_blocks / 8));
-  p.kb_per_split = (p.k_blocks + splits - 1) / splits;
-  p.splits = (p.k_blocks + p.kb_per_split - 1) / p.kb_per_split;
-  p.items = p.tiles * p.splits;
-  p.C = C.data_ptr<float>(); p.c_ls = C.stride(0); p.c_ms = C.stride(1);
-  p.err = err.data_ptr<int>();
-  // MN-major operands: [64 k-rows][64 cols] boxes over dims {cols, rows, L}
-  const CUtensorMap ta = make_map(A.data_ptr(), M, K, L, A.stride(1), A.stride(0), tc::BK, p.a_mode);
-  const CUtensorMap tb = make_map(B.data_ptr(), N, K, L, B.stride(1), B.stride(0), tc::BK, p.b_mode);
-  auto go = [&](auto kern, int bn, int stages) {
-    const size_t smem = size_t(stages) * (tc::BM * tc::BK * 2 + bn * tc::BK * 2) + 1024 + 1024;
-    PD_CHECK_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem)));
-    const int grid = p.items < num_sms() ? p.items : num_sms();
-    kern<<<grid, tc::kThreads, smem, stream()>>>(ta, tb, p);
-  };
-  if (BN == 256) go(tc::wgrad_kernel<256, 4>, 256, 4);
-  else if (BN == 128) go(tc::wgrad_kernel<128, 6>, 128, 6);
-  else go(tc::wgrad_kernel<64, 8>, 64, 8);
-  PD_CHECK_LAUNCH();
+  run_wgrad(A, B, C, wgrad_plan(L, K, M, N, l_sum), err, false);
+}
+
+// The weight gradient of tc_wgrad as a new tensor [L, M, N] (l_sum: [M, N]) of a type (fp32 or bf16). Where one split covers
+// the rows a tile leaves in that type at once; else it is added up in fp32 and converted.
+at::Tensor tc_wgrad_as(at::Tensor A, at::Tensor B, at::Tensor err, bool l_sum, int64_t dtype) {
+  check_operand(A, "A");
+  check_operand(B, "B");
+  const int64_t L = A.size(0), K = A.size(1), M = A.size(2), N = B.size(2);
+  const auto type = at::ScalarType(dtype);
+  PD_CHECK(B.size(0) == L && B.size(1) == K, "B must be [L, K, N] over the same rows as A");
+  PD_CHECK(M % 64 == 0 && N % 64 == 0, "wgrad: M and N must be multiples of 64");
+  PD_CHECK(B.device() == A.device() && err.device() == A.device(), "wgrad: operands lie on two devices");
+  const c10::cuda::CUDAGuard guard(A.device());
+  const int64_t LC = l_sum ? 1 : L;
+  const auto fp32 = A.options().dtype(at::kFloat);
+  at::Tensor C;
+  if (K == 0 || L == 0) {
+    C = at::zeros({LC, M, N}, A.options().dtype(type));
+  } else {
+    const tc::WgParams p = wgrad_plan(L, K, M, N, l_sum);
+    const bool direct = p.splits == 1 && (type == at::kFloat || type == at::kBFloat16);
+    C = direct ? at::empty({LC, M, N}, A.options().dtype(type)) : at::zeros({LC, M, N}, fp32);
+    run_wgrad(A, B, C, p, err, direct);
+    C = C.to(type);
+  }
+  return l_sum ? C.squeeze(0) : C;
 }
 
 }  // namespace pd

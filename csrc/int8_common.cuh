@@ -57,5 +57,26 @@ __device__ __forceinline__ void ints4(uint32_t codes, float* f) {
     f[i] = __fsub_rn(__uint_as_float(__byte_perm(u, 0x4b000000u, 0x7540 + i)), 8388736.0f);
 }
 
+// Whole rows with a 32-bit scale: max(amax / 127, 2^-126) and its reciprocal; a row without numbers has codes of 0 and a
+// scale of NaN.
+struct RowScale { float scale, inv, most; };
+__device__ __forceinline__ RowScale row_scale(uint32_t amax_bits) {
+  const bool fine = amax_bits < 0x7f800000u;
+  RowScale r;
+  r.scale = fine ? fmaxf(__fmul_rn(__uint_as_float(amax_bits), 1.0f / 127.0f), 1.17549435e-38f) : __uint_as_float(0x7fc00000u);
+  r.inv = fine ? __frcp_rn(r.scale) : 0.0f;
+  r.most = fine ? 127.0f : 0.0f;
+  return r;
+}
+
+enum Act : int { kIdentity = 0, kGelu = 1, kRelu = 2 };
+
+// GELU of what lies below -1e30 is 0, of a sum that overflowed to -infinity too (-infinity * 0 would be NaN); NaN stays.
+__device__ __forceinline__ float from_below(float v) {
+  float r;
+  asm("max.NaN.f32 %0, %1, 0fF149F2CA;" : "=f"(r) : "f"(v));          // -1e30
+  return r;
+}
+
 }  // namespace i8
 }  // namespace pd

@@ -1,4 +1,5 @@
 // Host side of the 8-bit integer products (int8_gemm.cuh).
+#include "int8_few.cuh"
 #include "int8_gemm.cuh"
 
 #include <c10/cuda/CUDAGuard.h>
@@ -43,6 +44,7 @@ at::Tensor linear(at::Tensor x, at::Tensor codes, at::Tensor scale, int64_t K, b
                scale.scalar_type() == at::kFloat && scale.is_contiguous() && scale.size(0) == codes.size(0) &&
                scale.size(1) == codes.size(1) && (grouped || codes.size(0) == 1) && act >= kIdentity && act <= kRelu,
            "int8_linear: a weight laid out by Int8Weight is expected");
+  PD_CHECK(reinterpret_cast<uintptr_t>(codes.data_ptr()) % 16 == 0, "int8_linear: a weight's codes must lie on 16 bytes");
   PD_CHECK(codes.device() == x.device() && scale.device() == x.device(), "int8_linear: x and the weight lie on two devices");
   const int64_t L = codes.size(0), N = codes.size(1), Kp = codes.size(2);
   PD_CHECK(Kp % 16 == 0 && K <= Kp && K >= 1 && N >= 1 && N < (int64_t(1) << 31) && K <= 131072,
@@ -73,11 +75,28 @@ at::Tensor linear(at::Tensor x, at::Tensor codes, at::Tensor scale, int64_t K, b
   }
   if (M == 0) return y;
 
+  const int64_t size = y.element_size();
+  const int64_t r_ls = residual && L > 1 ? residual->stride(1) : 0, r_ms = residual && M > 1 ? residual->stride(0) : 0;
+  if (M <= kFewRows && few_bytes(M, Kp) <= kFewBytes && L <= 65535) {
+    FewParams f{};
+    f.M = int(M); f.N = int(N); f.L = int(L); f.K = int(K); f.Kp = int(Kp);
+    f.x = x.data_ptr();
+    f.x_outer = M > 1 ? x.stride(0) : 0; f.x_inner = L > 1 ? x.stride(1) : 0;
+    f.W = codes.data_ptr<int8_t>();
+    f.t = scale.data_ptr<float>();
+    f.bias = p.bias;
+    f.R_ = residual ? residual->data_ptr() : nullptr; f.r_ls = r_ls; f.r_ms = r_ms;
+    f.C = y.data_ptr(); f.c_ls = N; f.c_ms = N * L;
+    f.act = int(act);
+    few(f, dtype, K % 8 == 0 && reinterpret_cast<uintptr_t>(f.x) % 16 == 0 && f.x_outer * size % 16 == 0 &&
+                      f.x_inner * size % 16 == 0);
+    return y;
+  }
+
   at::Tensor a = at::empty({M * L, Kp}, codes.options());
   at::Tensor s = at::empty({M * L}, scale.options());
   quantize_into(x, a.data_ptr<int8_t>(), Kp, s.data_ptr<float>());
 
-  const int64_t size = y.element_size();
   p.M = int(M); p.N = int(N); p.L = int(L);
   p.m_blocks = int((M + BM - 1) / BM);
   p.k_blocks = int((K + BK - 1) / BK);
@@ -86,8 +105,7 @@ at::Tensor linear(at::Tensor x, at::Tensor codes, at::Tensor scale, int64_t K, b
   p.C = y.data_ptr(); p.c_ls = N; p.c_ms = N * L;
   if (residual) {
     p.R = residual->data_ptr();
-    p.r_ls = L == 1 ? 0 : residual->stride(1);
-    p.r_ms = M == 1 ? 0 : residual->stride(0);
+    p.r_ls = r_ls; p.r_ms = r_ms;
     p.r_vec = reinterpret_cast<uintptr_t>(p.R) % 16 == 0 && p.r_ls * size % 16 == 0 && p.r_ms * size % 16 == 0;
   }
   p.act = int(act);

@@ -36,8 +36,6 @@ constexpr int kEpiWarps = 12;
 constexpr int kParts = kEpiWarps / 4;   // warps that share 32 rows, by 32-column chunks
 constexpr int kThreads = 64 + 32 * kEpiWarps;
 
-enum Act : int { kIdentity = 0, kGelu = 1, kRelu = 2 };
-
 struct Params {
   int M, N, L;
   int m_blocks, n_blocks, k_blocks, tiles;
@@ -68,13 +66,6 @@ __device__ __forceinline__ uint4 pack16(const float* v) {
 #pragma unroll
   for (int i = 0; i < 16 / int(sizeof(T)); ++i) e[i] = kv::from_f<T>(v[i]);
   return u;
-}
-
-// GELU of what lies below -1e30 is 0, of a sum that overflowed to -infinity too (-infinity * 0 would be NaN); NaN stays.
-__device__ __forceinline__ float from_below(float v) {
-  float r;
-  asm("max.NaN.f32 %0, %1, 0fF149F2CA;" : "=f"(r) : "f"(v));          // -1e30
-  return r;
 }
 
 __device__ __forceinline__ void mma_i8(uint32_t d, uint64_t da, uint64_t db, uint32_t idesc, uint32_t acc) {

@@ -54,83 +54,126 @@ __device__ __forceinline__ uint32_t most_bits(const float* f) {
   return m;
 }
 
-// save8. A warp takes 8 rows x 4 blocks at a time: four lanes hold a block, so
-// its maximum takes two shuffles, a row's 64 to 128 bytes of each load are
-// whole sectors and four loads of a lane are on their way. Scale bytes lie
-// block-major ([blocks, rows]): that is how the GEMM epilogues, whose threads
-// own rows, write and read them in whole sectors.
-constexpr int kRows = 8, kBlocks = 4;
-template <bool VEC, typename T>
+// save8 and load8. Scale bytes lie block-major ([blocks, rows]): that is how the
+// GEMM epilogues, whose threads own rows, write and read them in whole sectors.
+// Rows on 16 bytes (VEC): a warp takes 8 rows x 4 blocks at a time; four lanes
+// hold a block, so its maximum takes two shuffles, a row's 64 to 128 bytes of a
+// load are whole sectors and four loads of a lane are on their way.
+// Other rows: a lane is an element, so loads and stores of any alignment are
+// whole runs of 32 and the maximum is one warp reduction; 8 blocks on their way.
+// Blocks of the grid go over row groups (x) and groups of blocks (y).
+constexpr int kRows = 8, kBlocks = 4, kLong = 8;
+
+template <typename T>
 __global__ void __launch_bounds__(256) save_kernel(const T* __restrict__ x, int64_t x_stride, int8_t* __restrict__ codes,
-                                                   uint8_t* __restrict__ exps, int64_t rows, int64_t K, int64_t blocks,
+                                                   uint8_t* __restrict__ exps, int64_t rows, int K, int blocks,
                                                    uint32_t top) {
   const int lane = threadIdx.x & 31, q = lane & 3;
-  const int64_t across = (blocks + kBlocks - 1) / kBlocks;
-  const int64_t tiles = (rows + kRows - 1) / kRows * across;
-  for (int64_t t = int64_t(blockIdx.x) * 8 + (threadIdx.x >> 5); t < tiles; t += int64_t(gridDim.x) * 8) {
-    const int64_t row = t / across * kRows + (lane >> 2), b0 = t % across * kBlocks;
+  for (int64_t r0 = (int64_t(blockIdx.x) * 8 + (threadIdx.x >> 5)) * kRows; r0 < rows; r0 += int64_t(gridDim.x) * 8 * kRows) {
+    const int64_t row = r0 + (lane >> 2);
     const bool there = row < rows;
     const T* src = x + (there ? row : 0) * x_stride;
-    Eight<VEC, T> raw[kBlocks];
+    for (int b0 = blockIdx.y * kBlocks; b0 < blocks; b0 += gridDim.y * kBlocks) {
+      Eight<true, T> raw[kBlocks];
 #pragma unroll
-    for (int j = 0; j < kBlocks; ++j) raw[j].load(src, (b0 + j) * kBlock + q * 8, there ? K : 0);
-    uint32_t mine = 0;
+      for (int j = 0; j < kBlocks; ++j) raw[j].load(src, (b0 + j) * kBlock + q * 8, there ? K : 0);
+      uint32_t mine = 0;
 #pragma unroll
-    for (int j = 0; j < kBlocks; ++j) {
-      float f[8];
-      raw[j].floats(f);
-      uint32_t m = most_bits(f);
-      m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
-      m = max(m, __shfl_xor_sync(0xffffffffu, m, 2));
-      const uint32_t b = scale_byte(m);
-      if (q == j) mine = b;
-      const float inv = inv_scale(b), most = most_code(b, top);
-      const uint2 c = make_uint2(codes4(f[0], f[1], f[2], f[3], inv, most), codes4(f[4], f[5], f[6], f[7], inv, most));
-      if (there) store_codes<VEC>(codes + row * K, (b0 + j) * kBlock + q * 8, K, c);
+      for (int j = 0; j < kBlocks; ++j) {
+        const int k = (b0 + j) * kBlock + q * 8;
+        float f[8];
+        raw[j].floats(f);
+        uint32_t m = most_bits(f);
+        m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
+        m = max(m, __shfl_xor_sync(0xffffffffu, m, 2));
+        const uint32_t b = scale_byte(m);
+        if (q == j) mine = b;
+        const float inv = inv_scale(b), most = most_code(b, top);
+        const uint2 c = make_uint2(codes4(f[0], f[1], f[2], f[3], inv, most), codes4(f[4], f[5], f[6], f[7], inv, most));
+        if (there && k < K) *reinterpret_cast<uint2*>(codes + row * K + k) = c;
+      }
+      if (there && b0 + q < blocks) exps[(b0 + q) * rows + row] = uint8_t(mine);
     }
-    if (there && b0 + q < blocks) exps[(b0 + q) * rows + row] = uint8_t(mine);
   }
 }
 
-template <bool VEC, typename T>
+template <typename T>
+__global__ void __launch_bounds__(256) save_any_kernel(const T* __restrict__ x, int64_t x_stride, int8_t* __restrict__ codes,
+                                                       uint8_t* __restrict__ exps, int64_t rows, int K, int blocks,
+                                                       uint32_t top) {
+  const int lane = threadIdx.x & 31;
+  for (int64_t row = int64_t(blockIdx.x) * 8 + (threadIdx.x >> 5); row < rows; row += int64_t(gridDim.x) * 8) {
+    const T* src = x + row * x_stride;
+    for (int b0 = blockIdx.y * kLong; b0 < blocks; b0 += gridDim.y * kLong) {
+      float f[kLong];
+#pragma unroll
+      for (int j = 0; j < kLong; ++j) {
+        const int k = (b0 + j) * kBlock + lane;
+        f[j] = k < K ? kv::to_f(src[k]) : 0.0f;
+      }
+      uint32_t mine = 0;
+#pragma unroll
+      for (int j = 0; j < kLong; ++j) {
+        const int k = (b0 + j) * kBlock + lane;
+        const uint32_t b = scale_byte(__reduce_max_sync(0xffffffffu, abs_bits(f[j])));
+        if (lane == j) mine = b;
+        const uint32_t c = codes4(f[j], 0.0f, 0.0f, 0.0f, inv_scale(b), most_code(b, top));
+        if (k < K) codes[row * K + k] = int8_t(c);
+      }
+      if (lane < kLong && b0 + lane < blocks) exps[(b0 + lane) * rows + row] = uint8_t(mine);
+    }
+  }
+}
+
+template <typename T>
 __global__ void __launch_bounds__(256) load_kernel(const int8_t* __restrict__ codes, const uint8_t* __restrict__ exps,
-                                                   T* __restrict__ y, int64_t rows, int64_t K, int64_t blocks) {
+                                                   T* __restrict__ y, int64_t rows, int K, int blocks) {
   const int lane = threadIdx.x & 31, q = lane & 3;
-  const int64_t across = (blocks + kBlocks - 1) / kBlocks;
-  const int64_t tiles = (rows + kRows - 1) / kRows * across;
-  for (int64_t t = int64_t(blockIdx.x) * 8 + (threadIdx.x >> 5); t < tiles; t += int64_t(gridDim.x) * 8) {
-    const int64_t row = t / across * kRows + (lane >> 2), b0 = t % across * kBlocks;
+  for (int64_t r0 = (int64_t(blockIdx.x) * 8 + (threadIdx.x >> 5)) * kRows; r0 < rows; r0 += int64_t(gridDim.x) * 8 * kRows) {
+    const int64_t row = r0 + (lane >> 2);
     if (row >= rows) continue;
-    uint2 c[kBlocks];
-    uint32_t e[kBlocks];
+    for (int b0 = blockIdx.y * kBlocks; b0 < blocks; b0 += gridDim.y * kBlocks) {
+      uint2 c[kBlocks];
+      uint32_t e[kBlocks];
 #pragma unroll
-    for (int j = 0; j < kBlocks; ++j) {
-      const int64_t k = (b0 + j) * kBlock + q * 8;
-      c[j] = make_uint2(0, 0);
-      e[j] = b0 + j < blocks ? exps[(b0 + j) * rows + row] : 1;
-      if constexpr (VEC) {
-        if (k < K) c[j] = *reinterpret_cast<const uint2*>(codes + row * K + k);
-      } else {
+      for (int j = 0; j < kBlocks; ++j) {
+        const int k = (b0 + j) * kBlock + q * 8;
+        c[j] = k < K ? *reinterpret_cast<const uint2*>(codes + row * K + k) : make_uint2(0, 0);
+        e[j] = b0 + j < blocks ? exps[(b0 + j) * rows + row] : 1;
+      }
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
-          if (k + i < K) (i < 4 ? c[j].x : c[j].y) |= uint32_t(uint8_t(codes[row * K + k + i])) << (8 * (i & 3));
+      for (int j = 0; j < kBlocks; ++j) {
+        const int k = (b0 + j) * kBlock + q * 8;
+        float f[8];
+        ints4(c[j].x, f);
+        ints4(c[j].y, f + 4);
+        const float s = scale_of(e[j]);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) f[i] *= s;
+        if (k < K) kv::store_v<8, T>(y + row * K + k, f);
       }
     }
+  }
+}
+
+template <typename T>
+__global__ void __launch_bounds__(256) load_any_kernel(const int8_t* __restrict__ codes, const uint8_t* __restrict__ exps,
+                                                       T* __restrict__ y, int64_t rows, int K, int blocks) {
+  const int lane = threadIdx.x & 31;
+  for (int64_t row = int64_t(blockIdx.x) * 8 + (threadIdx.x >> 5); row < rows; row += int64_t(gridDim.x) * 8) {
+    for (int b0 = blockIdx.y * kLong; b0 < blocks; b0 += gridDim.y * kLong) {
+      int c[kLong];
+      uint32_t e[kLong];
 #pragma unroll
-    for (int j = 0; j < kBlocks; ++j) {
-      const int64_t k = (b0 + j) * kBlock + q * 8;
-      float f[8];
-      ints4(c[j].x, f);
-      ints4(c[j].y, f + 4);
-      const float s = scale_of(e[j]);
+      for (int j = 0; j < kLong; ++j) {
+        const int k = (b0 + j) * kBlock + lane;
+        c[j] = k < K ? codes[row * K + k] : 0;
+        e[j] = b0 + j < blocks ? exps[(b0 + j) * rows + row] : 1;
+      }
 #pragma unroll
-      for (int i = 0; i < 8; ++i) f[i] *= s;
-      if constexpr (VEC) {
-        if (k < K) kv::store_v<8, T>(y + row * K + k, f);
-      } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-          if (k + i < K) y[row * K + k + i] = kv::from_f<T>(f[i]);
+      for (int j = 0; j < kLong; ++j) {
+        const int k = (b0 + j) * kBlock + lane;
+        if (k < K) y[row * K + k] = kv::from_f<T>(float(c[j]) * scale_of(e[j]));
       }
     }
   }
@@ -176,15 +219,13 @@ __global__ void __launch_bounds__(256) rows_kernel(const T* __restrict__ x, int6
 #pragma unroll
       for (int w = 0; w < TPR / 32; ++w) m = max(m, s_most[threadIdx.x / TPR * (TPR / 32) + w]);
     }
-    const bool fine = m < 0x7f800000u;
-    const float s = fine ? fmaxf(__fmul_rn(__uint_as_float(m), 1.0f / 127.0f), 1.17549435e-38f) : __uint_as_float(0x7fc00000u);
-    const float inv = fine ? __frcp_rn(s) : 0.0f, most = fine ? 127.0f : 0.0f;
+    const RowScale sc = row_scale(m);
     if (!there) continue;
-    if (part == 0) scale[row] = s;
+    if (part == 0) scale[row] = sc.scale;
     int8_t* dst = codes + row * pitch;
     auto put = [&](const float* f, int64_t k) {
-      store_codes<VEC>(dst, k, pitch, make_uint2(codes4(f[0], f[1], f[2], f[3], inv, most),
-                                                 codes4(f[4], f[5], f[6], f[7], inv, most)));
+      store_codes<VEC>(dst, k, pitch, make_uint2(codes4(f[0], f[1], f[2], f[3], sc.inv, sc.most),
+                                                 codes4(f[4], f[5], f[6], f[7], sc.inv, sc.most)));
     };
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
@@ -211,6 +252,13 @@ int grid_for(int64_t work, int per_sm) {
   return int(std::max<int64_t>(1, std::min<int64_t>(work, int64_t(num_sms()) * per_sm)));
 }
 
+// Blocks of 256 threads for row groups and, where those are few, for groups of blocks along a row too.
+dim3 pack_grid(int64_t row_groups, int64_t block_groups) {
+  const int64_t x = std::min<int64_t>(std::max<int64_t>(row_groups, 1), int64_t(num_sms()) * 8);
+  const int64_t y = std::min<int64_t>(block_groups, std::max<int64_t>(1, int64_t(num_sms()) * 8 / x));
+  return dim3(unsigned(x), unsigned(std::min<int64_t>(y, 65535)));
+}
+
 template <typename F>
 void by_type(int dtype, F&& f) {
   if (dtype == kv::kBf16) f(static_cast<__nv_bfloat16*>(nullptr));
@@ -230,16 +278,19 @@ std::vector<at::Tensor> save8(at::Tensor x) {
   at::Tensor exps = at::empty({blocks, rows}, x.options().dtype(at::kByte));
   if (rows == 0 || K == 0) return {codes, exps};
   PD_CHECK(K == 1 || x.stride(1) == 1, "save8: unit stride over the last dim is expected");
-  const int64_t tiles = (rows + kRows - 1) / kRows * ((blocks + kBlocks - 1) / kBlocks);
-  const int grid = grid_for((tiles + 7) / 8, 8);
+  PD_CHECK(K < (int64_t(1) << 30), "save8: rows of fewer than 2^30 values are expected");
   by_type(dtype, [&](auto* tag) {
     using T = std::remove_pointer_t<decltype(tag)>;
     const T* p = static_cast<const T*>(x.data_ptr());
     const int64_t stride = rows == 1 ? K : x.stride(0);
+    const uint32_t top = dtype == kv::kF16 ? kTopHalf : kTopWide;
     const bool vec = K % 8 == 0 && aligned16(p) && stride * int64_t(sizeof(T)) % 16 == 0;
-    auto* kern = vec ? save_kernel<true, T> : save_kernel<false, T>;
-    kern<<<grid, 256, 0, stream()>>>(p, stride, codes.data_ptr<int8_t>(), exps.data_ptr<uint8_t>(), rows, K, blocks,
-                                     dtype == kv::kF16 ? kTopHalf : kTopWide);
+    if (vec)
+      save_kernel<T><<<pack_grid((rows + 8 * kRows - 1) / (8 * kRows), (blocks + kBlocks - 1) / kBlocks), 256, 0, stream()>>>(
+          p, stride, codes.data_ptr<int8_t>(), exps.data_ptr<uint8_t>(), rows, int(K), int(blocks), top);
+    else
+      save_any_kernel<T><<<pack_grid((rows + 7) / 8, (blocks + kLong - 1) / kLong), 256, 0, stream()>>>(
+          p, stride, codes.data_ptr<int8_t>(), exps.data_ptr<uint8_t>(), rows, int(K), int(blocks), top);
   });
   PD_CHECK_LAUNCH();
   return {codes, exps};
@@ -256,13 +307,16 @@ at::Tensor load8(at::Tensor codes, at::Tensor exps, int64_t dtype) {
   at::Tensor y = at::empty({rows, K}, codes.options().dtype(at::ScalarType(dtype)));
   const int t = kv::dtype_of(y, "load8");
   if (rows == 0 || K == 0) return y;
-  const int64_t tiles = (rows + kRows - 1) / kRows * ((blocks + kBlocks - 1) / kBlocks);
-  const int grid = grid_for((tiles + 7) / 8, 8);
+  PD_CHECK(K < (int64_t(1) << 30), "load8: rows of fewer than 2^30 values are expected");
   by_type(t, [&](auto* tag) {
     using T = std::remove_pointer_t<decltype(tag)>;
-    auto* kern = K % 8 == 0 ? load_kernel<true, T> : load_kernel<false, T>;
-    kern<<<grid, 256, 0, stream()>>>(codes.data_ptr<int8_t>(), exps.data_ptr<uint8_t>(), static_cast<T*>(y.data_ptr()),
-                                     rows, K, blocks);
+    T* out = static_cast<T*>(y.data_ptr());
+    if (K % 8 == 0 && aligned16(codes.data_ptr()))
+      load_kernel<T><<<pack_grid((rows + 8 * kRows - 1) / (8 * kRows), (blocks + kBlocks - 1) / kBlocks), 256, 0, stream()>>>(
+          codes.data_ptr<int8_t>(), exps.data_ptr<uint8_t>(), out, rows, int(K), int(blocks));
+    else
+      load_any_kernel<T><<<pack_grid((rows + 7) / 8, (blocks + kLong - 1) / kLong), 256, 0, stream()>>>(
+          codes.data_ptr<int8_t>(), exps.data_ptr<uint8_t>(), out, rows, int(K), int(blocks));
   });
   PD_CHECK_LAUNCH();
   return y;

@@ -227,8 +227,24 @@ def _mixed_torch(x, n_s, ws, wn):
     return y
 
 
+def _dw_parts(dy, x, n_s, wdt):
+    """Weight gradients of a mixed projection, S and NS rows apart, in the weights' types (tcgen05)."""
+    B, T, N = dy.shape
+    K, run = x.shape[-1], _ext.gemm().tc_wgrad_as
+    err = _err(dy.device)
+    tr = lambda t: t[:, n_s:].transpose(0, 1)  # noqa: E731
+    dwn = run(tr(dy), tr(x), err, False, wdt[1]) if T > n_s else torch.zeros(0, N, K, dtype=wdt[1], device=dy.device)
+    if T == n_s:
+        dws = run(dy.reshape(1, -1, N), x.reshape(1, -1, K), err, True, wdt[0])
+    else:                                                    # one sum over the samples' S rows, read in place
+        dws = run(dy[:, :n_s], x[:, :n_s], err, True, wdt[0])
+    return dws, dwn
+
+
 def _dw_torch(dy, x, n_s, wdt):
     """Weight gradients of :func:`_mixed_torch`."""
+    if x.is_cuda and _wgrad_ok(dy, dy.shape[-1], x.shape[-1]) and _gemm_ok(x):
+        return _dw_parts(dy, x, n_s, wdt)
     if x.is_cuda and x.dtype == torch.bfloat16:
         return _dw(dy, x, n_s, wdt)
     dws = torch.matmul(dy[:, :n_s].reshape(-1, dy.shape[-1]).t(), x[:, :n_s].reshape(-1, x.shape[-1]))
