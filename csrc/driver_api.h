@@ -8,7 +8,7 @@
 #include <cstdio>
 #include <cuda.h>
 #include <cuda_runtime.h>
-#include <torch/extension.h>
+#include <c10/util/Exception.h>
 
 namespace pd {
 

@@ -91,13 +91,21 @@ __device__ __forceinline__ void tile_coords(const Params& p, int t, int& l, int&
   l = r / p.m_blocks;
 }
 
+// The 8-bit forms' epilogues are bound by instructions and the waits between them: 16 warps in place of 12 (a tile of 256
+// columns is then two chunks each) took the gradient's product of 100,608 x 256 x 1024 from 186 to 146 us; 8 took 171. Two
+// staged blocks a warp leave room for the same ring.
+__host__ __device__ constexpr int epi_warps(int saved8) { return saved8 == kNotSaved ? kEpiWarps : 16; }
+__host__ __device__ constexpr int stage_bufs(int saved8) { return saved8 == kNotSaved ? 3 : 2; }
+__host__ __device__ constexpr int threads_of(int saved8) { return 64 + 32 * epi_warps(saved8); }
+
 template <int BN, int STAGES, int SAVED8 = kNotSaved>
-__global__ void __launch_bounds__(kThreads, 1) gemm_kernel(const __grid_constant__ CUtensorMap tmA,
+__global__ void __launch_bounds__(threads_of(SAVED8), 1) gemm_kernel(const __grid_constant__ CUtensorMap tmA,
                                                            const __grid_constant__ CUtensorMap tmB,
                                                            const __grid_constant__ CUtensorMap tmC,
                                                            const __grid_constant__ CUtensorMap tmX,
                                                            const __grid_constant__ CUtensorMap tmR,
                                                            const Params p) {
+  constexpr int kEw = epi_warps(SAVED8), kBufs = stage_bufs(SAVED8);
   constexpr uint32_t kABytes = BM * BK * 2;
   constexpr uint32_t kBBytes = BN * BK * 2;
   constexpr uint32_t kTmemCols = 2 * BN;  // power of two for BN in {64, 128, 256}
@@ -110,8 +118,8 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_kernel(const __grid_constant
   uint64_t* tfull = empty + STAGES;     // [2]
   uint64_t* tempty = tfull + 2;         // [2]
   uint64_t* mma_done = tempty + 2;      // [1]
-  uint64_t* rbar_all = mma_done + 1;    // [kEpiWarps][2]: R blocks landed (TMA)
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(rbar_all + 2 * kEpiWarps);
+  uint64_t* rbar_all = mma_done + 1;    // [epilogue warps][2]: R blocks landed (TMA)
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(rbar_all + 2 * kEw);
   // per epilogue warp: 32 x 32 bf16 staging blocks for C and R / AUX (64-byte
   // rows, 16-byte chunks XOR-swizzled by (row >> 1) & 3: conflict-free both
   // when a thread writes its own row and when 4 lanes cover one row)
@@ -123,9 +131,9 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_kernel(const __grid_constant
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
     for (int s = 0; s < STAGES; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], 1); }
-    for (int a = 0; a < 2; ++a) { mbar_init(&tfull[a], 1); mbar_init(&tempty[a], kEpiWarps * 32); }
+    for (int a = 0; a < 2; ++a) { mbar_init(&tfull[a], 1); mbar_init(&tempty[a], kEw * 32); }
     mbar_init(mma_done, 1);
-    for (int i = 0; i < 2 * kEpiWarps; ++i) mbar_init(&rbar_all[i], 1);
+    for (int i = 0; i < 2 * kEw; ++i) mbar_init(&rbar_all[i], 1);
     *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     asm volatile("prefetch.tensormap [%0];" ::"l"(&tmA) : "memory");
@@ -227,8 +235,8 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_kernel(const __grid_constant
     const int ew = warp - 2;
     const int q = warp & 3;
     const int part = ew >> 2;
-    constexpr int kParts = kEpiWarps / 4;
-    uint8_t* stC = stage_base + ew * 3 * 2048;
+    constexpr int kParts = kEw / 4;
+    uint8_t* stC = stage_base + ew * kBufs * 2048;
     uint8_t* stR0 = stC + 2048;   // R ring: buffers stR0 and stR0 + 2048
     uint64_t* rbar = rbar_all + 2 * ew;
     const bool r_tma = p.r_tma != 0;
@@ -336,14 +344,8 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_kernel(const __grid_constant
 #pragma unroll
         for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
         if constexpr (SAVED8 == kSave) {
-          uint32_t most = 0;
-#pragma unroll
-          for (int i = 0; i < 32; ++i) most = max(most, i8::abs_bits(v[i]));
-          const uint32_t byte = i8::scale_byte(most);
-          const float inv = i8::inv_scale(byte), lim = i8::most_code(byte, i8::kTopWide);
           uint32_t w[8];
-#pragma unroll
-          for (int i = 0; i < 8; ++i) w[i] = i8::codes4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3], inv, lim);
+          const uint32_t byte = i8::save_block(v, i8::kTopWide, w);
           if (m0 + lane < p.M) {
             uint4* dst = reinterpret_cast<uint4*>(p.X8 + l * p.x8_ls + int64_t(m0 + lane) * p.x8_ms + n0 + c);
             dst[0] = make_uint4(w[0], w[1], w[2], w[3]);
@@ -364,24 +366,22 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_kernel(const __grid_constant
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
             float g[8];
-            i8::ints4(w[2 * j], g);
-            i8::ints4(w[2 * j + 1], g + 4);
+            i8::values4(w[2 * j], scale, g);
+            i8::values4(w[2 * j + 1], scale, g + 4);
 #pragma unroll
             for (int e = 0; e < 8; e += 2) {
               float d0, d1;
-              pk2_split(pk2_mul(pk2(g[e], g[e + 1]), pk2s(scale)), g[e], g[e + 1]);
               gelu_grad2<true>(g[e], g[e + 1], d0, d1);
               v[8 * j + e] *= d0;
               v[8 * j + e + 1] *= d1;
             }
-            uint4 pk;
-            __nv_bfloat162 h0 = __floats2bfloat162_rn(g[0], g[1]);
-            __nv_bfloat162 h1 = __floats2bfloat162_rn(g[2], g[3]);
-            __nv_bfloat162 h2 = __floats2bfloat162_rn(g[4], g[5]);
-            __nv_bfloat162 h3 = __floats2bfloat162_rn(g[6], g[7]);
-            pk.x = *reinterpret_cast<uint32_t*>(&h0); pk.y = *reinterpret_cast<uint32_t*>(&h1);
-            pk.z = *reinterpret_cast<uint32_t*>(&h2); pk.w = *reinterpret_cast<uint32_t*>(&h3);
-            *reinterpret_cast<uint4*>(stX + sw(lane, j)) = pk;
+            uint32_t h[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const __nv_bfloat162 b = __floats2bfloat162_rn(g[2 * e], g[2 * e + 1]);
+              h[e] = *reinterpret_cast<const uint32_t*>(&b);
+            }
+            *reinterpret_cast<uint4*>(stX + sw(lane, j)) = make_uint4(h[0], h[1], h[2], h[3]);
           }
         } else if (has_r && p.epi != kDGelu && p.epi != kMul && p.epi != kMaskPos && p.epi != kMulAdd) {
           // addend before the activation: residual, or a bias broadcast through a zero row stride
@@ -896,7 +896,8 @@ void check_operand(const at::Tensor& t, const char* name) {
 template <int BN, int STAGES, int SAVED8 = tc::kNotSaved>
 void launch(const CUtensorMap& ta, const CUtensorMap& tb, const CUtensorMap& tcm, const CUtensorMap& txm,
             const CUtensorMap& trm, const tc::Params& p) {
-  constexpr size_t smem = STAGES * (tc::BM * tc::BK * 2 + BN * tc::BK * 2) + 1024 + 1024 + tc::kEpiWarps * 3 * 2048;
+  constexpr size_t smem = STAGES * (tc::BM * tc::BK * 2 + BN * tc::BK * 2) + 1024 + 1024 +
+                          tc::epi_warps(SAVED8) * tc::stage_bufs(SAVED8) * 2048;
   static_assert(smem <= 232448, "GEMM shared memory over the 227 KB per-block limit");
   static bool attr = false;
   if (!attr) {
@@ -905,7 +906,7 @@ void launch(const CUtensorMap& ta, const CUtensorMap& tb, const CUtensorMap& tcm
     attr = true;
   }
   int grid = p.tiles < num_sms() ? p.tiles : num_sms();
-  tc::gemm_kernel<BN, STAGES, SAVED8><<<grid, tc::kThreads, smem, stream()>>>(ta, tb, tcm, txm, trm, p);
+  tc::gemm_kernel<BN, STAGES, SAVED8><<<grid, tc::threads_of(SAVED8), smem, stream()>>>(ta, tb, tcm, txm, trm, p);
   PD_CHECK_LAUNCH();
 }
 

@@ -49,12 +49,45 @@ __device__ __forceinline__ uint32_t codes4(float a, float b, float c, float d, f
   const uint32_t lo = __byte_perm(one(a), one(b), 0x0040), hi = __byte_perm(one(c), one(d), 0x0040);
   return __byte_perm(lo, hi, 0x5410);
 }
-// The integers of four codes: byte + 128 below 2^23's mantissa, less 2^23 + 128.
-__device__ __forceinline__ void ints4(uint32_t codes, float* f) {
+// Four codes of a block by its power-of-two scale: x * inv is exact, so one fused multiply-add rounds it to the integer.
+__device__ __forceinline__ uint32_t block_codes4(const float* x, float inv) {
+  uint32_t c[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) c[i] = __float_as_uint(fmaf(x[i], inv, 12582912.0f));
+  return __byte_perm(__byte_perm(c[0], c[1], 0x0040), __byte_perm(c[2], c[3], 0x0040), 0x5410);
+}
+// max(|a|, |b|, |c|); NaN where one of them is.
+__device__ __forceinline__ float max_abs3(float a, float b, float c) {
+  float r;
+  asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+// The 32 values of a block in one thread's registers: its codes, and its scale byte.
+__device__ __forceinline__ uint32_t save_block(const float* v, uint32_t top, uint32_t (&w)[8]) {
+  float m0 = 0.0f, m1 = 0.0f;
+#pragma unroll
+  for (int i = 0; i < 32; i += 4) {
+    m0 = max_abs3(m0, v[i], v[i + 1]);
+    m1 = max_abs3(m1, v[i + 2], v[i + 3]);
+  }
+  const uint32_t byte = scale_byte(__float_as_uint(max_abs3(m0, m1, 0.0f)));
+  const float inv = inv_scale(byte);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) w[i] = block_codes4(v + 4 * i, inv);
+  if (byte >= top) {                                      // no numbers, or codes held to 63: rare
+    const float most = most_code(byte, top);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) w[i] = codes4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3], inv, most);
+  }
+  return byte;
+}
+
+// The values of four codes: byte + 128 below 2^23's mantissa, less 2^23 + 128, times the block's scale.
+__device__ __forceinline__ void values4(uint32_t codes, float scale, float* f) {
   const uint32_t u = codes ^ 0x80808080u;
 #pragma unroll
   for (int i = 0; i < 4; ++i)
-    f[i] = __fsub_rn(__uint_as_float(__byte_perm(u, 0x4b000000u, 0x7540 + i)), 8388736.0f);
+    f[i] = __fmul_rn(__fsub_rn(__uint_as_float(__byte_perm(u, 0x4b000000u, 0x7540 + i)), 8388736.0f), scale);
 }
 
 // Whole rows with a 32-bit scale: max(amax / 127, 2^-126) and its reciprocal; a row without numbers has codes of 0 and a

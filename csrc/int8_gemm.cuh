@@ -3,19 +3,23 @@
 //   C[l, m, n] = act( (sum_k A[l, m, k] B[l, n, k]) * (s[l, m] t[l, n]) + bias[n] ) + R[l, m, n]
 //
 // A: a token's codes with its scale s, B: a weight's codes with the scale t of
-// each output channel. Persistent, one block an SM, 14 warps, the roles of the
-// bf16 GEMM (gemm_tc.cu):
+// each output channel; kind::i8, M = 128, K = 32 an instruction. Sums stay below
+// 2^31 for K up to 131072 (codes down to -128).
+//
+// product_kernel is persistent, one block an SM, 14 warps, the roles of the bf16
+// GEMM (gemm_tc.cu):
 //   warp 0       TMA producer: 128 x 128 and BN x 128 byte tiles (128-byte
-//                swizzle) into a ring of STAGES; rows and columns past the
-//                operands' ends arrive as zeros
-//   warp 1       TMEM (2 x BN columns of s32) and the tcgen05.mma of one lane:
-//                kind::i8, M = 128, N = BN, K = 32
+//                swizzle) into a ring; rows and columns past the operands' ends
+//                arrive as zeros
+//   warp 1       TMEM (2 x BN columns of s32) and the tcgen05.mma of one lane
 //   warps 2..13  epilogue: a thread owns a row of 32 columns at a time; scales,
 //                bias and activation in 32-bit floats, one rounding to the
 //                output type, out through a swizzled 32 x 32 block in shared
 //                memory and a TMA store (or row by row, where C's rows do not
 //                lie on 16 bytes)
-// Sums stay below 2^31 for K up to 133,000 (codes within +-127).
+// split_kernel is for calls whose tiles leave most SMs idle (few rows, a long
+// axis): a cluster shares a tile and splits K; every block leaves its sums in
+// shared memory, and each takes a part of the rows from all of them.
 #pragma once
 
 #include "int8_common.cuh"
@@ -35,14 +39,21 @@ constexpr int BK = 128;                 // bytes, four instructions of 32
 constexpr int kEpiWarps = 12;
 constexpr int kParts = kEpiWarps / 4;   // warps that share 32 rows, by 32-column chunks
 constexpr int kThreads = 64 + 32 * kEpiWarps;
+constexpr int kMaxStages = 8;
+constexpr int kSplitN = 64;             // columns of a tile whose K is split
+constexpr int kSplitStages = 4;
+constexpr int kSplitThreads = 192;      // TMA, MMA, four warps of 32 rows
+constexpr int kSplitPitch = 4 * kSplitN + 16;             // bytes of a row of sums: 16-byte stores of 8 rows on all banks
 
 struct Params {
   int M, N, L;
   int m_blocks, n_blocks, k_blocks, tiles;
+  int bn, stages;
+  int splits, kb_per_split;
   const float* s; int64_t s_ls, s_ms;
   const float* t; int64_t t_ls;
   const float* bias;
-  const void* R; int64_t r_ls, r_ms; int r_vec;     // r_vec: rows of R on 16 bytes, whole chunks
+  const void* R; int64_t r_ls, r_ms; int r_vec;           // r_vec: rows of R on 16 bytes
   void* C; int64_t c_ls, c_ms;
   int act;
   int a_mode, c_mode, c_tma;
@@ -50,7 +61,7 @@ struct Params {
   int* err;
 };
 
-template <typename T> struct Out { static constexpr int kStage = 32 * 32 * int(sizeof(T)); };
+template <typename T> constexpr int kStageBytes = 32 * 32 * int(sizeof(T));
 
 // Byte offset of 16-byte chunk c of row r in a staged 32 x 32 block: the TMA
 // swizzle of 64-byte (2-byte types) or 128-byte rows.
@@ -60,12 +71,32 @@ __device__ __forceinline__ int staged(int r, int c) {
 }
 
 template <typename T>
+__device__ __forceinline__ uint32_t pack2(float a, float b) {
+  if constexpr (std::is_same_v<T, __nv_bfloat16>) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  } else {
+    const __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  }
+}
+template <typename T>
 __device__ __forceinline__ uint4 pack16(const float* v) {
-  uint4 u;
-  T* e = reinterpret_cast<T*>(&u);
-#pragma unroll
-  for (int i = 0; i < 16 / int(sizeof(T)); ++i) e[i] = kv::from_f<T>(v[i]);
-  return u;
+  if constexpr (sizeof(T) == 4) {
+    return make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3]));
+  } else {
+    return make_uint4(pack2<T>(v[0], v[1]), pack2<T>(v[2], v[3]), pack2<T>(v[4], v[5]), pack2<T>(v[6], v[7]));
+  }
+}
+
+template <typename T>
+__device__ __forceinline__ void gelu_pair(float& a, float& b) {
+  if constexpr (sizeof(T) == 4) {                         // the polynomial of the 16-bit types is 5.5e-6 off
+    a *= fmaf(0.5f, erff(a * 0.70710678f), 0.5f);
+    b *= fmaf(0.5f, erff(b * 0.70710678f), 0.5f);
+  } else {
+    gelu2(a, b);
+  }
 }
 
 __device__ __forceinline__ void mma_i8(uint32_t d, uint64_t da, uint64_t db, uint32_t idesc, uint32_t acc) {
@@ -76,7 +107,7 @@ __device__ __forceinline__ void mma_i8(uint32_t d, uint64_t da, uint64_t db, uin
       ::"r"(d), "l"(da), "l"(db), "r"(idesc), "r"(acc) : "memory");
 }
 // kind::i8: s32 accumulators, signed A and B, both K-major
-constexpr uint32_t instr_i8(int m, int n) {
+__host__ __device__ constexpr uint32_t instr_i8(int m, int n) {
   return (2u << 4) | (1u << 7) | (1u << 10) | (uint32_t(n >> 3) << 17) | (uint32_t(m >> 4) << 24);
 }
 
@@ -87,48 +118,52 @@ __device__ __forceinline__ void tile_at(const Params& p, int w, int& l, int& mb,
   l = r / p.m_blocks;
 }
 
-template <int BN, int STAGES, typename T>
+// The launch before this one (the rows' codes) has finished and its writes are seen. The kernel may have been launched
+// while it ran: what comes before this wait reads nothing that it writes.
+__device__ __forceinline__ void wait_for_launch_before() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
+template <typename T>
 __global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_constant__ CUtensorMap tmA,
                                                               const __grid_constant__ CUtensorMap tmB,
                                                               const __grid_constant__ CUtensorMap tmC, const Params p) {
-  constexpr uint32_t kA = BM * BK, kB = BN * BK, kCols = 2 * BN;
-  extern __shared__ __align__(1024) uint8_t ring[];       // A and B tiles, then a staged block for each epilogue warp
-  __shared__ uint64_t full[STAGES], empty[STAGES], tfull[2], tempty[2], mma_done;
+  extern __shared__ __align__(1024) uint8_t ring[];       // A tiles, B tiles, then a staged block for each epilogue warp
+  __shared__ uint64_t full[kMaxStages], empty[kMaxStages], tfull[2], tempty[2], mma_done;
   __shared__ uint32_t tmem_slot;
   __shared__ volatile int abort_flag;
+  __shared__ __align__(16) float s_cols[kEpiWarps][64];   // a chunk's channel scales and biases, as t0 t1 b0 b1, ...
+  const uint32_t kA = BM * BK, kB = p.bn * BK;
   uint8_t* sA = ring;
-  uint8_t* sB = ring + STAGES * kA;
-
+  uint8_t* sB = ring + p.stages * kA;
   if (tcx::smem_u32(ring) % 1024 != 0) {                  // the swizzled tiles need it
     set_error(p.err, 4);
     return;
   }
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
-    for (int s = 0; s < STAGES; ++s) { tcx::mbar_init(&full[s], 1); tcx::mbar_init(&empty[s], 1); }
+    for (int s = 0; s < p.stages; ++s) { tcx::mbar_init(&full[s], 1); tcx::mbar_init(&empty[s], 1); }
     for (int a = 0; a < 2; ++a) { tcx::mbar_init(&tfull[a], 1); tcx::mbar_init(&tempty[a], kEpiWarps * 32); }
     tcx::mbar_init(&mma_done, 1);
     abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    asm volatile("prefetch.tensormap [%0];" ::"l"(&tmA) : "memory");
+    asm volatile("prefetch.tensormap [%0];" ::"l"(&tmB) : "memory");
   }
   if (warp == 1) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;"
-                 ::"r"(tcx::smem_u32(&tmem_slot)), "r"(kCols) : "memory");
+                 ::"r"(tcx::smem_u32(&tmem_slot)), "r"(2 * p.bn) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
   tcx::tc_fence_before();
   __syncthreads();
   tcx::tc_fence_after();
   const uint32_t tmem = tmem_slot;
+  wait_for_launch_before();
 
   if (warp == 0) {
     // ---------------- TMA producer ----------------
     if (lane == 0) {
-      int stage = 0;
+      int stage = 0, issued = 0;
       uint32_t phase = 1;
-      int issued_on[STAGES];
-#pragma unroll
-      for (int s = 0; s < STAGES; ++s) issued_on[s] = 0;
       for (int w = blockIdx.x; w < p.tiles && !abort_flag; w += gridDim.x) {
         int l, mb, nb;
         tile_at(p, w, l, mb, nb);
@@ -136,20 +171,22 @@ __global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_const
           if (!tcx::mbar_wait(&empty[stage], phase, p.err)) { abort_flag = 1; break; }
           tcx::mbar_expect_tx(&full[stage], kA + kB);
           tcx::tma_load_rows(sA + stage * kA, &tmA, &full[stage], p.a_mode, kb * BK, mb * BM, l);
-          tcx::tma_load_rows(sB + stage * kB, &tmB, &full[stage], 0, kb * BK, nb * BN, p.b_shared ? 0 : l);
-          ++issued_on[stage];
-          if (++stage == STAGES) { stage = 0; phase ^= 1; }
+          tcx::tma_load_rows(sB + stage * kB, &tmB, &full[stage], 0, kb * BK, nb * p.bn, p.b_shared ? 0 : l);
+          ++issued;
+          if (++stage == p.stages) { stage = 0; phase ^= 1; }
         }
       }
       if (abort_flag) {                                   // every issued load lands before the block may exit
-#pragma unroll
-        for (int s = 0; s < STAGES; ++s)
-          if (issued_on[s] > 0) (void)tcx::mbar_wait(&full[s], uint32_t(issued_on[s] - 1) & 1u, p.err);
+        for (int s = 0; s < p.stages; ++s) {
+          const int n = (issued - s + p.stages - 1) / p.stages;     // loads issued on this stage
+          if (n > 0) (void)tcx::mbar_wait(&full[s], uint32_t(n - 1) & 1u, p.err);
+        }
       }
     }
   } else if (warp == 1) {
     // ---------------- MMA issuer ----------------
     if (lane == 0) {
+      const uint32_t idesc = instr_i8(BM, p.bn);
       int stage = 0;
       uint32_t phase = 0;
       int local = 0;
@@ -157,18 +194,17 @@ __global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_const
         const int a = local & 1;
         if (!tcx::mbar_wait(&tempty[a], ((local >> 1) & 1) ^ 1, p.err)) { abort_flag = 1; break; }
         tcx::tc_fence_after();
-        const uint32_t d = tmem + uint32_t(a * BN);
+        const uint32_t d = tmem + uint32_t(a * p.bn);
         bool ok = true;
         for (int kb = 0; kb < p.k_blocks; ++kb) {
           if (!tcx::mbar_wait(&full[stage], phase, p.err)) { abort_flag = 1; ok = false; break; }
           tcx::tc_fence_after();
-          const uint32_t a_addr = tcx::smem_u32(sA + stage * kA), b_addr = tcx::smem_u32(sB + stage * kB);
+          const uint64_t da = tcx::smem_desc(tcx::smem_u32(sA + stage * kA)), db = tcx::smem_desc(tcx::smem_u32(sB + stage * kB));
 #pragma unroll
-          for (int k = 0; k < BK / 32; ++k)
-            mma_i8(d, tcx::smem_desc(a_addr + k * 32), tcx::smem_desc(b_addr + k * 32), instr_i8(BM, BN),
-                   (kb | k) ? 1u : 0u);
+          for (int k = 0; k < BK / 32; ++k)               // 32 bytes further: 2 in the descriptors' units of 16
+            mma_i8(d, da + 2 * k, db + 2 * k, idesc, (kb | k) ? 1u : 0u);
           tcx::tc_commit(&empty[stage]);
-          if (++stage == STAGES) { stage = 0; phase ^= 1; }
+          if (++stage == p.stages) { stage = 0; phase ^= 1; }
         }
         if (!ok) break;
         tcx::tc_commit(&tfull[a]);
@@ -179,49 +215,63 @@ __global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_const
   } else {
     // ---------------- epilogue ----------------
     const int ew = warp - 2, q = warp & 3, part = ew >> 2;
-    uint8_t* stage_c = ring + STAGES * (kA + kB) + ew * Out<T>::kStage;
+    uint8_t* stage_c = ring + p.stages * (kA + kB) + ew * kStageBytes<T>;
+    float* cols = s_cols[ew];
+    const int slot = (lane >> 1) * 4 + (lane & 1);        // t of column `lane`; its bias two further
     int local = 0;
     for (int w = blockIdx.x; w < p.tiles; w += gridDim.x, ++local) {
       const int a = local & 1;
       int l, mb, nb;
       tile_at(p, w, l, mb, nb);
-      const int m0 = mb * BM + q * 32, n0 = nb * BN, row = m0 + lane;
+      const int m0 = mb * BM + q * 32, n0 = nb * p.bn, row = m0 + lane;
       const bool there = row < p.M;
       const float s = there ? p.s[l * p.s_ls + row * p.s_ms] : 0.0f;
+      // sums are below 2^31: past this no scaled one overflows (a NaN scale counts as large)
+      const uint32_t s_most = p.act == kGelu ? __reduce_max_sync(0xffffffffu, abs_bits(s)) : 0;
+      const int c_end = min(p.bn, p.N - n0);
+      auto column = [&](int c) {                          // (t, bias) of this lane's column of chunk c
+        const int n = n0 + c + lane;
+        const bool in = c < c_end && n < p.N;
+        return make_float2(in ? __ldg(p.t + l * p.t_ls + n) : 0.0f, in && p.bias != nullptr ? __ldg(p.bias + n) : 0.0f);
+      };
+      float2 tb = column(part * 32);
       if (!tcx::mbar_wait(&tfull[a], (local >> 1) & 1, p.err)) { abort_flag = 1; break; }
       tcx::tc_fence_after();
-      const uint32_t tbase = tmem + (uint32_t(q * 32) << 16) + uint32_t(a * BN);
+      const uint32_t tbase = tmem + (uint32_t(q * 32) << 16) + uint32_t(a * p.bn);
 #pragma unroll 1
-      for (int c = part * 32; c < BN && n0 + c < p.N; c += kParts * 32) {
-        const int n = n0 + c, cols = min(32, p.N - n);
+      for (int c = part * 32; c < c_end; c += kParts * 32) {
+        const int n = n0 + c, width = min(32, p.N - n);
         uint32_t r[32];
         tcx::tc_ld32_issue(tbase + c, r);
-        const float tl = lane < cols ? p.t[l * p.t_ls + n + lane] : 0.0f;
-        const float bl = p.bias != nullptr && lane < cols ? p.bias[n + lane] : 0.0f;
+        cols[slot] = tb.x;
+        cols[slot + 2] = tb.y;
+        // |sum * s * t| < 2^31 * s * t: GELU's guard is needed where that may pass the largest number
+        const bool guard = p.act == kGelu &&
+                           __uint_as_float(s_most) * __uint_as_float(__reduce_max_sync(0xffffffffu, abs_bits(tb.x))) > 1e28f;
+        __syncwarp();
+        tb = column(c + kParts * 32);                             // the next chunk's, on its way
         tcx::tc_ld_wait(r);
         float v[32];
+        const uint64_t s2 = pk2s(s);
 #pragma unroll
-        for (int i = 0; i < 32; ++i)
-          v[i] = fmaf(float(int(r[i])), s * __shfl_sync(0xffffffffu, tl, i), __shfl_sync(0xffffffffu, bl, i));
+        for (int i = 0; i < 32; i += 2) {
+          const ulonglong2 tb2 = *reinterpret_cast<const ulonglong2*>(cols + 2 * i);
+          pk2_split(pk2_fma(pk2(float(int(r[i])), float(int(r[i + 1]))), pk2_mul(s2, tb2.x), tb2.y), v[i], v[i + 1]);
+        }
         if (p.act == kGelu) {
+          if (guard || !(__uint_as_float(s_most) < 1e30f)) {
 #pragma unroll
-          for (int i = 0; i < 32; i += 2) {
-            v[i] = from_below(v[i]);
-            v[i + 1] = from_below(v[i + 1]);
-            if constexpr (sizeof(T) == 4) {               // the polynomial of the 16-bit types is 5.5e-6 off
-              v[i] *= fmaf(0.5f, erff(v[i] * 0.70710678f), 0.5f);
-              v[i + 1] *= fmaf(0.5f, erff(v[i + 1] * 0.70710678f), 0.5f);
-            } else {
-              gelu2(v[i], v[i + 1]);
-            }
+            for (int i = 0; i < 32; ++i) v[i] = from_below(v[i]);
           }
+#pragma unroll
+          for (int i = 0; i < 32; i += 2) gelu_pair<T>(v[i], v[i + 1]);
         } else if (p.act == kRelu) {
 #pragma unroll
           for (int i = 0; i < 32; ++i) v[i] = v[i] < 0.0f ? 0.0f : v[i];     // NaN stays
         }
         if (p.R != nullptr && there) {
           const T* res = static_cast<const T*>(p.R) + l * p.r_ls + row * p.r_ms + n;
-          if (p.r_vec && cols == 32) {
+          if (p.r_vec && width == 32) {
 #pragma unroll
             for (int i = 0; i < 32; i += 8) {
               kv::Raw<8, T> x;
@@ -234,7 +284,7 @@ __global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_const
           } else {
 #pragma unroll
             for (int i = 0; i < 32; ++i)
-              if (i < cols) v[i] += kv::to_f(res[i]);
+              if (i < width) v[i] += kv::to_f(res[i]);
           }
         }
         if (lane == 0) tcx::bulk_wait_read_all();         // the staged block's last store has read it
@@ -252,11 +302,13 @@ __global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_const
           }
         } else {
           __syncwarp();
-          T* out = static_cast<T*>(p.C) + l * p.c_ls + n;
-          for (int i = 0; i < 32 && m0 + i < p.M; ++i)
-            if (lane < cols)
-              out[(m0 + i) * p.c_ms + lane] =
-                  *reinterpret_cast<const T*>(stage_c + staged<T>(i, lane / kPer) + lane % kPer * int(sizeof(T)));
+          if (lane < width) {
+            T* out = static_cast<T*>(p.C) + l * p.c_ls + m0 * p.c_ms + n + lane;
+            const int rows = min(32, p.M - m0);
+#pragma unroll 8
+            for (int i = 0; i < rows; ++i, out += p.c_ms)
+              *out = *reinterpret_cast<const T*>(stage_c + staged<T>(i, lane / kPer) + lane % kPer * int(sizeof(T)));
+          }
           __syncwarp();
         }
       }
@@ -270,7 +322,198 @@ __global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_const
   __syncthreads();
   if (warp == 1) {
     tcx::tc_fence_after();
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kCols) : "memory");
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(2 * p.bn) : "memory");
+  }
+}
+
+// ---------------------------------------------------------------------------
+__device__ __forceinline__ void cluster_barrier() {
+  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ int4 load_cluster(uint32_t addr, uint32_t rank) {
+  uint32_t a;
+  int4 v;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(addr), "r"(rank));
+  asm volatile("ld.shared::cluster.v4.u32 {%0, %1, %2, %3}, [%4];"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a) : "memory");
+  return v;
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kSplitThreads, 1) split_kernel(const __grid_constant__ CUtensorMap tmA,
+                                                                 const __grid_constant__ CUtensorMap tmB, const Params p) {
+  constexpr uint32_t kA = BM * BK, kB = kSplitN * BK;
+  extern __shared__ __align__(1024) uint8_t ring[];       // A and B tiles; later this block's sums [128][kSplitPitch]
+  __shared__ uint64_t full[kSplitStages], empty[kSplitStages], done;
+  __shared__ uint32_t tmem_slot;
+  __shared__ volatile int abort_flag;
+  uint8_t* sA = ring;
+  uint8_t* sB = ring + kSplitStages * kA;
+  uint8_t* sums = ring;                                   // once the products are done with the tiles
+  if (tcx::smem_u32(ring) % 1024 != 0) {                  // alike in every block of the cluster
+    set_error(p.err, 4);
+    return;
+  }
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int rank = blockIdx.x % p.splits;
+  int l, mb, nb;
+  tile_at(p, blockIdx.x / p.splits, l, mb, nb);
+  const int kb0 = rank * p.kb_per_split, kb1 = min(kb0 + p.kb_per_split, p.k_blocks);
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < kSplitStages; ++s) { tcx::mbar_init(&full[s], 1); tcx::mbar_init(&empty[s], 1); }
+    tcx::mbar_init(&done, 1);
+    abort_flag = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    asm volatile("prefetch.tensormap [%0];" ::"l"(&tmA) : "memory");
+    asm volatile("prefetch.tensormap [%0];" ::"l"(&tmB) : "memory");
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;"
+                 ::"r"(tcx::smem_u32(&tmem_slot)), "r"(kSplitN) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  tcx::tc_fence_before();
+  __syncthreads();
+  tcx::tc_fence_after();
+  const uint32_t tmem = tmem_slot;
+
+  if (warp == 0) {
+    if (lane == 0) {
+      int issued = 0;
+      // the weight's first tiles do not wait for the rows' codes
+      for (int kb = kb0; kb < min(kb1, kb0 + kSplitStages); ++kb) {
+        const int stage = kb - kb0;
+        tcx::mbar_expect_tx(&full[stage], kA + kB);
+        tcx::tma_load_rows(sB + stage * kB, &tmB, &full[stage], 0, kb * BK, nb * kSplitN, p.b_shared ? 0 : l);
+      }
+      wait_for_launch_before();
+      for (int kb = kb0; kb < kb1; ++kb, ++issued) {
+        const int stage = issued % kSplitStages;
+        if (issued >= kSplitStages) {
+          if (!tcx::mbar_wait(&empty[stage], uint32_t(issued / kSplitStages - 1) & 1u, p.err)) { abort_flag = 1; break; }
+          tcx::mbar_expect_tx(&full[stage], kA + kB);
+          tcx::tma_load_rows(sB + stage * kB, &tmB, &full[stage], 0, kb * BK, nb * kSplitN, p.b_shared ? 0 : l);
+        }
+        tcx::tma_load_rows(sA + stage * kA, &tmA, &full[stage], p.a_mode, kb * BK, mb * BM, l);
+      }
+      if (abort_flag) {                                   // every issued load lands before the block may exit
+        for (int s = 0; s < kSplitStages; ++s) {
+          const int n = (issued - s + kSplitStages - 1) / kSplitStages;
+          if (n > 0) (void)tcx::mbar_wait(&full[s], uint32_t(n - 1) & 1u, p.err);
+        }
+      }
+    }
+  } else if (warp == 1) {
+    if (lane == 0) {
+      bool ok = true;
+      for (int kb = kb0; kb < kb1 && ok; ++kb) {
+        const int i = kb - kb0, stage = i % kSplitStages;
+        ok = tcx::mbar_wait(&full[stage], uint32_t(i / kSplitStages) & 1u, p.err);
+        if (!ok) { abort_flag = 1; break; }
+        tcx::tc_fence_after();
+        const uint64_t da = tcx::smem_desc(tcx::smem_u32(sA + stage * kA)), db = tcx::smem_desc(tcx::smem_u32(sB + stage * kB));
+#pragma unroll
+        for (int k = 0; k < BK / 32; ++k) mma_i8(tmem, da + 2 * k, db + 2 * k, instr_i8(BM, kSplitN), (i | k) ? 1u : 0u);
+        tcx::tc_commit(&empty[stage]);
+      }
+      tcx::tc_commit(&done);
+      (void)tcx::mbar_wait(&done, 0, p.err);              // finished before TMEM is freed
+    }
+  } else {
+    // sums of this block's part of K, 32 rows a warp (TMEM lanes by the warp's place in its group of four)
+    const int q = warp & 3;
+    uint8_t* mine = sums + (q * 32 + lane) * kSplitPitch;
+    if (kb1 > kb0) {
+      (void)tcx::mbar_wait(&done, 0, p.err);
+      tcx::tc_fence_after();
+#pragma unroll
+      for (int c = 0; c < kSplitN; c += 32) {
+        uint32_t r[32];
+        tcx::tc_ld32_issue(tmem + (uint32_t(q * 32) << 16) + c, r);
+        tcx::tc_ld_wait(r);
+#pragma unroll
+        for (int i = 0; i < 32; i += 4)
+          *reinterpret_cast<uint4*>(mine + (c + i) * 4) = make_uint4(r[i], r[i + 1], r[i + 2], r[i + 3]);
+      }
+      tcx::tc_fence_before();
+    } else {
+#pragma unroll
+      for (int i = 0; i < kSplitN; i += 4) *reinterpret_cast<uint4*>(mine + i * 4) = make_uint4(0, 0, 0, 0);
+    }
+  }
+  __syncwarp();
+
+  // this block's share of the rows, eight columns a thread; what else they need is on its way during the barrier
+  constexpr int kWide = 8, kUnits = kSplitN / kWide;
+  const int rows = BM / p.splits, base = rank * rows;
+  float s = 0.0f, t[kWide], add[kWide], res[kWide];
+  int row, n, width;
+  auto operands = [&](int i) {
+    row = mb * BM + base + i / kUnits;
+    n = nb * kSplitN + i % kUnits * kWide;
+    width = i < rows * kUnits && row < p.M ? min(kWide, p.N - n) : 0;
+    if (width > 0) s = p.s[l * p.s_ls + row * p.s_ms];
+#pragma unroll
+    for (int e = 0; e < kWide; ++e) {
+      t[e] = e < width ? __ldg(p.t + l * p.t_ls + n + e) : 0.0f;
+      add[e] = e < width && p.bias != nullptr ? __ldg(p.bias + n + e) : 0.0f;
+      res[e] = e < width && p.R != nullptr ? kv::to_f(static_cast<const T*>(p.R)[l * p.r_ls + row * p.r_ms + n + e]) : 0.0f;
+    }
+  };
+  wait_for_launch_before();
+  operands(threadIdx.x);
+  cluster_barrier();                                      // every block's sums are in place
+  for (int i = threadIdx.x; i < rows * kUnits; i += kSplitThreads) {
+    if (i != threadIdx.x) operands(i);
+    if (width <= 0) continue;
+    const uint32_t at = tcx::smem_u32(sums) + (base + i / kUnits) * kSplitPitch + i % kUnits * kWide * 4;
+    int4 part[2][8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      if (k < p.splits) {
+        part[0][k] = load_cluster(at, uint32_t(k));
+        part[1][k] = load_cluster(at + 16, uint32_t(k));
+      }
+    }
+    float v[kWide];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      int4 sum = part[h][0];
+#pragma unroll
+      for (int k = 1; k < 8; ++k)
+        if (k < p.splits) { sum.x += part[h][k].x; sum.y += part[h][k].y; sum.z += part[h][k].z; sum.w += part[h][k].w; }
+      v[4 * h] = float(sum.x); v[4 * h + 1] = float(sum.y); v[4 * h + 2] = float(sum.z); v[4 * h + 3] = float(sum.w);
+    }
+#pragma unroll
+    for (int e = 0; e < kWide; ++e) {
+      v[e] = fmaf(v[e], s * t[e], add[e]);
+      if (p.act == kGelu) v[e] = from_below(v[e]);
+      if (p.act == kRelu) v[e] = v[e] < 0.0f ? 0.0f : v[e];
+    }
+    if (p.act == kGelu) {
+#pragma unroll
+      for (int e = 0; e < kWide; e += 2) gelu_pair<T>(v[e], v[e + 1]);
+    }
+    if (p.R != nullptr) {
+#pragma unroll
+      for (int e = 0; e < kWide; ++e) v[e] += res[e];
+    }
+    T* out = static_cast<T*>(p.C) + l * p.c_ls + row * p.c_ms + n;
+    if (p.c_tma && width == kWide) {                      // rows of C on 16 bytes
+      constexpr int kPer = 16 / int(sizeof(T));
+#pragma unroll
+      for (int e = 0; e < kWide; e += kPer) *reinterpret_cast<uint4*>(out + e) = pack16<T>(v + e);
+    } else {
+#pragma unroll
+      for (int e = 0; e < kWide; ++e)
+        if (e < width) out[e] = kv::from_f<T>(v[e]);
+    }
+  }
+  cluster_barrier();                                      // no block leaves while another reads its sums
+  if (warp == 1) {
+    tcx::tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kSplitN) : "memory");
   }
 }
 
@@ -278,7 +521,7 @@ __global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_const
 // 3-D map {inner, rows, L} of a [L, rows, inner] view; dims in the order {inner, L, rows} (mode 1) where the batches lie
 // inside the rows, so that strides ascend. Strides in bytes.
 inline CUtensorMap map_of(CUtensorMapDataType type, const void* base, int64_t inner, int64_t rows, int64_t L, int64_t row_bytes,
-                   int64_t l_bytes, int box_inner, int box_rows, CUtensorMapSwizzle swizzle, int& mode) {
+                          int64_t l_bytes, int box_inner, int box_rows, CUtensorMapSwizzle swizzle, int& mode) {
   CUtensorMap m;
   if (L <= 1) l_bytes = row_bytes * rows;
   mode = L > 1 && l_bytes < row_bytes ? 1 : 0;
@@ -296,42 +539,68 @@ inline CUtensorMap map_of(CUtensorMapDataType type, const void* base, int64_t in
   return m;
 }
 
-template <int BN, int STAGES, typename T>
-void launch(const CUtensorMap& ta, const CUtensorMap& tb, const CUtensorMap& tc, const Params& p) {
-  constexpr size_t smem = STAGES * size_t(BM + BN) * BK + kEpiWarps * size_t(Out<T>::kStage);
-  static_assert(smem + 1024 <= 232448, "shared memory of a block");
-  auto* kern = product_kernel<BN, STAGES, T>;
-  static std::atomic<uint64_t> allowed{0};               // by device: the call costs a small launch's time
+// Launch right behind the rows' codes (before they are done: the kernel waits for them itself), as clusters if asked.
+template <typename... Args>
+void launch_behind(void (*kern)(Args...), std::atomic<uint64_t>& allowed, int most_smem, int grid, int threads, size_t smem,
+                   int cluster, Args... args) {
   int dev = 0;
   PD_CHECK_CUDA(cudaGetDevice(&dev));
   const uint64_t bit = uint64_t(1) << (dev & 63);
-  if (!(allowed.load(std::memory_order_relaxed) & bit)) {
-    PD_CHECK_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem)));
+  if (!(allowed.load(std::memory_order_relaxed) & bit)) {  // once a device: the call costs a small launch's time
+    PD_CHECK_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, most_smem));
     allowed.fetch_or(bit, std::memory_order_relaxed);
   }
-  kern<<<std::min(p.tiles, num_sms()), kThreads, smem, stream()>>>(ta, tb, tc, p);
-  PD_CHECK_LAUNCH();
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(unsigned(grid));
+  cfg.blockDim = dim3(unsigned(threads));
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream();
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = unsigned(cluster);
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = cluster > 1 ? 2 : 1;
+  PD_CHECK_CUDA(cudaLaunchKernelEx(&cfg, kern, args...));
+  note_launch();
 }
 
 template <typename T>
 void product(const CUtensorMap& ta, const void* B, int64_t Kp, int64_t B_l, const CUtensorMap& tc, Params& p) {
-  auto go = [&](auto bn, auto stages) {
-    constexpr int BN = decltype(bn)::value;
-    p.n_blocks = (p.N + BN - 1) / BN;
-    const int64_t tiles = int64_t(p.L) * p.m_blocks * p.n_blocks;
-    PD_CHECK(tiles < (int64_t(1) << 31), "int8_linear: too many rows");
-    p.tiles = int(tiles);
+  constexpr int kMost = 226 * 1024;
+  const int64_t blocks = int64_t(p.L) * p.m_blocks, sms = num_sms();
+  auto weight = [&](int bn) {
     int mode;
-    const CUtensorMap tb = map_of(CU_TENSOR_MAP_DATA_TYPE_UINT8, B, Kp, p.N, B_l, Kp, Kp * p.N, BK, BN,
-                                  CU_TENSOR_MAP_SWIZZLE_128B, mode);
-    launch<BN, decltype(stages)::value, T>(ta, tb, tc, p);
+    return map_of(CU_TENSOR_MAP_DATA_TYPE_UINT8, B, Kp, p.N, B_l, Kp, Kp * p.N, BK, bn, CU_TENSOR_MAP_SWIZZLE_128B, mode);
   };
-  // The widest tile that still gives every SM one.
-  const int64_t rows = int64_t(p.L) * p.m_blocks, sms = num_sms();
-  constexpr bool two = sizeof(T) == 2;
-  if (rows * ((p.N + 255) / 256) >= sms) go(std::integral_constant<int, 256>(), std::integral_constant<int, two ? 4 : 3>());
-  else if (rows * ((p.N + 127) / 128) >= sms) go(std::integral_constant<int, 128>(), std::integral_constant<int, two ? 6 : 5>());
-  else go(std::integral_constant<int, 64>(), std::integral_constant<int, two ? 8 : 7>());
+  auto count = [&](int bn) {
+    p.n_blocks = (p.N + bn - 1) / bn;
+    const int64_t tiles = blocks * p.n_blocks;
+    PD_CHECK(tiles < (int64_t(1) << 28), "int8_linear: too many rows");
+    p.tiles = int(tiles);
+  };
+  const int64_t narrow = blocks * ((p.N + kSplitN - 1) / kSplitN);
+  if (narrow * 2 <= sms && p.k_blocks >= 2) {             // tiles of 64 columns leave half of the SMs idle: split K
+    count(kSplitN);
+    p.splits = 2;
+    while (p.splits < 8 && narrow * p.splits * 2 <= sms && p.splits * 2 <= p.k_blocks) p.splits *= 2;
+    p.kb_per_split = (p.k_blocks + p.splits - 1) / p.splits;
+    constexpr size_t smem = kSplitStages * size_t(BM + kSplitN) * BK;    // two blocks an SM: clusters of 8 fit everywhere
+    static_assert(smem >= size_t(BM) * kSplitPitch, "room for the sums");
+    static std::atomic<uint64_t> allowed{0};
+    launch_behind(split_kernel<T>, allowed, int(smem), p.tiles * p.splits, kSplitThreads, smem, p.splits, ta, weight(kSplitN), p);
+    return;
+  }
+  // the widest tile that still gives every SM one
+  p.bn = blocks * ((p.N + 255) / 256) >= sms ? 256 : blocks * ((p.N + 127) / 128) >= sms ? 128 : 64;
+  count(p.bn);
+  const int stage = (BM + p.bn) * BK, staging = kEpiWarps * kStageBytes<T>;
+  p.stages = std::min(kMaxStages, (kMost - 5 * 1024 - staging) / stage);
+  static std::atomic<uint64_t> allowed{0};
+  launch_behind(product_kernel<T>, allowed, kMost - 5 * 1024, std::min(p.tiles, int(sms)), kThreads,
+                size_t(p.stages) * stage + staging, 1, ta, weight(p.bn), tc, p);
 }
 
 }  // namespace i8

@@ -88,8 +88,12 @@ __global__ void __launch_bounds__(256) save_kernel(const T* __restrict__ x, int6
         m = max(m, __shfl_xor_sync(0xffffffffu, m, 2));
         const uint32_t b = scale_byte(m);
         if (q == j) mine = b;
-        const float inv = inv_scale(b), most = most_code(b, top);
-        const uint2 c = make_uint2(codes4(f[0], f[1], f[2], f[3], inv, most), codes4(f[4], f[5], f[6], f[7], inv, most));
+        const float inv = inv_scale(b);
+        uint2 c = make_uint2(block_codes4(f, inv), block_codes4(f + 4, inv));
+        if (b >= top) {                                   // no numbers, or codes held to 63: rare
+          const float most = most_code(b, top);
+          c = make_uint2(codes4(f[0], f[1], f[2], f[3], inv, most), codes4(f[4], f[5], f[6], f[7], inv, most));
+        }
         if (there && k < K) *reinterpret_cast<uint2*>(codes + row * K + k) = c;
       }
       if (there && b0 + q < blocks) exps[(b0 + q) * rows + row] = uint8_t(mine);
@@ -145,11 +149,9 @@ __global__ void __launch_bounds__(256) load_kernel(const int8_t* __restrict__ co
       for (int j = 0; j < kBlocks; ++j) {
         const int k = (b0 + j) * kBlock + q * 8;
         float f[8];
-        ints4(c[j].x, f);
-        ints4(c[j].y, f + 4);
         const float s = scale_of(e[j]);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) f[i] *= s;
+        values4(c[j].x, s, f);
+        values4(c[j].y, s, f + 4);
         if (k < K) kv::store_v<8, T>(y + row * K + k, f);
       }
     }
@@ -188,6 +190,7 @@ __global__ void __launch_bounds__(256) rows_kernel(const T* __restrict__ x, int6
                                                    int64_t rows, int64_t K) {
   constexpr int kPer = 256 / TPR;
   __shared__ uint32_t s_most[8];
+  asm volatile("griddepcontrol.launch_dependents;");       // the product may set itself up while this runs
   const int part = threadIdx.x % TPR;
   for (int64_t r0 = int64_t(blockIdx.x) * kPer; r0 < rows; r0 += int64_t(gridDim.x) * kPer) {
     const int64_t row = r0 + threadIdx.x / TPR;
