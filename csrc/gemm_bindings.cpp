@@ -2,6 +2,11 @@
 // pyramid attention (attn_fmha.cu) and the tcgen05 GEMMs (gemm_*.cu).
 #include <torch/extension.h>
 
+#include <ATen/core/dispatch/Dispatcher.h>
+#include <c10/core/DeviceGuard.h>
+
+#include <tuple>
+
 namespace pd {
 std::vector<at::Tensor> fmha_fwd(at::Tensor, at::Tensor, at::Tensor, double, int64_t);
 void fmha_bwd(at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor,
@@ -19,6 +24,194 @@ at::Tensor tc_wgrad_as(at::Tensor, at::Tensor, at::Tensor, bool, int64_t);
 at::Tensor tc_mma_rate(int64_t, int64_t, int64_t, int64_t, int64_t, int64_t, at::Tensor);
 at::Tensor tc_mma_burst(int64_t, int64_t, int64_t, int64_t, int64_t, int64_t, int64_t, int64_t, at::Tensor);
 }  // namespace pd
+
+// Layers that keep their activations in 8 bits. Their nodes are in C++: a step calls a dozen kernels, and a backward in
+// Python would hold the interpreter's lock on the autograd thread between them.
+namespace {
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+using OptTensor = c10::optional<at::Tensor>;
+
+std::tuple<at::Tensor, at::Tensor> save8(const at::Tensor& x) {
+  static auto op = c10::Dispatcher::singleton()
+                       .findSchemaOrThrow("primus_int8::save8", "")
+                       .typed<std::tuple<at::Tensor, at::Tensor>(const at::Tensor&)>();
+  return op.call(x);
+}
+at::Tensor load8(const at::Tensor& codes, const at::Tensor& scale_bytes) {          // exact in bf16
+  static auto op = c10::Dispatcher::singleton()
+                       .findSchemaOrThrow("primus_int8::load8", "")
+                       .typed<at::Tensor(const at::Tensor&, const at::Tensor&, at::ScalarType)>();
+  return op.call(codes, scale_bytes, at::kBFloat16);
+}
+
+// All rows of a [B, T, N] tensor, and its rows from n_s on as one batch for each of them.
+at::Tensor flat(const at::Tensor& t) { return t.reshape({1, t.size(0) * t.size(1), t.size(2)}); }
+at::Tensor tail(const at::Tensor& t, int64_t n_s) { return t.narrow(1, n_s, t.size(1) - n_s).transpose(0, 1); }
+
+constexpr int64_t kEpiNone = 0, kEpiResidual = 2;
+
+// out = x by the shared weight, the rows from n_s on by their own; b_kn: by the weights transposed.
+void mixed(const at::Tensor& x, int64_t n_s, const at::Tensor& ws, const at::Tensor& wn, const at::Tensor& out,
+           const at::Tensor& err, bool b_kn, const OptTensor& residual = c10::nullopt) {
+  const int64_t epi = residual ? kEpiResidual : kEpiNone;
+  pd::tc_gemm(flat(x), ws.unsqueeze(0), flat(out), epi, residual ? OptTensor(flat(*residual)) : residual, c10::nullopt, err,
+              b_kn, c10::nullopt);
+  if (x.size(1) > n_s)
+    pd::tc_gemm(tail(x, n_s), wn, tail(out, n_s), epi, residual ? OptTensor(tail(*residual, n_s)) : residual, c10::nullopt,
+                err, b_kn, c10::nullopt);
+}
+// The same around pre-activations in 8 bits (codes [B T, N], bytes [N / 32, B T]): without aux out = gelu(..) and the codes
+// are written, with it out = .. * gelu'(p), aux = gelu(p).
+void mixed_saved(const at::Tensor& x, int64_t n_s, const at::Tensor& ws, const at::Tensor& wn, const at::Tensor& out,
+                 const at::Tensor& codes, const at::Tensor& bytes, const OptTensor& aux, const at::Tensor& err, bool b_kn) {
+  const int64_t B = x.size(0), T = x.size(1);
+  pd::tc_gemm_saved8(flat(x), ws.unsqueeze(0), flat(out), codes.unsqueeze(0), bytes.t().unsqueeze(0),
+                     aux ? OptTensor(flat(*aux)) : aux, err, b_kn);
+  if (T > n_s)
+    pd::tc_gemm_saved8(tail(x, n_s), wn, tail(out, n_s), tail(codes.view({B, T, codes.size(1)}), n_s),
+                       bytes.view({bytes.size(0), B, T}).narrow(2, n_s, T - n_s).permute({2, 1, 0}),
+                       aux ? OptTensor(tail(*aux, n_s)) : aux, err, b_kn);
+}
+// Gradients of the shared weight (one sum over the samples' rows, read in place) and of the others.
+at::Tensor shared_grad(const at::Tensor& dy, const at::Tensor& x, int64_t n_s, const at::Tensor& err, int64_t type) {
+  if (x.size(1) == n_s) return pd::tc_wgrad_as(flat(dy), flat(x), err, true, type);
+  return pd::tc_wgrad_as(dy.narrow(1, 0, n_s), x.narrow(1, 0, n_s), err, true, type);
+}
+at::Tensor own_grad(const at::Tensor& dy, const at::Tensor& x, int64_t n_s, const at::Tensor& err, int64_t type) {
+  if (x.size(1) == n_s)
+    return at::zeros({0, dy.size(2), x.size(2)}, dy.options().dtype(at::ScalarType(type)));
+  return pd::tc_wgrad_as(tail(dy, n_s), tail(x, n_s), err, false, type);
+}
+
+at::Tensor rows_of(const at::Tensor& t) { return t.view({t.size(0) * t.size(1), t.size(2)}); }
+at::Tensor bf16(const at::Tensor& t) { return t.to(at::kBFloat16); }
+at::Tensor like(const at::Tensor& x, int64_t N) { return at::empty({x.size(0), x.size(1), N}, x.options()); }
+std::tuple<at::Tensor, at::Tensor> room(const at::Tensor& x, int64_t N) {            // codes and scale bytes of [B, T, N]
+  const int64_t rows = x.size(0) * x.size(1);
+  return {at::empty({rows, N}, x.options().dtype(at::kChar)), at::empty({N / 32, rows}, x.options().dtype(at::kByte))};
+}
+void once() {
+  TORCH_CHECK(!at::GradMode::is_enabled(), "a layer with activations in 8 bits is differentiable once (no create_graph)");
+}
+
+struct MixedLinearSaved8 : public torch::autograd::Function<MixedLinearSaved8> {
+  static at::Tensor forward(AutogradContext* ctx, at::Tensor x, at::Tensor w_s, at::Tensor w_ns, int64_t n_s, bool gelu,
+                            at::Tensor err) {
+    const at::Tensor xb = x.contiguous(), ws = bf16(w_s).contiguous(), wn = bf16(w_ns).contiguous();
+    const at::Tensor y = like(xb, ws.size(0));
+    at::Tensor pc, pb;
+    if (gelu) {
+      std::tie(pc, pb) = room(xb, ws.size(0));
+      mixed_saved(xb, n_s, ws, wn, y, pc, pb, c10::nullopt, err, false);
+    } else {
+      mixed(xb, n_s, ws, wn, y, err, false);
+    }
+    auto [xc, xs] = save8(rows_of(xb));
+    ctx->save_for_backward({ws, wn, xc, xs, pc, pb});
+    ctx->saved_data["err"] = err;
+    ctx->saved_data["n_s"] = n_s;
+    ctx->saved_data["ws"] = int64_t(w_s.scalar_type());
+    ctx->saved_data["wn"] = int64_t(w_ns.scalar_type());
+    return y;
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list g) {
+    once();
+    const auto v = ctx->get_saved_variables();
+    const at::Tensor &ws = v[0], &wn = v[1], err = ctx->saved_data["err"].toTensor();
+    const int64_t n_s = ctx->saved_data["n_s"].toInt();
+    at::Tensor dy = bf16(g[0]).contiguous(), dx, dws, dwn;
+    if (v[4].defined()) dy = at::gelu_backward(dy, load8(v[4], v[5]).view(dy.sizes()));
+    if (ctx->needs_input_grad(0)) {
+      dx = like(dy, ws.size(1));
+      mixed(dy, n_s, ws, wn, dx, err, true);
+    }
+    if (ctx->needs_input_grad(1) || ctx->needs_input_grad(2)) {
+      const at::Tensor x = load8(v[2], v[3]).view({dy.size(0), dy.size(1), ws.size(1)});
+      if (ctx->needs_input_grad(1)) dws = shared_grad(dy, x, n_s, err, ctx->saved_data["ws"].toInt());
+      if (ctx->needs_input_grad(2)) dwn = own_grad(dy, x, n_s, err, ctx->saved_data["wn"].toInt());
+    }
+    return {dx, dws, dwn, at::Tensor(), at::Tensor(), at::Tensor()};
+  }
+};
+
+struct MixedFFNSaved8 : public torch::autograd::Function<MixedFFNSaved8> {
+  static at::Tensor forward(AutogradContext* ctx, at::Tensor x, at::Tensor z, at::Tensor w1, at::Tensor w2, at::Tensor wn1,
+                            at::Tensor wn2, int64_t n_s, at::Tensor err) {
+    const at::Tensor xb = x.contiguous();
+    const at::Tensor w[4] = {bf16(w1).contiguous(), bf16(w2).contiguous(), bf16(wn1).contiguous(), bf16(wn2).contiguous()};
+    const at::Tensor h = like(xb, w[0].size(0)), out = like(xb, w[1].size(0));
+    auto [pc, pb] = room(xb, w[0].size(0));
+    mixed_saved(xb, n_s, w[0], w[2], h, pc, pb, c10::nullopt, err, false);
+    mixed(h, n_s, w[1], w[3], out, err, false, z);
+    auto [xc, xs] = save8(rows_of(xb));
+    ctx->save_for_backward({xc, xs, pc, pb, w[0], w[1], w[2], w[3]});
+    ctx->saved_data["err"] = err;
+    ctx->saved_data["n_s"] = n_s;
+    ctx->saved_data["types"] = std::vector<int64_t>{int64_t(w1.scalar_type()), int64_t(w2.scalar_type()),
+                                                    int64_t(wn1.scalar_type()), int64_t(wn2.scalar_type())};
+    return out;
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list g) {
+    once();
+    const auto v = ctx->get_saved_variables();
+    const at::Tensor &w1 = v[4], &w2 = v[5], &wn1 = v[6], &wn2 = v[7], err = ctx->saved_data["err"].toTensor();
+    const int64_t n_s = ctx->saved_data["n_s"].toInt();
+    const auto types = ctx->saved_data["types"].toIntVector();
+    const at::Tensor dy = bf16(g[0]).contiguous();
+    at::Tensor grads[6];
+    if (ctx->needs_input_grad(1)) grads[1] = g[0];
+    const at::Tensor dp = like(dy, w1.size(0));
+    {
+      const at::Tensor h = like(dy, w1.size(0));
+      mixed_saved(dy, n_s, w2, wn2, dp, v[2], v[3], h, err, true);
+      if (ctx->needs_input_grad(3)) grads[3] = shared_grad(dy, h, n_s, err, types[1]);
+      if (ctx->needs_input_grad(5)) grads[5] = own_grad(dy, h, n_s, err, types[3]);
+    }
+    if (ctx->needs_input_grad(0)) {
+      grads[0] = like(dy, w1.size(1));
+      mixed(dp, n_s, w1, wn1, grads[0], err, true);
+    }
+    if (ctx->needs_input_grad(2) || ctx->needs_input_grad(4)) {
+      const at::Tensor x = load8(v[0], v[1]).view({dy.size(0), dy.size(1), w1.size(1)});
+      if (ctx->needs_input_grad(2)) grads[2] = shared_grad(dp, x, n_s, err, types[0]);
+      if (ctx->needs_input_grad(4)) grads[4] = own_grad(dp, x, n_s, err, types[2]);
+    }
+    return {grads[0], grads[1], grads[2], grads[3], grads[4], grads[5], at::Tensor(), at::Tensor()};
+  }
+};
+
+// Forward-mode derivatives do not pass through the kernels: refused, not dropped.
+void no_tangents(std::initializer_list<at::Tensor> ts) {
+  for (const at::Tensor& t : ts)
+    TORCH_CHECK(!t._fw_grad(0).defined(), "a layer with activations in 8 bits has no forward-mode derivative");
+}
+void fits(const at::Tensor& x, int64_t n_s, const at::Tensor& ws, const at::Tensor& wn) {
+  TORCH_CHECK(x.dim() == 3 && x.scalar_type() == at::kBFloat16 && ws.dim() == 2 && wn.dim() == 3 && n_s >= 0 &&
+                  wn.size(0) == x.size(1) - n_s && wn.size(1) == ws.size(0) && wn.size(2) == ws.size(1) &&
+                  ws.size(1) == x.size(2) && ws.device() == x.device() && wn.device() == x.device(),
+              "x [B, T, K] must be bf16, the weights [N, K] and [T - n_s, N, K], on one device");
+}
+
+at::Tensor mixed_linear_saved8(at::Tensor x, at::Tensor w_s, at::Tensor w_ns, int64_t n_s, bool gelu, at::Tensor err) {
+  no_tangents({x, w_s, w_ns});
+  fits(x, n_s, w_s, w_ns);
+  const c10::DeviceGuard guard(x.device());
+  return MixedLinearSaved8::apply(x, w_s, w_ns, n_s, gelu, err);
+}
+at::Tensor mixed_ffn_saved8(at::Tensor x, at::Tensor z, at::Tensor w1, at::Tensor w2, at::Tensor wn1, at::Tensor wn2, int64_t n_s,
+                            at::Tensor err) {
+  no_tangents({x, z, w1, w2, wn1, wn2});
+  fits(x, n_s, w1, wn1);
+  TORCH_CHECK(z.sizes() == x.sizes() && z.scalar_type() == at::kBFloat16 && z.device() == x.device() && w2.dim() == 2 &&
+                  w2.size(0) == w1.size(1) && w2.size(1) == w1.size(0) && wn2.dim() == 3 && wn2.size(0) == wn1.size(0) &&
+                  wn2.size(1) == w2.size(0) && wn2.size(2) == w2.size(1) && w2.device() == x.device() &&
+                  wn2.device() == x.device(),
+              "z must be bf16 of x's shape, the second weights [K, F] and [T - n_s, K, F], on one device");
+  const c10::DeviceGuard guard(x.device());
+  return MixedFFNSaved8::apply(x, z, w1, w2, wn1, wn2, n_s, err);
+}
+}  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.doc() = "primus_dlrm_b200 sm_100a tensor-core kernels";
@@ -39,6 +232,8 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         py::arg("AUX"), py::arg("err"), py::arg("b_kn") = false,
         "the GEMMs around pre-activations in 8 bits (codes int8 [L,M,N], scale bytes [L,M,N/32]): without AUX "
         "C = gelu(A @ B^T) and codes, exps written; with AUX p from codes, C = (A @ B^T) gelu'(p), AUX = gelu(p)");
+  m.def("mixed_linear_saved8", &mixed_linear_saved8, "a mixed projection whose input waits for the backward in 8 bits");
+  m.def("mixed_ffn_saved8", &mixed_ffn_saved8, "a mixed FFN whose input and pre-activation wait for the backward in 8 bits");
   m.def("tc_wgrad", &pd::tc_wgrad, py::arg("A"), py::arg("B"), py::arg("C"), py::arg("err"), py::arg("l_sum") = false,
         "C[l] (fp32, zeroed) += A[l]^T B[l] over rows on tcgen05, split over rows (A [L,K,M], B [L,K,N] bf16 views); "
         "l_sum: one C summed over the batches too");

@@ -899,11 +899,14 @@ void launch(const CUtensorMap& ta, const CUtensorMap& tb, const CUtensorMap& tcm
   constexpr size_t smem = STAGES * (tc::BM * tc::BK * 2 + BN * tc::BK * 2) + 1024 + 1024 +
                           tc::epi_warps(SAVED8) * tc::stage_bufs(SAVED8) * 2048;
   static_assert(smem <= 232448, "GEMM shared memory over the 227 KB per-block limit");
-  static bool attr = false;
-  if (!attr) {
+  static std::atomic<uint64_t> allowed{0};               // by device
+  int dev = 0;
+  PD_CHECK_CUDA(cudaGetDevice(&dev));
+  const uint64_t bit = uint64_t(1) << (dev & 63);
+  if (!(allowed.load(std::memory_order_relaxed) & bit)) {
     PD_CHECK_CUDA(cudaFuncSetAttribute(tc::gemm_kernel<BN, STAGES, SAVED8>,
                                        cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem)));
-    attr = true;
+    allowed.fetch_or(bit, std::memory_order_relaxed);
   }
   int grid = p.tiles < num_sms() ? p.tiles : num_sms();
   tc::gemm_kernel<BN, STAGES, SAVED8><<<grid, tc::threads_of(SAVED8), smem, stream()>>>(ta, tb, tcm, txm, trm, p);

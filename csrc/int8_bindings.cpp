@@ -1,6 +1,8 @@
 // Python bindings of the 8-bit integer kernels (module `_int8`).
 #include <torch/extension.h>
+#include <torch/library.h>
 
+#include <tuple>
 #include <vector>
 
 namespace pd {
@@ -40,4 +42,19 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("linear", &linear, "act(x W^T + bias) + residual by 8-bit integers");
   m.def("error_code", &pd::i8::error_code, "the device's error word (2: a bounded wait ran out)");
   m.def("launch_count", &pd::launches);
+}
+
+// For the layers of the _gemm module, which keep their activations in 8 bits.
+namespace {
+std::tuple<at::Tensor, at::Tensor> save_rows(const at::Tensor& x) {
+  auto v = pd::i8::save8(x);
+  return {v[0], v[1]};
+}
+at::Tensor load_rows(const at::Tensor& codes, const at::Tensor& scale_bytes, at::ScalarType type) {
+  return pd::i8::load8(codes, scale_bytes, int64_t(type));
+}
+}  // namespace
+TORCH_LIBRARY(primus_int8, m) {
+  m.def("save8(Tensor x) -> (Tensor, Tensor)", save_rows);
+  m.def("load8(Tensor codes, Tensor scale_bytes, ScalarType type) -> Tensor", load_rows);
 }

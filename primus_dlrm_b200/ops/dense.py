@@ -206,19 +206,6 @@ class MixedFFNNative(torch.autograd.Function):
         return dx, dout, dw1, dw2, dwn1, dwn2, None
 
 
-def _mixed_saved(x, n_s, ws, wn, out, codes, exps, aux=None, b_kn=False):
-    """:func:`_mixed_tc` around pre-activations in 8 bits (codes [B T, N], exps [N / 32, B T]): without ``aux`` out =
-    gelu(mixed(x)), codes and exps are written; with it out = mixed(x) * gelu'(p), aux = gelu(p), p the codes' values."""
-    B, T, _ = x.shape
-    N, run = out.shape[-1], _ext.gemm().tc_gemm_saved8
-    v = lambda t: t.reshape(1, B * T, t.shape[-1]) if t is not None else None  # noqa: E731
-    run(v(x), ws.unsqueeze(0), v(out), codes.unsqueeze(0), exps.t().unsqueeze(0), v(aux), _err(x.device), b_kn)
-    if T > n_s:
-        tr = lambda t: t[:, n_s:].transpose(0, 1) if t is not None else None  # noqa: E731
-        run(tr(x), wn, tr(out), tr(codes.view(B, T, N)), exps.view(-1, B, T)[:, :, n_s:].permute(2, 1, 0), tr(aux),
-            _err(x.device), b_kn)
-
-
 def _mixed_torch(x, n_s, ws, wn):
     """Rows of x [B, T, K] by ws [N, K], rows from n_s on by their own wn [NS, N, K]."""
     y = torch.matmul(x, ws.t())
@@ -227,26 +214,8 @@ def _mixed_torch(x, n_s, ws, wn):
     return y
 
 
-def _dw_parts(dy, x, n_s, wdt):
-    """Weight gradients of a mixed projection, S and NS rows apart, in the weights' types (tcgen05)."""
-    B, T, N = dy.shape
-    K, run = x.shape[-1], _ext.gemm().tc_wgrad_as
-    err = _err(dy.device)
-    tr = lambda t: t[:, n_s:].transpose(0, 1)  # noqa: E731
-    dwn = run(tr(dy), tr(x), err, False, wdt[1]) if T > n_s else torch.zeros(0, N, K, dtype=wdt[1], device=dy.device)
-    if T == n_s:
-        dws = run(dy.reshape(1, -1, N), x.reshape(1, -1, K), err, True, wdt[0])
-    else:                                                    # one sum over the samples' S rows, read in place
-        dws = run(dy[:, :n_s], x[:, :n_s], err, True, wdt[0])
-    return dws, dwn
-
-
 def _dw_torch(dy, x, n_s, wdt):
     """Weight gradients of :func:`_mixed_torch`."""
-    if x.is_cuda and _wgrad_ok(dy, dy.shape[-1], x.shape[-1]) and _gemm_ok(x):
-        return _dw_parts(dy, x, n_s, wdt)
-    if x.is_cuda and x.dtype == torch.bfloat16:
-        return _dw(dy, x, n_s, wdt)
     dws = torch.matmul(dy[:, :n_s].reshape(-1, dy.shape[-1]).t(), x[:, :n_s].reshape(-1, x.shape[-1]))
     return dws.to(wdt[0]), torch.einsum("btn,btk->tnk", dy[:, n_s:], x[:, n_s:]).to(wdt[1])
 
@@ -266,58 +235,32 @@ def _ffn_forward(x, z, w1, w2, wn1, wn2, n_s: int):
 
 
 class _MixedFFNSaved8(torch.autograd.Function):
-    """:class:`MixedFFNNative` with its input x and pre-activation p kept in 8
-    bits.  The up projection's epilogue writes p's codes beside GELU(p); the down
-    projection's data-gradient GEMM turns them into the factor GELU'(p) and, for
-    its weight gradient, into GELU(p) again; x comes back as bf16, exactly, for
-    the up projection's weight gradient."""
+    """:func:`mixed_ffn` with ``save8`` where the native GEMM cannot run it: the formulas of the native layer
+    (``_gemm.mixed_ffn_saved8``) in PyTorch."""
 
     @staticmethod
     def forward(ctx, x, z, w1, w2, wn1, wn2, n_s: int):
+        bw = [w.to(x.dtype) for w in (w1, w2, wn1, wn2)]
         D, F_ = w2.shape[0], w1.shape[0]
-        native = _ffn_native_ok(x, z, D, F_)
-        xb = x.contiguous()
-        bw = [w.to(xb.dtype) for w in (w1, w2, wn1, wn2)]
-        B, T, _ = xb.shape
-        if native:
-            h = torch.empty(B, T, F_, dtype=xb.dtype, device=x.device)
-            codes = torch.empty(B * T, F_, dtype=torch.int8, device=x.device)
-            exps = torch.empty(F_ // 32, B * T, dtype=torch.uint8, device=x.device)
-            _mixed_saved(xb, n_s, bw[0], bw[2], h, codes, exps)
-            out = torch.empty(B, T, D, dtype=xb.dtype, device=x.device)
-            _mixed_tc(h, n_s, bw[1], bw[3], out, "residual", R=z)
-        else:
-            with _no_autocast(x):
-                p = _mixed_torch(xb, n_s, bw[0], bw[2])
-                out = z + _mixed_torch(F.gelu(p), n_s, bw[1], bw[3])
-                codes, exps = save_rows(p.view(B * T, F_))
-        ctx.save_for_backward(*save_rows(xb.view(B * T, D)), codes, exps, *bw)
-        ctx.meta = (native, n_s, x.shape, x.dtype, z.dtype, [w.dtype for w in (w1, w2, wn1, wn2)])
+        with _no_autocast(x):
+            p = _mixed_torch(x, n_s, bw[0], bw[2])
+            out = z + _mixed_torch(F.gelu(p), n_s, bw[1], bw[3])
+        ctx.save_for_backward(*save_rows(x.reshape(-1, D)), *save_rows(p.view(-1, F_)), *bw)
+        ctx.meta = (n_s, x.shape, x.dtype, z.dtype, [w.dtype for w in (w1, w2, wn1, wn2)])
         return out
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dout):
-        xc, xe, codes, exps, w1, w2, wn1, wn2 = ctx.saved_tensors
-        native, n_s, (B, T, D), dt, zdt, wdt = ctx.meta
-        F_ = w1.shape[0]
-        d = dout.contiguous().to(dt)
+        xc, xe, pc, pe, w1, w2, wn1, wn2 = ctx.saved_tensors
+        n_s, shape, dt, zdt, wdt = ctx.meta
+        d = dout.to(dt)
         with _no_autocast(d):
-            if native:
-                dpre = torch.empty(B, T, F_, dtype=dt, device=d.device)
-                h = torch.empty_like(dpre)
-                _mixed_saved(d, n_s, w2, wn2, dpre, codes, exps, aux=h, b_kn=True)
-            else:
-                p = load_rows(codes, exps, dt).view(B, T, F_)
-                h = F.gelu(p)
-                dpre = torch.ops.aten.gelu_backward(_mixed_torch(d, n_s, w2.t(), wn2.transpose(1, 2)), p)
-            dw2, dwn2 = _dw_torch(d, h, n_s, (wdt[1], wdt[3]))
-            del h
-            if native:
-                dx = _mixed_tc(dpre, n_s, w1, wn1, torch.empty(B, T, D, dtype=dt, device=d.device), b_kn=True)
-            else:
-                dx = _mixed_torch(dpre, n_s, w1.t(), wn1.transpose(1, 2))
-            dw1, dwn1 = _dw_torch(dpre, load_rows(xc, xe, dt).view(B, T, D), n_s, (wdt[0], wdt[2]))
+            p = load_rows(pc, pe, dt).view(*shape[:2], -1)
+            dpre = torch.ops.aten.gelu_backward(_mixed_torch(d, n_s, w2.t(), wn2.transpose(1, 2)), p)
+            dw2, dwn2 = _dw_torch(d, F.gelu(p), n_s, (wdt[1], wdt[3]))
+            dx = _mixed_torch(dpre, n_s, w1.t(), wn1.transpose(1, 2))
+            dw1, dwn1 = _dw_torch(dpre, load_rows(xc, xe, dt).view(shape), n_s, (wdt[0], wdt[2]))
         return dx, dout.to(zdt), dw1, dw2, dwn1, dwn2, None
 
 
@@ -336,9 +279,12 @@ def mixed_ffn(x: torch.Tensor, z: torch.Tensor, n_s: int, w1, w2, wn1, wn2, save
     for every input (through PyTorch where the native GEMM cannot), never None.
     """
     if save8:
-        if torch.is_grad_enabled() and any(t.requires_grad for t in (x, z, w1, w2, wn1, wn2)):
-            return _MixedFFNSaved8.apply(x, z, w1, w2, wn1, wn2, n_s)
-        return _ffn_forward(x, z, w1, w2, wn1, wn2, n_s)
+        if not (torch.is_grad_enabled() and any(t.requires_grad for t in (x, z, w1, w2, wn1, wn2))):
+            return _ffn_forward(x, z, w1, w2, wn1, wn2, n_s)
+        if _ffn_native_ok(x, z, w2.shape[0], w1.shape[0]):
+            _ext.int8()                                      # its kernels save and load
+            return _ext.gemm().mixed_ffn_saved8(x, z, w1, w2, wn1, wn2, n_s, _err(x.device))
+        return _MixedFFNSaved8.apply(x, z, w1, w2, wn1, wn2, n_s)
     if not _ffn_native_ok(x, z, w2.shape[0], w1.shape[0]):
         return None
     return MixedFFNNative.apply(x, z, w1, w2, wn1, wn2, n_s)
@@ -387,49 +333,33 @@ class _MixedLinearTorch(torch.autograd.Function):
 
 
 class _MixedLinearSaved8(torch.autograd.Function):
-    """The mixed projection with its input (and, before a GELU, its
-    pre-activation) kept in 8 bits for the backward pass."""
+    """:func:`mixed_linear` with ``save8`` where the native GEMM cannot run it: the formulas of the native layer
+    (``_gemm.mixed_linear_saved8``) in PyTorch."""
 
     @staticmethod
     def forward(ctx, x, w_s, w_ns, n_s: int, act: str):
-        K, N = x.shape[-1], w_s.shape[0]
-        native = _gemm_ok(x) and _tc_ok(x, K, N) and K % 64 == 0
-        xb = x.contiguous()
-        ws, wn = w_s.to(xb.dtype), w_ns.to(xb.dtype)
-        B, T, _ = xb.shape
+        ws, wn = w_s.to(x.dtype), w_ns.to(x.dtype)
         kept = ()
-        if native:
-            y = torch.empty(B, T, N, dtype=xb.dtype, device=x.device)
+        with _no_autocast(x):
+            y = _mixed_torch(x, n_s, ws, wn)
             if act == "gelu":
-                kept = (torch.empty(B * T, N, dtype=torch.int8, device=x.device),
-                        torch.empty(N // 32, B * T, dtype=torch.uint8, device=x.device))
-                _mixed_saved(xb, n_s, ws, wn, y, *kept)
-            else:
-                _mixed_tc(xb, n_s, ws, wn, y)
-        else:
-            with _no_autocast(x):
-                y = _mixed_torch(xb, n_s, ws, wn)
-                if act == "gelu":
-                    kept = save_rows(y.view(B * T, N))
-                    y = F.gelu(y)
-        ctx.save_for_backward(ws, wn, *save_rows(xb.view(B * T, K)), *kept)
-        ctx.meta = (native, n_s, x.shape, x.dtype, (w_s.dtype, w_ns.dtype))
+                kept = save_rows(y.view(-1, y.shape[-1]))
+                y = F.gelu(y)
+        ctx.save_for_backward(ws, wn, *save_rows(x.reshape(-1, x.shape[-1])), *kept)
+        ctx.meta = (n_s, x.shape, x.dtype, (w_s.dtype, w_ns.dtype))
         return y
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
         ws, wn, xc, xe, *kept = ctx.saved_tensors
-        native, n_s, (B, T, K), dt, wdt = ctx.meta
-        d = dy.contiguous().to(dt)
+        n_s, shape, dt, wdt = ctx.meta
+        d = dy.to(dt)
         with _no_autocast(d):
             if kept:
                 d = torch.ops.aten.gelu_backward(d, load_rows(*kept, dt).view(d.shape))
-            if native:
-                dx = _mixed_tc(d, n_s, ws, wn, torch.empty(B, T, K, dtype=dt, device=d.device), b_kn=True)
-            else:
-                dx = _mixed_torch(d, n_s, ws.t(), wn.transpose(1, 2))
-            dws, dwn = _dw_torch(d, load_rows(xc, xe, dt).view(B, T, K), n_s, wdt)
+            dx = _mixed_torch(d, n_s, ws.t(), wn.transpose(1, 2))
+            dws, dwn = _dw_torch(d, load_rows(xc, xe, dt).view(shape), n_s, wdt)
         return dx, dws, dwn, None, None
 
 
@@ -442,6 +372,9 @@ def mixed_linear(x: torch.Tensor, n_s: int, w_s: torch.Tensor, w_ns: torch.Tenso
     gradient are the same (with a GELU its derivative is taken at the 8-bit
     values), the weights' gradients carry the rounding of the 8-bit input."""
     if save8 and torch.is_grad_enabled() and any(t.requires_grad for t in (x, w_s, w_ns)):
+        if _gemm_ok(x) and _tc_ok(x, x.shape[-1], w_s.shape[0]) and x.shape[-1] % 64 == 0:
+            _ext.int8()                                      # its kernels save and load
+            return _ext.gemm().mixed_linear_saved8(x, w_s, w_ns, n_s, act == "gelu", _err(x.device))
         return _MixedLinearSaved8.apply(x, w_s, w_ns, n_s, act or "")
     if _gemm_ok(x) and _tc_ok(x, x.shape[-1], w_s.shape[0]):
         return _MixedLinearNative.apply(x, w_s, w_ns, n_s, act or "")

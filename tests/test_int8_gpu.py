@@ -238,6 +238,19 @@ def _within(got, ref, tol, what):
     assert not got.numel() or bad.max() <= 1, (what, bad.max().item())
 
 
+def _kept(f):
+    """(f(), the 8-bit tensors that it keeps for its backward pass, in order)."""
+    kept = []
+
+    def keep(t):
+        if t.dtype in (torch.int8, torch.uint8):
+            kept.append(t.detach())
+        return t
+
+    with torch.autograd.graph.saved_tensors_hooks(keep, lambda t: t):
+        return f(), kept
+
+
 SIZES = [(1, 1, 64, 64, 0), (2, 9, 64, 128, 3), (3, 130, 128, 320, 0), (5, 70, 256, 1024, 16), (1, 300, 192, 768, 8)]
 
 
@@ -246,11 +259,10 @@ SIZES = [(1, 1, 64, 64, 0), (2, 9, 64, 128, 3), (3, 130, 128, 320, 0), (5, 70, 2
 def test_ffn(B, T, D, F, NS, wdtype):
     parts = [t.requires_grad_() for t in _parts(B, T, D, F, NS, wdtype=wdtype)]
     n_s = T - NS
-    out = dense.mixed_ffn(parts[0], parts[1], n_s, *parts[2:], save8=True)
+    out, (xc, xe, pc, pe) = _kept(lambda: dense.mixed_ffn(parts[0], parts[1], n_s, *parts[2:], save8=True))
     assert torch.equal(out, dense.mixed_ffn(parts[0], parts[1], n_s, *parts[2:]))
     with torch.no_grad():
         assert torch.equal(out, dense.mixed_ffn(parts[0], parts[1], n_s, *parts[2:], save8=True))
-    xc, xe, pc, pe = out.grad_fn.saved_tensors[:4]
     assert xc.dtype == pc.dtype == torch.int8 and torch.equal(xc, save8(parts[0])._codes)
     d = [t.detach().bfloat16().double() for t in parts]
     p = _mixed64(d[0], n_s, d[2], d[4]).view(B * T, F)
@@ -296,15 +308,14 @@ def test_ffn(B, T, D, F, NS, wdtype):
 def test_projection(B, T, D, F, NS, act):
     x, _, w, _, wn, _ = (t.requires_grad_() for t in _parts(B, T, D, F, NS, seed=1))
     n_s = T - NS
-    y = dense.mixed_linear(x, n_s, w, wn, act=act, save8=True)
-    assert torch.equal(y, dense.mixed_linear(x, n_s, w, wn, act=act))
+    y, kept = _kept(lambda: dense.mixed_linear(x, n_s, w, wn, act=act, save8=True))
+    assert torch.equal(y, dense.mixed_linear(x, n_s, w, wn, act=act)) and len(kept) == (4 if act else 2)
     dy = torch.randn(y.shape, generator=_gen(2), device=DEV).bfloat16()
-    kept = y.grad_fn.saved_tensors[4:]
     grads = torch.autograd.grad(y, (x, w, wn), dy)
     xs = load8(save8(x)).double()
     dp, e_dp = dy.double(), 0 * dy.double()
     if act == "gelu":
-        ps = _load_ref(*kept, torch.float32).double().view(B, T, F)
+        ps = _load_ref(*kept[2:], torch.float32).double().view(B, T, F)
         slope = torch.special.ndtr(ps) + ps * torch.exp(-ps * ps / 2) / math.sqrt(2 * math.pi)
         dp = dp * slope
         e_dp = 2.0 ** -8 * dp.abs() + 1e-5 * dy.double().abs()
@@ -317,6 +328,33 @@ def test_projection(B, T, D, F, NS, act):
     sw = sw + 2 * swn.sum(0) + n * swn.abs().sum(0) + 2.0 ** -22 * _grads64(dp.abs(), xs.abs(), n_s)[1].sum(0)
     _within(grads[1], dw, sw + 2.0 ** -23 * dw.abs(), "w")
     _within(grads[2], dwn, swn + 2.0 ** -23 * dwn.abs(), "wn")
+
+
+def test_layer_refusals():
+    from torch.autograd import forward_ad
+    x, z, w1, w2, wn1, wn2 = (t.requires_grad_() for t in _parts(2, 7, 64, 128, 3))
+    n = lambda t: torch.zeros_like(t)[1:]  # noqa: E731
+    for bad in (lambda: dense.mixed_linear(x, 4, w1, n(wn1), save8=True), lambda: dense.mixed_linear(x, 3, w1, wn1, save8=True),
+                lambda: dense.mixed_linear(x, 8, w1, wn1[:0], save8=True),
+                lambda: dense.mixed_ffn(x, z[:, :6], 4, w1, w2, wn1, wn2, save8=True),
+                lambda: dense.mixed_ffn(x, z, 4, w1, w2, wn1, n(wn2), save8=True),
+                lambda: dense.mixed_ffn(x, z, 4, w1, w2[:, :64], wn1, wn2[:, :, :64], save8=True),
+                lambda: dense.mixed_ffn(x, z, 4, w1, w2.cpu(), wn1, wn2, save8=True)):
+        with pytest.raises(RuntimeError):
+            bad()
+    y = dense.mixed_linear(x, 4, w1, wn1, save8=True)
+    with pytest.raises(RuntimeError, match="once"):
+        torch.autograd.grad(y.sum(), x, create_graph=True)
+    with forward_ad.dual_level(), pytest.raises(RuntimeError, match="forward-mode"):
+        dense.mixed_linear(forward_ad.make_dual(x.detach(), x.detach()), 4, w1, wn1, save8=True)
+    # gradients of some inputs only
+    frozen = [t.detach() for t in (w1, w2, wn1, wn2)]
+    out = dense.mixed_ffn(x, z, 4, *frozen, save8=True)
+    full = dense.mixed_ffn(x, z, 4, w1, w2, wn1, wn2, save8=True)
+    (dx,), (dx2, dw) = (torch.autograd.grad(o.sum(), i) for o, i in ((out, (x,)), (full, (x, w1))))
+    assert torch.equal(dx, dx2) and dw.shape == w1.shape
+    empty = dense.mixed_ffn(x[:0], z[:0], 4, w1, w2, wn1, wn2, save8=True)
+    assert empty.shape == (0, 7, 64)
 
 
 def test_layers_that_the_gemm_cannot_run():
