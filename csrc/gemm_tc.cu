@@ -149,6 +149,8 @@ __global__ void __launch_bounds__(threads_of(SAVED8), 1) gemm_kernel(const __gri
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
+  wait_for_launch_before();
+  let_next_launch();
 
   if (warp == 0) {
     // ---------------- TMA producer ----------------
@@ -658,6 +660,8 @@ __global__ void __launch_bounds__(kThreads, 1) wgrad_kernel(const __grid_constan
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
+  wait_for_launch_before();
+  let_next_launch();
 
   if (warp == 0) {
     // ---------------- TMA producer: [64 k-rows][64 cols] boxes ----------------
@@ -909,8 +913,8 @@ void launch(const CUtensorMap& ta, const CUtensorMap& tb, const CUtensorMap& tcm
     allowed.fetch_or(bit, std::memory_order_relaxed);
   }
   int grid = p.tiles < num_sms() ? p.tiles : num_sms();
-  tc::gemm_kernel<BN, STAGES, SAVED8><<<grid, tc::threads_of(SAVED8), smem, stream()>>>(ta, tb, tcm, txm, trm, p);
-  PD_CHECK_LAUNCH();
+  tc::launch_behind(tc::gemm_kernel<BN, STAGES, SAVED8>, dim3(unsigned(grid)), tc::threads_of(SAVED8), smem, ta, tb, tcm, txm,
+                    trm, p);
 }
 
 }  // namespace
@@ -1087,7 +1091,7 @@ void run_wgrad(const at::Tensor& A, const at::Tensor& B, const at::Tensor& C, tc
     const size_t smem = size_t(stages) * (tc::BM * tc::BK * 2 + bn * tc::BK * 2) + 1024 + 1024;
     PD_CHECK_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem)));
     const int grid = p.items < num_sms() ? p.items : num_sms();
-    kern<<<grid, tc::kThreads, smem, stream()>>>(ta, tb, p);
+    tc::launch_behind(kern, dim3(unsigned(grid)), tc::kThreads, smem, ta, tb, p);
   };
   auto by_width = [&](auto* tag) {
     using Out = std::remove_pointer_t<decltype(tag)>;
@@ -1098,7 +1102,6 @@ void run_wgrad(const at::Tensor& A, const at::Tensor& B, const at::Tensor& C, tc
   if (!direct) by_width(static_cast<void*>(nullptr));
   else if (C.scalar_type() == at::kFloat) by_width(static_cast<float*>(nullptr));
   else by_width(static_cast<__nv_bfloat16*>(nullptr));
-  PD_CHECK_LAUNCH();
 }
 
 }  // namespace

@@ -2,6 +2,8 @@
 #include <torch/extension.h>
 #include <torch/library.h>
 
+#include <cstdlib>
+#include <cstring>
 #include <tuple>
 #include <vector>
 
@@ -25,11 +27,33 @@ void no_tangent(const OptTensor& t, const char* who) {
   TORCH_CHECK(!t.has_value() || !t->_fw_grad(0).defined(), who, " has no forward-mode derivative");
 }
 
-at::Tensor linear(at::Tensor x, at::Tensor codes, at::Tensor scale, int64_t K, bool grouped, OptTensor bias, int64_t act,
-                  OptTensor residual) {
-  for (const OptTensor& t : {OptTensor(x), bias, residual}) no_tangent(t, "int8_linear");
+at::Tensor product(const at::Tensor& x, const at::Tensor& codes, const at::Tensor& scale, int64_t K, bool grouped,
+                   const OptTensor& bias, int64_t act, const OptTensor& residual) {
   const at::NoGradGuard none;                     // the conversions inside make no graph
   return pd::i8::linear(x, codes, scale, K, grouped, bias, act, residual);
+}
+// A product of integers has no gradient: an output of inputs that require one says so where it is asked for.
+struct NoGradient : public torch::autograd::Function<NoGradient> {
+  static at::Tensor forward(torch::autograd::AutogradContext*, at::Tensor x, at::Tensor codes, at::Tensor scale, int64_t K,
+                            bool grouped, OptTensor bias, int64_t act, OptTensor residual) {
+    return product(x, codes, scale, K, grouped, bias, act, residual);
+  }
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext*, torch::autograd::variable_list) {
+    TORCH_CHECK(false, "int8_linear has no gradient: call it under no_grad, or with detached inputs");
+  }
+};
+// None where the eager form is asked for.
+OptTensor linear(const at::Tensor& x, const at::Tensor& codes, const at::Tensor& scale, int64_t K, bool grouped,
+                 const OptTensor& bias, int64_t act, const OptTensor& residual) {
+  const char* kernels = std::getenv("PD_KERNELS");
+  if (kernels != nullptr && std::strcmp(kernels, "eager") == 0) return c10::nullopt;
+  no_tangent(x, "int8_linear");
+  no_tangent(bias, "int8_linear");
+  no_tangent(residual, "int8_linear");
+  auto asks = [](const OptTensor& t) { return t.has_value() && t->requires_grad(); };
+  if (at::GradMode::is_enabled() && (x.requires_grad() || asks(bias) || asks(residual)))
+    return NoGradient::apply(x, codes, scale, K, grouped, bias, act, residual);
+  return product(x, codes, scale, K, grouped, bias, act, residual);
 }
 }  // namespace
 

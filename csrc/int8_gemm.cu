@@ -2,12 +2,15 @@
 #include "int8_few.cuh"
 #include "int8_gemm.cuh"
 
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
+#include <c10/util/SmallVector.h>
 
 namespace pd {
 namespace i8 {
 
-void quantize_into(const at::Tensor& x, int8_t* codes, int64_t pitch, float* scale);
+void quantize_into(const void* x, int dtype, int64_t outer, int64_t inner, int64_t K, int64_t so, int64_t si, int8_t* codes,
+                   int64_t pitch, float* scale);
 extern template void product<__nv_bfloat16>(const CUtensorMap&, const void*, int64_t, int64_t, const CUtensorMap&, Params&);
 extern template void product<__half>(const CUtensorMap&, const void*, int64_t, int64_t, const CUtensorMap&, Params&);
 extern template void product<float>(const CUtensorMap&, const void*, int64_t, int64_t, const CUtensorMap&, Params&);
@@ -34,6 +37,23 @@ int64_t error_code(int64_t device) {
   return v;
 }
 
+// Rows of a [..., K] tensor (or [..., L, K]) as they lie: row m of position l at `at` + m * outer + l * inner elements.
+struct Rows {
+  const void* at;
+  int64_t outer, inner;
+  at::Tensor held;                                        // where they had to be laid out anew
+};
+static Rows rows_of(at::Tensor t, int64_t M, int64_t L, int64_t K, bool grouped) {
+  if (K > 1 && t.stride(-1) != 1) t = t.contiguous();
+  const int64_t lead = t.dim() - (grouped ? 2 : 1);       // dims over rows
+  if (lead > 1 && !t.is_contiguous()) t = t.reshape({M, L, K});
+  const bool plain = lead > 1 && t.is_contiguous();       // the rows follow one another
+  Rows r{t.data_ptr(), 0, 0, t};
+  if (M > 1) r.outer = plain ? L * K : t.stride(0);
+  if (L > 1) r.inner = plain ? K : t.stride(-2);
+  return r;
+}
+
 // x [..., K] or, with a matrix for each of L positions, [..., L, K], by codes [L, N, Kp] (contiguous, zeros from K on)
 // with scales [L, N] -> y [..., N] of x's type.
 at::Tensor linear(at::Tensor x, at::Tensor codes, at::Tensor scale, int64_t K, bool grouped, c10::optional<at::Tensor> bias,
@@ -52,40 +72,37 @@ at::Tensor linear(at::Tensor x, at::Tensor codes, at::Tensor scale, int64_t K, b
   PD_CHECK(x.dim() >= (grouped ? 2 : 1) && x.size(-1) == K && (!grouped || x.size(-2) == L),
            "int8_linear: x does not fit the weight (its last dim is %lld, the weight takes %lld%s)",
            x.dim() ? (long long)x.size(-1) : -1, (long long)K, grouped ? " for each of its positions" : "");
-  std::vector<int64_t> shape = x.sizes().vec();
-  shape.back() = N;
   const c10::cuda::CUDAGuard guard(x.device());
-  at::Tensor y = at::empty(shape, x.options());
-  if (K > 1 && x.stride(-1) != 1) x = x.contiguous();
+  c10::SmallVector<int64_t, 5> shape(x.sizes().begin(), x.sizes().end());
+  shape.back() = N;
+  at::Tensor y = at::detail::empty_cuda(shape, x.scalar_type(), x.device(), c10::nullopt);
   const int64_t M = x.numel() / (L * K);
-  x = x.reshape({M, L, K});
   PD_CHECK(M < (int64_t(1) << 31) && M * L < (int64_t(1) << 40), "int8_linear: too many rows");
+  const Rows xr = rows_of(x, M, L, K, grouped);
   Params p{};
+  Rows rr{};
   if (bias) {
     PD_CHECK(bias->device() == x.device() && bias->is_floating_point() && bias->dim() == 1 && bias->size(0) == N,
              "int8_linear: bias must be [N] of a floating type on x's device");
-    bias = bias->to(at::kFloat).contiguous();
+    if (bias->scalar_type() != at::kFloat || !bias->is_contiguous()) bias = bias->to(at::kFloat).contiguous();
     p.bias = bias->data_ptr<float>();
   }
   if (residual) {
     PD_CHECK(residual->device() == x.device() && residual->scalar_type() == x.scalar_type() && residual->sizes() == y.sizes(),
              "int8_linear: residual must have the result's shape and x's type, on x's device");
-    if (N > 1 && residual->stride(-1) != 1) residual = residual->contiguous();
-    residual = residual->reshape({M, L, N});
+    rr = rows_of(*residual, M, L, N, grouped);
   }
   if (M == 0) return y;
 
   const int64_t size = y.element_size();
-  const int64_t r_ls = residual && L > 1 ? residual->stride(1) : 0, r_ms = residual && M > 1 ? residual->stride(0) : 0;
   if (M <= kFewRows && few_bytes(M, Kp) <= kFewBytes && L <= 65535) {
     FewParams f{};
     f.M = int(M); f.N = int(N); f.L = int(L); f.K = int(K); f.Kp = int(Kp);
-    f.x = x.data_ptr();
-    f.x_outer = M > 1 ? x.stride(0) : 0; f.x_inner = L > 1 ? x.stride(1) : 0;
+    f.x = xr.at; f.x_outer = xr.outer; f.x_inner = xr.inner;
     f.W = codes.data_ptr<int8_t>();
     f.t = scale.data_ptr<float>();
     f.bias = p.bias;
-    f.R_ = residual ? residual->data_ptr() : nullptr; f.r_ls = r_ls; f.r_ms = r_ms;
+    f.R_ = rr.at; f.r_ls = rr.inner; f.r_ms = rr.outer;
     f.C = y.data_ptr(); f.c_ls = N; f.c_ms = N * L;
     f.act = int(act);
     few(f, dtype, K % 8 == 0 && reinterpret_cast<uintptr_t>(f.x) % 16 == 0 && f.x_outer * size % 16 == 0 &&
@@ -93,9 +110,9 @@ at::Tensor linear(at::Tensor x, at::Tensor codes, at::Tensor scale, int64_t K, b
     return y;
   }
 
-  at::Tensor a = at::empty({M * L, Kp}, codes.options());
-  at::Tensor s = at::empty({M * L}, scale.options());
-  quantize_into(x, a.data_ptr<int8_t>(), Kp, s.data_ptr<float>());
+  at::Tensor a = at::detail::empty_cuda({M * L, Kp}, at::kChar, x.device(), c10::nullopt);
+  at::Tensor s = at::detail::empty_cuda({M * L}, at::kFloat, x.device(), c10::nullopt);
+  quantize_into(xr.at, dtype, M, L, K, xr.outer, xr.inner, a.data_ptr<int8_t>(), Kp, s.data_ptr<float>());
 
   p.M = int(M); p.N = int(N); p.L = int(L);
   p.m_blocks = int((M + BM - 1) / BM);
@@ -103,11 +120,8 @@ at::Tensor linear(at::Tensor x, at::Tensor codes, at::Tensor scale, int64_t K, b
   p.s = s.data_ptr<float>(); p.s_ls = 1; p.s_ms = L;
   p.t = scale.data_ptr<float>(); p.t_ls = N;
   p.C = y.data_ptr(); p.c_ls = N; p.c_ms = N * L;
-  if (residual) {
-    p.R = residual->data_ptr();
-    p.r_ls = r_ls; p.r_ms = r_ms;
-    p.r_vec = reinterpret_cast<uintptr_t>(p.R) % 16 == 0 && p.r_ls * size % 16 == 0 && p.r_ms * size % 16 == 0;
-  }
+  p.R = rr.at; p.r_ls = rr.inner; p.r_ms = rr.outer;
+  p.r_vec = reinterpret_cast<uintptr_t>(p.R) % 16 == 0 && p.r_ls * size % 16 == 0 && p.r_ms * size % 16 == 0;
   p.act = int(act);
   p.err = error_word();
   const CUtensorMap ta = map_of(CU_TENSOR_MAP_DATA_TYPE_UINT8, a.data_ptr(), Kp, M, L, Kp * L, Kp, BK, BM,

@@ -118,9 +118,7 @@ __device__ __forceinline__ void tile_at(const Params& p, int w, int& l, int& mb,
   l = r / p.m_blocks;
 }
 
-// The launch before this one (the rows' codes) has finished and its writes are seen. The kernel may have been launched
-// while it ran: what comes before this wait reads nothing that it writes.
-__device__ __forceinline__ void wait_for_launch_before() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+using tcx::wait_for_launch_before;
 
 template <typename T>
 __global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_constant__ CUtensorMap tmA,
@@ -539,7 +537,8 @@ inline CUtensorMap map_of(CUtensorMapDataType type, const void* base, int64_t in
   return m;
 }
 
-// Launch right behind the rows' codes (before they are done: the kernel waits for them itself), as clusters if asked.
+// Launch right behind the rows' codes (before they are done: the kernel waits for them itself), as clusters if asked. The
+// codes' kernel is launched in full order, so that the weight, read before that wait, is complete.
 template <typename... Args>
 void launch_behind(void (*kern)(Args...), std::atomic<uint64_t>& allowed, int most_smem, int grid, int threads, size_t smem,
                    int cluster, Args... args) {

@@ -3,6 +3,7 @@
 // 32-bit scale (quantize_rows, for integer products).
 #include "int8_common.cuh"
 #include "kv_common.cuh"
+#include "tc_common.cuh"
 
 #include <c10/cuda/CUDAGuard.h>
 
@@ -68,6 +69,8 @@ template <typename T>
 __global__ void __launch_bounds__(256) save_kernel(const T* __restrict__ x, int64_t x_stride, int8_t* __restrict__ codes,
                                                    uint8_t* __restrict__ exps, int64_t rows, int K, int blocks,
                                                    uint32_t top) {
+  tc::wait_for_launch_before();
+  tc::let_next_launch();
   const int lane = threadIdx.x & 31, q = lane & 3;
   for (int64_t r0 = (int64_t(blockIdx.x) * 8 + (threadIdx.x >> 5)) * kRows; r0 < rows; r0 += int64_t(gridDim.x) * 8 * kRows) {
     const int64_t row = r0 + (lane >> 2);
@@ -105,6 +108,8 @@ template <typename T>
 __global__ void __launch_bounds__(256) save_any_kernel(const T* __restrict__ x, int64_t x_stride, int8_t* __restrict__ codes,
                                                        uint8_t* __restrict__ exps, int64_t rows, int K, int blocks,
                                                        uint32_t top) {
+  tc::wait_for_launch_before();
+  tc::let_next_launch();
   const int lane = threadIdx.x & 31;
   for (int64_t row = int64_t(blockIdx.x) * 8 + (threadIdx.x >> 5); row < rows; row += int64_t(gridDim.x) * 8) {
     const T* src = x + row * x_stride;
@@ -121,7 +126,8 @@ __global__ void __launch_bounds__(256) save_any_kernel(const T* __restrict__ x, 
         const int k = (b0 + j) * kBlock + lane;
         const uint32_t b = scale_byte(__reduce_max_sync(0xffffffffu, abs_bits(f[j])));
         if (lane == j) mine = b;
-        const uint32_t c = codes4(f[j], 0.0f, 0.0f, 0.0f, inv_scale(b), most_code(b, top));
+        uint32_t c = __float_as_uint(fmaf(f[j], inv_scale(b), 12582912.0f));       // the low byte, as in block_codes4
+        if (b >= top) c = codes4(f[j], 0.0f, 0.0f, 0.0f, inv_scale(b), most_code(b, top));
         if (k < K) codes[row * K + k] = int8_t(c);
       }
       if (lane < kLong && b0 + lane < blocks) exps[(b0 + lane) * rows + row] = uint8_t(mine);
@@ -132,6 +138,8 @@ __global__ void __launch_bounds__(256) save_any_kernel(const T* __restrict__ x, 
 template <typename T>
 __global__ void __launch_bounds__(256) load_kernel(const int8_t* __restrict__ codes, const uint8_t* __restrict__ exps,
                                                    T* __restrict__ y, int64_t rows, int K, int blocks) {
+  tc::wait_for_launch_before();
+  tc::let_next_launch();
   const int lane = threadIdx.x & 31, q = lane & 3;
   for (int64_t r0 = (int64_t(blockIdx.x) * 8 + (threadIdx.x >> 5)) * kRows; r0 < rows; r0 += int64_t(gridDim.x) * 8 * kRows) {
     const int64_t row = r0 + (lane >> 2);
@@ -161,6 +169,8 @@ __global__ void __launch_bounds__(256) load_kernel(const int8_t* __restrict__ co
 template <typename T>
 __global__ void __launch_bounds__(256) load_any_kernel(const int8_t* __restrict__ codes, const uint8_t* __restrict__ exps,
                                                        T* __restrict__ y, int64_t rows, int K, int blocks) {
+  tc::wait_for_launch_before();
+  tc::let_next_launch();
   const int lane = threadIdx.x & 31;
   for (int64_t row = int64_t(blockIdx.x) * 8 + (threadIdx.x >> 5); row < rows; row += int64_t(gridDim.x) * 8) {
     for (int b0 = blockIdx.y * kLong; b0 < blocks; b0 += gridDim.y * kLong) {
@@ -190,7 +200,7 @@ __global__ void __launch_bounds__(256) rows_kernel(const T* __restrict__ x, int6
                                                    int64_t rows, int64_t K) {
   constexpr int kPer = 256 / TPR;
   __shared__ uint32_t s_most[8];
-  asm volatile("griddepcontrol.launch_dependents;");       // the product may set itself up while this runs
+  tc::let_next_launch();                                   // the product may set itself up while this runs
   const int part = threadIdx.x % TPR;
   for (int64_t r0 = int64_t(blockIdx.x) * kPer; r0 < rows; r0 += int64_t(gridDim.x) * kPer) {
     const int64_t row = r0 + threadIdx.x / TPR;
@@ -289,13 +299,12 @@ std::vector<at::Tensor> save8(at::Tensor x) {
     const uint32_t top = dtype == kv::kF16 ? kTopHalf : kTopWide;
     const bool vec = K % 8 == 0 && aligned16(p) && stride * int64_t(sizeof(T)) % 16 == 0;
     if (vec)
-      save_kernel<T><<<pack_grid((rows + 8 * kRows - 1) / (8 * kRows), (blocks + kBlocks - 1) / kBlocks), 256, 0, stream()>>>(
-          p, stride, codes.data_ptr<int8_t>(), exps.data_ptr<uint8_t>(), rows, int(K), int(blocks), top);
+      tc::launch_behind(save_kernel<T>, pack_grid((rows + 8 * kRows - 1) / (8 * kRows), (blocks + kBlocks - 1) / kBlocks), 256, 0,
+                        p, stride, codes.data_ptr<int8_t>(), exps.data_ptr<uint8_t>(), rows, int(K), int(blocks), top);
     else
-      save_any_kernel<T><<<pack_grid((rows + 7) / 8, (blocks + kLong - 1) / kLong), 256, 0, stream()>>>(
-          p, stride, codes.data_ptr<int8_t>(), exps.data_ptr<uint8_t>(), rows, int(K), int(blocks), top);
+      tc::launch_behind(save_any_kernel<T>, pack_grid((rows + 7) / 8, (blocks + kLong - 1) / kLong), 256, 0,
+                        p, stride, codes.data_ptr<int8_t>(), exps.data_ptr<uint8_t>(), rows, int(K), int(blocks), top);
   });
-  PD_CHECK_LAUNCH();
   return {codes, exps};
 }
 
@@ -315,24 +324,24 @@ at::Tensor load8(at::Tensor codes, at::Tensor exps, int64_t dtype) {
     using T = std::remove_pointer_t<decltype(tag)>;
     T* out = static_cast<T*>(y.data_ptr());
     if (K % 8 == 0 && aligned16(codes.data_ptr()))
-      load_kernel<T><<<pack_grid((rows + 8 * kRows - 1) / (8 * kRows), (blocks + kBlocks - 1) / kBlocks), 256, 0, stream()>>>(
-          codes.data_ptr<int8_t>(), exps.data_ptr<uint8_t>(), out, rows, int(K), int(blocks));
+      tc::launch_behind(load_kernel<T>, pack_grid((rows + 8 * kRows - 1) / (8 * kRows), (blocks + kBlocks - 1) / kBlocks), 256, 0,
+                        codes.data_ptr<int8_t>(), exps.data_ptr<uint8_t>(), out, rows, int(K), int(blocks));
     else
-      load_any_kernel<T><<<pack_grid((rows + 7) / 8, (blocks + kLong - 1) / kLong), 256, 0, stream()>>>(
-          codes.data_ptr<int8_t>(), exps.data_ptr<uint8_t>(), out, rows, int(K), int(blocks));
+      tc::launch_behind(load_any_kernel<T>, pack_grid((rows + 7) / 8, (blocks + kLong - 1) / kLong), 256, 0,
+                        codes.data_ptr<int8_t>(), exps.data_ptr<uint8_t>(), out, rows, int(K), int(blocks));
   });
-  PD_CHECK_LAUNCH();
   return y;
 }
 
-// Rows of x [outer, inner, K] into codes (rows of `pitch` bytes) and scale [outer * inner].
-void quantize_into(const at::Tensor& x, int8_t* codes, int64_t pitch, float* scale) {
-  const int64_t outer = x.size(0), inner = x.size(1), K = x.size(2), rows = outer * inner;
+// Rows of x (row `i` of position `l` at x + i * so + l * si elements) into codes (rows of `pitch` bytes) and scales, both in
+// the order [outer, inner].
+void quantize_into(const void* x, int dtype, int64_t outer, int64_t inner, int64_t K, int64_t so, int64_t si, int8_t* codes,
+                   int64_t pitch, float* scale) {
+  const int64_t rows = outer * inner;
   if (rows == 0) return;
-  by_type(kv::dtype_of(x, "quantize_rows"), [&](auto* tag) {
+  by_type(dtype, [&](auto* tag) {
     using T = std::remove_pointer_t<decltype(tag)>;
-    const T* p = static_cast<const T*>(x.data_ptr());
-    const int64_t so = outer == 1 ? 0 : x.stride(0), si = inner == 1 ? 0 : x.stride(1);
+    const T* p = static_cast<const T*>(x);
     const bool vec = K % 8 == 0 && pitch % 8 == 0 && aligned16(p) && so * int64_t(sizeof(T)) % 16 == 0 &&
                      si * int64_t(sizeof(T)) % 16 == 0;
     auto go = [&](auto* kern, int per_block) {
@@ -366,7 +375,9 @@ std::vector<at::Tensor> quantize_rows(at::Tensor x) {
   const c10::cuda::CUDAGuard guard(x.device());
   at::Tensor codes = at::empty(x.sizes(), x.options().dtype(at::kChar));
   at::Tensor scale = at::empty({x.size(0), x.size(1)}, x.options().dtype(at::kFloat));
-  quantize_into(x, codes.data_ptr<int8_t>(), x.size(2), scale.data_ptr<float>());
+  quantize_into(x.data_ptr(), kv::dtype_of(x, "quantize_rows"), x.size(0), x.size(1), x.size(2),
+                x.size(0) > 1 ? x.stride(0) : 0, x.size(1) > 1 ? x.stride(1) : 0, codes.data_ptr<int8_t>(), x.size(2),
+                scale.data_ptr<float>());
   return {codes, scale};
 }
 

@@ -163,5 +163,27 @@ __device__ __forceinline__ void tc_ld32(uint32_t taddr, float* v) {
   for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
 }
 
+// A kernel launched behind another one (launch_behind) may start, and set itself up, while that one still runs: this
+// waits until it has finished and its writes are seen. Before it nothing is read or written that other kernels touch.
+__device__ __forceinline__ void wait_for_launch_before() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+// From here on the next kernel may be set up on SMs that have room.
+__device__ __forceinline__ void let_next_launch() { asm volatile("griddepcontrol.launch_dependents;"); }
+
+template <typename... Args, typename... Given>
+void launch_behind(void (*kern)(Args...), dim3 grid, int threads, size_t smem, const Given&... given) {
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(unsigned(threads));
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream();
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  PD_CHECK_CUDA(cudaLaunchKernelEx(&cfg, kern, static_cast<Args>(given)...));
+  note_launch();
+}
+
 }  // namespace tc
 }  // namespace pd

@@ -148,29 +148,27 @@ def int8_linear(x: torch.Tensor, weight: Int8Weight, bias: torch.Tensor | None =
     ``[..., N]`` and ``x``'s type, which is the result's too.  A gradient asked
     of the result raises in the backward pass.
     """
-    if act not in _ACT:
+    code = _ACT.get(act)
+    if code is None:
         raise ValueError(f"int8_linear: act {act!r}: expected None, 'gelu' or 'relu'")
-    if _native(x):
-        y = _ext.int8().linear(x, weight._codes, weight._scale, weight.in_features, weight.grouped, bias, _ACT[act],
-                               residual)
-    else:
-        if x.dtype not in _TYPES:
-            raise ValueError(f"int8_linear: {x.dtype}: expected bf16, fp16 or fp32")
-        L = weight._codes.shape[0]
-        if x.dim() < 1 + weight.grouped or x.shape[-1] != weight.in_features or (weight.grouped and x.shape[-2] != L):
-            raise ValueError(f"int8_linear: x {tuple(x.shape)} does not fit a weight {tuple(weight.codes.shape)}")
-        shape = (*x.shape[:-1], weight.out_features)
-        if bias is not None and bias.shape != shape[-1:]:
-            raise ValueError("int8_linear: bias must be [N]")
-        if residual is not None and (residual.shape != shape or residual.dtype != x.dtype):
-            raise ValueError("int8_linear: residual must have the result's shape and x's type")
-        with torch.no_grad(), torch.autocast(x.device.type, enabled=False):
-            y = _linear_ref(x, weight, bias, act, residual)
-    if torch.is_grad_enabled():
-        inputs = [t for t in (x, bias, residual) if t is not None and t.requires_grad]
-        if inputs:
-            return _NoGradient.apply(y, *inputs)
-    return y
+    if x.is_cuda:
+        y = _ext.int8().linear(x, weight._codes, weight._scale, weight.in_features, weight.grouped, bias, code, residual)
+        if y is not None:                                    # None: PD_KERNELS=eager
+            return y
+    if x.dtype not in _TYPES:
+        raise ValueError(f"int8_linear: {x.dtype}: expected bf16, fp16 or fp32")
+    L = weight._codes.shape[0]
+    if x.dim() < 1 + weight.grouped or x.shape[-1] != weight.in_features or (weight.grouped and x.shape[-2] != L):
+        raise ValueError(f"int8_linear: x {tuple(x.shape)} does not fit a weight {tuple(weight.codes.shape)}")
+    shape = (*x.shape[:-1], weight.out_features)
+    if bias is not None and bias.shape != shape[-1:]:
+        raise ValueError("int8_linear: bias must be [N]")
+    if residual is not None and (residual.shape != shape or residual.dtype != x.dtype):
+        raise ValueError("int8_linear: residual must have the result's shape and x's type")
+    with torch.no_grad(), torch.autocast(x.device.type, enabled=False):
+        y = _linear_ref(x, weight, bias, act, residual)
+    inputs = [t for t in (x, bias, residual) if t is not None and t.requires_grad] if torch.is_grad_enabled() else []
+    return _NoGradient.apply(y, *inputs) if inputs else y
 
 
 def int8_error_code(device) -> int:
