@@ -11,9 +11,9 @@ namespace i8 {
 
 void quantize_into(const void* x, int dtype, int64_t outer, int64_t inner, int64_t K, int64_t so, int64_t si, int8_t* codes,
                    int64_t pitch, float* scale);
-extern template void product<__nv_bfloat16>(const CUtensorMap&, const void*, int64_t, int64_t, const CUtensorMap&, Params&);
-extern template void product<__half>(const CUtensorMap&, const void*, int64_t, int64_t, const CUtensorMap&, Params&);
-extern template void product<float>(const CUtensorMap&, const void*, int64_t, int64_t, const CUtensorMap&, Params&);
+extern template void product<__nv_bfloat16>(const CUtensorMap&, const void*, int64_t, int64_t, const CUtensorMap&, Params&, at::Device);
+extern template void product<__half>(const CUtensorMap&, const void*, int64_t, int64_t, const CUtensorMap&, Params&, at::Device);
+extern template void product<float>(const CUtensorMap&, const void*, int64_t, int64_t, const CUtensorMap&, Params&, at::Device);
 
 // The kernels' error word on each device: 2 a bounded wait ran out, 4 shared memory not aligned.
 __device__ int g_err;
@@ -134,9 +134,9 @@ at::Tensor linear(at::Tensor x, at::Tensor codes, at::Tensor scale, int64_t K, b
                 p.C, N, M, L, N * L * size, N * size, 32, 32,
                 size == 2 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B, p.c_mode);
   p.b_shared = L == 1;
-  if (dtype == kv::kBf16) product<__nv_bfloat16>(ta, codes.data_ptr(), Kp, L, tc, p);
-  else if (dtype == kv::kF16) product<__half>(ta, codes.data_ptr(), Kp, L, tc, p);
-  else product<float>(ta, codes.data_ptr(), Kp, L, tc, p);
+  if (dtype == kv::kBf16) product<__nv_bfloat16>(ta, codes.data_ptr(), Kp, L, tc, p, x.device());
+  else if (dtype == kv::kF16) product<__half>(ta, codes.data_ptr(), Kp, L, tc, p, x.device());
+  else product<float>(ta, codes.data_ptr(), Kp, L, tc, p, x.device());
   return y;
 }
 

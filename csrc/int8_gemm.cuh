@@ -18,14 +18,17 @@
 //                memory and a TMA store (or row by row, where C's rows do not
 //                lie on 16 bytes)
 // split_kernel is for calls whose tiles leave most SMs idle (few rows, a long
-// axis): a cluster shares a tile and splits K; every block leaves its sums in
-// shared memory, and each takes a part of the rows from all of them.
+// axis): a cluster shares a tile and splits K. Every block writes its sums to a
+// workspace, which stays in L2, and behind the cluster's barrier takes a part of
+// the rows from all of them (out of the others' shared memory the same 32 KB took
+// 3600 cycles a block, and a second barrier).
 #pragma once
 
 #include "int8_common.cuh"
 #include "kv_common.cuh"
 #include "tc_common.cuh"
 
+#include <ATen/cuda/EmptyTensor.h>
 #include <atomic>
 #include <type_traits>
 
@@ -43,13 +46,13 @@ constexpr int kMaxStages = 8;
 constexpr int kSplitN = 64;             // columns of a tile whose K is split
 constexpr int kSplitStages = 4;
 constexpr int kSplitThreads = 192;      // TMA, MMA, four warps of 32 rows
-constexpr int kSplitPitch = 4 * kSplitN + 16;             // bytes of a row of sums: 16-byte stores of 8 rows on all banks
 
 struct Params {
   int M, N, L;
   int m_blocks, n_blocks, k_blocks, tiles;
   int bn, stages;
   int splits, kb_per_split;
+  int* work;                                              // sums of a split tile [tiles][splits][128][64]
   const float* s; int64_t s_ls, s_ms;
   const float* t; int64_t t_ls;
   const float* bias;
@@ -329,26 +332,21 @@ __device__ __forceinline__ void cluster_barrier() {
   asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
   asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
-__device__ __forceinline__ int4 load_cluster(uint32_t addr, uint32_t rank) {
-  uint32_t a;
-  int4 v;
-  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(addr), "r"(rank));
-  asm volatile("ld.shared::cluster.v4.u32 {%0, %1, %2, %3}, [%4];"
-               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a) : "memory");
-  return v;
+__device__ __forceinline__ void store_sector(int* dst, const uint32_t* w) {          // 32 bytes
+  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};"
+               ::"l"(dst), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7]) : "memory");
 }
 
 template <typename T>
 __global__ void __launch_bounds__(kSplitThreads, 1) split_kernel(const __grid_constant__ CUtensorMap tmA,
                                                                  const __grid_constant__ CUtensorMap tmB, const Params p) {
   constexpr uint32_t kA = BM * BK, kB = kSplitN * BK;
-  extern __shared__ __align__(1024) uint8_t ring[];       // A and B tiles; later this block's sums [128][kSplitPitch]
+  extern __shared__ __align__(1024) uint8_t ring[];       // A and B tiles
   __shared__ uint64_t full[kSplitStages], empty[kSplitStages], done;
   __shared__ uint32_t tmem_slot;
   __shared__ volatile int abort_flag;
   uint8_t* sA = ring;
   uint8_t* sB = ring + kSplitStages * kA;
-  uint8_t* sums = ring;                                   // once the products are done with the tiles
   if (tcx::smem_u32(ring) % 1024 != 0) {                  // alike in every block of the cluster
     set_error(p.err, 4);
     return;
@@ -357,6 +355,7 @@ __global__ void __launch_bounds__(kSplitThreads, 1) split_kernel(const __grid_co
   const int rank = blockIdx.x % p.splits;
   int l, mb, nb;
   tile_at(p, blockIdx.x / p.splits, l, mb, nb);
+  int* tile_sums = p.work + int64_t(blockIdx.x / p.splits) * p.splits * (BM * kSplitN);
   const int kb0 = rank * p.kb_per_split, kb1 = min(kb0 + p.kb_per_split, p.k_blocks);
   if (threadIdx.x == 0) {
     for (int s = 0; s < kSplitStages; ++s) { tcx::mbar_init(&full[s], 1); tcx::mbar_init(&empty[s], 1); }
@@ -420,24 +419,29 @@ __global__ void __launch_bounds__(kSplitThreads, 1) split_kernel(const __grid_co
     }
   } else {
     // sums of this block's part of K, 32 rows a warp (TMEM lanes by the warp's place in its group of four)
-    const int q = warp & 3;
-    uint8_t* mine = sums + (q * 32 + lane) * kSplitPitch;
+    const int q = warp & 3, r_tile = q * 32 + lane;
+    const bool there = mb * BM + r_tile < p.M;
+    int* mine = tile_sums + (rank * BM + r_tile) * kSplitN;
     if (kb1 > kb0) {
       (void)tcx::mbar_wait(&done, 0, p.err);
       tcx::tc_fence_after();
+      wait_for_launch_before();                           // the workspace may be the last call's too
 #pragma unroll
       for (int c = 0; c < kSplitN; c += 32) {
         uint32_t r[32];
         tcx::tc_ld32_issue(tmem + (uint32_t(q * 32) << 16) + c, r);
         tcx::tc_ld_wait(r);
+        if (there) {
 #pragma unroll
-        for (int i = 0; i < 32; i += 4)
-          *reinterpret_cast<uint4*>(mine + (c + i) * 4) = make_uint4(r[i], r[i + 1], r[i + 2], r[i + 3]);
+          for (int i = 0; i < 32; i += 8) store_sector(mine + c + i, r + i);
+        }
       }
       tcx::tc_fence_before();
-    } else {
+    } else if (there) {
+      wait_for_launch_before();
+      const uint32_t none[8] = {};
 #pragma unroll
-      for (int i = 0; i < kSplitN; i += 4) *reinterpret_cast<uint4*>(mine + i * 4) = make_uint4(0, 0, 0, 0);
+      for (int i = 0; i < kSplitN; i += 8) store_sector(mine + i, none);
     }
   }
   __syncwarp();
@@ -465,13 +469,13 @@ __global__ void __launch_bounds__(kSplitThreads, 1) split_kernel(const __grid_co
   for (int i = threadIdx.x; i < rows * kUnits; i += kSplitThreads) {
     if (i != threadIdx.x) operands(i);
     if (width <= 0) continue;
-    const uint32_t at = tcx::smem_u32(sums) + (base + i / kUnits) * kSplitPitch + i % kUnits * kWide * 4;
+    const int4* at = reinterpret_cast<const int4*>(tile_sums + (base + i / kUnits) * kSplitN + i % kUnits * kWide);
     int4 part[2][8];
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
       if (k < p.splits) {
-        part[0][k] = load_cluster(at, uint32_t(k));
-        part[1][k] = load_cluster(at + 16, uint32_t(k));
+        part[0][k] = __ldcg(at + k * (BM * kSplitN / 4));
+        part[1][k] = __ldcg(at + k * (BM * kSplitN / 4) + 1);
       }
     }
     float v[kWide];
@@ -508,7 +512,6 @@ __global__ void __launch_bounds__(kSplitThreads, 1) split_kernel(const __grid_co
         if (e < width) out[e] = kv::from_f<T>(v[e]);
     }
   }
-  cluster_barrier();                                      // no block leaves while another reads its sums
   if (warp == 1) {
     tcx::tc_fence_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kSplitN) : "memory");
@@ -567,7 +570,8 @@ void launch_behind(void (*kern)(Args...), std::atomic<uint64_t>& allowed, int mo
 }
 
 template <typename T>
-void product(const CUtensorMap& ta, const void* B, int64_t Kp, int64_t B_l, const CUtensorMap& tc, Params& p) {
+void product(const CUtensorMap& ta, const void* B, int64_t Kp, int64_t B_l, const CUtensorMap& tc, Params& p, at::Device device) {
+  at::Tensor work;                                        // freed behind the launch, on its stream
   constexpr int kMost = 226 * 1024;
   const int64_t blocks = int64_t(p.L) * p.m_blocks, sms = num_sms();
   auto weight = [&](int bn) {
@@ -586,14 +590,20 @@ void product(const CUtensorMap& ta, const void* B, int64_t Kp, int64_t B_l, cons
     p.splits = 2;
     while (p.splits < 8 && narrow * p.splits * 2 <= sms && p.splits * 2 <= p.k_blocks) p.splits *= 2;
     p.kb_per_split = (p.k_blocks + p.splits - 1) / p.splits;
+    work = at::detail::empty_cuda({int64_t(p.tiles) * p.splits * BM * kSplitN}, at::kInt, device, c10::nullopt);
+    p.work = work.data_ptr<int>();
     constexpr size_t smem = kSplitStages * size_t(BM + kSplitN) * BK;    // two blocks an SM: clusters of 8 fit everywhere
-    static_assert(smem >= size_t(BM) * kSplitPitch, "room for the sums");
     static std::atomic<uint64_t> allowed{0};
     launch_behind(split_kernel<T>, allowed, int(smem), p.tiles * p.splits, kSplitThreads, smem, p.splits, ta, weight(kSplitN), p);
     return;
   }
-  // the widest tile that still gives every SM one
-  p.bn = blocks * ((p.N + 255) / 256) >= sms ? 256 : blocks * ((p.N + 127) / 128) >= sms ? 128 : 64;
+  // Waves of tiles, each taking its columns and about 64 more (its start and end): 2069 x 333 -> 1001 takes 6 us in one
+  // wave of 128 columns, 8 in two of 64; 16384 rows by 256 -> 1024 20 us in four of 256, 22 in seven of 128.
+  int64_t best = -1;
+  for (int bn : {256, 128, 64}) {
+    const int64_t waves = (blocks * ((p.N + bn - 1) / bn) + sms - 1) / sms, cost = waves * (bn + 64);
+    if (best < 0 || cost < best) { best = cost; p.bn = bn; }
+  }
   count(p.bn);
   const int stage = (BM + p.bn) * BK, staging = kEpiWarps * kStageBytes<T>;
   p.stages = std::min(kMaxStages, (kMost - 5 * 1024 - staging) / stage);

@@ -3,6 +3,6 @@
 
 namespace pd {
 namespace i8 {
-template void product<float>(const CUtensorMap&, const void*, int64_t, int64_t, const CUtensorMap&, Params&);
+template void product<float>(const CUtensorMap&, const void*, int64_t, int64_t, const CUtensorMap&, Params&, at::Device);
 }  // namespace i8
 }  // namespace pd

@@ -192,12 +192,13 @@ __global__ void __launch_bounds__(256) load_any_kernel(const int8_t* __restrict_
 }
 
 // quantize_rows: TPR threads share a row and keep it in registers between the
-// maximum and the codes (NV vectors of 8 a thread); longer rows are read again.
-// Codes lie in rows of `pitch` bytes, zeros behind a row's end.
+// maximum and the codes (NV vectors of 8 a thread, so that a row's loads are all
+// on their way at once); longer rows are read again. Codes lie in rows of `pitch`
+// bytes, zeros behind a row's end.
 template <bool VEC, int TPR, int NV, typename T>
-__global__ void __launch_bounds__(256) rows_kernel(const T* __restrict__ x, int64_t x_outer, int64_t x_inner, int64_t inner,
+__global__ void __launch_bounds__(256) rows_kernel(const T* __restrict__ x, int64_t x_outer, int64_t x_inner, int inner,
                                                    int8_t* __restrict__ codes, int64_t pitch, float* __restrict__ scale,
-                                                   int64_t rows, int64_t K) {
+                                                   int64_t rows, int K) {
   constexpr int kPer = 256 / TPR;
   __shared__ uint32_t s_most[8];
   tc::let_next_launch();                                   // the product may set itself up while this runs
@@ -205,26 +206,32 @@ __global__ void __launch_bounds__(256) rows_kernel(const T* __restrict__ x, int6
   for (int64_t r0 = int64_t(blockIdx.x) * kPer; r0 < rows; r0 += int64_t(gridDim.x) * kPer) {
     const int64_t row = r0 + threadIdx.x / TPR;
     const bool there = row < rows;
-    const T* src = x + (there ? row / inner * x_outer + row % inner * x_inner : 0);
+    const T* src = x;
+    if (there) src += inner == 1 ? row * x_outer : row / inner * x_outer + row % inner * x_inner;
     Eight<VEC, T> raw[NV];
     uint32_t m = 0;
-    const int64_t len = there ? K : 0;
+    const int len = there ? K : 0;
 #pragma unroll
-    for (int i = 0; i < NV; ++i) raw[i].load(src, (int64_t(i) * TPR + part) * 8, len);
+    for (int i = 0; i < NV; ++i) raw[i].load(src, (i * TPR + part) * 8, len);
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       float f[8];
       raw[i].floats(f);
       m = max(m, most_bits(f));
     }
-    for (int64_t k = int64_t(NV) * TPR * 8 + part * 8; k < len; k += TPR * 8) {
+    for (int k = NV * TPR * 8 + part * 8; k < len; k += TPR * 8) {
       Eight<VEC, T> e;
       float f[8];
       e.load(src, k, len);
       e.floats(f);
       m = max(m, most_bits(f));
     }
-    m = __reduce_max_sync(0xffffffffu, m);
+    if constexpr (TPR < 32) {
+#pragma unroll
+      for (int o = TPR / 2; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
+    } else {
+      m = __reduce_max_sync(0xffffffffu, m);
+    }
     if constexpr (TPR > 32) {
       __syncthreads();                                     // the row before has been read out of s_most
       if ((threadIdx.x & 31) == 0) s_most[threadIdx.x >> 5] = m;
@@ -236,7 +243,7 @@ __global__ void __launch_bounds__(256) rows_kernel(const T* __restrict__ x, int6
     if (!there) continue;
     if (part == 0) scale[row] = sc.scale;
     int8_t* dst = codes + row * pitch;
-    auto put = [&](const float* f, int64_t k) {
+    auto put = [&](const float* f, int k) {
       store_codes<VEC>(dst, k, pitch, make_uint2(codes4(f[0], f[1], f[2], f[3], sc.inv, sc.most),
                                                  codes4(f[4], f[5], f[6], f[7], sc.inv, sc.most)));
     };
@@ -244,15 +251,48 @@ __global__ void __launch_bounds__(256) rows_kernel(const T* __restrict__ x, int6
     for (int i = 0; i < NV; ++i) {
       float f[8];
       raw[i].floats(f);
-      put(f, (int64_t(i) * TPR + part) * 8);
+      put(f, (i * TPR + part) * 8);
     }
-    for (int64_t k = int64_t(NV) * TPR * 8 + part * 8; k < pitch; k += TPR * 8) {
+    for (int k = NV * TPR * 8 + part * 8; k < pitch; k += TPR * 8) {
       Eight<VEC, T> e;
       float f[8];
       e.load(src, k, len);
       e.floats(f);
       put(f, k);
     }
+  }
+}
+
+// A lane an element, for rows of any alignment: whole runs of 32 values a load, 8 of them on their way.
+template <typename T>
+__global__ void __launch_bounds__(256) rows_any_kernel(const T* __restrict__ x, int64_t x_outer, int64_t x_inner, int inner,
+                                                       int8_t* __restrict__ codes, int64_t pitch, float* __restrict__ scale,
+                                                       int64_t rows, int K) {
+  constexpr int kAhead = 16;
+  const int lane = threadIdx.x & 31;
+  tc::let_next_launch();
+  for (int64_t row = int64_t(blockIdx.x) * 8 + (threadIdx.x >> 5); row < rows; row += int64_t(gridDim.x) * 8) {
+    const T* src = x + (inner == 1 ? row * x_outer : row / inner * x_outer + row % inner * x_inner);
+    float f[kAhead];
+    float m = 0.0f;
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j) {
+      const int k = j * 32 + lane;
+      f[j] = k < K ? kv::to_f(src[k]) : 0.0f;
+    }
+#pragma unroll
+    for (int j = 0; j < kAhead; j += 2) m = max_abs3(m, f[j], f[j + 1]);
+    for (int k = kAhead * 32 + lane; k < K; k += 32) m = max_abs3(m, kv::to_f(src[k]), 0.0f);
+    const RowScale sc = row_scale(__reduce_max_sync(0xffffffffu, abs_bits(m)));
+    if (lane == 0) scale[row] = sc.scale;
+    int8_t* dst = codes + row * pitch;
+    auto code = [&](float v) { return int8_t(codes4(v, 0.0f, 0.0f, 0.0f, sc.inv, sc.most)); };
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j) {
+      const int k = j * 32 + lane;
+      if (k < pitch) dst[k] = code(f[j]);
+    }
+    for (int64_t k = kAhead * 32 + lane; k < pitch; k += 32) dst[k] = k < K ? code(kv::to_f(src[k])) : int8_t(0);
   }
 }
 
@@ -345,21 +385,21 @@ void quantize_into(const void* x, int dtype, int64_t outer, int64_t inner, int64
     const bool vec = K % 8 == 0 && pitch % 8 == 0 && aligned16(p) && so * int64_t(sizeof(T)) % 16 == 0 &&
                      si * int64_t(sizeof(T)) % 16 == 0;
     auto go = [&](auto* kern, int per_block) {
-      kern<<<grid_for((rows + per_block - 1) / per_block, 8), 256, 0, stream()>>>(p, so, si, inner, codes, pitch, scale,
-                                                                                rows, K);
+      kern<<<grid_for((rows + per_block - 1) / per_block, 8), 256, 0, stream()>>>(p, so, si, int(inner), codes, pitch, scale,
+                                                                                rows, int(K));
       PD_CHECK_LAUNCH();
     };
-    // few rows: a block for each, so that a row's reads are spread over threads
+    const bool few = rows < 1184;                          // a block for each, so that a row's reads are spread over threads
     if (!vec) {
-      if (rows >= 1184) go(rows_kernel<false, 32, 1, T>, 8);
-      else go(rows_kernel<false, 256, 1, T>, 1);
-    } else if (rows < 1184 && K > 256) {
+      if (few && K > 512) go(rows_kernel<false, 256, 1, T>, 1);
+      else go(rows_any_kernel<T>, 8);
+    } else if (few && K > 256) {
       if (K <= 2048) go(rows_kernel<true, 256, 1, T>, 1);
       else go(rows_kernel<true, 256, 2, T>, 1);
     } else if (K <= 256) {
-      go(rows_kernel<true, 32, 1, T>, 8);
+      go(rows_kernel<true, 8, 4, T>, 32);
     } else if (K <= 512) {
-      go(rows_kernel<true, 32, 2, T>, 8);
+      go(rows_kernel<true, 16, 4, T>, 16);
     } else if (K <= 1024) {
       go(rows_kernel<true, 32, 4, T>, 8);
     } else {
@@ -372,6 +412,7 @@ std::vector<at::Tensor> quantize_rows(at::Tensor x) {
   PD_CHECK(x.is_cuda() && x.dim() == 3, "quantize_rows: a CUDA tensor [outer, inner, K] is expected");
   kv::dtype_of(x, "quantize_rows");
   PD_CHECK(x.size(2) <= 1 || x.stride(2) == 1, "quantize_rows: unit stride over the last dim is expected");
+  PD_CHECK(x.size(1) < (int64_t(1) << 31) && x.size(2) < (int64_t(1) << 30), "quantize_rows: rows of fewer than 2^30 values are expected");
   const c10::cuda::CUDAGuard guard(x.device());
   at::Tensor codes = at::empty(x.sizes(), x.options().dtype(at::kChar));
   at::Tensor scale = at::empty({x.size(0), x.size(1)}, x.options().dtype(at::kFloat));
