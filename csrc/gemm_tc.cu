@@ -82,7 +82,10 @@ struct Params {
 // What the epilogue does with pre-activations in 8 bits. kSave: C = GELU(acc) and the pre-activation acc leaves as
 // codes: a thread holds 32 columns of its row, which is one block of codes, so the block's maximum and scale take no
 // exchange. kUse: p = the values of such codes, C = acc * GELU'(p) and AUX = GELU(p).
-enum Saved8 : int { kNotSaved = 0, kSave = 1, kUse = 2 };
+// kDeep (no codes): epilogues none and residual (R through registers) for products with a long K: 8 epilogue warps with two
+// staged blocks, so that the ring has one 48 KB stage more. Of a stage only A comes from DRAM, and three of them in flight
+// do not cover its latency.
+enum Saved8 : int { kNotSaved = 0, kSave = 1, kUse = 2, kDeep = 3 };
 
 __device__ __forceinline__ void tile_coords(const Params& p, int t, int& l, int& mb, int& nb) {
   nb = t % p.n_blocks;
@@ -94,7 +97,7 @@ __device__ __forceinline__ void tile_coords(const Params& p, int t, int& l, int&
 // The 8-bit forms' epilogues are bound by instructions and the waits between them: 16 warps in place of 12 (a tile of 256
 // columns is then two chunks each) took the gradient's product of 100,608 x 256 x 1024 from 186 to 146 us; 8 took 171. Two
 // staged blocks a warp leave room for the same ring.
-__host__ __device__ constexpr int epi_warps(int saved8) { return saved8 == kNotSaved ? kEpiWarps : 16; }
+__host__ __device__ constexpr int epi_warps(int saved8) { return saved8 == kNotSaved ? kEpiWarps : saved8 == kDeep ? 8 : 16; }
 __host__ __device__ constexpr int stage_bufs(int saved8) { return saved8 == kNotSaved ? 3 : 2; }
 __host__ __device__ constexpr int threads_of(int saved8) { return 64 + 32 * epi_warps(saved8); }
 
@@ -241,12 +244,12 @@ __global__ void __launch_bounds__(threads_of(SAVED8), 1) gemm_kernel(const __gri
     uint8_t* stC = stage_base + ew * kBufs * 2048;
     uint8_t* stR0 = stC + 2048;   // R ring: buffers stR0 and stR0 + 2048
     uint64_t* rbar = rbar_all + 2 * ew;
-    const bool r_tma = p.r_tma != 0;
+    const bool r_tma = SAVED8 == kNotSaved && p.r_tma != 0;
     int kc = 0;          // chunks processed by this warp (R ring position)
     int r_pending = 0;   // R blocks issued and not yet waited for
     const int cr = lane >> 2, cc = lane & 3;
     auto sw = [](int r, int c) { return r * 64 + ((c ^ ((r >> 1) & 3)) << 4); };
-    const bool has_r = SAVED8 == kNotSaved && p.R != nullptr;   // addend (bias / residual), or GELU's pre-activation for kDGelu
+    const bool has_r = (SAVED8 == kNotSaved || SAVED8 == kDeep) && p.R != nullptr;   // addend (bias / residual), or GELU's pre-activation for kDGelu
     // work items: (tile, chunk) in this warp's order
     auto first_chunk = [&]() { return part * 32; };
     auto next_work = [&](int& t, int& c) {
@@ -385,7 +388,7 @@ __global__ void __launch_bounds__(threads_of(SAVED8), 1) gemm_kernel(const __gri
             }
             *reinterpret_cast<uint4*>(stX + sw(lane, j)) = make_uint4(h[0], h[1], h[2], h[3]);
           }
-        } else if (has_r && p.epi != kDGelu && p.epi != kMul && p.epi != kMaskPos && p.epi != kMulAdd) {
+        } else if (has_r && (SAVED8 == kDeep || (p.epi != kDGelu && p.epi != kMul && p.epi != kMaskPos && p.epi != kMulAdd))) {
           // addend before the activation: residual, or a bias broadcast through a zero row stride
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
@@ -993,6 +996,48 @@ void tc_gemm(at::Tensor A, at::Tensor B, at::Tensor C, int64_t epi, c10::optiona
   if (BN == 256) launch<256, 3>(ta, tb, tcm, txm, trm, p);
   else if (BN == 128) launch<128, 4>(ta, tb, tcm, txm, trm, p);
   else launch<64, 6>(ta, tb, tcm, txm, trm, p);
+}
+
+// C[l] = A[l] @ B[l]^T (+ R[l]): tc_gemm's product of the same operands with a deeper ring (kDeep).
+void tc_gemm_deep(at::Tensor A, at::Tensor B, at::Tensor C, c10::optional<at::Tensor> R, at::Tensor err, bool b_kn) {
+  check_operand(A, "A");
+  check_operand(B, "B");
+  const int64_t L = A.size(0), M = A.size(1), K = A.size(2), N = b_kn ? B.size(2) : B.size(1);
+  PD_CHECK((b_kn ? B.size(1) : B.size(2)) == K && (B.size(0) == L || B.size(0) == 1), "B must fit A");
+  PD_CHECK(N % 64 == 0, "N must be a multiple of 64");
+  auto matrix = [&](const at::Tensor& t, const char* what) {
+    PD_CHECK(t.is_cuda() && t.device() == A.device() && t.scalar_type() == at::kBFloat16 && t.dim() == 3 && t.size(0) == L &&
+                 t.size(1) == M && t.size(2) == N && t.stride(2) == 1 && t.stride(1) % 8 == 0 &&
+                 (L == 1 || t.stride(0) % 8 == 0) && reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0,
+             "%s must be a [L, M, N] bf16 view with rows on 16 bytes", what);
+    check_extent(t, what);
+  };
+  matrix(C, "C");
+  if (R) matrix(*R, "R");
+  PD_CHECK(B.device() == A.device() && err.device() == A.device(), "operands lie on two devices");
+  if (M == 0 || L == 0) return;
+  const c10::cuda::CUDAGuard guard(A.device());
+  tc::Params p{};
+  p.M = int(M); p.N = int(N); p.K = int(K); p.L = int(L);
+  p.m_blocks = int((M + tc::BM - 1) / tc::BM);
+  p.k_blocks = int((K + tc::BK - 1) / tc::BK);
+  p.C = reinterpret_cast<__nv_bfloat16*>(C.data_ptr()); p.c_ls = C.stride(0); p.c_ms = C.stride(1);
+  if (R) { p.R = reinterpret_cast<const __nv_bfloat16*>(R->data_ptr()); p.r_ls = R->stride(0); p.r_ms = R->stride(1); }
+  p.epi = R ? tc::kResidual : tc::kNone;
+  p.err = err.data_ptr<int>();
+  const int BN = (N % 256 == 0) ? 256 : (N % 128 == 0 ? 128 : 64);
+  p.n_blocks = int(N / BN);
+  p.tiles = int(L) * p.m_blocks * p.n_blocks;
+  p.b_kn = b_kn ? 1 : 0;
+  p.b_shared = (B.size(0) == 1) ? 1 : 0;
+  const CUtensorMap ta = make_map(A.data_ptr(), K, M, L, A.stride(1), A.stride(0), tc::BM, p.a_mode);
+  const CUtensorMap tb = b_kn ? make_map(B.data_ptr(), N, K, B.size(0), B.stride(1), B.stride(0), tc::BK, p.b_mode)
+                              : make_map(B.data_ptr(), K, N, B.size(0), B.stride(1), B.stride(0), BN, p.b_mode);
+  const CUtensorMap tcm = make_store_map(C.data_ptr(), N, M, L, C.stride(1), C.stride(0), p.c_mode);
+  p.x_mode = p.c_mode;
+  if (BN == 256) launch<256, 4, tc::kDeep>(ta, tb, tcm, tcm, tcm, p);
+  else if (BN == 128) launch<128, 6, tc::kDeep>(ta, tb, tcm, tcm, tcm, p);
+  else launch<64, 7, tc::kDeep>(ta, tb, tcm, tcm, tcm, p);
 }
 
 // The two GEMMs around pre-activations kept in 8 bits: codes [L, M, N] int8 views with rows on 16 bytes, exps [L, M, N / 32]
