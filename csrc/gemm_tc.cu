@@ -81,7 +81,8 @@ struct Params {
 
 // What the epilogue does with pre-activations in 8 bits. kSave: C = GELU(acc) and the pre-activation acc leaves as
 // codes: a thread holds 32 columns of its row, which is one block of codes, so the block's maximum and scale take no
-// exchange. kUse: p = the values of such codes, C = acc * GELU'(p) and AUX = GELU(p).
+// exchange. kUse: p = the values of such codes, C = acc * GELU'(p) and AUX = GELU(p). 100,608 x 256 -> 1024: kSave 98 us for
+// 361 MB, kUse 146 for 566 MB; both are bound by their epilogues' instructions (17 and 26 an element).
 // kDeep (no codes): epilogues none and residual (R through registers) for products with a long K: 8 epilogue warps with two
 // staged blocks, so that the ring has one 48 KB stage more. Of a stage only A comes from DRAM, and three of them in flight
 // do not cover its latency.

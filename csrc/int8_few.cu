@@ -9,6 +9,10 @@
 // would multiply 128 rows, 112 of them empty, behind a TMEM allocation and three
 // barriers. The instruction's k index is permuted alike in both operands, so that
 // a lane's 16 bytes of a weight row are one load.
+//
+// Measured (1 B200): 1 x 1024 -> 4096 3.5 us on the device (4.2 MB; 0.65 us at the
+// memory's rate), 16 x 256 -> 768 3.4; a call takes 5.6, its host time (12.3 and
+// 12.1 as codes and a tcgen05 product).
 #include "int8_common.cuh"
 #include "int8_few.cuh"
 #include "kv_common.cuh"

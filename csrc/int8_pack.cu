@@ -1,6 +1,11 @@
 // Activations to 8-bit integers and back: blocks of 32 values with a
 // power-of-two scale (save8 / load8, for training), and whole rows with a
 // 32-bit scale (quantize_rows, for integer products).
+//
+// All are bound by memory. 233,472 x 256 bf16: save8 35 us for 181 MB (5.2 TB/s),
+// load8 28 us (6.4 TB/s); 7919 x 1001 fp32, off 16 bytes: 13 and 15 us for 40 MB
+// each (byte stores and loads of 32 lanes). quantize_rows: 16,417 x 1024 bf16 12
+// us for 50 MB, 16,384 x 256 4 us for 12.6 MB.
 #include "int8_common.cuh"
 #include "kv_common.cuh"
 #include "tc_common.cuh"
@@ -389,7 +394,9 @@ void quantize_into(const void* x, int dtype, int64_t outer, int64_t inner, int64
                                                                                 rows, int(K));
       PD_CHECK_LAUNCH();
     };
-    const bool few = rows < 1184;                          // a block for each, so that a row's reads are spread over threads
+    // few rows: a block for each, so that a row's reads are spread over threads (rows of 1024: 64 1.8 us against 2.2 by
+    // warps, 300 2.0 and 2.2, 1000 2.8 and 2.2)
+    const bool few = rows < 512;
     if (!vec) {
       if (few && K > 512) go(rows_kernel<false, 256, 1, T>, 1);
       else go(rows_any_kernel<T>, 8);
