@@ -618,17 +618,13 @@ __device__ __forceinline__ void red_add_v4(float* addr, float a, float b, float 
                : "memory");
 }
 
-// 32 bytes of one row in one store (a whole sector).
-__device__ __forceinline__ void store_sector(void* dst, const uint32_t* w) {
-  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};"
-               ::"l"(dst), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7]) : "memory");
-}
-
 // Out = void: partial tiles are added into fp32 C. Out = float or __nv_bfloat16 (one split): a tile is the whole sum, so
-// it is stored in the gradient's type at once, with no zeroing, no reductions in memory and no conversion afterwards.
+// it is stored in the gradient's type at once, with no zeroing, no reductions in memory and no conversion afterwards: eight
+// warps stage 32 rows of 128 bytes each for a TMA store, so that whole lines are written.
 template <int BN, int STAGES, typename Out = void>
 __global__ void __launch_bounds__(kThreads, 1) wgrad_kernel(const __grid_constant__ CUtensorMap tmA,
                                                             const __grid_constant__ CUtensorMap tmB,
+                                                            const __grid_constant__ CUtensorMap tmC,
                                                             const WgParams p) {
   constexpr uint32_t kABytes = BM * BK * 2;
   constexpr uint32_t kBBytes = BN * BK * 2;
@@ -644,6 +640,9 @@ __global__ void __launch_bounds__(kThreads, 1) wgrad_kernel(const __grid_constan
   uint64_t* mma_done = tempty + 2;      // [1]
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(mma_done + 1);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  // (direct) a staged block of 4 KB for each of eight warps
+  [[maybe_unused]] uint8_t* stage_base = reinterpret_cast<uint8_t*>(
+      (reinterpret_cast<uintptr_t>(tmem_slot) + 64 + 1023) & ~uintptr_t(1023));
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
@@ -749,41 +748,62 @@ __global__ void __launch_bounds__(kThreads, 1) wgrad_kernel(const __grid_constan
       wg_item(p, w, l, mb, nb, kb0, kb1);
       const int row = mb * BM + q * 32 + lane;
       const uint32_t tbase = tmem + (uint32_t(q * 32) << 16) + uint32_t(a * BN);
+      if constexpr (!std::is_void_v<Out>) {
+        constexpr int kWide = 128 / int(sizeof(Out));
+        uint8_t* st = stage_base + ew * 4096;
 #pragma unroll 1
-      for (int c = part * 32; c < BN; c += kParts * 32) {
-        uint32_t r[32];
-        tc_ld32_issue(tbase + c, r);
-        tc_ld_wait(r);
-        if constexpr (!std::is_void_v<Out>) {
-          if (row < p.M) {
-            Out* dst = static_cast<Out*>(p.C) + l * p.c_ls + int64_t(row) * p.c_ms + nb * BN + c;
-            if constexpr (sizeof(Out) == 4) {
+        for (int c = part * kWide; c < BN && part < 2; c += 2 * kWide) {
+          if (lane == 0) bulk_wait_read_all();            // the staged block's last store has read it
+          __syncwarp();
 #pragma unroll
-              for (int j = 0; j < 32; j += 8) store_sector(dst + j, r + j);
-            } else {
+          for (int h = 0; h < kWide; h += 32) {
+            uint32_t r[32];
+            tc_ld32_issue(tbase + c + h, r);
+            tc_ld_wait(r);
+            constexpr int kChunks = sizeof(Out) == 4 ? 8 : 4;                       // of 16 bytes
 #pragma unroll
-              for (int j = 0; j < 32; j += 16) {
-                uint32_t w[8];
+            for (int j = 0; j < kChunks; ++j) {
+              uint32_t w[4];
 #pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                  const __nv_bfloat162 h = __floats2bfloat162_rn(__uint_as_float(r[j + 2 * e]), __uint_as_float(r[j + 2 * e + 1]));
-                  w[e] = *reinterpret_cast<const uint32_t*>(&h);
+              for (int e = 0; e < 4; ++e) {
+                if constexpr (sizeof(Out) == 4) {
+                  w[e] = r[4 * j + e];
+                } else {
+                  const __nv_bfloat162 b = __floats2bfloat162_rn(__uint_as_float(r[8 * j + 2 * e]), __uint_as_float(r[8 * j + 2 * e + 1]));
+                  w[e] = *reinterpret_cast<const uint32_t*>(&b);
                 }
-                store_sector(dst + j, w);
               }
+              *reinterpret_cast<uint4*>(st + lane * 128 + (((h / 32 * kChunks + j) ^ (lane & 7)) << 4)) =
+                  make_uint4(w[0], w[1], w[2], w[3]);
             }
           }
-        } else if (row < p.M && kb1 > kb0) {
-          float* dst = static_cast<float*>(p.C) + l * p.c_ls + int64_t(row) * p.c_ms + nb * BN + c;
+          fence_async_smem();
+          __syncwarp();
+          if (lane == 0) {
+            tma_store_3d(&tmC, st, nb * BN + c, mb * BM + q * 32, l);
+            bulk_commit();
+          }
+        }
+      } else {
+#pragma unroll 1
+        for (int c = part * 32; c < BN; c += kParts * 32) {
+          uint32_t r[32];
+          tc_ld32_issue(tbase + c, r);
+          tc_ld_wait(r);
+          if (row < p.M && kb1 > kb0) {
+            float* dst = static_cast<float*>(p.C) + l * p.c_ls + int64_t(row) * p.c_ms + nb * BN + c;
 #pragma unroll
-          for (int j = 0; j < 32; j += 4)
-            red_add_v4(dst + j, __uint_as_float(r[j]), __uint_as_float(r[j + 1]), __uint_as_float(r[j + 2]),
-                       __uint_as_float(r[j + 3]));
+            for (int j = 0; j < 32; j += 4)
+              red_add_v4(dst + j, __uint_as_float(r[j]), __uint_as_float(r[j + 1]), __uint_as_float(r[j + 2]),
+                         __uint_as_float(r[j + 3]));
+          }
         }
       }
       tc_fence_before();
       mbar_arrive(&tempty[a]);
     }
+    if (!std::is_void_v<Out> && lane == 0) bulk_wait_all();
+    __syncwarp();
   }
   tc_fence_before();
   __syncthreads();
@@ -1240,6 +1260,22 @@ void tc_gemm_saved8(at::Tensor A, at::Tensor B, at::Tensor C, at::Tensor codes, 
 
 namespace {
 
+// Map of a contiguous [L, M, N] gradient for stores of 32 rows of 128 bytes (128-byte swizzle).
+CUtensorMap make_line_map(const at::Tensor& C, int64_t M, int64_t N) {
+  CUtensorMap m;
+  const int64_t size = C.element_size();
+  const cuuint64_t dims[3] = {cuuint64_t(N), cuuint64_t(M), cuuint64_t(C.size(0))};
+  const cuuint64_t strides[2] = {cuuint64_t(N * size), cuuint64_t(M * N * size)};
+  const cuuint32_t box[3] = {cuuint32_t(128 / size), 32, 1}, one[3] = {1, 1, 1};
+  check_encode(C.data_ptr(), dims, strides, box, 3, "gradient map");
+  const CUresult r = tensor_map_encode_tiled(
+      &m, size == 4 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, C.data_ptr(), dims, strides, box,
+      one, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_NONE,
+      CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  PD_CHECK(r == CUDA_SUCCESS, "cuTensorMapEncodeTiled (gradient) failed (%d)", int(r));
+  return m;
+}
+
 // Blocks, tiles and splits of a weight gradient [M, N] over L batches of K rows.
 tc::WgParams wgrad_plan(int64_t L, int64_t K, int64_t M, int64_t N, bool l_sum) {
   tc::WgParams p{};
@@ -1294,17 +1330,19 @@ void run_wgrad(const at::Tensor& A, const at::Tensor& B, const at::Tensor& C, tc
   // MN-major operands: [64 k-rows][64 cols] boxes over dims {cols, rows, L}
   const CUtensorMap ta = make_map(A.data_ptr(), p.M, p.K, p.L, A.stride(1), A.stride(0), tc::BK, p.a_mode);
   const CUtensorMap tb = make_map(B.data_ptr(), p.N, p.K, p.L, B.stride(1), B.stride(0), tc::BK, p.b_mode);
+  const CUtensorMap tcm = direct ? make_line_map(C, p.M, p.N) : ta;
   auto go = [&](auto kern, int bn, int stages) {
-    const size_t smem = size_t(stages) * (tc::BM * tc::BK * 2 + bn * tc::BK * 2) + 1024 + 1024;
+    const size_t smem = size_t(stages) * (tc::BM * tc::BK * 2 + bn * tc::BK * 2) + 1024 + 1024 + (direct ? 8 * 4096 + 1024 : 0);
     PD_CHECK_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem)));
     const int grid = p.items < num_sms() ? p.items : num_sms();
-    tc::launch_behind(kern, dim3(unsigned(grid)), tc::kThreads, smem, ta, tb, p);
+    tc::launch_behind(kern, dim3(unsigned(grid)), tc::kThreads, smem, ta, tb, tcm, p);
   };
   auto by_width = [&](auto* tag) {
     using Out = std::remove_pointer_t<decltype(tag)>;
-    if (p.N % 256 == 0) go(tc::wgrad_kernel<256, 4, Out>, 256, 4);
-    else if (p.N % 128 == 0) go(tc::wgrad_kernel<128, 6, Out>, 128, 6);
-    else go(tc::wgrad_kernel<64, 8, Out>, 64, 8);
+    constexpr int kLess = std::is_void_v<Out> ? 0 : 1;   // stages that make room for the staged blocks
+    if (p.N % 256 == 0) go(tc::wgrad_kernel<256, 4 - kLess, Out>, 256, 4 - kLess);
+    else if (p.N % 128 == 0) go(tc::wgrad_kernel<128, 6 - kLess, Out>, 128, 6 - kLess);
+    else go(tc::wgrad_kernel<64, 8 - kLess, Out>, 64, 8 - kLess);
   };
   if (!direct) by_width(static_cast<void*>(nullptr));
   else if (C.scalar_type() == at::kFloat) by_width(static_cast<float*>(nullptr));
