@@ -18,7 +18,7 @@ void fmha_bwd_tc(at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor, int
 int64_t fmha_bwd_tc_max_q();
 void tc_gemm(at::Tensor, at::Tensor, at::Tensor, int64_t, c10::optional<at::Tensor>, c10::optional<at::Tensor>,
              at::Tensor, bool, c10::optional<at::Tensor>);
-void tc_gemm_deep(at::Tensor, at::Tensor, at::Tensor, c10::optional<at::Tensor>, at::Tensor, bool);
+void tc_gemm_lines(at::Tensor, at::Tensor, at::Tensor, c10::optional<at::Tensor>, at::Tensor, bool);
 void tc_gemm_saved8(at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor, c10::optional<at::Tensor>, at::Tensor, bool);
 void tc_wgrad(at::Tensor, at::Tensor, at::Tensor, at::Tensor, bool);
 at::Tensor tc_wgrad_as(at::Tensor, at::Tensor, at::Tensor, bool, int64_t);
@@ -53,9 +53,9 @@ at::Tensor tail(const at::Tensor& t, int64_t n_s) { return t.narrow(1, n_s, t.si
 // out = x by the shared weight, the rows from n_s on by their own; b_kn: by the weights transposed.
 void mixed(const at::Tensor& x, int64_t n_s, const at::Tensor& ws, const at::Tensor& wn, const at::Tensor& out,
            const at::Tensor& err, bool b_kn, const OptTensor& residual = c10::nullopt) {
-  pd::tc_gemm_deep(flat(x), ws.unsqueeze(0), flat(out), residual ? OptTensor(flat(*residual)) : residual, err, b_kn);
+  pd::tc_gemm_lines(flat(x), ws.unsqueeze(0), flat(out), residual ? OptTensor(flat(*residual)) : residual, err, b_kn);
   if (x.size(1) > n_s)
-    pd::tc_gemm_deep(tail(x, n_s), wn, tail(out, n_s), residual ? OptTensor(tail(*residual, n_s)) : residual, err, b_kn);
+    pd::tc_gemm_lines(tail(x, n_s), wn, tail(out, n_s), residual ? OptTensor(tail(*residual, n_s)) : residual, err, b_kn);
 }
 // The same around pre-activations in 8 bits (codes [B T, N], bytes [N / 32, B T]): without aux out = gelu(..) and the codes
 // are written, with it out = .. * gelu'(p), aux = gelu(p).

@@ -32,7 +32,7 @@
 // in-flight operations (bounded) and the CTA frees its TMEM and exits.
 #include "common.cuh"
 #include "driver_api.h"
-#include "int8_common.cuh"
+#include "gemm_host.h"
 #include "tc_common.cuh"
 
 #include <cuda.h>
@@ -74,19 +74,7 @@ struct Params {
   int b_shared;         // B has one batch shared by every l
   int b_kn;             // B stored [L, K, N] (N contiguous: a weight used transposed), loaded MN-major
   int* err;
-  // pre-activations in 8 bits (int8_common.cuh): codes [L, M, N] and scale bytes [L, M, N / 32]
-  int8_t* X8; int64_t x8_ls, x8_ms;
-  uint8_t* E; int64_t e_ls, e_ms, e_bs;
 };
-
-// What the epilogue does with pre-activations in 8 bits. kSave: C = GELU(acc) and the pre-activation acc leaves as
-// codes: a thread holds 32 columns of its row, which is one block of codes, so the block's maximum and scale take no
-// exchange. kUse: p = the values of such codes, C = acc * GELU'(p) and AUX = GELU(p). 100,608 x 256 -> 1024: kSave 98 us for
-// 361 MB, kUse 146 for 566 MB; both are bound by their epilogues' instructions (17 and 26 an element).
-// kDeep (no codes): epilogues none and residual (R through registers) for products with a long K: 8 epilogue warps with two
-// staged blocks, so that the ring has one 48 KB stage more. Of a stage only A comes from DRAM, and three of them in flight
-// do not cover its latency.
-enum Saved8 : int { kNotSaved = 0, kSave = 1, kUse = 2, kDeep = 3 };
 
 __device__ __forceinline__ void tile_coords(const Params& p, int t, int& l, int& mb, int& nb) {
   nb = t % p.n_blocks;
@@ -95,21 +83,13 @@ __device__ __forceinline__ void tile_coords(const Params& p, int t, int& l, int&
   l = r / p.m_blocks;
 }
 
-// The 8-bit forms' epilogues are bound by instructions and the waits between them: 16 warps in place of 12 (a tile of 256
-// columns is then two chunks each) took the gradient's product of 100,608 x 256 x 1024 from 186 to 146 us; 8 took 171. Two
-// staged blocks a warp leave room for the same ring.
-__host__ __device__ constexpr int epi_warps(int saved8) { return saved8 == kNotSaved ? kEpiWarps : saved8 == kDeep ? 8 : 16; }
-__host__ __device__ constexpr int stage_bufs(int saved8) { return saved8 == kNotSaved ? 3 : 2; }
-__host__ __device__ constexpr int threads_of(int saved8) { return 64 + 32 * epi_warps(saved8); }
-
-template <int BN, int STAGES, int SAVED8 = kNotSaved>
-__global__ void __launch_bounds__(threads_of(SAVED8), 1) gemm_kernel(const __grid_constant__ CUtensorMap tmA,
+template <int BN, int STAGES>
+__global__ void __launch_bounds__(kThreads, 1) gemm_kernel(const __grid_constant__ CUtensorMap tmA,
                                                            const __grid_constant__ CUtensorMap tmB,
                                                            const __grid_constant__ CUtensorMap tmC,
                                                            const __grid_constant__ CUtensorMap tmX,
                                                            const __grid_constant__ CUtensorMap tmR,
                                                            const Params p) {
-  constexpr int kEw = epi_warps(SAVED8), kBufs = stage_bufs(SAVED8);
   constexpr uint32_t kABytes = BM * BK * 2;
   constexpr uint32_t kBBytes = BN * BK * 2;
   constexpr uint32_t kTmemCols = 2 * BN;  // power of two for BN in {64, 128, 256}
@@ -122,8 +102,8 @@ __global__ void __launch_bounds__(threads_of(SAVED8), 1) gemm_kernel(const __gri
   uint64_t* tfull = empty + STAGES;     // [2]
   uint64_t* tempty = tfull + 2;         // [2]
   uint64_t* mma_done = tempty + 2;      // [1]
-  uint64_t* rbar_all = mma_done + 1;    // [epilogue warps][2]: R blocks landed (TMA)
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(rbar_all + 2 * kEw);
+  uint64_t* rbar_all = mma_done + 1;    // [kEpiWarps][2]: R blocks landed (TMA)
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(rbar_all + 2 * kEpiWarps);
   // per epilogue warp: 32 x 32 bf16 staging blocks for C and R / AUX (64-byte
   // rows, 16-byte chunks XOR-swizzled by (row >> 1) & 3: conflict-free both
   // when a thread writes its own row and when 4 lanes cover one row)
@@ -135,9 +115,9 @@ __global__ void __launch_bounds__(threads_of(SAVED8), 1) gemm_kernel(const __gri
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
     for (int s = 0; s < STAGES; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], 1); }
-    for (int a = 0; a < 2; ++a) { mbar_init(&tfull[a], 1); mbar_init(&tempty[a], kEw * 32); }
+    for (int a = 0; a < 2; ++a) { mbar_init(&tfull[a], 1); mbar_init(&tempty[a], kEpiWarps * 32); }
     mbar_init(mma_done, 1);
-    for (int i = 0; i < 2 * kEw; ++i) mbar_init(&rbar_all[i], 1);
+    for (int i = 0; i < 2 * kEpiWarps; ++i) mbar_init(&rbar_all[i], 1);
     *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     asm volatile("prefetch.tensormap [%0];" ::"l"(&tmA) : "memory");
@@ -241,16 +221,16 @@ __global__ void __launch_bounds__(threads_of(SAVED8), 1) gemm_kernel(const __gri
     const int ew = warp - 2;
     const int q = warp & 3;
     const int part = ew >> 2;
-    constexpr int kParts = kEw / 4;
-    uint8_t* stC = stage_base + ew * kBufs * 2048;
+    constexpr int kParts = kEpiWarps / 4;
+    uint8_t* stC = stage_base + ew * 3 * 2048;
     uint8_t* stR0 = stC + 2048;   // R ring: buffers stR0 and stR0 + 2048
     uint64_t* rbar = rbar_all + 2 * ew;
-    const bool r_tma = SAVED8 == kNotSaved && p.r_tma != 0;
+    const bool r_tma = p.r_tma != 0;
     int kc = 0;          // chunks processed by this warp (R ring position)
     int r_pending = 0;   // R blocks issued and not yet waited for
     const int cr = lane >> 2, cc = lane & 3;
     auto sw = [](int r, int c) { return r * 64 + ((c ^ ((r >> 1) & 3)) << 4); };
-    const bool has_r = (SAVED8 == kNotSaved || SAVED8 == kDeep) && p.R != nullptr;   // addend (bias / residual), or GELU's pre-activation for kDGelu
+    const bool has_r = (p.R != nullptr);   // addend (bias / residual), or GELU's pre-activation for kDGelu
     // work items: (tile, chunk) in this warp's order
     auto first_chunk = [&]() { return part * 32; };
     auto next_work = [&](int& t, int& c) {
@@ -276,23 +256,6 @@ __global__ void __launch_bounds__(threads_of(SAVED8), 1) gemm_kernel(const __gri
       mbar_expect_tx(&rbar[buf], 32 * 32 * 2);
       tma_load_rows(stR0 + (buf << 11), &tmR, &rbar[buf], p.r_mode, nb * BN + c, mb * BM + q * 32, l);
     };
-    // the codes and scale byte of this thread's next row and chunk, on their way (kUse)
-    uint4 code0 = make_uint4(0, 0, 0, 0), code1 = code0;
-    uint32_t code_scale = 1;
-    auto load_codes = [&](int t, int c) {
-      int l, mb, nb;
-      tile_coords(p, t, l, mb, nb);
-      const int m = mb * BM + q * 32 + lane, n = nb * BN + c;
-      if (m < p.M) {
-        const uint4* src = reinterpret_cast<const uint4*>(p.X8 + l * p.x8_ls + int64_t(m) * p.x8_ms + n);
-        code0 = __ldcs(src);
-        code1 = __ldcs(src + 1);
-        code_scale = p.E[l * p.e_ls + m * p.e_ms + (n >> 5) * p.e_bs];
-      }
-    };
-    if constexpr (SAVED8 == kUse) {
-      if (first_chunk() < BN && blockIdx.x < p.tiles) load_codes(blockIdx.x, first_chunk());
-    }
     uint4 pref[4];
     if (has_r && first_chunk() < BN && blockIdx.x < p.tiles) {
       if (r_tma) {
@@ -349,47 +312,7 @@ __global__ void __launch_bounds__(threads_of(SAVED8), 1) gemm_kernel(const __gri
         float v[32];
 #pragma unroll
         for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
-        if constexpr (SAVED8 == kSave) {
-          uint32_t w[8];
-          const uint32_t byte = i8::save_block(v, i8::kTopWide, w);
-          if (m0 + lane < p.M) {
-            uint4* dst = reinterpret_cast<uint4*>(p.X8 + l * p.x8_ls + int64_t(m0 + lane) * p.x8_ms + n0 + c);
-            dst[0] = make_uint4(w[0], w[1], w[2], w[3]);
-            dst[1] = make_uint4(w[4], w[5], w[6], w[7]);
-            p.E[l * p.e_ls + (m0 + lane) * p.e_ms + ((n0 + c) >> 5) * p.e_bs] = uint8_t(byte);
-          }
-#pragma unroll
-          for (int j = 0; j < 32; j += 2) gelu2(v[j], v[j + 1]);
-        } else if constexpr (SAVED8 == kUse) {
-          const uint32_t w[8] = {code0.x, code0.y, code0.z, code0.w, code1.x, code1.y, code1.z, code1.w};
-          const float scale = i8::scale_of(code_scale);
-          {
-            int tn = t, cn = c;
-            next_work(tn, cn);
-            if (tn < p.tiles) load_codes(tn, cn);          // in flight during this chunk
-          }
-          wait_staging();
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            float g[8];
-            i8::values4(w[2 * j], scale, g);
-            i8::values4(w[2 * j + 1], scale, g + 4);
-#pragma unroll
-            for (int e = 0; e < 8; e += 2) {
-              float d0, d1;
-              gelu_grad2<true>(g[e], g[e + 1], d0, d1);
-              v[8 * j + e] *= d0;
-              v[8 * j + e + 1] *= d1;
-            }
-            uint32_t h[4];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const __nv_bfloat162 b = __floats2bfloat162_rn(g[2 * e], g[2 * e + 1]);
-              h[e] = *reinterpret_cast<const uint32_t*>(&b);
-            }
-            *reinterpret_cast<uint4*>(stX + sw(lane, j)) = make_uint4(h[0], h[1], h[2], h[3]);
-          }
-        } else if (has_r && (SAVED8 == kDeep || (p.epi != kDGelu && p.epi != kMul && p.epi != kMaskPos && p.epi != kMulAdd))) {
+        if (has_r && p.epi != kDGelu && p.epi != kMul && p.epi != kMaskPos && p.epi != kMulAdd) {
           // addend before the activation: residual, or a bias broadcast through a zero row stride
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
@@ -403,8 +326,7 @@ __global__ void __launch_bounds__(threads_of(SAVED8), 1) gemm_kernel(const __gri
             }
           }
         }
-        if (SAVED8 != kNotSaved) {
-        } else if (p.epi == kGelu && p.AUX) {
+        if (p.epi == kGelu && p.AUX) {
           wait_staging();
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
@@ -418,8 +340,7 @@ __global__ void __launch_bounds__(threads_of(SAVED8), 1) gemm_kernel(const __gri
             *reinterpret_cast<uint4*>(stX + sw(lane, j)) = pk;
           }
         }
-        if (SAVED8 != kNotSaved) {
-        } else if (p.epi == kGelu) {
+        if (p.epi == kGelu) {
           // GELU of the bf16-rounded pre-activation (the value AUX stores)
 #pragma unroll
           for (int j = 0; j < 32; j += 2) {
@@ -543,7 +464,7 @@ __global__ void __launch_bounds__(threads_of(SAVED8), 1) gemm_kernel(const __gri
         __syncwarp();
         if (lane == 0) {
           tma_store_rows(&tmC, stC, p.c_mode, n0 + c, m0, l);
-          if (SAVED8 == kUse || (SAVED8 == kNotSaved && (p.epi == kGelu || p.epi == kGeluD || p.epi == kMulAdd) && p.AUX))
+          if ((p.epi == kGelu || p.epi == kGeluD || p.epi == kMulAdd) && p.AUX)
             tma_store_rows(&tmX, stX, p.x_mode, n0 + c, m0, l);
           bulk_commit();
         }
@@ -954,125 +875,15 @@ __global__ void __launch_bounds__(kThreads, 1) wgrad_wide_kernel(const __grid_co
 // ---------------------------------------------------------------------------
 namespace {
 
-// 3-D tensor map over bf16 rows of length K (strides in elements).  mode 0:
-// dims {K, rows, L}; mode 1 (batch stride smaller than the row stride, e.g.
-// one batch per NS token): dims {K, L, rows} so the strides stay ascending.
-// Preconditions of cuTensorMapEncodeTiled checked on the host, so a bad view
-// fails with a message instead of reaching the driver: 16-byte aligned base,
-// extents in [1, 2^32), strides multiples of 16 bytes below 2^40, boxes of
-// 1..256 elements.
-void check_encode(const void* base, const cuuint64_t* dims, const cuuint64_t* strides, const cuuint32_t* box,
-                  int rank, const char* what) {
-  PD_CHECK(reinterpret_cast<uintptr_t>(base) % 16 == 0, "%s: base address not 16-byte aligned", what);
-  for (int i = 0; i < rank; ++i) {
-    PD_CHECK(dims[i] >= 1 && dims[i] < (cuuint64_t(1) << 32), "%s: extent %d out of range (%llu)", what, i,
-             (unsigned long long)dims[i]);
-    PD_CHECK(box[i] >= 1 && box[i] <= 256, "%s: box %d out of range (%u)", what, i, (unsigned)box[i]);
-  }
-  for (int i = 0; i + 1 < rank; ++i)
-    PD_CHECK(strides[i] % 16 == 0 && strides[i] > 0 && strides[i] < (cuuint64_t(1) << 40),
-             "%s: stride %d (%llu bytes) must be a positive multiple of 16 below 2^40", what, i,
-             (unsigned long long)strides[i]);
-}
-
-// Every element a [L, rows, K] view addresses lies inside its storage (a TMA
-// map of a view reaching past its allocation would read or write memory that
-// is not the tensor's).
-void check_extent(const at::Tensor& t, const char* name) {
-  if (t.numel() == 0) return;
-  int64_t last = t.storage_offset();
-  for (int64_t d = 0; d < t.dim(); ++d) {
-    PD_CHECK(t.stride(d) >= 0, "%s: negative strides are not supported", name);
-    last += (t.size(d) - 1) * t.stride(d);
-  }
-  PD_CHECK(int64_t((last + 1) * t.element_size()) <= int64_t(t.storage().nbytes()),
-           "%s: the view reaches past the end of its storage", name);
-}
-
-CUtensorMap make_map(const void* base, int64_t K, int64_t rows, int64_t L, int64_t row_stride, int64_t l_stride,
-                     int box_rows, int& mode) {
-  CUtensorMap m;
-  if (L <= 1) l_stride = row_stride * rows;
-  mode = (L > 1 && l_stride < row_stride) ? 1 : 0;
-  cuuint64_t dims[3], strides[2];
-  cuuint32_t box[3];
-  if (mode == 0) {
-    dims[0] = K; dims[1] = rows; dims[2] = L;
-    strides[0] = row_stride * 2; strides[1] = l_stride * 2;
-    box[0] = tc::BK; box[1] = box_rows; box[2] = 1;
-  } else {
-    dims[0] = K; dims[1] = L; dims[2] = rows;
-    strides[0] = l_stride * 2; strides[1] = row_stride * 2;
-    box[0] = tc::BK; box[1] = 1; box[2] = box_rows;
-  }
-  cuuint32_t estr[3] = {1, 1, 1};
-  check_encode(base, dims, strides, box, 3, "operand map");
-  CUresult r = tensor_map_encode_tiled(&m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(base), dims, strides,
-                                      box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
-                                      CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  PD_CHECK(r == CUDA_SUCCESS, "cuTensorMapEncodeTiled failed (%d): K=%lld rows=%lld L=%lld row_stride=%lld l_stride=%lld",
-           int(r), (long long)K, (long long)rows, (long long)L, (long long)row_stride, (long long)l_stride);
-  return m;
-}
-
-// Map of a [L, rows, N] bf16 epilogue operand (C / AUX stores, R loads):
-// 32 x 32 boxes, 64-byte swizzle (the epilogue's staging layout); dim order
-// as in make_map.
-CUtensorMap make_store_map(const void* base, int64_t N, int64_t rows, int64_t L, int64_t row_stride,
-                           int64_t l_stride, int& mode) {
-  CUtensorMap m;
-  if (L <= 1) l_stride = row_stride * rows;
-  mode = (L > 1 && l_stride < row_stride) ? 1 : 0;
-  cuuint64_t dims[3], strides[2];
-  cuuint32_t box[3];
-  if (mode == 0) {
-    dims[0] = N; dims[1] = rows; dims[2] = L;
-    strides[0] = row_stride * 2; strides[1] = l_stride * 2;
-    box[0] = 32; box[1] = 32; box[2] = 1;
-  } else {
-    dims[0] = N; dims[1] = L; dims[2] = rows;
-    strides[0] = l_stride * 2; strides[1] = row_stride * 2;
-    box[0] = 32; box[1] = 1; box[2] = 32;
-  }
-  cuuint32_t estr[3] = {1, 1, 1};
-  check_encode(base, dims, strides, box, 3, "epilogue map");
-  CUresult r = tensor_map_encode_tiled(&m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(base), dims, strides,
-                                      box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_64B,
-                                      CU_TENSOR_MAP_L2_PROMOTION_NONE, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  PD_CHECK(r == CUDA_SUCCESS,
-           "cuTensorMapEncodeTiled (store) failed (%d): N=%lld rows=%lld L=%lld row_stride=%lld l_stride=%lld",
-           int(r), (long long)N, (long long)rows, (long long)L, (long long)row_stride, (long long)l_stride);
-  return m;
-}
-
-// [L, rows, K] view (L may be 1): unit stride on K, 16-byte aligned rows.
-void check_operand(const at::Tensor& t, const char* name) {
-  PD_CHECK(t.is_cuda() && t.scalar_type() == at::kBFloat16, "%s: bf16 CUDA tensor required", name);
-  PD_CHECK(t.dim() == 3 && t.stride(2) == 1, "%s: [L, rows, K] with unit stride on K required", name);
-  PD_CHECK(t.stride(1) % 8 == 0 && (t.size(0) == 1 || t.stride(0) % 8 == 0) &&
-              reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0, "%s: rows must be 16-byte aligned", name);
-  PD_CHECK(t.size(2) % 8 == 0, "%s: K must be a multiple of 8", name);
-  check_extent(t, name);
-}
-
-template <int BN, int STAGES, int SAVED8 = tc::kNotSaved>
+template <int BN, int STAGES>
 void launch(const CUtensorMap& ta, const CUtensorMap& tb, const CUtensorMap& tcm, const CUtensorMap& txm,
             const CUtensorMap& trm, const tc::Params& p) {
-  constexpr size_t smem = STAGES * (tc::BM * tc::BK * 2 + BN * tc::BK * 2) + 1024 + 1024 +
-                          tc::epi_warps(SAVED8) * tc::stage_bufs(SAVED8) * 2048;
+  constexpr size_t smem = STAGES * (tc::BM * tc::BK * 2 + BN * tc::BK * 2) + 1024 + 1024 + tc::kEpiWarps * 3 * 2048;
   static_assert(smem <= 232448, "GEMM shared memory over the 227 KB per-block limit");
-  static std::atomic<uint64_t> allowed{0};               // by device
-  int dev = 0;
-  PD_CHECK_CUDA(cudaGetDevice(&dev));
-  const uint64_t bit = uint64_t(1) << (dev & 63);
-  if (!(allowed.load(std::memory_order_relaxed) & bit)) {
-    PD_CHECK_CUDA(cudaFuncSetAttribute(tc::gemm_kernel<BN, STAGES, SAVED8>,
-                                       cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem)));
-    allowed.fetch_or(bit, std::memory_order_relaxed);
-  }
-  int grid = p.tiles < num_sms() ? p.tiles : num_sms();
-  tc::launch_behind(tc::gemm_kernel<BN, STAGES, SAVED8>, dim3(unsigned(grid)), tc::threads_of(SAVED8), smem, ta, tb, tcm, txm,
-                    trm, p);
+  static tc::SharedLimit limit;
+  limit.allow(tc::gemm_kernel<BN, STAGES>, smem);
+  const int grid = p.tiles < num_sms() ? p.tiles : num_sms();
+  tc::launch_behind(tc::gemm_kernel<BN, STAGES>, dim3(unsigned(grid)), tc::kThreads, smem, ta, tb, tcm, txm, trm, p);
 }
 
 }  // namespace
@@ -1151,111 +962,6 @@ void tc_gemm(at::Tensor A, at::Tensor B, at::Tensor C, int64_t epi, c10::optiona
   if (BN == 256) launch<256, 3>(ta, tb, tcm, txm, trm, p);
   else if (BN == 128) launch<128, 4>(ta, tb, tcm, txm, trm, p);
   else launch<64, 6>(ta, tb, tcm, txm, trm, p);
-}
-
-// C[l] = A[l] @ B[l]^T (+ R[l]): tc_gemm's product of the same operands with a deeper ring (kDeep).
-void tc_gemm_deep(at::Tensor A, at::Tensor B, at::Tensor C, c10::optional<at::Tensor> R, at::Tensor err, bool b_kn) {
-  check_operand(A, "A");
-  check_operand(B, "B");
-  const int64_t L = A.size(0), M = A.size(1), K = A.size(2), N = b_kn ? B.size(2) : B.size(1);
-  PD_CHECK((b_kn ? B.size(1) : B.size(2)) == K && (B.size(0) == L || B.size(0) == 1), "B must fit A");
-  PD_CHECK(N % 64 == 0, "N must be a multiple of 64");
-  auto matrix = [&](const at::Tensor& t, const char* what) {
-    PD_CHECK(t.is_cuda() && t.device() == A.device() && t.scalar_type() == at::kBFloat16 && t.dim() == 3 && t.size(0) == L &&
-                 t.size(1) == M && t.size(2) == N && t.stride(2) == 1 && t.stride(1) % 8 == 0 &&
-                 (L == 1 || t.stride(0) % 8 == 0) && reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0,
-             "%s must be a [L, M, N] bf16 view with rows on 16 bytes", what);
-    check_extent(t, what);
-  };
-  matrix(C, "C");
-  if (R) matrix(*R, "R");
-  PD_CHECK(B.device() == A.device() && err.device() == A.device(), "operands lie on two devices");
-  if (M == 0 || L == 0) return;
-  const c10::cuda::CUDAGuard guard(A.device());
-  tc::Params p{};
-  p.M = int(M); p.N = int(N); p.K = int(K); p.L = int(L);
-  p.m_blocks = int((M + tc::BM - 1) / tc::BM);
-  p.k_blocks = int((K + tc::BK - 1) / tc::BK);
-  p.C = reinterpret_cast<__nv_bfloat16*>(C.data_ptr()); p.c_ls = C.stride(0); p.c_ms = C.stride(1);
-  if (R) { p.R = reinterpret_cast<const __nv_bfloat16*>(R->data_ptr()); p.r_ls = R->stride(0); p.r_ms = R->stride(1); }
-  p.epi = R ? tc::kResidual : tc::kNone;
-  p.err = err.data_ptr<int>();
-  const int BN = (N % 256 == 0) ? 256 : (N % 128 == 0 ? 128 : 64);
-  p.n_blocks = int(N / BN);
-  p.tiles = int(L) * p.m_blocks * p.n_blocks;
-  p.b_kn = b_kn ? 1 : 0;
-  p.b_shared = (B.size(0) == 1) ? 1 : 0;
-  const CUtensorMap ta = make_map(A.data_ptr(), K, M, L, A.stride(1), A.stride(0), tc::BM, p.a_mode);
-  const CUtensorMap tb = b_kn ? make_map(B.data_ptr(), N, K, B.size(0), B.stride(1), B.stride(0), tc::BK, p.b_mode)
-                              : make_map(B.data_ptr(), K, N, B.size(0), B.stride(1), B.stride(0), BN, p.b_mode);
-  const CUtensorMap tcm = make_store_map(C.data_ptr(), N, M, L, C.stride(1), C.stride(0), p.c_mode);
-  p.x_mode = p.c_mode;
-  if (BN == 256) launch<256, 4, tc::kDeep>(ta, tb, tcm, tcm, tcm, p);
-  else if (BN == 128) launch<128, 6, tc::kDeep>(ta, tb, tcm, tcm, tcm, p);
-  else launch<64, 7, tc::kDeep>(ta, tb, tcm, tcm, tcm, p);
-}
-
-// The two GEMMs around pre-activations kept in 8 bits: codes [L, M, N] int8 views with rows on 16 bytes, exps [L, M, N / 32]
-// uint8 views of any strides. With AUX undefined (the up projection): C = GELU(A @ B^T), codes and exps are written. With
-// AUX (the down projection's data gradient): p = the values of codes, C = (A @ B^T) * GELU'(p), AUX = GELU(p).
-void tc_gemm_saved8(at::Tensor A, at::Tensor B, at::Tensor C, at::Tensor codes, at::Tensor exps,
-                    c10::optional<at::Tensor> AUX, at::Tensor err, bool b_kn) {
-  check_operand(A, "A");
-  check_operand(B, "B");
-  const int64_t L = A.size(0), M = A.size(1), K = A.size(2), N = b_kn ? B.size(2) : B.size(1);
-  PD_CHECK((b_kn ? B.size(1) : B.size(2)) == K && (B.size(0) == L || B.size(0) == 1), "B must fit A");
-  PD_CHECK(N % 64 == 0, "N must be a multiple of 64");
-  auto matrix = [&](const at::Tensor& t, at::ScalarType type, int64_t n, const char* what) {
-    PD_CHECK(t.is_cuda() && t.device() == A.device() && t.scalar_type() == type && t.dim() == 3 && t.size(0) == L &&
-                 t.size(1) == M && t.size(2) == n, "%s does not fit the product", what);
-    check_extent(t, what);
-  };
-  auto rows16 = [&](const at::Tensor& t, const char* what) {
-    const int64_t e = t.element_size();
-    PD_CHECK(t.stride(2) == 1 && t.stride(1) * e % 16 == 0 && (L == 1 || t.stride(0) * e % 16 == 0) &&
-                 reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0, "%s: rows must lie on 16 bytes", what);
-  };
-  matrix(C, at::kBFloat16, N, "C");
-  rows16(C, "C");
-  matrix(codes, at::kChar, N, "codes");
-  rows16(codes, "codes");
-  matrix(exps, at::kByte, N / 32, "exps");
-  PD_CHECK(B.device() == A.device() && err.device() == A.device(), "operands lie on two devices");
-  if (M == 0 || L == 0) return;
-  const c10::cuda::CUDAGuard guard(A.device());
-  tc::Params p{};
-  p.M = int(M); p.N = int(N); p.K = int(K); p.L = int(L);
-  p.m_blocks = int((M + tc::BM - 1) / tc::BM);
-  p.k_blocks = int((K + tc::BK - 1) / tc::BK);
-  p.C = reinterpret_cast<__nv_bfloat16*>(C.data_ptr()); p.c_ls = C.stride(0); p.c_ms = C.stride(1);
-  p.err = err.data_ptr<int>();
-  p.X8 = codes.data_ptr<int8_t>(); p.x8_ls = codes.stride(0); p.x8_ms = codes.stride(1);
-  p.E = exps.data_ptr<uint8_t>(); p.e_ls = exps.stride(0); p.e_ms = exps.stride(1); p.e_bs = exps.stride(2);
-  const int BN = (N % 256 == 0) ? 256 : (N % 128 == 0 ? 128 : 64);
-  p.n_blocks = int(N / BN);
-  p.tiles = int(L) * p.m_blocks * p.n_blocks;
-  const CUtensorMap ta = make_map(A.data_ptr(), K, M, L, A.stride(1), A.stride(0), tc::BM, p.a_mode);
-  p.b_kn = b_kn ? 1 : 0;
-  const CUtensorMap tb = b_kn ? make_map(B.data_ptr(), N, K, B.size(0), B.stride(1), B.stride(0), tc::BK, p.b_mode)
-                              : make_map(B.data_ptr(), K, N, B.size(0), B.stride(1), B.stride(0), BN, p.b_mode);
-  p.b_shared = (B.size(0) == 1) ? 1 : 0;
-  const CUtensorMap tcm = make_store_map(C.data_ptr(), N, M, L, C.stride(1), C.stride(0), p.c_mode);
-  auto go = [&](auto mode, const CUtensorMap& tx) {
-    constexpr int kMode = decltype(mode)::value;
-    if (BN == 256) launch<256, 3, kMode>(ta, tb, tcm, tx, tcm, p);
-    else if (BN == 128) launch<128, 4, kMode>(ta, tb, tcm, tx, tcm, p);
-    else launch<64, 6, kMode>(ta, tb, tcm, tx, tcm, p);
-  };
-  if (AUX && AUX->defined()) {
-    matrix(*AUX, at::kBFloat16, N, "AUX");
-    rows16(*AUX, "AUX");
-    p.AUX = reinterpret_cast<__nv_bfloat16*>(AUX->data_ptr());
-    const CUtensorMap tx = make_store_map(AUX->data_ptr(), N, M, L, AUX->stride(1), AUX->stride(0), p.x_mode);
-    go(std::integral_constant<int, tc::kUse>(), tx);
-  } else {
-    p.x_mode = p.c_mode;
-    go(std::integral_constant<int, tc::kSave>(), tcm);
-  }
 }
 
 namespace {

@@ -9,6 +9,8 @@
 #include "common.cuh"
 #include "driver_api.h"
 
+#include <atomic>
+
 namespace pd {
 namespace tc {
 
@@ -168,6 +170,20 @@ __device__ __forceinline__ void tc_ld32(uint32_t taddr, float* v) {
 __device__ __forceinline__ void wait_for_launch_before() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 // From here on the next kernel may be set up on SMs that have room.
 __device__ __forceinline__ void let_next_launch() { asm volatile("griddepcontrol.launch_dependents;"); }
+
+// A kernel's limit of dynamic shared memory, set once for each device (the call costs a small launch's time).
+struct SharedLimit {
+  std::atomic<uint64_t> done{0};
+  template <typename Kern>
+  void allow(Kern* kern, size_t bytes) {
+    int dev = 0;
+    PD_CHECK_CUDA(cudaGetDevice(&dev));
+    const uint64_t bit = uint64_t(1) << (dev & 63);
+    if (done.load(std::memory_order_relaxed) & bit) return;
+    PD_CHECK_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, int(bytes)));
+    done.fetch_or(bit, std::memory_order_relaxed);
+  }
+};
 
 template <typename... Args, typename... Given>
 void launch_behind(void (*kern)(Args...), dim3 grid, int threads, size_t smem, const Given&... given) {
