@@ -9,11 +9,19 @@
 //
 // Roles as in gemm_tc.cu: TMA producer, one MMA lane, epilogue warps; sums
 // double-buffered in TMEM. The difference is the way out: an epilogue unit is 64
-// columns of 32 rows, so that a TMA store writes whole lines of 128 bytes (the
-// stores of 64-byte rows of gemm_tc.cu reach some 3.5 TB/s of writes, whole lines
-// 6), and the ring takes what 8 or 16 staged blocks of 4 KB leave. kUse has two
-// results and room for one block a warp: two warps share a unit, 32 columns each,
-// and its two blocks.
+// columns of 32 rows, so that a TMA store writes whole lines of 128 bytes, and the
+// ring takes what 8 or 16 staged blocks of 4 KB leave (four stages of 48 KB for
+// kPlain: of a stage only A comes from DRAM, and three in flight do not cover its
+// latency). kUse has two results and room for one block a warp: two warps share a
+// unit, 32 columns each, and its two blocks.
+//
+// Measured (1 B200, 100,608 rows): kSave 256 -> 1024 85 us for 361 MB (98 by
+// half lines), kUse 128 us for 566 MB (146), both bound by their epilogues'
+// instructions (17 and 26 an element); kPlain 1024 -> 256 with R 67 us for 308 MB,
+// without 50 for 257 (gemm_tc.cu's kernel 70 and 60), bound by the operands' way
+// into shared memory: about 1000 cycles a k-block of 48 KB. Two blocks on one tile
+// of 256 rows (cta_group::2, 32 KB) took 45 us without R, but 95 and 143 in the
+// forms with codes.
 #include "gemm_host.h"
 #include "int8_common.cuh"
 #include "tc_common.cuh"
@@ -31,8 +39,8 @@ constexpr int BK = 64;
 constexpr int kBlockBytes = 4096;       // a staged block: 32 rows of 128 bytes
 enum Mode : int { kPlain = 0, kSave = 1, kUse = 2 };
 
-// GELU's arithmetic wants more warps (kUse of 100,608 x 256 -> 1024 took 186 us with 12, 146 with 16), the plain products
-// want the room in shared memory.
+// GELU's arithmetic wants more warps (kUse, still by half lines, took 186 us with 12 and 146 with 16; 171 with 8), the plain
+// products want the room in shared memory.
 constexpr int epi_warps(int mode) { return mode == kPlain ? 8 : 16; }
 constexpr int threads_of(int mode) { return 64 + 32 * epi_warps(mode); }
 

@@ -17,7 +17,7 @@
 //                output type, out through a swizzled 32 x 32 block in shared
 //                memory and a TMA store (or row by row, where C's rows do not
 //                lie on 16 bytes)
-// Measured (1 B200, with the rows' codes): 16,417 x 1024 -> 4096 with GELU 98 us (1.4 PFLOP/s), 16 x 1024 rows by 256 ->
+// Measured (1 B200, with the rows' codes): 16,417 x 1024 -> 4096 with GELU 100 us (1.4 PFLOP/s), 16 x 1024 rows by 256 ->
 // 1024 with GELU 27, 2069 x 333 -> 1001 fp32 12. What bounds it: the epilogue's instructions (17 an element with GELU,
 // 14 of them its polynomial; a tile of 256 columns takes 8.5 thousand cycles of twelve warps) and, less, shared memory: a
 // k-block is written (48 KB) and read for 512 cycles of products, and takes 650 to 750.

@@ -252,7 +252,7 @@ def _kept(f):
 
 
 SIZES = [(1, 1, 64, 64, 0), (2, 9, 64, 128, 3), (3, 130, 128, 320, 0), (5, 70, 256, 1024, 16), (1, 300, 192, 768, 8),
-         (3, 500, 256, 512, 8), (2, 700, 512, 256, 40)]
+         (3, 500, 256, 512, 8), (2, 700, 512, 256, 40), (20, 515, 64, 320, 3), (9, 2300, 128, 192, 0)]
 
 
 @pytest.mark.parametrize("wdtype", [torch.float32, torch.bfloat16])
