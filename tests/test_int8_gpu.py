@@ -415,3 +415,92 @@ def test_a_captured_training_step():
     assert torch.equal(got[0], ref[0]) and torch.equal(got[1], ref[1])
     for a, b in zip(got[2:], ref[2:]):                       # weight gradients add up in no fixed order
         assert (a.double() - b.double()).abs().max() <= 1e-5 * b.abs().max() + 1e-6
+
+
+def test_every_row_has_its_own_weight():
+    """n_s = 0: the shared weights get gradients of zeros, nothing else changes."""
+    parts = [t.requires_grad_() for t in _parts(3, 5, 64, 128, 5, seed=3)]
+    out = dense.mixed_ffn(parts[0], parts[1], 0, *parts[2:], save8=True)
+    assert torch.equal(out, dense.mixed_ffn(parts[0], parts[1], 0, *parts[2:]))
+    g = torch.autograd.grad(out, parts, torch.ones_like(out))
+    assert g[2].eq(0).all() and g[3].eq(0).all() and g[4].ne(0).any() and g[5].ne(0).any()
+    y = dense.mixed_linear(parts[0], 0, parts[2], parts[4], save8=True)
+    dx, dw, dwn = torch.autograd.grad(y, (parts[0], parts[2], parts[4]), torch.ones_like(y))
+    assert dw.eq(0).all() and dwn.ne(0).any() and dx.isfinite().all()
+
+
+def test_calls_at_once():
+    """Two threads, each on its own stream, with rows for every form of the product."""
+    import threading
+    g = _gen(11)
+    w = Int8Weight.from_float(torch.randn(300, 640, generator=g, device=DEV))
+    xs = [torch.randn(m, 640, generator=g, device=DEV).bfloat16() for m in (1, 16, 90, 3000)]
+    want = [int8_linear(x, w, act="gelu") for x in xs]
+    saved = [load8(save8(x)) for x in xs]
+    torch.cuda.synchronize()
+    bad = []
+
+    def work():
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(20):
+                for x, y, v in zip(xs, want, saved):
+                    if not (torch.equal(int8_linear(x, w, act="gelu"), y) and torch.equal(load8(save8(x)), v)):
+                        bad.append(x.shape)
+
+    threads = [threading.Thread(target=work) for _ in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not bad
+
+
+def test_first_call_inside_a_capture():
+    """Kernels that a process has not launched yet, captured at once, forward and backward; then a captured backward pass
+    while an eager graph of the same leaves lives, which PyTorch's engine refuses (of its own operations alike) with an
+    error that the process outlives. In a process of its own."""
+    import subprocess
+    import sys
+    from pathlib import Path
+    code = """
+import sys
+sys.path.insert(0, %r)
+import torch
+from primus_dlrm_b200.ops import dense
+from primus_dlrm_b200.ops.int8 import Int8Weight, int8_linear
+x = torch.randn(40, 4096, device="cuda").bfloat16()
+w = Int8Weight.from_float(torch.randn(64, 4096, device="cuda"))
+torch.cuda.synchronize()
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    y = int8_linear(x, w)
+graph.replay()
+torch.cuda.synchronize()
+print("FORWARD", torch.equal(y, int8_linear(x, w)))
+
+r = lambda *s: torch.randn(*s, device="cuda").bfloat16()
+p = [t.requires_grad_() for t in (r(2, 90, 64), r(2, 90, 64), r(128, 64), r(64, 128), r(3, 128, 64), r(3, 64, 128))]
+dy = r(2, 90, 64)
+step = lambda: torch.autograd.grad(dense.mixed_ffn(p[0], p[1], 87, *p[2:], save8=True), p, dy)
+torch.cuda.synchronize()
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    got = step()
+graph.replay()
+torch.cuda.synchronize()
+near = lambda a, b: all(bool((u.double() - v.double()).abs().max() <= 2.0 ** -7 * v.abs().max()) for u, v in zip(a, b))
+want = step()
+print("BACKWARD", near(got, want))
+alive = dense.mixed_ffn(p[0], p[1], 87, *p[2:], save8=True)
+graph = torch.cuda.CUDAGraph()
+try:
+    with torch.cuda.graph(graph):
+        got = step()
+    print("CAPTURED")
+except RuntimeError as e:
+    print("REFUSED", str(e)[:200])
+print("AFTER", near(torch.autograd.grad(alive, p, dy), want))
+print("END")
+""" % str(Path(__file__).resolve().parent.parent)
+    r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300)
+    assert all(m in r.stdout for m in ("FORWARD True", "BACKWARD True", "AFTER True", "END")), r.stdout + r.stderr[-1500:]
