@@ -59,7 +59,8 @@ OptTensor linear(const at::Tensor& x, const at::Tensor& codes, const at::Tensor&
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.doc() = "primus_dlrm_b200 sm_100a kernels: activations in 8 bits, products of 8-bit integers";
-  m.def("save8", &pd::i8::save8, "x [rows, K] -> int8 codes [rows, K], scale bytes [blocks of 32, rows]");
+  m.def("save8", [](const at::Tensor& x) { no_tangent(x, "save8"); const at::NoGradGuard none; return pd::i8::save8(x); },
+        "x [..., K] -> int8 codes [rows, K], scale bytes [blocks of 32, rows]");
   m.def("load8", [](at::Tensor c, at::Tensor e, at::ScalarType t) { return pd::i8::load8(c, e, int64_t(t)); },
         "values of save8's codes and scale bytes in a type");
   m.def("quantize_rows", &pd::i8::quantize_rows, "x [outer, inner, K] -> int8 codes, fp32 scales [outer, inner]");

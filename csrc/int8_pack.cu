@@ -10,6 +10,7 @@
 #include "kv_common.cuh"
 #include "tc_common.cuh"
 
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 
 #include <algorithm>
@@ -326,21 +327,26 @@ void by_type(int dtype, F&& f) {
 
 }  // namespace
 
-// x [rows, K] (unit stride over K, any stride over rows) -> codes [rows, K], scale bytes [blocks, rows]
+// x [..., K] -> codes [rows, K], scale bytes [blocks, rows]
 std::vector<at::Tensor> save8(at::Tensor x) {
-  PD_CHECK(x.is_cuda() && x.dim() == 2, "save8: a CUDA matrix is expected");
+  PD_CHECK(x.is_cuda() && x.dim() >= 1, "save8: a CUDA tensor with a last dim is expected");
   const int dtype = kv::dtype_of(x, "save8");
   const c10::cuda::CUDAGuard guard(x.device());
-  const int64_t rows = x.size(0), K = x.size(1), blocks = (K + kBlock - 1) / kBlock;
-  at::Tensor codes = at::empty({rows, K}, x.options().dtype(at::kChar));
-  at::Tensor exps = at::empty({blocks, rows}, x.options().dtype(at::kByte));
+  const int64_t K = x.size(-1);
+  int64_t rows = 1;
+  for (int64_t d = 0; d + 1 < x.dim(); ++d) rows *= x.size(d);
+  const int64_t blocks = (K + kBlock - 1) / kBlock;
+  at::Tensor codes = at::detail::empty_cuda({rows, K}, at::kChar, x.device(), c10::nullopt);
+  at::Tensor exps = at::detail::empty_cuda({blocks, rows}, at::kByte, x.device(), c10::nullopt);
   if (rows == 0 || K == 0) return {codes, exps};
-  PD_CHECK(K == 1 || x.stride(1) == 1, "save8: unit stride over the last dim is expected");
+  if (K > 1 && x.stride(-1) != 1) x = x.contiguous();
+  if (x.dim() > 2 && !x.is_contiguous()) x = x.reshape({rows, K});
+  const int64_t row_stride = x.dim() == 2 ? x.stride(0) : K;
   PD_CHECK(K < (int64_t(1) << 30), "save8: rows of fewer than 2^30 values are expected");
   by_type(dtype, [&](auto* tag) {
     using T = std::remove_pointer_t<decltype(tag)>;
     const T* p = static_cast<const T*>(x.data_ptr());
-    const int64_t stride = rows == 1 ? K : x.stride(0);
+    const int64_t stride = rows == 1 ? K : row_stride;
     const uint32_t top = dtype == kv::kF16 ? kTopHalf : kTopWide;
     const bool vec = K % 8 == 0 && aligned16(p) && stride * int64_t(sizeof(T)) % 16 == 0;
     if (vec)
@@ -361,7 +367,7 @@ at::Tensor load8(at::Tensor codes, at::Tensor exps, int64_t dtype) {
                exps.dim() == 2 && exps.size(0) == blocks && exps.size(1) == rows,
            "load8: contiguous uint8 scale bytes [blocks, rows] are expected");
   const c10::cuda::CUDAGuard guard(codes.device());
-  at::Tensor y = at::empty({rows, K}, codes.options().dtype(at::ScalarType(dtype)));
+  at::Tensor y = at::detail::empty_cuda({rows, K}, at::ScalarType(dtype), codes.device(), c10::nullopt);
   const int t = kv::dtype_of(y, "load8");
   if (rows == 0 || K == 0) return y;
   PD_CHECK(K < (int64_t(1) << 30), "load8: rows of fewer than 2^30 values are expected");

@@ -35,7 +35,7 @@ class Saved8:
 
     def __init__(self, codes: torch.Tensor, scale_bytes: torch.Tensor, shape, dtype: torch.dtype):
         # [rows, K] and block-major [blocks, rows]: a GEMM epilogue's threads own rows
-        self._codes, self._bytes, self.shape, self.dtype = codes, scale_bytes, torch.Size(shape), dtype
+        self._codes, self._bytes, self.shape, self.dtype = codes, scale_bytes, shape, dtype
 
     @property
     def codes(self) -> torch.Tensor:
@@ -74,7 +74,7 @@ def _load_ref(codes: torch.Tensor, scale_bytes: torch.Tensor, dtype: torch.dtype
 
 
 def save_rows(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
-    """(codes [rows, K], scale bytes [blocks, rows]) of x [rows, K] in one piece along K."""
+    """(codes [rows, K], scale bytes [blocks, rows]) of x [rows, K]."""
     return tuple(_ext.int8().save8(x)) if _native(x) else _save_ref(x)
 
 
@@ -88,10 +88,11 @@ def save8(x: torch.Tensor) -> Saved8:
     differentiable: the result carries no graph."""
     if x.dim() == 0 or x.dtype not in _TYPES:
         raise ValueError(f"save8: a bf16, fp16 or fp32 tensor with a last dim is expected, not {x.dtype} of {x.dim()} dims")
-    x2 = x.detach().reshape(x.shape[:-1].numel(), x.shape[-1])
-    if x2.shape[1] > 1 and x2.stride(1) != 1:
-        x2 = x2.contiguous()
-    return Saved8(*save_rows(x2), x.shape, x.dtype)
+    if _native(x):
+        codes, scale_bytes = _ext.int8().save8(x)
+    else:
+        codes, scale_bytes = _save_ref(x.detach().reshape(x.shape[:-1].numel(), x.shape[-1]))
+    return Saved8(codes, scale_bytes, x.shape, x.dtype)
 
 
 def load8(saved: Saved8, dtype: torch.dtype | None = None) -> torch.Tensor:

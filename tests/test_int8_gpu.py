@@ -184,6 +184,9 @@ def test_product_refusals():
         y.sum().backward()
     with forward_ad.dual_level(), pytest.raises(RuntimeError, match="forward-mode"):
         int8_linear(forward_ad.make_dual(x, x), w)
+    with forward_ad.dual_level(), pytest.raises(RuntimeError, match="forward-mode"):
+        save8(forward_ad.make_dual(x, x))
+    assert not save8(x.clone().requires_grad_())._codes.requires_grad
 
 
 def test_product_on_another_stream_in_a_graph_and_twice():
