@@ -2,6 +2,8 @@
 // pyramid attention (attn_fmha.cu) and the tcgen05 GEMMs (gemm_*.cu).
 #include <torch/extension.h>
 
+#include "gemm_mat.h"
+
 #include <ATen/core/dispatch/Dispatcher.h>
 #include <c10/core/DeviceGuard.h>
 
@@ -18,10 +20,10 @@ void fmha_bwd_tc(at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor, int
 int64_t fmha_bwd_tc_max_q();
 void tc_gemm(at::Tensor, at::Tensor, at::Tensor, int64_t, c10::optional<at::Tensor>, c10::optional<at::Tensor>,
              at::Tensor, bool, c10::optional<at::Tensor>);
-void tc_gemm_lines(at::Tensor, at::Tensor, at::Tensor, c10::optional<at::Tensor>, at::Tensor, bool);
-void tc_gemm_saved8(at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor, c10::optional<at::Tensor>, at::Tensor, bool);
+void gemm_lines(const Mat&, const Mat&, const Mat&, const Mat*, int*, bool);
+void gemm_saved8(const Mat&, const Mat&, const Mat&, const MatCodes&, const Mat*, int*, bool);
+at::Tensor wgrad_as(const Mat&, const Mat&, const at::Device&, int*, bool, int64_t);
 void tc_wgrad(at::Tensor, at::Tensor, at::Tensor, at::Tensor, bool);
-at::Tensor tc_wgrad_as(at::Tensor, at::Tensor, at::Tensor, bool, int64_t);
 at::Tensor tc_mma_rate(int64_t, int64_t, int64_t, int64_t, int64_t, int64_t, at::Tensor);
 at::Tensor tc_mma_burst(int64_t, int64_t, int64_t, int64_t, int64_t, int64_t, int64_t, int64_t, at::Tensor);
 }  // namespace pd
@@ -46,42 +48,62 @@ at::Tensor load8(const at::Tensor& codes, const at::Tensor& scale_bytes) {      
   return op.call(codes, scale_bytes, at::kBFloat16);
 }
 
-// All rows of a [B, T, N] tensor, and its rows from n_s on as one batch for each of them.
-at::Tensor flat(const at::Tensor& t) { return t.reshape({1, t.size(0) * t.size(1), t.size(2)}); }
-at::Tensor tail(const at::Tensor& t, int64_t n_s) { return t.narrow(1, n_s, t.size(1) - n_s).transpose(0, 1); }
+// bf16, in one piece, on 16 bytes: what the products read (a copy only where t is not).
+at::Tensor whole(const at::Tensor& t) {
+  const at::Tensor c = t.to(at::kBFloat16).contiguous();
+  return reinterpret_cast<uintptr_t>(c.data_ptr()) % 16 == 0 ? c : c.clone();
+}
+// Rows of a whole [B, T, N] tensor: all of them; those of every sample before n_s, one batch for each sample; those from n_s
+// on, one batch for each of them. Taken from the sizes: a whole tensor's stride over an axis of length 1 may be anything.
+pd::Mat flat(const at::Tensor& t) {
+  return {t.data_ptr(), 1, t.size(0) * t.size(1), t.size(2), 0, t.size(2)};
+}
+pd::Mat head(const at::Tensor& t, int64_t n_s) {
+  return {t.data_ptr(), t.size(0), n_s, t.size(2), t.size(1) * t.size(2), t.size(2)};
+}
+pd::Mat tail(const at::Tensor& t, int64_t n_s) {
+  return {static_cast<char*>(t.data_ptr()) + n_s * t.size(2) * t.element_size(), t.size(1) - n_s, t.size(0), t.size(2),
+          t.size(2), t.size(1) * t.size(2)};
+}
+// A whole weight [N, K] or [L, N, K].
+pd::Mat weight(const at::Tensor& w) {
+  const int64_t n = w.size(-2), k = w.size(-1);
+  return {w.data_ptr(), w.dim() == 3 ? w.size(0) : 1, n, k, n * k, k};
+}
+pd::Mat* ref(pd::Mat&& m) { return &m; }                  // for the length of a call
 
 // out = x by the shared weight, the rows from n_s on by their own; b_kn: by the weights transposed.
-void mixed(const at::Tensor& x, int64_t n_s, const at::Tensor& ws, const at::Tensor& wn, const at::Tensor& out,
-           const at::Tensor& err, bool b_kn, const OptTensor& residual = c10::nullopt) {
-  pd::tc_gemm_lines(flat(x), ws.unsqueeze(0), flat(out), residual ? OptTensor(flat(*residual)) : residual, err, b_kn);
+void mixed(const at::Tensor& x, int64_t n_s, const at::Tensor& ws, const at::Tensor& wn, const at::Tensor& out, int* err,
+           bool b_kn, const at::Tensor& residual = at::Tensor()) {
+  const bool r = residual.defined();
+  pd::gemm_lines(flat(x), weight(ws), flat(out), r ? ref(flat(residual)) : nullptr, err, b_kn);
   if (x.size(1) > n_s)
-    pd::tc_gemm_lines(tail(x, n_s), wn, tail(out, n_s), residual ? OptTensor(tail(*residual, n_s)) : residual, err, b_kn);
+    pd::gemm_lines(tail(x, n_s), weight(wn), tail(out, n_s), r ? ref(tail(residual, n_s)) : nullptr, err, b_kn);
 }
 // The same around pre-activations in 8 bits (codes [B T, N], bytes [N / 32, B T]): without aux out = gelu(..) and the codes
 // are written, with it out = .. * gelu'(p), aux = gelu(p).
 void mixed_saved(const at::Tensor& x, int64_t n_s, const at::Tensor& ws, const at::Tensor& wn, const at::Tensor& out,
-                 const at::Tensor& codes, const at::Tensor& bytes, const OptTensor& aux, const at::Tensor& err, bool b_kn) {
-  const int64_t B = x.size(0), T = x.size(1);
-  pd::tc_gemm_saved8(flat(x), ws.unsqueeze(0), flat(out), codes.unsqueeze(0), bytes.t().unsqueeze(0),
-                     aux ? OptTensor(flat(*aux)) : aux, err, b_kn);
+                 const at::Tensor& codes, const at::Tensor& bytes, const at::Tensor& aux, int* err, bool b_kn) {
+  const int64_t T = x.size(1), N = codes.size(1), rows = codes.size(0);
+  int8_t* c = codes.data_ptr<int8_t>();
+  uint8_t* e = bytes.data_ptr<uint8_t>();
+  const bool use = aux.defined();
+  pd::gemm_saved8(flat(x), weight(ws), flat(out), pd::MatCodes{c, 0, N, e, 0, 1, rows}, use ? ref(flat(aux)) : nullptr, err,
+                  b_kn);
   if (T > n_s)
-    pd::tc_gemm_saved8(tail(x, n_s), wn, tail(out, n_s), tail(codes.view({B, T, codes.size(1)}), n_s),
-                       bytes.view({bytes.size(0), B, T}).narrow(2, n_s, T - n_s).permute({2, 1, 0}),
-                       aux ? OptTensor(tail(*aux, n_s)) : aux, err, b_kn);
+    pd::gemm_saved8(tail(x, n_s), weight(wn), tail(out, n_s), pd::MatCodes{c + n_s * N, N, T * N, e + n_s, 1, T, rows},
+                    use ? ref(tail(aux, n_s)) : nullptr, err, b_kn);
 }
 // Gradients of the shared weight (one sum over the samples' rows, read in place) and of the others.
-at::Tensor shared_grad(const at::Tensor& dy, const at::Tensor& x, int64_t n_s, const at::Tensor& err, int64_t type) {
-  if (x.size(1) == n_s) return pd::tc_wgrad_as(flat(dy), flat(x), err, true, type);
-  return pd::tc_wgrad_as(dy.narrow(1, 0, n_s), x.narrow(1, 0, n_s), err, true, type);
+at::Tensor shared_grad(const at::Tensor& dy, const at::Tensor& x, int64_t n_s, int* err, int64_t type) {
+  if (x.size(1) == n_s) return pd::wgrad_as(flat(dy), flat(x), dy.device(), err, true, type);
+  return pd::wgrad_as(head(dy, n_s), head(x, n_s), dy.device(), err, true, type);
 }
-at::Tensor own_grad(const at::Tensor& dy, const at::Tensor& x, int64_t n_s, const at::Tensor& err, int64_t type) {
-  if (x.size(1) == n_s)
-    return at::zeros({0, dy.size(2), x.size(2)}, dy.options().dtype(at::ScalarType(type)));
-  return pd::tc_wgrad_as(tail(dy, n_s), tail(x, n_s), err, false, type);
+at::Tensor own_grad(const at::Tensor& dy, const at::Tensor& x, int64_t n_s, int* err, int64_t type) {
+  return pd::wgrad_as(tail(dy, n_s), tail(x, n_s), dy.device(), err, false, type);
 }
 
 at::Tensor rows_of(const at::Tensor& t) { return t.view({t.size(0) * t.size(1), t.size(2)}); }
-at::Tensor bf16(const at::Tensor& t) { return t.to(at::kBFloat16); }
 at::Tensor like(const at::Tensor& x, int64_t N) { return at::empty({x.size(0), x.size(1), N}, x.options()); }
 std::tuple<at::Tensor, at::Tensor> room(const at::Tensor& x, int64_t N) {            // codes and scale bytes of [B, T, N]
   const int64_t rows = x.size(0) * x.size(1);
@@ -94,14 +116,14 @@ void once() {
 struct MixedLinearSaved8 : public torch::autograd::Function<MixedLinearSaved8> {
   static at::Tensor forward(AutogradContext* ctx, at::Tensor x, at::Tensor w_s, at::Tensor w_ns, int64_t n_s, bool gelu,
                             at::Tensor err) {
-    const at::Tensor xb = x.contiguous(), ws = bf16(w_s).contiguous(), wn = bf16(w_ns).contiguous();
+    const at::Tensor xb = whole(x), ws = whole(w_s), wn = whole(w_ns);
     const at::Tensor y = like(xb, ws.size(0));
     at::Tensor pc, pb;
     if (gelu) {
       std::tie(pc, pb) = room(xb, ws.size(0));
-      mixed_saved(xb, n_s, ws, wn, y, pc, pb, c10::nullopt, err, false);
+      mixed_saved(xb, n_s, ws, wn, y, pc, pb, at::Tensor(), err.data_ptr<int>(), false);
     } else {
-      mixed(xb, n_s, ws, wn, y, err, false);
+      mixed(xb, n_s, ws, wn, y, err.data_ptr<int>(), false);
     }
     auto [xc, xs] = save8(rows_of(xb));
     ctx->save_for_backward({ws, wn, xc, xs, pc, pb});
@@ -113,10 +135,12 @@ struct MixedLinearSaved8 : public torch::autograd::Function<MixedLinearSaved8> {
   }
   static variable_list backward(AutogradContext* ctx, variable_list g) {
     once();
+    const c10::DeviceGuard guard(g[0].device());
     const auto v = ctx->get_saved_variables();
-    const at::Tensor &ws = v[0], &wn = v[1], err = ctx->saved_data["err"].toTensor();
+    const at::Tensor &ws = v[0], &wn = v[1], word = ctx->saved_data["err"].toTensor();
+    int* err = word.data_ptr<int>();
     const int64_t n_s = ctx->saved_data["n_s"].toInt();
-    at::Tensor dy = bf16(g[0]).contiguous(), dx, dws, dwn;
+    at::Tensor dy = whole(g[0]), dx, dws, dwn;
     if (v[4].defined()) dy = at::gelu_backward(dy, load8(v[4], v[5]).view(dy.sizes()));
     if (ctx->needs_input_grad(0)) {
       dx = like(dy, ws.size(1));
@@ -134,12 +158,11 @@ struct MixedLinearSaved8 : public torch::autograd::Function<MixedLinearSaved8> {
 struct MixedFFNSaved8 : public torch::autograd::Function<MixedFFNSaved8> {
   static at::Tensor forward(AutogradContext* ctx, at::Tensor x, at::Tensor z, at::Tensor w1, at::Tensor w2, at::Tensor wn1,
                             at::Tensor wn2, int64_t n_s, at::Tensor err) {
-    const at::Tensor xb = x.contiguous();
-    const at::Tensor w[4] = {bf16(w1).contiguous(), bf16(w2).contiguous(), bf16(wn1).contiguous(), bf16(wn2).contiguous()};
+    const at::Tensor xb = whole(x), w[4] = {whole(w1), whole(w2), whole(wn1), whole(wn2)};
     const at::Tensor h = like(xb, w[0].size(0)), out = like(xb, w[1].size(0));
     auto [pc, pb] = room(xb, w[0].size(0));
-    mixed_saved(xb, n_s, w[0], w[2], h, pc, pb, c10::nullopt, err, false);
-    mixed(h, n_s, w[1], w[3], out, err, false, z);
+    mixed_saved(xb, n_s, w[0], w[2], h, pc, pb, at::Tensor(), err.data_ptr<int>(), false);
+    mixed(h, n_s, w[1], w[3], out, err.data_ptr<int>(), false, whole(z));
     auto [xc, xs] = save8(rows_of(xb));
     ctx->save_for_backward({xc, xs, pc, pb, w[0], w[1], w[2], w[3]});
     ctx->saved_data["err"] = err;
@@ -150,11 +173,13 @@ struct MixedFFNSaved8 : public torch::autograd::Function<MixedFFNSaved8> {
   }
   static variable_list backward(AutogradContext* ctx, variable_list g) {
     once();
+    const c10::DeviceGuard guard(g[0].device());
     const auto v = ctx->get_saved_variables();
-    const at::Tensor &w1 = v[4], &w2 = v[5], &wn1 = v[6], &wn2 = v[7], err = ctx->saved_data["err"].toTensor();
+    const at::Tensor &w1 = v[4], &w2 = v[5], &wn1 = v[6], &wn2 = v[7], word = ctx->saved_data["err"].toTensor();
+    int* err = word.data_ptr<int>();
     const int64_t n_s = ctx->saved_data["n_s"].toInt();
     const auto types = ctx->saved_data["types"].toIntVector();
-    const at::Tensor dy = bf16(g[0]).contiguous();
+    const at::Tensor dy = whole(g[0]);
     at::Tensor grads[6];
     if (ctx->needs_input_grad(1)) grads[1] = g[0];
     const at::Tensor dp = like(dy, w1.size(0));
@@ -224,18 +249,11 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         py::arg("R2") = py::none(),
         "C[l] = epi(A[l] @ B[l]^T) on tcgen05 (A [L,M,K], B [L|1,N,K] or with b_kn [L|1,K,N], C [L,M,N] bf16 views); "
         "epi 0 none, 1 gelu, 2 +R, 3 dgelu(R), 4 gelu+gelu' to AUX, 5 *R, 6 relu(+R), 7 acc where R>0, 8 R*acc+R2");
-  m.def("tc_gemm_saved8", &pd::tc_gemm_saved8, py::arg("A"), py::arg("B"), py::arg("C"), py::arg("codes"), py::arg("exps"),
-        py::arg("AUX"), py::arg("err"), py::arg("b_kn") = false,
-        "the GEMMs around pre-activations in 8 bits (codes int8 [L,M,N], scale bytes [L,M,N/32]): without AUX "
-        "C = gelu(A @ B^T) and codes, exps written; with AUX p from codes, C = (A @ B^T) gelu'(p), AUX = gelu(p)");
   m.def("mixed_linear_saved8", &mixed_linear_saved8, "a mixed projection whose input waits for the backward in 8 bits");
   m.def("mixed_ffn_saved8", &mixed_ffn_saved8, "a mixed FFN whose input and pre-activation wait for the backward in 8 bits");
   m.def("tc_wgrad", &pd::tc_wgrad, py::arg("A"), py::arg("B"), py::arg("C"), py::arg("err"), py::arg("l_sum") = false,
         "C[l] (fp32, zeroed) += A[l]^T B[l] over rows on tcgen05, split over rows (A [L,K,M], B [L,K,N] bf16 views); "
         "l_sum: one C summed over the batches too");
-  m.def("tc_wgrad_as", [](at::Tensor A, at::Tensor B, at::Tensor err, bool l_sum, at::ScalarType t) {
-          return pd::tc_wgrad_as(A, B, err, l_sum, int64_t(t)); },
-        "the weight gradient of tc_wgrad as a new tensor of a type (l_sum: [M, N])");
   m.def("tc_mma_rate", &pd::tc_mma_rate, py::arg("mode"), py::arg("n"), py::arg("iters"), py::arg("nacc"),
         py::arg("swz"), py::arg("issue"), py::arg("err"),
         "tcgen05.mma probe: int64 [SMs, 2] (issue cycles, issue + execution cycles) for `iters` M=128 x n x 16 "

@@ -23,10 +23,10 @@
 // of 256 rows (cta_group::2, 32 KB) took 45 us without R, but 95 and 143 in the
 // forms with codes.
 #include "gemm_host.h"
+#include "gemm_mat.h"
 #include "int8_common.cuh"
 #include "tc_common.cuh"
 
-#include <c10/cuda/CUDAGuard.h>
 #include <type_traits>
 
 namespace pd {
@@ -381,31 +381,29 @@ void launch(const CUtensorMap& ta, const CUtensorMap& tb, const CUtensorMap& tcm
                     lines::threads_of(MODE), smem, ta, tb, tcm, tx, tr, p);
 }
 
+void aligned(const Mat& t, const char* what) {            // bf16 rows on 16 bytes
+  PD_CHECK(reinterpret_cast<uintptr_t>(t.p) % 16 == 0 && t.ms % 8 == 0 && (t.L == 1 || t.ls % 8 == 0),
+           "%s: rows must lie on 16 bytes", what);
+}
+
 // The common part: operands checked, maps made; X or R where a mode has them.
-void run(const at::Tensor& A, const at::Tensor& B, const at::Tensor& C, const at::Tensor* X, const at::Tensor* R,
-         const at::Tensor* codes, const at::Tensor* exps, const at::Tensor& err, bool b_kn, int mode) {
-  check_operand(A, "A");
-  check_operand(B, "B");
-  const int64_t L = A.size(0), M = A.size(1), K = A.size(2), N = b_kn ? B.size(2) : B.size(1);
-  PD_CHECK((b_kn ? B.size(1) : B.size(2)) == K && (B.size(0) == L || B.size(0) == 1), "B must fit A");
-  PD_CHECK(N % 64 == 0, "N must be a multiple of 64");
-  auto matrix = [&](const at::Tensor& t, at::ScalarType type, int64_t n, bool rows16, const char* what) {
-    const int64_t e = t.element_size();
-    PD_CHECK(t.is_cuda() && t.device() == A.device() && t.scalar_type() == type && t.dim() == 3 && t.size(0) == L &&
-                 t.size(1) == M && t.size(2) == n, "%s does not fit the product", what);
-    PD_CHECK(!rows16 || (t.stride(2) == 1 && t.stride(1) * e % 16 == 0 && (L == 1 || t.stride(0) * e % 16 == 0) &&
-                         reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0), "%s: rows must lie on 16 bytes", what);
-    check_extent(t, what);
-  };
-  matrix(C, at::kBFloat16, N, true, "C");
-  if (X) matrix(*X, at::kBFloat16, N, true, "X");
-  if (R) matrix(*R, at::kBFloat16, N, true, "R");
-  if (codes) matrix(*codes, at::kChar, N, true, "codes");
-  if (exps) matrix(*exps, at::kByte, N / 32, false, "exps");
-  PD_CHECK(B.device() == A.device() && err.device() == A.device(), "operands lie on two devices");
+void run(const Mat& A, const Mat& B, const Mat& C, const Mat* X, const Mat* R, const MatCodes* codes, int* err, bool b_kn,
+         int mode) {
+  const int64_t L = A.L, M = A.rows, K = A.cols, N = b_kn ? B.cols : B.rows;
+  PD_CHECK((b_kn ? B.rows : B.cols) == K && (B.L == L || B.L == 1), "B must fit A");
+  PD_CHECK(K % 8 == 0 && N % 64 == 0, "K must be a multiple of 8, N of 64");
+  for (const Mat* t : {&C, X, R})
+    PD_CHECK(t == nullptr || (t->L == L && t->rows == M && t->cols == N), "a result or addend does not fit the product");
   PD_CHECK(M < (int64_t(1) << 31) && L < (int64_t(1) << 31), "too many rows");
   if (M == 0 || L == 0) return;
-  const c10::cuda::CUDAGuard guard(A.device());
+  aligned(A, "A");
+  aligned(B, "B");
+  aligned(C, "C");
+  if (X) aligned(*X, "X");
+  if (R) aligned(*R, "R");
+  if (codes)
+    PD_CHECK(reinterpret_cast<uintptr_t>(codes->codes) % 16 == 0 && codes->ms % 16 == 0 && (L == 1 || codes->ls % 16 == 0),
+             "codes: rows must lie on 16 bytes");
   lines::Params p{};
   p.M = int(M); p.N = int(N); p.L = int(L);
   p.m_blocks = int((M + lines::BM - 1) / lines::BM);
@@ -415,18 +413,20 @@ void run(const at::Tensor& A, const at::Tensor& B, const at::Tensor& C, const at
   PD_CHECK(L * p.m_blocks * p.n_blocks < (int64_t(1) << 30), "too many rows");
   p.tiles = int(L) * p.m_blocks * p.n_blocks;
   p.b_kn = b_kn ? 1 : 0;
-  p.b_shared = (B.size(0) == 1) ? 1 : 0;
+  p.b_shared = B.L == 1 ? 1 : 0;
   p.has_r = R ? 1 : 0;
-  p.err = err.data_ptr<int>();
-  if (codes) { p.X8 = codes->data_ptr<int8_t>(); p.x8_ls = codes->stride(0); p.x8_ms = codes->stride(1); }
-  if (exps) { p.E = exps->data_ptr<uint8_t>(); p.e_ls = exps->stride(0); p.e_ms = exps->stride(1); p.e_bs = exps->stride(2); }
-  const CUtensorMap ta = make_map(A.data_ptr(), K, M, L, A.stride(1), A.stride(0), lines::BM, p.a_mode);
-  const CUtensorMap tb = b_kn ? make_map(B.data_ptr(), N, K, B.size(0), B.stride(1), B.stride(0), lines::BK, p.b_mode)
-                              : make_map(B.data_ptr(), K, N, B.size(0), B.stride(1), B.stride(0), BN, p.b_mode);
+  p.err = err;
+  if (codes) {
+    p.X8 = codes->codes; p.x8_ls = codes->ls; p.x8_ms = codes->ms;
+    p.E = codes->bytes; p.e_ls = codes->e_ls; p.e_ms = codes->e_ms; p.e_bs = codes->e_bs;
+  }
+  auto map = [](const Mat& t, int box_rows, int& order) {
+    return make_map(t.p, t.cols, t.rows, t.L, t.ms, t.ls, box_rows, order);
+  };
+  const CUtensorMap ta = map(A, lines::BM, p.a_mode), tb = map(B, b_kn ? lines::BK : BN, p.b_mode);
   // blocks of 64 columns (128 bytes) x 32 rows: an operand's map with another number of rows
-  auto block = [&](const at::Tensor& t, int& order) { return make_map(t.data_ptr(), N, M, L, t.stride(1), t.stride(0), 32, order); };
-  const CUtensorMap tcm = block(C, p.c_mode);
-  const CUtensorMap tx = X ? block(*X, p.x_mode) : tcm, tr = R ? block(*R, p.r_mode) : tcm;
+  const CUtensorMap tcm = map(C, 32, p.c_mode);
+  const CUtensorMap tx = X ? map(*X, 32, p.x_mode) : tcm, tr = R ? map(*R, 32, p.r_mode) : tcm;
   // rings: three stages of 48 KB beside 16 staged blocks, four beside 8
   auto go = [&](auto m) {
     constexpr int kMode = decltype(m)::value, kMore = kMode == lines::kPlain ? 1 : 0;
@@ -441,18 +441,15 @@ void run(const at::Tensor& A, const at::Tensor& B, const at::Tensor& C, const at
 
 }  // namespace
 
-// C[l] = A[l] @ B[l]^T (+ R[l]): A [L, M, K], B [L or 1, N, K] -- or, with b_kn, [L or 1, K, N] -- C and R [L, M, N] bf16 views.
-void tc_gemm_lines(at::Tensor A, at::Tensor B, at::Tensor C, c10::optional<at::Tensor> R, at::Tensor err, bool b_kn) {
-  run(A, B, C, nullptr, R ? &*R : nullptr, nullptr, nullptr, err, b_kn, lines::kPlain);
+// All run on the current device and stream.
+// C[l] = A[l] @ B[l]^T (+ R[l]): bf16, A [L, M, K], B [L or 1, N, K] -- or, with b_kn, [L or 1, K, N] -- C and R [L, M, N].
+void gemm_lines(const Mat& A, const Mat& B, const Mat& C, const Mat* R, int* err, bool b_kn) {
+  run(A, B, C, nullptr, R, nullptr, err, b_kn, lines::kPlain);
 }
-
-// The two GEMMs around pre-activations kept in 8 bits: codes [L, M, N] int8 views with rows on 16 bytes, exps [L, M, N / 32]
-// uint8 views of any strides. With X undefined (the up projection): C = GELU(A @ B^T), codes and exps are written. With X
-// (the down projection's data gradient): p = the values of codes, C = (A @ B^T) * GELU'(p), X = GELU(p).
-void tc_gemm_saved8(at::Tensor A, at::Tensor B, at::Tensor C, at::Tensor codes, at::Tensor exps, c10::optional<at::Tensor> X,
-                    at::Tensor err, bool b_kn) {
-  const bool use = X && X->defined();
-  run(A, B, C, use ? &*X : nullptr, nullptr, &codes, &exps, err, b_kn, use ? lines::kUse : lines::kSave);
+// The two GEMMs around pre-activations kept in 8 bits. Without X (the up projection): C = GELU(A @ B^T), the codes are
+// written. With X (the down projection's data gradient): p = the codes' values, C = (A @ B^T) * GELU'(p), X = GELU(p).
+void gemm_saved8(const Mat& A, const Mat& B, const Mat& C, const MatCodes& codes, const Mat* X, int* err, bool b_kn) {
+  run(A, B, C, X, nullptr, &codes, err, b_kn, X ? lines::kUse : lines::kSave);
 }
 
 }  // namespace pd

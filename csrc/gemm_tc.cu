@@ -33,11 +33,11 @@
 #include "common.cuh"
 #include "driver_api.h"
 #include "gemm_host.h"
+#include "gemm_mat.h"
 #include "tc_common.cuh"
 
 #include <cuda.h>
 
-#include <c10/cuda/CUDAGuard.h>
 #include <type_traits>
 
 namespace pd {
@@ -1019,23 +1019,23 @@ tc::WgParams wgrad_wide_plan(int64_t L, int64_t K, int64_t M, int64_t N, bool l_
   return p;
 }
 
-void run_wgrad_wide(const at::Tensor& A, const at::Tensor& B, const at::Tensor& C, tc::WgParams p, const at::Tensor& err) {
+void run_wgrad_wide(const Mat& A, const Mat& B, const at::Tensor& C, tc::WgParams p, int* err) {
   p.C = C.data_ptr(); p.c_ls = C.stride(0); p.c_ms = C.stride(1);
-  p.err = err.data_ptr<int>();
-  const CUtensorMap ta = make_map(A.data_ptr(), p.M, p.K, p.L, A.stride(1), A.stride(0), tc::BK, p.a_mode);
-  const CUtensorMap tb = make_map(B.data_ptr(), p.N, p.K, p.L, B.stride(1), B.stride(0), tc::BK, p.b_mode);
+  p.err = err;
+  const CUtensorMap ta = make_map(A.p, p.M, p.K, p.L, A.ms, A.ls, tc::BK, p.a_mode);
+  const CUtensorMap tb = make_map(B.p, p.N, p.K, p.L, B.ms, B.ls, tc::BK, p.b_mode);
   constexpr int smem = tc::kWideStages * 2 * 256 * tc::BK * 2;
   PD_CHECK_CUDA(cudaFuncSetAttribute(tc::wgrad_wide_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
   tc::launch_behind(tc::wgrad_wide_kernel, dim3(unsigned(std::min(p.items, num_sms()))), tc::kThreads, size_t(smem), ta, tb, p);
 }
 
 // direct: C in its own type, stored by the one split.
-void run_wgrad(const at::Tensor& A, const at::Tensor& B, const at::Tensor& C, tc::WgParams p, const at::Tensor& err, bool direct) {
+void run_wgrad(const Mat& A, const Mat& B, const at::Tensor& C, tc::WgParams p, int* err, bool direct) {
   p.C = C.data_ptr(); p.c_ls = C.stride(0); p.c_ms = C.stride(1);
-  p.err = err.data_ptr<int>();
+  p.err = err;
   // MN-major operands: [64 k-rows][64 cols] boxes over dims {cols, rows, L}
-  const CUtensorMap ta = make_map(A.data_ptr(), p.M, p.K, p.L, A.stride(1), A.stride(0), tc::BK, p.a_mode);
-  const CUtensorMap tb = make_map(B.data_ptr(), p.N, p.K, p.L, B.stride(1), B.stride(0), tc::BK, p.b_mode);
+  const CUtensorMap ta = make_map(A.p, p.M, p.K, p.L, A.ms, A.ls, tc::BK, p.a_mode);
+  const CUtensorMap tb = make_map(B.p, p.N, p.K, p.L, B.ms, B.ls, tc::BK, p.b_mode);
   const CUtensorMap tcm = direct ? make_line_map(C, p.M, p.N) : ta;
   auto go = [&](auto kern, int bn, int stages) {
     const size_t smem = size_t(stages) * (tc::BM * tc::BK * 2 + bn * tc::BK * 2) + 1024 + 1024 + (direct ? 8 * 4096 + 1024 : 0);
@@ -1072,35 +1072,35 @@ void tc_wgrad(at::Tensor A, at::Tensor B, at::Tensor C, at::Tensor err, bool l_s
                   reinterpret_cast<uintptr_t>(C.data_ptr()) % 16 == 0,
               "wgrad: C must be an fp32 [L, M, N] view with 16-byte aligned rows");
   if (K == 0 || L == 0) return;
-  run_wgrad(A, B, C, wgrad_plan(L, K, M, N, l_sum), err, false);
+  auto mat = [](const at::Tensor& t) { return Mat{t.data_ptr(), t.size(0), t.size(1), t.size(2), t.stride(0), t.stride(1)}; };
+  run_wgrad(mat(A), mat(B), C, wgrad_plan(L, K, M, N, l_sum), err.data_ptr<int>(), false);
 }
 
-// The weight gradient of tc_wgrad as a new tensor [L, M, N] (l_sum: [M, N]) of a type (fp32 or bf16). Where one split covers
-// the rows a tile leaves in that type at once; else it is added up in fp32 and converted.
-at::Tensor tc_wgrad_as(at::Tensor A, at::Tensor B, at::Tensor err, bool l_sum, int64_t dtype) {
-  check_operand(A, "A");
-  check_operand(B, "B");
-  const int64_t L = A.size(0), K = A.size(1), M = A.size(2), N = B.size(2);
+// The weight gradient of tc_wgrad (A [L, K, M], B [L, K, N], bf16) as a new tensor [L, M, N] (l_sum: [M, N]) of a type, on the
+// current device and stream. Where one split covers the rows a tile leaves in that type at once (fp32 or bf16); else it is
+// added up in fp32 and converted.
+at::Tensor wgrad_as(const Mat& A, const Mat& B, const at::Device& device, int* err, bool l_sum, int64_t dtype) {
+  const int64_t L = A.L, K = A.rows, M = A.cols, N = B.cols, LC = l_sum ? 1 : L;
   const auto type = at::ScalarType(dtype);
-  PD_CHECK(B.size(0) == L && B.size(1) == K, "B must be [L, K, N] over the same rows as A");
+  PD_CHECK(B.L == L && B.rows == K, "B must be [L, K, N] over the same rows as A");
   PD_CHECK(M % 64 == 0 && N % 64 == 0, "wgrad: M and N must be multiples of 64");
-  PD_CHECK(B.device() == A.device() && err.device() == A.device(), "wgrad: operands lie on two devices");
-  const c10::cuda::CUDAGuard guard(A.device());
-  const int64_t LC = l_sum ? 1 : L;
-  const auto fp32 = A.options().dtype(at::kFloat);
+  PD_CHECK(K < (int64_t(1) << 31) && L * ((K + 63) / 64) < (int64_t(1) << 30), "wgrad: too many rows");
+  auto out = [&](bool zeros, at::ScalarType t) {
+    const auto options = at::TensorOptions().dtype(t).device(device);
+    const std::vector<int64_t> shape = {LC, M, N};
+    return zeros ? at::zeros(shape, options) : at::empty(shape, options);
+  };
   at::Tensor C;
   if (K == 0 || L == 0) {
-    C = at::zeros({LC, M, N}, A.options().dtype(type));
+    C = out(true, type);
+  } else if (const tc::WgParams wide = wgrad_wide_plan(L, K, M, N, l_sum); M % 256 == 0 && N % 256 == 0 && wide.splits > 1) {
+    C = out(true, at::kFloat);
+    run_wgrad_wide(A, B, C, wide, err);
+    C = C.to(type);
   } else {
-    if (M % 256 == 0 && N % 256 == 0 && wgrad_wide_plan(L, K, M, N, l_sum).splits > 1) {
-      C = at::zeros({LC, M, N}, fp32);
-      run_wgrad_wide(A, B, C, wgrad_wide_plan(L, K, M, N, l_sum), err);
-      C = C.to(type);
-      return l_sum ? C.squeeze(0) : C;
-    }
     const tc::WgParams p = wgrad_plan(L, K, M, N, l_sum);
     const bool direct = p.splits == 1 && (type == at::kFloat || type == at::kBFloat16);
-    C = direct ? at::empty({LC, M, N}, A.options().dtype(type)) : at::zeros({LC, M, N}, fp32);
+    C = out(!direct, direct ? type : at::kFloat);
     run_wgrad(A, B, C, p, err, direct);
     C = C.to(type);
   }

@@ -432,6 +432,29 @@ def test_every_row_has_its_own_weight():
     assert dw.eq(0).all() and dwn.ne(0).any() and dx.isfinite().all()
 
 
+@pytest.mark.parametrize("B,T,NS", [(40, 1, 0), (40, 1, 1), (4, 9, 3), (1, 9, 3)])
+def test_layers_of_views(B, T, NS):
+    """Any stride over an axis of length 1, samples in two orders, an incoming gradient off 16 bytes: as of copies.
+
+    One block of 64 rows covers each sum over rows, so no order of additions changes a weight's gradient."""
+    def layers(x, z, dy):
+        parts = [x.detach().requires_grad_(), z.detach().requires_grad_(),
+                 *(t.requires_grad_() for t in _parts(B, T, 64, 128, NS, seed=8)[2:])]
+        out = dense.mixed_ffn(parts[0], parts[1], T - NS, *parts[2:], save8=True)
+        y = dense.mixed_linear(parts[0], T - NS, parts[2][:64], parts[4][:, :64], act="gelu", save8=True)
+        return [out.detach(), y.detach(), *torch.autograd.grad((out, y), parts, (dy, dy))]
+
+    x, z, dy = (t.clone() for t in (*_parts(B, T, 64, 128, NS, seed=8)[:2], _parts(B, T, 64, 128, NS, seed=9)[0]))
+    turned = [t.transpose(0, 1).contiguous().transpose(0, 1) for t in (x, z)]
+    if T == 1 and B > 1:
+        turned = [t.as_strided(t.shape, (64, 64 * B, 1)) for t in (x, z)]
+        assert all(t.is_contiguous() and t.stride(1) == 64 * B for t in turned)
+    off = torch.cat([dy.new_zeros(1), dy.flatten()])[1:].view(dy.shape)
+    assert off.data_ptr() % 16
+    for a, b in zip(layers(*turned, off), layers(x, z, dy)):
+        assert torch.equal(a, b)
+
+
 def test_calls_at_once():
     """Two threads, each on its own stream, with rows for every form of the product."""
     import threading
