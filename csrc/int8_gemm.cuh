@@ -232,8 +232,7 @@ __global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_const
       const int m0 = mb * BM + q * 32, n0 = nb * p.bn, row = m0 + lane;
       const bool there = row < p.M;
       const float s = there ? p.s[l * p.s_ls + row * p.s_ms] : 0.0f;
-      // sums are below 2^31: past this no scaled one overflows (a NaN scale counts as large)
-      const uint32_t s_most = p.act == kGelu ? __reduce_max_sync(0xffffffffu, abs_bits(s)) : 0;
+      const float s_most = __uint_as_float(p.act == kGelu ? __reduce_max_sync(0xffffffffu, abs_bits(s)) : 0u);
       const int c_end = min(p.bn, p.N - n0);
       auto column = [&](int c) {                          // (t, bias) of this lane's column of chunk c
         const int n = n0 + c + lane;
@@ -251,9 +250,10 @@ __global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_const
         tcx::tc_ld32_issue(tbase + c, r);
         cols[slot] = tb.x;
         cols[slot + 2] = tb.y;
-        // |sum * s * t| < 2^31 * s * t: GELU's guard is needed where that may pass the largest number
+        // GELU's guard is needed where minus infinity may come out: |sum * s * t + bias| < 2^31 * s * t + |bias|, in range where
+        // neither passes 1e28. Each lane asks for its own column, so that a channel without a number hides no other; NaN asks.
         const bool guard = p.act == kGelu &&
-                           __uint_as_float(s_most) * __uint_as_float(__reduce_max_sync(0xffffffffu, abs_bits(tb.x))) > 1e28f;
+                           __any_sync(0xffffffffu, !(s_most * fabsf(tb.x) <= 1e28f && fabsf(tb.y) <= 1e28f));
         __syncwarp();
         tb = column(c + kParts * 32);                             // the next chunk's, on its way
         tcx::tc_ld_wait(r);
@@ -265,7 +265,7 @@ __global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_const
           pk2_split(pk2_fma(pk2(float(int(r[i])), float(int(r[i + 1]))), pk2_mul(s2, tb2.x), tb2.y), v[i], v[i + 1]);
         }
         if (p.act == kGelu) {
-          if (guard || !(__uint_as_float(s_most) < 1e30f)) {
+          if (guard) {
 #pragma unroll
             for (int i = 0; i < 32; ++i) v[i] = from_below(v[i]);
           }

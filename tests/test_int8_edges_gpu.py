@@ -1,0 +1,42 @@
+"""Products of 8-bit integers and layers with activations in 8 bits, where they meet values and calls at the edge."""
+import math
+
+import pytest
+import torch
+
+from primus_dlrm_b200.ops.int8 import Int8Weight, _linear_ref, int8_linear
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+TYPES = [torch.bfloat16, torch.float16, torch.float32]
+
+
+def _gen(seed=0):
+    return torch.Generator(device=DEV).manual_seed(seed)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows", [1, 40, 3000])
+def test_gelu_of_minus_infinity(rows, dtype):
+    """GELU of a bias of minus infinity, and of a sum that overflows to it, is 0 in every form of the product (chosen by the
+    rows), beside channels without a number too; NaN stays NaN and plus infinity stays."""
+    g = _gen(rows)
+    codes = torch.randint(-127, 128, (300, 256), generator=g, device=DEV, dtype=torch.int8)
+    scale = torch.full((300,), 1e-6, device=DEV)
+    codes[[3, 70]] = 127
+    scale[[3, 70]] = 1e33                                    # 127 * 127 * 256 * (1e4 / 127) * 1e33 passes every type
+    scale[4] = math.nan
+    bias = torch.zeros(300, device=DEV)
+    bias[[7, 133, 299]] = -math.inf
+    w = Int8Weight.from_tensors(codes, scale)
+    sign = torch.where(torch.arange(rows, device=DEV) % 2 == 0, -1.0, 1.0)[:, None]
+    x = (sign * 1e4).expand(rows, 256).to(dtype)
+    for b in (bias, None):
+        y, ref = int8_linear(x, w, b, act="gelu"), _linear_ref(x, w, b, "gelu", None)
+        assert y[:, 4].isnan().all() and torch.equal(y.isnan(), ref.isnan())
+        low = (sign < 0).expand(rows, 1)
+        for c in (3, 70):
+            assert torch.equal(y[:, c:c + 1], torch.where(low, 0.0, math.inf).to(dtype))
+        if b is not None:
+            assert y[:, [7, 133, 299]].eq(0).all()
+        assert torch.equal(y.isinf(), ref.isinf())
