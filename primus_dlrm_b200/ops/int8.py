@@ -22,6 +22,7 @@ import torch
 import torch.nn.functional as F
 
 from primus_dlrm_b200.ops import _ext
+from primus_dlrm_b200.ops.saved8 import no_tangent
 
 _TYPES = (torch.bfloat16, torch.float16, torch.float32)
 _ACT = {None: 0, "": 0, "gelu": 1, "relu": 2}
@@ -44,10 +45,12 @@ def _quantize_ref(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
 def quantize_rows(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     """Int8 codes of ``x`` ``[..., K]`` (bf16, fp16 or fp32) and the fp32 scale
     ``[...]`` of each row; ``codes * scale`` is within half a scale of ``x``.  A
-    row with a NaN or an infinity has codes of 0 and a scale of NaN."""
+    row with a NaN or an infinity has codes of 0 and a scale of NaN.  Not
+    differentiable: the results carry no graph."""
     if x.dim() == 0 or x.dtype not in _TYPES:
         raise ValueError(f"quantize_rows: a bf16, fp16 or fp32 tensor with a last dim is expected, not {x.dtype} of "
                          f"{x.dim()} dims")
+    no_tangent("quantize_rows", x)
     x = x.detach()
     if not _native(x):
         return _quantize_ref(x)
@@ -75,6 +78,7 @@ class Int8Weight:
             raise ValueError("codes must be int8 [N, K] or [L, N, K]")
         if scale.dtype != torch.float32 or scale.shape != codes.shape[:-1] or scale.device != codes.device:
             raise ValueError("scale must be fp32 with one value for each row of codes, on their device")
+        no_tangent("Int8Weight", scale)
         K = codes.shape[-1]
         if min(codes.shape) < 1 or K > MAX_FEATURES:
             raise ValueError(f"a weight of {tuple(codes.shape)}: 1 to {MAX_FEATURES} input features, and at least one "
@@ -146,7 +150,8 @@ def int8_linear(x: torch.Tensor, weight: Int8Weight, bias: torch.Tensor | None =
     where the weight has a matrix for each of L positions), ``bias`` ``[N]``,
     ``act`` None, ``"gelu"`` or ``"relu"``; ``residual`` has the result's shape
     ``[..., N]`` and ``x``'s type, which is the result's too.  A gradient asked
-    of the result raises in the backward pass.
+    of the result raises in the backward pass, a forward-mode tangent of an
+    input at once.
     """
     code = _ACT.get(act)
     if code is None:
@@ -165,6 +170,7 @@ def int8_linear(x: torch.Tensor, weight: Int8Weight, bias: torch.Tensor | None =
         raise ValueError("int8_linear: bias must be [N]")
     if residual is not None and (residual.shape != shape or residual.dtype != x.dtype):
         raise ValueError("int8_linear: residual must have the result's shape and x's type")
+    no_tangent("int8_linear", x, bias, residual)
     with torch.no_grad(), torch.autocast(x.device.type, enabled=False):
         y = _linear_ref(x, weight, bias, act, residual)
     inputs = [t for t in (x, bias, residual) if t is not None and t.requires_grad] if torch.is_grad_enabled() else []

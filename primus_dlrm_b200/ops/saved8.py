@@ -20,6 +20,7 @@ from __future__ import annotations
 import os
 
 import torch
+from torch.autograd import forward_ad
 
 from primus_dlrm_b200.ops import _ext
 
@@ -52,6 +53,13 @@ class Saved8:
 
 def _native(t: torch.Tensor) -> bool:
     return t.is_cuda and os.environ.get("PD_KERNELS") != "eager"
+
+
+def no_tangent(who: str, *tensors: torch.Tensor | None) -> None:
+    """Forward-mode derivatives do not pass through codes: refused, not dropped."""
+    for t in tensors:
+        if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+            raise RuntimeError(f"{who} has no forward-mode derivative")
 
 
 def _save_ref(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
@@ -91,6 +99,7 @@ def save8(x: torch.Tensor) -> Saved8:
     if _native(x):
         codes, scale_bytes = _ext.int8().save8(x)
     else:
+        no_tangent("save8", x)
         codes, scale_bytes = _save_ref(x.detach().reshape(x.shape[:-1].numel(), x.shape[-1]))
     return Saved8(codes, scale_bytes, x.shape, x.dtype)
 

@@ -1,0 +1,30 @@
+"""Products of 8-bit integers and layers with activations in 8 bits on the CPU: calls at the edge."""
+import pytest
+import torch
+from torch.autograd import forward_ad
+
+from primus_dlrm_b200.ops import dense
+from primus_dlrm_b200.ops.int8 import Int8Weight, int8_linear, quantize_rows
+from primus_dlrm_b200.ops.saved8 import load8, save8
+
+
+def test_tangents_are_refused():
+    """Forward-mode derivatives are refused as on the GPU, not dropped and not taken of the scales alone."""
+    w, x = Int8Weight.from_float(torch.randn(5, 20)), torch.randn(4, 20)
+    bias, res = torch.randn(5), torch.randn(4, 5)
+    layer = [torch.randn(s).requires_grad_() for s in ((2, 7, 64), (2, 7, 64), (64, 64), (64, 64), (3, 64, 64), (3, 64, 64))]
+    plain, saved = int8_linear(x, w, bias, residual=res), save8(x)
+    with forward_ad.dual_level():
+        dual = lambda t: forward_ad.make_dual(t.detach(), torch.ones_like(t))  # noqa: E731
+        for bad in (lambda: int8_linear(dual(x), w), lambda: int8_linear(x, w, dual(bias)),
+                    lambda: int8_linear(x, w, residual=dual(res)), lambda: quantize_rows(dual(x)),
+                    lambda: Int8Weight.from_float(dual(x)), lambda: Int8Weight.from_tensors(w.codes, dual(w.scale)),
+                    lambda: save8(dual(x)), lambda: dense.mixed_linear(dual(layer[0]), 4, layer[2], layer[4], save8=True),
+                    lambda: dense.mixed_ffn(dual(layer[0]), layer[1], 4, *layer[2:], save8=True)):
+            with pytest.raises(RuntimeError, match="forward"):
+                bad()
+        # inside a level, but without a tangent
+        assert torch.equal(int8_linear(x, w, bias, residual=res), plain) and torch.equal(save8(x).codes, saved.codes)
+        assert torch.equal(load8(saved), load8(save8(x)))
+    with torch.inference_mode():
+        assert torch.equal(int8_linear(x, w, bias, residual=res), plain)

@@ -4,7 +4,7 @@ import math
 import pytest
 import torch
 
-from primus_dlrm_b200.ops.int8 import Int8Weight, _linear_ref, int8_linear
+from primus_dlrm_b200.ops.int8 import Int8Weight, _linear_ref, int8_linear, quantize_rows
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda"
@@ -40,3 +40,12 @@ def test_gelu_of_minus_infinity(rows, dtype):
         if b is not None:
             assert y[:, [7, 133, 299]].eq(0).all()
         assert torch.equal(y.isinf(), ref.isinf())
+
+
+def test_row_codes_refuse_tangents():
+    from torch.autograd import forward_ad
+    x = torch.randn(4, 20, device=DEV)
+    with forward_ad.dual_level():
+        for bad in (lambda t: quantize_rows(t), lambda t: Int8Weight.from_float(t)):
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                bad(forward_ad.make_dual(x, x))
