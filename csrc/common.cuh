@@ -13,6 +13,7 @@
 #include <ATen/ops/zeros.h>
 #include <ATen/ops/zeros_like.h>
 #include <ATen/ops/from_blob.h>
+#include <c10/core/InferenceMode.h>
 #include <c10/cuda/CUDAStream.h>
 #include <c10/util/Exception.h>
 #include <atomic>
@@ -51,6 +52,14 @@ enum ErrorCode : int {
   kWaitTimeout = 2,
   kBadShape = 3,
 };
+
+// A static error word of the current device as a tensor [1], readable in a stream's order. Its memory belongs to the module:
+// no allocation, so a call inside a graph capture may be the first one.
+inline at::Tensor word_tensor(int* word, int64_t device) {
+  const c10::InferenceMode normal(false);                  // may be cleared, and named by a backward pass, in any mode
+  const at::Device cuda(at::kCUDA, c10::DeviceIndex(device));
+  return at::from_blob(word, {1}, [](void*) {}, at::TensorOptions().dtype(at::kInt).device(cuda), cuda);
+}
 
 // Number of kernels this library has launched (read by benchmarks to report
 // how many of their kernels ran inside a timed region).

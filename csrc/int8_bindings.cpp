@@ -14,7 +14,7 @@ at::Tensor load8(at::Tensor, at::Tensor, int64_t);
 std::vector<at::Tensor> quantize_rows(at::Tensor);
 at::Tensor linear(at::Tensor, at::Tensor, at::Tensor, int64_t, bool, c10::optional<at::Tensor>, int64_t,
                   c10::optional<at::Tensor>);
-int64_t error_code(int64_t);
+at::Tensor error_tensor(int64_t);
 }  // namespace i8
 long long launches();
 }  // namespace pd
@@ -65,7 +65,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         "values of save8's codes and scale bytes in a type");
   m.def("quantize_rows", &pd::i8::quantize_rows, "x [outer, inner, K] -> int8 codes, fp32 scales [outer, inner]");
   m.def("linear", &linear, "act(x W^T + bias) + residual by 8-bit integers");
-  m.def("error_code", &pd::i8::error_code, "the device's error word (2: a bounded wait ran out)");
+  m.def("error_word", &pd::i8::error_tensor, "the device's int32 error word (2: a bounded wait ran out)");
   m.def("launch_count", &pd::launches);
 }
 

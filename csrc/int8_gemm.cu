@@ -30,11 +30,9 @@ static int* error_word() {
   return w;
 }
 
-int64_t error_code(int64_t device) {
+at::Tensor error_tensor(int64_t device) {
   const c10::cuda::CUDAGuard guard{c10::DeviceIndex(device)};
-  int v = 0;
-  PD_CHECK_CUDA(cudaMemcpyFromSymbol(&v, g_err, sizeof(int)));
-  return v;
+  return word_tensor(error_word(), device);
 }
 
 // Rows of a [..., K] tensor (or [..., L, K]) as they lie: row m of position l at `at` + m * outer + l * inner elements.

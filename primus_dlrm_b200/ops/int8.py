@@ -177,8 +177,13 @@ def int8_linear(x: torch.Tensor, weight: Int8Weight, bias: torch.Tensor | None =
     return _NoGradient.apply(y, *inputs) if inputs else y
 
 
-def int8_error_code(device) -> int:
-    """Error word of the integer products on ``device`` (0 = ok, 2 = a bounded
-    wait ran out, 4 = a block's shared memory was not aligned)."""
+def _err_word(device) -> torch.Tensor:
     device = torch.device(device)
-    return _ext.int8().error_code(torch.cuda.current_device() if device.index is None else device.index)
+    return _ext.int8().error_word(torch.cuda.current_device() if device.index is None else device.index)
+
+
+def int8_error_code(device) -> int:
+    """Error word of the integer products on ``device``, behind what the current
+    stream holds (0 = ok, 2 = a bounded wait ran out, 4 = a block's shared
+    memory was not aligned)."""
+    return int(_err_word(device).item())

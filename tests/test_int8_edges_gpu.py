@@ -49,3 +49,20 @@ def test_row_codes_refuse_tangents():
         for bad in (lambda t: quantize_rows(t), lambda t: Int8Weight.from_float(t)):
             with pytest.raises(RuntimeError, match="forward-mode"):
                 bad(forward_ad.make_dual(x, x))
+
+
+def test_error_word_follows_the_current_stream():
+    """The code is that of the calls before it on the current stream, a stream of its own too; and 0 on a fresh word."""
+    from primus_dlrm_b200.ops.int8 import _err_word, int8_error_code
+    assert int8_error_code(DEV) == 0
+    word, side = _err_word(DEV), torch.cuda.Stream()
+    assert word.shape == (1,) and word.dtype == torch.int32 and not word.is_inference()
+    side.wait_stream(torch.cuda.current_stream())
+    try:
+        with torch.cuda.stream(side):
+            torch.cuda._sleep(20_000_000)                    # some 10 ms
+            word.fill_(2)
+            assert int8_error_code(DEV) == 2
+    finally:
+        word.zero_()
+    assert int8_error_code(DEV) == 0
