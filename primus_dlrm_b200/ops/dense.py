@@ -56,7 +56,10 @@ def _err(device) -> torch.Tensor:
 
 def gemm_error_code(device) -> int:
     """Error word of the tcgen05 GEMMs on ``device`` (2 = a pipeline wait timed out)."""
-    e = _err_words.get(torch.device(device))
+    device = torch.device(device)
+    if device.type == "cuda" and device.index is None:       # the words are kept by index
+        device = torch.device("cuda", torch.cuda.current_device())
+    e = _err_words.get(device)
     return int(e.item()) if e is not None else 0
 
 
