@@ -46,21 +46,19 @@ _EPI = {"": 0, None: 0, "gelu": 1, "residual": 2, "dgelu": 3, "gelu_d": 4, "mul"
 _err_words: dict = {}
 
 
-def _err(device) -> torch.Tensor:
+def _err(device: torch.device) -> torch.Tensor:
     e = _err_words.get(device)
     if e is None:
-        e = torch.zeros(1, dtype=torch.int32, device=device)
-        _err_words[device] = e
+        e = _err_words[device] = _ext.gemm().error_word(device.index)
     return e
 
 
 def gemm_error_code(device) -> int:
     """Error word of the tcgen05 GEMMs on ``device`` (2 = a pipeline wait timed out)."""
     device = torch.device(device)
-    if device.type == "cuda" and device.index is None:       # the words are kept by index
-        device = torch.device("cuda", torch.cuda.current_device())
-    e = _err_words.get(device)
-    return int(e.item()) if e is not None else 0
+    if device.type != "cuda":
+        return 0
+    return int(_err(torch.device("cuda", torch.cuda.current_device() if device.index is None else device.index)).item())
 
 
 def tc_gemm(A: torch.Tensor, B: torch.Tensor, C: torch.Tensor, epi: str | None = None,

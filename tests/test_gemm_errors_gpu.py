@@ -1,4 +1,7 @@
 """The error word of the GEMMs."""
+import subprocess
+import sys
+from pathlib import Path
 
 import pytest
 import torch
@@ -17,3 +20,35 @@ def test_a_device_without_an_index_is_the_current_one():
     finally:
         word.zero_()
     assert dense.gemm_error_code("cuda") == 0
+
+
+def test_a_first_call_inside_a_capture():
+    """The word of a process whose first GEMM is captured is 0 before the replay, and a replay does not clear what it holds;
+    made under inference mode, it serves a training step. In a process of its own."""
+    code = """
+import sys
+sys.path.insert(0, %r)
+import torch
+from primus_dlrm_b200.ops import dense
+t = [torch.zeros(1, 64, 64, device="cuda").bfloat16() for _ in range(3)]
+torch.cuda.synchronize()
+graph = torch.cuda.CUDAGraph()
+with torch.inference_mode(), torch.cuda.graph(graph):
+    dense.tc_gemm(*t)
+word = dense._err(t[0].device)
+print("INFERENCE", word.is_inference())
+print("BEFORE", int(word.item()))
+with torch.inference_mode():
+    word.fill_(2)
+graph.replay()
+print("AFTER", int(word.item()))
+with torch.inference_mode():
+    word.zero_()
+x, w = (torch.ones(1, 64, 64, device="cuda").bfloat16().requires_grad_() for _ in range(2))
+y = dense.mixed_linear(x, 64, w[0], w[:0], save8=True)
+y.sum().backward()
+print("TRAINED", float(x.grad[0, 0, 0]))
+""" % str(Path(__file__).resolve().parent.parent)
+    r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0, r.stdout + r.stderr[-1500:]
+    assert all(m in r.stdout for m in ("INFERENCE False", "BEFORE 0", "AFTER 2", "TRAINED 64.0")), r.stdout
