@@ -31,7 +31,7 @@ from primus_dlrm_b200.config import Config
 from primus_dlrm_b200.models.base import BaseModel
 from primus_dlrm_b200.models.embedding import Embeddings
 from primus_dlrm_b200.models.heads import fused_heads_loss
-from primus_dlrm_b200.ops import dense
+from primus_dlrm_b200.ops import dense, int8
 from primus_dlrm_b200.ops.attention import (
     _native_ok as _fmha_native_ok, causal_attention_all_rows, pyramid_attention, pyramid_attention_qkv,
 )
@@ -517,6 +517,8 @@ class OneTransModel(BaseModel):
             scores.append(self.heads[task](hh).squeeze(-1).float())
         for pages in cache if kv_cache else ():
             pages.cache.check_errors()
+        if weights and not (xs.is_cuda and torch.cuda.is_current_stream_capturing()):    # a graph's launches are read later
+            int8.check_errors(xs.device)
         return torch.cat(scores)
 
     def _ns_raw(self, batch: dict[str, torch.Tensor]) -> torch.Tensor:

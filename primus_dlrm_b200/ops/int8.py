@@ -187,3 +187,16 @@ def int8_error_code(device) -> int:
     stream holds (0 = ok, 2 = a bounded wait ran out, 4 = a block's shared
     memory was not aligned)."""
     return int(_err_word(device).item())
+
+
+def check_errors(device) -> None:
+    """Raises (and clears the word) if a product of integers on ``device`` gave
+    up: results behind it are not to be used.  Waits for the current stream."""
+    if torch.device(device).type != "cuda" or os.environ.get("PD_KERNELS") == "eager":
+        return
+    code = int8_error_code(device)
+    if code:
+        _err_word(device).zero_()
+        raise RuntimeError({2: "int8_linear: a bounded wait in a kernel ran out",
+                            4: "int8_linear: a kernel's shared memory is not aligned"}.get(
+                                code, f"int8_linear: error {code}"))

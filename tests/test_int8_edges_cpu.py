@@ -28,3 +28,30 @@ def test_tangents_are_refused():
         assert torch.equal(load8(saved), load8(save8(x)))
     with torch.inference_mode():
         assert torch.equal(int8_linear(x, w, bias, residual=res), plain)
+
+
+def test_scoring_reports_a_product_that_gave_up(monkeypatch):
+    """Scores of integer weights do not leave before the products' error word was read; those of others do not read it."""
+    from primus_dlrm_b200.ops import int8
+    from test_models_cpu import _batch
+    from test_onetrans_rotary import _model, _split
+    model = _model(rotary=True)
+    user, cand, _ = _split(_batch(B=5, L=30, windows=2, seed=5), 5)
+    w8, asked = model.int8_weights(), []
+    want = model.score_candidates(user, cand, "listen_plus", weights=w8)
+    monkeypatch.setattr(int8, "check_errors", lambda device: asked.append(device))
+    assert torch.equal(model.score_candidates(user, cand, "listen_plus", weights=w8), want) and asked == [torch.device("cpu")]
+    model.score_candidates(user, cand, "listen_plus")
+    assert len(asked) == 1
+
+    # the code that a kernel leaves, read from a stub: raised once, and cleared
+    monkeypatch.undo()
+    word = torch.tensor([2], dtype=torch.int32)
+    monkeypatch.setattr(int8, "_err_word", lambda device: word)
+    with pytest.raises(RuntimeError, match="wait"):
+        int8.check_errors("cuda")
+    int8.check_errors("cuda")
+    word.fill_(4)
+    int8.check_errors("cpu")
+    with pytest.raises(RuntimeError, match="aligned"):
+        int8.check_errors("cuda:0")

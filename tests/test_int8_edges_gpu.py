@@ -66,3 +66,18 @@ def test_error_word_follows_the_current_stream():
     finally:
         word.zero_()
     assert int8_error_code(DEV) == 0
+
+
+@pytest.mark.parametrize("kv_cache", [None, "fp8"])
+def test_scoring_reports_a_product_that_gave_up(kv_cache):
+    from primus_dlrm_b200.ops.int8 import _err_word
+    from test_models_cpu import _batch
+    from test_onetrans_rotary import _model, _split
+    model = _model(DEV, rotary=True, attention_impl="fav4")
+    user, cand, _ = _split({k: v.cuda() for k, v in _batch(B=9, L=40, windows=2, seed=5).items()}, 9)
+    w8 = model.int8_weights()
+    want = model.score_candidates(user, cand, "listen_plus", kv_cache=kv_cache, weights=w8)
+    _err_word(DEV).fill_(2)
+    with pytest.raises(RuntimeError, match="int8_linear: a bounded wait"):
+        model.score_candidates(user, cand, "listen_plus", kv_cache=kv_cache, weights=w8)
+    assert torch.equal(model.score_candidates(user, cand, "listen_plus", kv_cache=kv_cache, weights=w8), want)
