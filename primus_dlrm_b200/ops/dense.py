@@ -46,19 +46,29 @@ _EPI = {"": 0, None: 0, "gelu": 1, "residual": 2, "dgelu": 3, "gelu_d": 4, "mul"
 _err_words: dict = {}
 
 
-def _err(device: torch.device) -> torch.Tensor:
+def _err(device) -> torch.Tensor:
     e = _err_words.get(device)
     if e is None:
+        device = torch.device(device)
+        if device.index is None:
+            return _err(torch.device(device.type, torch.cuda.current_device()))
         e = _err_words[device] = _ext.gemm().error_word(device.index)
     return e
 
 
 def gemm_error_code(device) -> int:
     """Error word of the tcgen05 GEMMs on ``device`` (2 = a pipeline wait timed out)."""
-    device = torch.device(device)
-    if device.type != "cuda":
-        return 0
-    return int(_err(torch.device("cuda", torch.cuda.current_device() if device.index is None else device.index)).item())
+    return int(_err(device).item()) if torch.device(device).type == "cuda" else 0
+
+
+def check_errors(device) -> None:
+    """Raises (and clears the word) if a GEMM on ``device`` gave up: results
+    behind it are not to be used.  Waits for the current stream."""
+    code = gemm_error_code(device) if _ext.native_enabled(device) else 0
+    if code:
+        _err(device).zero_()
+        raise RuntimeError({2: "GEMM: a bounded wait in a kernel ran out",
+                            3: "GEMM: a kernel's shared memory is not aligned"}.get(code, f"GEMM: error {code}"))
 
 
 def tc_gemm(A: torch.Tensor, B: torch.Tensor, C: torch.Tensor, epi: str | None = None,
