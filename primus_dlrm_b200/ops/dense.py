@@ -236,6 +236,14 @@ def _no_autocast(x: torch.Tensor):
     return torch.autocast(x.device.type, enabled=False)
 
 
+def _as_products_take(x: torch.Tensor) -> torch.Tensor:
+    """x in the type in which the 16-bit layers multiply it: autocast's, but for bf16 on a GPU, which has its own kernels."""
+    kind = x.device.type
+    if torch.is_autocast_enabled(kind) and x.dtype != torch.float64 and not (x.is_cuda and x.dtype == torch.bfloat16):
+        return x.to(torch.get_autocast_dtype(kind))
+    return x
+
+
 def _ffn_forward(x, z, w1, w2, wn1, wn2, n_s: int):
     """z + W2(GELU(W1 x)) with nothing kept."""
     if _ffn_native_ok(x, z, w2.shape[0], w1.shape[0]):
@@ -290,6 +298,7 @@ def mixed_ffn(x: torch.Tensor, z: torch.Tensor, n_s: int, w1, w2, wn1, wn2, save
     for every input (through PyTorch where the native GEMM cannot), never None.
     """
     if save8:
+        x = _as_products_take(x)
         if not (torch.is_grad_enabled() and any(t.requires_grad for t in (x, z, w1, w2, wn1, wn2))):
             return _ffn_forward(x, z, w1, w2, wn1, wn2, n_s)
         if _ffn_native_ok(x, z, w2.shape[0], w1.shape[0]):
@@ -383,6 +392,7 @@ def mixed_linear(x: torch.Tensor, n_s: int, w_s: torch.Tensor, w_ns: torch.Tenso
     gradient are the same (with a GELU its derivative is taken at the 8-bit
     values), the weights' gradients carry the rounding of the 8-bit input."""
     if save8 and torch.is_grad_enabled() and any(t.requires_grad for t in (x, w_s, w_ns)):
+        x = _as_products_take(x)
         if _gemm_ok(x) and _tc_ok(x, x.shape[-1], w_s.shape[0]) and x.shape[-1] % 64 == 0:
             _ext.int8()                                      # its kernels save and load
             return _ext.gemm().mixed_linear_saved8(x, w_s, w_ns, n_s, act == "gelu", _err(x.device))

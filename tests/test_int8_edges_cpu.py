@@ -55,3 +55,40 @@ def test_scoring_reports_a_product_that_gave_up(monkeypatch):
     int8.check_errors("cpu")
     with pytest.raises(RuntimeError, match="aligned"):
         int8.check_errors("cuda:0")
+
+
+def _layer_parts(dtype, seed=0, D=64, F_=128):
+    g = torch.Generator().manual_seed(seed)
+    r = lambda *s: torch.randn(*s, generator=g)  # noqa: E731
+    x, z = r(2, 9, D).to(dtype), r(2, 9, D).to(dtype)
+    return [t.requires_grad_() for t in (x, z, r(F_, D) / D ** 0.5, r(D, F_) / F_ ** 0.5, r(3, F_, D) / D ** 0.5, r(3, D, F_) / F_ ** 0.5)]
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16, torch.float64])
+@pytest.mark.parametrize("act", [None, "gelu"])
+def test_projection_under_autocast(dtype, act):
+    """The output is that of the 16-bit layer, its type too; gradients come in the types of the inputs."""
+    x, _, w, _, wn, _ = _layer_parts(dtype)
+    w, wn = (t.detach().to(dtype if dtype == torch.float64 else torch.float32).requires_grad_() for t in (w, wn))
+    with torch.autocast("cpu", dtype=torch.bfloat16):
+        a, b = (dense.mixed_linear(x, 6, w, wn, act=act, save8=s) for s in (False, True))
+    assert a.dtype == b.dtype and torch.equal(a, b)
+    ga, gb = (torch.autograd.grad(y, (x, w, wn), torch.ones_like(y)) for y in (a, b))
+    for u, v, t in zip(ga, gb, (x, w, wn)):
+        assert v.dtype == t.dtype and (u.double() - v.double()).norm() <= 0.03 * u.double().norm()
+
+
+@pytest.mark.parametrize("ztype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+def test_ffn_under_autocast(dtype, ztype):
+    x, z, w1, w2, wn1, wn2 = _layer_parts(dtype)
+    z = z.detach().to(ztype).requires_grad_()
+    with torch.autocast("cpu", dtype=torch.bfloat16):
+        a = z + dense.mixed_linear(dense.mixed_linear(x, 6, w1, wn1, act="gelu"), 6, w2, wn2)
+        b = dense.mixed_ffn(x, z, 6, w1, w2, wn1, wn2, save8=True)
+        with torch.no_grad():
+            c = dense.mixed_ffn(x, z, 6, w1, w2, wn1, wn2, save8=True)
+    assert a.dtype == b.dtype == c.dtype and torch.equal(a, b) and torch.equal(a, c)
+    leaves = (x, z, w1, w2, wn1, wn2)
+    for u, v, t in zip(*(torch.autograd.grad(y, leaves, torch.ones_like(y)) for y in (a, b)), leaves):
+        assert v.dtype == t.dtype and (u.double() - v.double()).norm() <= 0.03 * u.double().norm()

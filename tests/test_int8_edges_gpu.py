@@ -4,6 +4,7 @@ import math
 import pytest
 import torch
 
+from primus_dlrm_b200.ops import dense
 from primus_dlrm_b200.ops.int8 import Int8Weight, _linear_ref, int8_linear, quantize_rows
 
 pytestmark = pytest.mark.gpu
@@ -81,3 +82,28 @@ def test_scoring_reports_a_product_that_gave_up(kv_cache):
     with pytest.raises(RuntimeError, match="int8_linear: a bounded wait"):
         model.score_candidates(user, cand, "listen_plus", kv_cache=kv_cache, weights=w8)
     assert torch.equal(model.score_candidates(user, cand, "listen_plus", kv_cache=kv_cache, weights=w8), want)
+
+
+@pytest.mark.parametrize("D,F_", [(64, 128), (40, 72)])
+@pytest.mark.parametrize("dtype,ztype", [(torch.float32, torch.float32), (torch.float32, torch.bfloat16),
+                                         (torch.bfloat16, torch.float32), (torch.float16, torch.float16)])
+def test_layers_under_autocast(dtype, ztype, D, F_):
+    """Output types are those of the 16-bit layers. Values differ by the roundings to bf16 (2^-8) of pre-activation, GELU,
+    result and sum, at other places: 2^-6 of the output's size; gradients by those and the 8-bit values' (0.04 together)."""
+    g = _gen(1)
+    r = lambda *s: torch.randn(*s, generator=g, device=DEV)  # noqa: E731
+    x, z = r(2, 9, D).to(dtype), r(2, 9, D).to(ztype)
+    leaves = [t.requires_grad_() for t in (x, z, r(F_, D) / D ** 0.5, r(D, F_) / F_ ** 0.5, r(3, F_, D) / D ** 0.5,
+                                           r(3, D, F_) / F_ ** 0.5)]
+    x, z, w1, w2, wn1, wn2 = leaves
+    with torch.autocast("cuda", dtype=torch.bfloat16):
+        for act in (None, "gelu"):
+            a, b = (dense.mixed_linear(x, 6, w1, wn1, act=act, save8=s) for s in (False, True))
+            assert a.dtype == b.dtype and (a - b).norm() <= 2.0 ** -6 * a.norm()
+        a = z + dense.mixed_linear(dense.mixed_linear(x, 6, w1, wn1, act="gelu"), 6, w2, wn2)
+        b = dense.mixed_ffn(x, z, 6, w1, w2, wn1, wn2, save8=True)
+        with torch.no_grad():
+            c = dense.mixed_ffn(x, z, 6, w1, w2, wn1, wn2, save8=True)
+    assert a.dtype == b.dtype == c.dtype and (a - b).norm() <= 2.0 ** -6 * a.norm() and (a - c).norm() <= 2.0 ** -6 * a.norm()
+    for u, v, t in zip(*(torch.autograd.grad(y, leaves, torch.ones_like(y)) for y in (a, b)), leaves):
+        assert v.dtype == t.dtype and (u.double() - v.double()).norm() <= 0.04 * u.double().norm()
