@@ -92,3 +92,19 @@ def test_ffn_under_autocast(dtype, ztype):
     leaves = (x, z, w1, w2, wn1, wn2)
     for u, v, t in zip(*(torch.autograd.grad(y, leaves, torch.ones_like(y)) for y in (a, b)), leaves):
         assert v.dtype == t.dtype and (u.double() - v.double()).norm() <= 0.03 * u.double().norm()
+
+
+@pytest.mark.parametrize("NS", [0, 3, 9])
+def test_gradients_have_their_inputs_shapes(NS):
+    """With no token of its own weight, some, and nothing else: an empty weight has an empty gradient."""
+    g = torch.Generator().manual_seed(1)
+    r = lambda *s: torch.randn(*s, generator=g).requires_grad_()  # noqa: E731
+    x, z, w1, w2, wn1, wn2 = r(2, 9, 64), r(2, 9, 64), r(128, 64), r(64, 128), r(NS, 128, 64), r(NS, 64, 128)
+    leaves = (x, z, w1, w2, wn1, wn2)
+    y = dense.mixed_ffn(x, z, 9 - NS, w1, w2, wn1, wn2, save8=True)
+    for t, d in zip(leaves, torch.autograd.grad(y.sum(), leaves)):
+        assert d.shape == t.shape and d.dtype == t.dtype and d.isfinite().all()
+    for act in (None, "gelu"):
+        y = dense.mixed_linear(x, 9 - NS, w1, wn1, act=act, save8=True)
+        for t, d in zip((x, w1, wn1), torch.autograd.grad(y.sum(), (x, w1, wn1))):
+            assert d.shape == t.shape and d.dtype == t.dtype and d.isfinite().all()

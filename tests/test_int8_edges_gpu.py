@@ -6,6 +6,7 @@ import torch
 
 from primus_dlrm_b200.ops import dense
 from primus_dlrm_b200.ops.int8 import Int8Weight, _linear_ref, int8_linear, quantize_rows
+from primus_dlrm_b200.ops.saved8 import load8, save8
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda"
@@ -107,3 +108,124 @@ def test_layers_under_autocast(dtype, ztype, D, F_):
     assert a.dtype == b.dtype == c.dtype and (a - b).norm() <= 2.0 ** -6 * a.norm() and (a - c).norm() <= 2.0 ** -6 * a.norm()
     for u, v, t in zip(*(torch.autograd.grad(y, leaves, torch.ones_like(y)) for y in (a, b)), leaves):
         assert v.dtype == t.dtype and (u.double() - v.double()).norm() <= 0.04 * u.double().norm()
+
+
+def test_training_with_sharded_parameters():
+    """FSDP frees a block's bf16 weights after its forward and gathers them again for its backward, which the layers' nodes
+    hold: gradients are those of the same model unsharded. They leave it in bf16, and the norms' weights enter in bf16: some
+    roundings of 2^-8 in each of two blocks, for which 2^-5 leaves room. One rank, in a process of its own."""
+    import subprocess
+    import sys
+    from pathlib import Path
+    root = Path(__file__).resolve().parent.parent
+    code = """
+import os, sys
+sys.path[:0] = [%r, %r]
+import datetime, socket, torch, torch.distributed as dist
+with socket.socket() as s:
+    s.bind(("127.0.0.1", 0))
+    port = s.getsockname()[1]
+torch.cuda.set_device(0)
+dist.init_process_group("nccl", init_method=f"tcp://127.0.0.1:{port}", rank=0, world_size=1, timeout=datetime.timedelta(seconds=60),
+                        device_id=torch.device("cuda", 0))
+from primus_dlrm_b200.parallel.fsdp import DTensor, full_tensor, shard_dense
+from test_models_cpu import _batch
+from test_onetrans_rotary import _model
+kw = dict(dropout=0.0, attention_impl="fav4", d_model=64, heads=2, activation_bits=8)
+a, b = _model("cuda", **kw).train(), _model("cuda", **kw).train()
+b.load_state_dict(a.state_dict())
+shard_dense(b, torch.device("cuda", 0), dist.group.WORLD, torch.bfloat16)
+batch = {k: v.cuda() for k, v in _batch(B=32, windows=2).items()}
+grads = []
+for m in (a, b):
+    for again in range(2):
+        m.zero_grad()
+        with torch.autocast("cuda", dtype=torch.bfloat16):
+            total, _, _ = m.forward_loss(batch, {"listen_plus": 1.0}, [])
+        total.backward()
+    grads.append((total.item(), {n: full_tensor(p.grad).float() for n, p in m.named_parameters() if p.grad is not None and n.startswith("blocks")}))
+(la, ga), (lb, gb) = grads
+assert isinstance(b.blocks[0].ffn.s_w1.weight, DTensor) and ga.keys() == gb.keys() and len(ga) > 10
+print("LOSS", abs(la - lb) <= 2.0 ** -8 * abs(la))
+worst = max((float((ga[n] - gb[n]).norm() / (ga[n].norm() + 1e-12)), n) for n in ga)
+print("GRADS", worst[0] <= 2.0 ** -5, worst)
+torch.cuda.synchronize()
+dist.destroy_process_group()
+""" % (str(root), str(root / "tests"))
+    r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and "LOSS True" in r.stdout and "GRADS True" in r.stdout, r.stdout + r.stderr[-2000:]
+
+
+def test_calls_at_once_all_end():
+    """Two threads with streams of their own, forward and backward through every form: each of their calls ends, with the
+    results of a call by itself; what a thread raises is seen."""
+    import threading
+    g = _gen(11)
+    w = Int8Weight.from_float(torch.randn(300, 640, generator=g, device=DEV))
+    xs = [torch.randn(m, 640, generator=g, device=DEV).bfloat16() for m in (1, 16, 90, 3000)]
+    r = lambda *s: torch.randn(*s, generator=g, device=DEV).bfloat16()  # noqa: E731
+    # at most 64 rows a sum, in one block: no order of additions changes a weight's gradient
+    layer = [r(4, 9, 64), r(4, 9, 64), r(128, 64), r(64, 128), r(3, 128, 64), r(3, 64, 128)]
+    dy = r(4, 9, 64)
+
+    def once(leaves):
+        out = [int8_linear(x, w, act="gelu") for x in xs] + [load8(save8(x)) for x in xs]
+        y = dense.mixed_ffn(leaves[0], leaves[1], 6, *leaves[2:], save8=True)
+        return out + [y.detach(), *torch.autograd.grad(y, leaves, dy)]
+
+    want = once([t.clone().requires_grad_() for t in layer])
+    torch.cuda.synchronize()
+    bad, done = [], []
+
+    def work():
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                leaves = [t.clone().requires_grad_() for t in layer]
+                for _ in range(20):
+                    for a, b in zip(once(leaves), want):
+                        if not torch.equal(a, b):
+                            bad.append(a.shape)
+                    done.append(1)
+        except Exception as e:  # noqa: BLE001 - any of them is a failure of this test
+            bad.append(repr(e))
+
+    threads = [threading.Thread(target=work) for _ in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not bad and len(done) == 40
+
+
+def test_a_backward_captured_beside_an_eager_graph_ends_in_an_error_or_a_result():
+    """A backward pass captured while an eager graph of the same leaves lives: PyTorch may refuse it, for its own operations
+    alike. Either way the process goes on, and exits as it should."""
+    import subprocess
+    import sys
+    from pathlib import Path
+    code = """
+import sys
+sys.path.insert(0, %r)
+import torch
+from primus_dlrm_b200.ops import dense
+r = lambda *s: torch.randn(*s, device="cuda").bfloat16()
+p = [t.requires_grad_() for t in (r(2, 9, 64), r(2, 9, 64), r(128, 64), r(64, 128), r(3, 128, 64), r(3, 64, 128))]
+dy = r(2, 9, 64)
+layer = lambda: dense.mixed_ffn(p[0], p[1], 6, *p[2:], save8=True)
+want = torch.autograd.grad(layer(), p, dy)
+alive = layer()
+torch.cuda.synchronize()
+graph = torch.cuda.CUDAGraph()
+try:
+    with torch.cuda.graph(graph):
+        got = torch.autograd.grad(layer(), p, dy)
+    graph.replay()
+    print("CAPTURED", all(torch.equal(a, b) for a, b in zip(got, want)))
+except RuntimeError as e:
+    print("REFUSED True", str(e)[:200])
+torch.cuda.synchronize()
+print("AFTER", all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(alive, p, dy), want)))
+""" % str(Path(__file__).resolve().parent.parent)
+    r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0, r.stdout + r.stderr[-1500:]
+    assert ("CAPTURED True" in r.stdout) != ("REFUSED True" in r.stdout) and "AFTER True" in r.stdout, r.stdout
