@@ -24,7 +24,7 @@ void gemm_lines(const Mat&, const Mat&, const Mat&, const Mat*, int*, bool);
 void gemm_saved8(const Mat&, const Mat&, const Mat&, const MatCodes&, const Mat*, int*, bool);
 at::Tensor wgrad_as(const Mat&, const Mat&, const at::Device&, int*, bool, int64_t);
 void tc_wgrad(at::Tensor, at::Tensor, at::Tensor, at::Tensor, bool);
-at::Tensor gemm_error_word(int64_t);
+at::Tensor gemm_error_word(int64_t, int64_t);
 at::Tensor tc_mma_rate(int64_t, int64_t, int64_t, int64_t, int64_t, int64_t, at::Tensor);
 at::Tensor tc_mma_burst(int64_t, int64_t, int64_t, int64_t, int64_t, int64_t, int64_t, int64_t, at::Tensor);
 }  // namespace pd
@@ -250,7 +250,8 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         py::arg("R2") = py::none(),
         "C[l] = epi(A[l] @ B[l]^T) on tcgen05 (A [L,M,K], B [L|1,N,K] or with b_kn [L|1,K,N], C [L,M,N] bf16 views); "
         "epi 0 none, 1 gelu, 2 +R, 3 dgelu(R), 4 gelu+gelu' to AUX, 5 *R, 6 relu(+R), 7 acc where R>0, 8 R*acc+R2");
-  m.def("error_word", &pd::gemm_error_word, "the device's int32 error word, for the calls that take one");
+  m.def("error_word", &pd::gemm_error_word, py::arg("device"), py::arg("which") = 0,
+        "the device's int32 error word for the calls that take one: 0 the GEMMs', 1 the attention's");
   m.def("mixed_linear_saved8", &mixed_linear_saved8, "a mixed projection whose input waits for the backward in 8 bits");
   m.def("mixed_ffn_saved8", &mixed_ffn_saved8, "a mixed FFN whose input and pre-activation wait for the backward in 8 bits");
   m.def("tc_wgrad", &pd::tc_wgrad, py::arg("A"), py::arg("B"), py::arg("C"), py::arg("err"), py::arg("l_sum") = false,

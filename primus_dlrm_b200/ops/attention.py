@@ -91,8 +91,10 @@ def _tc_bwd_ok(qkv: torch.Tensor, q_len: int) -> bool:
 def _err_word(device) -> torch.Tensor:
     w = _ERR.get(device)
     if w is None:
-        w = torch.zeros(1, dtype=torch.int32, device=device)
-        _ERR[device] = w
+        device = torch.device(device)
+        if device.index is None:
+            return _err_word(torch.device(device.type, torch.cuda.current_device()))
+        w = _ERR[device] = _ext.gemm().error_word(device.index, 1)
     return w
 
 
@@ -104,8 +106,16 @@ NATIVE_CALLS = {"fwd": 0, "bwd": 0}
 
 def attention_error_code(device) -> int:
     """Error word of the tcgen05 attention kernels (0 = ok, 2 = a bounded wait ran out)."""
-    w = _ERR.get(torch.device(device))
-    return int(w.item()) if w is not None else 0
+    return int(_err_word(device).item()) if torch.device(device).type == "cuda" else 0
+
+
+def check_errors(device) -> None:
+    """Raises (and clears the word) if an attention kernel on ``device`` gave up:
+    results behind it are not to be used.  Waits for the current stream."""
+    code = attention_error_code(device) if _ext.native_enabled(device) else 0
+    if code:
+        _err_word(device).zero_()
+        raise RuntimeError("attention: a bounded wait in a kernel ran out" if code == 2 else f"attention: error {code}")
 
 
 class _NativeFMHAFused(torch.autograd.Function):

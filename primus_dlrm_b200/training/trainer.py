@@ -32,7 +32,7 @@ import torch.distributed as dist
 
 from primus_dlrm_b200.config import Config
 from primus_dlrm_b200.data.batch import DeviceBatchStager, PackedBatch
-from primus_dlrm_b200.ops import dense
+from primus_dlrm_b200.ops import attention, dense
 from primus_dlrm_b200.parallel.health import HealthMonitor
 from primus_dlrm_b200.parallel.setup import barrier, get_rank, get_world_size, is_main_process
 from primus_dlrm_b200.training.checkpoint import save_checkpoint
@@ -187,6 +187,11 @@ class DistributedTrainer:
         finally:
             self.health.stop()
 
+    def _check_kernels(self) -> None:
+        """A kernel that gave up ends the run (where the host waits anyway)."""
+        dense.check_errors(self.device)
+        attention.check_errors(self.device)
+
     def _train(self) -> dict:
         tc = self.config.train
         world = get_world_size()
@@ -218,7 +223,7 @@ class DistributedTrainer:
                     mem = gather_max_gpu_memory(self.device) if tc.log_max_gpu_memory else ""
                     comm_ms = self.engine.exposed_comm_ms()
                     lv = float(loss)
-                    dense.check_errors(self.device)      # a GEMM that gave up ends the run
+                    self._check_kernels()
                     history.append(lv)
                     if is_main_process():
                         now = time.time()
@@ -241,7 +246,7 @@ class DistributedTrainer:
                 logger.info(f"=== Epoch {epoch} done === avg_loss={float(epoch_loss) / max(n, 1):.4f} | "
                             f"last_loss={float(last_loss):.4f} | time={dt:.1f}s | "
                             f"global_throughput={n * per_gpu * world / max(dt, 1e-9):.0f} samples/s")
-            dense.check_errors(self.device)              # before its results reach a checkpoint
+            self._check_kernels()                        # before the results reach a checkpoint
             barrier()
             if tc.save_checkpoint:
                 save_checkpoint(self.ckpt_dir / f"epoch_{epoch}.pt", self.model, epoch, self.engine.global_step,

@@ -50,6 +50,19 @@ def test_training_stops_at_the_next_look(fails_at, log_interval, seen_at, tmp_pa
     assert word.item() == 0                                  # raised once
 
 
+def test_training_stops_where_the_attention_gave_up(tmp_path, monkeypatch):
+    from primus_dlrm_b200.ops import attention
+    eng, tr = _trainer(tmp_path, 2, 1)
+    word = torch.full((1,), 2, dtype=torch.int32)
+    monkeypatch.setattr(attention, "_err_word", lambda device: word)
+    monkeypatch.setattr(attention, "attention_error_code", lambda device: int(word.item()))
+    monkeypatch.setattr(attention._ext, "native_enabled", lambda device=None: True)
+    monkeypatch.setattr(dense, "gemm_error_code", lambda device: 0)
+    with pytest.raises(RuntimeError, match="attention: a bounded wait"):
+        tr.train()
+    assert eng.global_step == 1 and word.item() == 0
+
+
 def test_training_without_errors_runs_and_saves(tmp_path):
     eng, tr = _trainer(tmp_path, 3, 1)
     tr.train()

@@ -52,3 +52,21 @@ print("TRAINED", float(x.grad[0, 0, 0]))
     r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300)
     assert r.returncode == 0, r.stdout + r.stderr[-1500:]
     assert all(m in r.stdout for m in ("INFERENCE False", "BEFORE 0", "AFTER 2", "TRAINED 64.0")), r.stdout
+
+
+def test_the_attention_has_a_word_of_its_own():
+    """Asked for without an index, apart from the GEMMs', made in any mode, raised once."""
+    from primus_dlrm_b200.ops import attention
+    with torch.inference_mode():
+        word = attention._err_word("cuda")
+    assert not word.is_inference() and word.data_ptr() != dense._err("cuda").data_ptr()
+    try:
+        word.fill_(2)
+        assert attention.attention_error_code("cuda") == attention.attention_error_code("cuda:0") == 2
+        assert dense.gemm_error_code("cuda") == 0
+        dense.check_errors("cuda")
+        with pytest.raises(RuntimeError, match="attention: a bounded wait"):
+            attention.check_errors("cuda")
+        attention.check_errors("cuda")
+    finally:
+        word.zero_()
