@@ -92,6 +92,7 @@ __global__ void __launch_bounds__(threads_of(MODE), 1) lines_kernel(const __grid
   __shared__ volatile int abort_flag;
   if (tcx::smem_u32(line_ring) % 1024 != 0) {             // the swizzled tiles need it
     set_error(p.err, kBadShape);
+    tcx::wait_for_launch_before();                        // kernels behind this one count on it
     return;
   }
   uint8_t* sA = line_ring;

@@ -748,6 +748,7 @@ __global__ void __launch_bounds__(kThreads, 1) wgrad_wide_kernel(const __grid_co
   __shared__ volatile int abort_flag;
   if (smem_u32(wide_ring) % 1024 != 0) {                  // the swizzled tiles need it
     set_error(p.err, kBadShape);
+    wait_for_launch_before();                             // kernels behind this one count on it
     return;
   }
   uint8_t* sA = wide_ring;

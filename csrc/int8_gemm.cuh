@@ -142,6 +142,7 @@ __global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_const
   uint8_t* sB = ring + p.stages * kA;
   if (tcx::smem_u32(ring) % 1024 != 0) {                  // the swizzled tiles need it
     set_error(p.err, 4);
+    wait_for_launch_before();                             // kernels behind this one count on it
     return;
   }
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -354,6 +355,7 @@ __global__ void __launch_bounds__(kSplitThreads, 1) split_kernel(const __grid_co
   uint8_t* sB = ring + kSplitStages * kA;
   if (tcx::smem_u32(ring) % 1024 != 0) {                  // alike in every block of the cluster
     set_error(p.err, 4);
+    wait_for_launch_before();                             // kernels behind this one count on it
     return;
   }
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
