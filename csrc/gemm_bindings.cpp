@@ -34,7 +34,6 @@ at::Tensor tc_mma_burst(int64_t, int64_t, int64_t, int64_t, int64_t, int64_t, in
 namespace {
 using torch::autograd::AutogradContext;
 using torch::autograd::variable_list;
-using OptTensor = c10::optional<at::Tensor>;
 
 std::tuple<at::Tensor, at::Tensor> save8(const at::Tensor& x) {
   static auto op = c10::Dispatcher::singleton()

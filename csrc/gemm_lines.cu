@@ -39,8 +39,8 @@ constexpr int BK = 64;
 constexpr int kBlockBytes = 4096;       // a staged block: 32 rows of 128 bytes
 enum Mode : int { kPlain = 0, kSave = 1, kUse = 2 };
 
-// GELU's arithmetic wants more warps (kUse, still by half lines, took 186 us with 12 and 146 with 16; 171 with 8), the plain
-// products want the room in shared memory.
+// GELU's arithmetic wants more warps (an FFN 256 -> 1024 over 100,608 rows, both launches: kSave 118 us with 16, 128 with 8;
+// kUse, with more arithmetic, has pairs of warps for 16 alone), the plain products want the room in shared memory.
 constexpr int epi_warps(int mode) { return mode == kPlain ? 8 : 16; }
 constexpr int threads_of(int mode) { return 64 + 32 * epi_warps(mode); }
 

@@ -65,7 +65,8 @@ def _aggregate(per_user: list[dict[str, float]], ks: list[int]) -> dict[str, flo
 
 def serving_weights(model, weights: str | None):
     """What :func:`score_candidates` takes for ``weights`` None or ``"int8"``: a OneTrans model's projection weights laid
-    out once as 8-bit integers."""
+    out once as 8-bit integers.  Under FSDP every rank holds them whole, and
+    scoring still gathers the units' own parameters (norms, tokenizers, heads)."""
     if weights is None:
         return None
     inner = getattr(model, "module", model)

@@ -294,8 +294,9 @@ def mixed_ffn(x: torch.Tensor, z: torch.Tensor, n_s: int, w1, w2, wn1, wn2, save
     With ``save8`` the input and the pre-activation wait for the backward pass
     in 8 bits (``ops.saved8``) in place of the input, GELU and GELU' in 16: 5
     bytes and a bit a feature instead of 18 (hidden width 4 D).  The output is
-    the same; gradients carry the rounding of the 8-bit values.  It then runs
-    for every input (through PyTorch where the native GEMM cannot), never None.
+    the same, under autocast too; gradients carry the rounding of the 8-bit
+    values.  It then runs for every input (through PyTorch where the native GEMM
+    cannot), never None.
     """
     if save8:
         x = _as_products_take(x)

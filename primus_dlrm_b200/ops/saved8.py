@@ -8,9 +8,11 @@ backward pass (``ops.dense.mixed_linear`` / ``mixed_ffn`` with ``save8=True``).
 
 A block's scale is the smallest power of two with ``max |x| <= 127 * scale`` (at
 least 2^-126), a code the integer nearest to ``x / scale``: values come back
-within half a scale, at most 2^-7 of the block's largest magnitude.  A code
-times its scale has 7 significant bits, so values are exact in bf16.  A block
-that holds a NaN or an infinity loads as NaN.
+within half a scale, at most 1/127 of the block's largest magnitude (2^-127 in
+blocks at the smallest scale).  At the type's largest values codes are held to
+63, so that nothing loads as an infinity: the top step is off by up to a whole
+scale.  A code times its scale has 7 significant bits, so values are exact in
+bf16.  A block that holds a NaN or an infinity loads as NaN.
 
 Native path: ``_int8`` kernels (bf16, fp16 or fp32).  Eager path (CPU tensors,
 or ``PD_KERNELS=eager``): the same bits in PyTorch.
