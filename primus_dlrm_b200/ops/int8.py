@@ -45,8 +45,9 @@ def _quantize_ref(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
 def quantize_rows(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     """Int8 codes of ``x`` ``[..., K]`` (bf16, fp16 or fp32) and the fp32 scale
     ``[...]`` of each row; ``codes * scale`` is within half a scale of ``x`` (and
-    2^-15 of one, by the roundings of the scale and its reciprocal).  A row with a NaN or an infinity has codes of 0 and a scale of NaN.  Not
-    differentiable: the results carry no graph."""
+    2^-15 of one, by the roundings of the scale and its reciprocal).  A row with
+    a NaN or an infinity has codes of 0 and a scale of NaN.  Not differentiable:
+    the results carry no graph."""
     if x.dim() == 0 or x.dtype not in _TYPES:
         raise ValueError(f"quantize_rows: a bf16, fp16 or fp32 tensor with a last dim is expected, not {x.dtype} of "
                          f"{x.dim()} dims")
